@@ -185,6 +185,75 @@ int b200q_bmm_s8(const int8_t* A, const int8_t* B, const int32_t* d_bias, const 
                  void* C, int batch, int M, int N, int K, int trans_a, int trans_b,
                  const b200q_epilogue* epi, void* stream);
 
+/* ---- decoder operators with 4-bit storage (no reference counterpart) ----
+ * Floating tensors are fp32, fp16 or bf16, one type per call (b200q_ftype); sums, norms and softmax
+ * statistics are held in fp32.  Strides are in elements; the last dimension is contiguous.
+ * A 4-bit code pair is one byte, low nibble first.  Positions, slots, page numbers and lengths live on
+ * the device: one that is out of range is left out of the result (nothing is read or written for it)
+ * and reported by the next b200q_device_error() as B200Q_ERR_INVALID_ARG. */
+enum b200q_ftype { B200Q_F32 = 0, B200Q_F16 = 1, B200Q_BF16 = 2 };
+
+/* y[m][n] = sum_k x[m][k] * (code[n][k] - zero[k / group][n]) * scale[k / group][n] (+ bias[n]).
+ * codes: [n][16 * ceil(k / 32)] bytes, 16-byte aligned (the nibbles past k are not used);
+ * scales: bf16 [ceil(k / group)][n]; zeros: uint8 in 0..15, same shape, or NULL for 8 everywhere;
+ * group 32, 64 or 128.  x [m][k] with row stride ldx, y [m][n] with row stride ldy.
+ * Made for the few rows of a decode step: weights are read once per 16 rows of x.  Finite x. */
+int b200q_linear_w4(const void* x, long long ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros,
+                    const void* bias, void* y, long long ldy, int ftype, int m, int n, int k, int group,
+                    void* stream);
+
+/* Per-head RMS norm of queries and keys, then the position rotation of each head's first `rot`
+ * channels, in one pass:  y = R(pos[t]) (x * rsqrt(mean(x^2) + eps) * w).
+ * q [t][hq][d], k [t][hk][d] with token / head strides; q_w, k_w [d] or NULL (all ones).
+ * table: fp32 [positions][rot], cos of the rot / 2 angles, then sin; rot even, <= d, 0 for none.
+ * Pairs are (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved.  q_out / k_out may be q / k. */
+int b200q_qk_norm_rope(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs,
+                       const void* q_w, const void* k_w, const float* table, int positions, const int32_t* pos,
+                       void* q_out, long long qo_ts, long long qo_hs, void* k_out, long long ko_ts,
+                       long long ko_hs, int ftype, int t, int hq, int hk, int d, int rot, int interleaved, float eps,
+                       void* stream);
+
+/* Gradient of b200q_qk_norm_rope: dq_out / dk_out are the gradients of its outputs, contiguous
+ * [t][h][d]; dq / dk (contiguous) those of its inputs; dq_w / dk_w [d] those of the weights, summed
+ * over tokens and heads in a fixed order (NULL: not wanted).  Recomputes the norms from
+ * q and k.  Uses the stream's workspace. */
+int b200q_qk_norm_rope_bprop(const void* dq_out, const void* dk_out, const void* q, long long q_ts, long long q_hs,
+                             const void* k, long long k_ts, long long k_hs, const void* q_w, const void* k_w,
+                             const float* table, int positions, const int32_t* pos, void* dq, void* dk, void* dq_w,
+                             void* dk_w, int ftype, int t, int hq, int hk, int d, int rot, int interleaved, float eps,
+                             void* stream);
+
+/* 4-bit paged key / value cache.  codes: [pages][heads][page_size][d / 2] bytes, 16-byte aligned;
+ * params: [pages][heads][page_size][d / group] words (bits 0-15 the bf16 scale, 16-23 the zero point);
+ * value = (code - zero) * scale.  d 64, 128 or 256; group 32 or 64.  Slot = page * page_size + place. */
+typedef struct b200q_kv4_cache {
+  uint8_t* k_codes;
+  uint32_t* k_params;
+  uint8_t* v_codes;
+  uint32_t* v_params;
+  int pages, heads, page_size, d, group;
+} b200q_kv4_cache;
+
+/* Quantizes k, v [t][heads][d] into slots[t] (int64; negative: not stored).  Per group, in fp32:
+ *   lo = min(0, x), hi = max(0, x), s = bf16((hi - lo) * (1 / 15)) (0 when below the smallest normal),
+ *   zero = clamp(rint(-lo * (1 / s)), 0, 15), code = clamp(rint(x * (1 / s)) + zero, 0, 15).
+ * Every slot is named at most once in a call. */
+int b200q_kv4_append(const b200q_kv4_cache* c, const void* k, long long k_ts, long long k_hs, const void* v,
+                     long long v_ts, long long v_hs, const int64_t* slots, int ftype, int t, void* stream);
+
+/* The values held in slots[t], contiguous [t][heads][d]; zeros for negative slots. */
+int b200q_kv4_read(const b200q_kv4_cache* c, const int64_t* slots, void* k, void* v, int ftype, int t, void* stream);
+
+/* Attention of tq new tokens per sequence over the cache, which already holds them:
+ * token i of sequence b sees the first lens[b] - tq + i + 1 places of its pages
+ * block_table[b][0 .. max_pages), row stride bt_stride; none seen: output 0, lse -inf.
+ * q [b][tq][hq][d] with strides; query head h reads cache head h / (hq / heads).
+ * out contiguous [b][tq][hq][d]; lse fp32 [b][tq][hq] or NULL: log of the sum of exp(scale * q.k).
+ * Uses the stream's workspace when a sequence is split over blocks. */
+int b200q_kv4_attention(const b200q_kv4_cache* c, const void* q, long long q_bs, long long q_ts, long long q_hs,
+                        const int32_t* block_table, long long bt_stride, const int32_t* lens, void* out, float* lse,
+                        int ftype, int b, int tq, int hq, int max_pages, float scale, void* stream);
+
 /* Packed low-channel int8 conv that allocates nothing (no counterpart in the reference).
  * For callers that may not allocate device memory at all: for example plugins inside a runtime
  * that owns and budgets every byte of GPU memory itself, or latency-critical loops where a
@@ -225,7 +294,8 @@ int b200q_conv_out_shape(int h, int w, int c, int r, int s, int k, const b200q_c
 const char* b200q_last_error(void);
 
 /* Synchronizes the device, then reads and clears the device-side error word that
- * kernels set when a bounded wait runs out.  Returns B200Q_OK or B200Q_ERR_TIMEOUT. */
+ * kernels set when a bounded wait runs out (B200Q_ERR_TIMEOUT) or when they meet a position, slot,
+ * page or length that is out of range (B200Q_ERR_INVALID_ARG).  B200Q_OK when it is clear. */
 int b200q_device_error(void);
 
 /* Which kernel family the last conv / bmm call on this thread dispatched to:
@@ -241,7 +311,8 @@ int b200q_device_error(void);
  * (3 x TF32 split GEMM), 14 CUDA-core fp32 (groups of a few channels, e.g. depthwise), 15 tcgen05
  * pixel-grouped 1x1 GEMM (G pixels per row against block-diagonal weights built in the stream's
  * workspace, for layers with G * K <= 256 and G * C <= 256), 16 tcgen05 int32 bmm (operands copied
- * to int8, CUDA-core recompute only when a value does not fit). */
+ * to int8, CUDA-core recompute only when a value does not fit), 17 4-bit weights linear, 18 per-head norm
+ * and rotation (either direction), 19 4-bit cache append / read, 20 4-bit cache attention. */
 int b200q_last_path(void);
 
 /* 0 = automatic dispatch (default); 1 = force the CUDA-core kernels (cross-checks). */

@@ -1,5 +1,7 @@
 """my_own_cnn_b200: B200-native (sm_100a) int8 NHWC convolution and batched GEMM, with the
-reference's fp32 conv (forward and both gradients) and fp32 bmm on the same tensor-core engine.
+reference's fp32 conv (forward and both gradients) and fp32 bmm on the same tensor-core engine,
+and decoder operators with 4-bit storage (weight-only linear, per-head norm with rotation, a 4-bit
+paged key / value cache and the attention over it).
 
 A from-scratch implementation of the quantized conv / bmm hot path of NikitaYak02/my_own_cnn
 behind the reference's own entry points.  The kernels live in ``libb200q.so`` (C ABI:
@@ -15,7 +17,10 @@ from .bmm import BMM_TRANSPOSE_NONE, BMM_TRANSPOSE_YES, bmm_matmul_i32, bmm_s8, 
 from .f32 import (BlockBiasMode, bmm_bprop, bmm_bprop_dA, bmm_bprop_dB, bmm_fprop, bmm_matmul, launch_block_bprop_nhwc,
                   launch_block_fprop_nhwc, launch_block_grad_nhwc, launch_bprop_nhwc, launch_fprop_nhwc,
                   launch_grad_nhwc)
-from ._lib import B200QError, last_path, set_path_policy, tc_launch_count
+from .w4 import W4Weight, linear_w4, pack_w4, quantize_w4
+from .rope import qk_norm_rope, qk_norm_rope_bprop, rope_table
+from .kv4 import KV4Cache, kv4_append, kv4_attention, kv4_read
+from ._lib import B200QError, device_error, last_path, set_path_policy, tc_launch_count
 
 __all__ = [
     "DataType", "QuantizationParametersU8", "QuantizationParametersS5", "get_zero_point", "qparams_to_device",
@@ -25,5 +30,6 @@ __all__ = [
     "bmm_s8_into", "B200QError", "last_path", "set_path_policy", "tc_launch_count",
     "BlockBiasMode", "launch_fprop_nhwc", "launch_bprop_nhwc", "launch_grad_nhwc", "launch_block_fprop_nhwc",
     "launch_block_bprop_nhwc", "launch_block_grad_nhwc", "bmm_matmul", "bmm_fprop", "bmm_bprop_dA", "bmm_bprop_dB",
-    "bmm_bprop",
+    "bmm_bprop", "W4Weight", "linear_w4", "pack_w4", "quantize_w4", "qk_norm_rope", "qk_norm_rope_bprop", "rope_table",
+    "KV4Cache", "kv4_append", "kv4_attention", "kv4_read", "device_error",
 ]

@@ -39,6 +39,10 @@ PATH_NAMES = {
     14: "cuda-core-f32",
     15: "tcgen05-tiled-grouped",
     16: "tcgen05-bmm-i32",
+    17: "linear-w4",
+    18: "qk-norm-rope",
+    19: "kv4-cache",
+    20: "kv4-attention",
 }
 
 
@@ -51,6 +55,11 @@ class CConvParams(Structure):
 
 class CEpilogue(Structure):
     _fields_ = [("out_kind", c_int), ("zp_out", c_int), ("clamp_lo", c_int), ("clamp_hi", c_int)]
+
+
+class CKV4Cache(Structure):
+    _fields_ = [("k_codes", c_void_p), ("k_params", c_void_p), ("v_codes", c_void_p), ("v_params", c_void_p),
+                ("pages", c_int), ("heads", c_int), ("page_size", c_int), ("d", c_int), ("group", c_int)]
 
 
 class B200QError(RuntimeError):
@@ -72,8 +81,8 @@ def lib() -> ctypes.CDLL:
         raise RuntimeError(f"{LIB_PATH} is not built; run __graft_entry__.build() "
                            "(the CUDA library is required, there is no CPU path)")
     L = ctypes.CDLL(str(LIB_PATH))
-    vp, i = c_void_p, c_int
-    pconv, pepi = POINTER(CConvParams), POINTER(CEpilogue)
+    vp, i, ll, f = c_void_p, c_int, c_longlong, c_float
+    pconv, pepi, pkv4 = POINTER(CConvParams), POINTER(CEpilogue), POINTER(CKV4Cache)
     sig = {
         "b200q_fprop_nhwc_qi32": [i, vp, vp, vp, i, i, i, i, i, i, i, pconv, vp, vp, vp],
         "b200q_block_fprop_nhwc_qi32": [i, vp, vp, vp, i, i, i, i, i, i, i, pconv, i, i, vp, vp, vp],
@@ -96,11 +105,19 @@ def lib() -> ctypes.CDLL:
         "b200q_conv_bprop_f32": [vp, vp, vp, i, i, i, i, i, i, i, pconv, i, i, vp],
         "b200q_conv_grad_f32": [vp, vp, vp, vp, i, i, i, i, i, i, i, i, pconv, i, i, vp],
         "b200q_bmm_f32": [vp, vp, vp, i, i, i, i, i, i, vp],
+        "b200q_linear_w4": [vp, ll, vp, vp, vp, vp, vp, ll, i, i, i, i, i, vp],
+        "b200q_qk_norm_rope": [vp, ll, ll, vp, ll, ll, vp, vp, vp, i, vp, vp, ll, ll, vp, ll, ll, i, i, i, i, i, i, i, f,
+                               vp],
+        "b200q_qk_norm_rope_bprop": [vp, vp, vp, ll, ll, vp, ll, ll, vp, vp, vp, i, vp, vp, vp, vp, vp, i, i, i, i, i, i,
+                                     i, f, vp],
+        "b200q_kv4_append": [pkv4, vp, ll, ll, vp, ll, ll, vp, i, i, vp],
+        "b200q_kv4_read": [pkv4, vp, vp, vp, i, i, vp],
+        "b200q_kv4_attention": [pkv4, vp, ll, ll, ll, vp, ll, vp, vp, vp, i, i, i, i, i, f, vp],
     }
     for name, args in sig.items():
-        f = getattr(L, name)
-        f.argtypes = args
-        f.restype = c_int
+        fn = getattr(L, name)
+        fn.argtypes = args
+        fn.restype = c_int
     L.b200q_last_error.argtypes = []
     L.b200q_last_error.restype = c_char_p
     L.b200q_set_path_policy.argtypes = [c_int]
@@ -117,6 +134,12 @@ def check(rc: int) -> None:
     if rc != B200Q_OK:
         msg = lib().b200q_last_error().decode(errors="replace")
         raise B200QError(rc, msg)
+
+
+def device_error() -> None:
+    """Synchronizes the device and raises B200QError for what its error word holds (see
+    b200q_device_error): a wait that ran out, or a position, slot, page or length out of range."""
+    check(lib().b200q_device_error())
 
 
 def last_path() -> str:
@@ -139,4 +162,6 @@ EXPORTED_SYMBOLS = [
     "b200q_selftest_wait_timeout", "b200q_conv2d_s8_packed_noalloc", "b200q_noalloc_scratch_bytes",
     "b200q_conv_fprop_f32", "b200q_conv_bprop_f32", "b200q_conv_grad_f32", "b200q_bmm_f32",
     "b200q_conv2d_s8_add", "b200q_maxpool_s8", "b200q_global_avgpool_s8", "b200q_conv2d_s8_plan",
+    "b200q_linear_w4", "b200q_qk_norm_rope", "b200q_qk_norm_rope_bprop", "b200q_kv4_append", "b200q_kv4_read",
+    "b200q_kv4_attention",
 ]

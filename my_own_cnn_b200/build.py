@@ -23,6 +23,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -65,10 +66,22 @@ def reference_root() -> Path:
 
 
 def build_library(force: bool = False) -> Path:
-    deps = sorted(CSRC.glob("*.cu*")) + [ROOT / "include" / "b200q.h"]
-    if force or _stale(LIB, deps):
-        _run([_nvcc(), *ARCH, *NVCC_FLAGS, "-shared", "-Xlinker", "-soname,libb200q.so",
-              "-o", str(LIB), str(CSRC / "b200q.cu")])
+    """Every csrc/*.cu becomes an object (compiled side by side), then one library."""
+    headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [ROOT / "include" / "b200q.h"]
+    sources = sorted(CSRC.glob("*.cu"))
+    if not (force or _stale(LIB, headers + sources)):
+        return LIB
+    out = PKG / "_build"
+    out.mkdir(exist_ok=True)
+    todo = []
+    for src in sources:
+        obj = out / (src.stem + ".o")
+        if force or _stale(obj, headers + [src]):
+            todo.append([_nvcc(), *ARCH, *NVCC_FLAGS, "-c", "-o", str(obj), str(src)])
+    with ThreadPoolExecutor(max_workers=max(1, min(len(todo), os.cpu_count() or 1))) as pool:
+        list(pool.map(_run, todo))
+    _run([_nvcc(), *ARCH, "-shared", "-Xlinker", "-soname,libb200q.so", "-o", str(LIB),
+          *[str(out / (src.stem + ".o")) for src in sources]])
     return LIB
 
 

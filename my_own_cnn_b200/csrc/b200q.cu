@@ -29,6 +29,7 @@
 
 #include "../../include/b200q.h"
 #include "common.cuh"
+#include "host.h"
 #include "simt.cuh"
 #include "tc_gemm.cuh"
 #include "qi32_tc.cuh"
@@ -1005,7 +1006,54 @@ int f32_grad(const DeviceState& st, const float* x, const float* dy, float* dw, 
   return B200Q_OK;
 }
 
+// Arrival counters of kernels whose last block joins the others' partial results: zeroed once here,
+// and returned to zero by the block that sees the last arrival.
+std::map<std::pair<int, cudaStream_t>, unsigned*> g_counters;
+
 }  // namespace
+
+int host_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_errmsg, sizeof(g_errmsg), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int host_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+int host_check_launch(const char* what) { return check_launch(what); }
+
+int host_device(int* sms, int** err) {
+  DeviceState* st = nullptr;
+  int rc = device_state(&st);
+  if (rc) return rc;
+  *sms = st->sms;
+  *err = st->err;
+  return B200Q_OK;
+}
+
+int host_workspace(size_t bytes, cudaStream_t stream, void** out) { return get_workspace(bytes, stream, out); }
+
+int host_counters(cudaStream_t stream, unsigned** out) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  std::lock_guard<std::mutex> lk(g_ws_mu);
+  unsigned*& c = g_counters[{dev, stream}];
+  if (!c) {
+    void* p = nullptr;
+    e = cudaMallocAsync(&p, kSplitCounters * sizeof(unsigned), stream);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync(counters)");
+    e = cudaMemsetAsync(p, 0, kSplitCounters * sizeof(unsigned), stream);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(counters)");
+    c = static_cast<unsigned*>(p);
+  }
+  *out = c;
+  return B200Q_OK;
+}
+
+void host_set_path(int path) { g_last_path = path; }
+
 }  // namespace b200q
 
 using namespace b200q;
@@ -1837,7 +1885,13 @@ int b200q_device_error(void) {
   if (v != 0) {
     const int zero = 0;
     cudaMemcpy(st->err, &zero, sizeof(int), cudaMemcpyHostToDevice);
-    return fail(B200Q_ERR_TIMEOUT, "device wait ran out (code 0x%x)", v);
+    switch (v) {
+      case kDevErrBadPosition: return fail(B200Q_ERR_INVALID_ARG, "a position lies outside the rotation table");
+      case kDevErrBadSlot: return fail(B200Q_ERR_INVALID_ARG, "a slot lies outside the cache");
+      case kDevErrBadPage: return fail(B200Q_ERR_INVALID_ARG, "a block table names a page outside the cache");
+      case kDevErrBadLength: return fail(B200Q_ERR_INVALID_ARG, "a length exceeds its block table");
+      default: return fail(B200Q_ERR_TIMEOUT, "device wait ran out (code 0x%x)", v);
+    }
   }
   return B200Q_OK;
 }

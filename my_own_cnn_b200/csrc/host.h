@@ -1,0 +1,36 @@
+// Host services of the library shared by its translation units (defined in b200q.cu): error
+// messages, per-device state, stream workspaces.  Internal: hidden from the library's users.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "../../include/b200q.h"
+
+namespace b200q {
+
+#define B200Q_HIDDEN __attribute__((visibility("hidden")))
+
+// Sets the calling thread's message and returns `code`.
+B200Q_HIDDEN int host_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+B200Q_HIDDEN int host_cuda_fail(cudaError_t e, const char* what);
+// cudaGetLastError() after a launch as a status.
+B200Q_HIDDEN int host_check_launch(const char* what);
+// SM count of the current device and the device address of its error word.
+B200Q_HIDDEN int host_device(int* sms, int** err);
+// Grow-only scratch of the (device, stream) pair.
+B200Q_HIDDEN int host_workspace(size_t bytes, cudaStream_t stream, void** out);
+// kSplitCounters arrival counters of the (device, stream) pair, zero before and after every kernel
+// that uses them.
+constexpr int kSplitCounters = 1 << 16;
+B200Q_HIDDEN int host_counters(cudaStream_t stream, unsigned** out);
+B200Q_HIDDEN void host_set_path(int path);
+
+// Codes of g_dev_err for bad values that only the device sees; 0x1xx are timeouts (common.cuh).
+constexpr int kDevErrBadPosition = 0x201;
+constexpr int kDevErrBadSlot = 0x202;
+constexpr int kDevErrBadPage = 0x203;
+constexpr int kDevErrBadLength = 0x204;
+
+}  // namespace b200q
