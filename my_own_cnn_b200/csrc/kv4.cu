@@ -1,16 +1,14 @@
 // The 4-bit paged key / value cache and the attention over it (b200q_kv4_append, b200q_kv4_read,
 // b200q_kv4_attention).
+#include <algorithm>
+#include <atomic>
+
 #include "host.h"
+#include "kv4_attention.cuh"
 #include "lowbit.cuh"
 
 namespace b200q {
 namespace {
-
-struct Cache {
-  uint8_t* codes[2];
-  uint32_t* params[2];
-  int pages, heads, page_size, d, group;
-};
 
 // Row (slot, head) of the cache: offset in units of one token's head.
 __device__ __forceinline__ size_t cache_row(const Cache& c, long long slot, int h) {
@@ -94,65 +92,6 @@ __global__ void kv4_read_kernel(Cache c, const int64_t* slots, T* k, T* v, int t
   out[1] = from_f32<T>((static_cast<float>(byte >> 4) - param_zero(p)) * param_scale(p));
 }
 
-struct AttnArgs {
-  const void* q;
-  long long q_bs, q_ts, q_hs;
-  const int32_t* table;
-  long long table_stride;
-  const int32_t* lens;
-  void* out;
-  float* lse;
-  int b, tq, hq, max_pages;
-  float scale;
-  int* err;
-};
-
-// One warp per (sequence, new token, query head): running maximum and sum over the tokens.
-template <typename T>
-__global__ void kv4_attention_kernel(Cache c, AttnArgs a) {
-  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32;
-  if (row >= static_cast<long long>(a.b) * a.tq * a.hq) return;
-  const int h = static_cast<int>(row % a.hq), i = static_cast<int>(row / a.hq % a.tq);
-  const int b = static_cast<int>(row / a.hq / a.tq);
-  const int hk = h / (a.hq / c.heads);
-  int len = a.lens[b];
-  if (len < 0 || len > static_cast<long long>(a.max_pages) * c.page_size) {
-    atomicCAS(a.err, 0, kDevErrBadLength);
-    len = 0;
-  }
-  const T* q = static_cast<const T*>(a.q) + b * a.q_bs + i * a.q_ts + h * a.q_hs;
-  const int per = c.d / 32;  // channels of a lane, one after another
-  const int groups = c.d / c.group;
-  float qv[8], o[8] = {}, m = -INFINITY, l = 0.0f;
-  for (int j = 0; j < per; ++j) qv[j] = to_f32(q[lane * per + j]) * a.scale;
-  const int until = len - a.tq + i + 1;
-  for (int t = 0; t < until; ++t) {
-    const int page = a.table[b * a.table_stride + t / c.page_size];
-    if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.pages)) {
-      atomicCAS(a.err, 0, kDevErrBadPage);
-      continue;
-    }
-    const size_t at = (static_cast<size_t>(page) * c.heads + hk) * c.page_size + t % c.page_size;
-    auto value = [&](int which, int j) {
-      const int ch = lane * per + j;
-      const uint32_t p = c.params[which][at * groups + ch / c.group];
-      const uint32_t byte = c.codes[which][at * (c.d / 2) + ch / 2];
-      return (static_cast<float>(ch & 1 ? byte >> 4 : byte & 15u) - param_zero(p)) * param_scale(p);
-    };
-    float dot = 0.0f;
-    for (int j = 0; j < per; ++j) dot += qv[j] * value(0, j);
-    dot = warp_sum(dot);
-    const float top = fmaxf(m, dot), old = expf(m - top), w = expf(dot - top);
-    l = l * old + w;
-    for (int j = 0; j < per; ++j) o[j] = o[j] * old + w * value(1, j);
-    m = top;
-  }
-  T* out = static_cast<T*>(a.out) + row * c.d;
-  for (int j = 0; j < per; ++j) out[lane * per + j] = from_f32<T>(l > 0.0f ? o[j] / l : 0.0f);
-  if (a.lse && lane == 0) a.lse[row] = l > 0.0f ? m + logf(l) : -INFINITY;
-}
-
 int check_cache(const b200q_kv4_cache* p, Cache* c) {
   if (!p) return host_fail(B200Q_ERR_INVALID_ARG, "null argument");
   if (p->pages < 0 || p->heads <= 0 || p->page_size <= 0) return host_fail(B200Q_ERR_INVALID_ARG, "bad cache shape");
@@ -168,6 +107,42 @@ int check_cache(const b200q_kv4_cache* p, Cache* c) {
     return host_fail(B200Q_ERR_INVALID_ARG, "cache tensors must be 16-byte aligned");
   *c = Cache{{p->k_codes, p->v_codes}, {p->k_params, p->v_params}, p->pages, p->heads, p->page_size, p->d, p->group};
   return B200Q_OK;
+}
+
+template <int D, int G, int NT, bool F32>
+int launch_attention(const Cache& c, AttnArgs a, int sms, cudaStream_t stream) {
+  using Shape = AttnShape<D, G, NT, F32>;
+  auto kernel = kv4_attention_kernel<D, G, NT, F32>;
+  // blocks that an SM holds, found once (and on the way, leave for the shared memory that they take)
+  static std::atomic<int> per_sm{0};
+  int resident = per_sm.load(std::memory_order_relaxed);
+  if (resident == 0) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute(kv4_attention_kernel)");
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kWarps * 32, Shape::kSmem);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
+    resident = std::max(1, resident);
+    per_sm.store(resident, std::memory_order_relaxed);
+  }
+  a.row_tiles = (a.tq * (a.hq / c.heads) + 8 * NT - 1) / (8 * NT);
+  const long long units = static_cast<long long>(a.b) * c.heads * a.row_tiles;
+  long long blocks = units;
+  const int target = sms * resident * kWaves;
+  const long long most = (static_cast<long long>(a.max_pages) * c.page_size + kMinChunk - 1) / kMinChunk;
+  if (most > 1 && units < target) {
+    // units split so that each block has 1 / target of the tokens: at most one block more per unit
+    blocks = std::min<long long>(target + units, units * most);
+    a.target = target;
+    const size_t rows = static_cast<size_t>(blocks) * 8 * NT;
+    void* ws = nullptr;
+    int rc = host_workspace(rows * (D + 2) * sizeof(float), stream, &ws);
+    if (rc || (rc = host_counters(stream, &a.counters))) return rc;
+    a.partial = static_cast<float*>(ws);
+    a.partial_ml = a.partial + rows * D;
+  }
+  if (blocks > (a.target ? kSplitCounters : 0x7fffffffll)) return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
+  kernel<<<static_cast<int>(blocks), kWarps * 32, Shape::kSmem, stream>>>(c, a);
+  return host_check_launch("kv4_attention_kernel launch");
 }
 
 int check_ftype(int ftype) {
@@ -234,14 +209,26 @@ extern "C" int b200q_kv4_attention(const b200q_kv4_cache* cache, const void* q, 
   if (!q || !out || !lens || (max_pages > 0 && !block_table)) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
   if (static_cast<long long>(max_pages) * c.page_size > (1 << 30) || b > (1 << 20) || tq > (1 << 16) || hq > (1 << 16))
     return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
-  AttnArgs a{q, q_bs, q_ts, q_hs, block_table, bt_stride, lens, out, lse, b, tq, hq, max_pages, scale, nullptr};
+  AttnArgs a{q, q_bs, q_ts, q_hs, block_table, bt_stride, lens, out, lse, ftype, b, tq, hq, max_pages, scale};
   int sms = 0;
   if ((rc = host_device(&sms, &a.err))) return rc;
-  const long long blocks = (static_cast<long long>(b) * tq * hq + 3) / 4;
-  if (blocks > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
-  B200Q_DISPATCH_FTYPE(ftype, (kv4_attention_kernel<T><<<static_cast<int>(blocks), 128, 0,
-                                                         static_cast<cudaStream_t>(stream)>>>(c, a)));
-  rc = host_check_launch("kv4_attention_kernel launch");
+  a.page_shift = -1;
+  for (int i = 0; i <= 20; ++i)
+    if (c.page_size == 1 << i) a.page_shift = i;
+  // 16 rows a pass where a head has more than 8; heads of 256 channels keep to 8, whose sums fill the registers
+  const int rows = tq * (hq / c.heads);
+  const bool two = rows > 8 && c.d <= 128;
+  const bool f32 = ftype == B200Q_F32;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+#define B200Q_ATTN(D, G)                                                      \
+  (two ? f32 ? launch_attention<D, G, D == 256 ? 1 : 2, true>(c, a, sms, cs)  \
+             : launch_attention<D, G, D == 256 ? 1 : 2, false>(c, a, sms, cs) \
+       : f32 ? launch_attention<D, G, 1, true>(c, a, sms, cs)                 \
+             : launch_attention<D, G, 1, false>(c, a, sms, cs))
+  rc = c.d == 64    ? c.group == 32 ? B200Q_ATTN(64, 32) : B200Q_ATTN(64, 64)
+       : c.d == 128 ? c.group == 32 ? B200Q_ATTN(128, 32) : B200Q_ATTN(128, 64)
+                    : c.group == 32 ? B200Q_ATTN(256, 32) : B200Q_ATTN(256, 64);
+#undef B200Q_ATTN
   if (rc == B200Q_OK) host_set_path(20);
   return rc;
 }

@@ -1,0 +1,580 @@
+// Attention of a few query rows over the 4-bit cache, on tensor cores.
+//
+// For one sequence and cache head with rows r (new tokens x query heads that share the head), tokens t:
+//   S[t][r] = sum_g ks[t,g] (sum_{d in g} kc[t,d] q[r,d]  -  kz[t,g] sum_{d in g} q[r,d])
+//   O[d][r] = sum_t vc[t,d] P[t,r]  -  sum_t vz[t,g] P[t,r],   P[t,r] = vs[t,g] exp2(f[r] S[t][r] - m[r])
+// Both products take the codes as the 16-row operand A of m16n8k16 (tokens x channels, then channels x tokens)
+// and the rows as its 8 columns, so 8 rows cost one instruction per 256 codes.
+//   Keys: a nibble in the low bits of an fp16 is the subnormal code * 2^-24, exactly, and one place higher
+//   code * 2^-20: a word of 8 codes becomes four operands by masking, and every second query value is divided
+//   by 16 instead.  Query rows are scaled by a power of two to a maximum in [2^14, 2^15), so that they fit
+//   fp16 whatever their type; fp32 rows are split into two fp16 terms (22 bits).
+//   Values: the bf16 with mantissa bits 0 to 3 set to the code is 128 + code; bf16 keeps P's range, which follows
+//   the scales.  The zero points (as 128 + vz) go through the same instruction as a 16-row operand of their own,
+//   and the difference of the two sums loses the 128.  fp32 calls subtract before the product instead, and split P
+//   into three bf16 terms: there the 128 would cost 5 bits of the sum.
+//   P leaves the first product as (token, row) and must enter the second as (row, token): movmatrix.
+// The maximum m[r] is a running reference, raised (and the sums rescaled) only when a score passes it by more than
+// 2^8: P stays far inside its range, and a warp-wide maximum is taken a few times per sequence, not per tile.
+//
+// What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head.  Each warp owns a ring of kStages tiles of
+// kTile tokens that it fills with 16-byte asynchronous copies and empties on its own: no block-wide barrier until
+// the end.  A row of codes is padded by 16 bytes in shared memory: then lanes (g, t) reading 4 bytes at g rows down,
+// and 2t rows down, both touch 32 banks once.
+#pragma once
+#include "host.h"
+#include "lowbit.cuh"
+
+namespace b200q {
+
+struct Cache {
+  uint8_t* codes[2];
+  uint32_t* params[2];
+  int pages, heads, page_size, d, group;
+};
+
+struct AttnArgs {
+  const void* q;
+  long long q_bs, q_ts, q_hs;
+  const int32_t* table;
+  long long table_stride;
+  const int32_t* lens;
+  void* out;
+  float* lse;
+  int ftype, b, tq, hq, max_pages;
+  float scale;
+  int page_shift;       // log2 of the page size, or -1
+  int row_tiles;        // tiles of 8 * NT rows of a cache head
+  int target;           // blocks that the tokens are split over, or 0: one block per (sequence, head, row tile)
+  float* partial;       // [block][8 NT][d] sums of a split unit
+  float* partial_ml;    // [block][8 NT][2] maximum and total
+  unsigned* counters;   // [block]
+  int* err;
+};
+
+constexpr int kMinChunk = 256;  // tokens of a block at least
+constexpr int kWaves = 2;       // blocks that the tokens are split over, in units of what the GPU holds at once
+
+constexpr int kTile = 32;    // tokens of a warp's step
+constexpr int kWarps = 4;    // a block's warps take tiles in turn
+constexpr int kStages = 3;
+
+template <int D, int G, int NT, bool F32>
+struct AttnShape {
+  static constexpr int kPitch = D / 2 + 16;
+  static constexpr int kGroups = D / G;
+  static constexpr int kCodes = kTile * kPitch;
+  static constexpr int kParams = kTile * kGroups * 4;
+  static constexpr int kStage = 2 * (kCodes + kParams);
+  static constexpr int kTerms = F32 ? 2 : 1;                       // fp16 terms of a query value
+  static constexpr int kQuery = (D / 32) * kTerms * NT * 32 * 16;  // operand B of the first product
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kJoin = kWarps * 8 * NT * (D + 4) * 4;      // the warps' sums, over the ring
+  static constexpr int kBody = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kRowsMl = kWarps * 8 * NT * 2 * 4;
+  static constexpr int kSmem = kBody + kQuery + kRowsMl + (8 * NT * (kGroups + 1)) * 4;
+};
+
+// Row of the cache that holds token `tok`, or ~0 where there is none to read.
+__device__ __forceinline__ uint32_t token_row(const Cache& c, const AttnArgs& a, const int32_t* pages, int head, int tok,
+                                              int until) {
+  if (tok >= until) return ~0u;
+  const int at = a.page_shift >= 0 ? tok >> a.page_shift : static_cast<int>(static_cast<unsigned>(tok) / static_cast<unsigned>(c.page_size));
+  const int page = __ldg(pages + at);
+  if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.pages)) {
+    atomicCAS(a.err, 0, kDevErrBadPage);
+    return ~0u;
+  }
+  return (static_cast<uint32_t>(page) * c.heads + head) * c.page_size + (tok - at * c.page_size);
+}
+
+// Tokens of a sequence; none where the length is not one that the block table can hold.
+__device__ __forceinline__ int valid_length(const Cache& c, const AttnArgs& a, int seq) {
+  const int len = __ldg(a.lens + seq);
+  if (len >= 0 && len <= static_cast<long long>(a.max_pages) * c.page_size) return len;
+  atomicCAS(a.err, 0, kDevErrBadLength);
+  return 0;
+}
+
+template <typename T>
+__device__ __forceinline__ float load_as_f32(const void* p, long long i) {
+  return to_f32(static_cast<const T*>(p)[i]);
+}
+__device__ __forceinline__ float load_any(int ftype, const void* p, long long i) {
+  return ftype == B200Q_F32   ? load_as_f32<float>(p, i)
+         : ftype == B200Q_F16 ? load_as_f32<__half>(p, i)
+                              : load_as_f32<__nv_bfloat16>(p, i);
+}
+__device__ __forceinline__ void store_any(int ftype, void* p, long long i, float v) {
+  if (ftype == B200Q_F32)
+    static_cast<float*>(p)[i] = v;
+  else if (ftype == B200Q_F16)
+    static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else
+    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// Issues the copies of one tile: lane l holds the cache row of token l.
+template <int D, int G>
+__device__ __forceinline__ void load_tile(const Cache& c, uint32_t stage, uint32_t row, int lane) {
+  constexpr int kChunks = D / 32, kPitch = D / 2 + 16, kCodes = kTile * kPitch, kGroups = D / G;
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j) {
+    const int i = j * 32 + lane, tok = i / kChunks, chunk = i % kChunks;
+    const uint32_t r = __shfl_sync(~0u, row, tok);
+    if (r != ~0u) {
+      const size_t from = static_cast<size_t>(r) * (D / 2) + chunk * 16;
+      const uint32_t to = stage + tok * kPitch + chunk * 16;
+      copy_async<16>(to, c.codes[0] + from);
+      copy_async<16>(to + kCodes, c.codes[1] + from);
+    }
+  }
+  if (row != ~0u) {
+    constexpr int kBytes = kGroups * 4 < 16 ? kGroups * 4 : 16;
+    const uint32_t to = stage + 2 * kCodes + lane * kGroups * 4;
+#pragma unroll
+    for (int b = 0; b < kGroups * 4; b += kBytes) {
+      copy_async<kBytes>(to + b, reinterpret_cast<const uint8_t*>(c.params[0]) + static_cast<size_t>(row) * kGroups * 4 + b);
+      copy_async<kBytes>(to + kTile * kGroups * 4 + b,
+                         reinterpret_cast<const uint8_t*>(c.params[1]) + static_cast<size_t>(row) * kGroups * 4 + b);
+    }
+  }
+}
+
+// The zero point as a float: bits 16-23 under the exponent of 2^23.
+__device__ __forceinline__ float zero_point(uint32_t p) {
+  return __uint_as_float(__byte_perm(p, 0x4B000000u, 0x7542)) - 8388608.0f;
+}
+
+template <int D, int G, int NT, bool F32>
+__global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, AttnArgs a) {
+  using Shape = AttnShape<D, G, NT, F32>;
+  constexpr int kGroups = Shape::kGroups, kPitch = Shape::kPitch, kRows = 8 * NT, kTerms = Shape::kTerms;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint4* const query = reinterpret_cast<uint4*>(smem + Shape::kBody);
+  float* const row_ml = reinterpret_cast<float*>(smem + Shape::kBody + Shape::kQuery);
+  float* const row_sum = row_ml + kWarps * kRows * 2;  // [kGroups][kRows] sums of the scaled query, times 2^-24
+  float* const row_f = row_sum + kRows * kGroups;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4;
+
+  // A unit is (sequence, head, row tile); a sequence's units are split over the same number of blocks, so that every
+  // block has about 1 / target of all tokens, whatever the lengths (which only the device knows).
+  const int units = c.heads * a.row_tiles;
+  int seq = 0, local, splits = 1, chunk = 1 << 30;
+  long long base = 0;  // first block of the sequence
+  if (a.target == 0) {
+    seq = blockIdx.x / units;
+    local = blockIdx.x % units;
+  } else {
+    long long total = 0;
+    for (int i = lane; i < a.b; i += 32) total += valid_length(c, a, i);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
+    chunk = max(kMinChunk, static_cast<int>(min(1ll << 30, (total * units / a.target + 128) / 128 * 128)));
+    for (;; seq += 32) {
+      if (seq >= a.b) return;  // more blocks were launched than these lengths need
+      const int n = seq + lane < a.b ? max(1, (valid_length(c, a, seq + lane) + chunk - 1) / chunk) : 0;
+      int sum = n;
+#pragma unroll
+      for (int x = 1; x < 32; x <<= 1) {
+        const int v = __shfl_up_sync(~0u, sum, x);
+        if (lane >= x) sum += v;
+      }
+      const unsigned past = __ballot_sync(~0u, base + static_cast<long long>(sum) * units > blockIdx.x);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        seq += at;
+        splits = __shfl_sync(~0u, n, at);
+        base += static_cast<long long>(__shfl_sync(~0u, sum, at) - splits) * units;
+        break;
+      }
+      base += static_cast<long long>(__shfl_sync(~0u, sum, 31)) * units;
+    }
+    local = static_cast<int>(blockIdx.x - base);
+  }
+  // blocks of the same tokens run next to each other: their heads lie side by side in a page
+  const int split = local / units, unit = local % units;
+  const int tile = unit % a.row_tiles, head = unit / a.row_tiles;
+  const int ratio = a.hq / c.heads, rows = min(kRows, a.tq * ratio - tile * kRows);
+  const int len = valid_length(c, a, seq);
+  // the last row of the tile sees the most tokens
+  const int seen = max(0, len - a.tq + (tile * kRows + rows - 1) / ratio + 1);
+  const int begin = split * chunk, until = min(seen, begin + chunk);
+  const int32_t* pages = a.table + seq * a.table_stride;
+
+  // ring: the first tiles are on their way before the query is looked at
+  const uint32_t ring = shared_address(smem) + warp * (kStages * Shape::kStage);
+  const int tiles = max(0, (until - begin + kTile - 1) / kTile);
+  const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+  const int first = begin + warp * kTile + lane;  // this lane's token of the warp's tile i: first + i * step
+  constexpr int kStep = kWarps * kTile;
+  uint32_t held[kStages];  // which tokens of the tiles on their way are there
+  uint32_t row = token_row(c, a, pages, head, first, until);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    held[i] = __ballot_sync(~0u, row != ~0u);
+    if (i < mine) load_tile<D, G>(c, ring + i * Shape::kStage, row, lane);
+    copy_commit();
+    row = token_row(c, a, pages, head, first + (i + 1) * kStep, until);
+  }
+
+  // query rows: scaled to fp16, laid out as operand B; a warp takes rows in turn
+  for (int r = warp; r < kRows; r += kWarps) {
+    constexpr int kPer = D / 32;
+    const int rr = tile * kRows + r;
+    float v[kPer];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {  // channel 32 i + lane
+      v[i] = r < rows ? load_any(a.ftype, a.q, seq * a.q_bs + (rr / ratio) * a.q_ts + (head * ratio + rr % ratio) * a.q_hs + 32 * i + lane)
+                      : 0.0f;
+      top = fmaxf(top, fabsf(v[i]));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    // 2^up brings the maximum into [2^14, 2^15)
+    const int up = top > 0.0f ? min(120, 14 + 127 - static_cast<int>(__float_as_uint(top) >> 23)) : 0;
+    const float factor = __uint_as_float(static_cast<uint32_t>(127 + max(-126, up)) << 23);
+    if (lane == 0) row_f[r] = __uint_as_float(static_cast<uint32_t>(127 - max(-126, up)) << 23) * a.scale * 1.4426950408889634f * 16777216.0f;
+    // lane: channel p = lane % 8 of the 8 that thread lane / 8 of a quad holds; pairs are (0,4) (1,5) (2,6) (3,7)
+    const int p = lane % 8, owner = (r % 8) * 4 + lane / 8;
+    __half* at = reinterpret_cast<__half*>(query);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      float x = v[i] * factor;
+#pragma unroll
+      for (int term = 0; term < kTerms; ++term) {
+        const __half hv = __float2half_rn(x);
+        const float back = __half2float(hv);
+        sum += back;
+        x -= back;
+        at[(((i * kTerms + term) * NT + r / 8) * 32 + owner) * 8 + (p % 4) * 2 + p / 4] =
+            p % 2 ? __float2half_rn(back * 0.0625f) : hv;
+      }
+      if ((i + 1) % (G / 32) == 0) {
+        sum = warp_sum(sum);
+        if (lane == 0) row_sum[(i / (G / 32)) * kRows + r] = sum * (1.0f / 16777216.0f);
+        sum = 0.0f;
+      }
+    }
+  }
+  __syncthreads();
+
+  // this lane's columns: rows 2t, 2t + 1 of each 8
+  float f[NT][2], qsum[NT][kGroups][2], m[NT][2], l[NT][2];
+  int limit[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = n * 8 + 2 * t + e;
+      f[n][e] = row_f[r];
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) qsum[n][k][e] = row_sum[k * kRows + r];
+      m[n][e] = -INFINITY;
+      l[n][e] = 0.0f;
+      limit[n][e] = len - a.tq + (tile * kRows + min(r, rows - 1)) / ratio + 1;
+    }
+  const int all_see = len - a.tq + tile * kRows / ratio + 1;  // tokens that every row of the tile sees
+  float o[D / 16][NT][4], z[kGroups][NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j) z[j][n][0] = z[j][n][1] = z[j][n][2] = z[j][n][3] = 0.0f;
+  }
+
+  int slot = 0, fill = kStages - 1;
+  for (int it = 0; it < mine; ++it) {
+    copy_wait<kStages - 2>();
+    __syncwarp();
+    held[kStages - 1] = __ballot_sync(~0u, row != ~0u);
+    if (it + kStages - 1 < mine) load_tile<D, G>(c, ring + fill * Shape::kStage, row, lane);
+    copy_commit();
+    row = token_row(c, a, pages, head, first + (it + kStages) * kStep, until);
+    const uint8_t* stage = smem + warp * (kStages * Shape::kStage) + slot * Shape::kStage;
+    const uint8_t* kc = stage;
+    const uint8_t* vc = stage + Shape::kCodes;
+    const uint32_t* kp = reinterpret_cast<const uint32_t*>(stage + 2 * Shape::kCodes);
+    const uint32_t* vp = kp + kTile * kGroups;
+    const uint32_t here = held[0];
+    const int base = begin + (it * kWarps + warp) * kTile;
+    const bool whole = here == ~0u && base + kTile <= all_see;
+
+    // scores
+    float s[2][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[mt][n][0] = s[mt][n][1] = s[mt][n][2] = s[mt][n][3] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      float part[2][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) part[mt][n][0] = part[mt][n][1] = part[mt][n][2] = part[mt][n][3] = 0.0f;
+#pragma unroll
+      for (int i = k * (G / 32); i < (k + 1) * (G / 32); ++i) {
+        uint4 b[kTerms][NT];
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) b[term][n] = query[((i * kTerms + term) * NT + n) * 32 + lane];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(kc + (mt * 16 + g) * kPitch + 16 * i + 4 * t);
+          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(kc + (mt * 16 + g + 8) * kPitch + 16 * i + 4 * t);
+          const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
+#pragma unroll
+          for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_f16(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
+                      b[term][n].x, b[term][n].y);
+              mma_f16(part[mt][n], v0 & 0x000F000Fu, v1 & 0x000F000Fu, v0 & 0x00F000F0u, v1 & 0x00F000F0u,
+                      b[term][n].z, b[term][n].w);
+            }
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t p = kp[(mt * 16 + u * 8 + g) * kGroups + k];
+          const float ks = param_scale(p), kz = zero_point(p);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              s[mt][n][2 * u + e] = fmaf(ks, fmaf(-kz, qsum[n][k][e], part[mt][n][2 * u + e]), s[mt][n][2 * u + e]);
+        }
+    }
+
+    // weights
+    bool raise = false;
+    float top[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[n][e] = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float& x = s[mt][n][2 * u + e];
+            x *= f[n][e];
+            if (!whole) {
+              const int tok = mt * 16 + u * 8 + g;
+              if (!(here >> tok & 1) || base + tok >= limit[n][e]) x = -INFINITY;
+            }
+            top[n][e] = fmaxf(top[n][e], x);
+          }
+        raise |= top[n][e] > m[n][e] + 8.0f;
+      }
+    if (__any_sync(~0u, raise)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(~0u, top[n][e], x));
+          const float now = fmaxf(m[n][e], top[n][e]);
+          const float keep = now == -INFINITY ? 1.0f : exp2_approx(m[n][e] - now);
+          m[n][e] = now;
+          l[n][e] *= keep;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) o[j][n][e] *= keep, o[j][n][2 + e] *= keep;
+#pragma unroll
+          for (int j = 0; j < kGroups; ++j) z[j][n][e] *= keep, z[j][n][2 + e] *= keep;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float ref = m[n][e] == -INFINITY ? 0.0f : m[n][e];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float& x = s[mt][n][2 * u + e];
+            x = exp2_approx(x - ref);
+            l[n][e] += x;
+          }
+      }
+
+    // values
+    constexpr int kPTerms = F32 ? 3 : 1;
+    constexpr uint32_t kMagic = 0x43004300u;  // two bf16 128
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        // operand B: P of this group, as (row g, tokens 2t, 2t + 1) of each 8 tokens
+        uint32_t b[kPTerms][NT][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int tok = mt * 16 + u * 8 + g;
+          float vs = param_scale(vp[tok * kGroups + k]);
+          if (!whole && !(here >> tok & 1)) vs = 0.0f;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float x0 = s[mt][n][2 * u] * vs, x1 = s[mt][n][2 * u + 1] * vs;
+#pragma unroll
+            for (int term = 0; term < kPTerms; ++term) {
+              const uint32_t v = pack_bf16(x0, x1);
+              x0 -= __uint_as_float(v << 16);
+              x1 -= __uint_as_float(v & 0xFFFF0000u);
+              b[term][n][u] = transpose_8x8(v);
+            }
+          }
+        }
+        // operand A: tokens 2t, 2t + 1 (u = 0) and 2t + 8, 2t + 9 (u = 1) of this lane's G / 8 channels, the lower
+        // half of them as row g of the group's G / 16 products, the upper as row g + 8
+        uint32_t lower[2], upper[2], zero[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int tok = mt * 16 + u * 8 + 2 * t;
+          const uint8_t* at = vc + tok * kPitch + k * (G / 2) + g * (G / 16);
+          if constexpr (G == 64) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(at), y = *reinterpret_cast<const uint32_t*>(at + kPitch);
+            lower[u] = __byte_perm(x, y, 0x5410);
+            upper[u] = __byte_perm(x, y, 0x7632);
+          } else {
+            const uint32_t x = *reinterpret_cast<const uint16_t*>(at), y = *reinterpret_cast<const uint16_t*>(at + kPitch);
+            lower[u] = x | y << 16;
+            upper[u] = lower[u] >> 8;
+          }
+          zero[u] = __byte_perm(vp[tok * kGroups + k], vp[(tok + 1) * kGroups + k], 0x7632) & 0x00FF00FFu | kMagic;
+        }
+#pragma unroll
+        for (int j = 0; j < G / 16; ++j) {
+          uint32_t a0 = and_or(lower[0] >> (4 * j), 0x000F000Fu, kMagic), a1 = and_or(upper[0] >> (4 * j), 0x000F000Fu, kMagic);
+          uint32_t a2 = and_or(lower[1] >> (4 * j), 0x000F000Fu, kMagic), a3 = and_or(upper[1] >> (4 * j), 0x000F000Fu, kMagic);
+          if constexpr (F32) {
+            a0 = sub_bf16x2(a0, zero[0]);
+            a1 = sub_bf16x2(a1, zero[0]);
+            a2 = sub_bf16x2(a2, zero[1]);
+            a3 = sub_bf16x2(a3, zero[1]);
+          }
+#pragma unroll
+          for (int term = 0; term < kPTerms; ++term)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16(o[k * (G / 16) + j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
+        }
+        if constexpr (!F32) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_bf16(z[k][n], zero[0], zero[0], zero[1], zero[1], b[0][n][0], b[0][n][1]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) held[i] = held[i + 1];
+    slot = slot + 1 == kStages ? 0 : slot + 1;
+    fill = fill + 1 == kStages ? 0 : fill + 1;
+  }
+
+  // join the warps: maxima and totals, then the sums through shared memory (the rings are done with)
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(~0u, l[n][e], x);
+      if (g == 0) {
+        float* ml = row_ml + (warp * kRows + n * 8 + 2 * t + e) * 2;
+        ml[0] = m[n][e];
+        ml[1] = l[n][e];
+      }
+    }
+  copy_wait<0>();
+  __syncthreads();
+  float* const sums = reinterpret_cast<float*>(smem);  // [kWarps][kRows][D + 4]
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = n * 8 + 2 * t + e;
+      float now = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) now = fmaxf(now, row_ml[(w * kRows + r) * 2]);
+      const float keep = m[n][e] == -INFINITY ? 0.0f : exp2_approx(m[n][e] - now);
+      float* to = sums + (warp * kRows + r) * (D + 4);
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float v[G / 16];
+#pragma unroll
+          for (int j = 0; j < G / 16; ++j) v[j] = (o[k * (G / 16) + j][n][2 * u + e] - z[k][n][2 * u + e]) * keep;
+          float* p = to + k * G + g * (G / 8) + u * (G / 16);
+          if constexpr (G == 64)
+            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+          else
+            *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+        }
+    }
+  __syncthreads();
+
+  // the block's rows: straight to the output, or to the workspace for the unit's last block to join
+  auto out_index = [&](int r) {
+    const int rr = tile * kRows + r;
+    return (static_cast<long long>(seq) * a.tq + rr / ratio) * a.hq + head * ratio + rr % ratio;
+  };
+  constexpr int kThreads = kWarps * 32;
+  const size_t unit_rows = static_cast<size_t>(base + static_cast<long long>(unit) * splits) * kRows;
+  for (int i = tid; i < rows * D; i += kThreads) {
+    const int r = i / D, d = i % D;
+    float now = -INFINITY, total = 0.0f, v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) now = fmaxf(now, row_ml[(w * kRows + r) * 2]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = row_ml[(w * kRows + r) * 2];
+      total += mw == -INFINITY ? 0.0f : row_ml[(w * kRows + r) * 2 + 1] * exp2_approx(mw - now);
+      v += sums[(w * kRows + r) * (D + 4) + d];
+    }
+    if (splits == 1) {
+      store_any(a.ftype, a.out, out_index(r) * D + d, total > 0.0f ? v / total : total == 0.0f ? 0.0f : total);
+      if (d == 0 && a.lse) a.lse[out_index(r)] = total > 0.0f ? (now + log2f(total)) * 0.69314718055994531f : total == 0.0f ? -INFINITY : total;
+    } else {
+      a.partial[(unit_rows + split * kRows + r) * D + d] = v;
+      if (d == 0) {
+        float* ml = a.partial_ml + (unit_rows + split * kRows + r) * 2;
+        ml[0] = now;
+        ml[1] = total;
+      }
+    }
+  }
+  if (splits == 1) return;
+
+  __shared__ unsigned arrived;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    arrived = atomicAdd(a.counters + base + unit, 1u);
+    if (arrived + 1 == static_cast<unsigned>(splits)) a.counters[base + unit] = 0;  // for the next launch
+  }
+  __syncthreads();
+  if (arrived + 1 != static_cast<unsigned>(splits)) return;
+  __threadfence();
+  for (int i = tid; i < rows * D; i += kThreads) {
+    const int r = i / D, d = i % D;
+    float now = -INFINITY, total = 0.0f, v = 0.0f;
+    for (int j = 0; j < splits; ++j) now = fmaxf(now, __ldcg(a.partial_ml + (unit_rows + j * kRows + r) * 2));
+    for (int j = 0; j < splits; ++j) {
+      const float mj = __ldcg(a.partial_ml + (unit_rows + j * kRows + r) * 2);
+      const float keep = mj == -INFINITY ? 0.0f : exp2_approx(mj - now);
+      total += keep * __ldcg(a.partial_ml + (unit_rows + j * kRows + r) * 2 + 1);
+      v += keep * __ldcg(a.partial + (unit_rows + j * kRows + r) * D + d);
+    }
+    store_any(a.ftype, a.out, out_index(r) * D + d, total > 0.0f ? v / total : total == 0.0f ? 0.0f : total);
+    if (d == 0 && a.lse) a.lse[out_index(r)] = total > 0.0f ? (now + log2f(total)) * 0.69314718055994531f : total == 0.0f ? -INFINITY : total;
+  }
+}
+
+}  // namespace b200q
