@@ -30,66 +30,126 @@ struct AppendArgs {
   long long ts[2], hs[2];
   const int64_t* slots;
   int t;
+  bool vec;  // rows are 16-byte aligned
   int* err;
 };
 
-// One thread per group.
+// Appending and reading move bytes: a row (one token's head, of the keys or the values) lies in D / 8 lanes of 8
+// channels, one word of codes; a lane has kAhead rows on their way at a time, and a block's lanes take rows side by
+// side in memory.
+constexpr int kMoveThreads = 128;
+constexpr int kAhead = 4;
+
+// Row i of a call: token, keys or values, head.
+struct MoveRow {
+  int t, which, h;
+  bool ok;
+  long long slot;
+};
+__device__ __forceinline__ MoveRow move_row(const Cache& c, long long i, int t, const int64_t* slots, int* err) {
+  MoveRow r;
+  r.t = static_cast<int>(i / (2 * c.heads));
+  const int rest = static_cast<int>(i - static_cast<long long>(r.t) * 2 * c.heads);
+  r.which = rest >= c.heads;
+  r.h = rest - (r.which ? c.heads : 0);
+  r.ok = r.t < t;
+  r.slot = r.ok ? slots[r.t] : -1;
+  if (r.ok) r.ok = slot_ok(c, r.slot, err);
+  return r;
+}
+
+// Eight channels as fp32; `vec`: rows are 16-byte aligned.
 template <typename T>
-__global__ void kv4_append_kernel(Cache c, AppendArgs a) {
-  const int groups = c.d / c.group;
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= 2ll * a.t * c.heads * groups) return;
-  const int g = static_cast<int>(i % groups), h = static_cast<int>(i / groups % c.heads);
-  const long long r = i / groups / c.heads;
-  const int which = static_cast<int>(r % 2), t = static_cast<int>(r / 2);
-  const long long slot = a.slots[t];
-  if (!slot_ok(c, slot, a.err)) return;
-  const T* x = static_cast<const T*>(a.x[which]) + t * a.ts[which] + h * a.hs[which] + g * c.group;
-  float lo = 0.0f, hi = 0.0f;
-  for (int j = 0; j < c.group; ++j) {
-    const float v = to_f32(x[j]);
-    lo = fminf(lo, v);
-    hi = fmaxf(hi, v);
-  }
-  const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
-  float s = __bfloat162float(sb);
-  uint32_t bits = __bfloat16_as_ushort(sb);
-  if (!(s >= 1.17549435e-38f)) {
-    s = 0.0f;
-    bits = 0;
-  }
-  const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
-  const float z = fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f);
-  const size_t row = cache_row(c, slot, h);
-  c.params[which][row * groups + g] = bits | static_cast<uint32_t>(z) << 16;
-  uint8_t* out = c.codes[which] + row * (c.d / 2) + g * c.group / 2;
-  for (int j = 0; j < c.group; j += 2) {
-    uint32_t q[2];
-    for (int u = 0; u < 2; ++u)
-      q[u] = static_cast<uint32_t>(fminf(fmaxf(rintf(__fmul_rn(to_f32(x[j + u]), inv)) + z, 0.0f), 15.0f));
-    out[j / 2] = static_cast<uint8_t>(q[0] | q[1] << 4);
+__device__ __forceinline__ void load_eight(const T* p, bool ok, bool vec, T (&v)[8]) {
+  uint4* to = reinterpret_cast<uint4*>(v);
+  if (vec || !ok) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+      to[i] = ok ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = p[j];
   }
 }
 
-template <typename T>
-__global__ void kv4_read_kernel(Cache c, const int64_t* slots, T* k, T* v, int t, int* err) {
-  const int bytes = c.d / 2;
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= 2ll * t * c.heads * bytes) return;
-  const int b = static_cast<int>(i % bytes), h = static_cast<int>(i / bytes % c.heads);
-  const long long r = i / bytes / c.heads;
-  const int which = static_cast<int>(r % 2), tok = static_cast<int>(r / 2);
-  T* out = (which ? v : k) + (static_cast<long long>(tok) * c.heads + h) * c.d + 2 * b;
-  const long long slot = slots[tok];
-  if (!slot_ok(c, slot, err)) {
-    out[0] = out[1] = from_f32<T>(0.0f);
-    return;
+template <typename T, int D>
+__global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Cache c, AppendArgs a) {
+  constexpr int kLanes = D / 8, kRows = kMoveThreads / kLanes;
+  const int l = threadIdx.x % kLanes;
+  const long long first = static_cast<long long>(blockIdx.x) * (kRows * kAhead) + threadIdx.x / kLanes;
+  MoveRow row[kAhead];
+  alignas(16) T raw[kAhead][8];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    row[u] = move_row(c, first + u * kRows, a.t, a.slots, a.err);
+    const MoveRow& r = row[u];
+    load_eight(static_cast<const T*>(a.x[r.which]) + r.t * a.ts[r.which] + r.h * a.hs[r.which] + l * 8, r.ok, a.vec, raw[u]);
   }
-  const size_t row = cache_row(c, slot, h);
-  const uint32_t byte = c.codes[which][row * bytes + b];
-  const uint32_t p = c.params[which][row * (c.d / c.group) + 2 * b / c.group];
-  out[0] = from_f32<T>((static_cast<float>(byte & 15u) - param_zero(p)) * param_scale(p));
-  out[1] = from_f32<T>((static_cast<float>(byte >> 4) - param_zero(p)) * param_scale(p));
+  const int per_group = c.group / 8;  // lanes of a group
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    const MoveRow& r = row[u];
+    float x[8], lo = 0.0f, hi = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = to_f32(raw[u][j]);
+      lo = fminf(lo, x[j]);
+      hi = fmaxf(hi, x[j]);
+    }
+    for (int o = per_group / 2; o; o >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
+    }
+    // the format's own fp32 steps, each rounded once; bf16 scales keep fp32's range
+    const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
+    float s = __bfloat162float(sb);
+    uint32_t bits = __bfloat16_as_ushort(sb);
+    if (!(s >= 1.17549435e-38f)) s = 0.0f, bits = 0;
+    const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+    const float z = fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f);
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      word |= static_cast<uint32_t>(fminf(fmaxf(rintf(__fmul_rn(x[j], inv)) + z, 0.0f), 15.0f)) << (4 * j);
+    if (r.ok) {
+      const size_t at = cache_row(c, r.slot, r.h);
+      reinterpret_cast<uint32_t*>(c.codes[r.which])[at * (D / 8) + l] = word;
+      if (l % per_group == 0)
+        c.params[r.which][at * (D / c.group) + l / per_group] = bits | static_cast<uint32_t>(z) << 16;
+    }
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(Cache c, const int64_t* slots, T* k, T* v, int t, int* err) {
+  constexpr int kLanes = D / 8, kRows = kMoveThreads / kLanes;
+  const int l = threadIdx.x % kLanes;
+  const long long first = static_cast<long long>(blockIdx.x) * (kRows * kAhead) + threadIdx.x / kLanes;
+  MoveRow row[kAhead];
+  uint32_t word[kAhead], param[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    row[u] = move_row(c, first + u * kRows, t, slots, err);
+    const MoveRow& r = row[u];
+    word[u] = param[u] = 0;  // a scale of zero
+    if (r.ok) {
+      const size_t at = cache_row(c, r.slot, r.h);
+      word[u] = __ldg(reinterpret_cast<const uint32_t*>(c.codes[r.which]) + at * (D / 8) + l);
+      param[u] = __ldg(c.params[r.which] + at * (D / c.group) + l * 8 / c.group);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    const MoveRow& r = row[u];
+    if (r.t >= t) continue;
+    const float s = param_scale(param[u]), z = param_zero(param[u]);
+    alignas(16) T out[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = from_f32<T>((static_cast<float>((word[u] >> (4 * j)) & 15u) - z) * s);
+    uint4* to = reinterpret_cast<uint4*>((r.which ? v : k) + (static_cast<long long>(r.t) * c.heads + r.h) * D + l * 8);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) to[i] = reinterpret_cast<const uint4*>(out)[i];
+  }
 }
 
 int check_cache(const b200q_kv4_cache* p, Cache* c) {
@@ -106,6 +166,14 @@ int check_cache(const b200q_kv4_cache* p, Cache* c) {
        reinterpret_cast<uintptr_t>(p->k_params) | reinterpret_cast<uintptr_t>(p->v_params)) & 15u)
     return host_fail(B200Q_ERR_INVALID_ARG, "cache tensors must be 16-byte aligned");
   *c = Cache{{p->k_codes, p->v_codes}, {p->k_params, p->v_params}, p->pages, p->heads, p->page_size, p->d, p->group};
+  return B200Q_OK;
+}
+
+int move_blocks(const Cache& c, int t, int* blocks) {
+  const int rows = kMoveThreads / (c.d / 8) * kAhead;
+  const long long n = (2ll * t * c.heads + rows - 1) / rows;
+  if (n > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many tokens");
+  *blocks = static_cast<int>(n);
   return B200Q_OK;
 }
 
@@ -164,13 +232,18 @@ extern "C" int b200q_kv4_append(const b200q_kv4_cache* cache, const void* k, lon
   if (t < 0) return host_fail(B200Q_ERR_INVALID_ARG, "negative token count");
   if (t == 0) return B200Q_OK;
   if (!k || !v || !slots) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
-  AppendArgs a{{k, v}, {k_ts, v_ts}, {k_hs, v_hs}, slots, t, nullptr};
+  const int size = ftype == B200Q_F32 ? 4 : 2;
+  const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 &&
+                   ((k_ts | k_hs | v_ts | v_hs) * size) % 16 == 0;
+  AppendArgs a{{k, v}, {k_ts, v_ts}, {k_hs, v_hs}, slots, t, vec, nullptr};
   int sms = 0;
   if ((rc = host_device(&sms, &a.err))) return rc;
-  const long long blocks = (2ll * t * c.heads * (c.d / c.group) + 127) / 128;
-  if (blocks > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many tokens");
-  B200Q_DISPATCH_FTYPE(ftype, (kv4_append_kernel<T><<<static_cast<int>(blocks), 128, 0,
-                                                      static_cast<cudaStream_t>(stream)>>>(c, a)));
+  int blocks = 0;
+  if ((rc = move_blocks(c, t, &blocks))) return rc;
+  B200Q_DISPATCH_FTYPE(ftype, (c.d == 64    ? kv4_append_kernel<T, 64>
+                               : c.d == 128 ? kv4_append_kernel<T, 128>
+                                            : kv4_append_kernel<T, 256>)<<<blocks, kMoveThreads, 0,
+                                                                           static_cast<cudaStream_t>(stream)>>>(c, a));
   rc = host_check_launch("kv4_append_kernel launch");
   if (rc == B200Q_OK) host_set_path(19);
   return rc;
@@ -186,11 +259,15 @@ extern "C" int b200q_kv4_read(const b200q_kv4_cache* cache, const int64_t* slots
   if (!k || !v || !slots) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
   int sms = 0, *err = nullptr;
   if ((rc = host_device(&sms, &err))) return rc;
-  const long long blocks = (2ll * t * c.heads * (c.d / 2) + 255) / 256;
-  if (blocks > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many tokens");
-  B200Q_DISPATCH_FTYPE(ftype, (kv4_read_kernel<T><<<static_cast<int>(blocks), 256, 0,
-                                                    static_cast<cudaStream_t>(stream)>>>(
-                                  c, slots, static_cast<T*>(k), static_cast<T*>(v), t, err)));
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u)
+    return host_fail(B200Q_ERR_INVALID_ARG, "kv4_read outputs must be 16-byte aligned");
+  int blocks = 0;
+  if ((rc = move_blocks(c, t, &blocks))) return rc;
+  B200Q_DISPATCH_FTYPE(ftype, (c.d == 64    ? kv4_read_kernel<T, 64>
+                               : c.d == 128 ? kv4_read_kernel<T, 128>
+                                            : kv4_read_kernel<T, 256>)<<<blocks, kMoveThreads, 0,
+                                                                         static_cast<cudaStream_t>(stream)>>>(
+                                  c, slots, static_cast<T*>(k), static_cast<T*>(v), t, err));
   rc = host_check_launch("kv4_read_kernel launch");
   if (rc == B200Q_OK) host_set_path(19);
   return rc;
