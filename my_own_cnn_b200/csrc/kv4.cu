@@ -193,23 +193,19 @@ int launch_attention(const Cache& c, AttnArgs a, int sms, cudaStream_t stream) {
     per_sm.store(resident, std::memory_order_relaxed);
   }
   a.row_tiles = (a.tq * (a.hq / c.heads) + 8 * NT - 1) / (8 * NT);
-  const long long units = static_cast<long long>(a.b) * c.heads * a.row_tiles;
-  long long blocks = units;
-  const int target = sms * resident * kWaves;
-  const long long most = (static_cast<long long>(a.max_pages) * c.page_size + kMinChunk - 1) / kMinChunk;
-  if (most > 1 && units < target) {
-    // units split so that each block has 1 / target of the tokens: at most one block more per unit
-    blocks = std::min<long long>(target + units, units * most);
-    a.target = target;
-    const size_t rows = static_cast<size_t>(blocks) * 8 * NT;
-    void* ws = nullptr;
-    int rc = host_workspace(rows * (D + 2) * sizeof(float), stream, &ws);
-    if (rc || (rc = host_counters(stream, &a.counters))) return rc;
-    a.partial = static_cast<float*>(ws);
-    a.partial_ml = a.partial + rows * D;
-  }
-  if (blocks > (a.target ? kSplitCounters : 0x7fffffffll)) return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
-  kernel<<<static_cast<int>(blocks), kWarps * 32, Shape::kSmem, stream>>>(c, a);
+  // one block for each that the GPU holds at once; fewer when even the longest lengths have fewer steps
+  const long long steps = (static_cast<long long>(a.max_pages) * c.page_size + kStepTokens - 1) / kStepTokens;
+  const long long most = static_cast<long long>(a.b) * c.heads * a.row_tiles * std::max(1ll, (steps + kMinSteps - 1) / kMinSteps);
+  // (a unit's parts, one per block at most, leave their shares in shared memory when they are joined)
+  const int blocks = static_cast<int>(std::min<long long>(std::min(sms * resident, Shape::kBody / (8 * NT * 4)), most));
+  const size_t rows = static_cast<size_t>(blocks) * 2 * 8 * NT;
+  void* ws = nullptr;
+  int rc = host_workspace(rows * (D + 2) * sizeof(float), stream, &ws);
+  if (rc || (rc = host_counters(stream, &a.counters))) return rc;
+  a.partial = static_cast<float*>(ws);
+  a.partial_ml = a.partial + rows * D;
+  if (blocks > kSplitCounters) return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
+  kernel<<<blocks, kWarps * 32, Shape::kSmem, stream>>>(c, a);
   return host_check_launch("kv4_attention_kernel launch");
 }
 

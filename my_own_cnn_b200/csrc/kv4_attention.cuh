@@ -9,13 +9,18 @@
 //   code * 2^-20: a word of 8 codes becomes four operands by masking, and every second query value is divided
 //   by 16 instead.  Query rows are scaled by a power of two to a maximum in [2^14, 2^15), so that they fit
 //   fp16 whatever their type; fp32 rows are split into two fp16 terms (22 bits).
-//   Values: the bf16 with mantissa bits 0 to 3 set to the code is 128 + code; bf16 keeps P's range, which follows
-//   the scales.  The zero points (as 128 + vz) go through the same instruction as a 16-row operand of their own,
-//   and the difference of the two sums loses the 128.  fp32 calls subtract before the product instead, and split P
-//   into three bf16 terms: there the 128 would cost 5 bits of the sum.
+//   Values: the same subnormals, channels as rows: a channel whose nibble lies one place higher has its sum divided by
+//   16 at the end, the zero points go through the same instruction as a 16-row operand of their own and are
+//   subtracted last.  P is fp16 (11 bits; two terms, 22 bits, in fp32 calls) times a power of two that follows the largest
+//   vs that the warp has met, so that full precision holds for tokens whose vs is up to 2^20 below that.
 //   P leaves the first product as (token, row) and must enter the second as (row, token): movmatrix.
 // The maximum m[r] is a running reference, raised (and the sums rescaled) only when a score passes it by more than
-// 2^8: P stays far inside its range, and a warp-wide maximum is taken a few times per sequence, not per tile.
+// 2^8: a warp-wide maximum is taken a few times per sequence, not per tile.
+//
+// Work: a unit is (sequence, cache head, tile of rows), in steps of kWarps tiles of kTile tokens.  All units' steps lie
+// end to end, and block i takes steps [i * per, (i + 1) * per) of them, whatever the lengths (which only the device knows):
+// every block has the same work, and none waits for a last wave.  The parts of a unit that several blocks share go to
+// the workspace, and the block that finishes last joins them in order.
 //
 // What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head.  Each warp owns a ring of kStages tiles of
 // kTile tokens that it fills with 16-byte asynchronous copies and empties on its own: no block-wide barrier until
@@ -45,19 +50,19 @@ struct AttnArgs {
   float scale;
   int page_shift;       // log2 of the page size, or -1
   int row_tiles;        // tiles of 8 * NT rows of a cache head
-  int target;           // blocks that the tokens are split over, or 0: one block per (sequence, head, row tile)
-  float* partial;       // [block][8 NT][d] sums of a split unit
-  float* partial_ml;    // [block][8 NT][2] maximum and total
-  unsigned* counters;   // [block]
+  float* partial;       // [block][2][8 NT][d] sums of a part: of a unit begun by an earlier block, of one begun here
+  float* partial_ml;    // [block][2][8 NT][2] maximum and total
+  unsigned* counters;   // [block], for the unit begun here
   int* err;
 };
 
-constexpr int kMinChunk = 256;  // tokens of a block at least
-constexpr int kWaves = 2;       // blocks that the tokens are split over, in units of what the GPU holds at once
+constexpr int kMinSteps = 2;  // steps of a block at least
+constexpr int kUnitSteps = 3; // what a unit costs besides its steps (its queries, its first tiles' way, its join), in steps
 
 constexpr int kTile = 32;    // tokens of a warp's step
 constexpr int kWarps = 4;    // a block's warps take tiles in turn
 constexpr int kStages = 3;
+constexpr int kStepTokens = kWarps * kTile;
 
 template <int D, int G, int NT, bool F32>
 struct AttnShape {
@@ -147,59 +152,62 @@ __device__ __forceinline__ float zero_point(uint32_t p) {
 }
 
 template <int D, int G, int NT, bool F32>
-__global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_attention_kernel(Cache c, AttnArgs a) {
   using Shape = AttnShape<D, G, NT, F32>;
   constexpr int kGroups = Shape::kGroups, kPitch = Shape::kPitch, kRows = 8 * NT, kTerms = Shape::kTerms;
   extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ unsigned arrived;
   uint4* const query = reinterpret_cast<uint4*>(smem + Shape::kBody);
   float* const row_ml = reinterpret_cast<float*>(smem + Shape::kBody + Shape::kQuery);
   float* const row_sum = row_ml + kWarps * kRows * 2;  // [kGroups][kRows] sums of the scaled query, times 2^-24
   float* const row_f = row_sum + kRows * kGroups;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4;
 
-  // A unit is (sequence, head, row tile); a sequence's units are split over the same number of blocks, so that every
-  // block has about 1 / target of all tokens, whatever the lengths (which only the device knows).
-  const int units = c.heads * a.row_tiles;
-  int seq = 0, local, splits = 1, chunk = 1 << 30;
-  long long base = 0;  // first block of the sequence
-  if (a.target == 0) {
-    seq = blockIdx.x / units;
-    local = blockIdx.x % units;
-  } else {
-    long long total = 0;
-    for (int i = lane; i < a.b; i += 32) total += valid_length(c, a, i);
+  const int units = c.heads * a.row_tiles, ratio = a.hq / c.heads;
+  auto steps_of = [&](int i) { return kUnitSteps + max(1, (valid_length(c, a, i) + kStepTokens - 1) / kStepTokens); };
+  long long total = 0;
+  for (int i = lane; i < a.b; i += 32) total += steps_of(i);
 #pragma unroll
-    for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
-    chunk = max(kMinChunk, static_cast<int>(min(1ll << 30, (total * units / a.target + 128) / 128 * 128)));
-    for (;; seq += 32) {
-      if (seq >= a.b) return;  // more blocks were launched than these lengths need
-      const int n = seq + lane < a.b ? max(1, (valid_length(c, a, seq + lane) + chunk - 1) / chunk) : 0;
-      int sum = n;
+  for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
+  total *= units;
+  const long long per = max(static_cast<long long>(kMinSteps), (total + gridDim.x - 1) / gridDim.x);
+  long long at = blockIdx.x * per;  // the block's next step
+  const long long stop = min(total, at + per);
+  if (at >= stop) return;
+  int seq = 0;
+  long long base = 0;  // first step of the sequence
+  for (;; seq += 32) {
+    long long sum = seq + lane < a.b ? static_cast<long long>(steps_of(seq + lane)) * units : 0;
 #pragma unroll
-      for (int x = 1; x < 32; x <<= 1) {
-        const int v = __shfl_up_sync(~0u, sum, x);
-        if (lane >= x) sum += v;
-      }
-      const unsigned past = __ballot_sync(~0u, base + static_cast<long long>(sum) * units > blockIdx.x);
-      if (past) {
-        const int at = __ffs(past) - 1;
-        seq += at;
-        splits = __shfl_sync(~0u, n, at);
-        base += static_cast<long long>(__shfl_sync(~0u, sum, at) - splits) * units;
-        break;
-      }
-      base += static_cast<long long>(__shfl_sync(~0u, sum, 31)) * units;
+    for (int x = 1; x < 32; x <<= 1) {
+      const long long v = __shfl_up_sync(~0u, sum, x);
+      if (lane >= x) sum += v;
     }
-    local = static_cast<int>(blockIdx.x - base);
+    const unsigned past = __ballot_sync(~0u, base + sum > at);
+    const int first = past ? __ffs(past) - 1 : 31;
+    const long long before = __shfl_sync(~0u, sum, past ? first - 1 : 31);  // lane -1 is lane 31, and not used
+    if (!past || first > 0) base += before;
+    if (past) {
+      seq += first;
+      break;
+    }
   }
-  // blocks of the same tokens run next to each other: their heads lie side by side in a page
-  const int split = local / units, unit = local % units;
-  const int tile = unit % a.row_tiles, head = unit / a.row_tiles;
-  const int ratio = a.hq / c.heads, rows = min(kRows, a.tq * ratio - tile * kRows);
-  const int len = valid_length(c, a, seq);
+
+ for (; at < stop;) {
+  // steps [off, off + count) of the unit; its first kUnitSteps steps stand for what it costs besides
+  const int n = steps_of(seq), len = valid_length(c, a, seq);
+  const int unit = static_cast<int>((at - base) / n);
+  const long long unit_at = base + static_cast<long long>(unit) * n;
+  const long long end = min(unit_at + n, stop);
+  const int off = max(0, static_cast<int>(at - unit_at) - kUnitSteps), count = static_cast<int>(end - unit_at) - kUnitSteps - off;
+  at = end;
+  if (count <= 0) break;  // all of it lies with the next block
+  const int tile = unit % a.row_tiles, head = unit / a.row_tiles, rows = min(kRows, a.tq * ratio - tile * kRows);
+  const long long owner = (unit_at + kUnitSteps) / per;  // the block that its first step lies with
+  const int parts = static_cast<int>((unit_at + n - 1) / per - owner) + 1;
   // the last row of the tile sees the most tokens
   const int seen = max(0, len - a.tq + (tile * kRows + rows - 1) / ratio + 1);
-  const int begin = split * chunk, until = min(seen, begin + chunk);
+  const int begin = off * kStepTokens, until = min(seen, begin + count * kStepTokens);
   const int32_t* pages = a.table + seq * a.table_stride;
 
   // ring: the first tiles are on their way before the query is looked at
@@ -230,26 +238,22 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
                       : 0.0f;
       top = fmaxf(top, fabsf(v[i]));
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    // 2^up brings the maximum into [2^14, 2^15)
-    const int up = top > 0.0f ? min(120, 14 + 127 - static_cast<int>(__float_as_uint(top) >> 23)) : 0;
-    const float factor = __uint_as_float(static_cast<uint32_t>(127 + max(-126, up)) << 23);
-    if (lane == 0) row_f[r] = __uint_as_float(static_cast<uint32_t>(127 - max(-126, up)) << 23) * a.scale * 1.4426950408889634f * 16777216.0f;
+    const Power power = power_for(warp_max(top));
+    if (lane == 0) row_f[r] = power.down * a.scale * 1.4426950408889634f * 16777216.0f;
     // lane: channel p = lane % 8 of the 8 that thread lane / 8 of a quad holds; pairs are (0,4) (1,5) (2,6) (3,7)
-    const int p = lane % 8, owner = (r % 8) * 4 + lane / 8;
-    __half* at = reinterpret_cast<__half*>(query);
+    const int p = lane % 8, holder = (r % 8) * 4 + lane / 8;
+    __half* to = reinterpret_cast<__half*>(query);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      float x = v[i] * factor;
+      float x = v[i] * power.up;
 #pragma unroll
       for (int term = 0; term < kTerms; ++term) {
         const __half hv = __float2half_rn(x);
         const float back = __half2float(hv);
         sum += back;
         x -= back;
-        at[(((i * kTerms + term) * NT + r / 8) * 32 + owner) * 8 + (p % 4) * 2 + p / 4] =
+        to[(((i * kTerms + term) * NT + r / 8) * 32 + holder) * 8 + (p % 4) * 2 + p / 4] =
             p % 2 ? __float2half_rn(back * 0.0625f) : hv;
       }
       if ((i + 1) % (G / 32) == 0) {
@@ -286,6 +290,9 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
     for (int j = 0; j < kGroups; ++j) z[j][n][0] = z[j][n][1] = z[j][n][2] = z[j][n][3] = 0.0f;
   }
 
+  // P's power of two: 2^(127 - v_exp), for a largest vs of 2^(v_exp - 127)
+  int v_exp = 127;
+  float v_factor = 1.0f, v_limit = -1.0f;
   int slot = 0, fill = kStages - 1;
   for (int it = 0; it < mine; ++it) {
     copy_wait<kStages - 2>();
@@ -306,16 +313,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
     // scores
     float s[2][NT][4];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[mt][n][0] = s[mt][n][1] = s[mt][n][2] = s[mt][n][3] = 0.0f;
-#pragma unroll
     for (int k = 0; k < kGroups; ++k) {
       float part[2][NT][4];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) part[mt][n][0] = part[mt][n][1] = part[mt][n][2] = part[mt][n][3] = 0.0f;
 #pragma unroll
       for (int i = k * (G / 32); i < (k + 1) * (G / 32); ++i) {
         uint4 b[kTerms][NT];
@@ -332,8 +331,12 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
           for (int term = 0; term < kTerms; ++term)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              mma_f16(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
-                      b[term][n].x, b[term][n].y);
+              if (i == k * (G / 32) && term == 0)
+                mma_f16_first(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
+                              b[term][n].x, b[term][n].y);
+              else
+                mma_f16(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
+                        b[term][n].x, b[term][n].y);
               mma_f16(part[mt][n], v0 & 0x000F000Fu, v1 & 0x000F000Fu, v0 & 0x00F000F0u, v1 & 0x00F000F0u,
                       b[term][n].z, b[term][n].w);
             }
@@ -348,13 +351,29 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-              s[mt][n][2 * u + e] = fmaf(ks, fmaf(-kz, qsum[n][k][e], part[mt][n][2 * u + e]), s[mt][n][2 * u + e]);
+            for (int e = 0; e < 2; ++e) {
+              const float v = fmaf(-kz, qsum[n][k][e], part[mt][n][2 * u + e]);
+              s[mt][n][2 * u + e] = k == 0 ? ks * v : fmaf(ks, v, s[mt][n][2 * u + e]);
+            }
         }
     }
 
+    // this lane's scales of the values, tokens mt * 16 + u * 8 + g
+    float vs[2][2][kGroups], v_top = 0.0f;
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+          const int tok = mt * 16 + u * 8 + g;
+          vs[mt][u][k] = param_scale(vp[tok * kGroups + k]);
+          if (!whole && !(here >> tok & 1)) vs[mt][u][k] = 0.0f;
+          v_top = fmaxf(v_top, vs[mt][u][k]);
+        }
+
     // weights
-    bool raise = false;
+    bool raise = v_top > v_limit;
     float top[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -376,6 +395,17 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
         raise |= top[n][e] > m[n][e] + 8.0f;
       }
     if (__any_sync(~0u, raise)) {
+      float v_keep = 1.0f;
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) v_top = fmaxf(v_top, __shfl_xor_sync(~0u, v_top, x));
+      if (v_top > v_limit) {
+        const int now = max(1, min(247, static_cast<int>(__float_as_uint(v_top) >> 23)));
+        v_keep = now - v_exp < 127 ? __uint_as_float(static_cast<uint32_t>(127 + v_exp - now) << 23) : 0.0f;
+        if (v_limit < 0.0f) v_keep = 1.0f;  // no sums yet
+        v_exp = now;
+        v_factor = __uint_as_float(static_cast<uint32_t>(254 - now) << 23);
+        v_limit = __uint_as_float(static_cast<uint32_t>(now + 6) << 23);
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -383,9 +413,10 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(~0u, top[n][e], x));
           const float now = fmaxf(m[n][e], top[n][e]);
-          const float keep = now == -INFINITY ? 1.0f : exp2_approx(m[n][e] - now);
+          float keep = now == -INFINITY ? 1.0f : exp2_approx(m[n][e] - now);
           m[n][e] = now;
           l[n][e] *= keep;
+          keep *= v_keep;
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) o[j][n][e] *= keep, o[j][n][2 + e] *= keep;
 #pragma unroll
@@ -408,8 +439,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
       }
 
     // values
-    constexpr int kPTerms = F32 ? 3 : 1;
-    constexpr uint32_t kMagic = 0x43004300u;  // two bf16 128
+    constexpr int kPTerms = F32 ? 2 : 1;
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -418,17 +448,18 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
         uint32_t b[kPTerms][NT][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int tok = mt * 16 + u * 8 + g;
-          float vs = param_scale(vp[tok * kGroups + k]);
-          if (!whole && !(here >> tok & 1)) vs = 0.0f;
+          const float scale = vs[mt][u][k] * v_factor;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float x0 = s[mt][n][2 * u] * vs, x1 = s[mt][n][2 * u + 1] * vs;
+            float x0 = s[mt][n][2 * u] * scale, x1 = s[mt][n][2 * u + 1] * scale;
 #pragma unroll
             for (int term = 0; term < kPTerms; ++term) {
-              const uint32_t v = pack_bf16(x0, x1);
-              x0 -= __uint_as_float(v << 16);
-              x1 -= __uint_as_float(v & 0xFFFF0000u);
+              const uint32_t v = pack_f16(x0, x1);
+              if (term + 1 < kPTerms) {
+                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                x0 -= back.x;
+                x1 -= back.y;
+              }
               b[term][n][u] = transpose_8x8(v);
             }
           }
@@ -449,27 +480,24 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
             lower[u] = x | y << 16;
             upper[u] = lower[u] >> 8;
           }
-          zero[u] = __byte_perm(vp[tok * kGroups + k], vp[(tok + 1) * kGroups + k], 0x7632) & 0x00FF00FFu | kMagic;
+          zero[u] = __byte_perm(vp[tok * kGroups + k], vp[(tok + 1) * kGroups + k], 0x7632);
+          if (!whole) zero[u] &= 0x00FF00FFu;  // places that hold nothing hold any bits
         }
 #pragma unroll
         for (int j = 0; j < G / 16; ++j) {
-          uint32_t a0 = and_or(lower[0] >> (4 * j), 0x000F000Fu, kMagic), a1 = and_or(upper[0] >> (4 * j), 0x000F000Fu, kMagic);
-          uint32_t a2 = and_or(lower[1] >> (4 * j), 0x000F000Fu, kMagic), a3 = and_or(upper[1] >> (4 * j), 0x000F000Fu, kMagic);
-          if constexpr (F32) {
-            a0 = sub_bf16x2(a0, zero[0]);
-            a1 = sub_bf16x2(a1, zero[0]);
-            a2 = sub_bf16x2(a2, zero[1]);
-            a3 = sub_bf16x2(a3, zero[1]);
-          }
+          const int down = j / 2 * 8;
+          const uint32_t mask = j % 2 ? 0x00F000F0u : 0x000F000Fu;
+          const uint32_t a0 = lower[0] >> down & mask, a1 = upper[0] >> down & mask;
+          const uint32_t a2 = lower[1] >> down & mask, a3 = upper[1] >> down & mask;
 #pragma unroll
           for (int term = 0; term < kPTerms; ++term)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_bf16(o[k * (G / 16) + j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
+            for (int n = 0; n < NT; ++n) mma_f16(o[k * (G / 16) + j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
         }
-        if constexpr (!F32) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma_bf16(z[k][n], zero[0], zero[0], zero[1], zero[1], b[0][n][0], b[0][n][1]);
-        }
+        for (int term = 0; term < kPTerms; ++term)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_f16(z[k][n], zero[0], zero[0], zero[1], zero[1], b[term][n][0], b[term][n][1]);
       }
     }
 #pragma unroll
@@ -503,6 +531,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) now = fmaxf(now, row_ml[(w * kRows + r) * 2]);
       const float keep = m[n][e] == -INFINITY ? 0.0f : exp2_approx(m[n][e] - now);
+      const float value = __uint_as_float(static_cast<uint32_t>(v_exp) << 23);
       float* to = sums + (warp * kRows + r) * (D + 4);
 #pragma unroll
       for (int k = 0; k < kGroups; ++k)
@@ -510,7 +539,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
         for (int u = 0; u < 2; ++u) {
           float v[G / 16];
 #pragma unroll
-          for (int j = 0; j < G / 16; ++j) v[j] = (o[k * (G / 16) + j][n][2 * u + e] - z[k][n][2 * u + e]) * keep;
+          for (int j = 0; j < G / 16; ++j) v[j] = fmaf(o[k * (G / 16) + j][n][2 * u + e], j % 2 ? 0.0625f : 1.0f, -z[k][n][2 * u + e]) * 16777216.0f * value * keep;
           float* p = to + k * G + g * (G / 8) + u * (G / 16);
           if constexpr (G == 64)
             *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
@@ -525,56 +554,83 @@ __global__ void __launch_bounds__(kWarps * 32) kv4_attention_kernel(Cache c, Att
     const int rr = tile * kRows + r;
     return (static_cast<long long>(seq) * a.tq + rr / ratio) * a.hq + head * ratio + rr % ratio;
   };
+  auto finish = [&](int r, int d, float v, float sum, float now) {
+    store_any(a.ftype, a.out, out_index(r) * D + d, sum > 0.0f ? v / sum : sum == 0.0f ? 0.0f : sum);
+    if (d == 0 && a.lse) a.lse[out_index(r)] = sum > 0.0f ? (now + log2f(sum)) * 0.69314718055994531f : sum == 0.0f ? -INFINITY : sum;
+  };
   constexpr int kThreads = kWarps * 32;
-  const size_t unit_rows = static_cast<size_t>(base + static_cast<long long>(unit) * splits) * kRows;
+  const int mine_at = (2 * blockIdx.x + (off == 0)) * kRows;
   for (int i = tid; i < rows * D; i += kThreads) {
     const int r = i / D, d = i % D;
-    float now = -INFINITY, total = 0.0f, v = 0.0f;
+    float now = -INFINITY, sum = 0.0f, v = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) now = fmaxf(now, row_ml[(w * kRows + r) * 2]);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float mw = row_ml[(w * kRows + r) * 2];
-      total += mw == -INFINITY ? 0.0f : row_ml[(w * kRows + r) * 2 + 1] * exp2_approx(mw - now);
+      sum += mw == -INFINITY ? 0.0f : row_ml[(w * kRows + r) * 2 + 1] * exp2_approx(mw - now);
       v += sums[(w * kRows + r) * (D + 4) + d];
     }
-    if (splits == 1) {
-      store_any(a.ftype, a.out, out_index(r) * D + d, total > 0.0f ? v / total : total == 0.0f ? 0.0f : total);
-      if (d == 0 && a.lse) a.lse[out_index(r)] = total > 0.0f ? (now + log2f(total)) * 0.69314718055994531f : total == 0.0f ? -INFINITY : total;
+    if (parts == 1) {
+      finish(r, d, v, sum, now);
     } else {
-      a.partial[(unit_rows + split * kRows + r) * D + d] = v;
+      a.partial[static_cast<size_t>(mine_at + r) * D + d] = v;
       if (d == 0) {
-        float* ml = a.partial_ml + (unit_rows + split * kRows + r) * 2;
+        float* ml = a.partial_ml + static_cast<size_t>(mine_at + r) * 2;
         ml[0] = now;
-        ml[1] = total;
+        ml[1] = sum;
       }
     }
   }
-  if (splits == 1) return;
-
-  __shared__ unsigned arrived;
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) {
-    arrived = atomicAdd(a.counters + base + unit, 1u);
-    if (arrived + 1 == static_cast<unsigned>(splits)) a.counters[base + unit] = 0;  // for the next launch
-  }
-  __syncthreads();
-  if (arrived + 1 != static_cast<unsigned>(splits)) return;
-  __threadfence();
-  for (int i = tid; i < rows * D; i += kThreads) {
-    const int r = i / D, d = i % D;
-    float now = -INFINITY, total = 0.0f, v = 0.0f;
-    for (int j = 0; j < splits; ++j) now = fmaxf(now, __ldcg(a.partial_ml + (unit_rows + j * kRows + r) * 2));
-    for (int j = 0; j < splits; ++j) {
-      const float mj = __ldcg(a.partial_ml + (unit_rows + j * kRows + r) * 2);
-      const float keep = mj == -INFINITY ? 0.0f : exp2_approx(mj - now);
-      total += keep * __ldcg(a.partial_ml + (unit_rows + j * kRows + r) * 2 + 1);
-      v += keep * __ldcg(a.partial + (unit_rows + j * kRows + r) * D + d);
+  if (parts > 1) {
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      arrived = atomicAdd(a.counters + owner, 1u);
+      if (arrived + 1 == static_cast<unsigned>(parts)) a.counters[owner] = 0;  // for the next launch
     }
-    store_any(a.ftype, a.out, out_index(r) * D + d, total > 0.0f ? v / total : total == 0.0f ? 0.0f : total);
-    if (d == 0 && a.lse) a.lse[out_index(r)] = total > 0.0f ? (now + log2f(total)) * 0.69314718055994531f : total == 0.0f ? -INFINITY : total;
+    __syncthreads();
+    if (arrived + 1 == static_cast<unsigned>(parts)) {
+      __threadfence();
+      // part j lies with block owner + j: the first as the unit begun there, the others as the one begun before
+      auto part_row = [&](int j, int r) { return static_cast<size_t>((2 * (owner + j) + (j == 0)) * kRows + r); };
+      // what each part counts for, [row][part], and the rows' totals
+      float* const share = reinterpret_cast<float*>(smem);
+      for (int r = warp; r < rows; r += kWarps) {
+        float now = -INFINITY, sum = 0.0f;
+        for (int j = lane; j < parts; j += 32) now = fmaxf(now, __ldcg(a.partial_ml + part_row(j, r) * 2));
+#pragma unroll
+        for (int x = 16; x; x >>= 1) now = fmaxf(now, __shfl_xor_sync(~0u, now, x));
+        for (int j = lane; j < parts; j += 32) {
+          const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.partial_ml + part_row(j, r) * 2));
+          const float keep = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - now);
+          share[r * parts + j] = keep;
+          sum += keep * ml.y;
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) row_ml[2 * r] = now, row_ml[2 * r + 1] = sum;
+      }
+      __syncthreads();
+      for (int i = tid; i < rows * D / 4; i += kThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+        for (int j = 0; j < parts; ++j) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(a.partial + part_row(j, r) * D + d));
+          const float keep = share[r * parts + j];
+          v.x = fmaf(keep, x.x, v.x), v.y = fmaf(keep, x.y, v.y), v.z = fmaf(keep, x.z, v.z), v.w = fmaf(keep, x.w, v.w);
+        }
+        const float now = row_ml[2 * r], sum = row_ml[2 * r + 1];
+        finish(r, d, v.x, sum, now);
+        finish(r, d + 1, v.y, sum, now);
+        finish(r, d + 2, v.z, sum, now);
+        finish(r, d + 3, v.w, sum, now);
+      }
+    }
   }
+  __syncthreads();  // shared memory is free for the next unit
+  if (at == base + static_cast<long long>(n) * units) base = at, ++seq;
+ }
 }
 
 }  // namespace b200q

@@ -21,6 +21,21 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// A power of two that brings `top` into [2^14, 2^15), as fp16 operands want it, and its inverse (1 for 0).
+struct Power {
+  float up, down;
+};
+__device__ __forceinline__ Power power_for(float top) {
+  const int e = top > 0.0f ? max(-113, min(113, 14 + 127 - static_cast<int>(__float_as_uint(top) >> 23))) : 0;
+  return {__uint_as_float(static_cast<uint32_t>(127 + e) << 23), __uint_as_float(static_cast<uint32_t>(127 - e) << 23)};
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
+  return v;
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
@@ -31,51 +46,34 @@ __device__ __forceinline__ float warp_sum(float v) {
 __device__ __forceinline__ float param_scale(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float param_zero(uint32_t p) { return static_cast<float>((p >> 16) & 0xffu); }
 
-// D = A B + C on one warp, m16 n8 k16: fp16 or bf16 operands, fp32 sums.  Lane (g = lane / 4, t = lane % 4):
+// C += A B on one warp, m16 n8 k16: fp16 operands, fp32 sums.  Lane (g = lane / 4, t = lane % 4):
 // a0, a2 hold row g (k 2t, 2t+1 and 2t+8, 2t+9), a1, a3 row g + 8; b0, b1 the same k of column g;
 // c0, c1 row g, columns 2t, 2t+1; c2, c3 row g + 8.
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// D = A B
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // Transposes an 8 x 8 matrix of 16-bit values held as row g, columns 2t, 2t+1.
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// a - b on two bf16 values (exact for the small integers that it is used on).
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-// (a & mask) | bits
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
   return r;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -84,7 +82,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return r;
 }
 
-// Asynchronous copies of 4, 8 or 16 bytes into shared memory.  `from` bytes are read, the rest is zero.
+// Asynchronous copies of 4, 8 or 16 bytes into shared memory.
 __device__ __forceinline__ uint32_t shared_address(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

@@ -1,21 +1,22 @@
 // Linear layers with 4-bit weights and group scales (b200q_linear_w4).
 //
-//   y[m][n] = sum_g s[g][n] (sum_{k in g} c[n][k] x[m][k]  -  z[g][n] sum_{k in g} x[m][k])
+//   y[m][n] = sum_g s[g][n] sum_{k in g} c[n][k] x[m][k]  -  sum_g s[g][n] z[g][n] sum_{k in g} x[m][k]
 //
 // Bytes bound it: K / 2 of codes and 2 or 3 per group for each weight row.  The codes are the 16-row operand A of
 // m16n8k16 (weight rows x K) and up to 16 rows of x its 8 columns, once or twice; m16n8k16 from registers because a
-// code leaves its word as an operand in about one instruction, while tcgen05 operands would have to be written to
+// code leaves its word as an operand in less than one instruction, while tcgen05 operands would have to be written to
 // shared memory first, four times the bytes that were read.
+//   Operands: a nibble in the low bits of an fp16 is the subnormal code * 2^-24, exactly, and one place higher
+//   code * 2^-20: a word of 8 codes becomes four operands, the pairs (0,4) (1,5) (2,6) (3,7), by one shift and four
+//   masks, and every second value of x is divided by 16 instead.  x is scaled by a power of two per row and step to a
+//   maximum in [2^14, 2^15), so that it fits fp16 whatever its type; fp32 becomes two fp16 terms (22 bits).
+//   The zero points' sum is kept apart, one row per lane.
 //
-// A block owns kRowsW rows and one slice of K; the blocks of a cluster have the same rows and the other slices, and
-// add their sums up through each other's shared memory in a fixed order.  Each warp streams its 32 rows through a
-// ring of its own (kStages steps of 256 columns, 16-byte asynchronous copies), so nothing but x is shared:
-// x lies in shared memory in the order of operand B, put there once per kilobyte or so of every row.
-//
-// How a lane's word of 8 codes becomes operands: pairs (0,4) (1,5) (2,6) (3,7) by shift and mask, with
-//   fp16: the code in the low bits of an fp16 is the subnormal code * 2^-24, exactly; 2^24 goes into the scale;
-//   bf16: under the exponent of 128 it is 128 + code; the 128 is taken off with the zero point, as (128 + z) sum x;
-//   fp32: 128 + code less 128 + z, exactly, and x as three bf16 terms, which hold all its 24 bits.
+// A block owns kRowsW rows and one slice of K in steps of kStep columns; the blocks of a cluster have the same rows and
+// the other slices, and add their sums up through each other's shared memory in a fixed order.  Each warp streams its
+// 32 rows through a ring of its own (16-byte asynchronous copies).  x is shared: while a step is computed the next
+// one's x is written to the other of two buffers, in the order of operand B, from registers that it was read into a step
+// before.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -36,34 +37,28 @@ struct W4Args {
   void* y;
   long long ldy;
   int m, n, k;
-  int steps;        // of the whole K
-  int slice;        // steps of a block
-  int phase;        // steps whose x is in shared memory at a time
-  int x_vec;        // x rows may be read 16 bytes at a time
+  int steps;  // of the whole K
+  int slice;  // steps of a block
+  int x_vec;  // x rows may be read 16 bytes at a time
 };
 
 constexpr int kWarps = 4;
 constexpr int kRowsW = 32 * kWarps;  // weight rows of a block
 constexpr int kStep = 256;           // columns of a step: 128 bytes of codes per row
-constexpr int kStages = 4;
-constexpr int kRing = kWarps * kStages * 32 * (kStep / 2);
-constexpr int kXBytes = 36 * 1024;   // for x: with the ring, two blocks an SM
+constexpr int kStages = 3;
+constexpr int kStage = 32 * (kStep / 2);
+constexpr int kRing = kWarps * kStages * kStage;
 constexpr int kMaxSplit = 8;
 
-template <typename T>
-struct Terms {
-  static constexpr int n = 1;
-};
-template <>
-struct Terms<float> {
-  static constexpr int n = 3;
-};
-
-// Shared memory: the rings, the sums [8 NT][kRowsW], x, and x's sums per group.
-template <int G, int NT>
+// Shared memory: the rings (over them at the end the sums [8 NT][kRowsW]), then two buffers of x.
+template <typename T, int G, int NT>
 struct Layout {
-  static constexpr int kSums = kRing, kX = kSums + 8 * NT * kRowsW * 4, kXSum = kX + kXBytes;
-  static constexpr int kBytes = kXSum + kXBytes / (2 * G) * 2 * 4 + 64;
+  static constexpr int kTerms = std::is_same<T, float>::value ? 2 : 1;
+  static constexpr int kX = kStep * 2 * kTerms * 8 * NT;    // [block of 32][term][row][t] 16 bytes
+  static constexpr int kXSum = (kStep / G) * 8 * NT * 4;    // [group][row] sums of x
+  static constexpr int kXPower = 8 * NT * 4;                // [row] what a sum of products is multiplied by
+  static constexpr int kBuffer = kX + kXSum + kXPower;
+  static constexpr int kBytes = kRing + 2 * kBuffer;
 };
 
 // Where 16-byte piece `piece` of row `row` of a step lies: lanes (g, t) that read pieces of 4, 8 or 16 bytes at
@@ -84,131 +79,161 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Puts columns [k0, k0 + columns) of up to 8 NT rows of x into shared memory as operand B, and the rows' sums over
-// each group beside it (fp32 calls do without).
-template <typename T, int G>
-__device__ __forceinline__ void stage_x(const W4Args& a, uint4* xs, float* xsum, int m0, int rows, int k0, int columns) {
-  constexpr int kTerms = Terms<T>::n, kWords = G / 32;
-  const int chunks = columns / 8;
-  for (int i = threadIdx.x; i < chunks * rows; i += kWarps * 32) {
-    const int m = i / chunks, q = i % chunks, k = k0 + 8 * q;
-    const T* from = static_cast<const T*>(a.x) + (m0 + m) * a.ldx + k;
-    float v[8];
-    if (a.x_vec && k + 8 <= a.k) {
-      T raw[8];
+// A step's x on its way: warp w has rows w, w + 4, ..., lane l columns 8 l to 8 l + 7 of the step.
+template <typename T, int NT>
+struct XRows {
+  alignas(16) T v[2 * NT][8];
+
+  __device__ __forceinline__ void load(const W4Args& a, int m0, int rows, int k0) {
+    const int warp = threadIdx.x / 32, k = k0 + threadIdx.x % 32 * 8;
 #pragma unroll
-      for (int b = 0; b < static_cast<int>(sizeof(raw)) / 16; ++b)
-        reinterpret_cast<uint4*>(raw)[b] = __ldg(reinterpret_cast<const uint4*>(from) + b);
+    for (int i = 0; i < 2 * NT; ++i) {
+      const int m = i * kWarps + warp;
+      if (m < rows) {
+        const T* from = static_cast<const T*>(a.x) + (m0 + m) * a.ldx + k;
+        if (a.x_vec && k + 8 <= a.k) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = to_f32(raw[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = k + j < a.k ? to_f32(from[j]) : 0.0f;
-    }
-    // thread t of a quad owns G / 4 columns of a group, kWords words of 8
-    const int group = q / (G / 8), t = q % (G / 8) / kWords, word = q % kWords;
-    const int block = group * kWords + word;
-    if constexpr (kTerms == 1) {
-      float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-#pragma unroll
-      for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
-      if (q % (G / 8) == 0) xsum[group * ((rows + 1) & ~1) + m] = sum;
-    }
-#pragma unroll
-    for (int term = 0; term < kTerms; ++term) {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value) {
-          w[j] = pack_f16(v[j], v[j + 4]);
+          for (int b = 0; b < static_cast<int>(sizeof(T)) / 2; ++b)
+            reinterpret_cast<uint4*>(v[i])[b] = __ldg(reinterpret_cast<const uint4*>(from) + b);
         } else {
-          w[j] = pack_bf16(v[j], v[j + 4]);
-          v[j] -= __uint_as_float(w[j] << 16);
-          v[j + 4] -= __uint_as_float(w[j] & 0xFFFF0000u);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i][j] = k + j < a.k ? from[j] : from_f32<T>(0.0f);
         }
       }
-      xs[((block * kTerms + term) * rows + m) * 4 + t] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-}
+
+  template <int G>
+  __device__ __forceinline__ void store(uint8_t* buffer, int rows) const {
+    using L = Layout<T, G, NT>;
+    constexpr int kWords = G / 32;
+    uint4* const xs = reinterpret_cast<uint4*>(buffer);
+    float* const xsum = reinterpret_cast<float*>(buffer + L::kX);
+    float* const xpower = reinterpret_cast<float*>(buffer + L::kX + L::kXSum);
+    const int warp = threadIdx.x / 32, q = threadIdx.x % 32;
+    // thread t of a quad owns G / 4 columns of a group, kWords words of 8
+    const int group = q / (G / 8), t = q % (G / 8) / kWords, block = group * kWords + q % kWords;
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      const int m = i * kWarps + warp;
+      if (m < rows) {
+        float f[8], top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          f[j] = to_f32(v[i][j]);
+          top = fmaxf(top, fabsf(f[j]));
+        }
+        float sum = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+#pragma unroll
+        for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
+        if (q % (G / 8) == 0) xsum[group * (8 * NT) + m] = sum;
+        const Power p = power_for(warp_max(top));
+        if (q == 0) xpower[m] = p.down;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= p.up;
+#pragma unroll
+        for (int term = 0; term < L::kTerms; ++term) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w[j] = pack_f16(f[j], f[j + 4]);
+            if (term + 1 < L::kTerms || j % 2) {
+              const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+              f[j] -= back.x;
+              f[j + 4] -= back.y;
+              if (j % 2) w[j] = pack_f16(back.x * 0.0625f, back.y * 0.0625f);
+            }
+          }
+          xs[((block * L::kTerms + term) * (8 * NT) + m) * 4 + t] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+  }
+};
 
 template <typename T, int G, int NT>
-__global__ void __launch_bounds__(kWarps * 32) linear_w4_kernel(W4Args a) {
-  constexpr bool kHalf = std::is_same<T, __half>::value, kF32 = std::is_same<T, float>::value;
-  constexpr int kTerms = Terms<T>::n, kWords = G / 32, kGroups = kStep / G;
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) linear_w4_kernel(W4Args a) {
+  using L = Layout<T, G, NT>;
+  constexpr int kTerms = L::kTerms, kWords = G / 32, kGroups = kStep / G;
   extern __shared__ __align__(128) uint8_t smem[];
-  float* const sums = reinterpret_cast<float*>(smem + Layout<G, NT>::kSums);
-  uint4* const xs = reinterpret_cast<uint4*>(smem + Layout<G, NT>::kX);
-  float* const xsum = reinterpret_cast<float*>(smem + Layout<G, NT>::kXSum);  // [group][rows, made even]
+  float* const sums = reinterpret_cast<float*>(smem);  // [8 NT][kRowsW]
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const int splits = max(1, (a.steps + a.slice - 1) / a.slice);  // the cluster
   const int rank = blockIdx.x % splits, n0 = blockIdx.x / splits * kRowsW;
   const int m0 = blockIdx.y * 8 * NT, rows = min(8 * NT, a.m - m0);
   const int step0 = rank * a.slice, steps = min(a.slice, a.steps - step0);
 
-  // copies: lane l brings piece l % 8 of rows l / 8, 4 rows on each time; rows past the last repeat it
+  // copies: lane l brings piece l % 8 of rows l / 8, l / 8 + 4, ...
   const long long pitch = static_cast<long long>((a.k + 31) / 32) * 16;
-  const uint32_t ring = shared_address(smem) + warp * (kStages * 32 * (kStep / 2));
-  const int piece = lane % 8;
-  const int row0 = n0 + warp * 32;
-  auto load_step = [&](int s) {
-    const long long at = static_cast<long long>(step0 + s) * (kStep / 2) + piece * 16;
-    const uint32_t to = ring + (s % kStages) * (32 * (kStep / 2));
-    if (at < pitch) {
+  const int row0 = n0 + warp * 32, here = min(32, a.n - row0) - lane / 8;  // rows past the last are left out
+  const uint32_t ring = shared_address(smem) + warp * (kStages * kStage);
+  const long long piece0 = static_cast<long long>(step0) * (kStep / 2) + lane % 8 * 16;
+  const uint8_t* const codes = a.codes + (row0 + lane / 8) * pitch + piece0;
+  auto load_step = [&](int s, int slot) {
+    const int at = s * (kStep / 2);
+    if (piece0 + at < pitch) {
+      const uint8_t* from = codes + at;
+      const uint32_t to = ring + slot * kStage;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int r = j * 4 + lane / 8;
-        copy_async<16>(to + piece_at(r, piece), a.codes + min(row0 + r, a.n - 1) * pitch + at);
+        if (j * 4 < here) copy_async<16>(to + piece_at(j * 4 + lane / 8, lane % 8), from);
+        from += 4 * pitch;
       }
     }
   };
-  // scales and zero points: lane l holds those of row l, two steps ahead of their use
+  // scales and zero points: lane l holds those of row l, read a step before their use
   const int my_row = min(row0 + lane, a.n - 1), groups = (a.k + G - 1) / G;
-  uint32_t scale[3][kGroups], zero[3][kGroups];
-  auto load_params = [&](int s, uint32_t (&sc)[kGroups], uint32_t (&zp)[kGroups]) {
+  uint32_t scale[kGroups], zero[kGroups], next_scale[kGroups], next_zero[kGroups];
+  auto load_params = [&](int s) {
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       const long long at = static_cast<long long>(min((step0 + s) * kGroups + i, groups - 1)) * a.n + my_row;
-      sc[i] = __ldg(a.scales + at);
-      zp[i] = a.zeros ? __ldg(a.zeros + at) : 8u;
+      next_scale[i] = __ldg(a.scales + at);
+      next_zero[i] = a.zeros ? __ldg(a.zeros + at) : 8u;
     }
   };
+
+  float acc[2][NT][4], less[8 * NT];  // sums of products; lane l's row: sums of zero points
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[0][n][e] = acc[1][n][e] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) less[n * 8 + e] = 0.0f;
+  }
+  XRows<T, NT> x;
+  if (steps > 0) {
+    x.load(a, m0, rows, step0 * kStep);
+    load_params(0);
+  }
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
-    if (s < steps) load_step(s);
+    if (s < steps) load_step(s, s);
     copy_commit();
   }
-  if (steps > 0) {
-    load_params(0, scale[0], zero[0]);
-    load_params(1, scale[1], zero[1]);
-  }
+  if (steps > 0) x.template store<G>(smem + kRing, rows);
+  if (steps > 1) x.load(a, m0, rows, (step0 + 1) * kStep);
+  __syncthreads();
 
-  float acc[2][NT][4];
-#pragma unroll
-  for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-    for (int n = 0; n < NT; ++n) acc[mt][n][0] = acc[mt][n][1] = acc[mt][n][2] = acc[mt][n][3] = 0.0f;
-
+  int slot = 0, fill = kStages - 1;
   for (int s = 0; s < steps; ++s) {
-    if (s % a.phase == 0) {
-      if (s) __syncthreads();
-      stage_x<T, G>(a, xs, xsum, m0, rows, (step0 + s) * kStep, min(a.phase, steps - s) * kStep);
-      __syncthreads();
-    }
+    const uint8_t* const buffer = smem + kRing + (s & 1) * L::kBuffer;
+    if (s + 1 < steps) x.template store<G>(smem + kRing + (~s & 1) * L::kBuffer, rows);
+    if (s + 2 < steps) x.load(a, m0, rows, (step0 + s + 2) * kStep);
     copy_wait<kStages - 2>();
     __syncwarp();
-    if (s + kStages - 1 < steps) load_step(s + kStages - 1);
+    if (s + kStages - 1 < steps) load_step(s + kStages - 1, fill);
     copy_commit();
-    load_params(s + 2, scale[2], zero[2]);
-    const uint8_t* stage = smem + warp * (kStages * 32 * (kStep / 2)) + (s % kStages) * (32 * (kStep / 2));
-    const int block0 = s % a.phase * (kStep / 32);
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) scale[i] = next_scale[i] << 16, zero[i] = next_zero[i];
+    if (s + 1 < steps) load_params(s + 1);
+    const uint4* const xs = reinterpret_cast<const uint4*>(buffer);
+    const float* const xsum = reinterpret_cast<const float*>(buffer + L::kX);
+    const float* const xpower = reinterpret_cast<const float*>(buffer + L::kX + L::kXSum);
+    const uint8_t* const stage = smem + warp * (kStages * kStage) + slot * kStage;
+    float sum[2][NT][4];
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-      float part[2][NT][4];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) part[mt][n][0] = part[mt][n][1] = part[mt][n][2] = part[mt][n][3] = 0.0f;
       uint32_t w[4][kWords];  // rows g, g + 8, g + 16, g + 24
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -224,14 +249,7 @@ __global__ void __launch_bounds__(kWarps * 32) linear_w4_kernel(W4Args a) {
           w[r][0] = v.x, w[r][1] = v.y, w[r][2] = v.z, w[r][3] = v.w;
         }
       }
-      uint32_t par[4];  // scale bits, zero point << 16
-#pragma unroll
-      for (int r = 0; r < 4; ++r) par[r] = __shfl_sync(~0u, scale[0][i] | zero[0][i] << 16, r * 8 + g);
-      uint32_t zpair[4];
-      if constexpr (kF32) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) zpair[r] = (par[r] >> 16) * 0x00010001u + 0x43004300u;
-      }
+      float part[2][NT][4];
 #pragma unroll
       for (int word = 0; word < kWords; ++word) {
         uint4 b[kTerms][NT];
@@ -239,60 +257,59 @@ __global__ void __launch_bounds__(kWarps * 32) linear_w4_kernel(W4Args a) {
         for (int term = 0; term < kTerms; ++term)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
-            b[term][n] = n * 8 + g < rows ? xs[(((block0 + i * kWords + word) * kTerms + term) * rows + n * 8 + g) * 4 + t]
+            b[term][n] = n * 8 + g < rows ? xs[(((i * kWords + word) * kTerms + term) * (8 * NT) + n * 8 + g) * 4 + t]
                                           : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
-          uint32_t c[2][4];
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t v = w[2 * mt + u][word] >> (4 * j);
-              if constexpr (kHalf) {
-                c[u][j] = v & 0x000F000Fu;
-              } else {
-                c[u][j] = and_or(v, 0x000F000Fu, 0x43004300u);
-                if constexpr (kF32) c[u][j] = sub_bf16x2(c[u][j], zpair[2 * mt + u]);
-              }
-            }
+          const uint32_t w0 = w[2 * mt][word], w1 = w[2 * mt + 1][word], v0 = w0 >> 8, v1 = w1 >> 8;
 #pragma unroll
           for (int term = 0; term < kTerms; ++term)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              if constexpr (kHalf) {
-                mma_f16(part[mt][n], c[0][0], c[1][0], c[0][1], c[1][1], b[term][n].x, b[term][n].y);
-                mma_f16(part[mt][n], c[0][2], c[1][2], c[0][3], c[1][3], b[term][n].z, b[term][n].w);
-              } else {
-                mma_bf16(part[mt][n], c[0][0], c[1][0], c[0][1], c[1][1], b[term][n].x, b[term][n].y);
-                mma_bf16(part[mt][n], c[0][2], c[1][2], c[0][3], c[1][3], b[term][n].z, b[term][n].w);
-              }
+              if (word == 0 && term == 0)
+                mma_f16_first(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
+                              b[term][n].x, b[term][n].y);
+              else
+                mma_f16(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
+                        b[term][n].x, b[term][n].y);
+              mma_f16(part[mt][n], v0 & 0x000F000Fu, v1 & 0x000F000Fu, v0 & 0x00F000F0u, v1 & 0x00F000F0u, b[term][n].z,
+                      b[term][n].w);
             }
         }
       }
-      // the group's scale, and its zero point times the sum of x (columns 2t, 2t + 1)
-      const int group = block0 / kWords + i;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float2 sx = make_float2(0.0f, 0.0f);
-        if constexpr (!kF32) sx = *reinterpret_cast<const float2*>(xsum + group * ((rows + 1) & ~1) + n * 8 + 2 * t);
-        if constexpr (kHalf) sx.x *= 1.0f / 16777216.0f, sx.y *= 1.0f / 16777216.0f;
+      for (int r = 0; r < 4; ++r) {
+        const float sc = __uint_as_float(__shfl_sync(~0u, scale[i], r * 8 + g));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float sc = __uint_as_float(par[r] << 16);
-          const float zr = static_cast<float>(par[r] >> 16) + (kHalf ? 0.0f : 128.0f);
-          float* p = part[r / 2][n] + r % 2 * 2;
-          float* to = acc[r / 2][n] + r % 2 * 2;
-          to[0] = fmaf(sc, kF32 ? p[0] : fmaf(-zr, sx.x, p[0]), to[0]);
-          to[1] = fmaf(sc, kF32 ? p[1] : fmaf(-zr, sx.y, p[1]), to[1]);
-        }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& to = sum[r / 2][n][r % 2 * 2 + e];
+            to = i == 0 ? sc * part[r / 2][n][r % 2 * 2 + e] : fmaf(sc, part[r / 2][n][r % 2 * 2 + e], to);
+          }
       }
+      const float sz = __uint_as_float(scale[i]) * static_cast<float>(zero[i]);
+#pragma unroll
+      for (int m = 0; m < 8 * NT; m += 4)
+        if (m < rows) {
+          const float4 v = *reinterpret_cast<const float4*>(xsum + i * (8 * NT) + m);
+          less[m] = fmaf(sz, v.x, less[m]);
+          less[m + 1] = fmaf(sz, v.y, less[m + 1]);
+          less[m + 2] = fmaf(sz, v.z, less[m + 2]);
+          less[m + 3] = fmaf(sz, v.w, less[m + 3]);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
-      scale[0][i] = scale[1][i], scale[1][i] = scale[2][i];
-      zero[0][i] = zero[1][i], zero[1][i] = zero[2][i];
+    for (int n = 0; n < NT; ++n) {
+      const float2 p = *reinterpret_cast<const float2*>(xpower + n * 8 + 2 * t);
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[mt][n][e] = fmaf(e % 2 ? p.y : p.x, sum[mt][n][e], acc[mt][n][e]);
     }
+    slot = slot + 1 == kStages ? 0 : slot + 1;
+    fill = fill + 1 == kStages ? 0 : fill + 1;
+    __syncthreads();  // this step's x has been read, the next one's is there
   }
   copy_wait<0>();
 
@@ -302,8 +319,10 @@ __global__ void __launch_bounds__(kWarps * 32) linear_w4_kernel(W4Args a) {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        sums[(n * 8 + 2 * t + e % 2) * kRowsW + warp * 32 + mt * 16 + e / 2 * 8 + g] =
-            kHalf ? acc[mt][n][e] * 16777216.0f : acc[mt][n][e];
+        sums[(n * 8 + 2 * t + e % 2) * kRowsW + warp * 32 + mt * 16 + e / 2 * 8 + g] = acc[mt][n][e] * 16777216.0f;
+  __syncwarp();
+#pragma unroll
+  for (int m = 0; m < 8 * NT; ++m) sums[m * kRowsW + warp * 32 + lane] -= less[m];
   if (splits > 1)
     cluster_sync();
   else
@@ -328,7 +347,7 @@ __global__ void __launch_bounds__(kWarps * 32) linear_w4_kernel(W4Args a) {
 
 template <typename T, int G, int NT>
 int launch_linear(W4Args a, int sms, cudaStream_t stream) {
-  constexpr int kSmem = Layout<G, NT>::kBytes;
+  constexpr int kSmem = Layout<T, G, NT>::kBytes;
   auto kernel = linear_w4_kernel<T, G, NT>;
   static std::atomic<bool> ready{false};
   if (!ready.load(std::memory_order_relaxed)) {
@@ -342,8 +361,6 @@ int launch_linear(W4Args a, int sms, cudaStream_t stream) {
   const int want = std::max(1, std::min(kMaxSplit, static_cast<int>(2ll * sms / (static_cast<long long>(tiles) * passes))));
   a.slice = std::max(1, (a.steps + want - 1) / want);
   const int splits = std::max(1, (a.steps + a.slice - 1) / a.slice);
-  const int rows = std::min(a.m, 8 * NT);
-  a.phase = std::max(1, std::min(a.slice, kXBytes / (rows * kStep * 2 * Terms<T>::n)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(tiles * splits, passes);
   cfg.blockDim = dim3(kWarps * 32);
