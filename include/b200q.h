@@ -196,32 +196,45 @@ enum b200q_ftype { B200Q_F32 = 0, B200Q_F16 = 1, B200Q_BF16 = 2 };
 /* y[m][n] = sum_k x[m][k] * (code[n][k] - zero[k / group][n]) * scale[k / group][n] (+ bias[n]).
  * codes: [n][16 * ceil(k / 32)] bytes, 16-byte aligned (the nibbles past k are not used);
  * scales: bf16 [ceil(k / group)][n]; zeros: uint8 in 0..15, same shape, or NULL for 8 everywhere;
- * group 32, 64 or 128.  x [m][k] with row stride ldx, y [m][n] with row stride ldy.
+ * group 32, 64 or 128.  x [m][k] with row stride ldx, y [m][n] with row stride ldy; bias [n] or NULL.
  * Made for the few rows of a decode step: weights are read once per 16 rows of x.  Finite x. */
-int b200q_linear_w4(const void* x, long long ldx, const uint8_t* codes, const void* scales, const uint8_t* zeros,
-                    const void* bias, void* y, long long ldy, int ftype, int m, int n, int k, int group,
-                    void* stream);
+typedef struct b200q_linear_w4_args {
+  const void* x;
+  int64_t ldx;
+  const uint8_t* codes;
+  const void* scales;
+  const uint8_t* zeros;
+  const void* bias;
+  void* y;
+  int64_t ldy;
+  int ftype, m, n, k, group;
+} b200q_linear_w4_args;
+int b200q_linear_w4(const b200q_linear_w4_args* args, void* stream);
 
 /* Per-head RMS norm of queries and keys, then the position rotation of each head's first `rot`
  * channels, in one pass:  y = R(pos[t]) (x * rsqrt(mean(x^2) + eps) * w).
  * q [t][hq][d], k [t][hk][d] with token / head strides; q_w, k_w [d] or NULL (all ones).
  * table: fp32 [positions][rot], cos of the rot / 2 angles, then sin; rot even, <= d, 0 for none.
- * Pairs are (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved.  q_out / k_out may be q / k. */
-int b200q_qk_norm_rope(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts, long long k_hs,
-                       const void* q_w, const void* k_w, const float* table, int positions, const int32_t* pos,
-                       void* q_out, long long qo_ts, long long qo_hs, void* k_out, long long ko_ts,
-                       long long ko_hs, int ftype, int t, int hq, int hk, int d, int rot, int interleaved, float eps,
-                       void* stream);
+ * Pairs are (i, i + rot / 2), or (2 i, 2 i + 1) when interleaved.  q_out / k_out (with strides) may be
+ * q / k.  The gradient's fields are not read. */
+typedef struct b200q_qk_norm_args {
+  const void *q, *k, *q_w, *k_w;
+  const float* table;
+  const int32_t* pos;
+  void *q_out, *k_out;
+  const void *q_grad, *k_grad;
+  void *q_w_grad, *k_w_grad;
+  int64_t q_ts, q_hs, k_ts, k_hs, qo_ts, qo_hs, ko_ts, ko_hs;
+  int positions, ftype, t, hq, hk, d, rot, interleaved;
+  float eps;
+} b200q_qk_norm_args;
+int b200q_qk_norm_rope(const b200q_qk_norm_args* args, void* stream);
 
-/* Gradient of b200q_qk_norm_rope: dq_out / dk_out are the gradients of its outputs, contiguous
- * [t][h][d]; dq / dk (contiguous) those of its inputs; dq_w / dk_w [d] those of the weights, summed
- * over tokens and heads in a fixed order (NULL: not wanted).  Recomputes the norms from
- * q and k.  Uses the stream's workspace. */
-int b200q_qk_norm_rope_bprop(const void* dq_out, const void* dk_out, const void* q, long long q_ts, long long q_hs,
-                             const void* k, long long k_ts, long long k_hs, const void* q_w, const void* k_w,
-                             const float* table, int positions, const int32_t* pos, void* dq, void* dk, void* dq_w,
-                             void* dk_w, int ftype, int t, int hq, int hk, int d, int rot, int interleaved, float eps,
-                             void* stream);
+/* Gradient of b200q_qk_norm_rope: q_grad / k_grad are the gradients of its outputs, contiguous
+ * [t][h][d]; q_out / k_out (contiguous, their strides not read) receive those of its inputs, q_w_grad /
+ * k_w_grad [d] (NULL: not wanted) those of the weights, summed over tokens and heads in a fixed order.
+ * Recomputes the norms from q and k.  Uses the stream's workspace. */
+int b200q_qk_norm_rope_bprop(const b200q_qk_norm_args* args, void* stream);
 
 /* 4-bit paged key / value cache.  codes: [pages][heads][page_size][d / 2] bytes, 16-byte aligned;
  * params: [pages][heads][page_size][d / group] words (bits 0-15 the bf16 scale, 16-23 the zero point);
@@ -249,10 +262,19 @@ int b200q_kv4_read(const b200q_kv4_cache* c, const int64_t* slots, void* k, void
  * block_table[b][0 .. max_pages), row stride bt_stride; none seen: output 0, lse -inf.
  * q [b][tq][hq][d] with strides; query head h reads cache head h / (hq / heads).
  * out contiguous [b][tq][hq][d]; lse fp32 [b][tq][hq] or NULL: log of the sum of exp(scale * q.k).
- * Uses the stream's workspace when a sequence is split over blocks. */
-int b200q_kv4_attention(const b200q_kv4_cache* c, const void* q, long long q_bs, long long q_ts, long long q_hs,
-                        const int32_t* block_table, long long bt_stride, const int32_t* lens, void* out, float* lse,
-                        int ftype, int b, int tq, int hq, int max_pages, float scale, void* stream);
+ * Uses the stream's workspace: sequences are split over blocks. */
+typedef struct b200q_kv4_attention_args {
+  const void* q;
+  int64_t q_bs, q_ts, q_hs;
+  const int32_t* block_table;
+  int64_t bt_stride;
+  const int32_t* lens;
+  void* out;
+  float* lse;
+  int ftype, b, tq, hq, max_pages;
+  float scale;
+} b200q_kv4_attention_args;
+int b200q_kv4_attention(const b200q_kv4_cache* c, const b200q_kv4_attention_args* args, void* stream);
 
 /* Packed low-channel int8 conv that allocates nothing (no counterpart in the reference).
  * For callers that may not allocate device memory at all: for example plugins inside a runtime

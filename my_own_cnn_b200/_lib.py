@@ -7,6 +7,7 @@ use anything but the CUDA kernels.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import POINTER, Structure, c_int, c_int8, c_int32, c_int64, c_longlong, c_size_t, c_uint8
 from ctypes import c_uint64, c_void_p, c_float, c_char_p
 from pathlib import Path
@@ -62,6 +63,34 @@ class CKV4Cache(Structure):
                 ("pages", c_int), ("heads", c_int), ("page_size", c_int), ("d", c_int), ("group", c_int)]
 
 
+class CLinearW4Args(Structure):
+    _fields_ = [("x", c_void_p), ("ldx", c_int64), ("codes", c_void_p), ("scales", c_void_p), ("zeros", c_void_p),
+                ("bias", c_void_p), ("y", c_void_p), ("ldy", c_int64), ("ftype", c_int), ("m", c_int), ("n", c_int),
+                ("k", c_int), ("group", c_int)]
+
+
+class CQKNormArgs(Structure):
+    _fields_ = [(f, c_void_p) for f in ("q", "k", "q_w", "k_w", "table", "pos", "q_out", "k_out", "q_grad", "k_grad",
+                                        "q_w_grad", "k_w_grad")]
+    _fields_ += [(f, c_int64) for f in ("q_ts", "q_hs", "k_ts", "k_hs", "qo_ts", "qo_hs", "ko_ts", "ko_hs")]
+    _fields_ += [(f, c_int) for f in ("positions", "ftype", "t", "hq", "hk", "d", "rot", "interleaved")]
+    _fields_ += [("eps", c_float)]
+
+
+class CKV4AttentionArgs(Structure):
+    _fields_ = [("q", c_void_p), ("q_bs", c_int64), ("q_ts", c_int64), ("q_hs", c_int64), ("block_table", c_void_p),
+                ("bt_stride", c_int64), ("lens", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("ftype", c_int),
+                ("b", c_int), ("tq", c_int), ("hq", c_int), ("max_pages", c_int), ("scale", c_float)]
+
+
+def packer(layout) -> "struct.Struct":
+    """The bytes of a ctypes structure's fields in order: an argument block is packed and handed over in a fraction
+    of the time that filling the structure takes."""
+    code = {c_void_p: "P", c_int64: "q", c_int: "i", c_float: "f"}
+    fmt = "".join(code[t] for _, t in layout._fields_)
+    return struct.Struct(fmt + "x" * (ctypes.sizeof(layout) - struct.calcsize(fmt)))
+
+
 class B200QError(RuntimeError):
     """Raised for a non-zero status; ``code`` is the b200q_status value."""
 
@@ -81,8 +110,8 @@ def lib() -> ctypes.CDLL:
         raise RuntimeError(f"{LIB_PATH} is not built; run __graft_entry__.build() "
                            "(the CUDA library is required, there is no CPU path)")
     L = ctypes.CDLL(str(LIB_PATH))
-    vp, i, ll, f = c_void_p, c_int, c_longlong, c_float
-    pconv, pepi, pkv4 = POINTER(CConvParams), POINTER(CEpilogue), POINTER(CKV4Cache)
+    vp, i, ll = c_void_p, c_int, c_longlong
+    pconv, pepi, packed = POINTER(CConvParams), POINTER(CEpilogue), c_char_p
     sig = {
         "b200q_fprop_nhwc_qi32": [i, vp, vp, vp, i, i, i, i, i, i, i, pconv, vp, vp, vp],
         "b200q_block_fprop_nhwc_qi32": [i, vp, vp, vp, i, i, i, i, i, i, i, pconv, i, i, vp, vp, vp],
@@ -105,14 +134,12 @@ def lib() -> ctypes.CDLL:
         "b200q_conv_bprop_f32": [vp, vp, vp, i, i, i, i, i, i, i, pconv, i, i, vp],
         "b200q_conv_grad_f32": [vp, vp, vp, vp, i, i, i, i, i, i, i, i, pconv, i, i, vp],
         "b200q_bmm_f32": [vp, vp, vp, i, i, i, i, i, i, vp],
-        "b200q_linear_w4": [vp, ll, vp, vp, vp, vp, vp, ll, i, i, i, i, i, vp],
-        "b200q_qk_norm_rope": [vp, ll, ll, vp, ll, ll, vp, vp, vp, i, vp, vp, ll, ll, vp, ll, ll, i, i, i, i, i, i, i, f,
-                               vp],
-        "b200q_qk_norm_rope_bprop": [vp, vp, vp, ll, ll, vp, ll, ll, vp, vp, vp, i, vp, vp, vp, vp, vp, i, i, i, i, i, i,
-                                     i, f, vp],
-        "b200q_kv4_append": [pkv4, vp, ll, ll, vp, ll, ll, vp, i, i, vp],
-        "b200q_kv4_read": [pkv4, vp, vp, vp, i, i, vp],
-        "b200q_kv4_attention": [pkv4, vp, ll, ll, ll, vp, ll, vp, vp, vp, i, i, i, i, i, f, vp],
+        "b200q_linear_w4": [packed, vp],
+        "b200q_qk_norm_rope": [packed, vp],
+        "b200q_qk_norm_rope_bprop": [packed, vp],
+        "b200q_kv4_append": [packed, vp, ll, ll, vp, ll, ll, vp, i, i, vp],
+        "b200q_kv4_read": [packed, vp, vp, vp, i, i, vp],
+        "b200q_kv4_attention": [packed, packed, vp],
     }
     for name, args in sig.items():
         fn = getattr(L, name)

@@ -269,20 +269,21 @@ extern "C" int b200q_kv4_read(const b200q_kv4_cache* cache, const int64_t* slots
   return rc;
 }
 
-extern "C" int b200q_kv4_attention(const b200q_kv4_cache* cache, const void* q, long long q_bs, long long q_ts,
-                                   long long q_hs, const int32_t* block_table, long long bt_stride,
-                                   const int32_t* lens, void* out, float* lse, int ftype, int b, int tq, int hq,
-                                   int max_pages, float scale, void* stream) {
+extern "C" int b200q_kv4_attention(const b200q_kv4_cache* cache, const b200q_kv4_attention_args* p, void* stream) {
   Cache c;
   int rc = check_cache(cache, &c);
-  if (rc || (rc = check_ftype(ftype))) return rc;
+  if (rc) return rc;
+  if (!p) return host_fail(B200Q_ERR_INVALID_ARG, "null argument");
+  const int ftype = p->ftype, b = p->b, tq = p->tq, hq = p->hq, max_pages = p->max_pages;
+  if ((rc = check_ftype(ftype))) return rc;
   if (b < 0 || tq < 0 || hq < 0 || max_pages < 0) return host_fail(B200Q_ERR_INVALID_ARG, "negative attention dimension");
   if (hq % c.heads) return host_fail(B200Q_ERR_INVALID_ARG, "%d query heads do not divide over %d cache heads", hq, c.heads);
   if (b == 0 || tq == 0 || hq == 0) return B200Q_OK;
-  if (!q || !out || !lens || (max_pages > 0 && !block_table)) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
+  if (!p->q || !p->out || !p->lens || (max_pages > 0 && !p->block_table)) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
   if (static_cast<long long>(max_pages) * c.page_size > (1 << 30) || b > (1 << 20) || tq > (1 << 16) || hq > (1 << 16))
     return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
-  AttnArgs a{q, q_bs, q_ts, q_hs, block_table, bt_stride, lens, out, lse, ftype, b, tq, hq, max_pages, scale};
+  AttnArgs a{p->q,   p->q_bs, p->q_ts, p->q_hs, p->block_table, p->bt_stride, p->lens, p->out,
+             p->lse, ftype,   b,       tq,      hq,             max_pages,    p->scale};
   int sms = 0;
   if ((rc = host_device(&sms, &a.err))) return rc;
   a.page_shift = -1;

@@ -266,18 +266,19 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
   __syncthreads();
 
   // this lane's columns: rows 2t, 2t + 1 of each 8
-  float f[NT][2], qsum[NT][kGroups][2], m[NT][2], l[NT][2];
+  float2 f[NT], qsum[NT][kGroups], l[NT];
+  float m[NT][2];
   int limit[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = n * 8 + 2 * t + e;
-      f[n][e] = row_f[r];
+      (e ? f[n].y : f[n].x) = row_f[r];
 #pragma unroll
-      for (int k = 0; k < kGroups; ++k) qsum[n][k][e] = row_sum[k * kRows + r];
+      for (int k = 0; k < kGroups; ++k) (e ? qsum[n][k].y : qsum[n][k].x) = row_sum[k * kRows + r];
       m[n][e] = -INFINITY;
-      l[n][e] = 0.0f;
+      l[n] = both(0.0f);
       limit[n][e] = len - a.tq + (tile * kRows + min(r, rows - 1)) / ratio + 1;
     }
   const int all_see = len - a.tq + tile * kRows / ratio + 1;  // tokens that every row of the tile sees
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
     const bool whole = here == ~0u && base + kTile <= all_see;
 
     // scores
-    float s[2][NT][4];
+    float2 s[2][NT][2];  // [tokens g, g + 8], rows 2t and 2t + 1
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) {
       float part[2][NT][4];
@@ -347,14 +348,13 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const uint32_t p = kp[(mt * 16 + u * 8 + g) * kGroups + k];
-          const float ks = param_scale(p), kz = zero_point(p);
+          const float2 ks = both(param_scale(p)), kz = both(-zero_point(p));
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float v = fmaf(-kz, qsum[n][k][e], part[mt][n][2 * u + e]);
-              s[mt][n][2 * u + e] = k == 0 ? ks * v : fmaf(ks, v, s[mt][n][2 * u + e]);
-            }
+          for (int n = 0; n < NT; ++n) {
+            const float* at = part[mt][n] + 2 * u;
+            const float2 v = fma2(kz, qsum[n][k], make_float2(at[0], at[1]));
+            s[mt][n][u] = k == 0 ? mul2(ks, v) : fma2(ks, v, s[mt][n][u]);
+          }
         }
     }
 
@@ -376,24 +376,23 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
     bool raise = v_top > v_limit;
     float top[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        top[n][e] = -INFINITY;
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float& x = s[mt][n][2 * u + e];
-            x *= f[n][e];
-            if (!whole) {
-              const int tok = mt * 16 + u * 8 + g;
-              if (!(here >> tok & 1) || base + tok >= limit[n][e]) x = -INFINITY;
-            }
-            top[n][e] = fmaxf(top[n][e], x);
+        for (int u = 0; u < 2; ++u) {
+          float2& x = s[mt][n][u];
+          x = mul2(x, f[n]);
+          if (!whole) {
+            const int tok = mt * 16 + u * 8 + g;
+            if (!(here >> tok & 1) || base + tok >= limit[n][0]) x.x = -INFINITY;
+            if (!(here >> tok & 1) || base + tok >= limit[n][1]) x.y = -INFINITY;
           }
-        raise |= top[n][e] > m[n][e] + 8.0f;
-      }
+        }
+      top[n][0] = fmaxf(fmaxf(s[0][n][0].x, s[0][n][1].x), fmaxf(s[1][n][0].x, s[1][n][1].x));
+      top[n][1] = fmaxf(fmaxf(s[0][n][0].y, s[0][n][1].y), fmaxf(s[1][n][0].y, s[1][n][1].y));
+      raise |= top[n][0] > m[n][0] + 8.0f || top[n][1] > m[n][1] + 8.0f;
+    }
     if (__any_sync(~0u, raise)) {
       float v_keep = 1.0f;
 #pragma unroll
@@ -415,7 +414,7 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
           const float now = fmaxf(m[n][e], top[n][e]);
           float keep = now == -INFINITY ? 1.0f : exp2_approx(m[n][e] - now);
           m[n][e] = now;
-          l[n][e] *= keep;
+          (e ? l[n].y : l[n].x) *= keep;
           keep *= v_keep;
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) o[j][n][e] *= keep, o[j][n][2 + e] *= keep;
@@ -424,19 +423,18 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
         }
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+      const float2 ref = make_float2(m[n][0] == -INFINITY ? 0.0f : -m[n][0], m[n][1] == -INFINITY ? 0.0f : -m[n][1]);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float ref = m[n][e] == -INFINITY ? 0.0f : m[n][e];
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float& x = s[mt][n][2 * u + e];
-            x = exp2_approx(x - ref);
-            l[n][e] += x;
-          }
-      }
+        for (int u = 0; u < 2; ++u) {
+          float2& x = s[mt][n][u];
+          x = add2(x, ref);
+          x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+          l[n] = add2(l[n], x);
+        }
+    }
 
     // values
     constexpr int kPTerms = F32 ? 2 : 1;
@@ -448,17 +446,16 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
         uint32_t b[kPTerms][NT][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float scale = vs[mt][u][k] * v_factor;
+          const float2 scale = both(vs[mt][u][k] * v_factor);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float x0 = s[mt][n][2 * u] * scale, x1 = s[mt][n][2 * u + 1] * scale;
+            float2 x = mul2(s[mt][n][u], scale);
 #pragma unroll
             for (int term = 0; term < kPTerms; ++term) {
-              const uint32_t v = pack_f16(x0, x1);
+              const uint32_t v = pack_f16(x.x, x.y);
               if (term + 1 < kPTerms) {
                 const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&v));
-                x0 -= back.x;
-                x1 -= back.y;
+                x = make_float2(x.x - back.x, x.y - back.y);
               }
               b[term][n][u] = transpose_8x8(v);
             }
@@ -511,12 +508,13 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
+      float all = e ? l[n].y : l[n].x;
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) l[n][e] += __shfl_xor_sync(~0u, l[n][e], x);
+      for (int x = 4; x < 32; x <<= 1) all += __shfl_xor_sync(~0u, all, x);
       if (g == 0) {
         float* ml = row_ml + (warp * kRows + n * 8 + 2 * t + e) * 2;
         ml[0] = m[n][e];
-        ml[1] = l[n][e];
+        ml[1] = all;
       }
     }
   copy_wait<0>();

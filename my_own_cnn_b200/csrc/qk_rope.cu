@@ -424,19 +424,34 @@ int heads_per_group(const NormArgs& a, int lanes, int sms) {
   return lanes_of_all >= 16 * full ? 8 : lanes_of_all >= 4 * full ? 4 : 1;
 }
 
-int check_norm(const void* q, const void* k, const float* table, int positions, const int32_t* pos, int ftype, int t,
-               int hq, int hk, int d, int rot) {
+// Checks what both directions share and fills in the kernels' arguments.
+int norm_args(const b200q_qk_norm_args* p, NormArgs* a, int* sms) {
+  if (!p) return host_fail(B200Q_ERR_INVALID_ARG, "null argument");
+  const int ftype = p->ftype, t = p->t, hq = p->hq, hk = p->hk, d = p->d, rot = p->rot;
   if (ftype < B200Q_F32 || ftype > B200Q_BF16) return host_fail(B200Q_ERR_INVALID_ARG, "bad floating type %d", ftype);
   if (t < 0 || hq < 0 || hk < 0 || d <= 0) return host_fail(B200Q_ERR_INVALID_ARG, "bad head dimensions");
   if (rot < 0 || rot > d || rot % 2)
     return host_fail(B200Q_ERR_INVALID_ARG, "rotated channels must be even and at most %d, got %d", d, rot);
   if (d > 1024) return host_fail(B200Q_ERR_UNSUPPORTED, "heads of more than 1024 channels");
   if (hq + hk > (1 << 20)) return host_fail(B200Q_ERR_UNSUPPORTED, "too many heads");
-  if (t == 0) return B200Q_OK;
-  if ((hq && !q) || (hk && !k)) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
-  if (rot && (!table || !pos || positions <= 0))
-    return host_fail(B200Q_ERR_INVALID_ARG, "a rotation needs its table and positions");
-  return B200Q_OK;
+  if (t > 0) {
+    if ((hq && (!p->q || !p->q_out)) || (hk && (!p->k || !p->k_out)))
+      return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
+    if (rot && (!p->table || !p->pos || p->positions <= 0))
+      return host_fail(B200Q_ERR_INVALID_ARG, "a rotation needs its table and positions");
+  }
+  a->side[0] = {p->q, p->q_ts, p->q_hs, p->q_w, p->q_out, p->qo_ts, p->qo_hs, p->q_grad, hq};
+  a->side[1] = {p->k, p->k_ts, p->k_hs, p->k_w, p->k_out, p->ko_ts, p->ko_hs, p->k_grad, hk};
+  a->table = p->table;
+  a->pos = p->pos;
+  a->positions = p->positions;
+  a->t = t;
+  a->d = d;
+  a->rot = rot;
+  a->interleaved = p->interleaved;
+  a->eps = p->eps;
+  if (t == 0 || hq + hk == 0) return B200Q_OK;
+  return host_device(sms, &a->err);
 }
 
 }  // namespace
@@ -444,28 +459,13 @@ int check_norm(const void* q, const void* k, const float* table, int positions, 
 
 using namespace b200q;
 
-extern "C" int b200q_qk_norm_rope(const void* q, long long q_ts, long long q_hs, const void* k, long long k_ts,
-                                  long long k_hs, const void* q_w, const void* k_w, const float* table, int positions,
-                                  const int32_t* pos, void* q_out, long long qo_ts, long long qo_hs, void* k_out,
-                                  long long ko_ts, long long ko_hs, int ftype, int t, int hq, int hk, int d, int rot,
-                                  int interleaved, float eps, void* stream) {
-  int rc = check_norm(q, k, table, positions, pos, ftype, t, hq, hk, d, rot);
-  if (rc) return rc;
-  if (t == 0 || hq + hk == 0) return B200Q_OK;
-  if ((hq && !q_out) || (hk && !k_out)) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
+extern "C" int b200q_qk_norm_rope(const b200q_qk_norm_args* args, void* stream) {
   NormArgs a{};
   int sms = 0;
-  if ((rc = host_device(&sms, &a.err))) return rc;
-  a.side[0] = {q, q_ts, q_hs, q_w, q_out, qo_ts, qo_hs, nullptr, hq};
-  a.side[1] = {k, k_ts, k_hs, k_w, k_out, ko_ts, ko_hs, nullptr, hk};
-  a.table = table;
-  a.pos = pos;
-  a.positions = positions;
-  a.t = t;
-  a.d = d;
-  a.rot = rot;
-  a.interleaved = interleaved;
-  a.eps = eps;
+  int rc = norm_args(args, &a, &sms);
+  if (rc) return rc;
+  const int ftype = args->ftype, t = a.t, hq = args->hq, hk = args->hk, d = a.d;
+  if (t == 0 || hq + hk == 0) return B200Q_OK;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const int size = ftype == B200Q_F32 ? 4 : 2;
   if (rows_fit(a, size, false)) {
@@ -485,28 +485,15 @@ extern "C" int b200q_qk_norm_rope(const void* q, long long q_ts, long long q_hs,
   return rc;
 }
 
-extern "C" int b200q_qk_norm_rope_bprop(const void* dq_out, const void* dk_out, const void* q, long long q_ts,
-                                        long long q_hs, const void* k, long long k_ts, long long k_hs, const void* q_w,
-                                        const void* k_w, const float* table, int positions, const int32_t* pos,
-                                        void* dq, void* dk, void* dq_w, void* dk_w, int ftype, int t, int hq, int hk,
-                                        int d, int rot, int interleaved, float eps, void* stream) {
-  int rc = check_norm(q, k, table, positions, pos, ftype, t, hq, hk, d, rot);
-  if (rc) return rc;
-  if (t > 0 && ((hq && (!dq_out || !dq)) || (hk && (!dk_out || !dk))))
-    return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
+extern "C" int b200q_qk_norm_rope_bprop(const b200q_qk_norm_args* args, void* stream) {
   NormArgs a{};
   int sms = 0;
-  if ((rc = host_device(&sms, &a.err))) return rc;
-  a.side[0] = {q, q_ts, q_hs, q_w, dq, 0, 0, dq_out, hq};
-  a.side[1] = {k, k_ts, k_hs, k_w, dk, 0, 0, dk_out, hk};
-  a.table = table;
-  a.pos = pos;
-  a.positions = positions;
-  a.t = t;
-  a.d = d;
-  a.rot = rot;
-  a.interleaved = interleaved;
-  a.eps = eps;
+  int rc = norm_args(args, &a, &sms);
+  if (rc) return rc;
+  const int ftype = args->ftype, t = a.t, hq = args->hq, hk = args->hk, d = a.d;
+  if (t > 0 && ((hq && !args->q_grad) || (hk && !args->k_grad)))
+    return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
+  if ((rc = host_device(&sms, &a.err))) return rc;  // no tokens still mean weight gradients of zero
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const int size = ftype == B200Q_F32 ? 4 : 2;
   const bool fast = rows_fit(a, size, true);
@@ -532,8 +519,8 @@ extern "C" int b200q_qk_norm_rope_bprop(const void* dq_out, const void* dk_out, 
       qk_norm_rope_bprop_kernel<T><<<blocks, kNormWarps * 32, smem, cs>>>(a);
     }
     if ((rc = host_check_launch("qk_norm_rope_bprop_kernel launch"))) return rc;
-    norm_weight_grad_kernel<T><<<(2 * d + 31) / 32, 1024, 0, cs>>>(a.partial, blocks, d, static_cast<T*>(dq_w),
-                                                                 static_cast<T*>(dk_w));
+    norm_weight_grad_kernel<T><<<(2 * d + 31) / 32, 1024, 0, cs>>>(a.partial, blocks, d, static_cast<T*>(args->q_w_grad),
+                                                                 static_cast<T*>(args->k_w_grad));
   });
   rc = host_check_launch("norm_weight_grad_kernel launch");
   if (rc == B200Q_OK) host_set_path(18);

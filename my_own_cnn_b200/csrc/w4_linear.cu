@@ -42,7 +42,7 @@ struct W4Args {
   int x_vec;  // x rows may be read 16 bytes at a time
 };
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;
 constexpr int kRowsW = 32 * kWarps;  // weight rows of a block
 constexpr int kStep = 256;           // columns of a step: 128 bytes of codes per row
 constexpr int kStages = 3;
@@ -79,15 +79,15 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// A step's x on its way: warp w has rows w, w + 4, ..., lane l columns 8 l to 8 l + 7 of the step.
+// A step's x on its way: warp w has rows w and w + 8, lane l columns 8 l to 8 l + 7 of the step.
 template <typename T, int NT>
 struct XRows {
-  alignas(16) T v[2 * NT][8];
+  alignas(16) T v[NT][8];
 
   __device__ __forceinline__ void load(const W4Args& a, int m0, int rows, int k0) {
     const int warp = threadIdx.x / 32, k = k0 + threadIdx.x % 32 * 8;
 #pragma unroll
-    for (int i = 0; i < 2 * NT; ++i) {
+    for (int i = 0; i < NT; ++i) {
       const int m = i * kWarps + warp;
       if (m < rows) {
         const T* from = static_cast<const T*>(a.x) + (m0 + m) * a.ldx + k;
@@ -114,35 +114,37 @@ struct XRows {
     // thread t of a quad owns G / 4 columns of a group, kWords words of 8
     const int group = q / (G / 8), t = q % (G / 8) / kWords, block = group * kWords + q % kWords;
 #pragma unroll
-    for (int i = 0; i < 2 * NT; ++i) {
+    for (int i = 0; i < NT; ++i) {
       const int m = i * kWarps + warp;
       if (m < rows) {
-        float f[8], top = 0.0f;
+        float2 f[4];  // pairs (j, j + 4)
+        float top = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          f[j] = to_f32(v[i][j]);
-          top = fmaxf(top, fabsf(f[j]));
+        for (int j = 0; j < 4; ++j) {
+          f[j] = make_float2(to_f32(v[i][j]), to_f32(v[i][j + 4]));
+          top = fmaxf(fmaxf(fabsf(f[j].x), fabsf(f[j].y)), top);
         }
-        float sum = ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+        const float2 half = add2(add2(f[0], f[1]), add2(f[2], f[3]));
+        float sum = half.x + half.y;
 #pragma unroll
         for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
         if (q % (G / 8) == 0) xsum[group * (8 * NT) + m] = sum;
         const Power p = power_for(warp_max(top));
         if (q == 0) xpower[m] = p.down;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] *= p.up;
+        for (int j = 0; j < 4; ++j) f[j] = mul2(f[j], both(p.up));
 #pragma unroll
         for (int term = 0; term < L::kTerms; ++term) {
           uint32_t w[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            w[j] = pack_f16(f[j], f[j + 4]);
-            if (term + 1 < L::kTerms || j % 2) {
-              const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-              f[j] -= back.x;
-              f[j + 4] -= back.y;
-              if (j % 2) w[j] = pack_f16(back.x * 0.0625f, back.y * 0.0625f);
+            w[j] = pack_f16(f[j].x, f[j].y);
+            __half2& h = *reinterpret_cast<__half2*>(&w[j]);
+            if (term + 1 < L::kTerms) {
+              const float2 back = __half22float2(h);
+              f[j] = make_float2(f[j].x - back.x, f[j].y - back.y);
             }
+            if (j % 2) h = __hmul2(h, __float2half2_rn(0.0625f));
           }
           xs[((block * L::kTerms + term) * (8 * NT) + m) * 4 + t] = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -152,7 +154,7 @@ struct XRows {
 };
 
 template <typename T, int G, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) linear_w4_kernel(W4Args a) {
+__global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
   using L = Layout<T, G, NT>;
   constexpr int kTerms = L::kTerms, kWords = G / 32, kGroups = kStep / G;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -181,25 +183,35 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) linear_w4_kernel
       }
     }
   };
-  // scales and zero points: lane l holds those of row l, read a step before their use
+  // scales and zero points: lane l holds those of row l, read a step before their use; past K's last group it repeats
   const int my_row = min(row0 + lane, a.n - 1), groups = (a.k + G - 1) / G;
   uint32_t scale[kGroups], zero[kGroups], next_scale[kGroups], next_zero[kGroups];
   auto load_params = [&](int s) {
+    const int first = (step0 + s) * kGroups;
+    const long long at = static_cast<long long>(first) * a.n + my_row;
+    const uint16_t* sp = a.scales + at;
+    const uint8_t* zp = a.zeros + at;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
-      const long long at = static_cast<long long>(min((step0 + s) * kGroups + i, groups - 1)) * a.n + my_row;
-      next_scale[i] = __ldg(a.scales + at);
-      next_zero[i] = a.zeros ? __ldg(a.zeros + at) : 8u;
+      next_scale[i] = __ldg(sp);
+      next_zero[i] = a.zeros ? __ldg(zp) : 8u;
+      if (first + i + 1 < groups) sp += a.n, zp += a.n;
     }
   };
 
-  float acc[2][NT][4], less[8 * NT];  // sums of products; lane l's row: sums of zero points
+  // sums of products, [16 rows][8 columns][row g or g + 8] for columns 2t, 2t + 1; of lane l's row, sums of zero points
+  float2 acc[2][NT][2], less[4 * NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
+    acc[0][n][0] = acc[0][n][1] = acc[1][n][0] = acc[1][n][1] = both(0.0f);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[0][n][e] = acc[1][n][e] = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) less[n * 8 + e] = 0.0f;
+    for (int e = 0; e < 4; ++e) less[n * 4 + e] = both(0.0f);
+  }
+  // columns that no row of x has stay zero in both buffers
+  for (int i = threadIdx.x; i < 2 * L::kX / 16; i += kWarps * 32) {
+    const int at = i % (L::kX / 16);
+    if (at / 4 % (8 * NT) >= rows)
+      *reinterpret_cast<uint4*>(smem + kRing + i / (L::kX / 16) * L::kBuffer + at * 16) = make_uint4(0, 0, 0, 0);
   }
   XRows<T, NT> x;
   if (steps > 0) {
@@ -231,7 +243,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) linear_w4_kernel
     const float* const xsum = reinterpret_cast<const float*>(buffer + L::kX);
     const float* const xpower = reinterpret_cast<const float*>(buffer + L::kX + L::kXSum);
     const uint8_t* const stage = smem + warp * (kStages * kStage) + slot * kStage;
-    float sum[2][NT][4];
+    float2 sum[2][NT][2];
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       uint32_t w[4][kWords];  // rows g, g + 8, g + 16, g + 24
@@ -257,8 +269,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) linear_w4_kernel
         for (int term = 0; term < kTerms; ++term)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
-            b[term][n] = n * 8 + g < rows ? xs[(((i * kWords + word) * kTerms + term) * (8 * NT) + n * 8 + g) * 4 + t]
-                                          : make_uint4(0, 0, 0, 0);
+            b[term][n] = xs[(((i * kWords + word) * kTerms + term) * (8 * NT) + n * 8 + g) * 4 + t];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           const uint32_t w0 = w[2 * mt][word], w1 = w[2 * mt + 1][word], v0 = w0 >> 8, v1 = w1 >> 8;
@@ -279,24 +290,21 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) linear_w4_kernel
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float sc = __uint_as_float(__shfl_sync(~0u, scale[i], r * 8 + g));
+        const float2 sc = both(__uint_as_float(__shfl_sync(~0u, scale[i], r * 8 + g)));
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& to = sum[r / 2][n][r % 2 * 2 + e];
-            to = i == 0 ? sc * part[r / 2][n][r % 2 * 2 + e] : fmaf(sc, part[r / 2][n][r % 2 * 2 + e], to);
-          }
+        for (int n = 0; n < NT; ++n) {
+          const float* p = part[r / 2][n] + r % 2 * 2;
+          float2& to = sum[r / 2][n][r % 2];
+          to = i == 0 ? mul2(sc, make_float2(p[0], p[1])) : fma2(sc, make_float2(p[0], p[1]), to);
+        }
       }
-      const float sz = __uint_as_float(scale[i]) * static_cast<float>(zero[i]);
+      const float2 sz = both(__uint_as_float(scale[i]) * static_cast<float>(zero[i]));
 #pragma unroll
       for (int m = 0; m < 8 * NT; m += 4)
         if (m < rows) {
           const float4 v = *reinterpret_cast<const float4*>(xsum + i * (8 * NT) + m);
-          less[m] = fmaf(sz, v.x, less[m]);
-          less[m + 1] = fmaf(sz, v.y, less[m + 1]);
-          less[m + 2] = fmaf(sz, v.z, less[m + 2]);
-          less[m + 3] = fmaf(sz, v.w, less[m + 3]);
+          less[m / 2] = fma2(sz, make_float2(v.x, v.y), less[m / 2]);
+          less[m / 2 + 1] = fma2(sz, make_float2(v.z, v.w), less[m / 2 + 1]);
         }
     }
 #pragma unroll
@@ -305,7 +313,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) linear_w4_kernel
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[mt][n][e] = fmaf(e % 2 ? p.y : p.x, sum[mt][n][e], acc[mt][n][e]);
+        for (int u = 0; u < 2; ++u) acc[mt][n][u] = fma2(p, sum[mt][n][u], acc[mt][n][u]);
     }
     slot = slot + 1 == kStages ? 0 : slot + 1;
     fill = fill + 1 == kStages ? 0 : fill + 1;
@@ -318,11 +326,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) linear_w4_kernel
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        sums[(n * 8 + 2 * t + e % 2) * kRowsW + warp * 32 + mt * 16 + e / 2 * 8 + g] = acc[mt][n][e] * 16777216.0f;
+      for (int u = 0; u < 2; ++u) {
+        float* to = sums + (n * 8 + 2 * t) * kRowsW + warp * 32 + mt * 16 + u * 8 + g;
+        to[0] = acc[mt][n][u].x * 16777216.0f;
+        to[kRowsW] = acc[mt][n][u].y * 16777216.0f;
+      }
   __syncwarp();
 #pragma unroll
-  for (int m = 0; m < 8 * NT; ++m) sums[m * kRowsW + warp * 32 + lane] -= less[m];
+  for (int m = 0; m < 8 * NT; ++m) sums[m * kRowsW + warp * 32 + lane] -= m % 2 ? less[m / 2].y : less[m / 2].x;
   if (splits > 1)
     cluster_sync();
   else
@@ -386,25 +397,25 @@ int launch_linear_rows(const W4Args& a, int sms, cudaStream_t stream) {
 
 using namespace b200q;
 
-extern "C" int b200q_linear_w4(const void* x, long long ldx, const uint8_t* codes, const void* scales,
-                               const uint8_t* zeros, const void* bias, void* y, long long ldy, int ftype, int m, int n,
-                               int k, int group, void* stream) {
+extern "C" int b200q_linear_w4(const b200q_linear_w4_args* p, void* stream) {
+  if (!p) return host_fail(B200Q_ERR_INVALID_ARG, "null argument");
+  const int ftype = p->ftype, m = p->m, n = p->n, k = p->k, group = p->group;
   if (ftype < B200Q_F32 || ftype > B200Q_BF16) return host_fail(B200Q_ERR_INVALID_ARG, "bad floating type %d", ftype);
   if (m < 0 || n < 0 || k < 0) return host_fail(B200Q_ERR_INVALID_ARG, "negative linear dimension");
   if (group != 32 && group != 64 && group != 128)
     return host_fail(B200Q_ERR_INVALID_ARG, "weight group must be 32, 64 or 128, got %d", group);
   if (m == 0 || n == 0) return B200Q_OK;
-  if (!y || (k > 0 && (!x || !codes || !scales))) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
-  if ((m > 1 && ldx < k) || (m > 1 && ldy < n)) return host_fail(B200Q_ERR_INVALID_ARG, "row stride below row length");
-  if (reinterpret_cast<uintptr_t>(codes) & 15u)
+  if (!p->y || (k > 0 && (!p->x || !p->codes || !p->scales))) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
+  if (m > 1 && (p->ldx < k || p->ldy < n)) return host_fail(B200Q_ERR_INVALID_ARG, "row stride below row length");
+  if (reinterpret_cast<uintptr_t>(p->codes) & 15u)
     return host_fail(B200Q_ERR_INVALID_ARG, "4-bit weight codes must be 16-byte aligned");
   if (n > (1 << 28) || k > (1 << 28) || m > (1 << 19)) return host_fail(B200Q_ERR_UNSUPPORTED, "linear too large");
   int sms = 0, *err = nullptr;
   int rc = host_device(&sms, &err);
   if (rc) return rc;
-  W4Args a{x, ldx, codes, static_cast<const uint16_t*>(scales), zeros, bias, y, ldy, m, n, k};
+  W4Args a{p->x, p->ldx, p->codes, static_cast<const uint16_t*>(p->scales), p->zeros, p->bias, p->y, p->ldy, m, n, k};
   const size_t size = ftype == B200Q_F32 ? 4 : 2;
-  a.x_vec = (reinterpret_cast<uintptr_t>(x) & 15u) == 0 && (m == 1 || ldx * size % 16 == 0);
+  a.x_vec = (reinterpret_cast<uintptr_t>(p->x) & 15u) == 0 && (m == 1 || p->ldx * size % 16 == 0);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   B200Q_DISPATCH_FTYPE(ftype, rc = group == 32   ? launch_linear_rows<T, 32>(a, sms, cs)
                                    : group == 64 ? launch_linear_rows<T, 64>(a, sms, cs)

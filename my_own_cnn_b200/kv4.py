@@ -7,13 +7,15 @@
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 from .conv import _stream
 from .w4 import FTYPES, _device_tensor, _ftype, _on
+
+
+_CACHE = _lib.packer(_lib.CKV4Cache)
+_ARGS = _lib.packer(_lib.CKV4AttentionArgs)
 
 
 class KV4Cache:
@@ -44,8 +46,8 @@ class KV4Cache:
         self.pages, self.heads, self.page_size = shape[0], shape[1], shape[2]
         self.head_dim = 2 * shape[3]
         self.group = self.head_dim // pshape[3]
-        self._c = _lib.CKV4Cache(k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(),
-                                 self.pages, self.heads, self.page_size, self.head_dim, self.group)
+        self._c = _CACHE.pack(k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(),
+                              self.pages, self.heads, self.page_size, self.head_dim, self.group)
 
     @staticmethod
     def empty(pages: int, heads: int, page_size: int, head_dim: int, group: int = 64, device="cuda") -> "KV4Cache":
@@ -87,7 +89,7 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.T
 
 def _append(cache, k, v, slots, ft, stream):
     (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
-    _lib.check(_lib.lib().b200q_kv4_append(ctypes.byref(cache._c), k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
+    _lib.check(_lib.lib().b200q_kv4_append(cache._c, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
                                            slots.data_ptr(), ft, k.shape[0], stream))
 
 
@@ -102,7 +104,7 @@ def kv4_read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.fl
         shape = (slots.shape[0], cache.heads, cache.head_dim)
         k = slots.new_empty(shape, dtype=dtype)
         v = slots.new_empty(shape, dtype=dtype)
-        _lib.check(_lib.lib().b200q_kv4_read(ctypes.byref(cache._c), slots.data_ptr(), k.data_ptr(), v.data_ptr(), ft,
+        _lib.check(_lib.lib().b200q_kv4_read(cache._c, slots.data_ptr(), k.data_ptr(), v.data_ptr(), ft,
                                              shape[0], _stream(stream)))
     return k, v
 
@@ -140,8 +142,9 @@ def _attention(q, cache, block_table, lens, scale, out, return_lse, ft, b, tq, h
     elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or not out.is_cuda:
         raise RuntimeError(f"out must be a contiguous {q.dtype} {list(q.shape)} CUDA tensor")
     lse = q.new_empty((b, tq, hq), dtype=torch.float32) if return_lse else None
-    _lib.check(_lib.lib().b200q_kv4_attention(ctypes.byref(cache._c), q.data_ptr(), qb, qt, qh, block_table.data_ptr(),
-                                              block_table.stride(0), lens.data_ptr(), out.data_ptr(),
-                                              lse.data_ptr() if return_lse else 0, ft, b, tq, hq,
-                                              block_table.shape[1], d ** -0.5 if scale is None else scale, stream))
+    _lib.check(_lib.lib().b200q_kv4_attention(cache._c, _ARGS.pack(q.data_ptr(), qb, qt, qh, block_table.data_ptr(),
+                                                                   block_table.stride(0), lens.data_ptr(),
+                                                                   out.data_ptr(), lse.data_ptr() if return_lse else 0,
+                                                                   ft, b, tq, hq, block_table.shape[1],
+                                                                   d ** -0.5 if scale is None else scale), stream))
     return (out, lse) if return_lse else out

@@ -13,6 +13,9 @@ from .conv import _stream
 from .w4 import _device_tensor, _ftype, _on
 
 
+_ARGS = _lib.packer(_lib.CQKNormArgs)
+
+
 def rope_table(positions: int, rot: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
     """cos, then sin, of position * base^(-2 i / rot), i < rot / 2 (angles in 64 bits, stored as fp32)."""
     f = base ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
@@ -84,10 +87,10 @@ def _norm(q, k, q_weight, k_weight, table, positions, eps, interleaved, q_out, k
         pt, ph = hk * d, d
     else:
         pt, ph = _out_strides(k_out, k, "k_out")
-    _lib.check(_lib.lib().b200q_qk_norm_rope(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, _p(q_weight), _p(k_weight),
-                                             _p(table), rows, _p(positions), q_out.data_ptr(), ot, oh,
-                                             k_out.data_ptr(), pt, ph, ft, t, hq, hk, d, rot, interleaved, eps,
-                                             stream))
+    _lib.check(_lib.lib().b200q_qk_norm_rope(_ARGS.pack(q.data_ptr(), k.data_ptr(), _p(q_weight), _p(k_weight), _p(table),
+                                                        _p(positions), q_out.data_ptr(), k_out.data_ptr(), 0, 0, 0, 0,
+                                                        qt, qh, kt, kh, ot, oh, pt, ph, rows, ft, t, hq, hk, d, rot,
+                                                        interleaved, eps), stream))
     return q_out, k_out
 
 
@@ -116,9 +119,9 @@ def qk_norm_rope_bprop(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: t
         gq, gk = q.new_empty(dq.shape), k.new_empty(dk.shape)
         gqw = None if q_weight is None else q.new_empty((d,))
         gkw = None if k_weight is None else q.new_empty((d,))
-        _lib.check(_lib.lib().b200q_qk_norm_rope_bprop(dq.data_ptr(), dk.data_ptr(), q.data_ptr(), q.stride(0),
-                                                       q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                                                       _p(q_weight), _p(k_weight), _p(table), rows, _p(positions),
-                                                       gq.data_ptr(), gk.data_ptr(), _p(gqw), _p(gkw), ft, t, hq, hk,
-                                                       d, rot, interleaved, eps, _stream(stream)))
+        _lib.check(_lib.lib().b200q_qk_norm_rope_bprop(
+            _ARGS.pack(q.data_ptr(), k.data_ptr(), _p(q_weight), _p(k_weight), _p(table), _p(positions), gq.data_ptr(),
+                       gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), _p(gqw), _p(gkw), q.stride(0), q.stride(1),
+                       k.stride(0), k.stride(1), 0, 0, 0, 0, rows, ft, t, hq, hk, d, rot, interleaved, eps),
+            _stream(stream)))
     return gq, gk, gqw, gkw

@@ -14,6 +14,7 @@ import torch
 from . import _lib
 from .conv import _stream
 
+_ARGS = _lib.packer(_lib.CLinearW4Args)
 FTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 GROUPS = (32, 64, 128)
 
@@ -138,8 +139,8 @@ def _linear(x, w, bias, out, ft, n, k, stream):
             y, ldy = out, n
         else:
             raise RuntimeError("out must be contiguous, or 2-D with contiguous rows")
-    _lib.check(_lib.lib().b200q_linear_w4(rows.data_ptr(), rows.stride(0), w.codes.data_ptr(), w.scales.data_ptr(),
-                                          0 if w.zeros is None else w.zeros.data_ptr(),
-                                          0 if bias is None else bias.data_ptr(), y.data_ptr(), ldy, ft, m, n, k,
-                                          w.group, stream))
+    _lib.check(_lib.lib().b200q_linear_w4(_ARGS.pack(rows.data_ptr(), rows.stride(0), w.codes.data_ptr(),
+                                                     w.scales.data_ptr(), 0 if w.zeros is None else w.zeros.data_ptr(),
+                                                     0 if bias is None else bias.data_ptr(), y.data_ptr(), ldy, ft, m,
+                                                     n, k, w.group), stream))
     return out

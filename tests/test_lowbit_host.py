@@ -43,13 +43,26 @@ def test_rotation_table():
     assert abs(t[3, 1] - want.cos()) < 1e-7 and abs(t[3, 4] - want.sin()) < 1e-7
 
 
+def block(layout, values):
+    return bytes(layout(*values))
+
+
 def cache(**over):
     v = dict(k_codes=4096, k_params=4096, v_codes=4096, v_params=4096, pages=1, heads=2, page_size=16, d=64, group=32)
     v.update(over)
-    return ctypes.byref(_lib.CKV4Cache(*v.values()))
+    return block(_lib.CKV4Cache, v.values())
 
 
 P = 1 << 20  # an address that is never used
+
+
+@pytest.mark.parametrize("layout,size", [(_lib.CLinearW4Args, 88), (_lib.CQKNormArgs, 200), (_lib.CKV4AttentionArgs, 96),
+                                         (_lib.CKV4Cache, 56)])
+def test_argument_blocks_have_the_header_layout(layout, size):
+    """Sizes as a C compiler gives them, and the packed bytes equal to the structure's."""
+    values = [(3 * i + 1) if t is not ctypes.c_float else 0.5 for i, (_, t) in enumerate(layout._fields_)]
+    assert ctypes.sizeof(layout) == size
+    assert _lib.packer(layout).pack(*values) == bytes(layout(*values))
 
 
 @pytest.mark.parametrize("rc,message,args", [
@@ -65,12 +78,13 @@ P = 1 << 20  # an address that is never used
 ])
 def test_linear_refusals(rc, message, args):
     L = _lib.lib()
-    assert L.b200q_linear_w4(*args) == rc
+    assert L.b200q_linear_w4(block(_lib.CLinearW4Args, args[:-1]), args[-1]) == rc
     assert message is None or message in L.b200q_last_error()
 
 
-def norm_args(ft=0, q=P, table=P, positions=8, pos=P, t=1, hq=2, hk=1, d=64, rot=64):
-    return (q, 0, 0, P, 0, 0, 0, 0, table, positions, pos, P, 0, 0, P, 0, 0, ft, t, hq, hk, d, rot, 0, 1e-6, 0)
+def norm_args(ft=0, q=P, table=P, positions=8, pos=P, t=1, hq=2, hk=1, d=64, rot=64, grad=P):
+    return block(_lib.CQKNormArgs, (q, P, 0, 0, table, pos, P, P, grad, grad, P, P, *[0] * 8, positions, ft, t, hq, hk, d, rot,
+                                    0, 1e-6))
 
 
 @pytest.mark.parametrize("rc,message,kw", [
@@ -81,11 +95,10 @@ def norm_args(ft=0, q=P, table=P, positions=8, pos=P, t=1, hq=2, hk=1, d=64, rot
 ])
 def test_norm_refusals(rc, message, kw):
     L = _lib.lib()
-    assert L.b200q_qk_norm_rope(*norm_args(**kw)) == rc
+    assert L.b200q_qk_norm_rope(norm_args(**kw), 0) == rc
     assert message is None or message in L.b200q_last_error()
     if rc != OK:
-        a = norm_args(**kw)
-        assert L.b200q_qk_norm_rope_bprop(P, P, *a[:11], P, P, P, P, *a[17:]) == rc
+        assert L.b200q_qk_norm_rope_bprop(norm_args(**kw), 0) == rc
 
 
 @pytest.mark.parametrize("rc,message,kw", [
@@ -96,15 +109,19 @@ def test_norm_refusals(rc, message, kw):
 def test_cache_refusals(rc, message, kw):
     L = _lib.lib()
     for call in (lambda c: L.b200q_kv4_append(c, P, 0, 0, P, 0, 0, P, 0, 1, 0), lambda c: L.b200q_kv4_read(c, P, P, P, 0, 1, 0),
-                 lambda c: L.b200q_kv4_attention(c, P, 0, 0, 0, P, 1, P, P, 0, 0, 1, 1, 2, 1, 1.0, 0)):
+                 lambda c: L.b200q_kv4_attention(c, attention_args(), 0)):
         assert call(cache(**kw)) == rc and message in L.b200q_last_error()
+
+
+def attention_args(hq=2, b=1, tq=1, lens=P, table=P, max_pages=1, ft=0):
+    return block(_lib.CKV4AttentionArgs, (P, 0, 0, 0, table, 1, lens, P, 0, ft, b, tq, hq, max_pages, 1.0))
 
 
 def test_attention_refusals():
     L = _lib.lib()
 
-    def call(hq=2, b=1, tq=1, lens=P, table=P, max_pages=1, ft=0):
-        return L.b200q_kv4_attention(cache(), P, 0, 0, 0, table, 1, lens, P, 0, ft, b, tq, hq, max_pages, 1.0, 0)
+    def call(**kw):
+        return L.b200q_kv4_attention(cache(), attention_args(**kw), 0)
 
     assert call(hq=3) == INVALID and b"divide" in L.b200q_last_error()
     assert call(lens=0) == INVALID and call(table=0) == INVALID and call(ft=7) == INVALID and call(tq=-1) == INVALID
