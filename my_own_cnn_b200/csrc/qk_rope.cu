@@ -4,11 +4,13 @@
 //   n = x r w, r = (mean x^2 + eps)^-1/2;  y = R(pos) n
 //   dn = R^T dy;  dw = sum dn x r;  with v = dn w: dx = r (v - x r^2 mean(v x))
 //
-// Bytes bound both: x in, y out; the gradient reads x and dy and writes dx.  A row of 64, 128 or 256 channels lies
-// in the registers of 8 to 32 lanes, 16 bytes or D / 32 channels each, from one read to one write: the mean is a
-// few shuffles, a rotation partner one more.  A group of lanes takes several heads of one token, so that it
-// reads the token's cosines and sines once, and has kUnroll rows on their way at a time.  Other head sizes, rotations
-// that are no power of two and unaligned rows go one warp per row through strided loops.
+// Bytes bound both: x in, y out; the gradient reads x and dy and writes dx.  A row of up to 256 channels lies in the
+// registers of 8, 16 or 32 lanes, 8 channels each, from one read to one write.  Which 8: four pairs that rotate
+// together, so that a rotation needs no other lane (half and half: 4 channels of the first half of the rotated ones and
+// the 4 that they turn with; interleaved: 8 in a row), and four cosines and sines.  The mean is a few shuffles.  A group
+// of lanes takes several heads of one token, so that it reads the token's angles and the weights once, and has
+// kAhead rows on their way at a time.  Rows that are not aligned, and sizes that are no multiple of 8, go one warp per row
+// through strided loops.
 #include <algorithm>
 
 #include "host.h"
@@ -161,221 +163,285 @@ __global__ void qk_norm_rope_bprop_kernel(NormArgs a) {
   }
 }
 
-// Rows of D channels in LPR lanes of V channels.
-template <typename T, int D>
-struct RowShape {
-  static constexpr int V = 16 / sizeof(T) > D / 32 ? 16 / sizeof(T) : D / 32;
-  static constexpr int LPR = D / V;
-};
 constexpr int kFastThreads = 128;
-constexpr int kUnroll = 4;
+constexpr int kAhead = 4;
 
-template <typename T, int V>
-__device__ __forceinline__ void load_row(const T* p, bool ok, T (&v)[V]) {
-  uint4* to = reinterpret_cast<uint4*>(v);
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(V * sizeof(T) / 16); ++i)
-    to[i] = ok ? *(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+// Four channels in memory, as two fp32 pairs.
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+  using Bits = uint4;
+  static __device__ __forceinline__ void get(const Bits& v, float2 (&x)[2]) {
+    x[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+    x[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+  }
+  static __device__ __forceinline__ Bits put(const float2 (&x)[2]) {
+    return make_uint4(__float_as_uint(x[0].x), __float_as_uint(x[0].y), __float_as_uint(x[1].x), __float_as_uint(x[1].y));
+  }
+};
+template <>
+struct Four<__half> {
+  using Bits = uint2;
+  static __device__ __forceinline__ void get(const Bits& v, float2 (&x)[2]) {
+    x[0] = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
+    x[1] = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+  }
+  static __device__ __forceinline__ Bits put(const float2 (&x)[2]) {
+    return make_uint2(pack_f16(x[0].x, x[0].y), pack_f16(x[1].x, x[1].y));
+  }
+};
+template <>
+struct Four<__nv_bfloat16> {
+  using Bits = uint2;
+  static __device__ __forceinline__ void get(const Bits& v, float2 (&x)[2]) {
+    x[0] = make_float2(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u));
+    x[1] = make_float2(__uint_as_float(v.y << 16), __uint_as_float(v.y & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ Bits put(const float2 (&x)[2]) {
+    return make_uint2(pack_bf16(x[0].x, x[0].y), pack_bf16(x[1].x, x[1].y));
+  }
+};
+
+// A lane's 8 channels of a row: two fours at `at[0]` and `at[1]`.
+struct Lane {
+  int at[2];
+  bool there;    // a row of fewer channels than its lanes can hold leaves the last lanes empty
+  bool rotated;
+};
+template <bool INTERLEAVED>
+__device__ __forceinline__ Lane lane_of(const NormArgs& a, int l) {
+  Lane r;
+  r.rotated = 8 * l < a.rot;
+  r.there = 8 * l < a.d;
+  r.at[0] = !INTERLEAVED && r.rotated ? 4 * l : 8 * l;
+  r.at[1] = !INTERLEAVED && r.rotated ? a.rot / 2 + 4 * l : 8 * l + 4;
+  return r;
 }
-template <typename T, int V>
-__device__ __forceinline__ void store_row(T* p, const float (&v)[V]) {
-  alignas(16) T out[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) out[j] = from_f32<T>(v[j]);
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(V * sizeof(T) / 16); ++i)
-    *(reinterpret_cast<uint4*>(p) + i) = reinterpret_cast<const uint4*>(out)[i];
+
+// The two fours as pairs that turn together: x[i].x with y[i].x, x[i].y with y[i].y, angles 2 i and 2 i + 1.
+template <bool INTERLEAVED>
+__device__ __forceinline__ void to_pairs(const float2 (&f0)[2], const float2 (&f1)[2], float2 (&x)[2], float2 (&y)[2]) {
+  if constexpr (INTERLEAVED) {
+    x[0] = make_float2(f0[0].x, f0[1].x), y[0] = make_float2(f0[0].y, f0[1].y);
+    x[1] = make_float2(f1[0].x, f1[1].x), y[1] = make_float2(f1[0].y, f1[1].y);
+  } else {
+    x[0] = f0[0], x[1] = f0[1], y[0] = f1[0], y[1] = f1[1];
+  }
+}
+template <bool INTERLEAVED>
+__device__ __forceinline__ void from_pairs(const float2 (&x)[2], const float2 (&y)[2], float2 (&f0)[2], float2 (&f1)[2]) {
+  if constexpr (INTERLEAVED) {
+    f0[0] = make_float2(x[0].x, y[0].x), f0[1] = make_float2(x[0].y, y[0].y);
+    f1[0] = make_float2(x[1].x, y[1].x), f1[1] = make_float2(x[1].y, y[1].y);
+  } else {
+    f0[0] = x[0], f0[1] = x[1], f1[0] = y[0], f1[1] = y[1];
+  }
 }
 
-// The rotation of a lane's V channels: y = x c + (partner) s, where the partner is the channel rot / 2 away, in lane
-// `lane ^ dist`, or the neighbour in the lane itself (interleaved).  The sine carries the sign.
-template <int V>
-struct Rotation {
-  float c[V], s[V];
-  int dist;
-  bool interleaved;
-
-  // Lane l of a row; `row` null: no rotation.
-  __device__ __forceinline__ void load(const NormArgs& a, const float* row, int l) {
-    interleaved = a.interleaved;
-    dist = interleaved ? 0 : a.rot / 2 / V;
-    const int ch = l * V;
-#pragma unroll
-    for (int j = 0; j < V; ++j) c[j] = 1.0f, s[j] = 0.0f;
-    if (!row || ch >= a.rot) return;
-    if (interleaved) {
-#pragma unroll
-      for (int j = 0; j < V; j += 2) {
-        c[j] = c[j + 1] = __ldg(row + (ch + j) / 2);
-        s[j + 1] = __ldg(row + a.rot / 2 + (ch + j) / 2);
-        s[j] = -s[j + 1];
-      }
-    } else {
-      const int at = ch & (a.rot / 2 - 1);
-#pragma unroll
-      for (int j = 0; j < V; j += 4) {
-        const float4 cv = __ldg(reinterpret_cast<const float4*>(row + at + j));
-        const float4 sv = __ldg(reinterpret_cast<const float4*>(row + a.rot / 2 + at + j));
-        c[j] = cv.x, c[j + 1] = cv.y, c[j + 2] = cv.z, c[j + 3] = cv.w;
-        s[j] = sv.x, s[j + 1] = sv.y, s[j + 2] = sv.z, s[j + 3] = sv.w;
-      }
-      if (ch < a.rot / 2) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = -s[j];
-      }
+template <typename T, bool INTERLEAVED>
+struct Row {
+  typename Four<T>::Bits bits[2];
+  __device__ __forceinline__ void load(const T* p, const Lane& l, bool ok) {
+    bits[0] = bits[1] = {};
+    if (ok) {
+      bits[0] = *reinterpret_cast<const typename Four<T>::Bits*>(p + l.at[0]);
+      bits[1] = *reinterpret_cast<const typename Four<T>::Bits*>(p + l.at[1]);
     }
   }
-  // Every lane of the warp takes part.
-  template <bool BACK>
-  __device__ __forceinline__ void apply(float (&v)[V]) const {
-    float other[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) other[j] = interleaved ? v[j ^ 1] : __shfl_xor_sync(~0u, v[j], dist);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = fmaf(other[j], BACK ? -s[j] : s[j], v[j] * c[j]);
+  __device__ __forceinline__ void get(float2 (&x)[2], float2 (&y)[2]) const {
+    float2 f0[2], f1[2];
+    Four<T>::get(bits[0], f0);
+    Four<T>::get(bits[1], f1);
+    to_pairs<INTERLEAVED>(f0, f1, x, y);
+  }
+  static __device__ __forceinline__ void store(T* p, const Lane& l, const float2 (&x)[2], const float2 (&y)[2]) {
+    float2 f0[2], f1[2];
+    from_pairs<INTERLEAVED>(x, y, f0, f1);
+    *reinterpret_cast<typename Four<T>::Bits*>(p + l.at[0]) = Four<T>::put(f0);
+    *reinterpret_cast<typename Four<T>::Bits*>(p + l.at[1]) = Four<T>::put(f1);
   }
 };
 
-template <typename T, int V>
-__device__ __forceinline__ void load_weights(const NormArgs& a, int which, int l, float (&w)[V]) {
-  const T* p = static_cast<const T*>(a.side[which].w);
-  if (p) {
-    alignas(16) T raw[V];
-    load_row<T, V>(p + l * V, true, raw);
-#pragma unroll
-    for (int j = 0; j < V; ++j) w[j] = to_f32(raw[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) w[j] = 1.0f;
+// Angles of a lane's four pairs (none: cosine 1, sine 0).
+struct Angles {
+  float2 c[2], s[2];
+  __device__ __forceinline__ void load(const NormArgs& a, const float* row, const Lane& lane, int l) {
+    c[0] = c[1] = both(1.0f);
+    s[0] = s[1] = both(0.0f);
+    if (row && lane.rotated) {
+      const float4 cv = __ldg(reinterpret_cast<const float4*>(row + 4 * l));
+      const float4 sv = __ldg(reinterpret_cast<const float4*>(row + a.rot / 2 + 4 * l));
+      c[0] = make_float2(cv.x, cv.y), c[1] = make_float2(cv.z, cv.w);
+      s[0] = make_float2(sv.x, sv.y), s[1] = make_float2(sv.z, sv.w);
+    }
+  }
+};
+
+template <typename T, bool INTERLEAVED>
+__device__ __forceinline__ void lane_weights(const void* w, const Lane& lane, float2 (&x)[2], float2 (&y)[2]) {
+  x[0] = x[1] = y[0] = y[1] = both(1.0f);
+  if (w) {
+    Row<T, INTERLEAVED> r;
+    r.load(static_cast<const T*>(w), lane, lane.there);
+    r.get(x, y);
   }
 }
 
 template <int LPR>
-__device__ __forceinline__ float row_sum(float v) {
+__device__ __forceinline__ float row_sum(float2 v) {
+  float s = v.x + v.y;
 #pragma unroll
-  for (int o = LPR / 2; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
+  for (int o = LPR / 2; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+  return s;
 }
 
-// A group of LPR lanes takes `per` heads (queries first, then keys) of one token.
-template <typename T, int D>
+// Unit: one side's heads [begin, end) of token t.
+struct Unit {
+  int t, which, begin, end;
+  const float* table;
+  bool ok;
+};
+__device__ __forceinline__ Unit unit_of(const NormArgs& a, long long unit, int per) {
+  const int parts_q = (a.side[0].heads + per - 1) / per, parts = parts_q + (a.side[1].heads + per - 1) / per;
+  Unit u;
+  u.t = static_cast<int>(unit / parts);
+  int part = static_cast<int>(unit - static_cast<long long>(u.t) * parts);
+  u.which = part >= parts_q;
+  if (u.which) part -= parts_q;
+  u.ok = u.t < a.t;
+  u.begin = part * per;
+  u.end = u.ok ? min(a.side[u.which].heads, u.begin + per) : u.begin;
+  u.table = nullptr;
+  if (u.ok && a.rot) u.ok = (u.table = table_row(a, u.t)) != nullptr;
+  return u;
+}
+
+// A group of LPR lanes takes `per` heads of one token's queries or keys.
+template <typename T, int LPR, bool INTERLEAVED>
 __global__ void __launch_bounds__(kFastThreads) qk_norm_rope_rows_kernel(NormArgs a, int per) {
-  constexpr int V = RowShape<T, D>::V, LPR = RowShape<T, D>::LPR;
-  const int l = threadIdx.x % LPR, hq = a.side[0].heads, heads = hq + a.side[1].heads;
-  const int parts = (heads + per - 1) / per;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kFastThreads / LPR) + threadIdx.x / LPR;
-  const int t = static_cast<int>(unit / parts);
-  bool ok = t < a.t;
-  const int begin = static_cast<int>(unit % parts) * per, end = ok ? min(heads, begin + per) : begin;
-  const float* tab = nullptr;
-  if (ok && a.rot) ok = (tab = table_row(a, t)) != nullptr;
-  Rotation<V> rotation;
-  bool known = false;  // the rotation is loaded behind the first rows
-  for (int h0 = begin; __any_sync(~0u, h0 < end); h0 += kUnroll) {
-    alignas(16) T raw[kUnroll][V];
+  const int l = threadIdx.x % LPR;
+  const Lane lane = lane_of<INTERLEAVED>(a, l);
+  const Unit unit = unit_of(a, static_cast<long long>(blockIdx.x) * (kFastThreads / LPR) + threadIdx.x / LPR, per);
+  const NormSide& s = a.side[unit.which];
+  const T* x = static_cast<const T*>(s.x) + unit.t * s.ts;
+  T* y = static_cast<T*>(s.y) + unit.t * s.yts;
+  const float over = 1.0f / static_cast<float>(a.d);
+  Angles angles;
+  float2 w[2], wy[2];
+  for (int h0 = unit.begin; __any_sync(~0u, h0 < unit.end); h0 += kAhead) {
+    Row<T, INTERLEAVED> row[kAhead];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int h = h0 + u, which = h >= hq;
-      const NormSide& s = a.side[which];
-      load_row<T, V>(static_cast<const T*>(s.x) + t * s.ts + (h - (which ? hq : 0)) * s.hs + l * V, h < end, raw[u]);
+    for (int u = 0; u < kAhead; ++u) row[u].load(x + (h0 + u) * s.hs, lane, lane.there && h0 + u < unit.end);
+    if (h0 == unit.begin) {  // behind the first rows
+      angles.load(a, unit.table, lane, l);
+      lane_weights<T, INTERLEAVED>(s.w, lane, w, wy);
     }
-    if (!known) rotation.load(a, tab, l);
-    known = true;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int h = h0 + u, which = h >= hq;
-      float v[V], w[V], sq = 0.0f;
+    for (int u = 0; u < kAhead; ++u) {
+      float2 p[2], q[2];
+      row[u].get(p, q);
+      const float2 sq = fma2(p[0], p[0], fma2(p[1], p[1], fma2(q[0], q[0], mul2(q[1], q[1]))));
+      const float2 r = both(rsqrtf(row_sum<LPR>(sq) * over + a.eps));
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        v[j] = to_f32(raw[u][j]);
-        sq = fmaf(v[j], v[j], sq);
+      for (int i = 0; i < 2; ++i) {
+        const float2 v = mul2(p[i], mul2(r, w[i])), z = mul2(q[i], mul2(r, wy[i]));
+        p[i] = fma2(make_float2(-z.x, -z.y), angles.s[i], mul2(v, angles.c[i]));
+        q[i] = fma2(v, angles.s[i], mul2(z, angles.c[i]));
       }
-      load_weights<T, V>(a, which, l, w);
-      const float r = rsqrtf(row_sum<LPR>(sq) * (1.0f / D) + a.eps);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = v[j] * r * w[j];
-      rotation.template apply<false>(v);
-      const NormSide& s = a.side[which];
-      if (ok && h < end)
-        store_row<T, V>(static_cast<T*>(s.y) + t * s.yts + (h - (which ? hq : 0)) * s.yhs + l * V, v);
+      if (unit.ok && lane.there && h0 + u < unit.end) Row<T, INTERLEAVED>::store(y + (h0 + u) * s.yhs, lane, p, q);
     }
   }
 }
 
-// The gradient: groups of lanes walk over (token, head) rows, the weights' sums stay in registers.
-template <typename T, int D>
-__global__ void __launch_bounds__(kFastThreads) qk_norm_rope_bprop_rows_kernel(NormArgs a, int per) {
-  constexpr int V = RowShape<T, D>::V, LPR = RowShape<T, D>::LPR, kGroups = kFastThreads / LPR;
-  constexpr int kRowsAhead = V > 4 ? 2 : 4;
-  __shared__ float sums[kGroups][2][D];
-  const int l = threadIdx.x % LPR, group = threadIdx.x / LPR, hq = a.side[0].heads, heads = hq + a.side[1].heads;
-  const int parts = (heads + per - 1) / per;
-  const long long units = static_cast<long long>(a.t) * parts;
-  float dw[2][V];
+// The gradient: groups of lanes walk over units, the weights' sums stay in registers.
+template <typename T, int LPR, bool INTERLEAVED>
+__global__ void __launch_bounds__(kFastThreads) qk_norm_rope_bprop_rows_kernel(NormArgs a, int per, long long units) {
+  constexpr int kGroups = kFastThreads / LPR, kRowsAhead = 2;
+  __shared__ float sums[kGroups][2][LPR * 8];
+  const int l = threadIdx.x % LPR, group = threadIdx.x / LPR;
+  const Lane lane = lane_of<INTERLEAVED>(a, l);
+  const float over = 1.0f / static_cast<float>(a.d);
+  float2 dw[2][2][2];  // [side][x or y][pair]
 #pragma unroll
-  for (int j = 0; j < V; ++j) dw[0][j] = dw[1][j] = 0.0f;
+  for (int i = 0; i < 8; ++i) dw[i / 4][i / 2 % 2][i % 2] = both(0.0f);
   for (long long first = static_cast<long long>(blockIdx.x) * kGroups; first < units;
        first += static_cast<long long>(gridDim.x) * kGroups) {
-    const long long unit = first + group;
-    const int t = static_cast<int>(unit / parts);
-    bool ok = unit < units;
-    const int begin = static_cast<int>(unit % parts) * per, end = ok ? min(heads, begin + per) : begin;
-    const float* tab = nullptr;
-    if (ok && a.rot) ok = (tab = table_row(a, t)) != nullptr;
-    Rotation<V> rotation;
-    bool known = false;
-    for (int h0 = begin; __any_sync(~0u, h0 < end); h0 += kRowsAhead) {
-      alignas(16) T raw[kRowsAhead][V], grad[kRowsAhead][V];
+    const Unit unit = unit_of(a, first + group, per);
+    const NormSide& s = a.side[unit.which];
+    const T* x = static_cast<const T*>(s.x) + unit.t * s.ts;
+    const long long flat = static_cast<long long>(unit.t) * s.heads * a.d;
+    const T* dy = static_cast<const T*>(s.dy) + flat;
+    T* dx = static_cast<T*>(s.y) + flat;
+    const bool live = unit.ok && lane.there;
+    Angles angles;
+    float2 w[2], wy[2], add[2][2];
+    add[0][0] = add[0][1] = add[1][0] = add[1][1] = both(0.0f);
+    for (int h0 = unit.begin; __any_sync(~0u, h0 < unit.end); h0 += kRowsAhead) {
+      Row<T, INTERLEAVED> row[kRowsAhead], grad[kRowsAhead];
 #pragma unroll
       for (int u = 0; u < kRowsAhead; ++u) {
-        const int h = h0 + u, which = h >= hq, hh = h - (which ? hq : 0);
-        const NormSide& s = a.side[which];
-        load_row<T, V>(static_cast<const T*>(s.x) + t * s.ts + hh * s.hs + l * V, ok && h < end, raw[u]);
-        load_row<T, V>(static_cast<const T*>(s.dy) + (static_cast<long long>(t) * s.heads + hh) * D + l * V, ok && h < end,
-                       grad[u]);
+        row[u].load(x + (h0 + u) * s.hs, lane, live && h0 + u < unit.end);
+        grad[u].load(dy + (h0 + u) * a.d, lane, live && h0 + u < unit.end);
       }
-      if (!known) rotation.load(a, tab, l);
-      known = true;
+      if (h0 == unit.begin) {
+        angles.load(a, unit.table, lane, l);
+        lane_weights<T, INTERLEAVED>(s.w, lane, w, wy);
+      }
 #pragma unroll
       for (int u = 0; u < kRowsAhead; ++u) {
-        const int h = h0 + u, which = h >= hq, hh = h - (which ? hq : 0);
-        const NormSide& s = a.side[which];
-        float x[V], v[V], w[V], sq = 0.0f, vx = 0.0f;
-        load_weights<T, V>(a, which, l, w);
+        float2 p[2], q[2], dp[2], dq[2];
+        row[u].get(p, q);
+        grad[u].get(dp, dq);
+        const float2 sq = fma2(p[0], p[0], fma2(p[1], p[1], fma2(q[0], q[0], mul2(q[1], q[1]))));
+        float2 vx = both(0.0f), v[2], z[2], np[2], nq[2];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          x[j] = to_f32(raw[u][j]);
-          v[j] = to_f32(grad[u][j]);
-          sq = fmaf(x[j], x[j], sq);
+        for (int i = 0; i < 2; ++i) {
+          const float2 back = make_float2(-angles.s[i].x, -angles.s[i].y);
+          const float2 dn = fma2(dq[i], angles.s[i], mul2(dp[i], angles.c[i]));
+          const float2 dm = fma2(dp[i], back, mul2(dq[i], angles.c[i]));
+          np[i] = mul2(dn, p[i]);
+          nq[i] = mul2(dm, q[i]);
+          v[i] = mul2(dn, w[i]);
+          z[i] = mul2(dm, wy[i]);
+          vx = fma2(v[i], p[i], fma2(z[i], q[i], vx));
         }
-        rotation.template apply<true>(v);
-        const float r = rsqrtf(row_sum<LPR>(sq) * (1.0f / D) + a.eps);
+        const float r = rsqrtf(row_sum<LPR>(sq) * over + a.eps), k = -r * r * (row_sum<LPR>(vx) * over);
+        const float2 rr = both(live && h0 + u < unit.end ? r : 0.0f);  // empty lanes: no 0 times infinity
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float add = ok && h < end ? v[j] * x[j] * r : 0.0f;
-          dw[0][j] += which ? 0.0f : add;
-          dw[1][j] += which ? add : 0.0f;
-          v[j] *= w[j];
-          vx = fmaf(v[j], x[j], vx);
+        for (int i = 0; i < 2; ++i) {
+          add[0][i] = fma2(rr, np[i], add[0][i]);
+          add[1][i] = fma2(rr, nq[i], add[1][i]);
+          p[i] = mul2(rr, fma2(both(k), p[i], v[i]));
+          q[i] = mul2(rr, fma2(both(k), q[i], z[i]));
         }
-        const float k = r * r * (row_sum<LPR>(vx) * (1.0f / D));
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = r * fmaf(-k, x[j], v[j]);
-        if (ok && h < end)
-          store_row<T, V>(static_cast<T*>(s.y) + (static_cast<long long>(t) * s.heads + hh) * D + l * V, v);
+        if (live && h0 + u < unit.end) Row<T, INTERLEAVED>::store(dx + (h0 + u) * a.d, lane, p, q);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = add[i / 2][i % 2];
+      if (unit.which)
+        dw[1][i / 2][i % 2] = add2(dw[1][i / 2][i % 2], v);
+      else
+        dw[0][i / 2][i % 2] = add2(dw[0][i / 2][i % 2], v);
     }
   }
 #pragma unroll
-  for (int which = 0; which < 2; ++which)
-#pragma unroll
-    for (int j = 0; j < V; ++j) sums[group][which][l * V + j] = dw[which][j];
+  for (int which = 0; which < 2; ++which) {
+    float2 f0[2], f1[2];
+    from_pairs<INTERLEAVED>(dw[which][0], dw[which][1], f0, f1);
+    if (lane.there) {
+      *reinterpret_cast<float4*>(&sums[group][which][lane.at[0]]) = make_float4(f0[0].x, f0[0].y, f0[1].x, f0[1].y);
+      *reinterpret_cast<float4*>(&sums[group][which][lane.at[1]]) = make_float4(f1[0].x, f1[0].y, f1[1].x, f1[1].y);
+    }
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * D; i += kFastThreads) {
+  for (int i = threadIdx.x; i < 2 * a.d; i += kFastThreads) {
     float v = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j) v += (&sums[j][0][0])[i];
-    a.partial[static_cast<size_t>(blockIdx.x) * 2 * D + i] = v;
+    for (int j = 0; j < kGroups; ++j) v += sums[j][i / a.d][i % a.d];
+    a.partial[static_cast<size_t>(blockIdx.x) * 2 * a.d + i] = v;
   }
 }
 
@@ -399,11 +465,11 @@ __global__ void norm_weight_grad_kernel(const float* partial, int blocks, int d,
   }
 }
 
-// Whether the rows kernels take the call: d and rot in their shapes, and every row 16-byte aligned.
-bool rows_fit(const NormArgs& a, int size, bool back) {
-  const int v = std::max(16 / size, a.d / 32);
-  if (a.d != 64 && a.d != 128 && a.d != 256) return false;
-  if (a.rot && ((a.rot & (a.rot - 1)) || a.rot < 2 * v || (reinterpret_cast<uintptr_t>(a.table) & 15u))) return false;
+// Lanes of a row, 0 where the rows kernels do not take the call: channels, rotated ones and strides are multiples of
+// what a lane moves at a time.
+int row_lanes(const NormArgs& a, int size, bool back) {
+  const unsigned mask = 4 * size - 1;  // alignment of four channels
+  if (a.d > 256 || a.d % 8 || a.rot % 8 || (a.rot && (reinterpret_cast<uintptr_t>(a.table) & 15u))) return 0;
   for (const NormSide& s : a.side) {
     uintptr_t bits = reinterpret_cast<uintptr_t>(s.x) | reinterpret_cast<uintptr_t>(s.y) | reinterpret_cast<uintptr_t>(s.w);
     long long strides = s.ts | s.hs;
@@ -411,18 +477,26 @@ bool rows_fit(const NormArgs& a, int size, bool back) {
       bits |= reinterpret_cast<uintptr_t>(s.dy);
     else
       strides |= s.yts | s.yhs;
-    if (s.heads && ((bits & 15u) || (strides * size) % 16)) return false;
+    if (s.heads && ((bits & mask) || strides % 4)) return 0;
   }
-  return true;
+  return a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32;
 }
 
-// Heads of a token that one group of lanes takes: many when there are enough rows to fill the GPU with eights (the
-// cosines are read less often), one when there are few (a row's latency is all there is).
+// Heads that one group of lanes takes of a token: many when there are enough rows to fill the GPU with eights (angles
+// and weights are read less often), one when there are few (a row's latency is all there is).
 int heads_per_group(const NormArgs& a, int lanes, int sms) {
   const long long lanes_of_all = static_cast<long long>(a.t) * (a.side[0].heads + a.side[1].heads) * lanes;
   const long long full = 1024ll * sms;
   return lanes_of_all >= 16 * full ? 8 : lanes_of_all >= 4 * full ? 4 : 1;
 }
+
+#define B200Q_NORM_ROWS(kernel, ...)                                                                                \
+  (a.interleaved ? (lanes == 8    ? kernel<T, 8, true>                                                              \
+                    : lanes == 16 ? kernel<T, 16, true>                                                             \
+                                  : kernel<T, 32, true>)                                                            \
+                 : (lanes == 8    ? kernel<T, 8, false>                                                             \
+                    : lanes == 16 ? kernel<T, 16, false>                                                            \
+                                  : kernel<T, 32, false>))<<<static_cast<int>(blocks), kFastThreads, 0, cs>>>(__VA_ARGS__)
 
 // Checks what both directions share and fills in the kernels' arguments.
 int norm_args(const b200q_qk_norm_args* p, NormArgs* a, int* sms) {
@@ -468,13 +542,12 @@ extern "C" int b200q_qk_norm_rope(const b200q_qk_norm_args* args, void* stream) 
   if (t == 0 || hq + hk == 0) return B200Q_OK;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const int size = ftype == B200Q_F32 ? 4 : 2;
-  if (rows_fit(a, size, false)) {
-    const int lanes = d / std::max(16 / size, d / 32), per = heads_per_group(a, lanes, sms);
-    const long long blocks = (static_cast<long long>(t) * ((hq + hk + per - 1) / per) * lanes + kFastThreads - 1) / kFastThreads;
+  if (const int lanes = row_lanes(a, size, false)) {
+    const int per = heads_per_group(a, lanes, sms);
+    const long long units = static_cast<long long>(t) * ((hq + per - 1) / per + (hk + per - 1) / per);
+    const long long blocks = (units * lanes + kFastThreads - 1) / kFastThreads;
     if (blocks > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
-    B200Q_DISPATCH_FTYPE(ftype, (d == 64    ? qk_norm_rope_rows_kernel<T, 64>
-                                 : d == 128 ? qk_norm_rope_rows_kernel<T, 128>
-                                            : qk_norm_rope_rows_kernel<T, 256>)<<<static_cast<int>(blocks), kFastThreads, 0, cs>>>(a, per));
+    B200Q_DISPATCH_FTYPE(ftype, (B200Q_NORM_ROWS(qk_norm_rope_rows_kernel, a, per)));
   } else {
     const long long blocks = (static_cast<long long>(t) * (hq + hk) + kNormWarps - 1) / kNormWarps;
     if (blocks > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
@@ -496,20 +569,18 @@ extern "C" int b200q_qk_norm_rope_bprop(const b200q_qk_norm_args* args, void* st
   if ((rc = host_device(&sms, &a.err))) return rc;  // no tokens still mean weight gradients of zero
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const int size = ftype == B200Q_F32 ? 4 : 2;
-  const bool fast = rows_fit(a, size, true);
-  const int lanes = fast ? d / std::max(16 / size, d / 32) : 32, per = fast ? heads_per_group(a, lanes, sms) : 1;
-  const int threads = fast ? kFastThreads : kNormWarps * 32;
-  const long long want = (static_cast<long long>(t) * ((hq + hk + per - 1) / per) * lanes + threads - 1) / threads;
-  const int blocks = static_cast<int>(std::max(1ll, std::min<long long>(want, sms * (fast ? 8 : 4))));
+  const int lanes = row_lanes(a, size, true), per = lanes ? heads_per_group(a, lanes, sms) : 1;
+  const long long units = static_cast<long long>(t) * ((hq + per - 1) / per + (hk + per - 1) / per);
+  const int units_per_block = lanes ? kFastThreads / lanes : kNormWarps;
+  const int blocks = static_cast<int>(
+      std::max(1ll, std::min<long long>((units + units_per_block - 1) / units_per_block, sms * (lanes ? 8 : 4))));
   void* ws = nullptr;
   if ((rc = host_workspace(static_cast<size_t>(blocks) * 2 * d * sizeof(float), cs, &ws))) return rc;
   a.partial = static_cast<float*>(ws);
   const size_t smem = static_cast<size_t>(kNormWarps) * 2 * d * sizeof(float);
   B200Q_DISPATCH_FTYPE(ftype, {
-    if (fast) {
-      (d == 64    ? qk_norm_rope_bprop_rows_kernel<T, 64>
-       : d == 128 ? qk_norm_rope_bprop_rows_kernel<T, 128>
-                  : qk_norm_rope_bprop_rows_kernel<T, 256>)<<<blocks, kFastThreads, 0, cs>>>(a, per);
+    if (lanes) {
+      B200Q_NORM_ROWS(qk_norm_rope_bprop_rows_kernel, a, per, units);
     } else {
       if (smem > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(qk_norm_rope_bprop_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -37,14 +37,14 @@ class KV4Cache:
             raise TypeError("cache codes must be uint8")
         if k_params.dtype != torch.int32 or v_params.dtype != torch.int32:
             raise TypeError("cache params must be int32")
-        if not (k_codes.is_contiguous() and v_codes.is_contiguous() and k_params.is_contiguous()
-                and v_params.is_contiguous()):
-            raise RuntimeError("cache tensors must be contiguous")
-        if not (k_codes.is_cuda and v_codes.is_cuda and k_params.is_cuda and v_params.is_cuda):
-            raise RuntimeError("tensor arguments must be CUDA device tensors")
+        for x in (k_codes, k_params, v_codes, v_params):
+            if not x.is_contiguous():
+                raise RuntimeError("cache tensors must be contiguous")
+            if not x.is_cuda:
+                raise RuntimeError("tensor arguments must be CUDA device tensors")
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
-        self.pages, self.heads, self.page_size = shape[0], shape[1], shape[2]
-        self.head_dim = 2 * shape[3]
+        self.pages, self.heads, self.page_size, half = shape
+        self.head_dim = 2 * half
         self.group = self.head_dim // pshape[3]
         self._c = _CACHE.pack(k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(),
                               self.pages, self.heads, self.page_size, self.head_dim, self.group)
@@ -65,7 +65,8 @@ class KV4Cache:
 
 
 def _check_slots(slots, t=None):
-    _device_tensor(slots, torch.int64, "slots")
+    if slots.dtype != torch.int64 or not slots.is_cuda:
+        _device_tensor(slots, torch.int64, "slots")
     if slots.dim() != 1 or not slots.is_contiguous() or (t is not None and slots.shape[0] != t):
         raise RuntimeError(f"slots must be contiguous [{'tokens' if t is None else t}]")
 
@@ -73,24 +74,22 @@ def _check_slots(slots, t=None):
 def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, stream=None) -> None:
     """k, v [t, heads, d] (views with contiguous channels will do) into slots int64 [t]; negative slots are
     skipped, and no slot may be named twice."""
-    ft = _ftype(k, "k")
-    _device_tensor(v, k.dtype, "v")
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != cache.heads or k.shape[2] != cache.head_dim:
-        raise RuntimeError(f"k and v must be [tokens, {cache.heads}, {cache.head_dim}], got {list(k.shape)} and "
+    ft = FTYPES.get(k.dtype)
+    if ft is None or not k.is_cuda:
+        _ftype(k, "k")
+    if v.dtype != k.dtype or not v.is_cuda:
+        _device_tensor(v, k.dtype, "v")
+    shape = k.shape
+    if len(shape) != 3 or v.shape != shape or shape[1] != cache.heads or shape[2] != cache.head_dim:
+        raise RuntimeError(f"k and v must be [tokens, {cache.heads}, {cache.head_dim}], got {list(shape)} and "
                            f"{list(v.shape)}")
-    _check_slots(slots, k.shape[0])
-    if k.stride(2) != 1 or v.stride(2) != 1:
+    _check_slots(slots, shape[0])
+    (kt, kh, kc), (vt, vh, vc) = k.stride(), v.stride()
+    if kc != 1 or vc != 1:
         with _on(stream):
-            k, v = k.contiguous(), v.contiguous()
-            _append(cache, k, v, slots, ft, _stream(stream))
-    else:
-        _append(cache, k, v, slots, ft, _stream(stream))
-
-
-def _append(cache, k, v, slots, ft, stream):
-    (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
-    _lib.check(_lib.lib().b200q_kv4_append(cache._c, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh,
-                                           slots.data_ptr(), ft, k.shape[0], stream))
+            return kv4_append(cache, k.contiguous(), v.contiguous(), slots, stream)
+    _lib.check(_lib.lib().b200q_kv4_append(cache._c, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, slots.data_ptr(), ft,
+                                           shape[0], _stream(stream)))
 
 
 def kv4_read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.float32,
@@ -100,12 +99,17 @@ def kv4_read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.fl
     if ft is None:
         raise TypeError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     _check_slots(slots)
-    with _on(stream):
-        shape = (slots.shape[0], cache.heads, cache.head_dim)
-        k = slots.new_empty(shape, dtype=dtype)
-        v = slots.new_empty(shape, dtype=dtype)
-        _lib.check(_lib.lib().b200q_kv4_read(cache._c, slots.data_ptr(), k.data_ptr(), v.data_ptr(), ft,
-                                             shape[0], _stream(stream)))
+    if stream is not None:
+        with _on(stream):
+            return _read(cache, slots, dtype, ft, _stream(stream))
+    return _read(cache, slots, dtype, ft, _stream(None))
+
+
+def _read(cache, slots, dtype, ft, stream):
+    t = slots.shape[0]
+    k = slots.new_empty((t, cache.heads, cache.head_dim), dtype=dtype)
+    v = torch.empty_like(k)
+    _lib.check(_lib.lib().b200q_kv4_read(cache._c, slots.data_ptr(), k.data_ptr(), v.data_ptr(), ft, t, stream))
     return k, v
 
 
@@ -116,35 +120,42 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, l
     the first lens - tq + i + 1 places; where that is none the output is 0 (lse -inf).  Query head h reads cache
     head h // (hq / heads).  scale: 1 / sqrt(d) when None.  Returns out [b, tq, hq, d], and lse fp32 [b, tq, hq]
     (log of the sum of exp(scale * q.k)) when return_lse."""
-    ft = _ftype(q, "q")
-    if q.dim() != 4 or q.shape[3] != cache.head_dim:
-        raise RuntimeError(f"q must be [sequences, tokens, heads, {cache.head_dim}], got {list(q.shape)}")
-    b, tq, hq, d = q.shape
-    _device_tensor(block_table, torch.int32, "block_table")
-    _device_tensor(lens, torch.int32, "lens")
-    if block_table.dim() != 2 or block_table.shape[0] != b or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
-        raise RuntimeError(f"block_table must be [{b}, pages] with contiguous rows, got {list(block_table.shape)}")
+    ft = FTYPES.get(q.dtype)
+    if ft is None or not q.is_cuda:
+        _ftype(q, "q")
+    shape = q.shape
+    if len(shape) != 4 or shape[3] != cache.head_dim:
+        raise RuntimeError(f"q must be [sequences, tokens, heads, {cache.head_dim}], got {list(shape)}")
+    b = shape[0]
+    if block_table.dtype != torch.int32 or not block_table.is_cuda:
+        _device_tensor(block_table, torch.int32, "block_table")
+    if lens.dtype != torch.int32 or not lens.is_cuda:
+        _device_tensor(lens, torch.int32, "lens")
+    table = block_table.shape
+    if len(table) != 2 or table[0] != b or (table[1] > 1 and block_table.stride(1) != 1):
+        raise RuntimeError(f"block_table must be [{b}, pages] with contiguous rows, got {list(table)}")
     if lens.shape != (b,) or not lens.is_contiguous():
         raise RuntimeError(f"lens must be contiguous [{b}]")
-    if stream is None:
-        return _attention(q, cache, block_table, lens, scale, out, return_lse, ft, b, tq, hq, d, _stream(None))
-    with _on(stream):
-        return _attention(q, cache, block_table, lens, scale, out, return_lse, ft, b, tq, hq, d, _stream(stream))
+    if stream is not None:
+        with _on(stream):
+            return _attention(q, cache, block_table, lens, scale, out, return_lse, ft, shape, table[1], _stream(stream))
+    return _attention(q, cache, block_table, lens, scale, out, return_lse, ft, shape, table[1], _stream(None))
 
 
-def _attention(q, cache, block_table, lens, scale, out, return_lse, ft, b, tq, hq, d, stream):
+def _attention(q, cache, block_table, lens, scale, out, return_lse, ft, shape, max_pages, stream):
+    b, tq, hq, d = shape
     qb, qt, qh, qc = q.stride()
     if qc != 1:
         q = q.contiguous()
         qb, qt, qh, _ = q.stride()
     if out is None:
-        out = q.new_empty((b, tq, hq, d))
-    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() or not out.is_cuda:
-        raise RuntimeError(f"out must be a contiguous {q.dtype} {list(q.shape)} CUDA tensor")
-    lse = q.new_empty((b, tq, hq), dtype=torch.float32) if return_lse else None
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+    elif out.dtype != q.dtype or out.shape != shape or not out.is_contiguous() or not out.is_cuda:
+        raise RuntimeError(f"out must be a contiguous {q.dtype} {list(shape)} CUDA tensor")
+    lse = lens.new_empty((b, tq, hq), dtype=torch.float32) if return_lse else None
     _lib.check(_lib.lib().b200q_kv4_attention(cache._c, _ARGS.pack(q.data_ptr(), qb, qt, qh, block_table.data_ptr(),
                                                                    block_table.stride(0), lens.data_ptr(),
                                                                    out.data_ptr(), lse.data_ptr() if return_lse else 0,
-                                                                   ft, b, tq, hq, block_table.shape[1],
+                                                                   ft, b, tq, hq, max_pages,
                                                                    d ** -0.5 if scale is None else scale), stream))
     return (out, lse) if return_lse else out

@@ -10,7 +10,7 @@ import torch
 
 from . import _lib
 from .conv import _stream
-from .w4 import _device_tensor, _ftype, _on
+from .w4 import FTYPES, _device_tensor, _ftype, _on
 
 
 _ARGS = _lib.packer(_lib.CQKNormArgs)
@@ -24,29 +24,35 @@ def rope_table(positions: int, rot: int, base: float = 10000.0, device="cuda") -
 
 
 def _checked(q, k, q_weight, k_weight, table, positions):
-    ft = _ftype(q, "q")
-    _device_tensor(k, q.dtype, "k")
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+    dtype = q.dtype
+    ft = FTYPES.get(dtype)
+    if ft is None or not q.is_cuda:
+        _ftype(q, "q")
+    if k.dtype != dtype or not k.is_cuda:
+        _device_tensor(k, dtype, "k")
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2]:
         raise RuntimeError(f"q and k must be [tokens, heads, channels] of the same tokens and channels, got "
-                           f"{list(q.shape)} and {list(k.shape)}")
-    t, hq, d = q.shape
+                           f"{list(qs)} and {list(ks)}")
+    t, hq, d = qs
     for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None:
-            _device_tensor(w, q.dtype, what)
-            if w.shape != (d,) or not w.is_contiguous():
-                raise RuntimeError(f"{what} must be contiguous [{d}]")
+        if w is not None and (w.dtype != dtype or not w.is_cuda or w.shape != (d,) or not w.is_contiguous()):
+            _device_tensor(w, dtype, what)
+            raise RuntimeError(f"{what} must be contiguous [{d}]")
     rot = rows = 0
     if table is not None:
-        _device_tensor(table, torch.float32, "table")
+        if table.dtype != torch.float32 or not table.is_cuda:
+            _device_tensor(table, torch.float32, "table")
         if table.dim() != 2 or not table.is_contiguous():
             raise RuntimeError("table must be a contiguous [positions, rotated channels] tensor")
         rows, rot = table.shape
         if positions is None:
             raise RuntimeError("a rotation needs positions")
-        _device_tensor(positions, torch.int32, "positions")
+        if positions.dtype != torch.int32 or not positions.is_cuda:
+            _device_tensor(positions, torch.int32, "positions")
         if positions.shape != (t,) or not positions.is_contiguous():
             raise RuntimeError(f"positions must be contiguous [{t}]")
-    return ft, t, hq, k.shape[1], d, rot, rows
+    return ft, t, hq, ks[1], d, rot, rows
 
 
 def _p(t) -> int:
@@ -78,12 +84,12 @@ def _norm(q, k, q_weight, k_weight, table, positions, eps, interleaved, q_out, k
         k = k.contiguous()
         kt, kh, _ = k.stride()
     if q_out is None:
-        q_out = q.new_empty((t, hq, d))
+        q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((t, hq, d))
         ot, oh = hq * d, d
     else:
         ot, oh = _out_strides(q_out, q, "q_out")
     if k_out is None:
-        k_out = k.new_empty((t, hk, d))
+        k_out = torch.empty_like(k) if k.is_contiguous() else k.new_empty((t, hk, d))
         pt, ph = hk * d, d
     else:
         pt, ph = _out_strides(k_out, k, "k_out")

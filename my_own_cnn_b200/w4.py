@@ -106,41 +106,44 @@ def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None, ou
               stream=None) -> torch.Tensor:
     """x [..., k] (fp32, fp16 or bf16; rows may be strided) -> [..., n] of the same type; fp32 sums.
     bias: [n] of x's type."""
-    ft = _ftype(x, "x")
-    n, k = w.n, w.k
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise RuntimeError(f"x has {x.shape[-1] if x.dim() else 0} columns, the weight {k}")
+    ft = FTYPES.get(x.dtype)
+    if ft is None or not x.is_cuda:
+        _ftype(x, "x")
+    n, k, shape = w.n, w.k, x.shape
+    if not shape or shape[-1] != k:
+        raise RuntimeError(f"x has {shape[-1] if shape else 0} columns, the weight {k}")
     if not w.codes.is_cuda:
         raise RuntimeError("tensor arguments must be CUDA device tensors")
     if bias is not None:
         _device_tensor(bias, x.dtype, "bias")
         if bias.shape != (n,) or not bias.is_contiguous():
             raise RuntimeError(f"bias must be contiguous [{n}]")
-    if stream is None:
-        return _linear(x, w, bias, out, ft, n, k, _stream(None))
-    with _on(stream):
-        return _linear(x, w, bias, out, ft, n, k, _stream(stream))
+    if stream is not None:
+        with _on(stream):
+            return _linear(x, w, bias, out, ft, n, k, _stream(stream))
+    return _linear(x, w, bias, out, ft, n, k, _stream(None))
 
 
 def _linear(x, w, bias, out, ft, n, k, stream):
     rows = x if x.dim() == 2 else x.reshape(-1, k)
-    if rows.stride(1) != 1:
+    ldx, step = rows.stride()
+    if step != 1:
         rows = rows.contiguous()
+        ldx = k
     m = rows.shape[0]
+    y, ldy = out, n
     if out is None:
-        y = out = x.new_empty(x.shape[:-1] + (n,))
-        ldy = n
+        out = y = x.new_empty((m, n) if rows is x else x.shape[:-1] + (n,))
     else:
         if out.dtype != x.dtype or out.shape != x.shape[:-1] + (n,):
             raise RuntimeError(f"out must be {x.dtype} {list(x.shape[:-1] + (n,))}")
         if out.dim() == 2 and (out.stride(1) == 1 or n == 1):
-            y, ldy = out, out.stride(0)
-        elif out.is_contiguous():
-            y, ldy = out, n
-        else:
+            ldy = out.stride(0)
+        elif not out.is_contiguous():
             raise RuntimeError("out must be contiguous, or 2-D with contiguous rows")
-    _lib.check(_lib.lib().b200q_linear_w4(_ARGS.pack(rows.data_ptr(), rows.stride(0), w.codes.data_ptr(),
-                                                     w.scales.data_ptr(), 0 if w.zeros is None else w.zeros.data_ptr(),
+    zeros = w.zeros
+    _lib.check(_lib.lib().b200q_linear_w4(_ARGS.pack(rows.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(),
+                                                     0 if zeros is None else zeros.data_ptr(),
                                                      0 if bias is None else bias.data_ptr(), y.data_ptr(), ldy, ft, m,
                                                      n, k, w.group), stream))
     return out
