@@ -254,7 +254,7 @@ typedef struct b200q_kv4_cache {
 int b200q_kv4_append(const b200q_kv4_cache* c, const void* k, long long k_ts, long long k_hs, const void* v,
                      long long v_ts, long long v_hs, const int64_t* slots, int ftype, int t, void* stream);
 
-/* The values held in slots[t], contiguous [t][heads][d], 16-byte aligned; zeros for negative slots. */
+/* The values held in slots[t], contiguous [t][heads][d], 32-byte aligned; zeros for negative slots. */
 int b200q_kv4_read(const b200q_kv4_cache* c, const int64_t* slots, void* k, void* v, int ftype, int t, void* stream);
 
 /* Attention of tq new tokens per sequence over the cache, which already holds them:

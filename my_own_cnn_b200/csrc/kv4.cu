@@ -11,14 +11,14 @@ namespace b200q {
 namespace {
 
 // Row (slot, head) of the cache: offset in units of one token's head.
-__device__ __forceinline__ size_t cache_row(const Cache& c, long long slot, int h) {
-  const long long page = slot / c.page_size;
-  return (static_cast<size_t>(page) * c.heads + h) * c.page_size + static_cast<size_t>(slot - page * c.page_size);
+__device__ __forceinline__ size_t cache_row(const Cache& c, uint32_t slot, int h) {
+  const uint32_t page = c.page.of(slot);
+  return (static_cast<size_t>(page) * c.heads + h) * c.page_size + (slot - page * c.page_size);
 }
 
 __device__ __forceinline__ bool slot_ok(const Cache& c, long long slot, int* err) {
   if (slot < 0) return false;
-  if (slot >= static_cast<long long>(c.pages) * c.page_size) {
+  if (slot >= c.slots) {
     atomicCAS(err, 0, kDevErrBadSlot);
     return false;
   }
@@ -30,7 +30,7 @@ struct AppendArgs {
   long long ts[2], hs[2];
   const int64_t* slots;
   int t;
-  bool vec;  // rows are 16-byte aligned
+  bool vec;  // rows may be moved 8 channels at a time
   int* err;
 };
 
@@ -43,60 +43,83 @@ constexpr int kAhead = 4;
 // Row i of a call: token, keys or values, head.
 struct MoveRow {
   int t, which, h;
-  bool ok;
   long long slot;
 };
-__device__ __forceinline__ MoveRow move_row(const Cache& c, long long i, int t, const int64_t* slots, int* err) {
+__device__ __forceinline__ MoveRow move_row(const Cache& c, uint32_t i, int t, const int64_t* slots) {
   MoveRow r;
-  r.t = static_cast<int>(i / (2 * c.heads));
-  const int rest = static_cast<int>(i - static_cast<long long>(r.t) * 2 * c.heads);
+  r.t = static_cast<int>(c.both_heads.of(i));
+  const int rest = static_cast<int>(i - static_cast<uint32_t>(r.t) * (2 * c.heads));
   r.which = rest >= c.heads;
   r.h = rest - (r.which ? c.heads : 0);
-  r.ok = r.t < t;
-  r.slot = r.ok ? slots[r.t] : -1;
-  if (r.ok) r.ok = slot_ok(c, r.slot, err);
+  r.slot = r.t < t ? __ldg(slots + r.t) : -1;
   return r;
 }
 
-// Eight channels as fp32; `vec`: rows are 16-byte aligned.
+// Eight channels; `vec`: whole rows may be moved 8 channels at a time.
 template <typename T>
-__device__ __forceinline__ void load_eight(const T* p, bool ok, bool vec, T (&v)[8]) {
-  uint4* to = reinterpret_cast<uint4*>(v);
-  if (vec || !ok) {
+__device__ __forceinline__ void load_eight(T (&v)[8], const T* p, bool ok, bool vec) {
+  if (!ok) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
-      to[i] = ok ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
-  } else {
+    for (int j = 0; j < 8; ++j) v[j] = from_f32<T>(0.0f);
+  } else if (!vec) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = p[j];
-  }
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Cache c, AppendArgs a) {
-  constexpr int kLanes = D / 8, kRows = kMoveThreads / kLanes;
-  const int l = threadIdx.x % kLanes;
-  const long long first = static_cast<long long>(blockIdx.x) * (kRows * kAhead) + threadIdx.x / kLanes;
-  MoveRow row[kAhead];
-  alignas(16) T raw[kAhead][8];
+  } else if constexpr (sizeof(T) == 4) {
+    uint32_t bits[8];
+    load_32(bits, p);
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u) {
-    row[u] = move_row(c, first + u * kRows, a.t, a.slots, a.err);
-    const MoveRow& r = row[u];
-    load_eight(static_cast<const T*>(a.x[r.which]) + r.t * a.ts[r.which] + r.h * a.hs[r.which] + l * 8, r.ok, a.vec, raw[u]);
-  }
-  const int per_group = c.group / 8;  // lanes of a group
-#pragma unroll
-  for (int u = 0; u < kAhead; ++u) {
-    const MoveRow& r = row[u];
-    float x[8], lo = 0.0f, hi = 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(bits[j]);
+  } else {
+    const uint4 bits = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      x[j] = to_f32(raw[u][j]);
-      lo = fminf(lo, x[j]);
-      hi = fmaxf(hi, x[j]);
+      const unsigned short half = static_cast<unsigned short>(w[j / 2] >> (16 * (j % 2)));
+      v[j] = *reinterpret_cast<const T*>(&half);
     }
-    for (int o = per_group / 2; o; o >>= 1) {
+  }
+}
+__device__ __forceinline__ void store_eight(float* p, const float (&v)[8]) {
+  uint32_t bits[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) bits[j] = __float_as_uint(v[j]);
+  store_32(p, bits);
+}
+__device__ __forceinline__ void store_eight(__half* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]), pack_f16(v[4], v[5]), pack_f16(v[6], v[7]));
+}
+__device__ __forceinline__ void store_eight(__nv_bfloat16* p, const float (&v)[8]) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
+template <typename T, int D, int G>
+__global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Cache c, AppendArgs a) {
+  constexpr int V = 8, kLanes = D / V, kRows = kMoveThreads / kLanes, kPerGroup = G / V;
+  const int l = threadIdx.x % kLanes;
+  const uint32_t first = blockIdx.x * (kRows * kAhead) + threadIdx.x / kLanes;
+  MoveRow row[kAhead];
+  T raw[kAhead][V];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    row[u] = move_row(c, first + u * kRows, a.t, a.slots);
+    const MoveRow& r = row[u];
+    const T* from = static_cast<const T*>(a.x[r.which]) + r.t * a.ts[r.which] + r.h * a.hs[r.which] + l * V;
+    load_eight(raw[u], from, r.t < a.t, a.vec);
+  }
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    const MoveRow& r = row[u];
+    float x[V], lo = 0.0f, hi = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = to_f32(raw[u][j]);
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      lo = fminf(fminf(x[j], x[j + 1]), lo);
+      hi = fmaxf(fmaxf(x[j], x[j + 1]), hi);
+    }
+#pragma unroll
+    for (int o = kPerGroup / 2; o; o >>= 1) {
       lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
       hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
     }
@@ -107,48 +130,60 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Cache c, Appen
     if (!(s >= 1.17549435e-38f)) s = 0.0f, bits = 0;
     const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
     const float z = fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f);
+    // rint(v) + z in the low bits of 1.5 2^23 + rint(v) + z (the sum rounds half to even, as rint does); v + z >= 0, since
+    // x >= lo and z = rint(-lo / s).  The words add up, the exponents' bits with them.
     uint32_t word = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      word |= static_cast<uint32_t>(fminf(fmaxf(rintf(__fmul_rn(x[j], inv)) + z, 0.0f), 15.0f)) << (4 * j);
-    if (r.ok) {
-      const size_t at = cache_row(c, r.slot, r.h);
-      reinterpret_cast<uint32_t*>(c.codes[r.which])[at * (D / 8) + l] = word;
-      if (l % per_group == 0)
-        c.params[r.which][at * (D / c.group) + l / per_group] = bits | static_cast<uint32_t>(z) << 16;
+    for (int j = 0; j < V; ++j) {
+      const float v = __fadd_rn(__fadd_rn(__fmul_rn(x[j], inv), 12582912.0f), z);
+      word += __float_as_uint(fminf(v, 12582927.0f)) << (4 * j);
+    }
+    word -= 0x4B400000u * 0x11111111u;
+    if (slot_ok(c, r.slot, a.err)) {
+      const size_t at = cache_row(c, static_cast<uint32_t>(r.slot), r.h);
+      reinterpret_cast<uint32_t*>(c.codes[r.which])[at * kLanes + l] = word;
+      if (l % kPerGroup == 0)
+        c.params[r.which][at * (D / G) + l / kPerGroup] = bits | static_cast<uint32_t>(z) << 16;
     }
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int G>
 __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(Cache c, const int64_t* slots, T* k, T* v, int t, int* err) {
-  constexpr int kLanes = D / 8, kRows = kMoveThreads / kLanes;
+  constexpr int V = 8, kLanes = D / V, kRows = kMoveThreads / kLanes, kPerGroup = G / V;
   const int l = threadIdx.x % kLanes;
-  const long long first = static_cast<long long>(blockIdx.x) * (kRows * kAhead) + threadIdx.x / kLanes;
+  const uint32_t first = blockIdx.x * (kRows * kAhead) + threadIdx.x / kLanes;
   MoveRow row[kAhead];
   uint32_t word[kAhead], param[kAhead];
 #pragma unroll
   for (int u = 0; u < kAhead; ++u) {
-    row[u] = move_row(c, first + u * kRows, t, slots, err);
+    row[u] = move_row(c, first + u * kRows, t, slots);
     const MoveRow& r = row[u];
     word[u] = param[u] = 0;  // a scale of zero
-    if (r.ok) {
-      const size_t at = cache_row(c, r.slot, r.h);
-      word[u] = __ldg(reinterpret_cast<const uint32_t*>(c.codes[r.which]) + at * (D / 8) + l);
-      param[u] = __ldg(c.params[r.which] + at * (D / c.group) + l * 8 / c.group);
+    if (slot_ok(c, r.slot, err)) {
+      const size_t at = cache_row(c, static_cast<uint32_t>(r.slot), r.h);
+      word[u] = __ldg(reinterpret_cast<const uint32_t*>(c.codes[r.which]) + at * kLanes + l);
+      param[u] = __ldg(c.params[r.which] + at * (D / G) + l / kPerGroup);
     }
   }
 #pragma unroll
   for (int u = 0; u < kAhead; ++u) {
     const MoveRow& r = row[u];
     if (r.t >= t) continue;
-    const float s = param_scale(param[u]), z = param_zero(param[u]);
-    alignas(16) T out[8];
+    const float s = param_scale(param[u]), zs = -zero_point(param[u]) * s;
+    // 1024 + code and 1024 + 16 code as fp16 pairs of the codes 16 bits apart; code s and z s are exact, and so is their
+    // difference
+    float out[V];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) out[j] = from_f32<T>((static_cast<float>((word[u] >> (4 * j)) & 15u) - z) * s);
-    uint4* to = reinterpret_cast<uint4*>((r.which ? v : k) + (static_cast<long long>(r.t) * c.heads + r.h) * D + l * 8);
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) to[i] = reinterpret_cast<const uint4*>(out)[i];
+    for (int j = 0; j < V / 2; ++j) {
+      const uint32_t bits = and_or(word[u] >> (j / 2 * 8), j % 2 ? 0x00F000F0u : 0x000F000Fu, 0x64006400u);
+      const __half2 h = j % 2 ? __hfma2(*reinterpret_cast<const __half2*>(&bits), __float2half2_rn(0.0625f), __float2half2_rn(-64.0f))
+                              : __hadd2(*reinterpret_cast<const __half2*>(&bits), __float2half2_rn(-1024.0f));
+      const float2 f = fma2(__half22float2(h), both(s), both(zs));
+      out[j] = f.x;
+      out[j + V / 2] = f.y;
+    }
+    store_eight((r.which ? v : k) + (static_cast<long long>(r.t) * c.heads + r.h) * D + l * V, out);
   }
 }
 
@@ -160,19 +195,27 @@ int check_cache(const b200q_kv4_cache* p, Cache* c) {
   if (p->group != 32 && p->group != 64)
     return host_fail(B200Q_ERR_UNSUPPORTED, "4-bit cache groups are 32 or 64 channels, got %d", p->group);
   if (p->page_size > (1 << 20) || p->heads > (1 << 16)) return host_fail(B200Q_ERR_UNSUPPORTED, "cache too large");
+  if (static_cast<long long>(p->pages) * p->page_size > 0x7fffffffll)
+    return host_fail(B200Q_ERR_UNSUPPORTED, "cache of more than 2^31 slots");
   if (p->pages > 0 && (!p->k_codes || !p->k_params || !p->v_codes || !p->v_params))
     return host_fail(B200Q_ERR_INVALID_ARG, "null cache pointer");
   if ((reinterpret_cast<uintptr_t>(p->k_codes) | reinterpret_cast<uintptr_t>(p->v_codes) |
        reinterpret_cast<uintptr_t>(p->k_params) | reinterpret_cast<uintptr_t>(p->v_params)) & 15u)
     return host_fail(B200Q_ERR_INVALID_ARG, "cache tensors must be 16-byte aligned");
-  *c = Cache{{p->k_codes, p->v_codes}, {p->k_params, p->v_params}, p->pages, p->heads, p->page_size, p->d, p->group};
+  *c = Cache{{p->k_codes, p->v_codes}, {p->k_params, p->v_params}, p->pages, p->heads, p->page_size, p->d, p->group,
+             static_cast<int64_t>(p->pages) * p->page_size, Divisor(p->page_size), Divisor(2 * p->heads)};
   return B200Q_OK;
 }
+
+#define B200Q_MOVE(kernel, ...)                                                                                    \
+  (c.group == 32 ? (c.d == 64 ? kernel<T, 64, 32> : c.d == 128 ? kernel<T, 128, 32> : kernel<T, 256, 32>)           \
+                 : (c.d == 64 ? kernel<T, 64, 64> : c.d == 128 ? kernel<T, 128, 64> : kernel<T, 256, 64>))<<<       \
+      blocks, kMoveThreads, 0, static_cast<cudaStream_t>(stream)>>>(__VA_ARGS__)
 
 int move_blocks(const Cache& c, int t, int* blocks) {
   const int rows = kMoveThreads / (c.d / 8) * kAhead;
   const long long n = (2ll * t * c.heads + rows - 1) / rows;
-  if (n > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many tokens");
+  if (n * rows > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many tokens");
   *blocks = static_cast<int>(n);
   return B200Q_OK;
 }
@@ -229,17 +272,14 @@ extern "C" int b200q_kv4_append(const b200q_kv4_cache* cache, const void* k, lon
   if (t == 0) return B200Q_OK;
   if (!k || !v || !slots) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
   const int size = ftype == B200Q_F32 ? 4 : 2;
-  const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 &&
-                   ((k_ts | k_hs | v_ts | v_hs) * size) % 16 == 0;
+  const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & (8 * size - 1)) == 0 &&
+                   (k_ts | k_hs | v_ts | v_hs) % 8 == 0;
   AppendArgs a{{k, v}, {k_ts, v_ts}, {k_hs, v_hs}, slots, t, vec, nullptr};
   int sms = 0;
   if ((rc = host_device(&sms, &a.err))) return rc;
   int blocks = 0;
   if ((rc = move_blocks(c, t, &blocks))) return rc;
-  B200Q_DISPATCH_FTYPE(ftype, (c.d == 64    ? kv4_append_kernel<T, 64>
-                               : c.d == 128 ? kv4_append_kernel<T, 128>
-                                            : kv4_append_kernel<T, 256>)<<<blocks, kMoveThreads, 0,
-                                                                           static_cast<cudaStream_t>(stream)>>>(c, a));
+  B200Q_DISPATCH_FTYPE(ftype, (B200Q_MOVE(kv4_append_kernel, c, a)));
   rc = host_check_launch("kv4_append_kernel launch");
   if (rc == B200Q_OK) host_set_path(19);
   return rc;
@@ -255,15 +295,11 @@ extern "C" int b200q_kv4_read(const b200q_kv4_cache* cache, const int64_t* slots
   if (!k || !v || !slots) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
   int sms = 0, *err = nullptr;
   if ((rc = host_device(&sms, &err))) return rc;
-  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u)
-    return host_fail(B200Q_ERR_INVALID_ARG, "kv4_read outputs must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 31u)
+    return host_fail(B200Q_ERR_INVALID_ARG, "kv4_read outputs must be 32-byte aligned");
   int blocks = 0;
   if ((rc = move_blocks(c, t, &blocks))) return rc;
-  B200Q_DISPATCH_FTYPE(ftype, (c.d == 64    ? kv4_read_kernel<T, 64>
-                               : c.d == 128 ? kv4_read_kernel<T, 128>
-                                            : kv4_read_kernel<T, 256>)<<<blocks, kMoveThreads, 0,
-                                                                         static_cast<cudaStream_t>(stream)>>>(
-                                  c, slots, static_cast<T*>(k), static_cast<T*>(v), t, err));
+  B200Q_DISPATCH_FTYPE(ftype, (B200Q_MOVE(kv4_read_kernel, c, slots, static_cast<T*>(k), static_cast<T*>(v), t, err)));
   rc = host_check_launch("kv4_read_kernel launch");
   if (rc == B200Q_OK) host_set_path(19);
   return rc;
@@ -286,9 +322,6 @@ extern "C" int b200q_kv4_attention(const b200q_kv4_cache* cache, const b200q_kv4
              p->lse, ftype,   b,       tq,      hq,             max_pages,    p->scale};
   int sms = 0;
   if ((rc = host_device(&sms, &a.err))) return rc;
-  a.page_shift = -1;
-  for (int i = 0; i <= 20; ++i)
-    if (c.page_size == 1 << i) a.page_shift = i;
   // 16 rows a pass where a head has more than 8; heads of 256 channels keep to 8, whose sums fill the registers
   const int rows = tq * (hq / c.heads);
   const bool two = rows > 8 && c.d <= 128;

@@ -36,6 +36,8 @@ struct Cache {
   uint8_t* codes[2];
   uint32_t* params[2];
   int pages, heads, page_size, d, group;
+  int64_t slots;
+  Divisor page, both_heads;  // by the page size, by 2 * heads
 };
 
 struct AttnArgs {
@@ -48,7 +50,6 @@ struct AttnArgs {
   float* lse;
   int ftype, b, tq, hq, max_pages;
   float scale;
-  int page_shift;       // log2 of the page size, or -1
   int row_tiles;        // tiles of 8 * NT rows of a cache head
   float* partial;       // [block][2][8 NT][d] sums of a part: of a unit begun by an earlier block, of one begun here
   float* partial_ml;    // [block][2][8 NT][2] maximum and total
@@ -84,7 +85,7 @@ struct AttnShape {
 __device__ __forceinline__ uint32_t token_row(const Cache& c, const AttnArgs& a, const int32_t* pages, int head, int tok,
                                               int until) {
   if (tok >= until) return ~0u;
-  const int at = a.page_shift >= 0 ? tok >> a.page_shift : static_cast<int>(static_cast<unsigned>(tok) / static_cast<unsigned>(c.page_size));
+  const int at = static_cast<int>(c.page.of(static_cast<uint32_t>(tok)));
   const int page = __ldg(pages + at);
   if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.pages)) {
     atomicCAS(a.err, 0, kDevErrBadPage);
@@ -144,11 +145,6 @@ __device__ __forceinline__ void load_tile(const Cache& c, uint32_t stage, uint32
                          reinterpret_cast<const uint8_t*>(c.params[1]) + static_cast<size_t>(row) * kGroups * 4 + b);
     }
   }
-}
-
-// The zero point as a float: bits 16-23 under the exponent of 2^23.
-__device__ __forceinline__ float zero_point(uint32_t p) {
-  return __uint_as_float(__byte_perm(p, 0x4B000000u, 0x7542)) - 8388608.0f;
 }
 
 template <int D, int G, int NT, bool F32>

@@ -42,9 +42,28 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// n / d for 0 <= n < 2^31 by one multiplication: with l = ceil(log2 d), floor(n m / 2^(31 + l)) for m = ceil(2^(31 + l) / d)
+// is off by less than n / (d 2^31) < 1 / d, too little to reach the next whole number.
+struct Divisor {
+  uint32_t d, m;
+  int shift;
+  Divisor() = default;
+  explicit Divisor(uint32_t divisor) : d(divisor), m(0), shift(0) {
+    if (d < 2) return;
+    int l = 0;
+    while ((1u << l) < d && l < 31) ++l;
+    m = static_cast<uint32_t>(((1ull << (31 + l)) + d - 1) / d);
+    shift = l - 1;
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return d < 2 ? n : __umulhi(n, m) >> shift; }
+};
+
 // Scale and zero point of a cache parameter word.
 __device__ __forceinline__ float param_scale(uint32_t p) { return __uint_as_float(p << 16); }
-__device__ __forceinline__ float param_zero(uint32_t p) { return static_cast<float>((p >> 16) & 0xffu); }
+// (bits 16-23 under the exponent of 2^23)
+__device__ __forceinline__ float zero_point(uint32_t p) {
+  return __uint_as_float(__byte_perm(p, 0x4B000000u, 0x7542)) - 8388608.0f;
+}
 
 // C += A B on one warp, m16 n8 k16: fp16 operands, fp32 sums.  Lane (g = lane / 4, t = lane % 4):
 // a0, a2 hold row g (k 2t, 2t+1 and 2t+8, 2t+9), a1, a3 row g + 8; b0, b1 the same k of column g;
@@ -81,6 +100,12 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// (a & mask) | bits
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
+  return r;
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -114,6 +139,19 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return pair_of_bits(r);
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// 32 bytes in one instruction (32-byte aligned): neighbouring lanes then touch whole sectors, where two 16-byte halves
+// would each touch half of every sector.
+__device__ __forceinline__ void load_32(uint32_t (&v)[8], const void* p) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void store_32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 
 // Asynchronous copies of 4, 8 or 16 bytes into shared memory.
 __device__ __forceinline__ uint32_t shared_address(const void* p) {

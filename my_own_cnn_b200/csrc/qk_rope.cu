@@ -296,22 +296,27 @@ __device__ __forceinline__ float row_sum(float2 v) {
   return s;
 }
 
+// A token's units: `per` heads each of the queries, then of the keys.
+struct Split {
+  int per, parts_q;
+  Divisor parts;
+};
+
 // Unit: one side's heads [begin, end) of token t.
 struct Unit {
   int t, which, begin, end;
   const float* table;
   bool ok;
 };
-__device__ __forceinline__ Unit unit_of(const NormArgs& a, long long unit, int per) {
-  const int parts_q = (a.side[0].heads + per - 1) / per, parts = parts_q + (a.side[1].heads + per - 1) / per;
+__device__ __forceinline__ Unit unit_of(const NormArgs& a, uint32_t unit, const Split& split) {
   Unit u;
-  u.t = static_cast<int>(unit / parts);
-  int part = static_cast<int>(unit - static_cast<long long>(u.t) * parts);
-  u.which = part >= parts_q;
-  if (u.which) part -= parts_q;
+  u.t = static_cast<int>(split.parts.of(unit));
+  int part = static_cast<int>(unit - static_cast<uint32_t>(u.t) * split.parts.d);
+  u.which = part >= split.parts_q;
+  if (u.which) part -= split.parts_q;
   u.ok = u.t < a.t;
-  u.begin = part * per;
-  u.end = u.ok ? min(a.side[u.which].heads, u.begin + per) : u.begin;
+  u.begin = part * split.per;
+  u.end = u.ok ? min(a.side[u.which].heads, u.begin + split.per) : u.begin;
   u.table = nullptr;
   if (u.ok && a.rot) u.ok = (u.table = table_row(a, u.t)) != nullptr;
   return u;
@@ -319,28 +324,27 @@ __device__ __forceinline__ Unit unit_of(const NormArgs& a, long long unit, int p
 
 // A group of LPR lanes takes `per` heads of one token's queries or keys.
 template <typename T, int LPR, bool INTERLEAVED>
-__global__ void __launch_bounds__(kFastThreads) qk_norm_rope_rows_kernel(NormArgs a, int per) {
+__global__ void __launch_bounds__(kFastThreads) qk_norm_rope_rows_kernel(NormArgs a, Split split) {
   const int l = threadIdx.x % LPR;
   const Lane lane = lane_of<INTERLEAVED>(a, l);
-  const Unit unit = unit_of(a, static_cast<long long>(blockIdx.x) * (kFastThreads / LPR) + threadIdx.x / LPR, per);
+  const Unit unit = unit_of(a, blockIdx.x * (kFastThreads / LPR) + threadIdx.x / LPR, split);
   const NormSide& s = a.side[unit.which];
   const T* x = static_cast<const T*>(s.x) + unit.t * s.ts;
   T* y = static_cast<T*>(s.y) + unit.t * s.yts;
   const float over = 1.0f / static_cast<float>(a.d);
   Angles angles;
   float2 w[2], wy[2];
-  for (int h0 = unit.begin; __any_sync(~0u, h0 < unit.end); h0 += kAhead) {
-    Row<T, INTERLEAVED> row[kAhead];
+  Row<T, INTERLEAVED> row[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) row[u].load(x + (h0 + u) * s.hs, lane, lane.there && h0 + u < unit.end);
-    if (h0 == unit.begin) {  // behind the first rows
-      angles.load(a, unit.table, lane, l);
-      lane_weights<T, INTERLEAVED>(s.w, lane, w, wy);
-    }
+  for (int u = 0; u < kAhead; ++u) row[u].load(x + (unit.begin + u) * s.hs, lane, lane.there && unit.begin + u < unit.end);
+  angles.load(a, unit.table, lane, l);
+  lane_weights<T, INTERLEAVED>(s.w, lane, w, wy);
+  for (int h0 = unit.begin; __any_sync(~0u, h0 < unit.end); h0 += kAhead) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       float2 p[2], q[2];
       row[u].get(p, q);
+      row[u].load(x + (h0 + u + kAhead) * s.hs, lane, lane.there && h0 + u + kAhead < unit.end);
       const float2 sq = fma2(p[0], p[0], fma2(p[1], p[1], fma2(q[0], q[0], mul2(q[1], q[1]))));
       const float2 r = both(rsqrtf(row_sum<LPR>(sq) * over + a.eps));
 #pragma unroll
@@ -356,7 +360,7 @@ __global__ void __launch_bounds__(kFastThreads) qk_norm_rope_rows_kernel(NormArg
 
 // The gradient: groups of lanes walk over units, the weights' sums stay in registers.
 template <typename T, int LPR, bool INTERLEAVED>
-__global__ void __launch_bounds__(kFastThreads) qk_norm_rope_bprop_rows_kernel(NormArgs a, int per, long long units) {
+__global__ void __launch_bounds__(kFastThreads) qk_norm_rope_bprop_rows_kernel(NormArgs a, Split split, uint32_t units) {
   constexpr int kGroups = kFastThreads / LPR, kRowsAhead = 2;
   __shared__ float sums[kGroups][2][LPR * 8];
   const int l = threadIdx.x % LPR, group = threadIdx.x / LPR;
@@ -365,9 +369,8 @@ __global__ void __launch_bounds__(kFastThreads) qk_norm_rope_bprop_rows_kernel(N
   float2 dw[2][2][2];  // [side][x or y][pair]
 #pragma unroll
   for (int i = 0; i < 8; ++i) dw[i / 4][i / 2 % 2][i % 2] = both(0.0f);
-  for (long long first = static_cast<long long>(blockIdx.x) * kGroups; first < units;
-       first += static_cast<long long>(gridDim.x) * kGroups) {
-    const Unit unit = unit_of(a, first + group, per);
+  for (uint32_t first = blockIdx.x * kGroups; first < units; first += gridDim.x * kGroups) {
+    const Unit unit = unit_of(a, first + group, split);
     const NormSide& s = a.side[unit.which];
     const T* x = static_cast<const T*>(s.x) + unit.t * s.ts;
     const long long flat = static_cast<long long>(unit.t) * s.heads * a.d;
@@ -377,22 +380,22 @@ __global__ void __launch_bounds__(kFastThreads) qk_norm_rope_bprop_rows_kernel(N
     Angles angles;
     float2 w[2], wy[2], add[2][2];
     add[0][0] = add[0][1] = add[1][0] = add[1][1] = both(0.0f);
-    for (int h0 = unit.begin; __any_sync(~0u, h0 < unit.end); h0 += kRowsAhead) {
-      Row<T, INTERLEAVED> row[kRowsAhead], grad[kRowsAhead];
+    Row<T, INTERLEAVED> row[kRowsAhead], grad[kRowsAhead];
+    auto load = [&](int u, int h) {
+      row[u].load(x + h * s.hs, lane, live && h < unit.end);
+      grad[u].load(dy + h * a.d, lane, live && h < unit.end);
+    };
 #pragma unroll
-      for (int u = 0; u < kRowsAhead; ++u) {
-        row[u].load(x + (h0 + u) * s.hs, lane, live && h0 + u < unit.end);
-        grad[u].load(dy + (h0 + u) * a.d, lane, live && h0 + u < unit.end);
-      }
-      if (h0 == unit.begin) {
-        angles.load(a, unit.table, lane, l);
-        lane_weights<T, INTERLEAVED>(s.w, lane, w, wy);
-      }
+    for (int u = 0; u < kRowsAhead; ++u) load(u, unit.begin + u);
+    angles.load(a, unit.table, lane, l);
+    lane_weights<T, INTERLEAVED>(s.w, lane, w, wy);
+    for (int h0 = unit.begin; __any_sync(~0u, h0 < unit.end); h0 += kRowsAhead) {
 #pragma unroll
       for (int u = 0; u < kRowsAhead; ++u) {
         float2 p[2], q[2], dp[2], dq[2];
         row[u].get(p, q);
         grad[u].get(dp, dq);
+        load(u, h0 + u + kRowsAhead);
         const float2 sq = fma2(p[0], p[0], fma2(p[1], p[1], fma2(q[0], q[0], mul2(q[1], q[1]))));
         float2 vx = both(0.0f), v[2], z[2], np[2], nq[2];
 #pragma unroll
@@ -452,7 +455,7 @@ __global__ void norm_weight_grad_kernel(const float* partial, int blocks, int d,
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, i = blockIdx.x * 32 + lane;
   float v = 0.0f;
   if (i < 2 * d) {
-#pragma unroll 4
+#pragma unroll 10
     for (int b = warp; b < blocks; b += 32) v += partial[static_cast<size_t>(b) * 2 * d + i];
   }
   sums[warp][lane] = v;
@@ -482,12 +485,16 @@ int row_lanes(const NormArgs& a, int size, bool back) {
   return a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32;
 }
 
-// Heads that one group of lanes takes of a token: many when there are enough rows to fill the GPU with eights (angles
+// Heads that one group of lanes takes: many when there are enough rows to fill the GPU with eights (angles
 // and weights are read less often), one when there are few (a row's latency is all there is).
-int heads_per_group(const NormArgs& a, int lanes, int sms) {
-  const long long lanes_of_all = static_cast<long long>(a.t) * (a.side[0].heads + a.side[1].heads) * lanes;
-  const long long full = 1024ll * sms;
-  return lanes_of_all >= 16 * full ? 8 : lanes_of_all >= 4 * full ? 4 : 1;
+Split split_heads(const NormArgs& a, int lanes, int sms) {
+  const int hq = a.side[0].heads, hk = a.side[1].heads;
+  const long long lanes_of_all = static_cast<long long>(a.t) * (hq + hk) * lanes, full = 1024ll * sms;
+  Split s;
+  s.per = lanes_of_all >= 16 * full ? 8 : lanes_of_all >= 4 * full ? 4 : 1;
+  s.parts_q = (hq + s.per - 1) / s.per;
+  s.parts = Divisor(s.parts_q + (hk + s.per - 1) / s.per);
+  return s;
 }
 
 #define B200Q_NORM_ROWS(kernel, ...)                                                                                \
@@ -543,11 +550,11 @@ extern "C" int b200q_qk_norm_rope(const b200q_qk_norm_args* args, void* stream) 
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const int size = ftype == B200Q_F32 ? 4 : 2;
   if (const int lanes = row_lanes(a, size, false)) {
-    const int per = heads_per_group(a, lanes, sms);
-    const long long units = static_cast<long long>(t) * ((hq + per - 1) / per + (hk + per - 1) / per);
+    const Split split = split_heads(a, lanes, sms);
+    const long long units = static_cast<long long>(t) * split.parts.d;
     const long long blocks = (units * lanes + kFastThreads - 1) / kFastThreads;
-    if (blocks > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
-    B200Q_DISPATCH_FTYPE(ftype, (B200Q_NORM_ROWS(qk_norm_rope_rows_kernel, a, per)));
+    if (units > 0x7ffffff0ll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
+    B200Q_DISPATCH_FTYPE(ftype, (B200Q_NORM_ROWS(qk_norm_rope_rows_kernel, a, split)));
   } else {
     const long long blocks = (static_cast<long long>(t) * (hq + hk) + kNormWarps - 1) / kNormWarps;
     if (blocks > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
@@ -569,18 +576,20 @@ extern "C" int b200q_qk_norm_rope_bprop(const b200q_qk_norm_args* args, void* st
   if ((rc = host_device(&sms, &a.err))) return rc;  // no tokens still mean weight gradients of zero
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const int size = ftype == B200Q_F32 ? 4 : 2;
-  const int lanes = row_lanes(a, size, true), per = lanes ? heads_per_group(a, lanes, sms) : 1;
-  const long long units = static_cast<long long>(t) * ((hq + per - 1) / per + (hk + per - 1) / per);
+  const int lanes = row_lanes(a, size, true);
+  const Split split = split_heads(a, lanes ? lanes : 32, sms);
+  const long long units = static_cast<long long>(t) * (lanes ? static_cast<int>(split.parts.d) : hq + hk);
+  if (units > 0x7f000000ll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
   const int units_per_block = lanes ? kFastThreads / lanes : kNormWarps;
   const int blocks = static_cast<int>(
-      std::max(1ll, std::min<long long>((units + units_per_block - 1) / units_per_block, sms * (lanes ? 8 : 4))));
+      std::max(1ll, std::min<long long>((units + units_per_block - 1) / units_per_block, sms * 4)));
   void* ws = nullptr;
   if ((rc = host_workspace(static_cast<size_t>(blocks) * 2 * d * sizeof(float), cs, &ws))) return rc;
   a.partial = static_cast<float*>(ws);
   const size_t smem = static_cast<size_t>(kNormWarps) * 2 * d * sizeof(float);
   B200Q_DISPATCH_FTYPE(ftype, {
     if (lanes) {
-      B200Q_NORM_ROWS(qk_norm_rope_bprop_rows_kernel, a, per, units);
+      B200Q_NORM_ROWS(qk_norm_rope_bprop_rows_kernel, a, split, static_cast<uint32_t>(units));
     } else {
       if (smem > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(qk_norm_rope_bprop_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
