@@ -20,6 +20,7 @@ from .f32 import (BlockBiasMode, bmm_bprop, bmm_bprop_dA, bmm_bprop_dB, bmm_fpro
 from .w4 import W4Weight, linear_w4, pack_w4, quantize_w4
 from .rope import qk_norm_rope, qk_norm_rope_bprop, rope_table
 from .kv4 import KV4Cache, kv4_append, kv4_attention, kv4_read
+from .decoder import W4Attention
 from ._lib import B200QError, device_error, last_path, set_path_policy, tc_launch_count
 
 __all__ = [
@@ -31,5 +32,5 @@ __all__ = [
     "BlockBiasMode", "launch_fprop_nhwc", "launch_bprop_nhwc", "launch_grad_nhwc", "launch_block_fprop_nhwc",
     "launch_block_bprop_nhwc", "launch_block_grad_nhwc", "bmm_matmul", "bmm_fprop", "bmm_bprop_dA", "bmm_bprop_dB",
     "bmm_bprop", "W4Weight", "linear_w4", "pack_w4", "quantize_w4", "qk_norm_rope", "qk_norm_rope_bprop", "rope_table",
-    "KV4Cache", "kv4_append", "kv4_attention", "kv4_read", "device_error",
+    "KV4Cache", "kv4_append", "kv4_attention", "kv4_read", "W4Attention", "device_error",
 ]

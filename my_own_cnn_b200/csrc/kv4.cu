@@ -35,10 +35,9 @@ struct AppendArgs {
 };
 
 // Appending and reading move bytes: a row (one token's head, of the keys or the values) lies in D / 8 lanes of 8
-// channels, one word of codes; a lane has kAhead rows on their way at a time, and a block's lanes take rows side by
-// side in memory.
+// channels, one word of codes; a lane has AHEAD rows on their way at a time, and a block's lanes take rows side by side
+// in memory.
 constexpr int kMoveThreads = 128;
-constexpr int kAhead = 4;
 
 // Row i of a call: token, keys or values, head.
 struct MoveRow {
@@ -93,22 +92,22 @@ __device__ __forceinline__ void store_eight(__nv_bfloat16* p, const float (&v)[8
       make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
 }
 
-template <typename T, int D, int G>
+template <typename T, int D, int G, int AHEAD>
 __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Cache c, AppendArgs a) {
   constexpr int V = 8, kLanes = D / V, kRows = kMoveThreads / kLanes, kPerGroup = G / V;
   const int l = threadIdx.x % kLanes;
-  const uint32_t first = blockIdx.x * (kRows * kAhead) + threadIdx.x / kLanes;
-  MoveRow row[kAhead];
-  T raw[kAhead][V];
+  const uint32_t first = blockIdx.x * (kRows * AHEAD) + threadIdx.x / kLanes;
+  MoveRow row[AHEAD];
+  T raw[AHEAD][V];
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u) {
+  for (int u = 0; u < AHEAD; ++u) {
     row[u] = move_row(c, first + u * kRows, a.t, a.slots);
     const MoveRow& r = row[u];
     const T* from = static_cast<const T*>(a.x[r.which]) + r.t * a.ts[r.which] + r.h * a.hs[r.which] + l * V;
     load_eight(raw[u], from, r.t < a.t, a.vec);
   }
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u) {
+  for (int u = 0; u < AHEAD; ++u) {
     const MoveRow& r = row[u];
     float x[V], lo = 0.0f, hi = 0.0f;
 #pragma unroll
@@ -148,15 +147,15 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Cache c, Appen
   }
 }
 
-template <typename T, int D, int G>
+template <typename T, int D, int G, int AHEAD>
 __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(Cache c, const int64_t* slots, T* k, T* v, int t, int* err) {
   constexpr int V = 8, kLanes = D / V, kRows = kMoveThreads / kLanes, kPerGroup = G / V;
   const int l = threadIdx.x % kLanes;
-  const uint32_t first = blockIdx.x * (kRows * kAhead) + threadIdx.x / kLanes;
-  MoveRow row[kAhead];
-  uint32_t word[kAhead], param[kAhead];
+  const uint32_t first = blockIdx.x * (kRows * AHEAD) + threadIdx.x / kLanes;
+  MoveRow row[AHEAD];
+  uint32_t word[AHEAD], param[AHEAD];
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u) {
+  for (int u = 0; u < AHEAD; ++u) {
     row[u] = move_row(c, first + u * kRows, t, slots);
     const MoveRow& r = row[u];
     word[u] = param[u] = 0;  // a scale of zero
@@ -167,7 +166,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(Cache c, const i
     }
   }
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u) {
+  for (int u = 0; u < AHEAD; ++u) {
     const MoveRow& r = row[u];
     if (r.t >= t) continue;
     const float s = param_scale(param[u]), zs = -zero_point(param[u]) * s;
@@ -207,15 +206,21 @@ int check_cache(const b200q_kv4_cache* p, Cache* c) {
   return B200Q_OK;
 }
 
-#define B200Q_MOVE(kernel, ...)                                                                                    \
-  (c.group == 32 ? (c.d == 64 ? kernel<T, 64, 32> : c.d == 128 ? kernel<T, 128, 32> : kernel<T, 256, 32>)           \
-                 : (c.d == 64 ? kernel<T, 64, 64> : c.d == 128 ? kernel<T, 128, 64> : kernel<T, 256, 64>))<<<       \
+#define B200Q_MOVE_D(kernel, G, A) (c.d == 64 ? kernel<T, 64, G, A> : c.d == 128 ? kernel<T, 128, G, A> : kernel<T, 256, G, A>)
+#define B200Q_MOVE(kernel, ...)                                                                      \
+  (ahead == 1 ? c.group == 32 ? B200Q_MOVE_D(kernel, 32, 1) : B200Q_MOVE_D(kernel, 64, 1)            \
+              : c.group == 32 ? B200Q_MOVE_D(kernel, 32, 4) : B200Q_MOVE_D(kernel, 64, 4))<<<        \
       blocks, kMoveThreads, 0, static_cast<cudaStream_t>(stream)>>>(__VA_ARGS__)
 
-int move_blocks(const Cache& c, int t, int* blocks) {
-  const int rows = kMoveThreads / (c.d / 8) * kAhead;
-  const long long n = (2ll * t * c.heads + rows - 1) / rows;
-  if (n * rows > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many tokens");
+// Rows that a lane has on their way: four when there are rows for many blocks (append and read of 8191 tokens x 4 heads x
+// 256 fp32: 42 us, 46 with two; 2048 x 8 x 128 bf16: 13.0, 18.6 with one), one when a call is all latency (64 x 8 x 128:
+// 4.2 us, 6.2 with four).  Up to kMoveSmall blocks an SM of one row per lane count as such (4 to 16 time alike).
+constexpr int kMoveSmall = 8;
+int move_blocks(const Cache& c, int t, int sms, int* ahead, int* blocks) {
+  const long long rows = 2ll * t * c.heads, per = kMoveThreads / (c.d / 8);
+  *ahead = (rows + per - 1) / per <= static_cast<long long>(kMoveSmall) * sms ? 1 : 4;
+  const long long n = (rows + per * *ahead - 1) / (per * *ahead);
+  if (n * per * *ahead > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many tokens");
   *blocks = static_cast<int>(n);
   return B200Q_OK;
 }
@@ -277,8 +282,8 @@ extern "C" int b200q_kv4_append(const b200q_kv4_cache* cache, const void* k, lon
   AppendArgs a{{k, v}, {k_ts, v_ts}, {k_hs, v_hs}, slots, t, vec, nullptr};
   int sms = 0;
   if ((rc = host_device(&sms, &a.err))) return rc;
-  int blocks = 0;
-  if ((rc = move_blocks(c, t, &blocks))) return rc;
+  int ahead = 0, blocks = 0;
+  if ((rc = move_blocks(c, t, sms, &ahead, &blocks))) return rc;
   B200Q_DISPATCH_FTYPE(ftype, (B200Q_MOVE(kv4_append_kernel, c, a)));
   rc = host_check_launch("kv4_append_kernel launch");
   if (rc == B200Q_OK) host_set_path(19);
@@ -297,8 +302,8 @@ extern "C" int b200q_kv4_read(const b200q_kv4_cache* cache, const int64_t* slots
   if ((rc = host_device(&sms, &err))) return rc;
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 31u)
     return host_fail(B200Q_ERR_INVALID_ARG, "kv4_read outputs must be 32-byte aligned");
-  int blocks = 0;
-  if ((rc = move_blocks(c, t, &blocks))) return rc;
+  int ahead = 0, blocks = 0;
+  if ((rc = move_blocks(c, t, sms, &ahead, &blocks))) return rc;
   B200Q_DISPATCH_FTYPE(ftype, (B200Q_MOVE(kv4_read_kernel, c, slots, static_cast<T*>(k), static_cast<T*>(v), t, err)));
   rc = host_check_launch("kv4_read_kernel launch");
   if (rc == B200Q_OK) host_set_path(19);
