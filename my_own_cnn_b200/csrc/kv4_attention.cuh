@@ -147,6 +147,33 @@ __device__ __forceinline__ void load_tile(const Cache& c, uint32_t stage, uint32
   }
 }
 
+// The same where a tile's tokens lie in one page (pages of a multiple of kTile tokens): `row` is that of the tile's first
+// token in every lane, and what is copied is contiguous.  n: tokens to copy.
+template <int D, int G>
+__device__ __forceinline__ void load_tile_page(const Cache& c, uint32_t stage, uint32_t row, int n, int lane) {
+  constexpr int kChunks = D / 32, kPitch = D / 2 + 16, kCodes = kTile * kPitch, kGroups = D / G, kRows = 32 / kChunks;
+  const size_t from = static_cast<size_t>(row) * (D / 2) + lane * 16;
+  const uint8_t* k = c.codes[0] + from;
+  const uint8_t* v = c.codes[1] + from;
+  const uint32_t to = stage + lane / kChunks * kPitch + lane % kChunks * 16;
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j)
+    if (n >= kTile || j * kRows + lane / kChunks < n) {
+      copy_async<16>(to + j * kRows * kPitch, k + j * 512);
+      copy_async<16>(to + j * kRows * kPitch + kCodes, v + j * 512);
+    }
+  if (lane < n) {
+    constexpr int kBytes = kGroups * 4 < 16 ? kGroups * 4 : 16;
+    const size_t param = (static_cast<size_t>(row) + lane) * (kGroups * 4);
+    const uint32_t at = stage + 2 * kCodes + lane * kGroups * 4;
+#pragma unroll
+    for (int b = 0; b < kGroups * 4; b += kBytes) {
+      copy_async<kBytes>(at + b, reinterpret_cast<const uint8_t*>(c.params[0]) + param + b);
+      copy_async<kBytes>(at + kTile * kGroups * 4 + b, reinterpret_cast<const uint8_t*>(c.params[1]) + param + b);
+    }
+  }
+}
+
 template <int D, int G, int NT, bool F32>
 __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_attention_kernel(Cache c, AttnArgs a) {
   using Shape = AttnShape<D, G, NT, F32>;
@@ -210,14 +237,25 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
   const uint32_t ring = shared_address(smem) + warp * (kStages * Shape::kStage);
   const int tiles = max(0, (until - begin + kTile - 1) / kTile);
   const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
-  const int first = begin + warp * kTile + lane;  // this lane's token of the warp's tile i: first + i * step
+  // this lane's token of the warp's tile i, or the tile's first where its tokens lie in one page: first + i * step
+  const bool paged = c.page_size % kTile == 0;
+  const int first = begin + warp * kTile + (paged ? 0 : lane);
   constexpr int kStep = kWarps * kTile;
   uint32_t held[kStages];  // which tokens of the tiles on their way are there
   uint32_t row = token_row(c, a, pages, head, first, until);
+  auto load = [&](int i, uint32_t stage, bool ok) {  // tile i, whose row was looked up; the tokens that are there
+    if (paged) {
+      const int n = row == ~0u ? 0 : min(kTile, until - first - i * kStep);
+      if (ok) load_tile_page<D, G>(c, stage, row, n, lane);
+      return n >= kTile ? ~0u : (1u << max(0, n)) - 1;
+    }
+    const uint32_t there = __ballot_sync(~0u, row != ~0u);
+    if (ok) load_tile<D, G>(c, stage, row, lane);
+    return there;
+  };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
-    held[i] = __ballot_sync(~0u, row != ~0u);
-    if (i < mine) load_tile<D, G>(c, ring + i * Shape::kStage, row, lane);
+    held[i] = load(i, ring + i * Shape::kStage, i < mine);
     copy_commit();
     row = token_row(c, a, pages, head, first + (i + 1) * kStep, until);
   }
@@ -294,8 +332,7 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
   for (int it = 0; it < mine; ++it) {
     copy_wait<kStages - 2>();
     __syncwarp();
-    held[kStages - 1] = __ballot_sync(~0u, row != ~0u);
-    if (it + kStages - 1 < mine) load_tile<D, G>(c, ring + fill * Shape::kStage, row, lane);
+    held[kStages - 1] = load(it + kStages - 1, ring + fill * Shape::kStage, it + kStages - 1 < mine);
     copy_commit();
     row = token_row(c, a, pages, head, first + (it + kStages) * kStep, until);
     const uint8_t* stage = smem + warp * (kStages * Shape::kStage) + slot * Shape::kStage;

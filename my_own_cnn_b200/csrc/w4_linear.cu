@@ -12,11 +12,14 @@
 //   maximum in [2^14, 2^15), so that it fits fp16 whatever its type; fp32 becomes two fp16 terms (22 bits).
 //   The zero points' sum is kept apart, one row per lane.
 //
-// A block owns kRowsW rows and one slice of K in steps of kStep columns; the blocks of a cluster have the same rows and
-// the other slices, and add their sums up through each other's shared memory in a fixed order.  Each warp streams its
-// 32 rows through a ring of its own (16-byte asynchronous copies).  x is shared: while a step is computed the next
-// one's x is written to the other of two buffers, in the order of operand B, from registers that it was read into a step
-// before.
+// Each warp streams 32 rows through a ring of its own (16-byte asynchronous copies) in steps of kStep columns.  x is
+// shared by the block's warps, in the order of operand B; the blocks of a cluster have the same rows and other slices
+// of K, and add their sums up through each other's shared memory in a fixed order.
+//   Several rows of x: a block owns 8 x 32 weight rows, so that x is brought in once per 32 KB of codes; while a
+//   step is computed the next one's x is written to the other of two buffers, from registers that it was read into a
+//   step before.
+//   One row (and up to kFewRows, where there are few weight rows): a block owns 32 weight rows and its warps share out K: x is small enough to lie in shared memory whole, no
+//   barrier is met between the first step and the last, and a cluster is needed only for few weight rows.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -43,22 +46,26 @@ struct W4Args {
 };
 
 constexpr int kWarps = 8;
-constexpr int kRowsW = 32 * kWarps;  // weight rows of a block
+constexpr int kFewRows = 4;
 constexpr int kStep = 256;           // columns of a step: 128 bytes of codes per row
-constexpr int kStages = 3;
 constexpr int kStage = 32 * (kStep / 2);
-constexpr int kRing = kWarps * kStages * kStage;
 constexpr int kMaxSplit = 8;
 
-// Shared memory: the rings (over them at the end the sums [8 NT][kRowsW]), then two buffers of x.
-template <typename T, int G, int NT>
+// FEW: 0, or how many rows of x at most a block has that keeps all of them in shared memory.
+// Shared memory: the rings (over them at the end the sums), then x: two steps of it, or (FEW) every step of the block's
+// slice.  A step of x: operand B [block of 32 columns][term][row][t] 16 bytes, sums [group][row], powers [row].
+template <typename T, int G, int NT, int FEW>
 struct Layout {
   static constexpr int kTerms = std::is_same<T, float>::value ? 2 : 1;
-  static constexpr int kX = kStep * 2 * kTerms * 8 * NT;    // [block of 32][term][row][t] 16 bytes
-  static constexpr int kXSum = (kStep / G) * 8 * NT * 4;    // [group][row] sums of x
-  static constexpr int kXPower = 8 * NT * 4;                // [row] what a sum of products is multiplied by
-  static constexpr int kBuffer = kX + kXSum + kXPower;
-  static constexpr int kBytes = kRing + 2 * kBuffer;
+  static constexpr int kRowsX = FEW ? FEW : 8 * NT;    // rows of x that there is room for
+  static constexpr int kStages = FEW ? 2 : 3;
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kRowsW = FEW ? 32 : 32 * kWarps;     // weight rows of a block
+  static constexpr int kX = kStep * 2 * kTerms * kRowsX;
+  static constexpr int kXSum = (kStep / G) * kRowsX * 4;
+  static constexpr int kBuffer = (kX + kXSum + kRowsX * 4 + 15) / 16 * 16;
+  static constexpr int kBuffers = FEW ? (46 * 1024) / kBuffer : 2;
+  static constexpr int kBytes = kRing + kBuffers * kBuffer;
 };
 
 // Where 16-byte piece `piece` of row `row` of a step lies: lanes (g, t) that read pieces of 4, 8 or 16 bytes at
@@ -79,100 +86,92 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// A step's x on its way: warp w has rows w and w + 8, lane l columns 8 l to 8 l + 7 of the step.
-template <typename T, int NT>
-struct XRows {
-  alignas(16) T v[NT][8];
+// One row's columns of a step on their way: lane l has columns 8 l to 8 l + 7.
+template <typename T>
+struct XRow {
+  alignas(16) T v[8];
 
-  __device__ __forceinline__ void load(const W4Args& a, int m0, int rows, int k0) {
-    const int warp = threadIdx.x / 32, k = k0 + threadIdx.x % 32 * 8;
+  __device__ __forceinline__ void load(const W4Args& a, int m, int k0) {
+    const int k = k0 + threadIdx.x % 32 * 8;
+    const T* from = static_cast<const T*>(a.x) + m * a.ldx + k;
+    if (a.x_vec && k + 8 <= a.k) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int m = i * kWarps + warp;
-      if (m < rows) {
-        const T* from = static_cast<const T*>(a.x) + (m0 + m) * a.ldx + k;
-        if (a.x_vec && k + 8 <= a.k) {
+      for (int b = 0; b < static_cast<int>(sizeof(T)) / 2; ++b)
+        reinterpret_cast<uint4*>(v)[b] = __ldg(reinterpret_cast<const uint4*>(from) + b);
+    } else {
 #pragma unroll
-          for (int b = 0; b < static_cast<int>(sizeof(T)) / 2; ++b)
-            reinterpret_cast<uint4*>(v[i])[b] = __ldg(reinterpret_cast<const uint4*>(from) + b);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] = k + j < a.k ? from[j] : from_f32<T>(0.0f);
-        }
-      }
+      for (int j = 0; j < 8; ++j) v[j] = k + j < a.k ? from[j] : from_f32<T>(0.0f);
     }
   }
 
-  template <int G>
-  __device__ __forceinline__ void store(uint8_t* buffer, int rows) const {
-    using L = Layout<T, G, NT>;
+  // Into row m of a step's buffer; the whole warp takes part.
+  template <int G, typename L>
+  __device__ __forceinline__ void store(uint8_t* buffer, int m) const {
     constexpr int kWords = G / 32;
     uint4* const xs = reinterpret_cast<uint4*>(buffer);
     float* const xsum = reinterpret_cast<float*>(buffer + L::kX);
     float* const xpower = reinterpret_cast<float*>(buffer + L::kX + L::kXSum);
-    const int warp = threadIdx.x / 32, q = threadIdx.x % 32;
+    const int q = threadIdx.x % 32;
     // thread t of a quad owns G / 4 columns of a group, kWords words of 8
     const int group = q / (G / 8), t = q % (G / 8) / kWords, block = group * kWords + q % kWords;
+    float2 f[4];  // pairs (j, j + 4)
+    float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const int m = i * kWarps + warp;
-      if (m < rows) {
-        float2 f[4];  // pairs (j, j + 4)
-        float top = 0.0f;
+    for (int j = 0; j < 4; ++j) {
+      f[j] = make_float2(to_f32(v[j]), to_f32(v[j + 4]));
+      top = fmaxf(fmaxf(fabsf(f[j].x), fabsf(f[j].y)), top);
+    }
+    const float2 half = add2(add2(f[0], f[1]), add2(f[2], f[3]));
+    float sum = half.x + half.y;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f[j] = make_float2(to_f32(v[i][j]), to_f32(v[i][j + 4]));
-          top = fmaxf(fmaxf(fabsf(f[j].x), fabsf(f[j].y)), top);
+    for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (q % (G / 8) == 0) xsum[group * L::kRowsX + m] = sum;
+    const Power p = power_for(warp_max(top));
+    if (q == 0) xpower[m] = p.down;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = mul2(f[j], both(p.up));
+#pragma unroll
+    for (int term = 0; term < L::kTerms; ++term) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = pack_f16(f[j].x, f[j].y);
+        __half2& h = *reinterpret_cast<__half2*>(&w[j]);
+        if (term + 1 < L::kTerms) {
+          const float2 back = __half22float2(h);
+          f[j] = make_float2(f[j].x - back.x, f[j].y - back.y);
         }
-        const float2 half = add2(add2(f[0], f[1]), add2(f[2], f[3]));
-        float sum = half.x + half.y;
-#pragma unroll
-        for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        if (q % (G / 8) == 0) xsum[group * (8 * NT) + m] = sum;
-        const Power p = power_for(warp_max(top));
-        if (q == 0) xpower[m] = p.down;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = mul2(f[j], both(p.up));
-#pragma unroll
-        for (int term = 0; term < L::kTerms; ++term) {
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            w[j] = pack_f16(f[j].x, f[j].y);
-            __half2& h = *reinterpret_cast<__half2*>(&w[j]);
-            if (term + 1 < L::kTerms) {
-              const float2 back = __half22float2(h);
-              f[j] = make_float2(f[j].x - back.x, f[j].y - back.y);
-            }
-            if (j % 2) h = __hmul2(h, __float2half2_rn(0.0625f));
-          }
-          xs[((block * L::kTerms + term) * (8 * NT) + m) * 4 + t] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        if (j % 2) h = __hmul2(h, __float2half2_rn(0.0625f));
       }
+      xs[((block * L::kTerms + term) * L::kRowsX + m) * 4 + t] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 };
 
-template <typename T, int G, int NT>
+template <typename T, int G, int NT, int FEW>
 __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
-  using L = Layout<T, G, NT>;
-  constexpr int kTerms = L::kTerms, kWords = G / 32, kGroups = kStep / G;
+  using L = Layout<T, G, NT, FEW>;
+  constexpr int kTerms = L::kTerms, kWords = G / 32, kGroups = kStep / G, kStages = L::kStages, kRowsW = L::kRowsW;
+  constexpr int kRowsX = L::kRowsX;
   extern __shared__ __align__(128) uint8_t smem[];
-  float* const sums = reinterpret_cast<float*>(smem);  // [8 NT][kRowsW]
+  uint8_t* const buffers = smem + L::kRing;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const int splits = max(1, (a.steps + a.slice - 1) / a.slice);  // the cluster
   const int rank = blockIdx.x % splits, n0 = blockIdx.x / splits * kRowsW;
-  const int m0 = blockIdx.y * 8 * NT, rows = min(8 * NT, a.m - m0);
-  const int step0 = rank * a.slice, steps = min(a.slice, a.steps - step0);
+  const int m0 = blockIdx.y * kRowsX, rows = min(kRowsX, a.m - m0);
+  // the block's steps are step0 to step0 + count; the warp's are its first, its first + stride, ...
+  const int step0 = rank * a.slice, count = min(a.slice, a.steps - step0);
+  constexpr int kStride = FEW ? kWarps : 1;
+  const int first = step0 + (FEW ? warp : 0), steps = FEW ? (count - warp + kWarps - 1) / kWarps : count;
 
   // copies: lane l brings piece l % 8 of rows l / 8, l / 8 + 4, ...
   const long long pitch = static_cast<long long>((a.k + 31) / 32) * 16;
-  const int row0 = n0 + warp * 32, here = min(32, a.n - row0) - lane / 8;  // rows past the last are left out
+  const int row0 = n0 + (FEW ? 0 : warp * 32), here = min(32, a.n - row0) - lane / 8;  // rows past the last are left out
   const uint32_t ring = shared_address(smem) + warp * (kStages * kStage);
-  const long long piece0 = static_cast<long long>(step0) * (kStep / 2) + lane % 8 * 16;
+  const long long piece0 = static_cast<long long>(first) * (kStep / 2) + lane % 8 * 16;
   const uint8_t* const codes = a.codes + (row0 + lane / 8) * pitch + piece0;
   auto load_step = [&](int s, int slot) {
-    const int at = s * (kStep / 2);
+    const int at = s * kStride * (kStep / 2);
     if (piece0 + at < pitch) {
       const uint8_t* from = codes + at;
       const uint32_t to = ring + slot * kStage;
@@ -187,51 +186,73 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
   const int my_row = min(row0 + lane, a.n - 1), groups = (a.k + G - 1) / G;
   uint32_t scale[kGroups], zero[kGroups], next_scale[kGroups], next_zero[kGroups];
   auto load_params = [&](int s) {
-    const int first = (step0 + s) * kGroups;
-    const long long at = static_cast<long long>(first) * a.n + my_row;
+    const int group0 = (first + s * kStride) * kGroups;
+    const long long at = static_cast<long long>(group0) * a.n + my_row;
     const uint16_t* sp = a.scales + at;
     const uint8_t* zp = a.zeros + at;
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       next_scale[i] = __ldg(sp);
       next_zero[i] = a.zeros ? __ldg(zp) : 8u;
-      if (first + i + 1 < groups) sp += a.n, zp += a.n;
+      if (group0 + i + 1 < groups) sp += a.n, zp += a.n;
     }
   };
 
   // sums of products, [16 rows][8 columns][row g or g + 8] for columns 2t, 2t + 1; of lane l's row, sums of zero points
-  float2 acc[2][NT][2], less[4 * NT];
+  constexpr int kLess = (kRowsX + 1) / 2;
+  float2 acc[2][NT][2], less[kLess];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    acc[0][n][0] = acc[0][n][1] = acc[1][n][0] = acc[1][n][1] = both(0.0f);
+  for (int n = 0; n < NT; ++n) acc[0][n][0] = acc[0][n][1] = acc[1][n][0] = acc[1][n][1] = both(0.0f);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) less[n * 4 + e] = both(0.0f);
-  }
-  // columns that no row of x has stay zero in both buffers
-  for (int i = threadIdx.x; i < 2 * L::kX / 16; i += kWarps * 32) {
-    const int at = i % (L::kX / 16);
-    if (at / 4 % (8 * NT) >= rows)
-      *reinterpret_cast<uint4*>(smem + kRing + i / (L::kX / 16) * L::kBuffer + at * 16) = make_uint4(0, 0, 0, 0);
-  }
-  XRows<T, NT> x;
-  if (steps > 0) {
-    x.load(a, m0, rows, step0 * kStep);
-    load_params(0);
-  }
+  for (int m = 0; m < kLess; ++m) less[m] = both(0.0f);
+  if (steps > 0) load_params(0);
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) {
     if (s < steps) load_step(s, s);
     copy_commit();
   }
-  if (steps > 0) x.template store<G>(smem + kRing, rows);
-  if (steps > 1) x.load(a, m0, rows, (step0 + 1) * kStep);
+  constexpr int kRowsWarp = FEW ? 4 : NT;  // rows of a step that a warp has on their way at a time
+  XRow<T> x[kRowsWarp];
+  auto load_x = [&](int step) {  // rows w, w + 8 of one step
+#pragma unroll
+    for (int i = 0; i < kRowsWarp; ++i)
+      if (i * kWarps + warp < rows) x[i].load(a, m0 + i * kWarps + warp, (step0 + step) * kStep);
+  };
+  auto store_x = [&](int buffer) {
+#pragma unroll
+    for (int i = 0; i < kRowsWarp; ++i)
+      if (i * kWarps + warp < rows) x[i].template store<G, L>(buffers + buffer * L::kBuffer, i * kWarps + warp);
+  };
+  if constexpr (FEW) {  // every row of every step, dealt out to the warps
+    for (int p0 = warp; p0 < rows * count; p0 += kWarps * kRowsWarp) {
+#pragma unroll
+      for (int i = 0; i < kRowsWarp; ++i) {
+        const int p = p0 + i * kWarps;
+        if (p < rows * count) x[i].load(a, m0 + p % rows, (step0 + p / rows) * kStep);
+      }
+#pragma unroll
+      for (int i = 0; i < kRowsWarp; ++i) {
+        const int p = p0 + i * kWarps;
+        if (p < rows * count) x[i].template store<G, L>(buffers + p / rows * L::kBuffer, p % rows);
+      }
+    }
+  } else {
+    if (steps > 0) {
+      load_x(0);
+      store_x(0);
+    }
+    if (steps > 1) load_x(1);
+  }
   __syncthreads();
+  const int column = min(g, rows - 1);  // columns that no row of x has repeat one that has, and are not used
 
   int slot = 0, fill = kStages - 1;
   for (int s = 0; s < steps; ++s) {
-    const uint8_t* const buffer = smem + kRing + (s & 1) * L::kBuffer;
-    if (s + 1 < steps) x.template store<G>(smem + kRing + (~s & 1) * L::kBuffer, rows);
-    if (s + 2 < steps) x.load(a, m0, rows, (step0 + s + 2) * kStep);
+    const uint8_t* const buffer = buffers + (FEW ? warp + s * kWarps : s & 1) * L::kBuffer;
+    if constexpr (!FEW) {
+      if (s + 1 < steps) store_x(~s & 1);
+      if (s + 2 < steps) load_x(s + 2);
+    }
     copy_wait<kStages - 2>();
     __syncwarp();
     if (s + kStages - 1 < steps) load_step(s + kStages - 1, fill);
@@ -269,7 +290,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
         for (int term = 0; term < kTerms; ++term)
 #pragma unroll
           for (int n = 0; n < NT; ++n)
-            b[term][n] = xs[(((i * kWords + word) * kTerms + term) * (8 * NT) + n * 8 + g) * 4 + t];
+            b[term][n] = xs[(((i * kWords + word) * kTerms + term) * kRowsX + (FEW ? column : n * 8 + g)) * 4 + t];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
           const uint32_t w0 = w[2 * mt][word], w1 = w[2 * mt + 1][word], v0 = w0 >> 8, v1 = w1 >> 8;
@@ -300,16 +321,21 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
       }
       const float2 sz = both(__uint_as_float(scale[i]) * static_cast<float>(zero[i]));
 #pragma unroll
-      for (int m = 0; m < 8 * NT; m += 4)
+      for (int m = 0; m < kRowsX; m += 4)
         if (m < rows) {
-          const float4 v = *reinterpret_cast<const float4*>(xsum + i * (8 * NT) + m);
-          less[m / 2] = fma2(sz, make_float2(v.x, v.y), less[m / 2]);
-          less[m / 2 + 1] = fma2(sz, make_float2(v.z, v.w), less[m / 2 + 1]);
+          const float* at = xsum + i * kRowsX + m;
+          if constexpr (kRowsX == 1) {
+            less[0].x = fmaf(sz.x, at[0], less[0].x);
+          } else {
+            const float4 v = *reinterpret_cast<const float4*>(at);
+            less[m / 2] = fma2(sz, make_float2(v.x, v.y), less[m / 2]);
+            less[m / 2 + 1] = fma2(sz, make_float2(v.z, v.w), less[m / 2 + 1]);
+          }
         }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float2 p = *reinterpret_cast<const float2*>(xpower + n * 8 + 2 * t);
+      const float2 p = *reinterpret_cast<const float2*>(xpower + (FEW ? 2 * t % kRowsX : n * 8 + 2 * t));
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -317,59 +343,69 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
     }
     slot = slot + 1 == kStages ? 0 : slot + 1;
     fill = fill + 1 == kStages ? 0 : fill + 1;
-    __syncthreads();  // this step's x has been read, the next one's is there
+    if constexpr (!FEW) __syncthreads();  // this step's x has been read, the next one's is there
   }
   copy_wait<0>();
+  if constexpr (FEW) __syncthreads();  // the rings are done with
 
+  float* const all = reinterpret_cast<float*>(smem);  // [warp][kRowsX][32]
+  float* const sums = all + warp * (kRowsX * 32);
 #pragma unroll
   for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        float* to = sums + (n * 8 + 2 * t) * kRowsW + warp * 32 + mt * 16 + u * 8 + g;
+        if (FEW && 2 * t >= kRowsX) continue;
+        float* to = sums + (n * 8 + 2 * t) * 32 + mt * 16 + u * 8 + g;
         to[0] = acc[mt][n][u].x * 16777216.0f;
-        to[kRowsW] = acc[mt][n][u].y * 16777216.0f;
+        if (kRowsX > 1) to[32] = acc[mt][n][u].y * 16777216.0f;
       }
   __syncwarp();
 #pragma unroll
-  for (int m = 0; m < 8 * NT; ++m) sums[m * kRowsW + warp * 32 + lane] -= m % 2 ? less[m / 2].y : less[m / 2].x;
+  for (int m = 0; m < kRowsX; ++m) sums[m * 32 + lane] -= m % 2 ? less[m / 2].y : less[m / 2].x;
   if (splits > 1)
     cluster_sync();
   else
     __syncthreads();
-  // block `rank` of the cluster adds up its share of the rows
-  const int share = (kRowsW + splits - 1) / splits, from = rank * share, wide = min(share, kRowsW - from);
-  const uint32_t mine = shared_address(sums);
+  // block `rank` of the cluster adds up its share of the weight rows, over the blocks and (FEW) their warps
+  const int share = (kRowsW + splits - 1) / splits, from = rank * share, wide = max(0, min(share, kRowsW - from));
+  const uint32_t mine = shared_address(all);
   for (int i = threadIdx.x; i < wide * rows; i += kWarps * 32) {
     const int m = i / wide, r = from + i % wide, n = n0 + r;
     if (n >= a.n) continue;
+    const int at = (FEW ? 0 : r / 32 * (kRowsX * 32)) + m * 32 + r % 32;
     float v = 0.0f;
-    if (splits > 1) {
-      for (int j = 0; j < splits; ++j) v += peer_load(mine + (m * kRowsW + r) * 4, j);
-    } else {
-      v = sums[m * kRowsW + r];
-    }
+    for (int j = 0; j < splits; ++j)
+#pragma unroll
+      for (int w = 0; w < (FEW ? kWarps : 1); ++w) {
+        const int each = at + w * (kRowsX * 32);
+        v += splits > 1 ? peer_load(mine + each * 4, j) : all[each];
+      }
     if (a.bias) v += to_f32(static_cast<const T*>(a.bias)[n]);
     static_cast<T*>(a.y)[(m0 + m) * a.ldy + n] = from_f32<T>(v);
   }
   if (splits > 1) cluster_sync();  // a block's sums stay until all have read them
 }
 
-template <typename T, int G, int NT>
+template <typename T, int G, int NT, int FEW>
 int launch_linear(W4Args a, int sms, cudaStream_t stream) {
-  constexpr int kSmem = Layout<T, G, NT>::kBytes;
-  auto kernel = linear_w4_kernel<T, G, NT>;
+  using L = Layout<T, G, NT, FEW>;
+  constexpr int kSmem = L::kBytes;
+  auto kernel = linear_w4_kernel<T, G, NT, FEW>;
   static std::atomic<bool> ready{false};
   if (!ready.load(std::memory_order_relaxed)) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute(linear_w4_kernel)");
     ready.store(true, std::memory_order_relaxed);
   }
-  // K is split so that two blocks an SM are busy, and no further: fewer, longer streams read faster
-  const int tiles = (a.n + kRowsW - 1) / kRowsW, passes = (a.m + 8 * NT - 1) / (8 * NT);
+  // K is split so that two blocks an SM are busy (FEW: and every warp has a step), and no further: fewer, longer streams
+  // read faster
+  const int tiles = (a.n + L::kRowsW - 1) / L::kRowsW, passes = (a.m + L::kRowsX - 1) / L::kRowsX;
   a.steps = (a.k + kStep - 1) / kStep;
-  const int want = std::max(1, std::min(kMaxSplit, static_cast<int>(2ll * sms / (static_cast<long long>(tiles) * passes))));
+  int want = static_cast<int>(std::min<long long>(kMaxSplit, 2ll * sms / (static_cast<long long>(tiles) * passes)));
+  if (FEW) want = std::max(std::min(want, a.steps / kWarps), (a.steps + L::kBuffers - 1) / L::kBuffers);
+  want = std::max(1, want);
   a.slice = std::max(1, (a.steps + want - 1) / want);
   const int splits = std::max(1, (a.steps + a.slice - 1) / a.slice);
   cudaLaunchConfig_t cfg{};
@@ -389,7 +425,13 @@ int launch_linear(W4Args a, int sms, cudaStream_t stream) {
 
 template <typename T, int G>
 int launch_linear_rows(const W4Args& a, int sms, cudaStream_t stream) {
-  return a.m <= 8 ? launch_linear<T, G, 1>(a, sms, stream) : launch_linear<T, G, 2>(a, sms, stream);
+  // One row of x: 1 x 8192 x 8192 bf16 11.0 us, 12.0 with blocks of 256 weight rows; 1 x 16000 x 1000 7.2 and 12.9;
+  // 1 x 768 x 768 3.1 and 4.5.  Two to four: only while those blocks, K split eight ways, would leave SMs idle
+  // (2 x 16000 x 1000 fp32 8.9 and 16.1 us, but 4 x 8192 x 8192 bf16 22.2 and 13.0: each block brings x in).
+  if (a.m == 1 && a.k <= kMaxSplit * kStep * Layout<T, G, 1, 1>::kBuffers) return launch_linear<T, G, 1, 1>(a, sms, stream);
+  if (a.m <= kFewRows && (a.n + 255) / 256 * kMaxSplit < sms && a.k <= kMaxSplit * kStep * Layout<T, G, 1, kFewRows>::kBuffers)
+    return launch_linear<T, G, 1, kFewRows>(a, sms, stream);
+  return a.m <= 8 ? launch_linear<T, G, 1, 0>(a, sms, stream) : launch_linear<T, G, 2, 0>(a, sms, stream);
 }
 
 }  // namespace
