@@ -27,6 +27,27 @@ constexpr int kSplitCounters = 1 << 16;
 B200Q_HIDDEN int host_counters(cudaStream_t stream, unsigned** out);
 B200Q_HIDDEN void host_set_path(int path);
 
+// Launches a kernel that begins with wait_for_previous(): its blocks may take their places while the stream's previous kernel
+// drains, and wait there until that one has ended and its writes can be seen.  `cluster` blocks make a cluster.
+template <typename... P, typename... A>
+int host_launch(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                int cluster, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+  return e == cudaSuccess ? host_check_launch(what) : host_cuda_fail(e, what);
+}
+
 // Codes of g_dev_err for bad values that only the device sees; 0x1xx are timeouts (common.cuh).
 constexpr int kDevErrBadPosition = 0x201;
 constexpr int kDevErrBadSlot = 0x202;

@@ -94,6 +94,7 @@ __device__ __forceinline__ void store_eight(__nv_bfloat16* p, const float (&v)[8
 
 template <typename T, int D, int G, int AHEAD>
 __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Cache c, AppendArgs a) {
+  wait_for_previous();
   constexpr int V = 8, kLanes = D / V, kRows = kMoveThreads / kLanes, kPerGroup = G / V;
   const int l = threadIdx.x % kLanes;
   const uint32_t first = blockIdx.x * (kRows * AHEAD) + threadIdx.x / kLanes;
@@ -149,6 +150,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Cache c, Appen
 
 template <typename T, int D, int G, int AHEAD>
 __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(Cache c, const int64_t* slots, T* k, T* v, int t, int* err) {
+  wait_for_previous();
   constexpr int V = 8, kLanes = D / V, kRows = kMoveThreads / kLanes, kPerGroup = G / V;
   const int l = threadIdx.x % kLanes;
   const uint32_t first = blockIdx.x * (kRows * AHEAD) + threadIdx.x / kLanes;
@@ -207,10 +209,9 @@ int check_cache(const b200q_kv4_cache* p, Cache* c) {
 }
 
 #define B200Q_MOVE_D(kernel, G, A) (c.d == 64 ? kernel<T, 64, G, A> : c.d == 128 ? kernel<T, 128, G, A> : kernel<T, 256, G, A>)
-#define B200Q_MOVE(kernel, ...)                                                                      \
-  (ahead == 1 ? c.group == 32 ? B200Q_MOVE_D(kernel, 32, 1) : B200Q_MOVE_D(kernel, 64, 1)            \
-              : c.group == 32 ? B200Q_MOVE_D(kernel, 32, 4) : B200Q_MOVE_D(kernel, 64, 4))<<<        \
-      blocks, kMoveThreads, 0, static_cast<cudaStream_t>(stream)>>>(__VA_ARGS__)
+#define B200Q_MOVE(kernel)                                                                         \
+  (ahead == 1 ? c.group == 32 ? B200Q_MOVE_D(kernel, 32, 1) : B200Q_MOVE_D(kernel, 64, 1)          \
+              : c.group == 32 ? B200Q_MOVE_D(kernel, 32, 4) : B200Q_MOVE_D(kernel, 64, 4))
 
 // Rows that a lane has on their way: four when there are rows for many blocks (append and read of 8191 tokens x 4 heads x
 // 256 fp32: 42 us, 46 with two; 2048 x 8 x 128 bf16: 13.0, 18.6 with one), one when a call is all latency (64 x 8 x 128:
@@ -253,8 +254,7 @@ int launch_attention(const Cache& c, AttnArgs a, int sms, cudaStream_t stream) {
   a.partial = static_cast<float*>(ws);
   a.partial_ml = a.partial + rows * D;
   if (blocks > kSplitCounters) return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
-  kernel<<<blocks, kWarps * 32, Shape::kSmem, stream>>>(c, a);
-  return host_check_launch("kv4_attention_kernel launch");
+  return host_launch("kv4_attention_kernel launch", kernel, dim3(blocks), kWarps * 32, Shape::kSmem, stream, 1, c, a);
 }
 
 int check_ftype(int ftype) {
@@ -284,8 +284,8 @@ extern "C" int b200q_kv4_append(const b200q_kv4_cache* cache, const void* k, lon
   if ((rc = host_device(&sms, &a.err))) return rc;
   int ahead = 0, blocks = 0;
   if ((rc = move_blocks(c, t, sms, &ahead, &blocks))) return rc;
-  B200Q_DISPATCH_FTYPE(ftype, (B200Q_MOVE(kv4_append_kernel, c, a)));
-  rc = host_check_launch("kv4_append_kernel launch");
+  B200Q_DISPATCH_FTYPE(ftype, rc = host_launch("kv4_append_kernel launch", B200Q_MOVE(kv4_append_kernel), dim3(blocks),
+                                               kMoveThreads, 0, static_cast<cudaStream_t>(stream), 1, c, a));
   if (rc == B200Q_OK) host_set_path(19);
   return rc;
 }
@@ -304,8 +304,9 @@ extern "C" int b200q_kv4_read(const b200q_kv4_cache* cache, const int64_t* slots
     return host_fail(B200Q_ERR_INVALID_ARG, "kv4_read outputs must be 32-byte aligned");
   int ahead = 0, blocks = 0;
   if ((rc = move_blocks(c, t, sms, &ahead, &blocks))) return rc;
-  B200Q_DISPATCH_FTYPE(ftype, (B200Q_MOVE(kv4_read_kernel, c, slots, static_cast<T*>(k), static_cast<T*>(v), t, err)));
-  rc = host_check_launch("kv4_read_kernel launch");
+  B200Q_DISPATCH_FTYPE(ftype, rc = host_launch("kv4_read_kernel launch", B200Q_MOVE(kv4_read_kernel), dim3(blocks),
+                                               kMoveThreads, 0, static_cast<cudaStream_t>(stream), 1, c, slots,
+                                               static_cast<T*>(k), static_cast<T*>(v), t, err));
   if (rc == B200Q_OK) host_set_path(19);
   return rc;
 }

@@ -180,6 +180,7 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
   constexpr int kGroups = Shape::kGroups, kPitch = Shape::kPitch, kRows = 8 * NT, kTerms = Shape::kTerms;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ unsigned arrived;
+  wait_for_previous();
   uint4* const query = reinterpret_cast<uint4*>(smem + Shape::kBody);
   float* const row_ml = reinterpret_cast<float*>(smem + Shape::kBody + Shape::kQuery);
   float* const row_sum = row_ml + kWarps * kRows * 2;  // [kGroups][kRows] sums of the scaled query, times 2^-24

@@ -65,6 +65,7 @@ __device__ __forceinline__ float weight(const T* w, int i) {
 // One warp per row.  A lane writes only the channels that it has read, so y may be x.
 template <typename T>
 __global__ void qk_norm_rope_kernel(NormArgs a) {
+  wait_for_previous();
   const int heads = a.side[0].heads + a.side[1].heads;
   const long long row = static_cast<long long>(blockIdx.x) * kNormWarps + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
@@ -99,6 +100,7 @@ __global__ void qk_norm_rope_kernel(NormArgs a) {
 // shared memory need no atomics.
 template <typename T>
 __global__ void qk_norm_rope_bprop_kernel(NormArgs a) {
+  wait_for_previous();
   extern __shared__ float sums[];  // [kNormWarps][2][d]
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   float* mine = sums + warp * 2 * a.d;
@@ -325,6 +327,7 @@ __device__ __forceinline__ Unit unit_of(const NormArgs& a, uint32_t unit, const 
 // A group of LPR lanes takes `per` heads of one token's queries or keys.
 template <typename T, int LPR, bool INTERLEAVED>
 __global__ void __launch_bounds__(kFastThreads) qk_norm_rope_rows_kernel(NormArgs a, Split split) {
+  wait_for_previous();
   const int l = threadIdx.x % LPR;
   const Lane lane = lane_of<INTERLEAVED>(a, l);
   const Unit unit = unit_of(a, blockIdx.x * (kFastThreads / LPR) + threadIdx.x / LPR, split);
@@ -361,6 +364,7 @@ __global__ void __launch_bounds__(kFastThreads) qk_norm_rope_rows_kernel(NormArg
 // The gradient: groups of lanes walk over units, the weights' sums stay in registers.
 template <typename T, int LPR, bool INTERLEAVED>
 __global__ void __launch_bounds__(kFastThreads) qk_norm_rope_bprop_rows_kernel(NormArgs a, Split split, uint32_t units) {
+  wait_for_previous();
   constexpr int kGroups = kFastThreads / LPR, kRowsAhead = 2;
   __shared__ float sums[kGroups][2][LPR * 8];
   const int l = threadIdx.x % LPR, group = threadIdx.x / LPR;
@@ -451,6 +455,7 @@ __global__ void __launch_bounds__(kFastThreads) qk_norm_rope_bprop_rows_kernel(N
 // Adds the blocks' weight gradients up in a fixed order: 32 columns a block, the partial sums shared out to 32 warps.
 template <typename T>
 __global__ void norm_weight_grad_kernel(const float* partial, int blocks, int d, T* dqw, T* dkw) {
+  wait_for_previous();
   __shared__ float sums[32][33];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, i = blockIdx.x * 32 + lane;
   float v = 0.0f;
@@ -497,13 +502,9 @@ Split split_heads(const NormArgs& a, int lanes, int sms) {
   return s;
 }
 
-#define B200Q_NORM_ROWS(kernel, ...)                                                                                \
-  (a.interleaved ? (lanes == 8    ? kernel<T, 8, true>                                                              \
-                    : lanes == 16 ? kernel<T, 16, true>                                                             \
-                                  : kernel<T, 32, true>)                                                            \
-                 : (lanes == 8    ? kernel<T, 8, false>                                                             \
-                    : lanes == 16 ? kernel<T, 16, false>                                                            \
-                                  : kernel<T, 32, false>))<<<static_cast<int>(blocks), kFastThreads, 0, cs>>>(__VA_ARGS__)
+#define B200Q_NORM_ROWS(kernel)                                                                                  \
+  (a.interleaved ? (lanes == 8 ? kernel<T, 8, true> : lanes == 16 ? kernel<T, 16, true> : kernel<T, 32, true>)   \
+                 : (lanes == 8 ? kernel<T, 8, false> : lanes == 16 ? kernel<T, 16, false> : kernel<T, 32, false>))
 
 // Checks what both directions share and fills in the kernels' arguments.
 int norm_args(const b200q_qk_norm_args* p, NormArgs* a, int* sms) {
@@ -554,13 +555,14 @@ extern "C" int b200q_qk_norm_rope(const b200q_qk_norm_args* args, void* stream) 
     const long long units = static_cast<long long>(t) * split.parts.d;
     const long long blocks = (units * lanes + kFastThreads - 1) / kFastThreads;
     if (units > 0x7ffffff0ll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
-    B200Q_DISPATCH_FTYPE(ftype, (B200Q_NORM_ROWS(qk_norm_rope_rows_kernel, a, split)));
+    B200Q_DISPATCH_FTYPE(ftype, rc = host_launch("qk_norm_rope_kernel launch", B200Q_NORM_ROWS(qk_norm_rope_rows_kernel), dim3(static_cast<unsigned>(blocks)),
+                                                 kFastThreads, 0, cs, 1, a, split));
   } else {
     const long long blocks = (static_cast<long long>(t) * (hq + hk) + kNormWarps - 1) / kNormWarps;
     if (blocks > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
-    B200Q_DISPATCH_FTYPE(ftype, (qk_norm_rope_kernel<T><<<static_cast<int>(blocks), kNormWarps * 32, 0, cs>>>(a)));
+    B200Q_DISPATCH_FTYPE(ftype, rc = host_launch("qk_norm_rope_kernel launch", qk_norm_rope_kernel<T>, dim3(static_cast<unsigned>(blocks)),
+                                                 kNormWarps * 32, 0, cs, 1, a));
   }
-  rc = host_check_launch("qk_norm_rope_kernel launch");
   if (rc == B200Q_OK) host_set_path(18);
   return rc;
 }
@@ -589,20 +591,21 @@ extern "C" int b200q_qk_norm_rope_bprop(const b200q_qk_norm_args* args, void* st
   const size_t smem = static_cast<size_t>(kNormWarps) * 2 * d * sizeof(float);
   B200Q_DISPATCH_FTYPE(ftype, {
     if (lanes) {
-      B200Q_NORM_ROWS(qk_norm_rope_bprop_rows_kernel, a, split, static_cast<uint32_t>(units));
+      rc = host_launch("qk_norm_rope_bprop_kernel launch", B200Q_NORM_ROWS(qk_norm_rope_bprop_rows_kernel), dim3(blocks),
+                       kFastThreads, 0, cs, 1, a, split, static_cast<uint32_t>(units));
     } else {
       if (smem > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(qk_norm_rope_bprop_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              static_cast<int>(smem));
         if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute(qk_norm_rope_bprop_kernel)");
       }
-      qk_norm_rope_bprop_kernel<T><<<blocks, kNormWarps * 32, smem, cs>>>(a);
+      rc = host_launch("qk_norm_rope_bprop_kernel launch", qk_norm_rope_bprop_kernel<T>, dim3(blocks), kNormWarps * 32,
+                       smem, cs, 1, a);
     }
-    if ((rc = host_check_launch("qk_norm_rope_bprop_kernel launch"))) return rc;
-    norm_weight_grad_kernel<T><<<(2 * d + 31) / 32, 1024, 0, cs>>>(a.partial, blocks, d, static_cast<T*>(args->q_w_grad),
-                                                                 static_cast<T*>(args->k_w_grad));
+    if (rc) return rc;
+    rc = host_launch("norm_weight_grad_kernel launch", norm_weight_grad_kernel<T>, dim3((2 * d + 31) / 32), 1024, 0, cs, 1,
+                     a.partial, blocks, d, static_cast<T*>(args->q_w_grad), static_cast<T*>(args->k_w_grad));
   });
-  rc = host_check_launch("norm_weight_grad_kernel launch");
   if (rc == B200Q_OK) host_set_path(18);
   return rc;
 }

@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
   constexpr int kTerms = L::kTerms, kWords = G / 32, kGroups = kStep / G, kStages = L::kStages, kRowsW = L::kRowsW;
   constexpr int kRowsX = L::kRowsX;
   extern __shared__ __align__(128) uint8_t smem[];
+  wait_for_previous();
   uint8_t* const buffers = smem + L::kRing;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const int splits = max(1, (a.steps + a.slice - 1) / a.slice);  // the cluster
@@ -408,19 +409,7 @@ int launch_linear(W4Args a, int sms, cudaStream_t stream) {
   want = std::max(1, want);
   a.slice = std::max(1, (a.steps + want - 1) / want);
   const int splits = std::max(1, (a.steps + a.slice - 1) / a.slice);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(tiles * splits, passes);
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim = {static_cast<unsigned>(splits), 1, 1};
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e != cudaSuccess) return host_cuda_fail(e, "linear_w4_kernel launch");
-  return host_check_launch("linear_w4_kernel launch");
+  return host_launch("linear_w4_kernel launch", kernel, dim3(tiles * splits, passes), kWarps * 32, kSmem, stream, splits, a);
 }
 
 template <typename T, int G>
