@@ -245,15 +245,16 @@ int launch_attention(const Cache& c, AttnArgs a, int sms, cudaStream_t stream) {
   // one block for each that the GPU holds at once; fewer when even the longest lengths have fewer steps
   const long long steps = (static_cast<long long>(a.max_pages) * c.page_size + kStepTokens - 1) / kStepTokens;
   const long long most = static_cast<long long>(a.b) * c.heads * a.row_tiles * std::max(1ll, (steps + kMinSteps - 1) / kMinSteps);
+  if (static_cast<long long>(a.b) * c.heads * a.row_tiles * (steps + kUnitSteps + 1) > 0x7fffffffll)
+    return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
   // (a unit's parts, one per block at most, leave their shares in shared memory when they are joined)
-  const int blocks = static_cast<int>(std::min<long long>(std::min(sms * resident, Shape::kBody / (8 * NT * 4)), most));
+  const int blocks = static_cast<int>(std::min<long long>(std::min({sms * resident, Shape::kBody / (8 * NT * 4), kSplitCounters}), most));
   const size_t rows = static_cast<size_t>(blocks) * 2 * 8 * NT;
   void* ws = nullptr;
   int rc = host_workspace(rows * (D + 2) * sizeof(float), stream, &ws);
   if (rc || (rc = host_counters(stream, &a.counters))) return rc;
   a.partial = static_cast<float*>(ws);
   a.partial_ml = a.partial + rows * D;
-  if (blocks > kSplitCounters) return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
   return host_launch("kv4_attention_kernel launch", kernel, dim3(blocks), kWarps * 32, Shape::kSmem, stream, 1, c, a);
 }
 

@@ -18,8 +18,8 @@
 // 2^8: a warp-wide maximum is taken a few times per sequence, not per tile.
 //
 // Work: a unit is (sequence, cache head, tile of rows), in steps of kWarps tiles of kTile tokens.  All units' steps lie
-// end to end, and block i takes steps [i * per, (i + 1) * per) of them, whatever the lengths (which only the device knows):
-// every block has the same work, and none waits for a last wave.  The parts of a unit that several blocks share go to
+// end to end, and each block takes the same number of them, whatever the lengths (which only the device knows): none waits
+// for a last wave.  The parts of a unit that several blocks share go to
 // the workspace, and the block that finishes last joins them in order.
 //
 // What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head.  Each warp owns a ring of kStages tiles of
@@ -27,6 +27,8 @@
 // the end.  A row of codes is padded by 16 bytes in shared memory: then lanes (g, t) reading 4 bytes at g rows down,
 // and 2t rows down, both touch 32 banks once.
 #pragma once
+#include <type_traits>
+
 #include "host.h"
 #include "lowbit.cuh"
 
@@ -57,12 +59,12 @@ struct AttnArgs {
   int* err;
 };
 
-constexpr int kMinSteps = 2;  // steps of a block at least
+constexpr int kMinSteps = 2;  // steps of a part at least
 constexpr int kUnitSteps = 3; // what a unit costs besides its steps (its queries, its first tiles' way, its join), in steps
 
 constexpr int kTile = 32;    // tokens of a warp's step
 constexpr int kWarps = 4;    // a block's warps take tiles in turn
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 constexpr int kStepTokens = kWarps * kTile;
 
 template <int D, int G, int NT, bool F32>
@@ -77,8 +79,9 @@ struct AttnShape {
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kJoin = kWarps * 8 * NT * (D + 4) * 4;      // the warps' sums, over the ring
   static constexpr int kBody = kRing > kJoin ? kRing : kJoin;
+  static constexpr int kTileParams = kTile * kGroups * 16;        // a warp's tile: see Prepared
   static constexpr int kRowsMl = kWarps * 8 * NT * 2 * 4;
-  static constexpr int kSmem = kBody + kQuery + kRowsMl + (8 * NT * (kGroups + 1)) * 4;
+  static constexpr int kSmem = kBody + kQuery + kWarps * kTileParams + kRowsMl + 8 * NT * (kGroups + 1) * 4 + 8 * NT * 20;
 };
 
 // Row of the cache that holds token `tok`, or ~0 where there is none to read.
@@ -102,22 +105,12 @@ __device__ __forceinline__ int valid_length(const Cache& c, const AttnArgs& a, i
   return 0;
 }
 
-template <typename T>
-__device__ __forceinline__ float load_as_f32(const void* p, long long i) {
-  return to_f32(static_cast<const T*>(p)[i]);
-}
-__device__ __forceinline__ float load_any(int ftype, const void* p, long long i) {
-  return ftype == B200Q_F32   ? load_as_f32<float>(p, i)
-         : ftype == B200Q_F16 ? load_as_f32<__half>(p, i)
-                              : load_as_f32<__nv_bfloat16>(p, i);
-}
-__device__ __forceinline__ void store_any(int ftype, void* p, long long i, float v) {
+__device__ __forceinline__ void store_four(int ftype, void* p, long long i, float4 v) {
   if (ftype == B200Q_F32)
-    static_cast<float*>(p)[i] = v;
-  else if (ftype == B200Q_F16)
-    static_cast<__half*>(p)[i] = __float2half_rn(v);
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = v;
   else
-    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) =
+        ftype == B200Q_F16 ? make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w)) : make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
 // Issues the copies of one tile: lane l holds the cache row of token l.
@@ -174,61 +167,122 @@ __device__ __forceinline__ void load_tile_page(const Cache& c, uint32_t stage, u
   }
 }
 
+// Where a block stands: in shared memory, so that it takes no registers while tiles are computed.
+struct Plan {
+  uint32_t total, stop, at, base;  // steps of all units, the block's end, its next step, its sequence's first
+  int seq, n;                      // the sequence, the steps of each of its units
+  // the unit at hand: its sequence, cache head and tile of rows, whether its first part is here, the block of that,
+  // how many parts it has
+  int unit_seq, head, tile, begins, owner, parts;
+};
+
 template <int D, int G, int NT, bool F32>
-__global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_attention_kernel(Cache c, AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128 ? 3 : 4) kv4_attention_kernel(Cache c, AttnArgs a) {
   using Shape = AttnShape<D, G, NT, F32>;
   constexpr int kGroups = Shape::kGroups, kPitch = Shape::kPitch, kRows = 8 * NT, kTerms = Shape::kTerms;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ unsigned arrived;
+  __shared__ Plan plan;
   wait_for_previous();
   uint4* const query = reinterpret_cast<uint4*>(smem + Shape::kBody);
-  float* const row_ml = reinterpret_cast<float*>(smem + Shape::kBody + Shape::kQuery);
+  uint8_t* const prepared = smem + Shape::kBody + Shape::kQuery + (threadIdx.x / 32) * Shape::kTileParams;
+  float* const row_ml = reinterpret_cast<float*>(smem + Shape::kBody + Shape::kQuery + kWarps * Shape::kTileParams);
   float* const row_sum = row_ml + kWarps * kRows * 2;  // [kGroups][kRows] sums of the scaled query, times 2^-24
   float* const row_f = row_sum + kRows * kGroups;
+  int64_t* const row_out = reinterpret_cast<int64_t*>(row_f + kRows);
+  float2* const row_all = reinterpret_cast<float2*>(row_out + kRows);
+  int* const row_limit = reinterpret_cast<int*>(row_all + kRows);  // tokens that a row sees
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4;
 
   const int units = c.heads * a.row_tiles, ratio = a.hq / c.heads;
   auto steps_of = [&](int i) { return kUnitSteps + max(1, (valid_length(c, a, i) + kStepTokens - 1) / kStepTokens); };
-  long long total = 0;
-  for (int i = lane; i < a.b; i += 32) total += steps_of(i);
+  // Block i takes total / blocks steps, and one more while i is below the remainder.  A cut that would leave a part of less
+  // than kMinSteps steps at a unit's start or end moves there.
+  auto blocks_for = [&](uint32_t total) { return min(gridDim.x, (total + kMinSteps - 1) / kMinSteps); };
+  {
+    uint32_t total = 0;
+    for (int i = lane; i < a.b; i += 32) total += steps_of(i);
 #pragma unroll
-  for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
-  total *= units;
-  const long long per = max(static_cast<long long>(kMinSteps), (total + gridDim.x - 1) / gridDim.x);
-  long long at = blockIdx.x * per;  // the block's next step
-  const long long stop = min(total, at + per);
-  if (at >= stop) return;
-  int seq = 0;
-  long long base = 0;  // first step of the sequence
-  for (;; seq += 32) {
-    long long sum = seq + lane < a.b ? static_cast<long long>(steps_of(seq + lane)) * units : 0;
+    for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
+    total *= units;
+    const uint32_t blocks = blocks_for(total);
+    if (blockIdx.x >= blocks) return;
+    const uint32_t per = total / blocks, more = total - per * blocks;
+    int seq = 0, n = 0;
+    uint32_t base = 0;
+    auto find = [&](uint32_t step) {  // the sequence of a step
+      base = 0;
+      for (seq = 0;; seq += 32) {
+        const int mine = seq + lane < a.b ? steps_of(seq + lane) : 0;
+        uint32_t sum = mine * units;
 #pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      const long long v = __shfl_up_sync(~0u, sum, x);
-      if (lane >= x) sum += v;
-    }
-    const unsigned past = __ballot_sync(~0u, base + sum > at);
-    const int first = past ? __ffs(past) - 1 : 31;
-    const long long before = __shfl_sync(~0u, sum, past ? first - 1 : 31);  // lane -1 is lane 31, and not used
-    if (!past || first > 0) base += before;
-    if (past) {
-      seq += first;
-      break;
+        for (int x = 1; x < 32; x <<= 1) {
+          const uint32_t v = __shfl_up_sync(~0u, sum, x);
+          if (lane >= x) sum += v;
+        }
+        const unsigned past = __ballot_sync(~0u, base + sum > step);
+        if (past) {
+          const int first = __ffs(past) - 1;
+          n = __shfl_sync(~0u, mine, first);
+          base += __shfl_sync(~0u, sum, first) - n * units;
+          seq += first;
+          return;
+        }
+        base += __shfl_sync(~0u, sum, 31);
+      }
+    };
+    auto cut = [&](uint32_t i) {
+      const uint32_t step = i * per + min(i, more);
+      if (step >= total) return total;
+      find(step);
+      const uint32_t unit_at = base + (step - base) / n * n;
+      return step - unit_at < kUnitSteps + kMinSteps ? unit_at : unit_at + n - step < kMinSteps ? unit_at + n : step;
+    };
+    const uint32_t stop = cut(blockIdx.x + 1), at = cut(blockIdx.x);
+    if (at >= stop) return;
+    if (at == base + static_cast<uint32_t>(n) * units) base = at, n = steps_of(++seq);
+    if (tid == 0) plan = Plan{total, stop, at, base, seq, n};
+  }
+  __syncthreads();
+
+ for (;;) {
+  // steps [off, off + count) of the unit; its first kUnitSteps steps stand for what it costs besides
+  const int seq = plan.seq, len = valid_length(c, a, seq), unit = static_cast<int>((plan.at - plan.base) / plan.n);
+  const uint32_t unit_at = plan.base + unit * plan.n, end = min(unit_at + plan.n, plan.stop);
+  const int off = max(0, static_cast<int>(plan.at - unit_at) - kUnitSteps), count = static_cast<int>(end - unit_at) - kUnitSteps - off;
+  const int tile = unit % a.row_tiles, head = unit / a.row_tiles, rows = min(kRows, a.tq * ratio - tile * kRows);
+  // the query rows are on their way first, in their own type
+  constexpr int kPer = D / 32, kRowsWarp = kRows / kWarps;
+  using Raw = std::conditional_t<F32, float, uint16_t>;
+  Raw q[kRowsWarp][kPer];
+#pragma unroll
+  for (int j = 0; j < kRowsWarp; ++j) {
+    const int r = warp + j * kWarps, rr = tile * kRows + r;
+    const Raw* from = static_cast<const Raw*>(a.q) + seq * a.q_bs + (rr / ratio) * a.q_ts + (head * ratio + rr % ratio) * a.q_hs + lane;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) q[j][i] = r < rows ? __ldg(from + 32 * i) : Raw(0);  // channel 32 i + lane
+  }
+  __syncthreads();
+  if (tid == kWarps * 32 - 1) {
+    // the cuts inside the unit, and the block that its first part lies with: the one after the last cut before them
+    const uint32_t total = plan.total, blocks = blocks_for(total), per = total / blocks, more = total - per * blocks;
+    auto cuts_to = [&](uint32_t step) {  // how many cuts lie at or before `step`
+      const uint32_t longer = more * (per + 1);
+      return step < longer ? step / (per + 1) + 1 : more + (step - longer) / per + 1;
+    };
+    const uint32_t before = cuts_to(unit_at + kUnitSteps + kMinSteps - 1);
+    plan.owner = static_cast<int>(before) - 1;
+    plan.parts = plan.n >= kUnitSteps + 2 * kMinSteps ? 1 + static_cast<int>(cuts_to(unit_at + plan.n - kMinSteps) - before) : 1;
+    plan.unit_seq = seq;
+    plan.head = head;
+    plan.tile = tile;
+    plan.begins = off == 0;
+    plan.at = end;
+    if (end == plan.base + static_cast<uint32_t>(plan.n) * units && end < plan.stop) {
+      plan.base = end;
+      plan.n = steps_of(++plan.seq);
     }
   }
-
- for (; at < stop;) {
-  // steps [off, off + count) of the unit; its first kUnitSteps steps stand for what it costs besides
-  const int n = steps_of(seq), len = valid_length(c, a, seq);
-  const int unit = static_cast<int>((at - base) / n);
-  const long long unit_at = base + static_cast<long long>(unit) * n;
-  const long long end = min(unit_at + n, stop);
-  const int off = max(0, static_cast<int>(at - unit_at) - kUnitSteps), count = static_cast<int>(end - unit_at) - kUnitSteps - off;
-  at = end;
-  if (count <= 0) break;  // all of it lies with the next block
-  const int tile = unit % a.row_tiles, head = unit / a.row_tiles, rows = min(kRows, a.tq * ratio - tile * kRows);
-  const long long owner = (unit_at + kUnitSteps) / per;  // the block that its first step lies with
-  const int parts = static_cast<int>((unit_at + n - 1) / per - owner) + 1;
   // the last row of the tile sees the most tokens
   const int seen = max(0, len - a.tq + (tile * kRows + rows - 1) / ratio + 1);
   const int begin = off * kStepTokens, until = min(seen, begin + count * kStepTokens);
@@ -261,20 +315,24 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
     row = token_row(c, a, pages, head, first + (i + 1) * kStep, until);
   }
 
-  // query rows: scaled to fp16, laid out as operand B; a warp takes rows in turn
-  for (int r = warp; r < kRows; r += kWarps) {
-    constexpr int kPer = D / 32;
-    const int rr = tile * kRows + r;
-    float v[kPer];
-    float top = 0.0f;
+  // query rows: scaled to fp16, laid out as operand B
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {  // channel 32 i + lane
-      v[i] = r < rows ? load_any(a.ftype, a.q, seq * a.q_bs + (rr / ratio) * a.q_ts + (head * ratio + rr % ratio) * a.q_hs + 32 * i + lane)
-                      : 0.0f;
+  for (int j = 0; j < kRowsWarp; ++j) {
+    const int r = warp + j * kWarps;
+    float v[kPer], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if constexpr (F32)
+        v[i] = q[j][i];
+      else
+        v[i] = a.ftype == B200Q_F16 ? __half2float(__ushort_as_half(q[j][i])) : __uint_as_float(static_cast<uint32_t>(q[j][i]) << 16);
       top = fmaxf(top, fabsf(v[i]));
     }
     const Power power = power_for(warp_max(top));
-    if (lane == 0) row_f[r] = power.down * a.scale * 1.4426950408889634f * 16777216.0f;
+    if (lane == 0) {
+      row_f[r] = power.down * a.scale * 1.4426950408889634f * 16777216.0f;
+      row_limit[r] = len - a.tq + (tile * kRows + min(r, rows - 1)) / ratio + 1;
+    }
     // lane: channel p = lane % 8 of the 8 that thread lane / 8 of a quad holds; pairs are (0,4) (1,5) (2,6) (3,7)
     const int p = lane % 8, holder = (r % 8) * 4 + lane / 8;
     __half* to = reinterpret_cast<__half*>(query);
@@ -301,21 +359,13 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
   __syncthreads();
 
   // this lane's columns: rows 2t, 2t + 1 of each 8
-  float2 f[NT], qsum[NT][kGroups], l[NT];
+  float2 l[NT];
   float m[NT][2];
-  int limit[NT][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = n * 8 + 2 * t + e;
-      (e ? f[n].y : f[n].x) = row_f[r];
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k) (e ? qsum[n][k].y : qsum[n][k].x) = row_sum[k * kRows + r];
-      m[n][e] = -INFINITY;
-      l[n] = both(0.0f);
-      limit[n][e] = len - a.tq + (tile * kRows + min(r, rows - 1)) / ratio + 1;
-    }
+  for (int n = 0; n < NT; ++n) {
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n] = both(0.0f);
+  }
   const int all_see = len - a.tq + tile * kRows / ratio + 1;  // tokens that every row of the tile sees
   float o[D / 16][NT][4], z[kGroups][NT][4];
 #pragma unroll
@@ -344,6 +394,44 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
     const uint32_t here = held[0];
     const int base = begin + (it * kWarps + warp) * kTile;
     const bool whole = here == ~0u && base + kTile <= all_see;
+
+    // lane l unpacks token l's scales and zero points for the lanes that use them: [group][token] (key scale, key zero
+    // point negated), then value scales times P's power, then value zero points as fp16 bits
+    float2* const k_prep = reinterpret_cast<float2*>(prepared);
+    float* const v_prep = reinterpret_cast<float*>(prepared + kTile * kGroups * 8);
+    uint16_t* const z_prep = reinterpret_cast<uint16_t*>(prepared + kTile * kGroups * 12);
+    {
+      float vs[kGroups], v_top = 0.0f;
+      const bool there = here >> lane & 1;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) {
+        const uint32_t p = kp[lane * kGroups + k], q = there ? vp[lane * kGroups + k] : 0u;  // places that hold nothing hold any bits
+        k_prep[k * kTile + lane] = make_float2(param_scale(p), -zero_point(p));
+        z_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 16);
+        vs[k] = param_scale(q);
+        v_top = fmaxf(v_top, vs[k]);
+      }
+      if (__any_sync(~0u, v_top > v_limit)) {
+        const int now = max(1, min(247, static_cast<int>(__float_as_uint(warp_max(v_top)) >> 23)));
+        float keep = now - v_exp < 127 ? __uint_as_float(static_cast<uint32_t>(127 + v_exp - now) << 23) : 0.0f;
+        if (v_limit < 0.0f) keep = 1.0f;  // no sums yet
+        v_exp = now;
+        v_factor = __uint_as_float(static_cast<uint32_t>(254 - now) << 23);
+        v_limit = __uint_as_float(static_cast<uint32_t>(now + 6) << 23);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) o[j][n][e] *= keep;
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j) z[j][n][e] *= keep;
+          }
+      }
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) v_prep[k * kTile + lane] = vs[k] * v_factor;
+    }
+    __syncwarp();
 
     // scores
     float2 s[2][NT][2];  // [tokens g, g + 8], rows 2t and 2t + 1
@@ -381,33 +469,19 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const uint32_t p = kp[(mt * 16 + u * 8 + g) * kGroups + k];
-          const float2 ks = both(param_scale(p)), kz = both(-zero_point(p));
+          const float2 p = k_prep[k * kTile + mt * 16 + u * 8 + g];
+          const float2 ks = both(p.x), kz = both(p.y);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const float* at = part[mt][n] + 2 * u;
-            const float2 v = fma2(kz, qsum[n][k], make_float2(at[0], at[1]));
+            const float2 v = fma2(kz, *reinterpret_cast<const float2*>(row_sum + k * kRows + n * 8 + 2 * t), make_float2(at[0], at[1]));
             s[mt][n][u] = k == 0 ? mul2(ks, v) : fma2(ks, v, s[mt][n][u]);
           }
         }
     }
 
-    // this lane's scales of the values, tokens mt * 16 + u * 8 + g
-    float vs[2][2][kGroups], v_top = 0.0f;
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int k = 0; k < kGroups; ++k) {
-          const int tok = mt * 16 + u * 8 + g;
-          vs[mt][u][k] = param_scale(vp[tok * kGroups + k]);
-          if (!whole && !(here >> tok & 1)) vs[mt][u][k] = 0.0f;
-          v_top = fmaxf(v_top, vs[mt][u][k]);
-        }
-
     // weights
-    bool raise = v_top > v_limit;
+    bool raise = false;
     float top[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -416,11 +490,12 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           float2& x = s[mt][n][u];
-          x = mul2(x, f[n]);
+          x = mul2(x, *reinterpret_cast<const float2*>(row_f + n * 8 + 2 * t));
           if (!whole) {
             const int tok = mt * 16 + u * 8 + g;
-            if (!(here >> tok & 1) || base + tok >= limit[n][0]) x.x = -INFINITY;
-            if (!(here >> tok & 1) || base + tok >= limit[n][1]) x.y = -INFINITY;
+            const int2 limit = *reinterpret_cast<const int2*>(row_limit + n * 8 + 2 * t);
+            if (!(here >> tok & 1) || base + tok >= limit.x) x.x = -INFINITY;
+            if (!(here >> tok & 1) || base + tok >= limit.y) x.y = -INFINITY;
           }
         }
       top[n][0] = fmaxf(fmaxf(s[0][n][0].x, s[0][n][1].x), fmaxf(s[1][n][0].x, s[1][n][1].x));
@@ -428,17 +503,6 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
       raise |= top[n][0] > m[n][0] + 8.0f || top[n][1] > m[n][1] + 8.0f;
     }
     if (__any_sync(~0u, raise)) {
-      float v_keep = 1.0f;
-#pragma unroll
-      for (int x = 4; x < 32; x <<= 1) v_top = fmaxf(v_top, __shfl_xor_sync(~0u, v_top, x));
-      if (v_top > v_limit) {
-        const int now = max(1, min(247, static_cast<int>(__float_as_uint(v_top) >> 23)));
-        v_keep = now - v_exp < 127 ? __uint_as_float(static_cast<uint32_t>(127 + v_exp - now) << 23) : 0.0f;
-        if (v_limit < 0.0f) v_keep = 1.0f;  // no sums yet
-        v_exp = now;
-        v_factor = __uint_as_float(static_cast<uint32_t>(254 - now) << 23);
-        v_limit = __uint_as_float(static_cast<uint32_t>(now + 6) << 23);
-      }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -446,10 +510,9 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(~0u, top[n][e], x));
           const float now = fmaxf(m[n][e], top[n][e]);
-          float keep = now == -INFINITY ? 1.0f : exp2_approx(m[n][e] - now);
+          const float keep = now == -INFINITY ? 1.0f : exp2_approx(m[n][e] - now);
           m[n][e] = now;
           (e ? l[n].y : l[n].x) *= keep;
-          keep *= v_keep;
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) o[j][n][e] *= keep, o[j][n][2 + e] *= keep;
 #pragma unroll
@@ -480,7 +543,7 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
         uint32_t b[kPTerms][NT][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const float2 scale = both(vs[mt][u][k] * v_factor);
+          const float2 scale = both(v_prep[k * kTile + mt * 16 + u * 8 + g]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float2 x = mul2(s[mt][n][u], scale);
@@ -511,8 +574,7 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
             lower[u] = x | y << 16;
             upper[u] = lower[u] >> 8;
           }
-          zero[u] = __byte_perm(vp[tok * kGroups + k], vp[(tok + 1) * kGroups + k], 0x7632);
-          if (!whole) zero[u] &= 0x00FF00FFu;  // places that hold nothing hold any bits
+          zero[u] = *reinterpret_cast<const uint32_t*>(z_prep + k * kTile + tok);
         }
 #pragma unroll
         for (int j = 0; j < G / 16; ++j) {
@@ -581,87 +643,109 @@ __global__ void __launch_bounds__(kWarps * 32, D <= 128 && NT == 1 ? 3 : 1) kv4_
     }
   __syncthreads();
 
-  // the block's rows: straight to the output, or to the workspace for the unit's last block to join
-  auto out_index = [&](int r) {
-    const int rr = tile * kRows + r;
-    return (static_cast<long long>(seq) * a.tq + rr / ratio) * a.hq + head * ratio + rr % ratio;
-  };
-  auto finish = [&](int r, int d, float v, float sum, float now) {
-    store_any(a.ftype, a.out, out_index(r) * D + d, sum > 0.0f ? v / sum : sum == 0.0f ? 0.0f : sum);
-    if (d == 0 && a.lse) a.lse[out_index(r)] = sum > 0.0f ? (now + log2f(sum)) * 0.69314718055994531f : sum == 0.0f ? -INFINITY : sum;
-  };
+  const int parts = plan.parts, unit_tile = plan.tile, unit_rows = min(kRows, a.tq * ratio - unit_tile * kRows);
+  // rows' places in the output, and their maxima and totals
   constexpr int kThreads = kWarps * 32;
-  const int mine_at = (2 * blockIdx.x + (off == 0)) * kRows;
-  for (int i = tid; i < rows * D; i += kThreads) {
-    const int r = i / D, d = i % D;
-    float now = -INFINITY, sum = 0.0f, v = 0.0f;
+  if (tid < kRows) {
+    const int rr = unit_tile * kRows + min(tid, unit_rows - 1);
+    row_out[tid] = (static_cast<int64_t>(plan.unit_seq) * a.tq + rr / ratio) * a.hq + plan.head * ratio + rr % ratio;
+    float now = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) now = fmaxf(now, row_ml[(w * kRows + r) * 2]);
+    for (int w = 0; w < kWarps; ++w) now = fmaxf(now, row_ml[(w * kRows + tid) * 2]);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float mw = row_ml[(w * kRows + r) * 2];
-      sum += mw == -INFINITY ? 0.0f : row_ml[(w * kRows + r) * 2 + 1] * exp2_approx(mw - now);
-      v += sums[(w * kRows + r) * (D + 4) + d];
+      const float mw = row_ml[(w * kRows + tid) * 2];
+      sum += mw == -INFINITY ? 0.0f : row_ml[(w * kRows + tid) * 2 + 1] * exp2_approx(mw - now);
+    }
+    row_all[tid] = make_float2(now, sum);
+  }
+  __syncthreads();
+
+  // the block's rows: straight to the output, or to the workspace for the unit's last block to join
+  auto finish = [&](int r, int d, float4 v) {
+    const float2 ml = row_all[r];
+    const float over = ml.y > 0.0f ? 1.0f / ml.y : 0.0f;  // no tokens: 0
+    const bool sound = ml.y >= 0.0f;                       // else a NaN to hand on
+    v = make_float4(v.x * over, v.y * over, v.z * over, v.w * over);
+    if (!sound) v = make_float4(ml.y, ml.y, ml.y, ml.y);
+    store_four(a.ftype, a.out, row_out[r] * D + d, v);
+    if (d == 0 && a.lse) a.lse[row_out[r]] = ml.y > 0.0f ? (ml.x + log2f(ml.y)) * 0.69314718055994531f : sound ? -INFINITY : ml.y;
+  };
+  const int mine_at = (2 * blockIdx.x + plan.begins) * kRows;
+  for (int i = tid; i < unit_rows * D / 4; i += kThreads) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float4 x = *reinterpret_cast<const float4*>(sums + (w * kRows + r) * (D + 4) + d);
+      v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
     }
     if (parts == 1) {
-      finish(r, d, v, sum, now);
+      finish(r, d, v);
     } else {
-      a.partial[static_cast<size_t>(mine_at + r) * D + d] = v;
-      if (d == 0) {
-        float* ml = a.partial_ml + static_cast<size_t>(mine_at + r) * 2;
-        ml[0] = now;
-        ml[1] = sum;
-      }
+      __stcg(reinterpret_cast<float4*>(a.partial + static_cast<size_t>(mine_at + r) * D + d), v);
+      if (d == 0) __stcg(reinterpret_cast<float2*>(a.partial_ml) + mine_at + r, row_all[r]);
     }
   }
   if (parts > 1) {
     __threadfence();
     __syncthreads();
     if (tid == 0) {
-      arrived = atomicAdd(a.counters + owner, 1u);
-      if (arrived + 1 == static_cast<unsigned>(parts)) a.counters[owner] = 0;  // for the next launch
+      arrived = atomicAdd(a.counters + plan.owner, 1u);
+      if (arrived + 1 == static_cast<unsigned>(parts)) a.counters[plan.owner] = 0;  // for the next launch
     }
     __syncthreads();
     if (arrived + 1 == static_cast<unsigned>(parts)) {
       __threadfence();
+      const int owner = plan.owner;
       // part j lies with block owner + j: the first as the unit begun there, the others as the one begun before
-      auto part_row = [&](int j, int r) { return static_cast<size_t>((2 * (owner + j) + (j == 0)) * kRows + r); };
+      auto part_row = [&](int j, int r) { return static_cast<size_t>(2 * (owner + j) + (j == 0)) * kRows + r; };
+      auto part_four = [&](int j, int r, int d) { return __ldcg(reinterpret_cast<const float4*>(a.partial + part_row(j, r) * D + d)); };
+      constexpr int kFirst = 8;  // parts of the thread's first four that are read along with the maxima
+      float4 first[kFirst];
+#pragma unroll
+      for (int j = 0; j < kFirst; ++j)
+        if (j < parts && tid < unit_rows * D / 4) first[j] = part_four(j, tid / (D / 4), tid % (D / 4) * 4);
       // what each part counts for, [row][part], and the rows' totals
       float* const share = reinterpret_cast<float*>(smem);
-      for (int r = warp; r < rows; r += kWarps) {
-        float now = -INFINITY, sum = 0.0f;
-        for (int j = lane; j < parts; j += 32) now = fmaxf(now, __ldcg(a.partial_ml + part_row(j, r) * 2));
-#pragma unroll
-        for (int x = 16; x; x >>= 1) now = fmaxf(now, __shfl_xor_sync(~0u, now, x));
+      for (int r = warp; r < unit_rows; r += kWarps) {
+        const float2* ml = reinterpret_cast<const float2*>(a.partial_ml);
+        const float2 mine = lane < parts ? __ldcg(ml + part_row(lane, r)) : make_float2(-INFINITY, 0.0f);
+        float now = mine.x, sum = 0.0f;
+        for (int j = lane + 32; j < parts; j += 32) now = fmaxf(now, __ldcg(ml + part_row(j, r)).x);
+        now = warp_max(now);
         for (int j = lane; j < parts; j += 32) {
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.partial_ml + part_row(j, r) * 2));
-          const float keep = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - now);
+          const float2 x = j == lane ? mine : __ldcg(ml + part_row(j, r));
+          const float keep = x.x == -INFINITY ? 0.0f : exp2_approx(x.x - now);
           share[r * parts + j] = keep;
-          sum += keep * ml.y;
+          sum += keep * x.y;
         }
         sum = warp_sum(sum);
-        if (lane == 0) row_ml[2 * r] = now, row_ml[2 * r + 1] = sum;
+        if (lane == 0) row_all[r] = make_float2(now, sum);
       }
       __syncthreads();
-      for (int i = tid; i < rows * D / 4; i += kThreads) {
+      for (int i = tid; i < unit_rows * D / 4; i += kThreads) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (int j = 0; j < parts; ++j) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(a.partial + part_row(j, r) * D + d));
+        auto add = [&](int j, float4 x) {
           const float keep = share[r * parts + j];
           v.x = fmaf(keep, x.x, v.x), v.y = fmaf(keep, x.y, v.y), v.z = fmaf(keep, x.z, v.z), v.w = fmaf(keep, x.w, v.w);
+        };
+        int j0 = 0;
+        if (i == tid) {
+#pragma unroll
+          for (int j = 0; j < kFirst; ++j)
+            if (j < parts) add(j, first[j]);
+          j0 = kFirst;
         }
-        const float now = row_ml[2 * r], sum = row_ml[2 * r + 1];
-        finish(r, d, v.x, sum, now);
-        finish(r, d + 1, v.y, sum, now);
-        finish(r, d + 2, v.z, sum, now);
-        finish(r, d + 3, v.w, sum, now);
+#pragma unroll 8
+        for (int j = j0; j < parts; ++j) add(j, part_four(j, r, d));
+        finish(r, d, v);
       }
     }
   }
+  if (plan.at >= plan.stop) return;
   __syncthreads();  // shared memory is free for the next unit
-  if (at == base + static_cast<long long>(n) * units) base = at, ++seq;
  }
 }
 
