@@ -244,7 +244,7 @@ int launch_attention(const Cache& c, AttnArgs a, int sms, cudaStream_t stream) {
   a.row_tiles = (a.tq * (a.hq / c.heads) + 8 * NT - 1) / (8 * NT);
   // one block for each that the GPU holds at once; fewer when even the longest lengths have fewer steps
   const long long steps = (static_cast<long long>(a.max_pages) * c.page_size + kStepTokens - 1) / kStepTokens;
-  const long long most = static_cast<long long>(a.b) * c.heads * a.row_tiles * std::max(1ll, (steps + kMinSteps - 1) / kMinSteps);
+  const long long most = static_cast<long long>(a.b) * c.heads * a.row_tiles * std::max(1ll, steps);
   if (static_cast<long long>(a.b) * c.heads * a.row_tiles * (steps + kUnitSteps + 1) > 0x7fffffffll)
     return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
   // (a unit's parts, one per block at most, leave their shares in shared memory when they are joined)

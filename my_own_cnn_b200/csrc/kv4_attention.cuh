@@ -59,7 +59,7 @@ struct AttnArgs {
   int* err;
 };
 
-constexpr int kMinSteps = 2;  // steps of a part at least
+constexpr int kMinSteps = 2;  // steps of a unit's first and last part at least
 constexpr int kUnitSteps = 3; // what a unit costs besides its steps (its queries, its first tiles' way, its join), in steps
 
 constexpr int kTile = 32;    // tokens of a warp's step
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
   auto steps_of = [&](int i) { return kUnitSteps + max(1, (valid_length(c, a, i) + kStepTokens - 1) / kStepTokens); };
   // Block i takes total / blocks steps, and one more while i is below the remainder.  A cut that would leave a part of less
   // than kMinSteps steps at a unit's start or end moves there.
-  auto blocks_for = [&](uint32_t total) { return min(gridDim.x, (total + kMinSteps - 1) / kMinSteps); };
+  auto blocks_for = [&](uint32_t total) { return min(gridDim.x, total); };
   {
     uint32_t total = 0;
     for (int i = lane; i < a.b; i += 32) total += steps_of(i);
@@ -245,508 +245,508 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
   }
   __syncthreads();
 
- for (;;) {
-  // steps [off, off + count) of the unit; its first kUnitSteps steps stand for what it costs besides
-  const int seq = plan.seq, len = valid_length(c, a, seq), unit = static_cast<int>((plan.at - plan.base) / plan.n);
-  const uint32_t unit_at = plan.base + unit * plan.n, end = min(unit_at + plan.n, plan.stop);
-  const int off = max(0, static_cast<int>(plan.at - unit_at) - kUnitSteps), count = static_cast<int>(end - unit_at) - kUnitSteps - off;
-  const int tile = unit % a.row_tiles, head = unit / a.row_tiles, rows = min(kRows, a.tq * ratio - tile * kRows);
-  // the query rows are on their way first, in their own type
-  constexpr int kPer = D / 32, kRowsWarp = kRows / kWarps;
-  using Raw = std::conditional_t<F32, float, uint16_t>;
-  Raw q[kRowsWarp][kPer];
+  for (;;) {
+    // steps [off, off + count) of the unit; its first kUnitSteps steps stand for what it costs besides
+    const int seq = plan.seq, len = valid_length(c, a, seq), unit = static_cast<int>((plan.at - plan.base) / plan.n);
+    const uint32_t unit_at = plan.base + unit * plan.n, end = min(unit_at + plan.n, plan.stop);
+    const int off = max(0, static_cast<int>(plan.at - unit_at) - kUnitSteps), count = static_cast<int>(end - unit_at) - kUnitSteps - off;
+    const int tile = unit % a.row_tiles, head = unit / a.row_tiles, rows = min(kRows, a.tq * ratio - tile * kRows);
+    // the query rows are on their way first, in their own type
+    constexpr int kPer = D / 32, kRowsWarp = kRows / kWarps;
+    using Raw = std::conditional_t<F32, float, uint16_t>;
+    Raw q[kRowsWarp][kPer];
 #pragma unroll
-  for (int j = 0; j < kRowsWarp; ++j) {
-    const int r = warp + j * kWarps, rr = tile * kRows + r;
-    const Raw* from = static_cast<const Raw*>(a.q) + seq * a.q_bs + (rr / ratio) * a.q_ts + (head * ratio + rr % ratio) * a.q_hs + lane;
+    for (int j = 0; j < kRowsWarp; ++j) {
+      const int r = warp + j * kWarps, rr = tile * kRows + r;
+      const Raw* from = static_cast<const Raw*>(a.q) + seq * a.q_bs + (rr / ratio) * a.q_ts + (head * ratio + rr % ratio) * a.q_hs + lane;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) q[j][i] = r < rows ? __ldg(from + 32 * i) : Raw(0);  // channel 32 i + lane
-  }
-  __syncthreads();
-  if (tid == kWarps * 32 - 1) {
-    // the cuts inside the unit, and the block that its first part lies with: the one after the last cut before them
-    const uint32_t total = plan.total, blocks = blocks_for(total), per = total / blocks, more = total - per * blocks;
-    auto cuts_to = [&](uint32_t step) {  // how many cuts lie at or before `step`
-      const uint32_t longer = more * (per + 1);
-      return step < longer ? step / (per + 1) + 1 : more + (step - longer) / per + 1;
+      for (int i = 0; i < kPer; ++i) q[j][i] = r < rows ? __ldg(from + 32 * i) : Raw(0);  // channel 32 i + lane
+    }
+    __syncthreads();
+    if (tid == kWarps * 32 - 1) {
+      // the cuts inside the unit, and the block that its first part lies with: the one after the last cut before them
+      const uint32_t total = plan.total, blocks = blocks_for(total), per = total / blocks, more = total - per * blocks;
+      auto cuts_to = [&](uint32_t step) {  // how many cuts lie at or before `step`
+        const uint32_t longer = more * (per + 1);
+        return step < longer ? step / (per + 1) + 1 : more + (step - longer) / per + 1;
+      };
+      const uint32_t before = cuts_to(unit_at + kUnitSteps + kMinSteps - 1);
+      plan.owner = static_cast<int>(before) - 1;
+      plan.parts = plan.n >= kUnitSteps + 2 * kMinSteps ? 1 + static_cast<int>(cuts_to(unit_at + plan.n - kMinSteps) - before) : 1;
+      plan.unit_seq = seq;
+      plan.head = head;
+      plan.tile = tile;
+      plan.begins = off == 0;
+      plan.at = end;
+      if (end == plan.base + static_cast<uint32_t>(plan.n) * units && end < plan.stop) {
+        plan.base = end;
+        plan.n = steps_of(++plan.seq);
+      }
+    }
+    // the last row of the tile sees the most tokens
+    const int seen = max(0, len - a.tq + (tile * kRows + rows - 1) / ratio + 1);
+    const int begin = off * kStepTokens, until = min(seen, begin + count * kStepTokens);
+    const int32_t* pages = a.table + seq * a.table_stride;
+
+    // ring: the first tiles are on their way before the query is looked at
+    const uint32_t ring = shared_address(smem) + warp * (kStages * Shape::kStage);
+    const int tiles = max(0, (until - begin + kTile - 1) / kTile);
+    const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+    // this lane's token of the warp's tile i, or the tile's first where its tokens lie in one page: first + i * step
+    const bool paged = c.page_size % kTile == 0;
+    const int first = begin + warp * kTile + (paged ? 0 : lane);
+    constexpr int kStep = kWarps * kTile;
+    uint32_t held[kStages];  // which tokens of the tiles on their way are there
+    uint32_t row = token_row(c, a, pages, head, first, until);
+    auto load = [&](int i, uint32_t stage, bool ok) {  // tile i, whose row was looked up; the tokens that are there
+      if (paged) {
+        const int n = row == ~0u ? 0 : min(kTile, until - first - i * kStep);
+        if (ok) load_tile_page<D, G>(c, stage, row, n, lane);
+        return n >= kTile ? ~0u : (1u << max(0, n)) - 1;
+      }
+      const uint32_t there = __ballot_sync(~0u, row != ~0u);
+      if (ok) load_tile<D, G>(c, stage, row, lane);
+      return there;
     };
-    const uint32_t before = cuts_to(unit_at + kUnitSteps + kMinSteps - 1);
-    plan.owner = static_cast<int>(before) - 1;
-    plan.parts = plan.n >= kUnitSteps + 2 * kMinSteps ? 1 + static_cast<int>(cuts_to(unit_at + plan.n - kMinSteps) - before) : 1;
-    plan.unit_seq = seq;
-    plan.head = head;
-    plan.tile = tile;
-    plan.begins = off == 0;
-    plan.at = end;
-    if (end == plan.base + static_cast<uint32_t>(plan.n) * units && end < plan.stop) {
-      plan.base = end;
-      plan.n = steps_of(++plan.seq);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      held[i] = load(i, ring + i * Shape::kStage, i < mine);
+      copy_commit();
+      row = token_row(c, a, pages, head, first + (i + 1) * kStep, until);
     }
-  }
-  // the last row of the tile sees the most tokens
-  const int seen = max(0, len - a.tq + (tile * kRows + rows - 1) / ratio + 1);
-  const int begin = off * kStepTokens, until = min(seen, begin + count * kStepTokens);
-  const int32_t* pages = a.table + seq * a.table_stride;
 
-  // ring: the first tiles are on their way before the query is looked at
-  const uint32_t ring = shared_address(smem) + warp * (kStages * Shape::kStage);
-  const int tiles = max(0, (until - begin + kTile - 1) / kTile);
-  const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
-  // this lane's token of the warp's tile i, or the tile's first where its tokens lie in one page: first + i * step
-  const bool paged = c.page_size % kTile == 0;
-  const int first = begin + warp * kTile + (paged ? 0 : lane);
-  constexpr int kStep = kWarps * kTile;
-  uint32_t held[kStages];  // which tokens of the tiles on their way are there
-  uint32_t row = token_row(c, a, pages, head, first, until);
-  auto load = [&](int i, uint32_t stage, bool ok) {  // tile i, whose row was looked up; the tokens that are there
-    if (paged) {
-      const int n = row == ~0u ? 0 : min(kTile, until - first - i * kStep);
-      if (ok) load_tile_page<D, G>(c, stage, row, n, lane);
-      return n >= kTile ? ~0u : (1u << max(0, n)) - 1;
-    }
-    const uint32_t there = __ballot_sync(~0u, row != ~0u);
-    if (ok) load_tile<D, G>(c, stage, row, lane);
-    return there;
-  };
+    // query rows: scaled to fp16, laid out as operand B
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    held[i] = load(i, ring + i * Shape::kStage, i < mine);
-    copy_commit();
-    row = token_row(c, a, pages, head, first + (i + 1) * kStep, until);
-  }
-
-  // query rows: scaled to fp16, laid out as operand B
+    for (int j = 0; j < kRowsWarp; ++j) {
+      const int r = warp + j * kWarps;
+      float v[kPer], top = 0.0f;
 #pragma unroll
-  for (int j = 0; j < kRowsWarp; ++j) {
-    const int r = warp + j * kWarps;
-    float v[kPer], top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if constexpr (F32)
-        v[i] = q[j][i];
-      else
-        v[i] = a.ftype == B200Q_F16 ? __half2float(__ushort_as_half(q[j][i])) : __uint_as_float(static_cast<uint32_t>(q[j][i]) << 16);
-      top = fmaxf(top, fabsf(v[i]));
-    }
-    const Power power = power_for(warp_max(top));
-    if (lane == 0) {
-      row_f[r] = power.down * a.scale * 1.4426950408889634f * 16777216.0f;
-      row_limit[r] = len - a.tq + (tile * kRows + min(r, rows - 1)) / ratio + 1;
-    }
-    // lane: channel p = lane % 8 of the 8 that thread lane / 8 of a quad holds; pairs are (0,4) (1,5) (2,6) (3,7)
-    const int p = lane % 8, holder = (r % 8) * 4 + lane / 8;
-    __half* to = reinterpret_cast<__half*>(query);
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      float x = v[i] * power.up;
-#pragma unroll
-      for (int term = 0; term < kTerms; ++term) {
-        const __half hv = __float2half_rn(x);
-        const float back = __half2float(hv);
-        sum += back;
-        x -= back;
-        to[(((i * kTerms + term) * NT + r / 8) * 32 + holder) * 8 + (p % 4) * 2 + p / 4] =
-            p % 2 ? __float2half_rn(back * 0.0625f) : hv;
+      for (int i = 0; i < kPer; ++i) {
+        if constexpr (F32)
+          v[i] = q[j][i];
+        else
+          v[i] = a.ftype == B200Q_F16 ? __half2float(__ushort_as_half(q[j][i])) : __uint_as_float(static_cast<uint32_t>(q[j][i]) << 16);
+        top = fmaxf(top, fabsf(v[i]));
       }
-      if ((i + 1) % (G / 32) == 0) {
-        sum = warp_sum(sum);
-        if (lane == 0) row_sum[(i / (G / 32)) * kRows + r] = sum * (1.0f / 16777216.0f);
-        sum = 0.0f;
+      const Power power = power_for(warp_max(top));
+      if (lane == 0) {
+        row_f[r] = power.down * a.scale * 1.4426950408889634f * 16777216.0f;
+        row_limit[r] = len - a.tq + (tile * kRows + min(r, rows - 1)) / ratio + 1;
+      }
+      // lane: channel p = lane % 8 of the 8 that thread lane / 8 of a quad holds; pairs are (0,4) (1,5) (2,6) (3,7)
+      const int p = lane % 8, holder = (r % 8) * 4 + lane / 8;
+      __half* to = reinterpret_cast<__half*>(query);
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        float x = v[i] * power.up;
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) {
+          const __half hv = __float2half_rn(x);
+          const float back = __half2float(hv);
+          sum += back;
+          x -= back;
+          to[(((i * kTerms + term) * NT + r / 8) * 32 + holder) * 8 + (p % 4) * 2 + p / 4] =
+              p % 2 ? __float2half_rn(back * 0.0625f) : hv;
+        }
+        if ((i + 1) % (G / 32) == 0) {
+          sum = warp_sum(sum);
+          if (lane == 0) row_sum[(i / (G / 32)) * kRows + r] = sum * (1.0f / 16777216.0f);
+          sum = 0.0f;
+        }
       }
     }
-  }
-  __syncthreads();
+    __syncthreads();
 
-  // this lane's columns: rows 2t, 2t + 1 of each 8
-  float2 l[NT];
-  float m[NT][2];
+    // this lane's columns: rows 2t, 2t + 1 of each 8
+    float2 l[NT];
+    float m[NT][2];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n] = both(0.0f);
-  }
-  const int all_see = len - a.tq + tile * kRows / ratio + 1;  // tokens that every row of the tile sees
-  float o[D / 16][NT][4], z[kGroups][NT][4];
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n] = both(0.0f);
+    }
+    const int all_see = len - a.tq + tile * kRows / ratio + 1;  // tokens that every row of the tile sees
+    float o[D / 16][NT][4], z[kGroups][NT][4];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.0f;
+      for (int j = 0; j < D / 16; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j) z[j][n][0] = z[j][n][1] = z[j][n][2] = z[j][n][3] = 0.0f;
-  }
+      for (int j = 0; j < kGroups; ++j) z[j][n][0] = z[j][n][1] = z[j][n][2] = z[j][n][3] = 0.0f;
+    }
 
-  // P's power of two: 2^(127 - v_exp), for a largest vs of 2^(v_exp - 127)
-  int v_exp = 127;
-  float v_factor = 1.0f, v_limit = -1.0f;
-  int slot = 0, fill = kStages - 1;
-  for (int it = 0; it < mine; ++it) {
-    copy_wait<kStages - 2>();
-    __syncwarp();
-    held[kStages - 1] = load(it + kStages - 1, ring + fill * Shape::kStage, it + kStages - 1 < mine);
-    copy_commit();
-    row = token_row(c, a, pages, head, first + (it + kStages) * kStep, until);
-    const uint8_t* stage = smem + warp * (kStages * Shape::kStage) + slot * Shape::kStage;
-    const uint8_t* kc = stage;
-    const uint8_t* vc = stage + Shape::kCodes;
-    const uint32_t* kp = reinterpret_cast<const uint32_t*>(stage + 2 * Shape::kCodes);
-    const uint32_t* vp = kp + kTile * kGroups;
-    const uint32_t here = held[0];
-    const int base = begin + (it * kWarps + warp) * kTile;
-    const bool whole = here == ~0u && base + kTile <= all_see;
+    // P's power of two: 2^(127 - v_exp), for a largest vs of 2^(v_exp - 127)
+    int v_exp = 127;
+    float v_factor = 1.0f, v_limit = -1.0f;
+    int slot = 0, fill = kStages - 1;
+    for (int it = 0; it < mine; ++it) {
+      copy_wait<kStages - 2>();
+      __syncwarp();
+      held[kStages - 1] = load(it + kStages - 1, ring + fill * Shape::kStage, it + kStages - 1 < mine);
+      copy_commit();
+      row = token_row(c, a, pages, head, first + (it + kStages) * kStep, until);
+      const uint8_t* stage = smem + warp * (kStages * Shape::kStage) + slot * Shape::kStage;
+      const uint8_t* kc = stage;
+      const uint8_t* vc = stage + Shape::kCodes;
+      const uint32_t* kp = reinterpret_cast<const uint32_t*>(stage + 2 * Shape::kCodes);
+      const uint32_t* vp = kp + kTile * kGroups;
+      const uint32_t here = held[0];
+      const int base = begin + (it * kWarps + warp) * kTile;
+      const bool whole = here == ~0u && base + kTile <= all_see;
 
-    // lane l unpacks token l's scales and zero points for the lanes that use them: [group][token] (key scale, key zero
-    // point negated), then value scales times P's power, then value zero points as fp16 bits
-    float2* const k_prep = reinterpret_cast<float2*>(prepared);
-    float* const v_prep = reinterpret_cast<float*>(prepared + kTile * kGroups * 8);
-    uint16_t* const z_prep = reinterpret_cast<uint16_t*>(prepared + kTile * kGroups * 12);
-    {
-      float vs[kGroups], v_top = 0.0f;
-      const bool there = here >> lane & 1;
+      // lane l unpacks token l's scales and zero points for the lanes that use them: [group][token] (key scale, key zero
+      // point negated), then value scales times P's power, then value zero points as fp16 bits
+      float2* const k_prep = reinterpret_cast<float2*>(prepared);
+      float* const v_prep = reinterpret_cast<float*>(prepared + kTile * kGroups * 8);
+      uint16_t* const z_prep = reinterpret_cast<uint16_t*>(prepared + kTile * kGroups * 12);
+      {
+        float vs[kGroups], v_top = 0.0f;
+        const bool there = here >> lane & 1;
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+          const uint32_t p = kp[lane * kGroups + k], q = there ? vp[lane * kGroups + k] : 0u;  // places that hold nothing hold any bits
+          k_prep[k * kTile + lane] = make_float2(param_scale(p), -zero_point(p));
+          z_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 16);
+          vs[k] = param_scale(q);
+          v_top = fmaxf(v_top, vs[k]);
+        }
+        if (__any_sync(~0u, v_top > v_limit)) {
+          const int now = max(1, min(247, static_cast<int>(__float_as_uint(warp_max(v_top)) >> 23)));
+          float keep = now - v_exp < 127 ? __uint_as_float(static_cast<uint32_t>(127 + v_exp - now) << 23) : 0.0f;
+          if (v_limit < 0.0f) keep = 1.0f;  // no sums yet
+          v_exp = now;
+          v_factor = __uint_as_float(static_cast<uint32_t>(254 - now) << 23);
+          v_limit = __uint_as_float(static_cast<uint32_t>(now + 6) << 23);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+              for (int j = 0; j < D / 16; ++j) o[j][n][e] *= keep;
+#pragma unroll
+              for (int j = 0; j < kGroups; ++j) z[j][n][e] *= keep;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) v_prep[k * kTile + lane] = vs[k] * v_factor;
+      }
+      __syncwarp();
+
+      // scores
+      float2 s[2][NT][2];  // [tokens g, g + 8], rows 2t and 2t + 1
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) {
-        const uint32_t p = kp[lane * kGroups + k], q = there ? vp[lane * kGroups + k] : 0u;  // places that hold nothing hold any bits
-        k_prep[k * kTile + lane] = make_float2(param_scale(p), -zero_point(p));
-        z_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 16);
-        vs[k] = param_scale(q);
-        v_top = fmaxf(v_top, vs[k]);
-      }
-      if (__any_sync(~0u, v_top > v_limit)) {
-        const int now = max(1, min(247, static_cast<int>(__float_as_uint(warp_max(v_top)) >> 23)));
-        float keep = now - v_exp < 127 ? __uint_as_float(static_cast<uint32_t>(127 + v_exp - now) << 23) : 0.0f;
-        if (v_limit < 0.0f) keep = 1.0f;  // no sums yet
-        v_exp = now;
-        v_factor = __uint_as_float(static_cast<uint32_t>(254 - now) << 23);
-        v_limit = __uint_as_float(static_cast<uint32_t>(now + 6) << 23);
+        float part[2][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j) o[j][n][e] *= keep;
-#pragma unroll
-            for (int j = 0; j < kGroups; ++j) z[j][n][e] *= keep;
-          }
-      }
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k) v_prep[k * kTile + lane] = vs[k] * v_factor;
-    }
-    __syncwarp();
-
-    // scores
-    float2 s[2][NT][2];  // [tokens g, g + 8], rows 2t and 2t + 1
-#pragma unroll
-    for (int k = 0; k < kGroups; ++k) {
-      float part[2][NT][4];
-#pragma unroll
-      for (int i = k * (G / 32); i < (k + 1) * (G / 32); ++i) {
-        uint4 b[kTerms][NT];
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) b[term][n] = query[((i * kTerms + term) * NT + n) * 32 + lane];
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(kc + (mt * 16 + g) * kPitch + 16 * i + 4 * t);
-          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(kc + (mt * 16 + g + 8) * kPitch + 16 * i + 4 * t);
-          const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
+        for (int i = k * (G / 32); i < (k + 1) * (G / 32); ++i) {
+          uint4 b[kTerms][NT];
 #pragma unroll
           for (int term = 0; term < kTerms; ++term)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              if (i == k * (G / 32) && term == 0)
-                mma_f16_first(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
-                              b[term][n].x, b[term][n].y);
-              else
-                mma_f16(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
-                        b[term][n].x, b[term][n].y);
-              mma_f16(part[mt][n], v0 & 0x000F000Fu, v1 & 0x000F000Fu, v0 & 0x00F000F0u, v1 & 0x00F000F0u,
-                      b[term][n].z, b[term][n].w);
-            }
+            for (int n = 0; n < NT; ++n) b[term][n] = query[((i * kTerms + term) * NT + n) * 32 + lane];
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(kc + (mt * 16 + g) * kPitch + 16 * i + 4 * t);
+            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(kc + (mt * 16 + g + 8) * kPitch + 16 * i + 4 * t);
+            const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
+#pragma unroll
+            for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                if (i == k * (G / 32) && term == 0)
+                  mma_f16_first(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
+                                b[term][n].x, b[term][n].y);
+                else
+                  mma_f16(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
+                          b[term][n].x, b[term][n].y);
+                mma_f16(part[mt][n], v0 & 0x000F000Fu, v1 & 0x000F000Fu, v0 & 0x00F000F0u, v1 & 0x00F000F0u,
+                        b[term][n].z, b[term][n].w);
+              }
+          }
         }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float2 p = k_prep[k * kTile + mt * 16 + u * 8 + g];
+            const float2 ks = both(p.x), kz = both(p.y);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const float* at = part[mt][n] + 2 * u;
+              const float2 v = fma2(kz, *reinterpret_cast<const float2*>(row_sum + k * kRows + n * 8 + 2 * t), make_float2(at[0], at[1]));
+              s[mt][n][u] = k == 0 ? mul2(ks, v) : fma2(ks, v, s[mt][n][u]);
+            }
+          }
+      }
+
+      // weights
+      bool raise = false;
+      float top[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float2& x = s[mt][n][u];
+            x = mul2(x, *reinterpret_cast<const float2*>(row_f + n * 8 + 2 * t));
+            if (!whole) {
+              const int tok = mt * 16 + u * 8 + g;
+              const int2 limit = *reinterpret_cast<const int2*>(row_limit + n * 8 + 2 * t);
+              if (!(here >> tok & 1) || base + tok >= limit.x) x.x = -INFINITY;
+              if (!(here >> tok & 1) || base + tok >= limit.y) x.y = -INFINITY;
+            }
+          }
+        top[n][0] = fmaxf(fmaxf(s[0][n][0].x, s[0][n][1].x), fmaxf(s[1][n][0].x, s[1][n][1].x));
+        top[n][1] = fmaxf(fmaxf(s[0][n][0].y, s[0][n][1].y), fmaxf(s[1][n][0].y, s[1][n][1].y));
+        raise |= top[n][0] > m[n][0] + 8.0f || top[n][1] > m[n][1] + 8.0f;
+      }
+      if (__any_sync(~0u, raise)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(~0u, top[n][e], x));
+            const float now = fmaxf(m[n][e], top[n][e]);
+            const float keep = now == -INFINITY ? 1.0f : exp2_approx(m[n][e] - now);
+            m[n][e] = now;
+            (e ? l[n].y : l[n].x) *= keep;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) o[j][n][e] *= keep, o[j][n][2 + e] *= keep;
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j) z[j][n][e] *= keep, z[j][n][2 + e] *= keep;
+          }
       }
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int n = 0; n < NT; ++n) {
+        const float2 ref = make_float2(m[n][0] == -INFINITY ? 0.0f : -m[n][0], m[n][1] == -INFINITY ? 0.0f : -m[n][1]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float2 p = k_prep[k * kTile + mt * 16 + u * 8 + g];
-          const float2 ks = both(p.x), kz = both(p.y);
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const float* at = part[mt][n] + 2 * u;
-            const float2 v = fma2(kz, *reinterpret_cast<const float2*>(row_sum + k * kRows + n * 8 + 2 * t), make_float2(at[0], at[1]));
-            s[mt][n][u] = k == 0 ? mul2(ks, v) : fma2(ks, v, s[mt][n][u]);
+          for (int u = 0; u < 2; ++u) {
+            float2& x = s[mt][n][u];
+            x = add2(x, ref);
+            x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+            l[n] = add2(l[n], x);
           }
-        }
-    }
+      }
 
-    // weights
-    bool raise = false;
-    float top[NT][2];
+      // values
+      constexpr int kPTerms = F32 ? 2 : 1;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+      for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+        for (int k = 0; k < kGroups; ++k) {
+          // operand B: P of this group, as (row g, tokens 2t, 2t + 1) of each 8 tokens
+          uint32_t b[kPTerms][NT][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float2& x = s[mt][n][u];
-          x = mul2(x, *reinterpret_cast<const float2*>(row_f + n * 8 + 2 * t));
-          if (!whole) {
-            const int tok = mt * 16 + u * 8 + g;
-            const int2 limit = *reinterpret_cast<const int2*>(row_limit + n * 8 + 2 * t);
-            if (!(here >> tok & 1) || base + tok >= limit.x) x.x = -INFINITY;
-            if (!(here >> tok & 1) || base + tok >= limit.y) x.y = -INFINITY;
-          }
-        }
-      top[n][0] = fmaxf(fmaxf(s[0][n][0].x, s[0][n][1].x), fmaxf(s[1][n][0].x, s[1][n][1].x));
-      top[n][1] = fmaxf(fmaxf(s[0][n][0].y, s[0][n][1].y), fmaxf(s[1][n][0].y, s[1][n][1].y));
-      raise |= top[n][0] > m[n][0] + 8.0f || top[n][1] > m[n][1] + 8.0f;
-    }
-    if (__any_sync(~0u, raise)) {
+          for (int u = 0; u < 2; ++u) {
+            const float2 scale = both(v_prep[k * kTile + mt * 16 + u * 8 + g]);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
+              float2 x = mul2(s[mt][n][u], scale);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top[n][e] = fmaxf(top[n][e], __shfl_xor_sync(~0u, top[n][e], x));
-          const float now = fmaxf(m[n][e], top[n][e]);
-          const float keep = now == -INFINITY ? 1.0f : exp2_approx(m[n][e] - now);
-          m[n][e] = now;
-          (e ? l[n].y : l[n].x) *= keep;
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j) o[j][n][e] *= keep, o[j][n][2 + e] *= keep;
-#pragma unroll
-          for (int j = 0; j < kGroups; ++j) z[j][n][e] *= keep, z[j][n][2 + e] *= keep;
-        }
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float2 ref = make_float2(m[n][0] == -INFINITY ? 0.0f : -m[n][0], m[n][1] == -INFINITY ? 0.0f : -m[n][1]);
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float2& x = s[mt][n][u];
-          x = add2(x, ref);
-          x = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-          l[n] = add2(l[n], x);
-        }
-    }
-
-    // values
-    constexpr int kPTerms = F32 ? 2 : 1;
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k) {
-        // operand B: P of this group, as (row g, tokens 2t, 2t + 1) of each 8 tokens
-        uint32_t b[kPTerms][NT][2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float2 scale = both(v_prep[k * kTile + mt * 16 + u * 8 + g]);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float2 x = mul2(s[mt][n][u], scale);
-#pragma unroll
-            for (int term = 0; term < kPTerms; ++term) {
-              const uint32_t v = pack_f16(x.x, x.y);
-              if (term + 1 < kPTerms) {
-                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&v));
-                x = make_float2(x.x - back.x, x.y - back.y);
+              for (int term = 0; term < kPTerms; ++term) {
+                const uint32_t v = pack_f16(x.x, x.y);
+                if (term + 1 < kPTerms) {
+                  const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                  x = make_float2(x.x - back.x, x.y - back.y);
+                }
+                b[term][n][u] = transpose_8x8(v);
               }
-              b[term][n][u] = transpose_8x8(v);
             }
           }
-        }
-        // operand A: tokens 2t, 2t + 1 (u = 0) and 2t + 8, 2t + 9 (u = 1) of this lane's G / 8 channels, the lower
-        // half of them as row g of the group's G / 16 products, the upper as row g + 8
-        uint32_t lower[2], upper[2], zero[2];
+          // operand A: tokens 2t, 2t + 1 (u = 0) and 2t + 8, 2t + 9 (u = 1) of this lane's G / 8 channels, the lower
+          // half of them as row g of the group's G / 16 products, the upper as row g + 8
+          uint32_t lower[2], upper[2], zero[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int tok = mt * 16 + u * 8 + 2 * t;
-          const uint8_t* at = vc + tok * kPitch + k * (G / 2) + g * (G / 16);
-          if constexpr (G == 64) {
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(at), y = *reinterpret_cast<const uint32_t*>(at + kPitch);
-            lower[u] = __byte_perm(x, y, 0x5410);
-            upper[u] = __byte_perm(x, y, 0x7632);
-          } else {
-            const uint32_t x = *reinterpret_cast<const uint16_t*>(at), y = *reinterpret_cast<const uint16_t*>(at + kPitch);
-            lower[u] = x | y << 16;
-            upper[u] = lower[u] >> 8;
+          for (int u = 0; u < 2; ++u) {
+            const int tok = mt * 16 + u * 8 + 2 * t;
+            const uint8_t* at = vc + tok * kPitch + k * (G / 2) + g * (G / 16);
+            if constexpr (G == 64) {
+              const uint32_t x = *reinterpret_cast<const uint32_t*>(at), y = *reinterpret_cast<const uint32_t*>(at + kPitch);
+              lower[u] = __byte_perm(x, y, 0x5410);
+              upper[u] = __byte_perm(x, y, 0x7632);
+            } else {
+              const uint32_t x = *reinterpret_cast<const uint16_t*>(at), y = *reinterpret_cast<const uint16_t*>(at + kPitch);
+              lower[u] = x | y << 16;
+              upper[u] = lower[u] >> 8;
+            }
+            zero[u] = *reinterpret_cast<const uint32_t*>(z_prep + k * kTile + tok);
           }
-          zero[u] = *reinterpret_cast<const uint32_t*>(z_prep + k * kTile + tok);
-        }
 #pragma unroll
-        for (int j = 0; j < G / 16; ++j) {
-          const int down = j / 2 * 8;
-          const uint32_t mask = j % 2 ? 0x00F000F0u : 0x000F000Fu;
-          const uint32_t a0 = lower[0] >> down & mask, a1 = upper[0] >> down & mask;
-          const uint32_t a2 = lower[1] >> down & mask, a3 = upper[1] >> down & mask;
+          for (int j = 0; j < G / 16; ++j) {
+            const int down = j / 2 * 8;
+            const uint32_t mask = j % 2 ? 0x00F000F0u : 0x000F000Fu;
+            const uint32_t a0 = lower[0] >> down & mask, a1 = upper[0] >> down & mask;
+            const uint32_t a2 = lower[1] >> down & mask, a3 = upper[1] >> down & mask;
+#pragma unroll
+            for (int term = 0; term < kPTerms; ++term)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_f16(o[k * (G / 16) + j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
+          }
 #pragma unroll
           for (int term = 0; term < kPTerms; ++term)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(o[k * (G / 16) + j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
+            for (int n = 0; n < NT; ++n) mma_f16(z[k][n], zero[0], zero[0], zero[1], zero[1], b[term][n][0], b[term][n][1]);
         }
-#pragma unroll
-        for (int term = 0; term < kPTerms; ++term)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma_f16(z[k][n], zero[0], zero[0], zero[1], zero[1], b[term][n][0], b[term][n][1]);
       }
-    }
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) held[i] = held[i + 1];
-    slot = slot + 1 == kStages ? 0 : slot + 1;
-    fill = fill + 1 == kStages ? 0 : fill + 1;
-  }
+      for (int i = 0; i < kStages - 1; ++i) held[i] = held[i + 1];
+      slot = slot + 1 == kStages ? 0 : slot + 1;
+      fill = fill + 1 == kStages ? 0 : fill + 1;
+    }
 
-  // join the warps: maxima and totals, then the sums through shared memory (the rings are done with)
+    // join the warps: maxima and totals, then the sums through shared memory (the rings are done with)
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float all = e ? l[n].y : l[n].x;
+      for (int e = 0; e < 2; ++e) {
+        float all = e ? l[n].y : l[n].x;
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) all += __shfl_xor_sync(~0u, all, x);
-      if (g == 0) {
-        float* ml = row_ml + (warp * kRows + n * 8 + 2 * t + e) * 2;
-        ml[0] = m[n][e];
-        ml[1] = all;
-      }
-    }
-  copy_wait<0>();
-  __syncthreads();
-  float* const sums = reinterpret_cast<float*>(smem);  // [kWarps][kRows][D + 4]
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = n * 8 + 2 * t + e;
-      float now = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) now = fmaxf(now, row_ml[(w * kRows + r) * 2]);
-      const float keep = m[n][e] == -INFINITY ? 0.0f : exp2_approx(m[n][e] - now);
-      const float value = __uint_as_float(static_cast<uint32_t>(v_exp) << 23);
-      float* to = sums + (warp * kRows + r) * (D + 4);
-#pragma unroll
-      for (int k = 0; k < kGroups; ++k)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float v[G / 16];
-#pragma unroll
-          for (int j = 0; j < G / 16; ++j) v[j] = fmaf(o[k * (G / 16) + j][n][2 * u + e], j % 2 ? 0.0625f : 1.0f, -z[k][n][2 * u + e]) * 16777216.0f * value * keep;
-          float* p = to + k * G + g * (G / 8) + u * (G / 16);
-          if constexpr (G == 64)
-            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-          else
-            *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+        for (int x = 4; x < 32; x <<= 1) all += __shfl_xor_sync(~0u, all, x);
+        if (g == 0) {
+          float* ml = row_ml + (warp * kRows + n * 8 + 2 * t + e) * 2;
+          ml[0] = m[n][e];
+          ml[1] = all;
         }
-    }
-  __syncthreads();
-
-  const int parts = plan.parts, unit_tile = plan.tile, unit_rows = min(kRows, a.tq * ratio - unit_tile * kRows);
-  // rows' places in the output, and their maxima and totals
-  constexpr int kThreads = kWarps * 32;
-  if (tid < kRows) {
-    const int rr = unit_tile * kRows + min(tid, unit_rows - 1);
-    row_out[tid] = (static_cast<int64_t>(plan.unit_seq) * a.tq + rr / ratio) * a.hq + plan.head * ratio + rr % ratio;
-    float now = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) now = fmaxf(now, row_ml[(w * kRows + tid) * 2]);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float mw = row_ml[(w * kRows + tid) * 2];
-      sum += mw == -INFINITY ? 0.0f : row_ml[(w * kRows + tid) * 2 + 1] * exp2_approx(mw - now);
-    }
-    row_all[tid] = make_float2(now, sum);
-  }
-  __syncthreads();
-
-  // the block's rows: straight to the output, or to the workspace for the unit's last block to join
-  auto finish = [&](int r, int d, float4 v) {
-    const float2 ml = row_all[r];
-    const float over = ml.y > 0.0f ? 1.0f / ml.y : 0.0f;  // no tokens: 0
-    const bool sound = ml.y >= 0.0f;                       // else a NaN to hand on
-    v = make_float4(v.x * over, v.y * over, v.z * over, v.w * over);
-    if (!sound) v = make_float4(ml.y, ml.y, ml.y, ml.y);
-    store_four(a.ftype, a.out, row_out[r] * D + d, v);
-    if (d == 0 && a.lse) a.lse[row_out[r]] = ml.y > 0.0f ? (ml.x + log2f(ml.y)) * 0.69314718055994531f : sound ? -INFINITY : ml.y;
-  };
-  const int mine_at = (2 * blockIdx.x + plan.begins) * kRows;
-  for (int i = tid; i < unit_rows * D / 4; i += kThreads) {
-    const int r = i / (D / 4), d = i % (D / 4) * 4;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float4 x = *reinterpret_cast<const float4*>(sums + (w * kRows + r) * (D + 4) + d);
-      v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-    }
-    if (parts == 1) {
-      finish(r, d, v);
-    } else {
-      __stcg(reinterpret_cast<float4*>(a.partial + static_cast<size_t>(mine_at + r) * D + d), v);
-      if (d == 0) __stcg(reinterpret_cast<float2*>(a.partial_ml) + mine_at + r, row_all[r]);
-    }
-  }
-  if (parts > 1) {
-    __threadfence();
+      }
+    copy_wait<0>();
     __syncthreads();
-    if (tid == 0) {
-      arrived = atomicAdd(a.counters + plan.owner, 1u);
-      if (arrived + 1 == static_cast<unsigned>(parts)) a.counters[plan.owner] = 0;  // for the next launch
+    float* const sums = reinterpret_cast<float*>(smem);  // [kWarps][kRows][D + 4]
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = n * 8 + 2 * t + e;
+        float now = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) now = fmaxf(now, row_ml[(w * kRows + r) * 2]);
+        const float keep = m[n][e] == -INFINITY ? 0.0f : exp2_approx(m[n][e] - now);
+        const float value = __uint_as_float(static_cast<uint32_t>(v_exp) << 23);
+        float* to = sums + (warp * kRows + r) * (D + 4);
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float v[G / 16];
+#pragma unroll
+            for (int j = 0; j < G / 16; ++j) v[j] = fmaf(o[k * (G / 16) + j][n][2 * u + e], j % 2 ? 0.0625f : 1.0f, -z[k][n][2 * u + e]) * 16777216.0f * value * keep;
+            float* p = to + k * G + g * (G / 8) + u * (G / 16);
+            if constexpr (G == 64)
+              *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+            else
+              *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+          }
+      }
+    __syncthreads();
+
+    const int parts = plan.parts, unit_tile = plan.tile, unit_rows = min(kRows, a.tq * ratio - unit_tile * kRows);
+    // rows' places in the output, and their maxima and totals
+    constexpr int kThreads = kWarps * 32;
+    if (tid < kRows) {
+      const int rr = unit_tile * kRows + min(tid, unit_rows - 1);
+      row_out[tid] = (static_cast<int64_t>(plan.unit_seq) * a.tq + rr / ratio) * a.hq + plan.head * ratio + rr % ratio;
+      float now = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) now = fmaxf(now, row_ml[(w * kRows + tid) * 2]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float mw = row_ml[(w * kRows + tid) * 2];
+        sum += mw == -INFINITY ? 0.0f : row_ml[(w * kRows + tid) * 2 + 1] * exp2_approx(mw - now);
+      }
+      row_all[tid] = make_float2(now, sum);
     }
     __syncthreads();
-    if (arrived + 1 == static_cast<unsigned>(parts)) {
+
+    // the block's rows: straight to the output, or to the workspace for the unit's last block to join
+    auto finish = [&](int r, int d, float4 v) {
+      const float2 ml = row_all[r];
+      const float over = ml.y > 0.0f ? 1.0f / ml.y : 0.0f;  // no tokens: 0
+      const bool sound = ml.y >= 0.0f;                       // else a NaN to hand on
+      v = make_float4(v.x * over, v.y * over, v.z * over, v.w * over);
+      if (!sound) v = make_float4(ml.y, ml.y, ml.y, ml.y);
+      store_four(a.ftype, a.out, row_out[r] * D + d, v);
+      if (d == 0 && a.lse) a.lse[row_out[r]] = ml.y > 0.0f ? (ml.x + log2f(ml.y)) * 0.69314718055994531f : sound ? -INFINITY : ml.y;
+    };
+    const int mine_at = (2 * blockIdx.x + plan.begins) * kRows;
+    for (int i = tid; i < unit_rows * D / 4; i += kThreads) {
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float4 x = *reinterpret_cast<const float4*>(sums + (w * kRows + r) * (D + 4) + d);
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      }
+      if (parts == 1) {
+        finish(r, d, v);
+      } else {
+        __stcg(reinterpret_cast<float4*>(a.partial + static_cast<size_t>(mine_at + r) * D + d), v);
+        if (d == 0) __stcg(reinterpret_cast<float2*>(a.partial_ml) + mine_at + r, row_all[r]);
+      }
+    }
+    if (parts > 1) {
       __threadfence();
-      const int owner = plan.owner;
-      // part j lies with block owner + j: the first as the unit begun there, the others as the one begun before
-      auto part_row = [&](int j, int r) { return static_cast<size_t>(2 * (owner + j) + (j == 0)) * kRows + r; };
-      auto part_four = [&](int j, int r, int d) { return __ldcg(reinterpret_cast<const float4*>(a.partial + part_row(j, r) * D + d)); };
-      constexpr int kFirst = 8;  // parts of the thread's first four that are read along with the maxima
-      float4 first[kFirst];
-#pragma unroll
-      for (int j = 0; j < kFirst; ++j)
-        if (j < parts && tid < unit_rows * D / 4) first[j] = part_four(j, tid / (D / 4), tid % (D / 4) * 4);
-      // what each part counts for, [row][part], and the rows' totals
-      float* const share = reinterpret_cast<float*>(smem);
-      for (int r = warp; r < unit_rows; r += kWarps) {
-        const float2* ml = reinterpret_cast<const float2*>(a.partial_ml);
-        const float2 mine = lane < parts ? __ldcg(ml + part_row(lane, r)) : make_float2(-INFINITY, 0.0f);
-        float now = mine.x, sum = 0.0f;
-        for (int j = lane + 32; j < parts; j += 32) now = fmaxf(now, __ldcg(ml + part_row(j, r)).x);
-        now = warp_max(now);
-        for (int j = lane; j < parts; j += 32) {
-          const float2 x = j == lane ? mine : __ldcg(ml + part_row(j, r));
-          const float keep = x.x == -INFINITY ? 0.0f : exp2_approx(x.x - now);
-          share[r * parts + j] = keep;
-          sum += keep * x.y;
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) row_all[r] = make_float2(now, sum);
+      __syncthreads();
+      if (tid == 0) {
+        arrived = atomicAdd(a.counters + plan.owner, 1u);
+        if (arrived + 1 == static_cast<unsigned>(parts)) a.counters[plan.owner] = 0;  // for the next launch
       }
       __syncthreads();
-      for (int i = tid; i < unit_rows * D / 4; i += kThreads) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        auto add = [&](int j, float4 x) {
-          const float keep = share[r * parts + j];
-          v.x = fmaf(keep, x.x, v.x), v.y = fmaf(keep, x.y, v.y), v.z = fmaf(keep, x.z, v.z), v.w = fmaf(keep, x.w, v.w);
-        };
-        int j0 = 0;
-        if (i == tid) {
+      if (arrived + 1 == static_cast<unsigned>(parts)) {
+        __threadfence();
+        const int owner = plan.owner;
+        // part j lies with block owner + j: the first as the unit begun there, the others as the one begun before
+        auto part_row = [&](int j, int r) { return static_cast<size_t>(2 * (owner + j) + (j == 0)) * kRows + r; };
+        auto part_four = [&](int j, int r, int d) { return __ldcg(reinterpret_cast<const float4*>(a.partial + part_row(j, r) * D + d)); };
+        constexpr int kFirst = 8;  // parts of the thread's first four that are read along with the maxima
+        float4 first[kFirst];
 #pragma unroll
-          for (int j = 0; j < kFirst; ++j)
-            if (j < parts) add(j, first[j]);
-          j0 = kFirst;
+        for (int j = 0; j < kFirst; ++j)
+          if (j < parts && tid < unit_rows * D / 4) first[j] = part_four(j, tid / (D / 4), tid % (D / 4) * 4);
+        // what each part counts for, [row][part], and the rows' totals
+        float* const share = reinterpret_cast<float*>(smem);
+        for (int r = warp; r < unit_rows; r += kWarps) {
+          const float2* ml = reinterpret_cast<const float2*>(a.partial_ml);
+          const float2 mine = lane < parts ? __ldcg(ml + part_row(lane, r)) : make_float2(-INFINITY, 0.0f);
+          float now = mine.x, sum = 0.0f;
+          for (int j = lane + 32; j < parts; j += 32) now = fmaxf(now, __ldcg(ml + part_row(j, r)).x);
+          now = warp_max(now);
+          for (int j = lane; j < parts; j += 32) {
+            const float2 x = j == lane ? mine : __ldcg(ml + part_row(j, r));
+            const float keep = x.x == -INFINITY ? 0.0f : exp2_approx(x.x - now);
+            share[r * parts + j] = keep;
+            sum += keep * x.y;
+          }
+          sum = warp_sum(sum);
+          if (lane == 0) row_all[r] = make_float2(now, sum);
         }
+        __syncthreads();
+        for (int i = tid; i < unit_rows * D / 4; i += kThreads) {
+          const int r = i / (D / 4), d = i % (D / 4) * 4;
+          float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          auto add = [&](int j, float4 x) {
+            const float keep = share[r * parts + j];
+            v.x = fmaf(keep, x.x, v.x), v.y = fmaf(keep, x.y, v.y), v.z = fmaf(keep, x.z, v.z), v.w = fmaf(keep, x.w, v.w);
+          };
+          int j0 = 0;
+          if (i == tid) {
+#pragma unroll
+            for (int j = 0; j < kFirst; ++j)
+              if (j < parts) add(j, first[j]);
+            j0 = kFirst;
+          }
 #pragma unroll 8
-        for (int j = j0; j < parts; ++j) add(j, part_four(j, r, d));
-        finish(r, d, v);
+          for (int j = j0; j < parts; ++j) add(j, part_four(j, r, d));
+          finish(r, d, v);
+        }
       }
     }
+    if (plan.at >= plan.stop) return;
+    __syncthreads();  // shared memory is free for the next unit
   }
-  if (plan.at >= plan.stop) return;
-  __syncthreads();  // shared memory is free for the next unit
- }
 }
 
 }  // namespace b200q
