@@ -2,17 +2,19 @@
 //
 // For one sequence and cache head with rows r (new tokens x query heads that share the head), tokens t:
 //   S[t][r] = sum_g ks[t,g] (sum_{d in g} kc[t,d] q[r,d]  -  kz[t,g] sum_{d in g} q[r,d])
-//   O[d][r] = sum_t vc[t,d] P[t,r]  -  sum_t vz[t,g] P[t,r],   P[t,r] = vs[t,g] exp2(f[r] S[t][r] - m[r])
+//   O[d][r] = sum_t (vc[t,d] - vz[t,g]) P[t,r],   P[t,r] = vs[t,g] exp2(f[r] S[t][r] - m[r])
 // Both products take the codes as the 16-row operand A of m16n8k16 (tokens x channels, then channels x tokens)
 // and the rows as its 8 columns, so 8 rows cost one instruction per 256 codes.
 //   Keys: a nibble in the low bits of an fp16 is the subnormal code * 2^-24, exactly, and one place higher
 //   code * 2^-20: a word of 8 codes becomes four operands by masking, and every second query value is divided
 //   by 16 instead.  Query rows are scaled by a power of two to a maximum in [2^14, 2^15), so that they fit
-//   fp16 whatever their type; fp32 rows are split into two fp16 terms (22 bits).
-//   Values: the same subnormals, channels as rows: a channel whose nibble lies one place higher has its sum divided by
-//   16 at the end, the zero points go through the same instruction as a 16-row operand of their own and are
-//   subtracted last.  P is fp16 (11 bits; two terms, 22 bits, in fp32 calls) times a power of two that follows the largest
-//   vs that the warp has met, so that full precision holds for tokens whose vs is up to 2^20 below that.
+//   fp16 whatever their type; fp32 rows are split into two fp16 terms (22 bits).  The adder lines subnormals up by
+//   their exponent field, which costs about 10 of the sum's bits: scores stay good to about 2e-5, enough for the 16-bit types.
+//   Values (and keys in fp32 calls): 1024 + code less 1024 + zero point, exact and normal (2 x 131072 fp16: off by 2.7e-4,
+//   6.6e-4 with subnormals); channels are rows, and one whose nibble lies one place higher has its sum divided by 16 at the
+//   end.  P is fp16 (11 bits; two terms, 22 bits, in fp32 calls) times a power of two that follows the largest
+//   vs that the warp has met, so that full precision holds for tokens whose vs is up to 2^20 below that.  The adder
+//   truncates, so fp32 calls add a tile's sums up outside of it.
 //   P leaves the first product as (token, row) and must enter the second as (row, token): movmatrix.
 // The maximum m[r] is a running reference, raised (and the sums rescaled) only when a score passes it by more than
 // 2^8: a warp-wide maximum is taken a few times per sequence, not per tile.
@@ -180,6 +182,7 @@ template <int D, int G, int NT, bool F32>
 __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128 ? 3 : 4) kv4_attention_kernel(Cache c, AttnArgs a) {
   using Shape = AttnShape<D, G, NT, F32>;
   constexpr int kGroups = Shape::kGroups, kPitch = Shape::kPitch, kRows = 8 * NT, kTerms = Shape::kTerms;
+  constexpr uint32_t kMagic = 0x64006400u;  // two fp16 1024: with a code in the low bits 1024 + code
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ unsigned arrived;
   __shared__ Plan plan;
@@ -330,7 +333,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
       }
       const Power power = power_for(warp_max(top));
       if (lane == 0) {
-        row_f[r] = power.down * a.scale * 1.4426950408889634f * 16777216.0f;
+        row_f[r] = power.down * a.scale * 1.4426950408889634f * (F32 ? 1.0f : 16777216.0f);
         row_limit[r] = len - a.tq + (tile * kRows + min(r, rows - 1)) / ratio + 1;
       }
       // lane: channel p = lane % 8 of the 8 that thread lane / 8 of a quad holds; pairs are (0,4) (1,5) (2,6) (3,7)
@@ -367,14 +370,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
       l[n] = both(0.0f);
     }
     const int all_see = len - a.tq + tile * kRows / ratio + 1;  // tokens that every row of the tile sees
-    float o[D / 16][NT][4], z[kGroups][NT][4];
+    float o[D / 16][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < kGroups; ++j) z[j][n][0] = z[j][n][1] = z[j][n][2] = z[j][n][3] = 0.0f;
-    }
 
     // P's power of two: 2^(127 - v_exp), for a largest vs of 2^(v_exp - 127)
     int v_exp = 127;
@@ -396,18 +396,22 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
       const bool whole = here == ~0u && base + kTile <= all_see;
 
       // lane l unpacks token l's scales and zero points for the lanes that use them: [group][token] (key scale, key zero
-      // point negated), then value scales times P's power, then value zero points as fp16 bits
+      // point), then value scales times P's power, then value zero points z as the fp16 1024 + z and 1024 + 16 z
       float2* const k_prep = reinterpret_cast<float2*>(prepared);
       float* const v_prep = reinterpret_cast<float*>(prepared + kTile * kGroups * 8);
       uint16_t* const z_prep = reinterpret_cast<uint16_t*>(prepared + kTile * kGroups * 12);
+      uint16_t* const z16_prep = z_prep + kTile * kGroups;
       {
         float vs[kGroups], v_top = 0.0f;
         const bool there = here >> lane & 1;
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) {
           const uint32_t p = kp[lane * kGroups + k], q = there ? vp[lane * kGroups + k] : 0u;  // places that hold nothing hold any bits
-          k_prep[k * kTile + lane] = make_float2(param_scale(p), -zero_point(p));
-          z_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 16);
+          // the key's zero point negated, or in fp32 calls as a pair of the fp16 1024 + z
+          k_prep[k * kTile + lane] = make_float2(
+              param_scale(p), F32 ? __uint_as_float((p >> 16 & 15u) * 0x00010001u | kMagic) : -zero_point(p));
+          z_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 16 & 15u | 0x6400u);
+          z16_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 12 & 0xF0u | 0x6400u);
           vs[k] = param_scale(q);
           v_top = fmaxf(v_top, vs[k]);
         }
@@ -421,12 +425,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-#pragma unroll
-              for (int j = 0; j < D / 16; ++j) o[j][n][e] *= keep;
-#pragma unroll
-              for (int j = 0; j < kGroups; ++j) z[j][n][e] *= keep;
-            }
+            for (int j = 0; j < D / 16; ++j) o[j][n][0] *= keep, o[j][n][1] *= keep, o[j][n][2] *= keep, o[j][n][3] *= keep;
         }
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) v_prep[k * kTile + lane] = vs[k] * v_factor;
@@ -447,21 +446,30 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
             for (int n = 0; n < NT; ++n) b[term][n] = query[((i * kTerms + term) * NT + n) * 32 + lane];
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
-            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(kc + (mt * 16 + g) * kPitch + 16 * i + 4 * t);
-            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(kc + (mt * 16 + g + 8) * kPitch + 16 * i + 4 * t);
-            const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
+            uint32_t c[2][4];  // pairs (0,4) (1,5) (2,6) (3,7) of tokens g and g + 8
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t w = *reinterpret_cast<const uint32_t*>(kc + (mt * 16 + u * 8 + g) * kPitch + 16 * i + 4 * t);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t mask = j % 2 ? 0x00F000F0u : 0x000F000Fu;
+                if constexpr (F32) {
+                  const uint32_t z = __float_as_uint(k_prep[k * kTile + mt * 16 + u * 8 + g].y);
+                  c[u][j] = sub_f16x2(and_or(w >> (j / 2 * 8), mask, kMagic), j % 2 ? and_or(z << 4, 0x00F000F0u, kMagic) : z);
+                } else {
+                  c[u][j] = w >> (j / 2 * 8) & mask;
+                }
+              }
+            }
 #pragma unroll
             for (int term = 0; term < kTerms; ++term)
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 if (i == k * (G / 32) && term == 0)
-                  mma_f16_first(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
-                                b[term][n].x, b[term][n].y);
+                  mma_f16_first(part[mt][n], c[0][0], c[1][0], c[0][1], c[1][1], b[term][n].x, b[term][n].y);
                 else
-                  mma_f16(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
-                          b[term][n].x, b[term][n].y);
-                mma_f16(part[mt][n], v0 & 0x000F000Fu, v1 & 0x000F000Fu, v0 & 0x00F000F0u, v1 & 0x00F000F0u,
-                        b[term][n].z, b[term][n].w);
+                  mma_f16(part[mt][n], c[0][0], c[1][0], c[0][1], c[1][1], b[term][n].x, b[term][n].y);
+                mma_f16(part[mt][n], c[0][2], c[1][2], c[0][3], c[1][3], b[term][n].z, b[term][n].w);
               }
           }
         }
@@ -474,7 +482,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const float* at = part[mt][n] + 2 * u;
-              const float2 v = fma2(kz, *reinterpret_cast<const float2*>(row_sum + k * kRows + n * 8 + 2 * t), make_float2(at[0], at[1]));
+              float2 v = make_float2(at[0], at[1]);
+              if constexpr (!F32) v = fma2(kz, *reinterpret_cast<const float2*>(row_sum + k * kRows + n * 8 + 2 * t), v);
               s[mt][n][u] = k == 0 ? mul2(ks, v) : fma2(ks, v, s[mt][n][u]);
             }
           }
@@ -515,8 +524,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
             (e ? l[n].y : l[n].x) *= keep;
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) o[j][n][e] *= keep, o[j][n][2 + e] *= keep;
-#pragma unroll
-            for (int j = 0; j < kGroups; ++j) z[j][n][e] *= keep, z[j][n][2 + e] *= keep;
           }
       }
 #pragma unroll
@@ -533,12 +540,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
           }
       }
 
-      // values
+      // values; in fp32 calls a tile's sums are made apart and added with rounding
       constexpr int kPTerms = F32 ? 2 : 1;
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
+      for (int k = 0; k < kGroups; ++k) {
+        float part[G / 16][NT][4];
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) {
+        for (int mt = 0; mt < 2; ++mt) {
           // operand B: P of this group, as (row g, tokens 2t, 2t + 1) of each 8 tokens
           uint32_t b[kPTerms][NT][2];
 #pragma unroll
@@ -560,7 +568,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
           }
           // operand A: tokens 2t, 2t + 1 (u = 0) and 2t + 8, 2t + 9 (u = 1) of this lane's G / 8 channels, the lower
           // half of them as row g of the group's G / 16 products, the upper as row g + 8
-          uint32_t lower[2], upper[2], zero[2];
+          uint32_t lower[2], upper[2], zero[2], zero16[2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int tok = mt * 16 + u * 8 + 2 * t;
@@ -575,22 +583,37 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
               upper[u] = lower[u] >> 8;
             }
             zero[u] = *reinterpret_cast<const uint32_t*>(z_prep + k * kTile + tok);
+            zero16[u] = *reinterpret_cast<const uint32_t*>(z16_prep + k * kTile + tok);
           }
 #pragma unroll
           for (int j = 0; j < G / 16; ++j) {
             const int down = j / 2 * 8;
             const uint32_t mask = j % 2 ? 0x00F000F0u : 0x000F000Fu;
-            const uint32_t a0 = lower[0] >> down & mask, a1 = upper[0] >> down & mask;
-            const uint32_t a2 = lower[1] >> down & mask, a3 = upper[1] >> down & mask;
+            const uint32_t z0 = j % 2 ? zero16[0] : zero[0], z1 = j % 2 ? zero16[1] : zero[1];
+            const uint32_t a0 = sub_f16x2(and_or(lower[0] >> down, mask, kMagic), z0);
+            const uint32_t a1 = sub_f16x2(and_or(upper[0] >> down, mask, kMagic), z0);
+            const uint32_t a2 = sub_f16x2(and_or(lower[1] >> down, mask, kMagic), z1);
+            const uint32_t a3 = sub_f16x2(and_or(upper[1] >> down, mask, kMagic), z1);
 #pragma unroll
             for (int term = 0; term < kPTerms; ++term)
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma_f16(o[k * (G / 16) + j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
+              for (int n = 0; n < NT; ++n) {
+                if (!F32)
+                  mma_f16(o[k * (G / 16) + j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
+                else if (mt == 0 && term == 0)
+                  mma_f16_first(part[j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
+                else
+                  mma_f16(part[j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
+              }
           }
+        }
+        if constexpr (F32) {
 #pragma unroll
-          for (int term = 0; term < kPTerms; ++term)
+          for (int j = 0; j < G / 16; ++j)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(z[k][n], zero[0], zero[0], zero[1], zero[1], b[term][n][0], b[term][n][1]);
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[k * (G / 16) + j][n][e] += part[j][n][e];
         }
       }
 #pragma unroll
@@ -633,7 +656,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
           for (int u = 0; u < 2; ++u) {
             float v[G / 16];
 #pragma unroll
-            for (int j = 0; j < G / 16; ++j) v[j] = fmaf(o[k * (G / 16) + j][n][2 * u + e], j % 2 ? 0.0625f : 1.0f, -z[k][n][2 * u + e]) * 16777216.0f * value * keep;
+            for (int j = 0; j < G / 16; ++j) v[j] = o[k * (G / 16) + j][n][2 * u + e] * ((j % 2 ? 0.0625f : 1.0f) * value) * keep;
             float* p = to + k * G + g * (G / 8) + u * (G / 16);
             if constexpr (G == 64)
               *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);

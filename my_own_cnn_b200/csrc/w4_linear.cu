@@ -10,7 +10,9 @@
 //   code * 2^-20: a word of 8 codes becomes four operands, the pairs (0,4) (1,5) (2,6) (3,7), by one shift and four
 //   masks, and every second value of x is divided by 16 instead.  x is scaled by a power of two per row and step to a
 //   maximum in [2^14, 2^15), so that it fits fp16 whatever its type; fp32 becomes two fp16 terms (22 bits).
-//   The zero points' sum is kept apart, one row per lane.
+//   The zero points' sum is kept apart, one row per lane.  The adder lines subnormals up by their exponent field, which
+//   costs about 10 of the sum's bits (results off by 2e-6, far below a 16-bit output's rounding): fp32 calls
+//   take 1024 + code less 1024 + zero point instead, exact and normal.
 //
 // Each warp streams 32 rows through a ring of its own (16-byte asynchronous copies) in steps of kStep columns.  x is
 // shared by the block's warps, in the order of operand B; the blocks of a cluster have the same rows and other slices
@@ -62,7 +64,7 @@ struct Layout {
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kRowsW = FEW ? 32 : 32 * kWarps;     // weight rows of a block
   static constexpr int kX = kStep * 2 * kTerms * kRowsX;
-  static constexpr int kXSum = (kStep / G) * kRowsX * 4;
+  static constexpr int kXSum = kTerms == 2 ? 0 : (kStep / G) * kRowsX * 4;
   static constexpr int kBuffer = (kX + kXSum + kRowsX * 4 + 15) / 16 * 16;
   static constexpr int kBuffers = FEW ? (46 * 1024) / kBuffer : 2;
   static constexpr int kBytes = kRing + kBuffers * kBuffer;
@@ -121,11 +123,13 @@ struct XRow {
       f[j] = make_float2(to_f32(v[j]), to_f32(v[j + 4]));
       top = fmaxf(fmaxf(fabsf(f[j].x), fabsf(f[j].y)), top);
     }
-    const float2 half = add2(add2(f[0], f[1]), add2(f[2], f[3]));
-    float sum = half.x + half.y;
+    if constexpr (L::kTerms == 1) {
+      const float2 half = add2(add2(f[0], f[1]), add2(f[2], f[3]));
+      float sum = half.x + half.y;
 #pragma unroll
-    for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (q % (G / 8) == 0) xsum[group * L::kRowsX + m] = sum;
+      for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
+      if (q % (G / 8) == 0) xsum[group * L::kRowsX + m] = sum;
+    }
     const Power p = power_for(warp_max(top));
     if (q == 0) xpower[m] = p.down;
 #pragma unroll
@@ -153,6 +157,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
   using L = Layout<T, G, NT, FEW>;
   constexpr int kTerms = L::kTerms, kWords = G / 32, kGroups = kStep / G, kStages = L::kStages, kRowsW = L::kRowsW;
   constexpr int kRowsX = L::kRowsX;
+  constexpr bool kF32 = kTerms == 2;
   extern __shared__ __align__(128) uint8_t smem[];
   wait_for_previous();
   uint8_t* const buffers = smem + L::kRing;
@@ -283,6 +288,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
           w[r][0] = v.x, w[r][1] = v.y, w[r][2] = v.z, w[r][3] = v.w;
         }
       }
+      constexpr uint32_t kMagic = 0x64006400u;  // two fp16 1024
+      uint32_t zpair[4];  // fp32 calls: the rows' zero points, twice
+      if constexpr (kF32) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) zpair[r] = __shfl_sync(~0u, zero[i], r * 8 + g) * 0x00010001u;
+      }
       float part[2][NT][4];
 #pragma unroll
       for (int word = 0; word < kWords; ++word) {
@@ -294,19 +305,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
             b[term][n] = xs[(((i * kWords + word) * kTerms + term) * kRowsX + (FEW ? column : n * 8 + g)) * 4 + t];
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
-          const uint32_t w0 = w[2 * mt][word], w1 = w[2 * mt + 1][word], v0 = w0 >> 8, v1 = w1 >> 8;
+          uint32_t c[2][4];  // pairs (0,4) (1,5) (2,6) (3,7) of rows g and g + 8
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t v = w[2 * mt + u][word] >> (j / 2 * 8), mask = j % 2 ? 0x00F000F0u : 0x000F000Fu;
+              if constexpr (kF32)
+                c[u][j] = sub_f16x2(and_or(v, mask, kMagic),
+                                    j % 2 ? and_or(zpair[2 * mt + u] << 4, mask, kMagic) : zpair[2 * mt + u] | kMagic);
+              else
+                c[u][j] = v & mask;
+            }
 #pragma unroll
           for (int term = 0; term < kTerms; ++term)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               if (word == 0 && term == 0)
-                mma_f16_first(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
-                              b[term][n].x, b[term][n].y);
+                mma_f16_first(part[mt][n], c[0][0], c[1][0], c[0][1], c[1][1], b[term][n].x, b[term][n].y);
               else
-                mma_f16(part[mt][n], w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u,
-                        b[term][n].x, b[term][n].y);
-              mma_f16(part[mt][n], v0 & 0x000F000Fu, v1 & 0x000F000Fu, v0 & 0x00F000F0u, v1 & 0x00F000F0u, b[term][n].z,
-                      b[term][n].w);
+                mma_f16(part[mt][n], c[0][0], c[1][0], c[0][1], c[1][1], b[term][n].x, b[term][n].y);
+              mma_f16(part[mt][n], c[0][2], c[1][2], c[0][3], c[1][3], b[term][n].z, b[term][n].w);
             }
         }
       }
@@ -320,19 +339,21 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
           to = i == 0 ? mul2(sc, make_float2(p[0], p[1])) : fma2(sc, make_float2(p[0], p[1]), to);
         }
       }
-      const float2 sz = both(__uint_as_float(scale[i]) * static_cast<float>(zero[i]));
+      if constexpr (!kF32) {
+        const float2 sz = both(__uint_as_float(scale[i]) * static_cast<float>(zero[i]));
 #pragma unroll
-      for (int m = 0; m < kRowsX; m += 4)
-        if (m < rows) {
-          const float* at = xsum + i * kRowsX + m;
-          if constexpr (kRowsX == 1) {
-            less[0].x = fmaf(sz.x, at[0], less[0].x);
-          } else {
-            const float4 v = *reinterpret_cast<const float4*>(at);
-            less[m / 2] = fma2(sz, make_float2(v.x, v.y), less[m / 2]);
-            less[m / 2 + 1] = fma2(sz, make_float2(v.z, v.w), less[m / 2 + 1]);
+        for (int m = 0; m < kRowsX; m += 4)
+          if (m < rows) {
+            const float* at = xsum + i * kRowsX + m;
+            if constexpr (kRowsX == 1) {
+              less[0].x = fmaf(sz.x, at[0], less[0].x);
+            } else {
+              const float4 v = *reinterpret_cast<const float4*>(at);
+              less[m / 2] = fma2(sz, make_float2(v.x, v.y), less[m / 2]);
+              less[m / 2 + 1] = fma2(sz, make_float2(v.z, v.w), less[m / 2 + 1]);
+            }
           }
-        }
+      }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -359,8 +380,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
       for (int u = 0; u < 2; ++u) {
         if (FEW && 2 * t >= kRowsX) continue;
         float* to = sums + (n * 8 + 2 * t) * 32 + mt * 16 + u * 8 + g;
-        to[0] = acc[mt][n][u].x * 16777216.0f;
-        if (kRowsX > 1) to[32] = acc[mt][n][u].y * 16777216.0f;
+        constexpr float kUnit = kF32 ? 1.0f : 16777216.0f;  // subnormal codes count 2^-24
+        to[0] = acc[mt][n][u].x * kUnit;
+        if (kRowsX > 1) to[32] = acc[mt][n][u].y * kUnit;
       }
   __syncwarp();
 #pragma unroll
