@@ -131,6 +131,33 @@ def test_attention_lengths(length):
     run(c, table, lens, 1, 4, torch.bfloat16)
 
 
+@pytest.mark.parametrize("page", [16, 32])
+@pytest.mark.parametrize("d,hk,ratio,tq", [(64, 2, 3, 1), (128, 1, 9, 1), (256, 1, 5, 3)])
+def test_attention_many_sequences(d, hk, ratio, tq, page):
+    """More sequences than a warp counts at a time, most of them short, some empty, a few split over several blocks."""
+    lens = [(0, 7, 1, 130, 33, 64, 300)[i % 7] for i in range(75)]
+    lens[40], lens[71] = 3000, 1500
+    c, table, n = filled(lens, hk, page, d, 32, seed=d)
+    run(c, table, n, tq, hk * ratio, torch.float16)
+
+
+@pytest.mark.parametrize("d,ratio", [(64, 4), (128, 4), (128, 16), (256, 8)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_long_context(dtype, d, ratio):
+    c, table, n = filled([20000], 1, 64, d, 64, seed=d + ratio)
+    run(c, table, n, 1, ratio, dtype)
+
+
+def test_attention_wide_table():
+    """A table with room for many more pages than the lengths name."""
+    c, table, lens = filled([500, 40], 2, 32, 64, 64)
+    wide = torch.full((2, 5000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    q = torch.randn(2, 1, 4, 64, generator=gen(6), device="cuda")
+    want, _, ob, _ = attention(q, c, table, lens, 0.125, torch.float32)
+    within(b2q.kv4_attention(q, c, wide, lens), want, ob)
+
+
 def test_attention_many_rows_of_a_head():
     c, table, lens = filled([90, 5], 1, 16, 64, 64)
     run(c, table, lens, 9, 11, torch.float16)
@@ -216,16 +243,17 @@ def test_offsets_past_32_bits():
     assert torch.equal(b2q.kv4_attention(q, c, order, lens), b2q.kv4_attention(q, small, line, lens))
 
 
-def test_values_out_of_range_are_reported_and_left_out():
-    c, table, lens = filled([40, 20], 1, 16, 64, 64)
+@pytest.mark.parametrize("page", [16, 32])
+def test_values_out_of_range_are_reported_and_left_out(page):
+    c, table, lens = filled([40, 20], 1, page, 64, 64)
     b2q.device_error()
     k = torch.randn(2, 1, 64, device="cuda")
     before = c.k_codes.clone()
-    b2q.kv4_append(c, k, k, torch.tensor([-1, c.pages * 16], device="cuda"))
+    b2q.kv4_append(c, k, k, torch.tensor([-1, c.pages * page], device="cuda"))
     with pytest.raises(b2q.B200QError, match="slot"):
         b2q.device_error()
     assert torch.equal(c.k_codes, before)
-    rk, _ = b2q.kv4_read(c, torch.tensor([c.pages * 16 + 5, 0], device="cuda"))
+    rk, _ = b2q.kv4_read(c, torch.tensor([c.pages * page + 5, 0], device="cuda"))
     with pytest.raises(b2q.B200QError, match="slot"):
         b2q.device_error()
     assert (rk[0] == 0).all()
@@ -239,7 +267,7 @@ def test_values_out_of_range_are_reported_and_left_out():
         with pytest.raises(b2q.B200QError, match=message):
             b2q.device_error()
         assert out.isfinite().all() and torch.equal(out[1], want[1])
-    for bad in (table.shape[1] * 16 + 1, -3):
+    for bad in (table.shape[1] * page + 1, -3):
         n = lens.clone()
         n[0] = bad
         out = b2q.kv4_attention(q, c, table, n)

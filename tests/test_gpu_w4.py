@@ -98,6 +98,16 @@ def test_leading_dimensions_and_none():
     assert torch.equal(b2q.linear_w4(x.new_empty(2, 0), empty, bias), bias.expand(2, 5))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 180001), (4, 64, 50001), (2, 700, 20000), (1, 9000, 300), (4, 5000, 700),
+                                   (6, 5000, 2500), (16, 40, 30000)])
+def test_shapes_of_every_split(dtype, m, n, k):
+    """One and few rows with K shared out to warps and clusters, and past what they hold; K split two to eight ways."""
+    w = case(n, k, 64)
+    x = torch.randn(m, k, generator=gen(11), device="cuda").to(dtype)
+    check(b2q.linear_w4(x, w), x, w)
+
+
 def test_columns_past_k_are_not_used():
     """The nibbles that pad a row, and x beyond its k columns, may hold anything."""
     w = case(48, 50, 32)
