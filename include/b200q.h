@@ -190,14 +190,18 @@ int b200q_bmm_s8(const int8_t* A, const int8_t* B, const int32_t* d_bias, const 
  * statistics are held in fp32.  Strides are in elements; the last dimension is contiguous.
  * A 4-bit code pair is one byte, low nibble first.  Positions, slots, page numbers and lengths live on
  * the device: one that is out of range is left out of the result (nothing is read or written for it)
- * and reported by the next b200q_device_error() as B200Q_ERR_INVALID_ARG. */
+ * and reported by the next b200q_device_error() as B200Q_ERR_INVALID_ARG.
+ * Attention and the gradient use 16 MiB of scratch that the first of their calls on a stream makes (not while the
+ * stream is captured: B200Q_ERR_UNSUPPORTED) and that never moves.  Graphs captured on one stream share it: do not
+ * replay two of them at the same time. */
 enum b200q_ftype { B200Q_F32 = 0, B200Q_F16 = 1, B200Q_BF16 = 2 };
 
 /* y[m][n] = sum_k x[m][k] * (code[n][k] - zero[k / group][n]) * scale[k / group][n] (+ bias[n]).
  * codes: [n][16 * ceil(k / 32)] bytes, 16-byte aligned (the nibbles past k are not used);
  * scales: bf16 [ceil(k / group)][n]; zeros: uint8 in 0..15, same shape, or NULL for 8 everywhere;
  * group 32, 64 or 128.  x [m][k] with row stride ldx, y [m][n] with row stride ldy; bias [n] or NULL.
- * Made for the few rows of a decode step: weights are read once per 16 rows of x.  Finite x. */
+ * Made for the few rows of a decode step: weights are read once per 16 rows of x.  Finite x; y shares no
+ * memory with x. */
 typedef struct b200q_linear_w4_args {
   const void* x;
   int64_t ldx;
@@ -233,7 +237,7 @@ int b200q_qk_norm_rope(const b200q_qk_norm_args* args, void* stream);
 /* Gradient of b200q_qk_norm_rope: q_grad / k_grad are the gradients of its outputs, contiguous
  * [t][h][d]; q_out / k_out (contiguous, their strides not read) receive those of its inputs, q_w_grad /
  * k_w_grad [d] (NULL: not wanted) those of the weights, summed over tokens and heads in a fixed order.
- * Recomputes the norms from q and k.  Uses the stream's workspace. */
+ * Recomputes the norms from q and k.  Uses the stream's scratch. */
 int b200q_qk_norm_rope_bprop(const b200q_qk_norm_args* args, void* stream);
 
 /* 4-bit paged key / value cache.  codes: [pages][heads][page_size][d / 2] bytes, 16-byte aligned;
@@ -262,7 +266,7 @@ int b200q_kv4_read(const b200q_kv4_cache* c, const int64_t* slots, void* k, void
  * block_table[b][0 .. max_pages), row stride bt_stride; none seen: output 0, lse -inf.
  * q [b][tq][hq][d] with strides; query head h reads cache head h / (hq / heads).
  * out contiguous [b][tq][hq][d]; lse fp32 [b][tq][hq] or NULL: log of the sum of exp(scale * q.k).
- * Uses the stream's workspace: sequences are split over blocks. */
+ * Uses the stream's scratch: sequences are split over blocks. */
 typedef struct b200q_kv4_attention_args {
   const void* q;
   int64_t q_bs, q_ts, q_hs;

@@ -73,7 +73,7 @@ struct DeviceState {
   int sms = 0;
   int* err = nullptr;  // device address of g_dev_err
 };
-DeviceState g_dev[64];
+DeviceState g_dev[kMaxDevices];
 std::mutex g_dev_mu;
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -99,7 +99,7 @@ int device_state(DeviceState** out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  if (dev < 0 || dev >= 64) return fail(B200Q_ERR_UNSUPPORTED, "device index %d out of range", dev);
+  if (dev < 0 || dev >= kMaxDevices) return fail(B200Q_ERR_UNSUPPORTED, "device index %d out of range", dev);
   std::lock_guard<std::mutex> lk(g_dev_mu);
   DeviceState& st = g_dev[dev];
   if (!st.init) {
@@ -756,7 +756,7 @@ int noalloc_scratch(int8_t** out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  if (dev < 0 || dev >= 64) return fail(B200Q_ERR_UNSUPPORTED, "device index %d out of range", dev);
+  if (dev < 0 || dev >= kMaxDevices) return fail(B200Q_ERR_UNSUPPORTED, "device index %d out of range", dev);
   std::lock_guard<std::mutex> lk(g_noalloc_mu);
   if (!g_noalloc_ptr[dev]) {
     void* ptr = nullptr;
@@ -1008,7 +1008,7 @@ int f32_grad(const DeviceState& st, const float* x, const float* dy, float* dw, 
 
 // Arrival counters of kernels whose last block joins the others' partial results: zeroed once here,
 // and returned to zero by the block that sees the last arrival.
-std::map<std::pair<int, cudaStream_t>, unsigned*> g_counters;
+std::map<std::pair<int, cudaStream_t>, unsigned*> g_scratch;
 
 }  // namespace
 
@@ -1023,32 +1023,40 @@ int host_fail(int code, const char* fmt, ...) {
 int host_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
 int host_check_launch(const char* what) { return check_launch(what); }
 
-int host_device(int* sms, int** err) {
+int host_device(int* sms, int** err, int* index) {
   DeviceState* st = nullptr;
   int rc = device_state(&st);
   if (rc) return rc;
   *sms = st->sms;
   *err = st->err;
+  if (index) *index = static_cast<int>(st - g_dev);
   return B200Q_OK;
 }
 
-int host_workspace(size_t bytes, cudaStream_t stream, void** out) { return get_workspace(bytes, stream, out); }
-
-int host_counters(cudaStream_t stream, unsigned** out) {
+int host_scratch(cudaStream_t stream, void** out, unsigned** counters) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   std::lock_guard<std::mutex> lk(g_ws_mu);
-  unsigned*& c = g_counters[{dev, stream}];
+  unsigned*& c = g_scratch[{dev, stream}];
   if (!c) {
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    e = cudaStreamIsCapturing(stream, &capturing);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
+    if (capturing != cudaStreamCaptureStatusNone)
+      return fail(B200Q_ERR_UNSUPPORTED, "make one call on the stream before capturing: its scratch is made by the first");
     void* p = nullptr;
-    e = cudaMallocAsync(&p, kSplitCounters * sizeof(unsigned), stream);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync(counters)");
+    e = cudaMallocAsync(&p, kSplitCounters * sizeof(unsigned) + kScratchBytes, stream);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync(scratch)");
     e = cudaMemsetAsync(p, 0, kSplitCounters * sizeof(unsigned), stream);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(counters)");
+    if (e != cudaSuccess) {
+      cudaFreeAsync(p, stream);
+      return cuda_fail(e, "cudaMemsetAsync(counters)");
+    }
     c = static_cast<unsigned*>(p);
   }
-  *out = c;
+  *out = c + kSplitCounters;
+  if (counters) *counters = c;
   return B200Q_OK;
 }
 

@@ -17,14 +17,15 @@ B200Q_HIDDEN int host_fail(int code, const char* fmt, ...) __attribute__((format
 B200Q_HIDDEN int host_cuda_fail(cudaError_t e, const char* what);
 // cudaGetLastError() after a launch as a status.
 B200Q_HIDDEN int host_check_launch(const char* what);
-// SM count of the current device and the device address of its error word.
-B200Q_HIDDEN int host_device(int* sms, int** err);
-// Grow-only scratch of the (device, stream) pair.
-B200Q_HIDDEN int host_workspace(size_t bytes, cudaStream_t stream, void** out);
-// kSplitCounters arrival counters of the (device, stream) pair, zero before and after every kernel
-// that uses them.
+// SM count of the current device, the device address of its error word and (index) its number.
+constexpr int kMaxDevices = 64;
+B200Q_HIDDEN int host_device(int* sms, int** err, int* index = nullptr);
+// Scratch of the (device, stream) pair: kScratchBytes, and kSplitCounters arrival counters that are zero before and
+// after every kernel that uses them.  Made by the first call on a stream and never moved, so that a graph that was
+// captured on the stream can be replayed whatever calls follow; refused while the stream is captured.
+constexpr size_t kScratchBytes = 16u << 20;
 constexpr int kSplitCounters = 1 << 16;
-B200Q_HIDDEN int host_counters(cudaStream_t stream, unsigned** out);
+B200Q_HIDDEN int host_scratch(cudaStream_t stream, void** out, unsigned** counters = nullptr);
 B200Q_HIDDEN void host_set_path(int path);
 
 // Launches a kernel that begins with wait_for_previous(): its blocks may take their places while the stream's previous kernel

@@ -198,6 +198,8 @@ int check_cache(const b200q_kv4_cache* p, Cache* c) {
   if (p->page_size > (1 << 20) || p->heads > (1 << 16)) return host_fail(B200Q_ERR_UNSUPPORTED, "cache too large");
   if (static_cast<long long>(p->pages) * p->page_size > 0x7fffffffll)
     return host_fail(B200Q_ERR_UNSUPPORTED, "cache of more than 2^31 slots");
+  if (static_cast<long long>(p->pages) * p->page_size * p->heads >= 0xffffffffll)  // rows are numbered in 32 bits
+    return host_fail(B200Q_ERR_UNSUPPORTED, "cache of more than 2^32 rows");
   if (p->pages > 0 && (!p->k_codes || !p->k_params || !p->v_codes || !p->v_params))
     return host_fail(B200Q_ERR_INVALID_ARG, "null cache pointer");
   if ((reinterpret_cast<uintptr_t>(p->k_codes) | reinterpret_cast<uintptr_t>(p->v_codes) |
@@ -227,19 +229,19 @@ int move_blocks(const Cache& c, int t, int sms, int* ahead, int* blocks) {
 }
 
 template <int D, int G, int NT, bool F32>
-int launch_attention(const Cache& c, AttnArgs a, int sms, cudaStream_t stream) {
+int launch_attention(const Cache& c, AttnArgs a, int sms, int device, cudaStream_t stream) {
   using Shape = AttnShape<D, G, NT, F32>;
   auto kernel = kv4_attention_kernel<D, G, NT, F32>;
   // blocks that an SM holds, found once (and on the way, leave for the shared memory that they take)
-  static std::atomic<int> per_sm{0};
-  int resident = per_sm.load(std::memory_order_relaxed);
+  static std::atomic<int> per_sm[kMaxDevices];
+  int resident = per_sm[device].load(std::memory_order_relaxed);
   if (resident == 0) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
     if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute(kv4_attention_kernel)");
     e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kWarps * 32, Shape::kSmem);
     if (e != cudaSuccess) return host_cuda_fail(e, "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
     resident = std::max(1, resident);
-    per_sm.store(resident, std::memory_order_relaxed);
+    per_sm[device].store(resident, std::memory_order_relaxed);
   }
   a.row_tiles = (a.tq * (a.hq / c.heads) + 8 * NT - 1) / (8 * NT);
   // one block for each that the GPU holds at once; fewer when even the longest lengths have fewer steps
@@ -247,12 +249,15 @@ int launch_attention(const Cache& c, AttnArgs a, int sms, cudaStream_t stream) {
   const long long most = static_cast<long long>(a.b) * c.heads * a.row_tiles * std::max(1ll, steps);
   if (static_cast<long long>(a.b) * c.heads * a.row_tiles * (steps + kUnitSteps + 1) > 0x7fffffffll)
     return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
-  // (a unit's parts, one per block at most, leave their shares in shared memory when they are joined)
-  const int blocks = static_cast<int>(std::min<long long>(std::min({sms * resident, Shape::kBody / (8 * NT * 4), kSplitCounters}), most));
-  const size_t rows = static_cast<size_t>(blocks) * 2 * 8 * NT;
+  // (a unit's parts, one per block at most, leave their shares in shared memory when they are joined; the scratch holds
+  // the parts of a thousand blocks)
+  constexpr int kPartRows = 2 * 8 * NT, kRoom = static_cast<int>(kScratchBytes / (kPartRows * (D + 2) * sizeof(float)));
+  const int blocks = static_cast<int>(
+      std::min<long long>(std::min({sms * resident, Shape::kBody / (8 * NT * 4), kSplitCounters, kRoom}), most));
+  const size_t rows = static_cast<size_t>(blocks) * kPartRows;
   void* ws = nullptr;
-  int rc = host_workspace(rows * (D + 2) * sizeof(float), stream, &ws);
-  if (rc || (rc = host_counters(stream, &a.counters))) return rc;
+  int rc = host_scratch(stream, &ws, &a.counters);
+  if (rc) return rc;
   a.partial = static_cast<float*>(ws);
   a.partial_ml = a.partial + rows * D;
   return host_launch("kv4_attention_kernel launch", kernel, dim3(blocks), kWarps * 32, Shape::kSmem, stream, 1, c, a);
@@ -325,20 +330,21 @@ extern "C" int b200q_kv4_attention(const b200q_kv4_cache* cache, const b200q_kv4
   if (!p->q || !p->out || !p->lens || (max_pages > 0 && !p->block_table)) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
   if (static_cast<long long>(max_pages) * c.page_size > (1 << 30) || b > (1 << 20) || tq > (1 << 16) || hq > (1 << 16))
     return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
+  if (static_cast<long long>(b) * tq * hq > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
   AttnArgs a{p->q,   p->q_bs, p->q_ts, p->q_hs, p->block_table, p->bt_stride, p->lens, p->out,
              p->lse, ftype,   b,       tq,      hq,             max_pages,    p->scale};
-  int sms = 0;
-  if ((rc = host_device(&sms, &a.err))) return rc;
+  int sms = 0, device = 0;
+  if ((rc = host_device(&sms, &a.err, &device))) return rc;
   // 16 rows a pass where a head has more than 8; heads of 256 channels keep to 8, whose sums fill the registers
   const int rows = tq * (hq / c.heads);
   const bool two = rows > 8 && c.d <= 128;
   const bool f32 = ftype == B200Q_F32;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
 #define B200Q_ATTN(D, G)                                                      \
-  (two ? f32 ? launch_attention<D, G, D == 256 ? 1 : 2, true>(c, a, sms, cs)  \
-             : launch_attention<D, G, D == 256 ? 1 : 2, false>(c, a, sms, cs) \
-       : f32 ? launch_attention<D, G, 1, true>(c, a, sms, cs)                 \
-             : launch_attention<D, G, 1, false>(c, a, sms, cs))
+  (two ? f32 ? launch_attention<D, G, D == 256 ? 1 : 2, true>(c, a, sms, device, cs)  \
+             : launch_attention<D, G, D == 256 ? 1 : 2, false>(c, a, sms, device, cs) \
+       : f32 ? launch_attention<D, G, 1, true>(c, a, sms, device, cs)                 \
+             : launch_attention<D, G, 1, false>(c, a, sms, device, cs))
   rc = c.d == 64    ? c.group == 32 ? B200Q_ATTN(64, 32) : B200Q_ATTN(64, 64)
        : c.d == 128 ? c.group == 32 ? B200Q_ATTN(128, 32) : B200Q_ATTN(128, 64)
                     : c.group == 32 ? B200Q_ATTN(256, 32) : B200Q_ATTN(256, 64);

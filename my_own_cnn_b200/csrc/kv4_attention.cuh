@@ -111,12 +111,22 @@ __device__ __forceinline__ int valid_length(const Cache& c, const AttnArgs& a, i
   return 0;
 }
 
+// Four channels of an output that may begin at any element.
 __device__ __forceinline__ void store_four(int ftype, void* p, long long i, float4 v) {
-  if (ftype == B200Q_F32)
-    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = v;
-  else
-    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) =
-        ftype == B200Q_F16 ? make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w)) : make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+  if (ftype == B200Q_F32) {
+    float* to = static_cast<float*>(p) + i;
+    if (reinterpret_cast<uintptr_t>(p) % 16 == 0)
+      *reinterpret_cast<float4*>(to) = v;
+    else
+      to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+  } else {
+    uint16_t* to = static_cast<uint16_t*>(p) + i;
+    const uint2 w = ftype == B200Q_F16 ? make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w)) : make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+    if (reinterpret_cast<uintptr_t>(p) % 8 == 0)
+      *reinterpret_cast<uint2*>(to) = w;
+    else
+      to[0] = w.x & 0xffff, to[1] = w.x >> 16, to[2] = w.y & 0xffff, to[3] = w.y >> 16;
+  }
 }
 
 // Issues the copies of one tile: lane l holds the cache row of token l.

@@ -584,10 +584,11 @@ extern "C" int b200q_qk_norm_rope_bprop(const b200q_qk_norm_args* args, void* st
   const long long units = static_cast<long long>(t) * (lanes ? static_cast<int>(split.parts.d) : hq + hk);
   if (units > 0x7f000000ll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
   const int units_per_block = lanes ? kFastThreads / lanes : kNormWarps;
+  const int room = static_cast<int>(kScratchBytes / (2 * d * sizeof(float)));  // at least 2048 blocks' partial sums
   const int blocks = static_cast<int>(
-      std::max(1ll, std::min<long long>((units + units_per_block - 1) / units_per_block, sms * 4)));
+      std::max(1ll, std::min<long long>((units + units_per_block - 1) / units_per_block, std::min(sms * 4, room))));
   void* ws = nullptr;
-  if ((rc = host_workspace(static_cast<size_t>(blocks) * 2 * d * sizeof(float), cs, &ws))) return rc;
+  if ((rc = host_scratch(cs, &ws))) return rc;
   a.partial = static_cast<float*>(ws);
   const size_t smem = static_cast<size_t>(kNormWarps) * 2 * d * sizeof(float);
   B200Q_DISPATCH_FTYPE(ftype, {

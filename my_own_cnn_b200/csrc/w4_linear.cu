@@ -413,15 +413,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
 }
 
 template <typename T, int G, int NT, int FEW>
-int launch_linear(W4Args a, int sms, cudaStream_t stream) {
+int launch_linear(W4Args a, int sms, int device, cudaStream_t stream) {
   using L = Layout<T, G, NT, FEW>;
   constexpr int kSmem = L::kBytes;
   auto kernel = linear_w4_kernel<T, G, NT, FEW>;
-  static std::atomic<bool> ready{false};
-  if (!ready.load(std::memory_order_relaxed)) {
+  static std::atomic<bool> ready[kMaxDevices];
+  if (!ready[device].load(std::memory_order_relaxed)) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute(linear_w4_kernel)");
-    ready.store(true, std::memory_order_relaxed);
+    ready[device].store(true, std::memory_order_relaxed);
   }
   // K is split so that two blocks an SM are busy (FEW: and every warp has a step), and no further: fewer, longer streams
   // read faster
@@ -436,14 +436,14 @@ int launch_linear(W4Args a, int sms, cudaStream_t stream) {
 }
 
 template <typename T, int G>
-int launch_linear_rows(const W4Args& a, int sms, cudaStream_t stream) {
+int launch_linear_rows(const W4Args& a, int sms, int device, cudaStream_t stream) {
   // One row of x: 1 x 8192 x 8192 bf16 11.0 us, 12.0 with blocks of 256 weight rows; 1 x 16000 x 1000 7.2 and 12.9;
   // 1 x 768 x 768 3.1 and 4.5.  Two to four: only while those blocks, K split eight ways, would leave SMs idle
   // (2 x 16000 x 1000 fp32 8.9 and 16.1 us, but 4 x 8192 x 8192 bf16 22.2 and 13.0: each block brings x in).
-  if (a.m == 1 && a.k <= kMaxSplit * kStep * Layout<T, G, 1, 1>::kBuffers) return launch_linear<T, G, 1, 1>(a, sms, stream);
+  if (a.m == 1 && a.k <= kMaxSplit * kStep * Layout<T, G, 1, 1>::kBuffers) return launch_linear<T, G, 1, 1>(a, sms, device, stream);
   if (a.m <= kFewRows && (a.n + 255) / 256 * kMaxSplit < sms && a.k <= kMaxSplit * kStep * Layout<T, G, 1, kFewRows>::kBuffers)
-    return launch_linear<T, G, 1, kFewRows>(a, sms, stream);
-  return a.m <= 8 ? launch_linear<T, G, 1, 0>(a, sms, stream) : launch_linear<T, G, 2, 0>(a, sms, stream);
+    return launch_linear<T, G, 1, kFewRows>(a, sms, device, stream);
+  return a.m <= 8 ? launch_linear<T, G, 1, 0>(a, sms, device, stream) : launch_linear<T, G, 2, 0>(a, sms, device, stream);
 }
 
 }  // namespace
@@ -464,16 +464,16 @@ extern "C" int b200q_linear_w4(const b200q_linear_w4_args* p, void* stream) {
   if (reinterpret_cast<uintptr_t>(p->codes) & 15u)
     return host_fail(B200Q_ERR_INVALID_ARG, "4-bit weight codes must be 16-byte aligned");
   if (n > (1 << 28) || k > (1 << 28) || m > (1 << 19)) return host_fail(B200Q_ERR_UNSUPPORTED, "linear too large");
-  int sms = 0, *err = nullptr;
-  int rc = host_device(&sms, &err);
+  int sms = 0, device = 0, *err = nullptr;
+  int rc = host_device(&sms, &err, &device);
   if (rc) return rc;
   W4Args a{p->x, p->ldx, p->codes, static_cast<const uint16_t*>(p->scales), p->zeros, p->bias, p->y, p->ldy, m, n, k};
   const size_t size = ftype == B200Q_F32 ? 4 : 2;
   a.x_vec = (reinterpret_cast<uintptr_t>(p->x) & 15u) == 0 && (m == 1 || p->ldx * size % 16 == 0);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  B200Q_DISPATCH_FTYPE(ftype, rc = group == 32   ? launch_linear_rows<T, 32>(a, sms, cs)
-                                   : group == 64 ? launch_linear_rows<T, 64>(a, sms, cs)
-                                                 : launch_linear_rows<T, 128>(a, sms, cs));
+  B200Q_DISPATCH_FTYPE(ftype, rc = group == 32   ? launch_linear_rows<T, 32>(a, sms, device, cs)
+                                   : group == 64 ? launch_linear_rows<T, 64>(a, sms, device, cs)
+                                                 : launch_linear_rows<T, 128>(a, sms, device, cs));
   if (rc == B200Q_OK) host_set_path(17);
   return rc;
 }

@@ -201,6 +201,54 @@ def test_attention_views_of_queries_and_tables():
     assert b2q.kv4_attention(q, c, table, lens, out=out) is out and torch.equal(out, want)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("length", [40, 9000])
+def test_attention_output_at_any_element(dtype, length):
+    c, table, lens = filled([length], 2, 16, 64, 32)
+    q = torch.randn(1, 1, 6, 64, generator=gen(6), device="cuda").to(dtype)
+    want = b2q.kv4_attention(q, c, table, lens)
+    for at in range(1, 9):
+        store = torch.full((q.numel() + 16,), 7.0, dtype=dtype, device="cuda")
+        out = store[at:at + q.numel()].view(q.shape)
+        b2q.kv4_attention(q, c, table, lens, out=out)
+        assert torch.equal(out, want) and (store[:at] == 7).all() and (store[at + q.numel():] == 7).all()
+
+
+def test_a_graph_outlives_larger_calls_on_its_stream():
+    c, table, lens = filled([3000], 1, 16, 64, 64)
+    q = torch.randn(1, 1, 4, 64, generator=gen(7), device="cuda").bfloat16()
+    big, big_table, big_lens = filled([2000] * 40, 4, 16, 256, 64)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    want = b2q.kv4_attention(q, c, table, lens, stream=s)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        y = b2q.kv4_attention(q, c, table, lens)
+    b2q.kv4_attention(torch.zeros(40, 1, 32, 256, device="cuda"), big, big_table, big_lens, stream=s)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            g.replay()
+            b2q.kv4_attention(torch.zeros(40, 1, 32, 256, device="cuda"), big, big_table, big_lens)
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+
+
+def test_a_stream_without_scratch_is_not_captured():
+    c, table, lens = filled([100], 1, 16, 64, 64)
+    q = torch.randn(1, 1, 4, 64, generator=gen(8), device="cuda")
+    s = torch.cuda.Stream(priority=-1)
+    s.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=s):
+            b2q.kv4_attention(q, c, table, lens)
+    y = b2q.kv4_attention(q, c, table, lens, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(y, b2q.kv4_attention(q, c, table, lens))
+
+
 def test_attention_repeats_and_streams_and_graph():
     c, table, lens = filled([3000, 100, 0], 2, 64, 128, 64)
     q = torch.randn(3, 1, 8, 128, generator=gen(5), device="cuda").half()
