@@ -33,9 +33,9 @@ class W4Attention:
                 block_table: torch.Tensor, lens: torch.Tensor, stream=None) -> torch.Tensor:
         """x [b, tq, hidden]: the next tq tokens of each sequence; positions int32 and slots int64 [b * tq] place them;
         lens int32 [b] counts each sequence's tokens with the new ones.  Returns [b, tq, wo.n]."""
-        b, tq, hidden = x.shape
+        b, tq, _ = x.shape
         h, hk, d = self.heads, self.kv_heads, self.head_dim
-        qkv = linear_w4(x.reshape(b * tq, hidden), self.wqkv, stream=stream).view(b * tq, h + 2 * hk, d)
+        qkv = linear_w4(x, self.wqkv, stream=stream).view(b * tq, h + 2 * hk, d)
         q, k, v = qkv[:, :h], qkv[:, h:h + hk], qkv[:, h + hk:]
         qk_norm_rope(q, k, self.q_norm, self.k_norm, self.table, positions, self.eps, self.interleaved, q_out=q, k_out=k,
                      stream=stream)

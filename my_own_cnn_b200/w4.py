@@ -62,6 +62,8 @@ class W4Weight:
         if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != by_group or not zeros.is_contiguous()):
             raise RuntimeError(f"zeros must be contiguous uint8 {list(by_group)}, got {zeros.dtype} "
                                f"{list(zeros.shape)}")
+        if scales.device != codes.device or (zeros is not None and zeros.device != codes.device):
+            raise RuntimeError("codes, scales and zeros must be on one device")
         self.codes, self.scales, self.zeros = codes, scales, zeros
         self.n, self.k, self.group = n, k, group
 
@@ -105,7 +107,7 @@ def quantize_w4(w: torch.Tensor, group: int = 64, symmetric: bool = False) -> W4
 def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None, out: torch.Tensor | None = None,
               stream=None) -> torch.Tensor:
     """x [..., k] (fp32, fp16 or bf16; rows may be strided) -> [..., n] of the same type; fp32 sums.
-    bias: [n] of x's type."""
+    bias: [n] of x's type; out shares no memory with x."""
     ft = FTYPES.get(x.dtype)
     if ft is None or not x.is_cuda:
         _ftype(x, "x")
@@ -127,16 +129,16 @@ def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None, ou
 def _linear(x, w, bias, out, ft, n, k, stream):
     rows = x if x.dim() == 2 else x.reshape(-1, k)
     ldx, step = rows.stride()
-    if step != 1:
+    m = rows.shape[0]
+    if step != 1 or (ldx < k and m > 1):  # columns apart, or rows that overlap (a broadcast)
         rows = rows.contiguous()
         ldx = k
-    m = rows.shape[0]
     y, ldy = out, n
     if out is None:
         out = y = x.new_empty((m, n) if rows is x else x.shape[:-1] + (n,))
     else:
-        if out.dtype != x.dtype or out.shape != x.shape[:-1] + (n,):
-            raise RuntimeError(f"out must be {x.dtype} {list(x.shape[:-1] + (n,))}")
+        if out.dtype != x.dtype or out.shape != x.shape[:-1] + (n,) or not out.is_cuda:
+            raise RuntimeError(f"out must be a {x.dtype} {list(x.shape[:-1] + (n,))} CUDA tensor")
         if out.dim() == 2 and (out.stride(1) == 1 or n == 1):
             ldy = out.stride(0)
         elif not out.is_contiguous():

@@ -81,3 +81,11 @@ def test_block_refuses_projections_that_do_not_fit():
     block, _, _ = setup(torch.float32)
     with pytest.raises(RuntimeError, match="do not fit"):
         b2q.W4Attention(block.wqkv, block.wo, None, None, None, 5, 2, 64)
+
+
+def test_block_takes_tokens_in_any_layout():
+    block, cache, table = setup(torch.bfloat16)
+    x = torch.randn(320, 2, 3, device="cuda").bfloat16().permute(2, 1, 0)
+    at = torch.arange(2, device="cuda").expand(3, 2)
+    args = cache, at.int().flatten(), place(table, 16, at).flatten(), table, torch.full((3,), 2, dtype=torch.int32, device="cuda")
+    assert torch.equal(block.forward(x, *args), block.forward(x.contiguous(), *args))

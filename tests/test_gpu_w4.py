@@ -85,6 +85,19 @@ def test_rows_with_strides_and_any_alignment():
     check(b2q.linear_w4(cols, w), cols, w)
 
 
+def test_broadcast_and_overlapping_rows():
+    w = case(70, 96, 32)
+    row = torch.randn(200, generator=gen(12), device="cuda")
+    for x in (row[:96].expand(5, 96), row.as_strided((9, 96), (7, 1)), row[:96].expand(2, 3, 96)):
+        assert torch.equal(b2q.linear_w4(x, w), b2q.linear_w4(x.contiguous(), w))
+
+
+def test_out_must_be_on_the_device():
+    w = case(8, 64, 32)
+    with pytest.raises(RuntimeError, match="out must be"):
+        b2q.linear_w4(torch.zeros(2, 64, device="cuda"), w, out=torch.zeros(2, 8))
+
+
 def test_leading_dimensions_and_none():
     w = case(40, 64, 64)
     x = torch.randn(2, 3, 64, generator=gen(6), device="cuda")

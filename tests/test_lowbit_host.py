@@ -126,7 +126,16 @@ def test_attention_refusals():
     assert call(hq=3) == INVALID and b"divide" in L.b200q_last_error()
     assert call(lens=0) == INVALID and call(table=0) == INVALID and call(ft=7) == INVALID and call(tq=-1) == INVALID
     assert call(max_pages=1 << 28) == UNSUPPORTED
+    assert call(b=1 << 20, tq=1 << 16, hq=1 << 16) == UNSUPPORTED and b"too large" in L.b200q_last_error()
     assert call(b=0) == OK and call(tq=0) == OK and call(hq=0) == OK
     assert L.b200q_kv4_append(cache(), P, 0, 0, P, 0, 0, 0, 0, 1, 0) == INVALID
     assert L.b200q_kv4_append(cache(), P, 0, 0, P, 0, 0, P, 0, -1, 0) == INVALID
     assert L.b200q_kv4_append(cache(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0) == OK
+
+
+def test_weights_on_one_device():
+    codes, scales = torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(1, 4, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="one device"):
+        b2q.W4Weight(codes, scales.to("meta"), None, 4, 32, 32)
+    with pytest.raises(RuntimeError, match="one device"):
+        b2q.W4Weight(codes, scales, torch.zeros(1, 4, dtype=torch.uint8, device="meta"), 4, 32, 32)
