@@ -3,10 +3,10 @@
 //   y[m][n] = sum_g s[g][n] sum_{k in g} c[n][k] x[m][k]  -  sum_g s[g][n] z[g][n] sum_{k in g} x[m][k]
 //
 // Bytes bound it: K / 2 of codes and 2 or 3 per group for each weight row; and, as measured, the latency of its instructions
-// with 16 warps an SM.  1 x 8192 x 8192 bf16: 10.7 us, 3.3 TB/s; 16 x 16384 x 8192: 35.6 us, 2.1 TB/s; 1 x 768 x 768: 2.9 us.  The codes are the 16-row operand A of
-// m16n8k16 (weight rows x K) and up to 16 rows of x its 8 columns, once or twice; m16n8k16 from registers because a
-// code leaves its word as an operand in less than one instruction, while tcgen05 operands would have to be written to
-// shared memory first, four times the bytes that were read.
+// with 16 warps an SM.  1 x 8192 x 8192 bf16: 10.7 us, 3.3 TB/s; 16 x 16384 x 8192: 34.7 us, 2.1 TB/s; 1 x 768 x 768: 2.9 us.
+// The codes are the 16-row operand A of m16n8k16 (weight rows x K) and up to 16 rows of x its 8 columns, once or twice;
+// m16n8k16 from registers because a code leaves its word as an operand in less than one instruction, while tcgen05
+// operands would have to be written to shared memory first, four times the bytes that were read.
 //   Operands: a nibble in the low bits of an fp16 is the subnormal code * 2^-24, exactly, and one place higher
 //   code * 2^-20: a word of 8 codes becomes four operands, the pairs (0,4) (1,5) (2,6) (3,7), by one shift and four
 //   masks, and every second value of x is divided by 16 instead.  x is scaled by a power of two per row and step to a
@@ -61,12 +61,14 @@ template <typename T, int G, int NT, int FEW>
 struct Layout {
   static constexpr int kTerms = std::is_same<T, float>::value ? 2 : 1;
   static constexpr int kRowsX = FEW ? FEW : 8 * NT;    // rows of x that there is room for
-  static constexpr int kStages = FEW ? 2 : 3;
-  static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kRowsW = FEW ? 32 : 32 * kWarps;     // weight rows of a block
   static constexpr int kX = kStep * 2 * kTerms * kRowsX;
   static constexpr int kXSum = kTerms == 2 ? 0 : (kStep / G) * kRowsX * 4;
   static constexpr int kBuffer = (kX + kXSum + kRowsX * 4 + 15) / 16 * 16;
+  // Three stages where two blocks still fit an SM (228 KB, 1 KB of it taken per block); 16 rows of fp32, or of 32 weights a
+  // group, leave room for two: 16 x 11000 x 12000 fp32 48 us, 69 with one block and three; 16 x 16384 x 8192 bf16 40, 61.
+  static constexpr int kStages = FEW || kWarps * 3 * kStage + 2 * kBuffer > 113 * 1024 ? 2 : 3;
+  static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kBuffers = FEW ? (46 * 1024) / kBuffer : 2;
   static constexpr int kBytes = kRing + kBuffers * kBuffer;
 };
@@ -212,12 +214,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
   for (int n = 0; n < NT; ++n) acc[0][n][0] = acc[0][n][1] = acc[1][n][0] = acc[1][n][1] = both(0.0f);
 #pragma unroll
   for (int m = 0; m < kLess; ++m) less[m] = both(0.0f);
-  if (steps > 0) load_params(0);
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    if (s < steps) load_step(s, s);
-    copy_commit();
-  }
   constexpr int kRowsWarp = FEW ? 4 : NT;  // rows of a step that a warp has on their way at a time
   XRow<T> x[kRowsWarp];
   auto load_x = [&](int step) {  // rows w, w + 8 of one step
@@ -230,6 +226,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
     for (int i = 0; i < kRowsWarp; ++i)
       if (i * kWarps + warp < rows) x[i].template store<G, L>(buffers + buffer * L::kBuffer, i * kWarps + warp);
   };
+  if constexpr (!FEW)
+    if (steps > 0) load_x(0);  // before the codes: it is needed first
+  if (steps > 0) load_params(0);
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) {
+    if (s < steps) load_step(s, s);
+    copy_commit();
+  }
   if constexpr (FEW) {  // every row of every step, dealt out to the warps
     for (int p0 = warp; p0 < rows * count; p0 += kWarps * kRowsWarp) {
 #pragma unroll
@@ -244,10 +248,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
       }
     }
   } else {
-    if (steps > 0) {
-      load_x(0);
-      store_x(0);
-    }
+    if (steps > 0) store_x(0);
     if (steps > 1) load_x(1);
   }
   __syncthreads();
@@ -371,8 +372,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
   copy_wait<0>();
   if constexpr (FEW) __syncthreads();  // the rings are done with
 
-  float* const all = reinterpret_cast<float*>(smem);  // [warp][kRowsX][32]
-  float* const sums = all + warp * (kRowsX * 32);
+  constexpr int kPitch = 36;  // of 32 weight rows: stores of rows 2 t, columns g touch every bank once
+  static_assert(kWarps * kRowsX * kPitch * 4 <= L::kRing, "the sums lie over the rings");
+  float* const all = reinterpret_cast<float*>(smem);  // [warp][kRowsX][kPitch]
+  float* const sums = all + warp * (kRowsX * kPitch);
 #pragma unroll
   for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -380,14 +383,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         if (FEW && 2 * t >= kRowsX) continue;
-        float* to = sums + (n * 8 + 2 * t) * 32 + mt * 16 + u * 8 + g;
+        float* to = sums + (n * 8 + 2 * t) * kPitch + mt * 16 + u * 8 + g;
         constexpr float kUnit = kF32 ? 1.0f : 16777216.0f;  // subnormal codes count 2^-24
         to[0] = acc[mt][n][u].x * kUnit;
-        if (kRowsX > 1) to[32] = acc[mt][n][u].y * kUnit;
+        if (kRowsX > 1) to[kPitch] = acc[mt][n][u].y * kUnit;
       }
   __syncwarp();
 #pragma unroll
-  for (int m = 0; m < kRowsX; ++m) sums[m * 32 + lane] -= m % 2 ? less[m / 2].y : less[m / 2].x;
+  for (int m = 0; m < kRowsX; ++m) sums[m * kPitch + lane] -= m % 2 ? less[m / 2].y : less[m / 2].x;
   if (splits > 1)
     cluster_sync();
   else
@@ -398,14 +401,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
   for (int i = threadIdx.x; i < wide * rows; i += kWarps * 32) {
     const int m = i / wide, r = from + i % wide, n = n0 + r;
     if (n >= a.n) continue;
-    const int at = (FEW ? 0 : r / 32 * (kRowsX * 32)) + m * 32 + r % 32;
+    const int at = (FEW ? 0 : r / 32 * (kRowsX * kPitch)) + m * kPitch + r % 32;
     float v = 0.0f;
-    for (int j = 0; j < splits; ++j)
+    constexpr int kEach = FEW ? kWarps : 1;
+    if (splits > 1) {
+      constexpr int kTogether = 4;  // blocks whose sums are on their way at a time
+      for (int j = 0; j < splits; j += kTogether) {
+        float part[kTogether][kEach];
 #pragma unroll
-      for (int w = 0; w < (FEW ? kWarps : 1); ++w) {
-        const int each = at + w * (kRowsX * 32);
-        v += splits > 1 ? peer_load(mine + each * 4, j) : all[each];
+        for (int u = 0; u < kTogether; ++u)
+#pragma unroll
+          for (int w = 0; w < kEach; ++w)
+            part[u][w] = j + u < splits ? peer_load(mine + (at + w * (kRowsX * kPitch)) * 4, j + u) : 0.0f;
+#pragma unroll
+        for (int u = 0; u < kTogether; ++u)
+#pragma unroll
+          for (int w = 0; w < kEach; ++w) v += part[u][w];
       }
+    } else {
+#pragma unroll
+      for (int w = 0; w < kEach; ++w) v += all[at + w * (kRowsX * kPitch)];
+    }
     if (a.bias) v += to_f32(static_cast<const T*>(a.bias)[n]);
     static_cast<T*>(a.y)[(m0 + m) * a.ldy + n] = from_f32<T>(v);
   }
