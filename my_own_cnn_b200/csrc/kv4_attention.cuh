@@ -13,7 +13,7 @@
 //   Values (and keys in fp32 calls): 1024 + code less 1024 + zero point, exact and normal (2 x 131072 fp16: off by 2.7e-4,
 //   6.6e-4 with subnormals); channels are rows, and one whose nibble lies one place higher has its sum divided by 16 at the
 //   end.  P is fp16 (11 bits; two terms, 22 bits, in fp32 calls) times a power of two that follows the largest
-//   vs that the warp has met, so that full precision holds for tokens whose vs is up to 2^20 below that.  The adder
+//   finite vs that the warp has met, so that full precision holds for tokens whose vs is up to 2^20 below that.  The adder
 //   truncates, so fp32 calls add a tile's sums up outside of it.
 //   P leaves the first product as (token, row) and must enter the second as (row, token): movmatrix.
 // The maximum m[r] is a running reference, raised (and the sums rescaled) only when a score passes it by more than
@@ -22,7 +22,7 @@
 // Work: a unit is (sequence, cache head, tile of rows), in steps of kWarps tiles of kTile tokens.  All units' steps lie
 // end to end, and each block takes the same number of them, whatever the lengths (which only the device knows): none waits
 // for a last wave.  The parts of a unit that several blocks share go to
-// the workspace, and the block that finishes last joins them in order.
+// the scratch, and the block that finishes last joins them in order.
 //
 // What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head; and, as measured, the latency of about 630
 // instructions per warp and tile with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 69 us,
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
           z_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 16 & 15u | 0x6400u);
           z16_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 12 & 0xF0u | 0x6400u);
           vs[k] = param_scale(q);
-          v_top = fmaxf(v_top, vs[k]);
+          v_top = fmaxf(v_top, vs[k] < INFINITY ? vs[k] : 0.0f);
         }
         if (__any_sync(~0u, v_top > v_limit)) {
           const int now = max(1, min(247, static_cast<int>(__float_as_uint(warp_max(v_top)) >> 23)));
@@ -444,7 +444,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
             for (int j = 0; j < D / 16; ++j) o[j][n][0] *= keep, o[j][n][1] *= keep, o[j][n][2] *= keep, o[j][n][3] *= keep;
         }
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) v_prep[k * kTile + lane] = vs[k] * v_factor;
+        for (int k = 0; k < kGroups; ++k)  // an infinite scale is for the rows that see it: P 0 times the largest number is 0
+          v_prep[k * kTile + lane] = fminf(vs[k] * v_factor, 3.402823466e38f);
       }
       __syncwarp();
 
@@ -700,7 +701,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
     }
     __syncthreads();
 
-    // the block's rows: straight to the output, or to the workspace for the unit's last block to join
+    // the block's rows: straight to the output, or to the scratch for the unit's last block to join
     auto finish = [&](int r, int d, float4 v) {
       const float2 ml = row_all[r];
       const float over = ml.y > 0.0f ? 1.0f / ml.y : 0.0f;  // no tokens: 0

@@ -202,6 +202,24 @@ def test_attention_views_of_queries_and_tables():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_attention_hides_what_a_row_does_not_see(dtype, what, bad):
+    """A token with an infinite or NaN channel is met by its own row and later ones, not by the rows before it."""
+    c, table, lens = filled([50], 2, 16, 64, 32)
+    q = torch.randn(1, 3, 4, 64, generator=gen(13), device="cuda").to(dtype)
+    want = b2q.kv4_attention(q, c, table, lens)
+    slot = (table[0, 48 // 16].long() * 16 + 48 % 16).view(1)  # the last row but one's own token
+    k, v = b2q.kv4_read(c, slot)
+    (k if what == "k" else v)[..., 5] = bad
+    b2q.kv4_append(c, k, v, slot)
+    out = b2q.kv4_attention(q, c, table, lens)
+    assert torch.equal(out[:, 0], want[:, 0])
+    if what == "v" and bad == bad:  # not hidden from those that see it (an infinite key may give a score of -inf, weight 0)
+        assert not out[:, 1:].isfinite().all(-1).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("length", [40, 9000])
 def test_attention_output_at_any_element(dtype, length):
     c, table, lens = filled([length], 2, 16, 64, 32)
