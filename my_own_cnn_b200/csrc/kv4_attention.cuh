@@ -1,18 +1,17 @@
 // Attention of a few query rows over the 4-bit cache, on tensor cores.
 //
 // For one sequence and cache head with rows r (new tokens x query heads that share the head), tokens t:
-//   S[t][r] = sum_g ks[t,g] (sum_{d in g} kc[t,d] q[r,d]  -  kz[t,g] sum_{d in g} q[r,d])
+//   S[t][r] = sum_g ks[t,g] sum_{d in g} (kc[t,d] - kz[t,g]) q[r,d]
 //   O[d][r] = sum_t (vc[t,d] - vz[t,g]) P[t,r],   P[t,r] = vs[t,g] exp2(f[r] S[t][r] - m[r])
 // Both products take the codes as the 16-row operand A of m16n8k16 (tokens x channels, then channels x tokens)
 // and the rows as its 8 columns, so 8 rows cost one instruction per 256 codes.
-//   Keys: a nibble in the low bits of an fp16 is the subnormal code * 2^-24, exactly, and one place higher
-//   code * 2^-20: a word of 8 codes becomes four operands by masking, and every second query value is divided
-//   by 16 instead.  Query rows are scaled by a power of two to a maximum in [2^14, 2^15), so that they fit
-//   fp16 whatever their type; fp32 rows are split into two fp16 terms (22 bits).  The adder lines subnormals up by
-//   their exponent field, which costs about 10 of the sum's bits: scores stay good to about 2e-5, enough for the 16-bit types.
-//   Values (and keys in fp32 calls): 1024 + code less 1024 + zero point, exact and normal (2 x 131072 fp16: off by 2.7e-4,
-//   6.6e-4 with subnormals); channels are rows, and one whose nibble lies one place higher has its sum divided by 16 at the
-//   end.  P is fp16 (11 bits; two terms, 22 bits, in fp32 calls) times a power of two that follows the largest
+//   Operands: a nibble put into the low bits of the fp16 1024 is 1024 + code, and one place higher 1024 + 16 code; less the
+//   same of the zero point it is exact and normal.  (The bare nibble, a subnormal, saves the subtraction, 69.0 against 71.3 us
+//   below, but the adder lines subnormals up by their exponent field and loses about 10 of the sum's bits: log-sums of
+//   short sequences off by 1.7e-6, 5e-8 so; 2 x 131072 fp16 outputs off by 6.6e-4, 2.7e-4 so.)
+//   Keys: every second query value is divided by 16 for the codes one place higher.  Query rows are scaled by a power of
+//   two to a maximum in [2^14, 2^15), so that they fit fp16 whatever their type; fp32 rows are split into two fp16 terms (22 bits).
+//   Values: channels are rows, and one whose nibble lies one place higher has its sum divided by 16 at the end.  P is fp16 (11 bits; two terms, 22 bits, in fp32 calls) times a power of two that follows the largest
 //   finite vs that the warp has met, so that full precision holds for tokens whose vs is up to 2^20 below that.  The adder
 //   truncates, so fp32 calls add a tile's sums up outside of it.
 //   P leaves the first product as (token, row) and must enter the second as (row, token): movmatrix.
@@ -24,9 +23,9 @@
 // for a last wave.  The parts of a unit that several blocks share go to
 // the scratch, and the block that finishes last joins them in order.
 //
-// What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head; and, as measured, the latency of about 630
-// instructions per warp and tile with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 69 us,
-// 3.3 TB/s; 2 x 131072, fp16: 87 us, 3.5 TB/s; 1 x 77 fp32: 6 us, all latency.
+// What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head; and, as measured, the latency of about 650
+// instructions per warp and tile with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 71 us,
+// 3.2 TB/s; 2 x 131072, fp16: 89 us, 3.4 TB/s; 1 x 77 fp32: 6 us, all latency.
 //   Each warp owns a ring of kStages tiles of kTile tokens that it fills with 16-byte asynchronous copies and empties on its
 // own: no block-wide barrier until the end.  A row of codes is padded by 16 bytes in shared memory: then lanes (g, t)
 // reading 4 bytes at g rows down, and 2t rows down, both touch 32 banks once.
@@ -87,7 +86,7 @@ struct AttnShape {
   static constexpr int kBody = kRing > kJoin ? kRing : kJoin;
   static constexpr int kTileParams = kTile * kGroups * 16;        // a warp's tile: see Prepared
   static constexpr int kRowsMl = kWarps * 8 * NT * 2 * 4;
-  static constexpr int kSmem = kBody + kQuery + kWarps * kTileParams + kRowsMl + 8 * NT * (kGroups + 1) * 4 + 8 * NT * 20;
+  static constexpr int kSmem = kBody + kQuery + kWarps * kTileParams + kRowsMl + 8 * NT * 24;
 };
 
 // Row of the cache that holds token `tok`, or ~0 where there is none to read.
@@ -206,8 +205,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
   uint4* const query = reinterpret_cast<uint4*>(smem + Shape::kBody);
   uint8_t* const prepared = smem + Shape::kBody + Shape::kQuery + (threadIdx.x / 32) * Shape::kTileParams;
   float* const row_ml = reinterpret_cast<float*>(smem + Shape::kBody + Shape::kQuery + kWarps * Shape::kTileParams);
-  float* const row_sum = row_ml + kWarps * kRows * 2;  // [kGroups][kRows] sums of the scaled query, times 2^-24
-  float* const row_f = row_sum + kRows * kGroups;
+  float* const row_f = row_ml + kWarps * kRows * 2;
   int64_t* const row_out = reinterpret_cast<int64_t*>(row_f + kRows);
   float2* const row_all = reinterpret_cast<float2*>(row_out + kRows);
   int* const row_limit = reinterpret_cast<int*>(row_all + kRows);  // tokens that a row sees
@@ -349,13 +347,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
       }
       const Power power = power_for(warp_max(top));
       if (lane == 0) {
-        row_f[r] = power.down * a.scale * 1.4426950408889634f * (F32 ? 1.0f : 16777216.0f);
+        row_f[r] = power.down * a.scale * 1.4426950408889634f;
         row_limit[r] = len - a.tq + (tile * kRows + min(r, rows - 1)) / ratio + 1;
       }
       // lane: channel p = lane % 8 of the 8 that thread lane / 8 of a quad holds; pairs are (0,4) (1,5) (2,6) (3,7)
       const int p = lane % 8, holder = (r % 8) * 4 + lane / 8;
       __half* to = reinterpret_cast<__half*>(query);
-      float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         float x = v[i] * power.up;
@@ -363,15 +360,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
         for (int term = 0; term < kTerms; ++term) {
           const __half hv = __float2half_rn(x);
           const float back = __half2float(hv);
-          sum += back;
           x -= back;
           to[(((i * kTerms + term) * NT + r / 8) * 32 + holder) * 8 + (p % 4) * 2 + p / 4] =
               p % 2 ? __float2half_rn(back * 0.0625f) : hv;
-        }
-        if ((i + 1) % (G / 32) == 0) {
-          sum = warp_sum(sum);
-          if (lane == 0) row_sum[(i / (G / 32)) * kRows + r] = sum * (1.0f / 16777216.0f);
-          sum = 0.0f;
         }
       }
     }
@@ -412,7 +403,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
       const bool whole = here == ~0u && base + kTile <= all_see;
 
       // lane l unpacks token l's scales and zero points for the lanes that use them: [group][token] (key scale, key zero
-      // point), then value scales times P's power, then value zero points z as the fp16 1024 + z and 1024 + 16 z
+      // point z as a pair of the fp16 1024 + z), then value scales times P's power, then value zero points z as the fp16 1024 + z and 1024 + 16 z
       float2* const k_prep = reinterpret_cast<float2*>(prepared);
       float* const v_prep = reinterpret_cast<float*>(prepared + kTile * kGroups * 8);
       uint16_t* const z_prep = reinterpret_cast<uint16_t*>(prepared + kTile * kGroups * 12);
@@ -423,9 +414,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) {
           const uint32_t p = kp[lane * kGroups + k], q = there ? vp[lane * kGroups + k] : 0u;  // places that hold nothing hold any bits
-          // the key's zero point negated, or in fp32 calls as a pair of the fp16 1024 + z
-          k_prep[k * kTile + lane] = make_float2(
-              param_scale(p), F32 ? __uint_as_float((p >> 16 & 15u) * 0x00010001u | kMagic) : -zero_point(p));
+          k_prep[k * kTile + lane] = make_float2(param_scale(p), __uint_as_float((p >> 16 & 15u) * 0x00010001u | kMagic));
           z_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 16 & 15u | 0x6400u);
           z16_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 12 & 0xF0u | 0x6400u);
           vs[k] = param_scale(q);
@@ -470,12 +459,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const uint32_t mask = j % 2 ? 0x00F000F0u : 0x000F000Fu;
-                if constexpr (F32) {
-                  const uint32_t z = __float_as_uint(k_prep[k * kTile + mt * 16 + u * 8 + g].y);
-                  c[u][j] = sub_f16x2(and_or(w >> (j / 2 * 8), mask, kMagic), j % 2 ? and_or(z << 4, 0x00F000F0u, kMagic) : z);
-                } else {
-                  c[u][j] = w >> (j / 2 * 8) & mask;
-                }
+                const uint32_t z = __float_as_uint(k_prep[k * kTile + mt * 16 + u * 8 + g].y);
+                c[u][j] = sub_f16x2(and_or(w >> (j / 2 * 8), mask, kMagic), j % 2 ? and_or(z << 4, 0x00F000F0u, kMagic) : z);
               }
             }
 #pragma unroll
@@ -494,13 +479,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const float2 p = k_prep[k * kTile + mt * 16 + u * 8 + g];
-            const float2 ks = both(p.x), kz = both(p.y);
+            const float2 ks = both(k_prep[k * kTile + mt * 16 + u * 8 + g].x);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const float* at = part[mt][n] + 2 * u;
-              float2 v = make_float2(at[0], at[1]);
-              if constexpr (!F32) v = fma2(kz, *reinterpret_cast<const float2*>(row_sum + k * kRows + n * 8 + 2 * t), v);
+              const float2 v = make_float2(at[0], at[1]);
               s[mt][n][u] = k == 0 ? mul2(ks, v) : fma2(ks, v, s[mt][n][u]);
             }
           }

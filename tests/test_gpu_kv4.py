@@ -202,6 +202,18 @@ def test_attention_views_of_queries_and_tables():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,group", [(64, 32), (128, 64), (256, 64)])
+def test_log_sums_are_fp32(dtype, d, group):
+    """One token: the log-sum is its score, d / 16 additions that may truncate at 2^-23, and the scaling after them."""
+    c, table, lens = filled([1] * 60, 2, 16, d, group)
+    q = torch.randn(60, 1, 6, d, generator=gen(14), device="cuda").to(dtype)
+    _, lse = b2q.kv4_attention(q, c, table, lens, return_lse=True)
+    k, _ = b2q.kv4_read(c, table[:, 0].long() * 16)
+    want = (q.double().view(60, 2, 3, d) * k.double()[:, :, None]).sum(-1).view(60, 1, 6) * d ** -0.5
+    assert (lse.double() - want).norm() <= 2.0 ** -23 * (d / 16 + 2) * want.norm()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("what", ["k", "v"])
 @pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
 def test_attention_hides_what_a_row_does_not_see(dtype, what, bad):
