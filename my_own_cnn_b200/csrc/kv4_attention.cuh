@@ -191,7 +191,7 @@ struct Plan {
   int unit_seq, head, tile, begins, owner, parts;
 };
 
-// Blocks an SM: three at up to 168 registers a thread for heads of 128 (2 x 131072 tokens: 88 us, 98 with four and spills),
+// Blocks an SM: three at up to 168 registers a thread for heads of 128 (2 x 131072 tokens: 89 us, 98 with four and spills),
 // four for heads of 64 (63 us, 69 with three); 16 rows a pass or 256 channels take what they need.
 template <int D, int G, int NT, bool F32>
 __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128 ? 3 : 4) kv4_attention_kernel(Cache c, AttnArgs a) {
