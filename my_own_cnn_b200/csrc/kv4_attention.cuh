@@ -5,15 +5,18 @@
 //   O[d][r] = sum_t (vc[t,d] - vz[t,g]) P[t,r],   P[t,r] = vs[t,g] exp2(f[r] S[t][r] - m[r])
 // Both products take the codes as the 16-row operand A of m16n8k16 (tokens x channels, then channels x tokens)
 // and the rows as its 8 columns, so 8 rows cost one instruction per 256 codes.
-//   Operands: a nibble put into the low bits of the fp16 1024 is 1024 + code, and one place higher 1024 + 16 code; less the
+//   Keys' operands: a nibble put into the low bits of the fp16 1024 is 1024 + code, and one place higher 1024 + 16 code; less the
 //   same of the zero point it is exact and normal.  (The bare nibble, a subnormal, saves the subtraction, 69.0 against 71.3 us
 //   below, but the adder lines subnormals up by their exponent field and loses about 10 of the sum's bits: log-sums of
 //   short sequences off by 1.7e-6, 5e-8 so; 2 x 131072 fp16 outputs off by 6.6e-4, 2.7e-4 so.)
 //   Keys: every second query value is divided by 16 for the codes one place higher.  Query rows are scaled by a power of
 //   two to a maximum in [2^14, 2^15), so that they fit fp16 whatever their type; fp32 rows are split into two fp16 terms (22 bits).
-//   Values: channels are rows, and one whose nibble lies one place higher has its sum divided by 16 at the end.  P is fp16 (11 bits; two terms, 22 bits, in fp32 calls) times a power of two that follows the largest
-//   finite vs that the warp has met, so that full precision holds for tokens whose vs is up to 2^20 below that.  The adder
-//   truncates, so fp32 calls add a tile's sums up outside of it.
+//   Values: 128 + code less 128 + zero point in bf16, exact. P is fp32's value in bf16 terms, each of which has fp32's range:
+//   two (17 bits or more) in 16-bit calls, three (24) in fp32 ones, for every token, however small its weight or its scale beside
+//   the others'.  (fp16 weights of 11 and 22 bits take 71 and 92 us below, but on a step of 2^-24 of the largest they put 16-bit
+//   outputs off by 2e-4 before their own rounding, and fp32 ones by 1e-5 to 6e-2 where one token or one group of channels
+//   outweighs the rest by 2^10 to 2^20.)
+//   The adder truncates, so fp32 calls add a tile's sums up outside of it.
 //   P leaves the first product as (token, row) and must enter the second as (row, token): movmatrix.
 // The maximum m[r] is a running reference, raised (and the sums rescaled) only when a score passes it by more than
 // 2^8: a warp-wide maximum is taken a few times per sequence, not per tile.
@@ -23,9 +26,9 @@
 // for a last wave.  The parts of a unit that several blocks share go to
 // the scratch, and the block that finishes last joins them in order.
 //
-// What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head; and, as measured, the latency of about 650
-// instructions per warp and tile with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 71 us,
-// 3.2 TB/s; 2 x 131072, fp16: 89 us, 3.4 TB/s; 1 x 77 fp32: 6 us, all latency.
+// What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head; and, as measured, the latency of its
+// instructions with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 79.5 us,
+// 2.8 TB/s; 2 x 131072, fp16: 101 us, 3.0 TB/s; 1 x 77 fp32: 6 us, all latency.
 //   Each warp owns a ring of kStages tiles of kTile tokens that it fills with 16-byte asynchronous copies and empties on its
 // own: no block-wide barrier until the end.  A row of codes is padded by 16 bytes in shared memory: then lanes (g, t)
 // reading 4 bytes at g rows down, and 2t rows down, both touch 32 banks once.
@@ -72,6 +75,9 @@ constexpr int kWarps = 4;    // a block's warps take tiles in turn
 constexpr int kStages = 2;   // tiles of a warp's ring: a third one costs a block an SM for heads of 256 (125 against 93 us)
 constexpr int kStepTokens = kWarps * kTile;
 
+// How far a weight may pass 1 before its row's reference is raised, and its logarithm.
+constexpr float kLag = 256.0f, kLagLog = 8.0f;
+
 template <int D, int G, int NT, bool F32>
 struct AttnShape {
   static constexpr int kPitch = D / 2 + 16;
@@ -84,7 +90,7 @@ struct AttnShape {
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kJoin = kWarps * 8 * NT * (D + 4) * 4;      // the warps' sums, over the ring
   static constexpr int kBody = kRing > kJoin ? kRing : kJoin;
-  static constexpr int kTileParams = kTile * kGroups * 16;        // a warp's tile: see Prepared
+  static constexpr int kTileParams = kTile * kGroups * 14;        // a warp's tile: what its lanes unpack for one another
   static constexpr int kRowsMl = kWarps * 8 * NT * 2 * 4;
   static constexpr int kSmem = kBody + kQuery + kWarps * kTileParams + kRowsMl + 8 * NT * 24;
 };
@@ -383,9 +389,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.0f;
 
-    // P's power of two: 2^(127 - v_exp), for a largest vs of 2^(v_exp - 127)
-    int v_exp = 127;
-    float v_factor = 1.0f, v_limit = -1.0f;
     int slot = 0, fill = kStages - 1;
     for (int it = 0; it < mine; ++it) {
       copy_wait<kStages - 2>();
@@ -403,39 +406,24 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
       const bool whole = here == ~0u && base + kTile <= all_see;
 
       // lane l unpacks token l's scales and zero points for the lanes that use them: [group][token] (key scale, key zero
-      // point z as a pair of the fp16 1024 + z), then value scales times P's power, then value zero points z as the fp16 1024 + z and 1024 + 16 z
+      // point z as a pair of the fp16 1024 + z), then value scales over kLag, then value zero points z as the bf16 128 + z
       float2* const k_prep = reinterpret_cast<float2*>(prepared);
       float* const v_prep = reinterpret_cast<float*>(prepared + kTile * kGroups * 8);
       uint16_t* const z_prep = reinterpret_cast<uint16_t*>(prepared + kTile * kGroups * 12);
-      uint16_t* const z16_prep = z_prep + kTile * kGroups;
+      bool unbounded = false;
       {
-        float vs[kGroups], v_top = 0.0f;
         const bool there = here >> lane & 1;
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) {
           const uint32_t p = kp[lane * kGroups + k], q = there ? vp[lane * kGroups + k] : 0u;  // places that hold nothing hold any bits
           k_prep[k * kTile + lane] = make_float2(param_scale(p), __uint_as_float((p >> 16 & 15u) * 0x00010001u | kMagic));
-          z_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 16 & 15u | 0x6400u);
-          z16_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 12 & 0xF0u | 0x6400u);
-          vs[k] = param_scale(q);
-          v_top = fmaxf(v_top, vs[k] < INFINITY ? vs[k] : 0.0f);
+          z_prep[k * kTile + lane] = static_cast<uint16_t>(q >> 16 & 15u | 0x4300u);
+          const float vs = param_scale(q);
+          unbounded |= !(fabsf(vs) < INFINITY);
+          v_prep[k * kTile + lane] = vs * (1.0f / kLag);
         }
-        if (__any_sync(~0u, v_top > v_limit)) {
-          const int now = max(1, min(247, static_cast<int>(__float_as_uint(warp_max(v_top)) >> 23)));
-          float keep = now - v_exp < 127 ? __uint_as_float(static_cast<uint32_t>(127 + v_exp - now) << 23) : 0.0f;
-          if (v_limit < 0.0f) keep = 1.0f;  // no sums yet
-          v_exp = now;
-          v_factor = __uint_as_float(static_cast<uint32_t>(254 - now) << 23);
-          v_limit = __uint_as_float(static_cast<uint32_t>(now + 6) << 23);
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j) o[j][n][0] *= keep, o[j][n][1] *= keep, o[j][n][2] *= keep, o[j][n][3] *= keep;
-        }
-#pragma unroll
-        for (int k = 0; k < kGroups; ++k)  // an infinite scale is for the rows that see it: P 0 times the largest number is 0
-          v_prep[k * kTile + lane] = fminf(vs[k] * v_factor, 3.402823466e38f);
       }
+      unbounded = __any_sync(~0u, unbounded);
       __syncwarp();
 
       // scores
@@ -509,7 +497,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
           }
         top[n][0] = fmaxf(fmaxf(s[0][n][0].x, s[0][n][1].x), fmaxf(s[1][n][0].x, s[1][n][1].x));
         top[n][1] = fmaxf(fmaxf(s[0][n][0].y, s[0][n][1].y), fmaxf(s[1][n][0].y, s[1][n][1].y));
-        raise |= top[n][0] > m[n][0] + 8.0f || top[n][1] > m[n][1] + 8.0f;
+        raise |= top[n][0] > m[n][0] + kLagLog || top[n][1] > m[n][1] + kLagLog;
       }
       if (__any_sync(~0u, raise)) {
 #pragma unroll
@@ -541,7 +529,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
       }
 
       // values; in fp32 calls a tile's sums are made apart and added with rounding
-      constexpr int kPTerms = F32 ? 2 : 1;
+      constexpr int kPTerms = F32 ? 3 : 2;
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) {
         float part[G / 16][NT][4];
@@ -555,12 +543,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               float2 x = mul2(s[mt][n][u], scale);
+              if (unbounded) {  // an infinite or NaN scale is for the rows that see its token
+                if (s[mt][n][u].x == 0.0f) x.x = 0.0f;
+                if (s[mt][n][u].y == 0.0f) x.y = 0.0f;
+              }
 #pragma unroll
               for (int term = 0; term < kPTerms; ++term) {
-                const uint32_t v = pack_f16(x.x, x.y);
+                const uint32_t v = pack_bf16(x.x, x.y);
                 if (term + 1 < kPTerms) {
-                  const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&v));
-                  x = make_float2(x.x - back.x, x.y - back.y);
+                  x = fma2(make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)), both(-1.0f), x);
+                  if (unbounded) {  // what is left of an infinity
+                    if (x.x != x.x) x.x = 0.0f;
+                    if (x.y != x.y) x.y = 0.0f;
+                  }
                 }
                 b[term][n][u] = transpose_8x8(v);
               }
@@ -568,7 +563,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
           }
           // operand A: tokens 2t, 2t + 1 (u = 0) and 2t + 8, 2t + 9 (u = 1) of this lane's G / 8 channels, the lower
           // half of them as row g of the group's G / 16 products, the upper as row g + 8
-          uint32_t lower[2], upper[2], zero[2], zero16[2];
+          uint32_t lower[2], upper[2], zero[2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int tok = mt * 16 + u * 8 + 2 * t;
@@ -583,27 +578,24 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
               upper[u] = lower[u] >> 8;
             }
             zero[u] = *reinterpret_cast<const uint32_t*>(z_prep + k * kTile + tok);
-            zero16[u] = *reinterpret_cast<const uint32_t*>(z16_prep + k * kTile + tok);
           }
 #pragma unroll
           for (int j = 0; j < G / 16; ++j) {
-            const int down = j / 2 * 8;
-            const uint32_t mask = j % 2 ? 0x00F000F0u : 0x000F000Fu;
-            const uint32_t z0 = j % 2 ? zero16[0] : zero[0], z1 = j % 2 ? zero16[1] : zero[1];
-            const uint32_t a0 = sub_f16x2(and_or(lower[0] >> down, mask, kMagic), z0);
-            const uint32_t a1 = sub_f16x2(and_or(upper[0] >> down, mask, kMagic), z0);
-            const uint32_t a2 = sub_f16x2(and_or(lower[1] >> down, mask, kMagic), z1);
-            const uint32_t a3 = sub_f16x2(and_or(upper[1] >> down, mask, kMagic), z1);
+            constexpr uint32_t kMask = 0x000F000Fu, kMagic128 = 0x43004300u;  // two bf16 128: with a code in the low bits 128 + code
+            const uint32_t a0 = sub_bf16x2(and_or(lower[0] >> 4 * j, kMask, kMagic128), zero[0]);
+            const uint32_t a1 = sub_bf16x2(and_or(upper[0] >> 4 * j, kMask, kMagic128), zero[0]);
+            const uint32_t a2 = sub_bf16x2(and_or(lower[1] >> 4 * j, kMask, kMagic128), zero[1]);
+            const uint32_t a3 = sub_bf16x2(and_or(upper[1] >> 4 * j, kMask, kMagic128), zero[1]);
 #pragma unroll
             for (int term = 0; term < kPTerms; ++term)
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 if (!F32)
-                  mma_f16(o[k * (G / 16) + j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
+                  mma_bf16(o[k * (G / 16) + j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
                 else if (mt == 0 && term == 0)
-                  mma_f16_first(part[j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
+                  mma_bf16_first(part[j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
                 else
-                  mma_f16(part[j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
+                  mma_bf16(part[j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
               }
           }
         }
@@ -648,7 +640,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) now = fmaxf(now, row_ml[(w * kRows + r) * 2]);
         const float keep = m[n][e] == -INFINITY ? 0.0f : exp2_approx(m[n][e] - now);
-        const float value = __uint_as_float(static_cast<uint32_t>(v_exp) << 23);
         float* to = sums + (warp * kRows + r) * (D + 4);
 #pragma unroll
         for (int k = 0; k < kGroups; ++k)
@@ -656,7 +647,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
           for (int u = 0; u < 2; ++u) {
             float v[G / 16];
 #pragma unroll
-            for (int j = 0; j < G / 16; ++j) v[j] = o[k * (G / 16) + j][n][2 * u + e] * ((j % 2 ? 0.0625f : 1.0f) * value) * keep;
+            for (int j = 0; j < G / 16; ++j) v[j] = o[k * (G / 16) + j][n][2 * u + e] * kLag * keep;
             float* p = to + k * G + g * (G / 8) + u * (G / 16);
             if constexpr (G == 64)
               *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
