@@ -669,7 +669,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float mw = row_ml[(w * kRows + tid) * 2];
-        sum += mw == -INFINITY ? 0.0f : row_ml[(w * kRows + tid) * 2 + 1] * exp2_approx(mw - now);
+        sum += row_ml[(w * kRows + tid) * 2 + 1] * (mw == -INFINITY ? 1.0f : exp2_approx(mw - now));  // none: 0, or NaN from scores that are
       }
       row_all[tid] = make_float2(now, sum);
     }
