@@ -241,7 +241,7 @@ int b200q_qk_norm_rope(const b200q_qk_norm_args* args, void* stream);
 int b200q_qk_norm_rope_bprop(const b200q_qk_norm_args* args, void* stream);
 
 /* 4-bit paged key / value cache.  codes: [pages][heads][page_size][d / 2] bytes, 16-byte aligned;
- * params: [pages][heads][page_size][d / group] words (bits 0-15 the bf16 scale, 16-23 the zero point);
+ * params: [pages][heads][page_size][d / group] words (bits 0-15 the bf16 scale, 16-23 the zero point, 0 to 15);
  * value = (code - zero) * scale.  d 64, 128 or 256; group 32 or 64.  Slot = page * page_size + place. */
 typedef struct b200q_kv4_cache {
   uint8_t* k_codes;
@@ -254,6 +254,8 @@ typedef struct b200q_kv4_cache {
 /* Quantizes k, v [t][heads][d] into slots[t] (int64; negative: not stored).  Per group, in fp32:
  *   lo = min(0, x), hi = max(0, x), s = bf16((hi - lo) * (1 / 15)) (0 when below the smallest normal),
  *   zero = clamp(rint(-lo * (1 / s)), 0, 15), code = clamp(rint(x * (1 / s)) + zero, 0, 15).
+ * A group with a NaN or an infinity in it (or whose hi - lo passes fp32's range) gets the scale NaN: its values read back as
+ * NaN, and attention rows that see it are NaN.
  * Every slot is named at most once in a call. */
 int b200q_kv4_append(const b200q_kv4_cache* c, const void* k, long long k_ts, long long k_hs, const void* v,
                      long long v_ts, long long v_hs, const int64_t* slots, int ftype, int t, void* stream);

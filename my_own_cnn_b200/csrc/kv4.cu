@@ -115,19 +115,20 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_append_kernel(Cache c, Appen
     for (int j = 0; j < V; ++j) x[j] = to_f32(raw[u][j]);
 #pragma unroll
     for (int j = 0; j < V; j += 2) {
-      lo = fminf(fminf(x[j], x[j + 1]), lo);
-      hi = fmaxf(fmaxf(x[j], x[j + 1]), hi);
+      lo = min_nan(min_nan(x[j], x[j + 1]), lo);
+      hi = max_nan(max_nan(x[j], x[j + 1]), hi);
     }
 #pragma unroll
     for (int o = kPerGroup / 2; o; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(~0u, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, o));
+      lo = min_nan(lo, __shfl_xor_sync(~0u, lo, o));
+      hi = max_nan(hi, __shfl_xor_sync(~0u, hi, o));
     }
     // the format's own fp32 steps, each rounded once; bf16 scales keep fp32's range
     const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f));
     float s = __bfloat162float(sb);
     uint32_t bits = __bfloat16_as_ushort(sb);
     if (!(s >= 1.17549435e-38f)) s = 0.0f, bits = 0;
+    if (!(hi - lo < INFINITY)) s = 0.0f, bits = 0x7FC0u;  // a range that is infinite or NaN has no codes: the scale says so
     const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
     const float z = fminf(fmaxf(rintf(__fmul_rn(-lo, inv)), 0.0f), 15.0f);
     // rint(v) + z in the low bits of 1.5 2^23 + rint(v) + z (the sum rounds half to even, as rint does); v + z >= 0, since

@@ -89,3 +89,43 @@ def test_value_scales_that_a_row_does_not_see(dtype, word):
     out = b2q.kv4_attention(q, c, table, lens)
     assert torch.equal(out[:, :2], want[:, :2]) and torch.equal(out[..., 32:], want[..., 32:])
     assert not out[:, 2:, :, :32].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("d,group", [(64, 32), (64, 64), (128, 32), (128, 64), (256, 32), (256, 64)])
+def test_append_keeps_what_is_not_finite(dtype, bad, d, group):
+    """Its group of channels reads back as NaN, wherever in the group it lies; all other groups as without it."""
+    t = d + 3  # a token for each channel, one with a whole group of them, and two without
+    c = b2q.KV4Cache.empty(-(-t // 16), 2, 16, d, group)
+    clean = b2q.KV4Cache.empty(c.pages, 2, 16, d, group)
+    slots = torch.arange(t, device="cuda")
+    k, v = normal(1, t, 2, d).to(dtype), normal(2, t, 2, d).to(dtype)
+    b2q.kv4_append(clean, k, v, slots)
+    want = b2q.kv4_read(clean, slots, dtype)
+    i = torch.arange(d, device="cuda")
+    hit = torch.zeros(t, 2, d, dtype=torch.bool, device="cuda")
+    hit[i, 1, i] = True
+    hit[d, 0, :group] = True
+    for x in (k, v):
+        x[hit] = bad
+    b2q.kv4_append(c, k, v, slots)
+    groups = hit.unflatten(-1, (-1, group)).any(-1, keepdim=True).expand(t, 2, d // group, group).flatten(-2)
+    for got, x in zip(b2q.kv4_read(c, slots, dtype), want):
+        assert got[groups].isnan().all() and torch.equal(got[~groups], x[~groups])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_attention_shows_what_was_appended(dtype, what, bad):
+    c, table, lens = held(50, 2, 64, 32)
+    q = normal(3, 1, 3, 4, 64).to(dtype)
+    want, sums = b2q.kv4_attention(q, c, table, lens, return_lse=True)
+    slot = torch.tensor([48], device="cuda")  # the last row but one's own token
+    k, v = b2q.kv4_read(c, slot)
+    (k if what == "k" else v)[..., 5] = bad
+    b2q.kv4_append(c, k, v, slot)
+    out, lse = b2q.kv4_attention(q, c, table, lens, return_lse=True)
+    assert torch.equal(out[:, 0], want[:, 0]) and torch.equal(lse[:, 0], sums[:, 0])
+    assert out[:, 1:, :, :32].isnan().all() and lse[:, 1:].isnan().all() == (what == "k")
