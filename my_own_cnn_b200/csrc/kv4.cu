@@ -172,16 +172,18 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_read_kernel(Cache c, const i
   for (int u = 0; u < AHEAD; ++u) {
     const MoveRow& r = row[u];
     if (r.t >= t) continue;
-    const float s = param_scale(param[u]), zs = -zero_point(param[u]) * s;
-    // 1024 + code and 1024 + 16 code as fp16 pairs of the codes 16 bits apart; code s and z s are exact, and so is their
-    // difference
+    const float s = param_scale(param[u]);
+    // 1024 + code and 1024 + 16 code as fp16 pairs of the codes 16 bits apart, less 1024 + zero point (a sixteenth of the
+    // latter: 64 + zero point): exact, and so is its product with the scale in fp32
+    const uint32_t z = (param[u] >> 16 & 0xFFu) * 0x00010001u | 0x64006400u;
+    const __half2 less = *reinterpret_cast<const __half2*>(&z), less_64 = __hsub2(__float2half2_rn(960.0f), less);
     float out[V];
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) {
       const uint32_t bits = and_or(word[u] >> (j / 2 * 8), j % 2 ? 0x00F000F0u : 0x000F000Fu, 0x64006400u);
-      const __half2 h = j % 2 ? __hfma2(*reinterpret_cast<const __half2*>(&bits), __float2half2_rn(0.0625f), __float2half2_rn(-64.0f))
-                              : __hadd2(*reinterpret_cast<const __half2*>(&bits), __float2half2_rn(-1024.0f));
-      const float2 f = fma2(__half22float2(h), both(s), both(zs));
+      const __half2 h = j % 2 ? __hfma2(*reinterpret_cast<const __half2*>(&bits), __float2half2_rn(0.0625f), less_64)
+                              : __hsub2(*reinterpret_cast<const __half2*>(&bits), less);
+      const float2 f = mul2(__half22float2(h), both(s));
       out[j] = f.x;
       out[j + V / 2] = f.y;
     }

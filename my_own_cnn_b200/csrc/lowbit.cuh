@@ -73,12 +73,8 @@ struct Divisor {
   __device__ __forceinline__ uint32_t of(uint32_t n) const { return d < 2 ? n : __umulhi(n, m) >> shift; }
 };
 
-// Scale and zero point of a cache parameter word.
+// Scale of a cache parameter word.
 __device__ __forceinline__ float param_scale(uint32_t p) { return __uint_as_float(p << 16); }
-// (bits 16-23 under the exponent of 2^23)
-__device__ __forceinline__ float zero_point(uint32_t p) {
-  return __uint_as_float(__byte_perm(p, 0x4B000000u, 0x7542)) - 8388608.0f;
-}
 
 // C += A B on one warp, m16 n8 k16: fp16 operands, fp32 sums.  Lane (g = lane / 4, t = lane % 4):
 // a0, a2 hold row g (k 2t, 2t+1 and 2t+8, 2t+9), a1, a3 row g + 8; b0, b1 the same k of column g;

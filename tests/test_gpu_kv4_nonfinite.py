@@ -129,3 +129,20 @@ def test_attention_shows_what_was_appended(dtype, what, bad):
     out, lse = b2q.kv4_attention(q, c, table, lens, return_lse=True)
     assert torch.equal(out[:, 0], want[:, 0]) and torch.equal(lse[:, 0], sums[:, 0])
     assert out[:, 1:, :, :32].isnan().all() and lse[:, 1:].isnan().all() == (what == "k")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,group", [(64, 32), (128, 64), (256, 32)])
+def test_read_of_any_word(dtype, d, group):
+    """(code - zero) * scale to the bit for every code and zero point, with scales that are finite, infinite and NaN."""
+    c = b2q.KV4Cache.empty(4, 1, 64, d, group)
+    scales = torch.tensor([0x3F80, 0x3DCD, 0xBE01, 0x0080, 0x7F00, INF, INF | 0x8000, NAN], device="cuda")
+    for i, (codes, params) in enumerate(((c.k_codes, c.k_params), (c.v_codes, c.v_params))):
+        codes.copy_(((torch.arange(codes.numel(), device="cuda") * (97 + 2 * i)) % 256).view_as(codes))
+        at = torch.arange(params.numel(), device="cuda").view_as(params)
+        params.copy_(scales[at % 8] | (at // 8 % 16) << 16)
+    slots = torch.arange(256, device="cuda")
+    for got, codes, params in zip(b2q.kv4_read(c, slots, dtype), (c.k_codes, c.v_codes), (c.k_params, c.v_params)):
+        want = cache_values(codes.flatten(0, 2), params.flatten(0, 2), group)[0].to(torch.float32).to(dtype)
+        assert torch.equal(got[:, 0].isnan(), want.isnan())
+        assert torch.equal(got[:, 0][~want.isnan()], want[~want.isnan()])
