@@ -1,19 +1,20 @@
 // Linear layers with 4-bit weights and group scales (b200q_linear_w4).
 //
-//   y[m][n] = sum_g s[g][n] sum_{k in g} c[n][k] x[m][k]  -  sum_g s[g][n] z[g][n] sum_{k in g} x[m][k]
+//   y[m][n] = sum_g s[g][n] sum_{k in g} (c[n][k] - z[g][n]) x[m][k]
 //
 // Bytes bound it: K / 2 of codes and 2 or 3 per group for each weight row; and, as measured, the latency of its instructions
-// with 16 warps an SM.  1 x 8192 x 8192 bf16: 10.7 us, 3.3 TB/s; 16 x 16384 x 8192: 34.7 us, 2.1 TB/s; 1 x 768 x 768: 2.9 us.
+// with 16 warps an SM.  1 x 8192 x 8192 bf16: 11.6 us, 3.0 TB/s; 16 x 16384 x 8192: 34.5 us, 2.1 TB/s; 1 x 768 x 768: 3.0 us.
 // The codes are the 16-row operand A of m16n8k16 (weight rows x K) and up to 16 rows of x its 8 columns, once or twice;
-// m16n8k16 from registers because a code leaves its word as an operand in less than one instruction, while tcgen05
+// m16n8k16 from registers because a code leaves its word as an operand in two instructions, while tcgen05
 // operands would have to be written to shared memory first, four times the bytes that were read.
-//   Operands: a nibble in the low bits of an fp16 is the subnormal code * 2^-24, exactly, and one place higher
-//   code * 2^-20: a word of 8 codes becomes four operands, the pairs (0,4) (1,5) (2,6) (3,7), by one shift and four
-//   masks, and every second value of x is divided by 16 instead.  x is scaled by a power of two per row and step to a
-//   maximum in [2^14, 2^15), so that it fits fp16 whatever its type; fp32 becomes two fp16 terms (22 bits).
-//   The zero points' sum is kept apart, one row per lane.  The adder lines subnormals up by their exponent field, which
-//   costs about 10 of the sum's bits (results off by 2e-6, far below a 16-bit output's rounding): fp32 calls
-//   take 1024 + code less 1024 + zero point instead, exact and normal.
+//   Operands: a nibble put into the low bits of the fp16 1024 is 1024 + code, and one place higher 1024 + 16 code; less the
+//   same of the zero point it is exact and normal.  A word of 8 codes becomes four operands, the pairs (0,4) (1,5) (2,6) (3,7),
+//   and every second value of x is divided by 16 instead.  x is scaled by a power of two per row and step to a maximum in
+//   [2^14, 2^15), so that it fits fp16 whatever its type; fp32 becomes two fp16 terms (22 bits).
+//   (The bare nibble, a subnormal, with the zero points' sum kept apart, saves the subtraction: 10.6 against 11.6 us for one
+//   row of 8192 x 8192, 34.9 against 34.5 for 16 rows.  But the adder lines subnormals up by their exponent field and truncates
+//   about 10 of the sum's bits, and where x has one sign the two sums are many times their difference: fp16 results after a
+//   squared ReLU were off by 6e-5, all one way.)
 //
 // Each warp streams 32 rows through a ring of its own (16-byte asynchronous copies) in steps of kStep columns.  x is
 // shared by the block's warps, in the order of operand B; the blocks of a cluster have the same rows and other slices
@@ -56,17 +57,16 @@ constexpr int kMaxSplit = 8;
 
 // FEW: 0, or how many rows of x at most a block has that keeps all of them in shared memory.
 // Shared memory: the rings (over them at the end the sums), then x: two steps of it, or (FEW) every step of the block's
-// slice.  A step of x: operand B [block of 32 columns][term][row][t] 16 bytes, sums [group][row], powers [row].
+// slice.  A step of x: operand B [block of 32 columns][term][row][t] 16 bytes, powers [row].
 template <typename T, int G, int NT, int FEW>
 struct Layout {
   static constexpr int kTerms = std::is_same<T, float>::value ? 2 : 1;
   static constexpr int kRowsX = FEW ? FEW : 8 * NT;    // rows of x that there is room for
   static constexpr int kRowsW = FEW ? 32 : 32 * kWarps;     // weight rows of a block
   static constexpr int kX = kStep * 2 * kTerms * kRowsX;
-  static constexpr int kXSum = kTerms == 2 ? 0 : (kStep / G) * kRowsX * 4;
-  static constexpr int kBuffer = (kX + kXSum + kRowsX * 4 + 15) / 16 * 16;
-  // Three stages where two blocks still fit an SM (228 KB, 1 KB of it taken per block); 16 rows of fp32, or of 32 weights a
-  // group, leave room for two: 16 x 11000 x 12000 fp32 48 us, 69 with one block and three; 16 x 16384 x 8192 bf16 40, 61.
+  static constexpr int kBuffer = (kX + kRowsX * 4 + 15) / 16 * 16;
+  // Three stages where two blocks still fit an SM (228 KB, 1 KB of it taken per block); 16 rows of fp32 leave room for two:
+  // 16 x 11000 x 12000 fp32 48 us, 69 with one block and three.
   static constexpr int kStages = FEW || kWarps * 3 * kStage + 2 * kBuffer > 113 * 1024 ? 2 : 3;
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kBuffers = FEW ? (46 * 1024) / kBuffer : 2;
@@ -114,8 +114,7 @@ struct XRow {
   __device__ __forceinline__ void store(uint8_t* buffer, int m) const {
     constexpr int kWords = G / 32;
     uint4* const xs = reinterpret_cast<uint4*>(buffer);
-    float* const xsum = reinterpret_cast<float*>(buffer + L::kX);
-    float* const xpower = reinterpret_cast<float*>(buffer + L::kX + L::kXSum);
+    float* const xpower = reinterpret_cast<float*>(buffer + L::kX);
     const int q = threadIdx.x % 32;
     // thread t of a quad owns G / 4 columns of a group, kWords words of 8
     const int group = q / (G / 8), t = q % (G / 8) / kWords, block = group * kWords + q % kWords;
@@ -125,13 +124,6 @@ struct XRow {
     for (int j = 0; j < 4; ++j) {
       f[j] = make_float2(to_f32(v[j]), to_f32(v[j + 4]));
       top = fmaxf(fmaxf(fabsf(f[j].x), fabsf(f[j].y)), top);
-    }
-    if constexpr (L::kTerms == 1) {
-      const float2 half = add2(add2(f[0], f[1]), add2(f[2], f[3]));
-      float sum = half.x + half.y;
-#pragma unroll
-      for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(~0u, sum, o);
-      if (q % (G / 8) == 0) xsum[group * L::kRowsX + m] = sum;
     }
     const Power p = power_for(warp_max(top));
     if (q == 0) xpower[m] = p.down;
@@ -160,7 +152,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
   using L = Layout<T, G, NT, FEW>;
   constexpr int kTerms = L::kTerms, kWords = G / 32, kGroups = kStep / G, kStages = L::kStages, kRowsW = L::kRowsW;
   constexpr int kRowsX = L::kRowsX;
-  constexpr bool kF32 = kTerms == 2;
   extern __shared__ __align__(128) uint8_t smem[];
   wait_for_previous();
   uint8_t* const buffers = smem + L::kRing;
@@ -207,13 +198,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
     }
   };
 
-  // sums of products, [16 rows][8 columns][row g or g + 8] for columns 2t, 2t + 1; of lane l's row, sums of zero points
-  constexpr int kLess = (kRowsX + 1) / 2;
-  float2 acc[2][NT][2], less[kLess];
+  // sums of products, [16 rows][8 columns][row g or g + 8] for columns 2t, 2t + 1
+  float2 acc[2][NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) acc[0][n][0] = acc[0][n][1] = acc[1][n][0] = acc[1][n][1] = both(0.0f);
-#pragma unroll
-  for (int m = 0; m < kLess; ++m) less[m] = both(0.0f);
   constexpr int kRowsWarp = FEW ? 4 : NT;  // rows of a step that a warp has on their way at a time
   XRow<T> x[kRowsWarp];
   auto load_x = [&](int step) {  // rows w, w + 8 of one step
@@ -269,8 +257,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
     for (int i = 0; i < kGroups; ++i) scale[i] = next_scale[i] << 16, zero[i] = next_zero[i];
     if (s + 1 < steps) load_params(s + 1);
     const uint4* const xs = reinterpret_cast<const uint4*>(buffer);
-    const float* const xsum = reinterpret_cast<const float*>(buffer + L::kX);
-    const float* const xpower = reinterpret_cast<const float*>(buffer + L::kX + L::kXSum);
+    const float* const xpower = reinterpret_cast<const float*>(buffer + L::kX);
     const uint8_t* const stage = smem + warp * (kStages * kStage) + slot * kStage;
     float2 sum[2][NT][2];
 #pragma unroll
@@ -291,11 +278,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
         }
       }
       constexpr uint32_t kMagic = 0x64006400u;  // two fp16 1024
-      uint32_t zpair[4];  // fp32 calls: the rows' zero points, twice
-      if constexpr (kF32) {
+      uint32_t zpair[4];  // the rows' zero points, twice
 #pragma unroll
-        for (int r = 0; r < 4; ++r) zpair[r] = __shfl_sync(~0u, zero[i], r * 8 + g) * 0x00010001u;
-      }
+      for (int r = 0; r < 4; ++r) zpair[r] = __shfl_sync(~0u, zero[i], r * 8 + g) * 0x00010001u;
       float part[2][NT][4];
 #pragma unroll
       for (int word = 0; word < kWords; ++word) {
@@ -313,11 +298,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const uint32_t v = w[2 * mt + u][word] >> (j / 2 * 8), mask = j % 2 ? 0x00F000F0u : 0x000F000Fu;
-              if constexpr (kF32)
-                c[u][j] = sub_f16x2(and_or(v, mask, kMagic),
-                                    j % 2 ? and_or(zpair[2 * mt + u] << 4, mask, kMagic) : zpair[2 * mt + u] | kMagic);
-              else
-                c[u][j] = v & mask;
+              c[u][j] = sub_f16x2(and_or(v, mask, kMagic),
+                                  j % 2 ? and_or(zpair[2 * mt + u] << 4, mask, kMagic) : zpair[2 * mt + u] | kMagic);
             }
 #pragma unroll
           for (int term = 0; term < kTerms; ++term)
@@ -340,21 +322,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
           float2& to = sum[r / 2][n][r % 2];
           to = i == 0 ? mul2(sc, make_float2(p[0], p[1])) : fma2(sc, make_float2(p[0], p[1]), to);
         }
-      }
-      if constexpr (!kF32) {
-        const float2 sz = both(__uint_as_float(scale[i]) * static_cast<float>(zero[i]));
-#pragma unroll
-        for (int m = 0; m < kRowsX; m += 4)
-          if (m < rows) {
-            const float* at = xsum + i * kRowsX + m;
-            if constexpr (kRowsX == 1) {
-              less[0].x = fmaf(sz.x, at[0], less[0].x);
-            } else {
-              const float4 v = *reinterpret_cast<const float4*>(at);
-              less[m / 2] = fma2(sz, make_float2(v.x, v.y), less[m / 2]);
-              less[m / 2 + 1] = fma2(sz, make_float2(v.z, v.w), less[m / 2 + 1]);
-            }
-          }
       }
     }
 #pragma unroll
@@ -384,13 +351,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
       for (int u = 0; u < 2; ++u) {
         if (FEW && 2 * t >= kRowsX) continue;
         float* to = sums + (n * 8 + 2 * t) * kPitch + mt * 16 + u * 8 + g;
-        constexpr float kUnit = kF32 ? 1.0f : 16777216.0f;  // subnormal codes count 2^-24
-        to[0] = acc[mt][n][u].x * kUnit;
-        if (kRowsX > 1) to[kPitch] = acc[mt][n][u].y * kUnit;
+        to[0] = acc[mt][n][u].x;
+        if (kRowsX > 1) to[kPitch] = acc[mt][n][u].y;
       }
-  __syncwarp();
-#pragma unroll
-  for (int m = 0; m < kRowsX; ++m) sums[m * kPitch + lane] -= m % 2 ? less[m / 2].y : less[m / 2].x;
   if (splits > 1)
     cluster_sync();
   else
