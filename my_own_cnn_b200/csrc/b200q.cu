@@ -1006,9 +1006,14 @@ int f32_grad(const DeviceState& st, const float* x, const float* dy, float* dw, 
   return B200Q_OK;
 }
 
-// Arrival counters of kernels whose last block joins the others' partial results: zeroed once here,
-// and returned to zero by the block that sees the last arrival.
-std::map<std::pair<int, cudaStream_t>, unsigned*> g_scratch;
+// A stream's scratch: arrival counters of kernels whose last block joins the others' partial results (zeroed once,
+// and returned to zero by the block that sees the last arrival), then kScratchBytes.
+struct Scratch {
+  std::mutex mu;  // held while a call that uses it is put into the stream
+  unsigned* base = nullptr;
+};
+std::mutex g_scratch_mu;
+std::map<std::pair<int, cudaStream_t>, Scratch> g_scratch;
 
 }  // namespace
 
@@ -1033,13 +1038,17 @@ int host_device(int* sms, int** err, int* index) {
   return B200Q_OK;
 }
 
-int host_scratch(cudaStream_t stream, void** out, unsigned** counters) {
+int host_scratch(cudaStream_t stream, ScratchHold* hold) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  std::lock_guard<std::mutex> lk(g_ws_mu);
-  unsigned*& c = g_scratch[{dev, stream}];
-  if (!c) {
+  Scratch* s = nullptr;
+  {
+    std::lock_guard<std::mutex> lk(g_scratch_mu);
+    s = &g_scratch[{dev, stream}];
+  }
+  hold->lock = std::unique_lock<std::mutex>(s->mu);
+  if (!s->base) {
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
     e = cudaStreamIsCapturing(stream, &capturing);
     if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
@@ -1053,10 +1062,10 @@ int host_scratch(cudaStream_t stream, void** out, unsigned** counters) {
       cudaFreeAsync(p, stream);
       return cuda_fail(e, "cudaMemsetAsync(counters)");
     }
-    c = static_cast<unsigned*>(p);
+    s->base = static_cast<unsigned*>(p);
   }
-  *out = c + kSplitCounters;
-  if (counters) *counters = c;
+  hold->bytes = s->base + kSplitCounters;
+  hold->counters = s->base;
   return B200Q_OK;
 }
 

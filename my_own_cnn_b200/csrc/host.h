@@ -5,6 +5,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <mutex>
 
 #include "../../include/b200q.h"
 
@@ -25,7 +26,13 @@ B200Q_HIDDEN int host_device(int* sms, int** err, int* index = nullptr);
 // captured on the stream can be replayed whatever calls follow; refused while the stream is captured.
 constexpr size_t kScratchBytes = 16u << 20;
 constexpr int kSplitCounters = 1 << 16;
-B200Q_HIDDEN int host_scratch(cudaStream_t stream, void** out, unsigned** counters = nullptr);
+// While it lives no other thread's call gets the same scratch: a call's launches lie together in the stream.
+struct ScratchHold {
+  std::unique_lock<std::mutex> lock;
+  void* bytes = nullptr;
+  unsigned* counters = nullptr;
+};
+B200Q_HIDDEN int host_scratch(cudaStream_t stream, ScratchHold* hold);
 B200Q_HIDDEN void host_set_path(int path);
 
 // Launches a kernel that begins with wait_for_previous(): its blocks may take their places while the stream's previous kernel

@@ -258,10 +258,11 @@ int launch_attention(const Cache& c, AttnArgs a, int sms, int device, cudaStream
   const int blocks = static_cast<int>(
       std::min<long long>(std::min({sms * resident, Shape::kBody / (8 * NT * 4), kSplitCounters, kRoom}), most));
   const size_t rows = static_cast<size_t>(blocks) * kPartRows;
-  void* ws = nullptr;
-  int rc = host_scratch(stream, &ws, &a.counters);
+  ScratchHold scratch;
+  int rc = host_scratch(stream, &scratch);
   if (rc) return rc;
-  a.partial = static_cast<float*>(ws);
+  a.counters = scratch.counters;
+  a.partial = static_cast<float*>(scratch.bytes);
   a.partial_ml = a.partial + rows * D;
   return host_launch("kv4_attention_kernel launch", kernel, dim3(blocks), kWarps * 32, Shape::kSmem, stream, 1, c, a);
 }

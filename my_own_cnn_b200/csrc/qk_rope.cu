@@ -587,9 +587,9 @@ extern "C" int b200q_qk_norm_rope_bprop(const b200q_qk_norm_args* args, void* st
   const int room = static_cast<int>(kScratchBytes / (2 * d * sizeof(float)));  // at least 2048 blocks' partial sums
   const int blocks = static_cast<int>(
       std::max(1ll, std::min<long long>((units + units_per_block - 1) / units_per_block, std::min(sms * 4, room))));
-  void* ws = nullptr;
-  if ((rc = host_scratch(cs, &ws))) return rc;
-  a.partial = static_cast<float*>(ws);
+  ScratchHold scratch;  // until both kernels are in the stream
+  if ((rc = host_scratch(cs, &scratch))) return rc;
+  a.partial = static_cast<float*>(scratch.bytes);
   const size_t smem = static_cast<size_t>(kNormWarps) * 2 * d * sizeof(float);
   B200Q_DISPATCH_FTYPE(ftype, {
     if (lanes) {

@@ -1,0 +1,64 @@
+"""Calls that use a stream's scratch (attention, the norms' gradient) beside one another: host threads, streams and graphs."""
+import threading
+
+import pytest
+import torch
+
+import my_own_cnn_b200 as b2q
+
+pytestmark = pytest.mark.gpu
+
+
+def normal(seed, *shape):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def gradient(seed, t=700, heads=4, d=128, dtype=torch.float32):
+    """A call of the gradient."""
+    q, k, dq, dk = (normal(10 * seed + i, t, heads, d).to(dtype) for i in range(4))
+    w = normal(seed, d).to(dtype)
+    return lambda **kw: b2q.qk_norm_rope_bprop(dq, dk, q, k, w, w, None, None, **kw)
+
+
+def attention(seed, n=3000, d=128):
+    """A call of attention over a sequence that several blocks share."""
+    c = b2q.KV4Cache.empty(-(-n // 64), 2, 64, d)
+    b2q.kv4_append(c, normal(10 * seed, n, 2, d), normal(10 * seed + 1, n, 2, d), torch.arange(n, device="cuda"))
+    table, lens = torch.arange(c.pages, device="cuda").int()[None], torch.tensor([n], device="cuda").int()
+    q = normal(10 * seed + 2, 1, 1, 4, d).bfloat16()
+    return lambda **kw: b2q.kv4_attention(q, c, table, lens, **kw)
+
+
+def same(got, want):
+    got, want = (x if isinstance(x, tuple) else (x,) for x in (got, want))
+    return all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def in_threads(calls, times, **kw):
+    """Each call by a thread of its own, again and again; which of them ever answered otherwise than alone."""
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    start, wrong = threading.Barrier(len(calls)), []
+
+    def work(i):
+        start.wait()
+        for _ in range(times):
+            got = [calls[i](**kw) for _ in range(4)]
+            torch.cuda.current_stream().synchronize()
+            if not all(same(x, want[i]) for x in got):
+                wrong.append(i)
+                return
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    return wrong
+
+
+def test_threads_of_one_stream():
+    """A call's launches lie together in the stream, whatever other threads put there."""
+    assert in_threads([gradient(1), gradient(2), attention(3), gradient(4, t=100, dtype=torch.bfloat16), attention(5, n=9000)], 60) == []
