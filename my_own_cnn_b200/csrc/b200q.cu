@@ -23,9 +23,12 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <utility>
+#include <vector>
 
 #include "../../include/b200q.h"
 #include "common.cuh"
@@ -1011,9 +1014,97 @@ int f32_grad(const DeviceState& st, const float* x, const float* dy, float* dw, 
 struct Scratch {
   std::mutex mu;  // held while a call that uses it is put into the stream
   unsigned* base = nullptr;
+  bool captured = false;  // a graph may use it
 };
-std::mutex g_scratch_mu;
-std::map<std::pair<int, cudaStream_t>, Scratch> g_scratch;
+// The tables (never destroyed: threads may outlive them).  Scratch is found by the stream's own number: a handle may be another
+// stream in each thread (cudaStreamPerThread), or later on (a new stream in a destroyed one's place, whose work may still run).
+struct ScratchTables {
+  std::mutex mu;
+  std::map<std::pair<int, unsigned long long>, std::unique_ptr<Scratch>> of_stream;  // (device, number)
+  std::map<std::pair<int, cudaStream_t>, unsigned long long> number;                 // of the handle's last stream
+  std::vector<std::unique_ptr<Scratch>> retired[kMaxDevices];  // of streams that are gone, whose last work may still run
+  std::vector<unsigned*> idle[kMaxDevices];                    // that nothing uses
+
+  void retire(int dev, unsigned long long id) {
+    auto it = of_stream.find({dev, id});
+    if (it == of_stream.end()) return;
+    if (it->second->base && !it->second->captured) retired[dev].push_back(std::move(it->second));
+    of_stream.erase(it);
+  }
+};
+ScratchTables& g_scratch = *new ScratchTables;
+constexpr size_t kRetiredMost = 8;
+
+// A thread's own streams (cudaStreamPerThread) end with it.
+struct ThreadStreams {
+  std::vector<std::pair<int, unsigned long long>> keys;
+  ~ThreadStreams() {
+    std::lock_guard<std::mutex> lk(g_scratch.mu);
+    for (const auto& k : keys) g_scratch.retire(k.first, k.second);
+  }
+};
+thread_local ThreadStreams g_thread_streams;
+
+// The stream's entry, made if need be.
+Scratch* scratch_of(int dev, cudaStream_t stream, unsigned long long id) {
+  std::lock_guard<std::mutex> lk(g_scratch.mu);
+  std::unique_ptr<Scratch>& s = g_scratch.of_stream[{dev, id}];
+  if (!s) {
+    s = std::make_unique<Scratch>();
+    if (stream == cudaStreamPerThread) {
+      g_thread_streams.keys.emplace_back(dev, id);
+    } else {
+      unsigned long long& last = g_scratch.number.try_emplace({dev, stream}, id).first->second;
+      if (last != id) g_scratch.retire(dev, last);
+      last = id;
+    }
+  }
+  return s.get();
+}
+
+// The entry that the handle had last (a stream that is captured does not tell its number), or null.
+Scratch* last_scratch_of(int dev, cudaStream_t stream) {
+  std::lock_guard<std::mutex> lk(g_scratch.mu);
+  std::pair<int, unsigned long long> key{dev, 0};
+  if (stream == cudaStreamPerThread) {
+    const auto& keys = g_thread_streams.keys;
+    const auto it = std::find_if(keys.begin(), keys.end(), [&](const auto& k) { return k.first == dev; });
+    if (it == keys.end()) return nullptr;
+    key = *it;
+  } else {
+    const auto it = g_scratch.number.find({dev, stream});
+    if (it == g_scratch.number.end()) return nullptr;
+    key.second = it->second;
+  }
+  const auto it = g_scratch.of_stream.find(key);
+  return it == g_scratch.of_stream.end() ? nullptr : it->second.get();
+}
+
+// Scratch for a stream that has none: one that nothing uses, else a new one.
+int new_scratch(int dev, cudaStream_t stream, unsigned** base) {
+  std::lock_guard<std::mutex> lk(g_scratch.mu);
+  std::vector<unsigned*>& idle = g_scratch.idle[dev];
+  auto& retired = g_scratch.retired[dev];
+  if (idle.empty() && retired.size() >= kRetiredMost && cudaDeviceSynchronize() == cudaSuccess) {
+    for (auto& s : retired) idle.push_back(s->base);
+    retired.clear();
+  }
+  void* p = nullptr;
+  cudaError_t e = cudaSuccess;
+  if (!idle.empty()) {
+    p = idle.back();
+    idle.pop_back();
+  } else if ((e = cudaMallocAsync(&p, kSplitCounters * sizeof(unsigned) + kScratchBytes, stream)) != cudaSuccess) {
+    return cuda_fail(e, "cudaMallocAsync(scratch)");
+  }
+  e = cudaMemsetAsync(p, 0, kSplitCounters * sizeof(unsigned), stream);
+  if (e != cudaSuccess) {
+    cudaFreeAsync(p, stream);
+    return cuda_fail(e, "cudaMemsetAsync(counters)");
+  }
+  *base = static_cast<unsigned*>(p);
+  return B200Q_OK;
+}
 
 }  // namespace
 
@@ -1040,32 +1131,27 @@ int host_device(int* sms, int** err, int* index) {
 
 int host_scratch(cudaStream_t stream, ScratchHold* hold) {
   int dev = 0;
+  unsigned long long id = 0;
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  Scratch* s = nullptr;
-  {
-    std::lock_guard<std::mutex> lk(g_scratch_mu);
-    s = &g_scratch[{dev, stream}];
-  }
-  hold->lock = std::unique_lock<std::mutex>(s->mu);
-  if (!s->base) {
-    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    e = cudaStreamIsCapturing(stream, &capturing);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
-    if (capturing != cudaStreamCaptureStatusNone)
+  if (dev < 0 || dev >= kMaxDevices) return fail(B200Q_ERR_UNSUPPORTED, "device index %d out of range", dev);
+  if ((e = cudaStreamIsCapturing(stream, &capturing)) != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
+  const bool captured = capturing != cudaStreamCaptureStatusNone;
+  if (!captured && (e = cudaStreamGetId(stream, &id)) != cudaSuccess) return cuda_fail(e, "cudaStreamGetId");
+  try {
+    Scratch* const s = captured ? last_scratch_of(dev, stream) : scratch_of(dev, stream, id);
+    if (s) hold->lock = std::unique_lock<std::mutex>(s->mu);
+    if (captured && (!s || !s->base))
       return fail(B200Q_ERR_UNSUPPORTED, "make one call on the stream before capturing: its scratch is made by the first");
-    void* p = nullptr;
-    e = cudaMallocAsync(&p, kSplitCounters * sizeof(unsigned) + kScratchBytes, stream);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaMallocAsync(scratch)");
-    e = cudaMemsetAsync(p, 0, kSplitCounters * sizeof(unsigned), stream);
-    if (e != cudaSuccess) {
-      cudaFreeAsync(p, stream);
-      return cuda_fail(e, "cudaMemsetAsync(counters)");
-    }
-    s->base = static_cast<unsigned*>(p);
+    if (!s->base)
+      if (int rc = new_scratch(dev, stream, &s->base)) return rc;
+    s->captured |= captured;
+    hold->bytes = s->base + kSplitCounters;
+    hold->counters = s->base;
+  } catch (const std::exception& error) {  // no memory for the host's tables
+    return fail(B200Q_ERR_UNSUPPORTED, "scratch: %s", error.what());
   }
-  hold->bytes = s->base + kSplitCounters;
-  hold->counters = s->base;
   return B200Q_OK;
 }
 

@@ -62,3 +62,53 @@ def in_threads(calls, times, **kw):
 def test_threads_of_one_stream():
     """A call's launches lie together in the stream, whatever other threads put there."""
     assert in_threads([gradient(1), gradient(2), attention(3), gradient(4, t=100, dtype=torch.bfloat16), attention(5, n=9000)], 60) == []
+
+
+def into(call):
+    """The call with an output of its own, made here: the stream that it then runs on allocates nothing."""
+    out = call()
+    return lambda **kw: call(out=out, **kw)
+
+
+def test_the_stream_that_each_thread_has():
+    """cudaStreamPerThread is one handle for as many streams as there are threads."""
+    calls = [into(attention(i, n=6000 + 500 * i)) for i in range(4)]
+    want = [call().clone() for call in calls]
+    torch.cuda.synchronize()
+    start, wrong = threading.Barrier(4), []
+
+    def work(i):
+        start.wait()
+        for _ in range(100):
+            out = calls[i](stream=2)
+            torch.cuda.ExternalStream(2).synchronize()
+            if not torch.equal(out, want[i]):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == []
+
+
+def test_streams_that_come_and_go():
+    """A destroyed stream's handle comes back with a new stream; the scratch of those that are gone is used again."""
+    import ctypes
+
+    cudart = ctypes.CDLL("libcudart.so.12")
+    call = into(attention(1))
+    want = call().clone()
+    free = None
+    for i in range(60):
+        s = ctypes.c_void_p()
+        assert cudart.cudaStreamCreateWithFlags(ctypes.byref(s), 1) == 0
+        torch.cuda.synchronize()
+        out = call(stream=s.value)
+        assert cudart.cudaStreamDestroy(s) == 0  # its work may still run
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        if i == 20:
+            free = torch.cuda.mem_get_info()[0]
+    assert torch.cuda.mem_get_info()[0] > free - (64 << 20)
