@@ -1009,26 +1009,27 @@ int f32_grad(const DeviceState& st, const float* x, const float* dy, float* dw, 
   return B200Q_OK;
 }
 
-// A stream's scratch: arrival counters of kernels whose last block joins the others' partial results (zeroed once,
+// Scratch of a stream, or of a graph for what was captured into it on one stream: arrival counters of kernels whose last block joins the others' partial results (zeroed once,
 // and returned to zero by the block that sees the last arrival), then kScratchBytes.
 struct Scratch {
   std::mutex mu;  // held while a call that uses it is put into the stream
   unsigned* base = nullptr;
-  bool captured = false;  // a graph may use it
 };
+using CaptureKey = std::pair<std::pair<int, cudaStream_t>, unsigned long long>;  // device, stream, the capture's number
 // The tables (never destroyed: threads may outlive them).  Scratch is found by the stream's own number: a handle may be another
 // stream in each thread (cudaStreamPerThread), or later on (a new stream in a destroyed one's place, whose work may still run).
 struct ScratchTables {
   std::mutex mu;
   std::map<std::pair<int, unsigned long long>, std::unique_ptr<Scratch>> of_stream;  // (device, number)
   std::map<std::pair<int, cudaStream_t>, unsigned long long> number;                 // of the handle's last stream
+  std::map<CaptureKey, std::shared_ptr<Scratch>> of_capture;   // until the graph is destroyed
   std::vector<std::unique_ptr<Scratch>> retired[kMaxDevices];  // of streams that are gone, whose last work may still run
   std::vector<unsigned*> idle[kMaxDevices];                    // that nothing uses
 
   void retire(int dev, unsigned long long id) {
     auto it = of_stream.find({dev, id});
     if (it == of_stream.end()) return;
-    if (it->second->base && !it->second->captured) retired[dev].push_back(std::move(it->second));
+    if (it->second->base) retired[dev].push_back(std::move(it->second));
     of_stream.erase(it);
   }
 };
@@ -1062,30 +1063,31 @@ Scratch* scratch_of(int dev, cudaStream_t stream, unsigned long long id) {
   return s.get();
 }
 
-// The entry that the handle had last (a stream that is captured does not tell its number), or null.
-Scratch* last_scratch_of(int dev, cudaStream_t stream) {
+// Whether the stream that the handle named last has scratch (a stream that is captured does not tell its number).
+bool had_scratch(int dev, cudaStream_t stream) {
   std::lock_guard<std::mutex> lk(g_scratch.mu);
   std::pair<int, unsigned long long> key{dev, 0};
   if (stream == cudaStreamPerThread) {
     const auto& keys = g_thread_streams.keys;
     const auto it = std::find_if(keys.begin(), keys.end(), [&](const auto& k) { return k.first == dev; });
-    if (it == keys.end()) return nullptr;
+    if (it == keys.end()) return false;
     key = *it;
   } else {
     const auto it = g_scratch.number.find({dev, stream});
-    if (it == g_scratch.number.end()) return nullptr;
+    if (it == g_scratch.number.end()) return false;
     key.second = it->second;
   }
   const auto it = g_scratch.of_stream.find(key);
-  return it == g_scratch.of_stream.end() ? nullptr : it->second.get();
+  return it != g_scratch.of_stream.end() && it->second->base;
 }
 
-// Scratch for a stream that has none: one that nothing uses, else a new one.
-int new_scratch(int dev, cudaStream_t stream, unsigned** base) {
+// Scratch that nothing uses, else new, with its counters zeroed in `stream`, which is not captured.  may_wait: for the device, so
+// that what destroyed streams left can be used.
+int new_scratch(int dev, cudaStream_t stream, bool may_wait, unsigned** base) {
   std::lock_guard<std::mutex> lk(g_scratch.mu);
   std::vector<unsigned*>& idle = g_scratch.idle[dev];
   auto& retired = g_scratch.retired[dev];
-  if (idle.empty() && retired.size() >= kRetiredMost && cudaDeviceSynchronize() == cudaSuccess) {
+  if (may_wait && idle.empty() && retired.size() >= kRetiredMost && cudaDeviceSynchronize() == cudaSuccess) {
     for (auto& s : retired) idle.push_back(s->base);
     retired.clear();
   }
@@ -1103,6 +1105,63 @@ int new_scratch(int dev, cudaStream_t stream, unsigned** base) {
     return cuda_fail(e, "cudaMemsetAsync(counters)");
   }
   *base = static_cast<unsigned*>(p);
+  return B200Q_OK;
+}
+
+// What a graph gives back when it and all that was instantiated from it are destroyed and have run.
+struct GraphScratch {
+  CaptureKey key;
+  unsigned* base;
+  static void destroy(void* p) {
+    std::unique_ptr<GraphScratch> g(static_cast<GraphScratch*>(p));
+    std::lock_guard<std::mutex> lk(g_scratch.mu);
+    g_scratch.of_capture.erase(g->key);
+    try {
+      g_scratch.idle[g->key.first.first].push_back(g->base);
+    } catch (const std::exception&) {  // no memory for the table: it is not used again
+    }
+  }
+};
+
+// The entry for what is captured on a stream: each graph has its own, so that graphs and eager calls may run side by side.
+int scratch_of_capture(int dev, cudaStream_t stream, std::shared_ptr<Scratch>* out) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  cudaGraph_t graph = nullptr;
+  cudaError_t e = cudaStreamGetCaptureInfo_v2(stream, &status, &id, &graph, nullptr, nullptr);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamGetCaptureInfo");
+  if (status != cudaStreamCaptureStatusActive) return fail(B200Q_ERR_CUDA, "the stream's capture is no longer valid");
+  const CaptureKey key{{dev, stream}, id};
+  {
+    std::lock_guard<std::mutex> lk(g_scratch.mu);
+    std::shared_ptr<Scratch>& s = g_scratch.of_capture[key];
+    if (!s) s = std::make_shared<Scratch>();
+    *out = s;
+  }
+  std::lock_guard<std::mutex> lk((*out)->mu);
+  if ((*out)->base) return B200Q_OK;
+  // made on a stream of its own, which the capture has nothing to do with
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if ((e = cudaThreadExchangeStreamCaptureMode(&mode)) != cudaSuccess) return cuda_fail(e, "cudaThreadExchangeStreamCaptureMode");
+  cudaStream_t side = nullptr;
+  unsigned* base = nullptr;
+  int rc = B200Q_OK;
+  if ((e = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking)) != cudaSuccess) rc = cuda_fail(e, "cudaStreamCreate(scratch)");
+  if (!rc) rc = new_scratch(dev, side, false, &base);
+  if (!rc && (e = cudaStreamSynchronize(side)) != cudaSuccess) rc = cuda_fail(e, "cudaStreamSynchronize(scratch)");
+  if (side) cudaStreamDestroy(side);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (rc) return rc;
+  auto owned = std::make_unique<GraphScratch>(GraphScratch{key, base});
+  cudaUserObject_t object = nullptr;
+  e = cudaUserObjectCreate(&object, owned.get(), GraphScratch::destroy, 1, cudaUserObjectNoDestructorSync);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaUserObjectCreate(scratch)");
+  owned.release();
+  if ((e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove)) != cudaSuccess) {
+    cudaUserObjectRelease(object, 1);
+    return cuda_fail(e, "cudaGraphRetainUserObject(scratch)");
+  }
+  (*out)->base = base;
   return B200Q_OK;
 }
 
@@ -1140,13 +1199,19 @@ int host_scratch(cudaStream_t stream, ScratchHold* hold) {
   const bool captured = capturing != cudaStreamCaptureStatusNone;
   if (!captured && (e = cudaStreamGetId(stream, &id)) != cudaSuccess) return cuda_fail(e, "cudaStreamGetId");
   try {
-    Scratch* const s = captured ? last_scratch_of(dev, stream) : scratch_of(dev, stream, id);
-    if (s) hold->lock = std::unique_lock<std::mutex>(s->mu);
-    if (captured && (!s || !s->base))
-      return fail(B200Q_ERR_UNSUPPORTED, "make one call on the stream before capturing: its scratch is made by the first");
+    Scratch* s = nullptr;
+    std::shared_ptr<Scratch> of_graph;
+    if (captured) {
+      if (!had_scratch(dev, stream))
+        return fail(B200Q_ERR_UNSUPPORTED, "make one call on the stream before capturing: its scratch is made by the first");
+      if (int rc = scratch_of_capture(dev, stream, &of_graph)) return rc;
+      s = of_graph.get();
+    } else {
+      s = scratch_of(dev, stream, id);
+    }
+    hold->lock = std::unique_lock<std::mutex>(s->mu);
     if (!s->base)
-      if (int rc = new_scratch(dev, stream, &s->base)) return rc;
-    s->captured |= captured;
+      if (int rc = new_scratch(dev, stream, true, &s->base)) return rc;
     hold->bytes = s->base + kSplitCounters;
     hold->counters = s->base;
   } catch (const std::exception& error) {  // no memory for the host's tables

@@ -21,10 +21,11 @@ B200Q_HIDDEN int host_check_launch(const char* what);
 // SM count of the current device, the device address of its error word and (index) its number.
 constexpr int kMaxDevices = 64;
 B200Q_HIDDEN int host_device(int* sms, int** err, int* index = nullptr);
-// Scratch of the (device, stream) pair: kScratchBytes, and kSplitCounters arrival counters that are zero before and
-// after every kernel that uses them.  Made by the first call on a stream and never moved, so that a graph that was
-// captured on the stream can be replayed whatever calls follow; refused while the stream is captured.
-constexpr size_t kScratchBytes = 16u << 20;
+// Scratch of a stream: kScratchBytes, and kSplitCounters arrival counters that are zero before and after every kernel that uses
+// them.  Made by the first call on the stream and never moved.  While the stream is captured it is the graph's own (refused
+// where the stream has none yet), so that a graph may be replayed beside other graphs and calls; it is used again when the
+// graph is destroyed.
+constexpr size_t kScratchBytes = 8u << 20;
 constexpr int kSplitCounters = 1 << 16;
 // While it lives no other thread's call gets the same scratch: a call's launches lie together in the stream.
 struct ScratchHold {

@@ -253,7 +253,7 @@ int launch_attention(const Cache& c, AttnArgs a, int sms, int device, cudaStream
   if (static_cast<long long>(a.b) * c.heads * a.row_tiles * (steps + kUnitSteps + 1) > 0x7fffffffll)
     return host_fail(B200Q_ERR_UNSUPPORTED, "attention too large");
   // (a unit's parts, one per block at most, leave their shares in shared memory when they are joined; the scratch holds
-  // the parts of a thousand blocks)
+  // the parts of five hundred blocks or more)
   constexpr int kPartRows = 2 * 8 * NT, kRoom = static_cast<int>(kScratchBytes / (kPartRows * (D + 2) * sizeof(float)));
   const int blocks = static_cast<int>(
       std::min<long long>(std::min({sms * resident, Shape::kBody / (8 * NT * 4), kSplitCounters, kRoom}), most));

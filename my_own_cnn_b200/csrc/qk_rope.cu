@@ -584,7 +584,7 @@ extern "C" int b200q_qk_norm_rope_bprop(const b200q_qk_norm_args* args, void* st
   const long long units = static_cast<long long>(t) * (lanes ? static_cast<int>(split.parts.d) : hq + hk);
   if (units > 0x7f000000ll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
   const int units_per_block = lanes ? kFastThreads / lanes : kNormWarps;
-  const int room = static_cast<int>(kScratchBytes / (2 * d * sizeof(float)));  // at least 2048 blocks' partial sums
+  const int room = static_cast<int>(kScratchBytes / (2 * d * sizeof(float)));  // at least 1024 blocks' partial sums
   const int blocks = static_cast<int>(
       std::max(1ll, std::min<long long>((units + units_per_block - 1) / units_per_block, std::min(sms * 4, room))));
   ScratchHold scratch;  // until both kernels are in the stream

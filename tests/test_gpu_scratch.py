@@ -112,3 +112,71 @@ def test_streams_that_come_and_go():
         if i == 20:
             free = torch.cuda.mem_get_info()[0]
     assert torch.cuda.mem_get_info()[0] > free - (64 << 20)
+
+
+def captured(call, s):
+    """A graph of the call on stream s, and its outputs."""
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out = call()
+    return g, out
+
+
+def test_graphs_of_one_stream_beside_each_other_and_eager_calls():
+    calls = [attention(1, n=20000), attention(2, n=30000), gradient(3, t=3000), gradient(4, t=3000), attention(5, n=25000)]
+    want = [call() for call in calls]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    attention(6)(stream=s)
+    torch.cuda.synchronize()
+    graphs = [captured(call, s) for call in calls[:4]]
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(100):
+        for (g, _), t in zip(graphs, streams):
+            with torch.cuda.stream(t):
+                g.replay()
+        eager = [calls[4](stream=s) for _ in range(3)]
+        torch.cuda.synchronize()
+        assert all(same(out, x) for (_, out), x in zip(graphs, want))
+        assert all(torch.equal(x, want[4]) for x in eager)
+
+
+def test_streams_within_one_capture():
+    """Calls on streams that fork from the captured one run beside each other in the replay."""
+    calls = [attention(1, n=20000), attention(2, n=20000)]
+    want = [call() for call in calls]
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    for x in (s, t):
+        x.wait_stream(torch.cuda.current_stream())
+        calls[0](stream=x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        t.wait_stream(s)
+        outs = [calls[0](stream=s), calls[1](stream=t)]
+        s.wait_stream(t)
+    for _ in range(50):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_a_graph_gives_its_scratch_back():
+    call = into(attention(1))
+    want = call().clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    call(stream=s)
+    torch.cuda.synchronize()
+    free = None
+    for i in range(40):
+        g, out = captured(call, s)
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        g.reset()
+        del g
+        if i == 10:
+            free = torch.cuda.mem_get_info()[0]
+    assert torch.cuda.mem_get_info()[0] > free - (48 << 20)
