@@ -11,7 +11,7 @@ import torch
 
 from . import _lib
 from .conv import _stream
-from .w4 import FTYPES, _device_tensor, _ftype, _on
+from .w4 import FTYPES, _device_tensor, _ftype, _on, _one_device
 
 
 _CACHE = _lib.packer(_lib.CKV4Cache)
@@ -42,6 +42,8 @@ class KV4Cache:
                 raise RuntimeError("cache tensors must be contiguous")
             if not x.is_cuda:
                 raise RuntimeError("tensor arguments must be CUDA device tensors")
+            if x.get_device() != k_codes.get_device():
+                raise RuntimeError("the tensors of a cache must be on one device")
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
         self.pages, self.heads, self.page_size, half = shape
         self.head_dim = 2 * half
@@ -84,12 +86,20 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.T
         raise RuntimeError(f"k and v must be [tokens, {cache.heads}, {cache.head_dim}], got {list(shape)} and "
                            f"{list(v.shape)}")
     _check_slots(slots, shape[0])
+    if stream is not None:
+        with _on(stream):
+            return _append(cache, k, v, slots, ft, stream)
+    return _append(cache, k, v, slots, ft, None)
+
+
+def _append(cache, k, v, slots, ft, stream):
+    _one_device(k.get_device(), v, slots, cache.k_codes)
     (kt, kh, kc), (vt, vh, vc) = k.stride(), v.stride()
     if kc != 1 or vc != 1:
-        with _on(stream):
-            return kv4_append(cache, k.contiguous(), v.contiguous(), slots, stream)
+        k, v = k.contiguous(), v.contiguous()
+        (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
     _lib.check(_lib.lib().b200q_kv4_append(cache._c, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, slots.data_ptr(), ft,
-                                           shape[0], _stream(stream)))
+                                           k.shape[0], _stream(stream)))
 
 
 def kv4_read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.float32,
@@ -101,15 +111,16 @@ def kv4_read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.fl
     _check_slots(slots)
     if stream is not None:
         with _on(stream):
-            return _read(cache, slots, dtype, ft, _stream(stream))
-    return _read(cache, slots, dtype, ft, _stream(None))
+            return _read(cache, slots, dtype, ft, stream)
+    return _read(cache, slots, dtype, ft, None)
 
 
 def _read(cache, slots, dtype, ft, stream):
+    _one_device(slots.get_device(), cache.k_codes)
     t = slots.shape[0]
     k = slots.new_empty((t, cache.heads, cache.head_dim), dtype=dtype)
     v = torch.empty_like(k)
-    _lib.check(_lib.lib().b200q_kv4_read(cache._c, slots.data_ptr(), k.data_ptr(), v.data_ptr(), ft, t, stream))
+    _lib.check(_lib.lib().b200q_kv4_read(cache._c, slots.data_ptr(), k.data_ptr(), v.data_ptr(), ft, t, _stream(stream)))
     return k, v
 
 
@@ -138,11 +149,12 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, l
         raise RuntimeError(f"lens must be contiguous [{b}]")
     if stream is not None:
         with _on(stream):
-            return _attention(q, cache, block_table, lens, scale, out, return_lse, ft, shape, table[1], _stream(stream))
-    return _attention(q, cache, block_table, lens, scale, out, return_lse, ft, shape, table[1], _stream(None))
+            return _attention(q, cache, block_table, lens, scale, out, return_lse, ft, shape, table[1], stream)
+    return _attention(q, cache, block_table, lens, scale, out, return_lse, ft, shape, table[1], None)
 
 
 def _attention(q, cache, block_table, lens, scale, out, return_lse, ft, shape, max_pages, stream):
+    _one_device(q.get_device(), cache.k_codes, block_table, lens, out)
     b, tq, hq, d = shape
     qb, qt, qh, qc = q.stride()
     if qc != 1:
@@ -157,5 +169,5 @@ def _attention(q, cache, block_table, lens, scale, out, return_lse, ft, shape, m
                                                                    block_table.stride(0), lens.data_ptr(),
                                                                    out.data_ptr(), lse.data_ptr() if return_lse else 0,
                                                                    ft, b, tq, hq, max_pages,
-                                                                   d ** -0.5 if scale is None else scale), stream))
+                                                                   d ** -0.5 if scale is None else scale), _stream(stream)))
     return (out, lse) if return_lse else out

@@ -35,6 +35,15 @@ def _device_tensor(t, dtype, what: str) -> None:
         raise RuntimeError("tensor arguments must be CUDA device tensors")
 
 
+def _one_device(at: int, *tensors) -> None:
+    """The launch goes to the current device, so all tensors of a call (and its first's number `at`) have to be there."""
+    for t in tensors:
+        if t is not None and t.get_device() != at:
+            raise RuntimeError("the tensors of a call must be on one device")
+    if at != torch.cuda.current_device():
+        raise RuntimeError(f"the tensors are on CUDA device {at}, the current device is {torch.cuda.current_device()}")
+
+
 def _on(stream):
     """Context whose allocations and copies belong to `stream` (the current one when None)."""
     if stream is None:
@@ -122,11 +131,12 @@ def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None, ou
             raise RuntimeError(f"bias must be contiguous [{n}]")
     if stream is not None:
         with _on(stream):
-            return _linear(x, w, bias, out, ft, n, k, _stream(stream))
-    return _linear(x, w, bias, out, ft, n, k, _stream(None))
+            return _linear(x, w, bias, out, ft, n, k, stream)
+    return _linear(x, w, bias, out, ft, n, k, None)
 
 
 def _linear(x, w, bias, out, ft, n, k, stream):
+    _one_device(x.get_device(), w.codes, bias, out)
     rows = x if x.dim() == 2 else x.reshape(-1, k)
     ldx, step = rows.stride()
     m = rows.shape[0]
@@ -147,5 +157,5 @@ def _linear(x, w, bias, out, ft, n, k, stream):
     _lib.check(_lib.lib().b200q_linear_w4(_ARGS.pack(rows.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(),
                                                      0 if zeros is None else zeros.data_ptr(),
                                                      0 if bias is None else bias.data_ptr(), y.data_ptr(), ldy, ft, m,
-                                                     n, k, w.group), stream))
+                                                     n, k, w.group), _stream(stream)))
     return out
