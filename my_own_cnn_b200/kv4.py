@@ -10,8 +10,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .conv import _stream
-from .w4 import FTYPES, _device_tensor, _ftype, _on, _one_device
+from .w4 import FTYPES, _device_tensor, _ftype, _launch_stream, _on
 
 
 _CACHE = _lib.packer(_lib.CKV4Cache)
@@ -37,12 +36,13 @@ class KV4Cache:
             raise TypeError("cache codes must be uint8")
         if k_params.dtype != torch.int32 or v_params.dtype != torch.int32:
             raise TypeError("cache params must be int32")
+        at = k_codes.get_device()
         for x in (k_codes, k_params, v_codes, v_params):
             if not x.is_contiguous():
                 raise RuntimeError("cache tensors must be contiguous")
             if not x.is_cuda:
                 raise RuntimeError("tensor arguments must be CUDA device tensors")
-            if x.get_device() != k_codes.get_device():
+            if x.get_device() != at:
                 raise RuntimeError("the tensors of a cache must be on one device")
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
         self.pages, self.heads, self.page_size, half = shape
@@ -93,13 +93,13 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.T
 
 
 def _append(cache, k, v, slots, ft, stream):
-    _one_device(k.get_device(), v, slots, cache.k_codes)
+    handle = _launch_stream(stream, k, v, slots, cache.k_codes)
     (kt, kh, kc), (vt, vh, vc) = k.stride(), v.stride()
     if kc != 1 or vc != 1:
         k, v = k.contiguous(), v.contiguous()
         (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
     _lib.check(_lib.lib().b200q_kv4_append(cache._c, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, slots.data_ptr(), ft,
-                                           k.shape[0], _stream(stream)))
+                                           k.shape[0], handle))
 
 
 def kv4_read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.float32,
@@ -116,11 +116,11 @@ def kv4_read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.fl
 
 
 def _read(cache, slots, dtype, ft, stream):
-    _one_device(slots.get_device(), cache.k_codes)
+    handle = _launch_stream(stream, slots, cache.k_codes)
     t = slots.shape[0]
     k = slots.new_empty((t, cache.heads, cache.head_dim), dtype=dtype)
     v = torch.empty_like(k)
-    _lib.check(_lib.lib().b200q_kv4_read(cache._c, slots.data_ptr(), k.data_ptr(), v.data_ptr(), ft, t, _stream(stream)))
+    _lib.check(_lib.lib().b200q_kv4_read(cache._c, slots.data_ptr(), k.data_ptr(), v.data_ptr(), ft, t, handle))
     return k, v
 
 
@@ -154,7 +154,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, l
 
 
 def _attention(q, cache, block_table, lens, scale, out, return_lse, ft, shape, max_pages, stream):
-    _one_device(q.get_device(), cache.k_codes, block_table, lens, out)
+    handle = _launch_stream(stream, q, cache.k_codes, block_table, lens, out)
     b, tq, hq, d = shape
     qb, qt, qh, qc = q.stride()
     if qc != 1:
@@ -169,5 +169,5 @@ def _attention(q, cache, block_table, lens, scale, out, return_lse, ft, shape, m
                                                                    block_table.stride(0), lens.data_ptr(),
                                                                    out.data_ptr(), lse.data_ptr() if return_lse else 0,
                                                                    ft, b, tq, hq, max_pages,
-                                                                   d ** -0.5 if scale is None else scale), _stream(stream)))
+                                                                   d ** -0.5 if scale is None else scale), handle))
     return (out, lse) if return_lse else out

@@ -9,8 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .conv import _stream
-from .w4 import FTYPES, _device_tensor, _ftype, _on, _one_device
+from .w4 import FTYPES, _device_tensor, _ftype, _launch_stream, _on
 
 
 _ARGS = _lib.packer(_lib.CQKNormArgs)
@@ -76,7 +75,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
 
 def _norm(q, k, q_weight, k_weight, table, positions, eps, interleaved, q_out, k_out, ft, t, hq, hk, d, rot, rows,
           stream):
-    _one_device(q.get_device(), k, q_weight, k_weight, table, positions, q_out, k_out)
+    handle = _launch_stream(stream, q, k, q_weight, k_weight, table, positions, q_out, k_out)
     (qt, qh, qc), (kt, kh, kc) = q.stride(), k.stride()
     if qc != 1:
         q = q.contiguous()
@@ -97,7 +96,7 @@ def _norm(q, k, q_weight, k_weight, table, positions, eps, interleaved, q_out, k
     _lib.check(_lib.lib().b200q_qk_norm_rope(_ARGS.pack(q.data_ptr(), k.data_ptr(), _p(q_weight), _p(k_weight), _p(table),
                                                         _p(positions), q_out.data_ptr(), k_out.data_ptr(), 0, 0, 0, 0,
                                                         qt, qh, kt, kh, ot, oh, pt, ph, rows, ft, t, hq, hk, d, rot,
-                                                        interleaved, eps), _stream(stream)))
+                                                        interleaved, eps), handle))
     return q_out, k_out
 
 
@@ -118,7 +117,7 @@ def qk_norm_rope_bprop(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: t
     _device_tensor(dq, q.dtype, "dq")
     _device_tensor(dk, q.dtype, "dk")
     with _on(stream):
-        _one_device(q.get_device(), k, dq, dk, q_weight, k_weight, table, positions)
+        handle = _launch_stream(stream, q, k, dq, dk, q_weight, k_weight, table, positions)
         if q.stride(2) != 1:
             q = q.contiguous()
         if k.stride(2) != 1:
@@ -131,5 +130,5 @@ def qk_norm_rope_bprop(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: t
             _ARGS.pack(q.data_ptr(), k.data_ptr(), _p(q_weight), _p(k_weight), _p(table), _p(positions), gq.data_ptr(),
                        gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), _p(gqw), _p(gkw), q.stride(0), q.stride(1),
                        k.stride(0), k.stride(1), 0, 0, 0, 0, rows, ft, t, hq, hk, d, rot, interleaved, eps),
-            _stream(stream)))
+            handle))
     return gq, gk, gqw, gkw

@@ -12,7 +12,7 @@ import contextlib
 import torch
 
 from . import _lib
-from .conv import _stream
+from .conv import _raw_stream, _stream
 
 _ARGS = _lib.packer(_lib.CLinearW4Args)
 FTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -35,13 +35,16 @@ def _device_tensor(t, dtype, what: str) -> None:
         raise RuntimeError("tensor arguments must be CUDA device tensors")
 
 
-def _one_device(at: int, *tensors) -> None:
-    """The launch goes to the current device, so all tensors of a call (and its first's number `at`) have to be there."""
+def _launch_stream(stream, *tensors) -> int:
+    """The handle of `stream` (the current one when None), to which the current device belongs: all CUDA tensors of the call have
+    to be there (each one's own check asks whether it is one)."""
+    at = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and t.get_device() != at:
-            raise RuntimeError("the tensors of a call must be on one device")
-    if at != torch.cuda.current_device():
-        raise RuntimeError(f"the tensors are on CUDA device {at}, the current device is {torch.cuda.current_device()}")
+        if t is not None and t.get_device() != at and t.is_cuda:
+            if any(x is not None and x.is_cuda and x.get_device() != t.get_device() for x in tensors):
+                raise RuntimeError("the tensors of a call must be on one device")
+            raise RuntimeError(f"the tensors are on CUDA device {t.get_device()}, the current device is {at}")
+    return _raw_stream(at) if stream is None and _raw_stream is not None else _stream(stream)
 
 
 def _on(stream):
@@ -136,7 +139,7 @@ def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None, ou
 
 
 def _linear(x, w, bias, out, ft, n, k, stream):
-    _one_device(x.get_device(), w.codes, bias, out)
+    handle = _launch_stream(stream, x, w.codes, bias, out)
     rows = x if x.dim() == 2 else x.reshape(-1, k)
     ldx, step = rows.stride()
     m = rows.shape[0]
@@ -157,5 +160,5 @@ def _linear(x, w, bias, out, ft, n, k, stream):
     _lib.check(_lib.lib().b200q_linear_w4(_ARGS.pack(rows.data_ptr(), ldx, w.codes.data_ptr(), w.scales.data_ptr(),
                                                      0 if zeros is None else zeros.data_ptr(),
                                                      0 if bias is None else bias.data_ptr(), y.data_ptr(), ldy, ft, m,
-                                                     n, k, w.group), _stream(stream)))
+                                                     n, k, w.group), handle))
     return out
