@@ -8,6 +8,7 @@
 from __future__ import annotations
 
 import contextlib
+import math
 
 import torch
 
@@ -140,7 +141,7 @@ def linear_w4(x: torch.Tensor, w: W4Weight, bias: torch.Tensor | None = None, ou
 
 def _linear(x, w, bias, out, ft, n, k, stream):
     handle = _launch_stream(stream, x, w.codes, bias, out)
-    rows = x if x.dim() == 2 else x.reshape(-1, k)
+    rows = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), k)
     ldx, step = rows.stride()
     m = rows.shape[0]
     if step != 1 or (ldx < k and m > 1):  # columns apart, or rows that overlap (a broadcast)
