@@ -269,7 +269,8 @@ int b200q_kv4_read(const b200q_kv4_cache* c, const int64_t* slots, void* k, void
  * block_table[b][0 .. max_pages), row stride bt_stride; none seen: output 0, lse -inf.
  * q [b][tq][hq][d] with strides; query head h reads cache head h / (hq / heads).
  * out contiguous [b][tq][hq][d]; lse fp32 [b][tq][hq] or NULL: log of the sum of exp(scale * q.k).
- * Uses the stream's scratch: sequences are split over blocks. */
+ * Uses the stream's scratch: sequences are split over blocks.  Lengths and tables stay as they are until the call has run: what
+ * changes them is put into the same stream, or waits. */
 typedef struct b200q_kv4_attention_args {
   const void* q;
   int64_t q_bs, q_ts, q_hs;

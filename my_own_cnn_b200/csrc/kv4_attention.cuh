@@ -191,7 +191,7 @@ __device__ __forceinline__ void load_tile_page(const Cache& c, uint32_t stage, u
 // Where a block stands: in shared memory, so that it takes no registers while tiles are computed.
 struct Plan {
   uint32_t total, stop, at, base;  // steps of all units, the block's end, its next step, its sequence's first
-  int seq, n;                      // the sequence, the steps of each of its units
+  int seq, len, n;                 // the sequence, its length, the steps of each of its units
   // the unit at hand: its sequence, cache head and tile of rows, whether its first part is here, the block of that,
   // how many parts it has
   int unit_seq, head, tile, begins, owner, parts;
@@ -218,25 +218,28 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, g = lane / 4, t = lane % 4;
 
   const int units = c.heads * a.row_tiles, ratio = a.hq / c.heads;
-  auto steps_of = [&](int i) { return kUnitSteps + max(1, (valid_length(c, a, i) + kStepTokens - 1) / kStepTokens); };
+  auto steps_of = [&](int len) { return kUnitSteps + max(1, (len + kStepTokens - 1) / kStepTokens); };
   // Block i takes total / blocks steps, and one more while i is below the remainder.  A cut that would leave a part of less
   // than kMinSteps steps at a unit's start or end moves there.
   auto blocks_for = [&](uint32_t total) { return min(gridDim.x, total); };
-  {
+  // (By one warp, and each length that a unit goes by is read once: a block's threads agree, stay in bounds and end even if a
+  // program changes the lengths meanwhile.)
+  auto plan_block = [&]() -> Plan {
     uint32_t total = 0;
-    for (int i = lane; i < a.b; i += 32) total += steps_of(i);
+    for (int i = lane; i < a.b; i += 32) total += steps_of(valid_length(c, a, i));
 #pragma unroll
     for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(~0u, total, x);
     total *= units;
     const uint32_t blocks = blocks_for(total);
-    if (blockIdx.x >= blocks) return;
+    if (blockIdx.x >= blocks) return Plan{};
     const uint32_t per = total / blocks, more = total - per * blocks;
-    int seq = 0, n = 0;
+    int seq = 0, len = 0, n = 0;
     uint32_t base = 0;
-    auto find = [&](uint32_t step) {  // the sequence of a step
+    // the sequence of a step; none only where lengths were changed since they were added up: the block then ends
+    auto find = [&](uint32_t step) {
       base = 0;
-      for (seq = 0;; seq += 32) {
-        const int mine = seq + lane < a.b ? steps_of(seq + lane) : 0;
+      for (seq = 0; seq < a.b; seq += 32) {
+        const int own = seq + lane < a.b ? valid_length(c, a, seq + lane) : 0, mine = seq + lane < a.b ? steps_of(own) : 0;
         uint32_t sum = mine * units;
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
@@ -246,31 +249,40 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
         const unsigned past = __ballot_sync(~0u, base + sum > step);
         if (past) {
           const int first = __ffs(past) - 1;
-          n = __shfl_sync(~0u, mine, first);
+          len = __shfl_sync(~0u, own, first);
+          n = steps_of(len);
           base += __shfl_sync(~0u, sum, first) - n * units;
           seq += first;
-          return;
+          return true;
         }
         base += __shfl_sync(~0u, sum, 31);
       }
+      return false;
     };
     auto cut = [&](uint32_t i) {
       const uint32_t step = i * per + min(i, more);
-      if (step >= total) return total;
-      find(step);
+      if (step >= total || !find(step)) return total;
       const uint32_t unit_at = base + (step - base) / n * n;
       return step - unit_at < kUnitSteps + kMinSteps ? unit_at : unit_at + n - step < kMinSteps ? unit_at + n : step;
     };
     const uint32_t stop = cut(blockIdx.x + 1), at = cut(blockIdx.x);
-    if (at >= stop) return;
-    if (at == base + static_cast<uint32_t>(n) * units) base = at, n = steps_of(++seq);
-    if (tid == 0) plan = Plan{total, stop, at, base, seq, n};
+    if (at >= stop || seq >= a.b) return Plan{};
+    if (at == base + static_cast<uint32_t>(n) * units) {
+      if (++seq >= a.b) return Plan{};
+      base = at, len = valid_length(c, a, seq), n = steps_of(len);
+    }
+    return Plan{total, stop, at, base, seq, len, n};
+  };
+  if (warp == 0) {
+    const Plan mine = plan_block();
+    if (lane == 0) plan = mine;
   }
   __syncthreads();
+  if (plan.at >= plan.stop) return;
 
   for (;;) {
     // steps [off, off + count) of the unit; its first kUnitSteps steps stand for what it costs besides
-    const int seq = plan.seq, len = valid_length(c, a, seq), unit = static_cast<int>((plan.at - plan.base) / plan.n);
+    const int seq = plan.seq, len = plan.len, unit = static_cast<int>((plan.at - plan.base) / plan.n);
     const uint32_t unit_at = plan.base + unit * plan.n, end = min(unit_at + plan.n, plan.stop);
     const int off = max(0, static_cast<int>(plan.at - unit_at) - kUnitSteps), count = static_cast<int>(end - unit_at) - kUnitSteps - off;
     const int tile = unit % a.row_tiles, head = unit / a.row_tiles, rows = min(kRows, a.tq * ratio - tile * kRows);
@@ -293,9 +305,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
         const uint32_t longer = more * (per + 1);
         return step < longer ? step / (per + 1) + 1 : more + (step - longer) / per + 1;
       };
-      const uint32_t before = cuts_to(unit_at + kUnitSteps + kMinSteps - 1);
+      const uint32_t before = min(cuts_to(unit_at + kUnitSteps + kMinSteps - 1), blocks);
       plan.owner = static_cast<int>(before) - 1;
-      plan.parts = plan.n >= kUnitSteps + 2 * kMinSteps ? 1 + static_cast<int>(cuts_to(unit_at + plan.n - kMinSteps) - before) : 1;
+      plan.parts = plan.n >= kUnitSteps + 2 * kMinSteps ? 1 + static_cast<int>(min(cuts_to(unit_at + plan.n - kMinSteps), blocks) - before) : 1;
       plan.unit_seq = seq;
       plan.head = head;
       plan.tile = tile;
@@ -303,7 +315,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
       plan.at = end;
       if (end == plan.base + static_cast<uint32_t>(plan.n) * units && end < plan.stop) {
         plan.base = end;
-        plan.n = steps_of(++plan.seq);
+        if (++plan.seq < a.b)
+          plan.len = valid_length(c, a, plan.seq), plan.n = steps_of(plan.len);
+        else
+          plan.stop = end;
       }
     }
     // the last row of the tile sees the most tokens
