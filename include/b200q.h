@@ -199,7 +199,7 @@ enum b200q_ftype { B200Q_F32 = 0, B200Q_F16 = 1, B200Q_BF16 = 2 };
 
 /* y[m][n] = sum_k x[m][k] * (code[n][k] - zero[k / group][n]) * scale[k / group][n] (+ bias[n]).
  * codes: [n][16 * ceil(k / 32)] bytes, 16-byte aligned (the nibbles past k are not used);
- * scales: bf16 [ceil(k / group)][n]; zeros: uint8 in 0..15, same shape, or NULL for 8 everywhere;
+ * scales: bf16 [ceil(k / group)][n]; zeros: uint8 (0 to 255), same shape, or NULL for 8 everywhere;
  * group 32, 64 or 128.  x [m][k] with row stride ldx, y [m][n] with row stride ldy; bias [n] or NULL.
  * Made for the few rows of a decode step: weights are read once per 16 rows of x.  A NaN or an
  * infinity in a row of x makes that row's results NaN or infinite.  y shares no memory with x. */

@@ -3,7 +3,7 @@
 //   y[m][n] = sum_g s[g][n] sum_{k in g} (c[n][k] - z[g][n]) x[m][k]
 //
 // Bytes bound it: K / 2 of codes and 2 or 3 per group for each weight row; and, as measured, the latency of its instructions
-// with 16 warps an SM.  1 x 8192 x 8192 bf16: 11.6 us, 3.0 TB/s; 16 x 16384 x 8192: 34.5 us, 2.1 TB/s; 1 x 768 x 768: 3.0 us.
+// with 16 warps an SM.  1 x 8192 x 8192 bf16: 11.3 us, 3.1 TB/s; 16 x 16384 x 8192: 35.3 us, 2.1 TB/s; 1 x 768 x 768: 3.0 us.
 // The codes are the 16-row operand A of m16n8k16 (weight rows x K) and up to 16 rows of x its 8 columns, once or twice;
 // m16n8k16 from registers because a code leaves its word as an operand in two instructions, while tcgen05
 // operands would have to be written to shared memory first, four times the bytes that were read.
@@ -11,8 +11,8 @@
 //   same of the zero point it is exact and normal.  A word of 8 codes becomes four operands, the pairs (0,4) (1,5) (2,6) (3,7),
 //   and every second value of x is divided by 16 instead.  x is scaled by a power of two per row and step to a maximum in
 //   [2^14, 2^15), so that it fits fp16 whatever its type; fp32 becomes two fp16 terms (22 bits).
-//   (The bare nibble, a subnormal, with the zero points' sum kept apart, saves the subtraction: 10.6 against 11.6 us for one
-//   row of 8192 x 8192, 34.9 against 34.5 for 16 rows.  But the adder lines subnormals up by their exponent field and truncates
+//   (The bare nibble, a subnormal, with the zero points' sum kept apart, saves the subtraction: 10.6 against 11.3 us for one
+//   row of 8192 x 8192, 34.9 against 35.3 for 16 rows.  But the adder lines subnormals up by their exponent field and truncates
 //   about 10 of the sum's bits, and where x has one sign the two sums are many times their difference: fp16 results after a
 //   squared ReLU were off by 6e-5, all one way.)
 //
@@ -78,6 +78,12 @@ struct Layout {
 __device__ __forceinline__ int piece_at(int row, int piece) {
   const int flip = (row & 1) << 2 | (row & 2) | (row >> 2 & 1);
   return row * (kStep / 2) + ((piece ^ flip) << 4);
+}
+
+// 1024 + 16 z of 1024 + z, on two fp16 values; exact for every z below 256.
+__device__ __forceinline__ uint32_t times_16(uint32_t v) {
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(16.0f), __float2half2_rn(-15360.0f));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 __device__ __forceinline__ float peer_load(uint32_t addr, int rank) {
@@ -278,9 +284,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
         }
       }
       constexpr uint32_t kMagic = 0x64006400u;  // two fp16 1024
-      uint32_t zpair[4];  // the rows' zero points, twice
+      uint32_t zpair[4];  // 1024 + the rows' zero points, twice
 #pragma unroll
-      for (int r = 0; r < 4; ++r) zpair[r] = __shfl_sync(~0u, zero[i], r * 8 + g) * 0x00010001u;
+      for (int r = 0; r < 4; ++r) zpair[r] = __shfl_sync(~0u, zero[i], r * 8 + g) * 0x00010001u | kMagic;
       float part[2][NT][4];
 #pragma unroll
       for (int word = 0; word < kWords; ++word) {
@@ -298,8 +304,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) linear_w4_kernel(W4Args a) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const uint32_t v = w[2 * mt + u][word] >> (j / 2 * 8), mask = j % 2 ? 0x00F000F0u : 0x000F000Fu;
-              c[u][j] = sub_f16x2(and_or(v, mask, kMagic),
-                                  j % 2 ? and_or(zpair[2 * mt + u] << 4, mask, kMagic) : zpair[2 * mt + u] | kMagic);
+              c[u][j] = sub_f16x2(and_or(v, mask, kMagic), j % 2 ? times_16(zpair[2 * mt + u]) : zpair[2 * mt + u]);
             }
 #pragma unroll
           for (int term = 0; term < kTerms; ++term)
