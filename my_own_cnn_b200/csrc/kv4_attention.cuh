@@ -16,7 +16,8 @@
 //   the others'.  (fp16 weights of 11 and 22 bits take 71 and 92 us below, but on a step of 2^-24 of the largest they put 16-bit
 //   outputs off by 2e-4 before their own rounding, and fp32 ones by 1e-5 to 6e-2 where one token or one group of channels
 //   outweighs the rest by 2^10 to 2^20.)
-//   The adder truncates, so fp32 calls add a tile's sums up outside of it.
+//   The adder truncates, always towards 0, so a tile's sums are added up outside of it (79 and 99 us below without, but 131072 tokens
+//   that one block adds up leave outputs 5e-5 low, and it grows with the length).
 //   P leaves the first product as (token, row) and must enter the second as (row, token): movmatrix.
 // The maximum m[r] is a running reference, raised (and the sums rescaled) only when a score passes it by more than
 // 2^8: a warp-wide maximum is taken a few times per sequence, not per tile.
@@ -27,8 +28,8 @@
 // the scratch, and the block that finishes last joins them in order.
 //
 // What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head; and, as measured, the latency of its
-// instructions with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 79.5 us,
-// 2.8 TB/s; 2 x 131072, fp16: 101 us, 3.0 TB/s; 1 x 77 fp32: 6 us, all latency.
+// instructions with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 81.7 us,
+// 2.8 TB/s; 2 x 131072, fp16: 102 us, 3.0 TB/s; 1 x 77 fp32: 6 us, all latency.
 //   Each warp owns a ring of kStages tiles of kTile tokens that it fills with 16-byte asynchronous copies and empties on its
 // own: no block-wide barrier until the end.  A row of codes is padded by 16 bytes in shared memory: then lanes (g, t)
 // reading 4 bytes at g rows down, and 2t rows down, both touch 32 banks once.
@@ -543,7 +544,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
           }
       }
 
-      // values; in fp32 calls a tile's sums are made apart and added with rounding
+      // values; a tile's sums are made apart and added with rounding
       constexpr int kPTerms = F32 ? 3 : 2;
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) {
@@ -605,23 +606,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128
             for (int term = 0; term < kPTerms; ++term)
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                if (!F32)
-                  mma_bf16(o[k * (G / 16) + j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
-                else if (mt == 0 && term == 0)
+                if (mt == 0 && term == 0)
                   mma_bf16_first(part[j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
                 else
                   mma_bf16(part[j][n], a0, a1, a2, a3, b[term][n][0], b[term][n][1]);
               }
           }
         }
-        if constexpr (F32) {
 #pragma unroll
-          for (int j = 0; j < G / 16; ++j)
+        for (int j = 0; j < G / 16; ++j)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[k * (G / 16) + j][n][e] += part[j][n][e];
-        }
+            for (int e = 0; e < 4; ++e) o[k * (G / 16) + j][n][e] += part[j][n][e];
       }
 #pragma unroll
       for (int i = 0; i < kStages - 1; ++i) held[i] = held[i + 1];

@@ -123,3 +123,21 @@ def test_scales_of_either_sign(dtype):
     out = b2q.kv4_attention(q, c, table, lens)[0, 0]
     want, _ = definition(q[0, 0], kk, vv, d ** -0.5)
     assert apart(out, want) <= (2.0 ** -20 if dtype == torch.float32 else UNIT[dtype] + 2.0 ** -16)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,mean", [(64, 0.0), (64, 1.0), (128, 1.0)])
+def test_long_sums_do_not_drift(dtype, d, mean):
+    """Sequences that one block each adds up from end to end (more units than blocks; they share their pages): with every tile's
+    sum rounded once to 2^-24, 4096 tiles in four warps are off by 2^-24 sqrt(1024) of the sum at most likely, below e."""
+    n, b = 131072, 640
+    k, v = normal(1, n, d), normal(2, n, d) + mean
+    c, table, lens, kk, vv = held(k, v, 64)
+    q = normal(3, b, 1, 1, d).to(dtype)
+    out = b2q.kv4_attention(q, c, table.expand(b, -1).contiguous(), lens.expand(b).contiguous(), scale=d ** -0.5)[::16, 0, 0]
+    want, _ = definition(q[::16, 0, 0], kk, vv, d ** -0.5)
+    if dtype == torch.float32:
+        assert apart(out, want) <= 2.0 ** -23 * (d / 16 + 2) + 2.0 ** -20
+    else:
+        once = want.to(dtype).double()
+        assert float((out.double() - once).norm() / once.norm()) <= (2 * UNIT[dtype] * 2.0 ** -16) ** 0.5
