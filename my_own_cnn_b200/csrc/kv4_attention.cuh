@@ -16,7 +16,7 @@
 //   the others'.  (fp16 weights of 11 and 22 bits take 71 and 92 us below, but on a step of 2^-24 of the largest they put 16-bit
 //   outputs off by 2e-4 before their own rounding, and fp32 ones by 1e-5 to 6e-2 where one token or one group of channels
 //   outweighs the rest by 2^10 to 2^20.)
-//   The adder truncates, always towards 0, so a tile's sums are added up outside of it (79 and 99 us below without, but 131072 tokens
+//   The adder truncates, always towards 0, so a tile's sums are added up outside of it (3 % of the time below, but 131072 tokens
 //   that one block adds up leave outputs 5e-5 low, and it grows with the length).
 //   P leaves the first product as (token, row) and must enter the second as (row, token): movmatrix.
 // The maximum m[r] is a running reference, raised (and the sums rescaled) only when a score passes it by more than
@@ -28,7 +28,7 @@
 // the scratch, and the block that finishes last joins them in order.
 //
 // What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head; and, as measured, the latency of its
-// instructions with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 81.7 us,
+// instructions with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 79.5 us,
 // 2.8 TB/s; 2 x 131072, fp16: 102 us, 3.0 TB/s; 1 x 77 fp32: 6 us, all latency.
 //   Each warp owns a ring of kStages tiles of kTile tokens that it fills with 16-byte asynchronous copies and empties on its
 // own: no block-wide barrier until the end.  A row of codes is padded by 16 bytes in shared memory: then lanes (g, t)
@@ -68,12 +68,12 @@ struct AttnArgs {
 
 constexpr int kMinSteps = 2;  // steps of a unit's first and last part at least
 // What a unit costs besides its steps (its queries, its first tiles' way, its join), in steps: 48 sequences of 128 to 8192
-// tokens 66 us with 2 or 3, 69 with 5 (and 109 to 79 from 1 to 3 when a step took longer).
-constexpr int kUnitSteps = 3;
+// tokens 79.5 us with 2, 80.9 with 1, 81.3 with 3, 84.6 with 5; 1 x 1024 10.5 us, 12.0, 11.7 and 12.0.
+constexpr int kUnitSteps = 2;
 
 constexpr int kTile = 32;    // tokens of a warp's step
 constexpr int kWarps = 4;    // a block's warps take tiles in turn
-constexpr int kStages = 2;   // tiles of a warp's ring: a third one costs a block an SM for heads of 256 (125 against 93 us)
+constexpr int kStages = 2;   // tiles of a warp's ring: a third one costs a block an SM for heads of 256 (85 against 60 us)
 constexpr int kStepTokens = kWarps * kTile;
 
 // How far a weight may pass 1 before its row's reference is raised, and its logarithm.
@@ -198,8 +198,8 @@ struct Plan {
   int unit_seq, head, tile, begins, owner, parts;
 };
 
-// Blocks an SM: three at up to 168 registers a thread for heads of 128 (2 x 131072 tokens: 89 us, 98 with four and spills),
-// four for heads of 64 (63 us, 69 with three); 16 rows a pass or 256 channels take what they need.
+// Blocks an SM: three at up to 168 registers a thread for heads of 128 (2 x 131072 tokens: 102 us, 128 with four and spills,
+// 111 with two), four for heads of 64 (48 sequences of up to 8192: 51.7 us, 53.6 with three); 16 rows a pass or 256 channels take what they need.
 template <int D, int G, int NT, bool F32>
 __global__ void __launch_bounds__(kWarps * 32, NT > 1 || D == 256 ? 1 : D == 128 ? 3 : 4) kv4_attention_kernel(Cache c, AttnArgs a) {
   using Shape = AttnShape<D, G, NT, F32>;

@@ -66,7 +66,7 @@ struct Layout {
   static constexpr int kX = kStep * 2 * kTerms * kRowsX;
   static constexpr int kBuffer = (kX + kRowsX * 4 + 15) / 16 * 16;
   // Three stages where two blocks still fit an SM (228 KB, 1 KB of it taken per block); 16 rows of fp32 leave room for two:
-  // 16 x 11000 x 12000 fp32 48 us, 69 with one block and three.
+  // 16 x 11000 x 12000 fp32 47 us, 69 with one block and three.
   static constexpr int kStages = FEW || kWarps * 3 * kStage + 2 * kBuffer > 113 * 1024 ? 2 : 3;
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kBuffers = FEW ? (46 * 1024) / kBuffer : 2;
@@ -421,9 +421,10 @@ int launch_linear(W4Args a, int sms, int device, cudaStream_t stream) {
 
 template <typename T, int G>
 int launch_linear_rows(const W4Args& a, int sms, int device, cudaStream_t stream) {
-  // One row of x: 1 x 8192 x 8192 bf16 11.0 us, 12.0 with blocks of 256 weight rows; 1 x 16000 x 1000 7.2 and 12.9;
-  // 1 x 768 x 768 3.1 and 4.5.  Two to four: only while those blocks, K split eight ways, would leave SMs idle
-  // (2 x 16000 x 1000 fp32 8.9 and 16.1 us, but 4 x 8192 x 8192 bf16 22.2 and 13.0: each block brings x in).
+  // (In a graph, weights that L2 does not hold.)  One row of x: 1 x 8192 x 8192 bf16 11.9 us, 12.2 with blocks of 256 weight
+  // rows; 1 x 16000 x 1000 8.2, 8.3 with kFewRows rows of room; 1 x 768 x 768 fp16 3.36 and 3.44.  Two to four: only while blocks of
+  // 256, K split eight ways, would leave SMs idle (2 x 16000 x 1000 fp32 9.6 us, 16.8 with those, 4 x 16000 x 1000 bf16 10.3 and
+  // 14.2, but 4 x 8192 x 8192 bf16 22.7 and 13.8: each block brings x in).
   if (a.m == 1 && a.k <= kMaxSplit * kStep * Layout<T, G, 1, 1>::kBuffers) return launch_linear<T, G, 1, 1>(a, sms, device, stream);
   if (a.m <= kFewRows && (a.n + 255) / 256 * kMaxSplit < sms && a.k <= kMaxSplit * kStep * Layout<T, G, 1, kFewRows>::kBuffers)
     return launch_linear<T, G, 1, kFewRows>(a, sms, device, stream);
