@@ -1081,9 +1081,26 @@ bool had_scratch(int dev, cudaStream_t stream) {
   return it != g_scratch.of_stream.end() && it->second->base;
 }
 
+// While it lives the thread may allocate and wait although some stream, here or in another thread, is captured: what it does has
+// nothing to do with the capture.
+class OutsideCapture {
+ public:
+  OutsideCapture() { ok_ = cudaThreadExchangeStreamCaptureMode(&mode_) == cudaSuccess; }
+  ~OutsideCapture() {
+    if (ok_) cudaThreadExchangeStreamCaptureMode(&mode_);
+  }
+  OutsideCapture(const OutsideCapture&) = delete;
+  OutsideCapture& operator=(const OutsideCapture&) = delete;
+
+ private:
+  cudaStreamCaptureMode mode_ = cudaStreamCaptureModeRelaxed;
+  bool ok_;
+};
+
 // Scratch that nothing uses, else new, with its counters zeroed in `stream`, which is not captured.  may_wait: for the device, so
 // that what destroyed streams left can be used.
 int new_scratch(int dev, cudaStream_t stream, bool may_wait, unsigned** base) {
+  const OutsideCapture outside;
   std::lock_guard<std::mutex> lk(g_scratch.mu);
   std::vector<unsigned*>& idle = g_scratch.idle[dev];
   auto& retired = g_scratch.retired[dev];
@@ -1141,17 +1158,16 @@ int scratch_of_capture(int dev, cudaStream_t stream, std::shared_ptr<Scratch>* o
   std::lock_guard<std::mutex> lk((*out)->mu);
   if ((*out)->base) return B200Q_OK;
   // made on a stream of its own, which the capture has nothing to do with
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  if ((e = cudaThreadExchangeStreamCaptureMode(&mode)) != cudaSuccess) return cuda_fail(e, "cudaThreadExchangeStreamCaptureMode");
-  cudaStream_t side = nullptr;
   unsigned* base = nullptr;
-  int rc = B200Q_OK;
-  if ((e = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking)) != cudaSuccess) rc = cuda_fail(e, "cudaStreamCreate(scratch)");
-  if (!rc) rc = new_scratch(dev, side, false, &base);
-  if (!rc && (e = cudaStreamSynchronize(side)) != cudaSuccess) rc = cuda_fail(e, "cudaStreamSynchronize(scratch)");
-  if (side) cudaStreamDestroy(side);
-  cudaThreadExchangeStreamCaptureMode(&mode);
-  if (rc) return rc;
+  {
+    const OutsideCapture outside;
+    cudaStream_t side = nullptr;
+    if ((e = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking)) != cudaSuccess) return cuda_fail(e, "cudaStreamCreate(scratch)");
+    int rc = new_scratch(dev, side, false, &base);
+    if (!rc && (e = cudaStreamSynchronize(side)) != cudaSuccess) rc = cuda_fail(e, "cudaStreamSynchronize(scratch)");
+    cudaStreamDestroy(side);
+    if (rc) return rc;
+  }
   auto owned = std::make_unique<GraphScratch>(GraphScratch{key, base});
   cudaUserObject_t object = nullptr;
   e = cudaUserObjectCreate(&object, owned.get(), GraphScratch::destroy, 1, cudaUserObjectNoDestructorSync);

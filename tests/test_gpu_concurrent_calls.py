@@ -180,3 +180,26 @@ def test_a_graph_gives_its_scratch_back():
         if i == 10:
             free = torch.cuda.mem_get_info()[0]
     assert torch.cuda.mem_get_info()[0] > free - (48 << 20)
+
+
+@pytest.mark.parametrize("mode", ["global", "thread_local", "relaxed"])
+def test_eager_calls_while_another_thread_captures(mode):
+    """Calls on other streams, one of them without scratch yet, leave a capture that runs in another thread as it is."""
+    calls = [into(attention(i, n=8000)) for i in range(3)]
+    want = [call().clone() for call in calls]
+    s, old, new = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.Stream(priority=-1)
+    for x in (s, old, new):
+        x.wait_stream(torch.cuda.current_stream())
+    calls[0](stream=s)
+    calls[1](stream=old)
+    torch.cuda.synchronize()
+    outs = []
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s, capture_error_mode=mode):
+        t = threading.Thread(target=lambda: outs.extend([calls[1](stream=old), calls[2](stream=new)]))
+        t.start()
+        t.join()
+        out = calls[0](stream=s)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip([out] + outs, want)) and len(outs) == 2
