@@ -27,8 +27,8 @@
 // for a last wave.  The parts of a unit that several blocks share go to
 // the scratch, and the block that finishes last joins them in order.
 //
-// What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head; and, as measured, the latency of its
-// instructions with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 79.5 us,
+// What bounds it: bytes, D / 2 + 4 D / G for each of K and V per token and head; and, as measured, the latency of about 855
+// instructions per warp and tile with 12 warps an SM.  48 sequences of up to 8192 tokens, 32 / 8 heads x 128, bf16: 79.5 us,
 // 2.8 TB/s; 2 x 131072, fp16: 102 us, 3.0 TB/s; 1 x 77 fp32: 6 us, all latency.
 //   Each warp owns a ring of kStages tiles of kTile tokens that it fills with 16-byte asynchronous copies and empties on its
 // own: no block-wide barrier until the end.  A row of codes is padded by 16 bytes in shared memory: then lanes (g, t)

@@ -75,7 +75,7 @@ def _check_slots(slots, t=None):
 
 def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, stream=None) -> None:
     """k, v [t, heads, d] (views with contiguous channels will do) into slots int64 [t]; negative slots are
-    skipped, and no slot may be named twice."""
+    skipped, and no slot may be named twice.  A group of channels with a NaN or an infinity in it is stored as NaN."""
     ft = FTYPES.get(k.dtype)
     if ft is None or not k.is_cuda:
         _ftype(k, "k")
@@ -129,7 +129,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor, l
     """q [b, tq, hq, d]: the last tq tokens of each sequence, whose keys and values the cache already holds;
     lens int32 [b] counts all tokens, block_table int32 [b, max_pages] names each sequence's pages.  Token i sees
     the first lens - tq + i + 1 places; where that is none the output is 0 (lse -inf).  Query head h reads cache
-    head h // (hq / heads).  scale: 1 / sqrt(d) when None.  Returns out [b, tq, hq, d], and lse fp32 [b, tq, hq]
+    head h // (hq / heads).  Table and lengths stay as they are until the call has run.  scale: 1 / sqrt(d) when None.  Returns out [b, tq, hq, d], and lse fp32 [b, tq, hq]
     (log of the sum of exp(scale * q.k)) when return_lse."""
     ft = FTYPES.get(q.dtype)
     if ft is None or not q.is_cuda:
