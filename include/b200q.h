@@ -193,8 +193,8 @@ int b200q_bmm_s8(const int8_t* A, const int8_t* B, const int32_t* d_bias, const 
  * and reported by the next b200q_device_error() as B200Q_ERR_INVALID_ARG.
  * Attention and the gradient use 8 MiB of scratch: a stream's, which the first of their calls on it makes (not while the
  * stream is captured: B200Q_ERR_UNSUPPORTED), or, for calls that are captured, the graph's own, which is given back when the
- * graph and what was instantiated from it are destroyed.  Graphs may be replayed beside one another and beside eager calls;
- * two instances of one graph may not. */
+ * graph and what was instantiated from it are destroyed.  A destroyed stream's is used again for later streams.  Graphs
+ * may be replayed beside one another and beside eager calls; two instances of one graph may not. */
 enum b200q_ftype { B200Q_F32 = 0, B200Q_F16 = 1, B200Q_BF16 = 2 };
 
 /* y[m][n] = sum_k x[m][k] * (code[n][k] - zero[k / group][n]) * scale[k / group][n] (+ bias[n]).

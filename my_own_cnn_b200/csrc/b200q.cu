@@ -1009,11 +1009,13 @@ int f32_grad(const DeviceState& st, const float* x, const float* dy, float* dw, 
   return B200Q_OK;
 }
 
-// Scratch of a stream, or of a graph for what was captured into it on one stream: arrival counters of kernels whose last block joins the others' partial results (zeroed once,
-// and returned to zero by the block that sees the last arrival), then kScratchBytes.
+// Scratch of a stream, or of a graph for what was captured into it on one stream: arrival counters of kernels whose last
+// block joins the others' partial results (zeroed once, and returned to zero by the block that sees the last arrival), then
+// kScratchBytes.
 struct Scratch {
   std::mutex mu;  // held while a call that uses it is put into the stream
   unsigned* base = nullptr;
+  cudaEvent_t after = nullptr;  // the stream's last call; recorded once streams have been seen to come and go
 };
 using CaptureKey = std::pair<std::pair<int, cudaStream_t>, unsigned long long>;  // device, stream, the capture's number
 // The tables (never destroyed: threads may outlive them).  Scratch is found by the stream's own number: a handle may be another
@@ -1023,18 +1025,22 @@ struct ScratchTables {
   std::map<std::pair<int, unsigned long long>, std::unique_ptr<Scratch>> of_stream;  // (device, number)
   std::map<std::pair<int, cudaStream_t>, unsigned long long> number;                 // of the handle's last stream
   std::map<CaptureKey, std::shared_ptr<Scratch>> of_capture;   // until the graph is destroyed
+  std::atomic<bool> streams_end{false};                        // some stream was destroyed
   std::vector<std::unique_ptr<Scratch>> retired[kMaxDevices];  // of streams that are gone, whose last work may still run
   std::vector<unsigned*> idle[kMaxDevices];                    // that nothing uses
 
-  void retire(int dev, unsigned long long id) {
+  void retire(int dev, unsigned long long id) noexcept {
+    streams_end = true;
     auto it = of_stream.find({dev, id});
     if (it == of_stream.end()) return;
-    if (it->second->base) retired[dev].push_back(std::move(it->second));
-    of_stream.erase(it);
+    try {
+      if (it->second && it->second->after) retired[dev].push_back(std::move(it->second));
+    } catch (const std::exception&) {  // no memory for the table: it is not used again
+    }
+    of_stream.erase(it);  // (nor is what has no event: of the few streams that were there before the first one ended)
   }
 };
 ScratchTables& g_scratch = *new ScratchTables;
-constexpr size_t kRetiredMost = 8;
 
 // A thread's own streams (cudaStreamPerThread) end with it.
 struct ThreadStreams {
@@ -1078,7 +1084,7 @@ bool had_scratch(int dev, cudaStream_t stream) {
     key.second = it->second;
   }
   const auto it = g_scratch.of_stream.find(key);
-  return it != g_scratch.of_stream.end() && it->second->base;
+  return it != g_scratch.of_stream.end() && it->second && it->second->base;
 }
 
 // While it lives the thread may allocate and wait although some stream, here or in another thread, is captured: what it does has
@@ -1097,30 +1103,45 @@ class OutsideCapture {
   bool ok_;
 };
 
-// Scratch that nothing uses, else new, with its counters zeroed in `stream`, which is not captured.  may_wait: for the device, so
-// that what destroyed streams left can be used.
-int new_scratch(int dev, cudaStream_t stream, bool may_wait, unsigned** base) {
+// Scratch that nothing uses, else new, with its counters zeroed.  The tables are not locked while CUDA is called: what a graph
+// gives back comes from a thread of the driver's.
+int new_scratch(int dev, unsigned** base) {
   const OutsideCapture outside;
-  std::lock_guard<std::mutex> lk(g_scratch.mu);
-  std::vector<unsigned*>& idle = g_scratch.idle[dev];
-  auto& retired = g_scratch.retired[dev];
-  if (may_wait && idle.empty() && retired.size() >= kRetiredMost && cudaDeviceSynchronize() == cudaSuccess) {
-    for (auto& s : retired) idle.push_back(s->base);
-    retired.clear();
-  }
+  cudaStream_t side = nullptr;
+  cudaError_t e = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamCreate(scratch)");
+  const auto end = [](cudaStream_t* x) { cudaStreamDestroy(*x); };
+  const std::unique_ptr<cudaStream_t, decltype(end)> ended(&side, end);
   void* p = nullptr;
-  cudaError_t e = cudaSuccess;
-  if (!idle.empty()) {
+  std::vector<std::unique_ptr<Scratch>> gone;
+  auto take_idle = [&] {
+    auto& idle = g_scratch.idle[dev];
+    if (idle.empty()) return;
     p = idle.back();
     idle.pop_back();
-  } else if ((e = cudaMallocAsync(&p, kSplitCounters * sizeof(unsigned) + kScratchBytes, stream)) != cudaSuccess) {
-    return cuda_fail(e, "cudaMallocAsync(scratch)");
+  };
+  {
+    std::lock_guard<std::mutex> lk(g_scratch.mu);
+    take_idle();
+    if (!p) gone.swap(g_scratch.retired[dev]);
   }
-  e = cudaMemsetAsync(p, 0, kSplitCounters * sizeof(unsigned), stream);
+  if (!gone.empty()) {
+    const auto busy = std::partition(gone.begin(), gone.end(), [](const auto& s) { return cudaEventQuery(s->after) == cudaSuccess; });
+    for (auto it = gone.begin(); it != busy; ++it) cudaEventDestroy((*it)->after);
+    std::lock_guard<std::mutex> lk(g_scratch.mu);
+    for (auto it = gone.begin(); it != busy; ++it) g_scratch.idle[dev].push_back((*it)->base);
+    for (auto it = busy; it != gone.end(); ++it) g_scratch.retired[dev].push_back(std::move(*it));
+    take_idle();
+  }
+  if (!p && (e = cudaMallocAsync(&p, kSplitCounters * sizeof(unsigned) + kScratchBytes, side)) != cudaSuccess)
+    return cuda_fail(e, "cudaMallocAsync(scratch)");
+  e = cudaMemsetAsync(p, 0, kSplitCounters * sizeof(unsigned), side);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(side);
   if (e != cudaSuccess) {
-    cudaFreeAsync(p, stream);
+    cudaFreeAsync(p, side);
     return cuda_fail(e, "cudaMemsetAsync(counters)");
   }
+  std::lock_guard<std::mutex> lk(g_scratch.mu);
   *base = static_cast<unsigned*>(p);
   return B200Q_OK;
 }
@@ -1157,17 +1178,8 @@ int scratch_of_capture(int dev, cudaStream_t stream, std::shared_ptr<Scratch>* o
   }
   std::lock_guard<std::mutex> lk((*out)->mu);
   if ((*out)->base) return B200Q_OK;
-  // made on a stream of its own, which the capture has nothing to do with
   unsigned* base = nullptr;
-  {
-    const OutsideCapture outside;
-    cudaStream_t side = nullptr;
-    if ((e = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking)) != cudaSuccess) return cuda_fail(e, "cudaStreamCreate(scratch)");
-    int rc = new_scratch(dev, side, false, &base);
-    if (!rc && (e = cudaStreamSynchronize(side)) != cudaSuccess) rc = cuda_fail(e, "cudaStreamSynchronize(scratch)");
-    cudaStreamDestroy(side);
-    if (rc) return rc;
-  }
+  if (int rc = new_scratch(dev, &base)) return rc;
   auto owned = std::make_unique<GraphScratch>(GraphScratch{key, base});
   cudaUserObject_t object = nullptr;
   e = cudaUserObjectCreate(&object, owned.get(), GraphScratch::destroy, 1, cudaUserObjectNoDestructorSync);
@@ -1227,13 +1239,25 @@ int host_scratch(cudaStream_t stream, ScratchHold* hold) {
     }
     hold->lock = std::unique_lock<std::mutex>(s->mu);
     if (!s->base)
-      if (int rc = new_scratch(dev, stream, true, &s->base)) return rc;
+      if (int rc = new_scratch(dev, &s->base)) return rc;
     hold->bytes = s->base + kSplitCounters;
     hold->counters = s->base;
+    hold->stream = stream;
+    hold->after = captured ? nullptr : &s->after;
   } catch (const std::exception& error) {  // no memory for the host's tables
     return fail(B200Q_ERR_UNSUPPORTED, "scratch: %s", error.what());
   }
   return B200Q_OK;
+}
+
+void ScratchHold::launched() const {
+  if (!after || !g_scratch.streams_end.load(std::memory_order_relaxed)) return;
+  if (!*after && cudaEventCreateWithFlags(after, cudaEventDisableTiming) != cudaSuccess) {
+    *after = nullptr;
+    cudaGetLastError();
+    return;
+  }
+  if (cudaEventRecord(*after, stream) != cudaSuccess) cudaGetLastError();
 }
 
 void host_set_path(int path) { g_last_path = path; }

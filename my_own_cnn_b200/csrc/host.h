@@ -32,6 +32,9 @@ struct ScratchHold {
   std::unique_lock<std::mutex> lock;
   void* bytes = nullptr;
   unsigned* counters = nullptr;
+  cudaStream_t stream = nullptr;
+  cudaEvent_t* after = nullptr;
+  B200Q_HIDDEN void launched() const;  // the call's last kernel is in the stream
 };
 B200Q_HIDDEN int host_scratch(cudaStream_t stream, ScratchHold* hold);
 B200Q_HIDDEN void host_set_path(int path);

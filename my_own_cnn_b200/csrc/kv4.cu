@@ -264,7 +264,9 @@ int launch_attention(const Cache& c, AttnArgs a, int sms, int device, cudaStream
   a.counters = scratch.counters;
   a.partial = static_cast<float*>(scratch.bytes);
   a.partial_ml = a.partial + rows * D;
-  return host_launch("kv4_attention_kernel launch", kernel, dim3(blocks), kWarps * 32, Shape::kSmem, stream, 1, c, a);
+  rc = host_launch("kv4_attention_kernel launch", kernel, dim3(blocks), kWarps * 32, Shape::kSmem, stream, 1, c, a);
+  scratch.launched();
+  return rc;
 }
 
 int check_ftype(int ftype) {

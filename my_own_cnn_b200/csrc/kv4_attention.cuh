@@ -6,9 +6,9 @@
 // Both products take the codes as the 16-row operand A of m16n8k16 (tokens x channels, then channels x tokens)
 // and the rows as its 8 columns, so 8 rows cost one instruction per 256 codes.
 //   Keys' operands: a nibble put into the low bits of the fp16 1024 is 1024 + code, and one place higher 1024 + 16 code; less the
-//   same of the zero point it is exact and normal.  (The bare nibble, a subnormal, saves the subtraction, 69.0 against 71.3 us
-//   below, but the adder lines subnormals up by their exponent field and loses about 10 of the sum's bits: log-sums of
-//   short sequences off by 1.7e-6, 5e-8 so; 2 x 131072 fp16 outputs off by 6.6e-4, 2.7e-4 so.)
+//   same of the zero point it is exact and normal.  (The bare nibble, a subnormal, saves the subtraction, 3 % of the time, but
+//   the adder lines subnormals up by their exponent field and loses about 10 of the sum's bits: log-sums of short sequences
+//   off by 1.7e-6, 5e-8 so.)
 //   Keys: every second query value is divided by 16 for the codes one place higher.  Query rows are scaled by a power of
 //   two to a maximum in [2^14, 2^15), so that they fit fp16 whatever their type; fp32 rows are split into two fp16 terms (22 bits).
 //   Values: 128 + code less 128 + zero point in bf16, exact. P is fp32's value in bf16 terms, each of which has fp32's range:

@@ -608,6 +608,7 @@ extern "C" int b200q_qk_norm_rope_bprop(const b200q_qk_norm_args* args, void* st
     rc = host_launch("norm_weight_grad_kernel launch", norm_weight_grad_kernel<T>, dim3((2 * d + 31) / 32), 1024, 0, cs, 1,
                      a.partial, blocks, d, static_cast<T*>(args->q_w_grad), static_cast<T*>(args->k_w_grad));
   });
+  scratch.launched();
   if (rc == B200Q_OK) host_set_path(18);
   return rc;
 }

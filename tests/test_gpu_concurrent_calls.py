@@ -203,3 +203,70 @@ def test_eager_calls_while_another_thread_captures(mode):
     g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip([out] + outs, want)) and len(outs) == 2
+
+
+def test_streams_that_come_and_go_while_another_thread_captures():
+    """Finding scratch that destroyed streams left waits for nothing that a capture forbids."""
+    import ctypes
+
+    cudart = ctypes.CDLL("libcudart.so.12")
+    calls = [into(attention(i, n=8000)) for i in range(2)]
+    want = [call().clone() for call in calls]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    calls[0](stream=s)
+    torch.cuda.synchronize()
+    outs = []
+
+    def churn():
+        for _ in range(30):
+            x = ctypes.c_void_p()
+            assert cudart.cudaStreamCreateWithFlags(ctypes.byref(x), 1) == 0
+            outs.append(calls[1](stream=x.value))
+            assert cudart.cudaStreamDestroy(x) == 0
+
+    for _ in range(3):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            t = threading.Thread(target=churn)
+            t.start()
+            out = calls[0](stream=s)
+            t.join()
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(outs[-1], want[1])
+        g.reset()
+    assert len(outs) == 90
+
+
+def test_graphs_that_come_and_go_beside_new_streams():
+    """What graphs give back, on a thread of the driver's, is taken by the first calls of new streams meanwhile."""
+    calls = [into(attention(i, n=8000)) for i in range(2)]
+    want = [call().clone() for call in calls]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    calls[0](stream=s)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def eager():
+        for i in range(40):
+            x = torch.cuda.Stream()
+            out = calls[1](stream=x)
+            x.synchronize()
+            if not torch.equal(out, want[1]):
+                wrong.append(i)
+
+    t = threading.Thread(target=eager)
+    t.start()
+    for _ in range(40):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s, capture_error_mode="relaxed"):
+            out = calls[0](stream=s)
+        g.replay()
+        torch.cuda.current_stream().synchronize()
+        assert torch.equal(out, want[0])
+        del g
+    t.join()
+    assert wrong == []
