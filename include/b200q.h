@@ -284,6 +284,76 @@ typedef struct b200q_kv4_attention_args {
 } b200q_kv4_attention_args;
 int b200q_kv4_attention(const b200q_kv4_cache* c, const b200q_kv4_attention_args* args, void* stream);
 
+/* 8-bit rows: codes int8 [t][n] with row stride ldc and one fp32 scale a row; value = code * scale.
+ * b200q_quantize_s8 rounds rows u = x; b200q_rms_norm_s8 rows
+ *   u = h * w (w [n] or NULL for all ones), h = x + residual (residual NULL: x), both sums and products rounded
+ *   once, h to the rows' own type: it is written to `sum`, which may be x or the residual.
+ * code = rint(u * fl(127 * fl(1 / max|u|))), the product exact, ties to even; scale = max|u| / 127, for the norm times
+ * (mean(h^2) + eps)^-1/2.  A row with a NaN or an infinity among u has the scale NaN (its values read as NaN) and codes 0; one
+ * with nothing above 2^-119 has scale and codes 0.  b200q_quantize_s8 reads x, codes, scales and sizes alone (the other pointers NULL). */
+typedef struct b200q_rows_s8_args {
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  const void* residual;
+  int64_t ldr;
+  void* sum;
+  int64_t lds;
+  int8_t* codes;
+  int64_t ldc;
+  float* scales;
+  int ftype, t, n;
+  float eps;
+} b200q_rows_s8_args;
+int b200q_quantize_s8(const b200q_rows_s8_args* args, void* stream);
+int b200q_rms_norm_s8(const b200q_rows_s8_args* args, void* stream);
+
+/* y[t][n] (row stride ldy, of ftype) = codes * scales, rounded once. */
+int b200q_read_s8(const int8_t* codes, long long ldc, const float* scales, void* y, long long ldy, int ftype, int t,
+                  int n, void* stream);
+
+/* y[m][n] = (sum_k x[m][k] * w[n][k]) * x_scale[m] * w_scale[n] (+ bias[n]) for 8-bit rows x [m][k] and w [n][k]: the sum exact in
+ * 32-bit integers (k <= 131071), the rest in fp32, y of ftype with row stride ldy; bias [n] of ftype or NULL.  Codes lie on
+ * 16-byte boundaries with row strides that are multiples of 16; what lies past k is not used.  A row or a channel with
+ * the scale NaN gives NaN.  y shares no memory with the other tensors. */
+typedef struct b200q_linear_s8_args {
+  const int8_t* x;
+  int64_t ldx;
+  const float* x_scales;
+  const int8_t* w;
+  int64_t ldw;
+  const float* w_scales;
+  const void* bias;
+  void* y;
+  int64_t ldy;
+  int ftype, m, n, k;
+} b200q_linear_s8_args;
+int b200q_linear_s8(const b200q_linear_s8_args* args, void* stream);
+
+/* Causal attention over packed prompts.  Sequence i has the query rows starts[i] .. starts[i + 1] of q [tq][hq][d] and the key rows
+ * k_starts[i] .. k_starts[i + 1] of k, v [tk][hk][d] (k_starts NULL: starts; all with token and head strides, channels
+ * contiguous); starts int32 [b + 1] on the device.  The last query is in line with the last key: row j of lq
+ * sees the first lk - lq + j + 1 keys; where that is none the output is 0 (lse -inf).  Query head h reads head
+ * h / (hq / hk).  out contiguous [tq][hq][d]; lse fp32 [tq][hq] or NULL: log of the sum of exp(scale * q.k).
+ * Rows outside every sequence are left as they are.  A sequence whose starts decrease or pass the rows is left out and
+ * reported by b200q_device_error().  What a row does not see has no part in it, NaN and infinities among it.
+ * d up to 256. */
+typedef struct b200q_prompt_attention_args {
+  const void* q;
+  int64_t q_ts, q_hs;
+  const void* k;
+  int64_t k_ts, k_hs;
+  const void* v;
+  int64_t v_ts, v_hs;
+  const int32_t* starts;
+  const int32_t* k_starts;
+  void* out;
+  float* lse;
+  int ftype, b, tq, tk, hq, hk, d;
+  float scale;
+} b200q_prompt_attention_args;
+int b200q_prompt_attention(const b200q_prompt_attention_args* args, void* stream);
+
 /* Packed low-channel int8 conv that allocates nothing (no counterpart in the reference).
  * For callers that may not allocate device memory at all: for example plugins inside a runtime
  * that owns and budgets every byte of GPU memory itself, or latency-critical loops where a
@@ -342,7 +412,9 @@ int b200q_device_error(void);
  * pixel-grouped 1x1 GEMM (G pixels per row against block-diagonal weights built in the stream's
  * workspace, for layers with G * K <= 256 and G * C <= 256), 16 tcgen05 int32 bmm (operands copied
  * to int8, CUDA-core recompute only when a value does not fit), 17 4-bit weights linear, 18 per-head norm
- * and rotation (either direction), 19 4-bit cache append / read, 20 4-bit cache attention. */
+ * and rotation (either direction), 19 4-bit cache append / read, 20 4-bit cache attention, 21 8-bit rows (quantized, normed or
+ * read), 22 linear of 8-bit rows, 23 prompt attention on tcgen05, 24 prompt attention on mma.sync (fp32; rows and heads that TMA
+ * cannot take). */
 int b200q_last_path(void);
 
 /* 0 = automatic dispatch (default); 1 = force the CUDA-core kernels (cross-checks). */

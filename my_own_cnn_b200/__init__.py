@@ -20,6 +20,8 @@ from .f32 import (BlockBiasMode, bmm_bprop, bmm_bprop_dA, bmm_bprop_dB, bmm_fpro
 from .w4 import W4Weight, linear_w4, pack_w4, quantize_w4
 from .rope import qk_norm_rope, qk_norm_rope_bprop, rope_table
 from .kv4 import KV4Cache, kv4_append, kv4_attention, kv4_read
+from .s8 import S8Rows, linear_s8, quantize_s8, rms_norm_s8
+from .prompt import prompt_attention
 from .decoder import W4Attention
 from ._lib import B200QError, device_error, last_path, set_path_policy, tc_launch_count
 
@@ -33,4 +35,5 @@ __all__ = [
     "launch_block_bprop_nhwc", "launch_block_grad_nhwc", "bmm_matmul", "bmm_fprop", "bmm_bprop_dA", "bmm_bprop_dB",
     "bmm_bprop", "W4Weight", "linear_w4", "pack_w4", "quantize_w4", "qk_norm_rope", "qk_norm_rope_bprop", "rope_table",
     "KV4Cache", "kv4_append", "kv4_attention", "kv4_read", "W4Attention", "device_error",
+    "S8Rows", "quantize_s8", "rms_norm_s8", "linear_s8", "prompt_attention",
 ]

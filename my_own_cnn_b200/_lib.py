@@ -44,6 +44,10 @@ PATH_NAMES = {
     18: "qk-norm-rope",
     19: "kv4-cache",
     20: "kv4-attention",
+    21: "rows-s8",
+    22: "linear-s8",
+    23: "tcgen05-prompt-attention",
+    24: "mma-prompt-attention",
 }
 
 
@@ -81,6 +85,26 @@ class CKV4AttentionArgs(Structure):
     _fields_ = [("q", c_void_p), ("q_bs", c_int64), ("q_ts", c_int64), ("q_hs", c_int64), ("block_table", c_void_p),
                 ("bt_stride", c_int64), ("lens", c_void_p), ("out", c_void_p), ("lse", c_void_p), ("ftype", c_int),
                 ("b", c_int), ("tq", c_int), ("hq", c_int), ("max_pages", c_int), ("scale", c_float)]
+
+
+class CRowsS8Args(Structure):
+    _fields_ = [("x", c_void_p), ("ldx", c_int64), ("w", c_void_p), ("residual", c_void_p), ("ldr", c_int64),
+                ("sum", c_void_p), ("lds", c_int64), ("codes", c_void_p), ("ldc", c_int64), ("scales", c_void_p),
+                ("ftype", c_int), ("t", c_int), ("n", c_int), ("eps", c_float)]
+
+
+class CLinearS8Args(Structure):
+    _fields_ = [("x", c_void_p), ("ldx", c_int64), ("x_scales", c_void_p), ("w", c_void_p), ("ldw", c_int64),
+                ("w_scales", c_void_p), ("bias", c_void_p), ("y", c_void_p), ("ldy", c_int64), ("ftype", c_int),
+                ("m", c_int), ("n", c_int), ("k", c_int)]
+
+
+class CPromptAttentionArgs(Structure):
+    _fields_ = [("q", c_void_p), ("q_ts", c_int64), ("q_hs", c_int64), ("k", c_void_p), ("k_ts", c_int64),
+                ("k_hs", c_int64), ("v", c_void_p), ("v_ts", c_int64), ("v_hs", c_int64), ("starts", c_void_p),
+                ("k_starts", c_void_p), ("out", c_void_p), ("lse", c_void_p)]
+    _fields_ += [(f, c_int) for f in ("ftype", "b", "tq", "tk", "hq", "hk", "d")]
+    _fields_ += [("scale", c_float)]
 
 
 def packer(layout) -> "struct.Struct":
@@ -140,6 +164,11 @@ def lib() -> ctypes.CDLL:
         "b200q_kv4_append": [packed, vp, ll, ll, vp, ll, ll, vp, i, i, vp],
         "b200q_kv4_read": [packed, vp, vp, vp, i, i, vp],
         "b200q_kv4_attention": [packed, packed, vp],
+        "b200q_quantize_s8": [packed, vp],
+        "b200q_rms_norm_s8": [packed, vp],
+        "b200q_read_s8": [vp, ll, vp, vp, ll, i, i, i, vp],
+        "b200q_linear_s8": [packed, vp],
+        "b200q_prompt_attention": [packed, vp],
     }
     for name, args in sig.items():
         fn = getattr(L, name)
@@ -190,5 +219,6 @@ EXPORTED_SYMBOLS = [
     "b200q_conv_fprop_f32", "b200q_conv_bprop_f32", "b200q_conv_grad_f32", "b200q_bmm_f32",
     "b200q_conv2d_s8_add", "b200q_maxpool_s8", "b200q_global_avgpool_s8", "b200q_conv2d_s8_plan",
     "b200q_linear_w4", "b200q_qk_norm_rope", "b200q_qk_norm_rope_bprop", "b200q_kv4_append", "b200q_kv4_read",
-    "b200q_kv4_attention",
+    "b200q_kv4_attention", "b200q_quantize_s8", "b200q_rms_norm_s8", "b200q_read_s8", "b200q_linear_s8",
+    "b200q_prompt_attention",
 ]

@@ -1261,6 +1261,24 @@ void ScratchHold::launched() const {
 }
 
 void host_set_path(int path) { g_last_path = path; }
+long long host_wait_limit() { return wait_limit(); }
+
+int host_tensor_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, std::array<uint64_t, 3> size, uint64_t stride1,
+                    uint64_t stride2, std::array<uint32_t, 3> box) {
+  const cuuint64_t dims[3] = {size[0], size[1], size[2]};
+  const cuuint64_t strides[2] = {stride1, stride2};
+  const cuuint32_t boxes[3] = {box[0], box[1], box[2]};
+  const cuuint32_t steps[3] = {1, 1, 1};
+  const CUresult r = g_encode_tiled(map, type, 3, const_cast<void*>(base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(B200Q_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): sizes %llu, %llu, %llu, strides %llu, %llu", static_cast<int>(r),
+                static_cast<unsigned long long>(size[0]), static_cast<unsigned long long>(size[1]),
+                static_cast<unsigned long long>(size[2]), static_cast<unsigned long long>(stride1),
+                static_cast<unsigned long long>(stride2));
+  return B200Q_OK;
+}
 
 }  // namespace b200q
 
@@ -2097,6 +2115,7 @@ int b200q_device_error(void) {
       case kDevErrBadPosition: return fail(B200Q_ERR_INVALID_ARG, "a position lies outside the rotation table");
       case kDevErrBadSlot: return fail(B200Q_ERR_INVALID_ARG, "a slot lies outside the cache");
       case kDevErrBadPage: return fail(B200Q_ERR_INVALID_ARG, "a block table names a page outside the cache");
+      case kDevErrBadStarts: return fail(B200Q_ERR_INVALID_ARG, "a sequence's starts decrease or pass the rows");
       case kDevErrBadLength: return fail(B200Q_ERR_INVALID_ARG, "a length exceeds its block table");
       default: return fail(B200Q_ERR_TIMEOUT, "device wait ran out (code 0x%x)", v);
     }

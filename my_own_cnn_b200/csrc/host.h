@@ -1,8 +1,10 @@
 // Host services of the library shared by its translation units (defined in b200q.cu): error
 // messages, per-device state, stream workspaces.  Internal: hidden from the library's users.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <array>
 #include <cstddef>
 #include <cstdint>
 #include <mutex>
@@ -38,6 +40,11 @@ struct ScratchHold {
 };
 B200Q_HIDDEN int host_scratch(cudaStream_t stream, ScratchHold* hold);
 B200Q_HIDDEN void host_set_path(int path);
+// Bound of a wait on an mbarrier, in SM clocks.
+B200Q_HIDDEN long long host_wait_limit();
+// A rank-3 tensor map with the 128-byte swizzle and zeros outside: sizes and box in elements, strides of the outer two in bytes.
+B200Q_HIDDEN int host_tensor_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, std::array<uint64_t, 3> size,
+                                 uint64_t stride1, uint64_t stride2, std::array<uint32_t, 3> box);
 
 // Launches a kernel that begins with wait_for_previous(): its blocks may take their places while the stream's previous kernel
 // drains, and wait there until that one has ended and its writes can be seen.  `cluster` blocks make a cluster.
@@ -65,5 +72,6 @@ constexpr int kDevErrBadPosition = 0x201;
 constexpr int kDevErrBadSlot = 0x202;
 constexpr int kDevErrBadPage = 0x203;
 constexpr int kDevErrBadLength = 0x204;
+constexpr int kDevErrBadStarts = 0x205;
 
 }  // namespace b200q

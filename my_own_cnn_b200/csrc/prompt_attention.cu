@@ -1,0 +1,354 @@
+// Causal attention over packed prompts (b200q_prompt_attention).
+//
+//   o_i = sum_j p_ij v_j / l_i,  p_ij = exp(s_ij - m_i),  s_ij = scale q_i k_j,  m_i = max_j s_ij,  l_i = sum_j p_ij,  j <= i + lk - lq
+//
+// prompt_mma_kernel: mma.sync.m16n8k16, for fp32 and for rows that TMA cannot take.  A block has 64 rows (token, query
+// head of one key head) in four warps and goes through the keys 64 at a time; scores, weights and sums stay in registers, the
+// maximum and the sum of a row run along.  fp32 operands are three bf16 terms, cut off one after another: 8 + 8 + 8
+// bits, so the terms are the value; six products (0 0, 0 1, 1 0, 1 1, 0 2, 2 0) leave 2^-24 of it out.  The first is added with
+// rounding.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+#include "prompt.cuh"
+
+namespace b200q {
+namespace {
+
+constexpr int kRows = 64;
+constexpr int kMmaThreads = 128;
+
+// Operand words: two 16-bit values in every term.
+template <typename T>
+struct Terms {
+  static constexpr int kCount = 1;
+  static __device__ __forceinline__ void cut(float a, float b, uint32_t (&w)[1]) {
+    if constexpr (sizeof(T) == 2) w[0] = std::is_same<T, __half>::value ? pack_f16(a, b) : pack_bf16(a, b);
+  }
+};
+template <>
+struct Terms<float> {
+  static constexpr int kCount = 3;
+  static __device__ __forceinline__ void cut(float a, float b, uint32_t (&w)[3]) {
+    float x[2] = {a, b};
+    uint32_t t[3][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      t[0][i] = __float_as_uint(x[i]) & 0xFFFF0000u;
+      const float r = fabsf(x[i]) < INFINITY ? x[i] - __uint_as_float(t[0][i]) : 0.0f;
+      t[1][i] = __float_as_uint(r) & 0xFFFF0000u;
+      t[2][i] = __float_as_uint(r - __uint_as_float(t[1][i]));
+      // a NaN may have its bits among those cut off
+      if (x[i] != x[i]) t[0][i] = 0x7FC00000u;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) w[i] = __byte_perm(t[i][0], t[i][1], 0x7632);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    mma_f16(c, a[0], a[1], a[2], a[3], b0, b1);
+  else
+    mma_bf16(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+// c += a b on bf16 with the addition rounded: the instruction's own adder truncates, which in 24 additions of a row of
+// scores adds up to 2e-6 of fp32 outputs (4e-7 so).
+__device__ __forceinline__ void add_product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  float r[4];
+  mma_bf16_first(r, a[0], a[1], a[2], a[3], b0, b1);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c[e] += r[e];
+}
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void load_matrices_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+template <typename T, int D>
+struct MmaShape {
+  static constexpr int kTerms = Terms<T>::kCount;
+  static constexpr int kKeys = kTerms == 3 && D == 256 ? 32 : 64;
+  static constexpr int kPitch = D * 2 + 16;  // bytes: eight rows of a matrix in eight bank groups
+  static constexpr int kQ = kRows * kPitch, kK = kKeys * kPitch;  // one term
+  static constexpr int kSmem = kTerms * (kQ + 2 * kK);
+};
+
+// `rows` rows of D channels (zeros past d and where there is no row) into the terms' tiles.
+template <typename T, int D, typename P>
+__device__ __forceinline__ void load_tile(uint32_t to, int term, int rows, int d, bool wide, P row_at) {
+  constexpr int kTerms = Terms<T>::kCount, kPitch = MmaShape<T, D>::kPitch;
+  for (int i = threadIdx.x; i < rows * (D / 4); i += kMmaThreads) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    const T* p = row_at(r);
+    float x[4] = {};
+    if (p) {
+      if (wide && c + 4 <= d) {
+        if constexpr (sizeof(T) == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p + c);
+          x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(p + c);
+          const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = to_f32(e[j]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c + j < d) x[j] = to_f32(p[c + j]);
+      }
+    }
+    uint32_t lo[kTerms], hi[kTerms];
+    Terms<T>::cut(x[0], x[1], lo);
+    Terms<T>::cut(x[2], x[3], hi);
+#pragma unroll
+    for (int t = 0; t < kTerms; ++t)
+      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + t * term + r * kPitch + c * 2), "r"(lo[t]), "r"(hi[t]) : "memory");
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(PromptArgs a, int wide) {
+  using S = MmaShape<T, D>;
+  constexpr int kTerms = S::kTerms, kKeys = S::kKeys;
+  // The products of the terms but for the first ones'.
+  constexpr int kA[5] = {2, 0, 1, 1, 0}, kB[5] = {0, 2, 1, 0, 1};
+  extern __shared__ __align__(16) uint8_t smem[];
+  wait_for_previous();
+  const int kv = static_cast<int>(blockIdx.x % a.hk), lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const PromptUnit u = prompt_unit(a, static_cast<int>(blockIdx.x / a.hk), blockIdx.x == 0 && threadIdx.x < 32);
+  if (!u.ok) return;
+  const int ratio = static_cast<int>(a.ratio.d), shift = u.s.lk - u.s.lq;
+  const int rows = u.s.lq * ratio, row0 = u.tile * kRows;  // of this key head's rows in the sequence
+  const uint32_t s_q = shared_address(smem), s_k = s_q + kTerms * S::kQ, s_v = s_k + kTerms * S::kK;
+  load_tile<T, D>(s_q, S::kQ, kRows, a.d, wide, [&](int r) -> const T* {
+    if (row0 + r >= rows) return nullptr;
+    const int token = static_cast<int>(a.ratio.of(row0 + r)), head = kv * ratio + row0 + r - token * ratio;
+    return static_cast<const T*>(a.q) + (u.s.q0 + token) * a.q_ts + head * a.q_hs;
+  });
+  // keys that a row of this lane sees: rows g and g + 8 of the warp's 16
+  const int g = lane / 4, t = lane % 4, last_row = min(rows, row0 + kRows) - 1;
+  int seen[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = row0 + warp * 16 + g + 8 * h;
+    seen[h] = r < rows ? max(0, static_cast<int>(a.ratio.of(r)) + shift + 1) : 0;
+  }
+  const int most = min(u.s.lk, static_cast<int>(a.ratio.of(last_row)) + shift + 1);
+  const float c = a.scale * kLog2e;
+  float o[D / 8][4] = {}, top[2] = {-INFINITY, -INFINITY}, sum[2] = {};
+  for (int j0 = 0; j0 < most; j0 += kKeys) {
+    __syncthreads();
+    load_tile<T, D>(s_k, S::kK, kKeys, a.d, wide, [&](int r) -> const T* {
+      return j0 + r < u.s.lk ? static_cast<const T*>(a.k) + (u.s.k0 + j0 + r) * a.k_ts + kv * a.k_hs : nullptr;
+    });
+    load_tile<T, D>(s_v, S::kK, kKeys, a.d, wide, [&](int r) -> const T* {
+      return j0 + r < u.s.lk ? static_cast<const T*>(a.v) + (u.s.k0 + j0 + r) * a.v_ts + kv * a.v_hs : nullptr;
+    });
+    __syncthreads();
+    float s[kKeys / 8][4] = {}, less[kTerms == 3 ? kKeys / 8 : 1][4] = {};
+#pragma unroll 2
+    for (int kc = 0; kc < D; kc += 16) {
+      uint32_t q[kTerms][4];
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i)
+        load_matrices(q[i], s_q + i * S::kQ + (warp * 16 + lane % 16) * S::kPitch + (kc + lane / 16 * 8) * 2);
+#pragma unroll
+      for (int n = 0; n < kKeys / 16; ++n) {
+        uint32_t k[kTerms][4];
+#pragma unroll
+        for (int i = 0; i < kTerms; ++i)
+          load_matrices(k[i], s_k + i * S::kK + (n * 16 + lane % 8 + lane / 16 * 8) * S::kPitch + (kc + lane / 8 % 2 * 8) * 2);
+        if constexpr (kTerms == 1) {
+          mma_16<T>(s[2 * n], q[0], k[0][0], k[0][1]);
+          mma_16<T>(s[2 * n + 1], q[0], k[0][2], k[0][3]);
+        } else {
+#pragma unroll
+          for (int p = 0; p < 5; ++p) {
+            mma_16<T>(less[2 * n], q[kA[p]], k[kB[p]][0], k[kB[p]][1]);
+            mma_16<T>(less[2 * n + 1], q[kA[p]], k[kB[p]][2], k[kB[p]][3]);
+          }
+          add_product(s[2 * n], q[0], k[0][0], k[0][1]);
+          add_product(s[2 * n + 1], q[0], k[0][2], k[0][3]);
+        }
+      }
+    }
+    if constexpr (kTerms == 3) {
+#pragma unroll
+      for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] += less[n][e];
+    }
+    // softmax: the exponent's base is 2, the scale is in it
+    float now[2] = {top[0], top[1]}, from[2];
+#pragma unroll
+    for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[n][e] = j0 + n * 8 + 2 * t + (e & 1) < seen[e / 2] ? s[n][e] * c : -INFINITY;
+        now[e / 2] = max_nan(now[e / 2], s[n][e]);
+      }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      now[h] = max_nan(now[h], __shfl_xor_sync(~0u, now[h], 1));
+      now[h] = max_nan(now[h], __shfl_xor_sync(~0u, now[h], 2));
+      from[h] = now[h] == -INFINITY ? 0.0f : now[h];
+      const float keep = exp2_approx(top[h] - from[h]);
+      top[h] = now[h];
+      sum[h] *= keep;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) o[n][2 * h] *= keep, o[n][2 * h + 1] *= keep;
+    }
+#pragma unroll
+    for (int n = 0; n < kKeys / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[n][e] = exp2_approx(s[n][e] - from[e / 2]);
+        sum[e / 2] += s[n][e];
+      }
+    uint32_t p[kKeys / 16][kTerms][4];
+#pragma unroll
+    for (int kc = 0; kc < kKeys / 16; ++kc)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t w[kTerms];
+        Terms<T>::cut(s[2 * kc + e / 2][e % 2 * 2], s[2 * kc + e / 2][e % 2 * 2 + 1], w);
+#pragma unroll
+        for (int i = 0; i < kTerms; ++i) p[kc][i][e] = w[i];
+      }
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) {
+      float small[2][4] = {};
+#pragma unroll
+      for (int kc = 0; kc < kKeys / 16; ++kc) {
+        uint32_t v[kTerms][4];
+#pragma unroll
+        for (int i = 0; i < kTerms; ++i)
+          load_matrices_t(v[i], s_v + i * S::kK + (kc * 16 + lane % 16) * S::kPitch + (n * 16 + lane / 16 * 8) * 2);
+        if constexpr (kTerms == 1) {
+          mma_16<T>(o[2 * n], p[kc][0], v[0][0], v[0][1]);
+          mma_16<T>(o[2 * n + 1], p[kc][0], v[0][2], v[0][3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 5; ++i) {
+            mma_16<T>(small[0], p[kc][kA[i]], v[kB[i]][0], v[kB[i]][1]);
+            mma_16<T>(small[1], p[kc][kA[i]], v[kB[i]][2], v[kB[i]][3]);
+          }
+          add_product(o[2 * n], p[kc][0], v[0][0], v[0][1]);
+          add_product(o[2 * n + 1], p[kc][0], v[0][2], v[0][3]);
+        }
+      }
+      if constexpr (kTerms == 3) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[2 * n][e] += small[0][e], o[2 * n + 1][e] += small[1][e];
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = row0 + warp * 16 + g + 8 * h;
+    float l = sum[h];
+    l += __shfl_xor_sync(~0u, l, 1);
+    l += __shfl_xor_sync(~0u, l, 2);
+    const int token = static_cast<int>(a.ratio.of(min(r, rows - 1))), head = kv * ratio + min(r, rows - 1) - token * ratio;
+    const long long at = static_cast<long long>(u.s.q0 + token) * a.hq + head;
+    const float by = l > 0.0f ? 1.0f / l : 0.0f;
+    bool fine = l > 0.0f && l < INFINITY;
+    if (r < rows) {
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float y = o[n][2 * h + e] * by;
+          fine = fine && fabsf(y) < INFINITY;
+          if (n * 8 + 2 * t + e < a.d) static_cast<T*>(a.out)[at * a.d + n * 8 + 2 * t + e] = from_f32<T>(seen[h] ? y : 0.0f);
+        }
+      if (a.lse && t == 0) a.lse[at] = seen[h] ? (top[h] + log2f(l)) * (1.0f / kLog2e) : -INFINITY;
+    }
+    unsigned again = __ballot_sync(~0u, r < rows && seen[h] && !fine);
+    again |= again >> 1;
+    again = (again | again >> 2) & 0x11111111u;  // one bit a row
+    __syncwarp();
+    for (; again; again &= again - 1) {
+      const int from = __ffs(again) - 1;
+      prompt_row_with_care<T>(a, u.s.q0 + __shfl_sync(~0u, token, from), __shfl_sync(~0u, head, from), u.s.k0,
+                              min(u.s.lk, __shfl_sync(~0u, seen[h], from)));
+    }
+  }
+}
+
+template <typename T, int D>
+int launch_mma(const PromptArgs& a, bool wide, long long units, int device, cudaStream_t cs) {
+  static std::atomic<bool> ready[kMaxDevices];
+  if (!ready[device].load(std::memory_order_relaxed)) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(prompt_mma_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, MmaShape<T, D>::kSmem);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute(prompt_mma_kernel)");
+    ready[device].store(true, std::memory_order_relaxed);
+  }
+  return host_launch("prompt_mma_kernel launch", prompt_mma_kernel<T, D>, dim3(static_cast<unsigned>(units)), kMmaThreads,
+                     MmaShape<T, D>::kSmem, cs, 1, a, wide ? 1 : 0);
+}
+
+}  // namespace
+}  // namespace b200q
+
+using namespace b200q;
+
+extern "C" int b200q_prompt_attention(const b200q_prompt_attention_args* p, void* stream) {
+  if (!p) return host_fail(B200Q_ERR_INVALID_ARG, "null argument");
+  if (p->ftype < B200Q_F32 || p->ftype > B200Q_BF16) return host_fail(B200Q_ERR_INVALID_ARG, "bad floating type %d", p->ftype);
+  if (p->b < 0 || p->tq < 0 || p->tk < 0 || p->hq < 0 || p->hk < 0) return host_fail(B200Q_ERR_INVALID_ARG, "negative dimensions");
+  if (p->d < 1 || p->d > 256) return host_fail(B200Q_ERR_UNSUPPORTED, "heads of 1 to 256 channels, got %d", p->d);
+  if (!std::isfinite(p->scale)) return host_fail(B200Q_ERR_INVALID_ARG, "the scale must be finite");
+  if (p->b == 0 || p->tq == 0 || p->hq == 0) return B200Q_OK;
+  if (p->hk == 0 || p->hq % p->hk)
+    return host_fail(B200Q_ERR_INVALID_ARG, "%d key heads do not divide %d query heads", p->hk, p->hq);
+  if (!p->q || !p->out || !p->starts || (p->tk && (!p->k || !p->v))) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
+  if (!p->k_starts && p->tk != p->tq)
+    return host_fail(B200Q_ERR_INVALID_ARG, "%d query and %d key rows without starts of the keys", p->tq, p->tk);
+  const long long ratio = p->hq / p->hk;
+  if (p->tq * ratio > 0x3fffffffll || p->tk > 0x3fffffff || p->b > 0x3fffffff)
+    return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
+  int sms = 0, device = 0;
+  PromptArgs a{};
+  if (int rc = host_device(&sms, &a.err, &device)) return rc;
+  a.q = p->q, a.q_ts = p->q_ts, a.q_hs = p->q_hs;
+  a.k = p->k, a.k_ts = p->k_ts, a.k_hs = p->k_hs;
+  a.v = p->v, a.v_ts = p->v_ts, a.v_hs = p->v_hs;
+  a.starts = p->starts;
+  a.k_starts = p->k_starts ? p->k_starts : p->starts;
+  a.out = p->out;
+  a.lse = p->lse;
+  a.b = p->b, a.tq = p->tq, a.tk = p->tk, a.hq = p->hq, a.hk = p->hk, a.d = p->d;
+  a.ratio = Divisor(static_cast<uint32_t>(ratio));
+  a.scale = p->scale;
+  a.limit = host_wait_limit();
+  const cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const int size = p->ftype == B200Q_F32 ? 4 : 2;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v);
+  const long long strides = p->q_ts | p->q_hs | p->k_ts | p->k_hs | p->v_ts | p->v_hs;
+  const bool wide = !(bits & (4 * size - 1)) && strides % 4 == 0;
+  a.tile_rows = kRows;
+  // as many tiles as there may be: every sequence's last one may be short
+  const long long tiles = p->tq * ratio / kRows + std::min<long long>(p->b, p->tq);
+  const long long units = tiles * p->hk;
+  if (units > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
+  int rc = B200Q_OK;
+  B200Q_DISPATCH_FTYPE(p->ftype, rc = a.d <= 64    ? launch_mma<T, 64>(a, wide, units, device, cs)
+                                      : a.d <= 128 ? launch_mma<T, 128>(a, wide, units, device, cs)
+                                                   : launch_mma<T, 256>(a, wide, units, device, cs));
+  if (rc == B200Q_OK) host_set_path(24);
+  return rc;
+}
