@@ -12,6 +12,7 @@
 #include <cmath>
 
 #include "prompt.cuh"
+#include "prompt_tc.cuh"
 
 namespace b200q {
 namespace {
@@ -119,7 +120,7 @@ __device__ __forceinline__ void load_tile(uint32_t to, int term, int rows, int d
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(PromptArgs a, int wide) {
+__global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_constant__ PromptArgs a, int wide) {
   using S = MmaShape<T, D>;
   constexpr int kTerms = S::kTerms, kKeys = S::kKeys;
   // The products of the terms but for the first ones'.
@@ -301,6 +302,43 @@ int launch_mma(const PromptArgs& a, bool wide, long long units, int device, cuda
                      MmaShape<T, D>::kSmem, cs, 1, a, wide ? 1 : 0);
 }
 
+// 16-bit heads of up to 128 channels whose addresses and strides a tensor map takes.  A scale of zero would multiply the
+// masked scores' infinities.
+bool tensor_core_takes(const b200q_prompt_attention_args& p, long long ratio) {
+  if (p.ftype == B200Q_F32 || p.d > 128 || p.d % 8 || ratio > 128 || p.scale == 0.0f || p.tk == 0) return false;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
+                         reinterpret_cast<uintptr_t>(p.out);
+  if (bits & 15u) return false;
+  const auto fits = [](int64_t stride, int count) { return count == 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); };
+  return fits(p.q_ts, p.tq) && fits(p.q_hs, p.hq) && fits(p.k_ts, p.tk) && fits(p.k_hs, p.hk) && fits(p.v_ts, p.tk) && fits(p.v_hs, p.hk);
+}
+
+template <typename T, int D>
+int launch_tc(const PromptArgs& a, long long units, int device, cudaStream_t cs) {
+  static std::atomic<bool> ready[kMaxDevices];
+  if (!ready[device].load(std::memory_order_relaxed)) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(prompt_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<D>::kSmem);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute(prompt_tc_kernel)");
+    ready[device].store(true, std::memory_order_relaxed);
+  }
+  const auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const auto map = [&](CUtensorMap* m, const void* base, int heads, int rows, long long ts, long long hs, uint32_t box_heads,
+                       uint32_t box_rows) {
+    const uint64_t one = static_cast<uint64_t>(a.d) * 2;  // a dimension of one row or head: any stride
+    return host_tensor_map(m, type, base, {static_cast<uint64_t>(a.d), static_cast<uint64_t>(heads), static_cast<uint64_t>(rows)},
+                           heads == 1 ? one : 2 * static_cast<uint64_t>(hs), rows == 1 ? one : 2 * static_cast<uint64_t>(ts),
+                           {64, box_heads, box_rows});
+  };
+  CUtensorMap tm_q, tm_k, tm_v;
+  int rc = map(&tm_q, a.q, a.hq, a.tq, a.q_ts, a.q_hs, a.ratio.d, static_cast<uint32_t>(a.tile_tokens / 2));
+  if (rc == B200Q_OK) rc = map(&tm_k, a.k, a.hk, a.tk, a.k_ts, a.k_hs, 1, kTcKeys);
+  if (rc == B200Q_OK) rc = map(&tm_v, a.v, a.hk, a.tk, a.v_ts, a.v_hs, 1, kTcKeys);
+  if (rc) return rc;
+  return host_launch("prompt_tc_kernel launch", prompt_tc_kernel<T, D>, dim3(static_cast<unsigned>(units)), kTcPromptThreads,
+                     TcShape<D>::kSmem, cs, 1, tm_q, tm_k, tm_v, a, a.scale < 0.0f ? 1u : 0u);
+}
+
 }  // namespace
 }  // namespace b200q
 
@@ -338,17 +376,26 @@ extern "C" int b200q_prompt_attention(const b200q_prompt_attention_args* p, void
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const int size = p->ftype == B200Q_F32 ? 4 : 2;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v);
-  const long long strides = p->q_ts | p->q_hs | p->k_ts | p->k_hs | p->v_ts | p->v_hs;
-  const bool wide = !(bits & (4 * size - 1)) && strides % 4 == 0;
+  const bool tensor = tensor_core_takes(*p, ratio);
   a.tile_rows = kRows;
-  // as many tiles as there may be: every sequence's last one may be short
-  const long long tiles = p->tq * ratio / kRows + std::min<long long>(p->b, p->tq);
+  a.tile_tokens = tensor ? 2 * static_cast<int>(128 / ratio) : 0;
+  // as many units as there may be: every sequence's last tile may be short
+  const long long tiles = (tensor ? p->tq / a.tile_tokens : p->tq * ratio / kRows) + std::min<long long>(p->b, p->tq);
   const long long units = tiles * p->hk;
   if (units > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
   int rc = B200Q_OK;
-  B200Q_DISPATCH_FTYPE(p->ftype, rc = a.d <= 64    ? launch_mma<T, 64>(a, wide, units, device, cs)
-                                      : a.d <= 128 ? launch_mma<T, 128>(a, wide, units, device, cs)
-                                                   : launch_mma<T, 256>(a, wide, units, device, cs));
-  if (rc == B200Q_OK) host_set_path(24);
+  if (tensor) {
+    if (p->ftype == B200Q_F16)
+      rc = a.d <= 64 ? launch_tc<__half, 64>(a, units, device, cs) : launch_tc<__half, 128>(a, units, device, cs);
+    else
+      rc = a.d <= 64 ? launch_tc<__nv_bfloat16, 64>(a, units, device, cs) : launch_tc<__nv_bfloat16, 128>(a, units, device, cs);
+  } else {
+    const long long strides = p->q_ts | p->q_hs | p->k_ts | p->k_hs | p->v_ts | p->v_hs;
+    const bool wide = !(bits & (4 * size - 1)) && strides % 4 == 0;
+    B200Q_DISPATCH_FTYPE(p->ftype, rc = a.d <= 64    ? launch_mma<T, 64>(a, wide, units, device, cs)
+                                        : a.d <= 128 ? launch_mma<T, 128>(a, wide, units, device, cs)
+                                                     : launch_mma<T, 256>(a, wide, units, device, cs));
+  }
+  if (rc == B200Q_OK) host_set_path(tensor ? 23 : 24);
   return rc;
 }
