@@ -23,13 +23,16 @@ namespace {
 
 constexpr int kBM = 128;  // channels of a block's tile
 constexpr int kBK = 128;  // bytes of a step: one 128-byte swizzle row
+constexpr int kSteps = 2;  // steps of a stage in the split kernel: one barrier for both
 constexpr int kMaxStages = 16;
 constexpr int kSmemMost = 227 * 1024;
 constexpr int kRing = 2048;                    // the tokens' scales and the barriers lie before it
 constexpr int kSmemFixed = 1024 + kRing;       // and the alignment
-// More than half: no two blocks that hold tensor memory share an SM, this library's other kernels' among them.  Blocks of a cluster
-// wait for each other; one that held tensor memory while its partner waited for some could wait for good.
+// Blocks of a cluster take more than half: no two that hold tensor memory then share an SM, this library's other kernels' among
+// them.  They wait for each other; one that held tensor memory while its partner waited for some could wait for good.  A block without
+// a cluster waits for no other once it has its tensor memory.
 constexpr int kSmemAlone = kSmemMost / 2 + 1024;
+constexpr int kTwosMost = 48;  // tokens of blocks that share an SM
 constexpr int kSplitThreads = 192;
 constexpr int kPairThreads = 320;
 
@@ -59,8 +62,22 @@ struct Channel {
     scale = ok ? __ldg(a.ws + c) : 0.0f;
     bias = ok && a.bias ? to_f32(static_cast<const T*>(a.bias)[c]) : 0.0f;
   }
-  __device__ __forceinline__ void put(const LinArgs& a, int token, int sum, float xs) const {
-    if (ok && token < a.m) y[token * a.ldy] = from_f32<T>(fmaf(static_cast<float>(sum) * scale, xs, bias));
+  // N tokens from t on.  All values first, then all stores: one after another a column took 136 clocks.
+  template <int N>
+  __device__ __forceinline__ void put(const LinArgs& a, int t, const uint32_t (&sum)[N], const float (&xs)[N]) const {
+    T v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = from_f32<T>(fmaf(static_cast<float>(static_cast<int>(sum[j])) * scale, xs[j], bias));
+    if (!ok) return;
+    T* p = y + t * a.ldy;
+    if (t + N <= a.m) {
+#pragma unroll
+      for (int j = 0; j < N; ++j, p += a.ldy) *p = v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j, p += a.ldy)
+        if (t + j < a.m) *p = v[j];
+    }
   }
 };
 
@@ -74,10 +91,16 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&v)
         "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
       : "r"(taddr));
 }
-__device__ __forceinline__ uint32_t load_shared_cluster(uint32_t addr) {
-  uint32_t r;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(r) : "r"(addr) : "memory");
-  return r;
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void store_shared_cluster(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// A producer that gave up: what it asked for lands before the block ends.
+__device__ __forceinline__ void land(uint32_t full0, int stages, int issued, const LinArgs& a) {
+  for (int i = max(0, issued - stages); i < issued; ++i)
+    mbar_wait_bounded(full0 + 8 * (i % stages), (i / stages) & 1, a.limit, a.err, kDevErrTimeoutProducer);
 }
 
 // One tile a cluster of `split` blocks.  Warp 0 loads, warp 1 issues, warps 2 to 5 write (warp w reads TMEM lanes 32 (w % 4)).
@@ -88,24 +111,39 @@ __global__ void __launch_bounds__(kSplitThreads)
   float* s_xs = reinterpret_cast<float*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_xs + 256);
   uint8_t* smem = reinterpret_cast<uint8_t*>(s_xs) + kRing;
-  const uint32_t stage_w = kBM * kBK, stage_x = a.bn * kBK, stage = stage_w + stage_x;
+  const uint32_t step = (kBM + a.bn) * kBK, stage = kSteps * step;
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kMaxStages, done = full0 + 16 * kMaxStages;
   uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 1);
+  uint32_t* landing = reinterpret_cast<uint32_t*>(smem + a.stages * stage);  // [split][bn / split][128]: the blocks' sums of my columns
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int rank = static_cast<int>(blockIdx.x % a.split), tile = static_cast<int>(blockIdx.x / a.split);
   const int t0 = tile / a.c_tiles * a.bn, c0 = tile % a.c_tiles * kBM;
   const int kb0 = static_cast<int>(static_cast<long long>(a.kblocks) * rank / a.split);
   const int kb1 = static_cast<int>(static_cast<long long>(a.kblocks) * (rank + 1) / a.split);
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < a.stages; ++i) {
-      mbar_init(full0 + 8 * i, 1);
-      mbar_init(empty0 + 8 * i, 1);
+  // Loads a stage: steps kb, kb + 1.
+  const auto load = [&](int s, int kb) {
+    const uint32_t bar = full0 + 8 * s, n = min(kSteps, kb1 - kb);
+    uint32_t at = smem_u32(smem) + s * stage;
+    mbar_arrive_expect_tx_elect(bar, n * step);
+    for (uint32_t i = 0; i < n; ++i, at += step) {
+      tma_load_3d_elect(at, &tm_w, bar, (kb + i) * kBK, c0, 0);
+      tma_load_3d_elect(at + kBM * kBK, &tm_x, bar, (kb + i) * kBK, t0, 0);
     }
-    mbar_init(done, 1);
-    fence_mbar_init();
-    tma_prefetch_desc(&tm_w);
-    tma_prefetch_desc(&tm_x);
+  };
+  int first = kb0;  // the ring is filled while the others set up
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < a.stages; ++i) {
+        mbar_init(full0 + 8 * i, 1);
+        mbar_init(empty0 + 8 * i, 1);
+      }
+      mbar_init(done, 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+    wait_for_previous();
+    for (int s = 0; s < a.stages && first < kb1; ++s, first += kSteps) load(s, first);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(slot), a.tmem_cols);
@@ -114,34 +152,34 @@ __global__ void __launch_bounds__(kSplitThreads)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (a.split > 1) cluster_arrive();
   const uint32_t acc = __shfl_sync(~0u, *slot, 0);
   wait_for_previous();
 
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait_bounded(empty0 + 8 * s, ph ^ 1u, a.limit, a.err, kDevErrTimeoutProducer)) break;
-        mbar_arrive_expect_tx(full0 + 8 * s, stage);
-        const uint32_t at = smem_u32(smem) + s * stage;
-        tma_load_3d(at, &tm_w, full0 + 8 * s, kb * kBK, c0, 0);
-        tma_load_3d(at + stage_w, &tm_x, full0 + 8 * s, kb * kBK, t0, 0);
-        if (++s == a.stages) s = 0, ph ^= 1u;
-      }
+    int s = 0, kb = first;
+    uint32_t ph = 0;
+    bool free = false;
+    for (; kb < kb1; kb += kSteps) {
+      if (!__all_sync(~0u, free || mbar_wait_bounded(empty0 + 8 * s, ph, a.limit, a.err, kDevErrTimeoutProducer))) break;
+      const int at = s;
+      if (++s == a.stages) s = 0, ph ^= 1u;
+      free = mbar_test(empty0 + 8 * s, ph);
+      load(at, kb);
     }
-    __syncwarp();
+    if (kb < kb1) land(full0, a.stages, (kb - kb0) / kSteps, a);
   } else if (warp == 1) {
     int s = 0;
     uint32_t ph = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (!__all_sync(~0u, mbar_wait_bounded(full0 + 8 * s, ph, a.limit, a.err, kDevErrTimeoutMma))) break;
-      const uint32_t at = smem_u32(smem) + s * stage;
-      const uint64_t dw = operand_desc(at), dx = operand_desc(at + stage_w);
-#pragma unroll
-      for (int j = 0; j < kBK / 32; ++j) tc_mma_i8_elect(acc, dw + 2 * j, dx + 2 * j, a.idesc, kb > kb0 || j ? 1u : 0u);
-      tc_commit_elect(empty0 + 8 * s);
+    bool full = false;
+    for (int kb = kb0; kb < kb1; kb += kSteps) {
+      if (!__all_sync(~0u, full || mbar_wait_bounded(full0 + 8 * s, ph, a.limit, a.err, kDevErrTimeoutMma))) break;
+      const uint32_t at = smem_u32(smem) + s * stage, bar = empty0 + 8 * s;
       if (++s == a.stages) s = 0, ph ^= 1u;
+      full = mbar_test(full0 + 8 * s, ph);  // an answer takes 130 clocks, as long as the products of a step of few tokens
+      tc_mma_i8_kblock4(acc, operand_desc(at), operand_desc(at + kBM * kBK), a.idesc, kb > kb0 ? 1u : 0u);
+      if (kb + 1 < kb1) tc_mma_i8_kblock4(acc, operand_desc(at + step), operand_desc(at + step + kBM * kBK), a.idesc, 1u);
+      tc_commit_elect(bar);
     }
     tc_commit_elect(done);
     mbar_wait_bounded(done, 0, a.limit, a.err, kDevErrTimeoutMma);
@@ -155,33 +193,57 @@ __global__ void __launch_bounds__(kSplitThreads)
     __syncwarp();
     tc_fence_after();
     const uint32_t from = acc + (static_cast<uint32_t>((warp % 4) * 32) << 16);
-    uint32_t* part = reinterpret_cast<uint32_t*>(smem);  // [bn][128]: the ring has been read by now
-    for (int c = 0; c < a.bn; c += 16) {
-      uint32_t v[16];
-      tmem_ld_32x32b_x16(from + c, v);
-      tmem_ld_wait();
+    const auto xs_at = [&](int c, float (&xs)[16]) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (a.split == 1)
-          ch.put(a, t0 + c + j, static_cast<int>(v[j]), s_xs[c + j]);
-        else
-          part[(c + j) * kBM + mine] = v[j];
+      for (int j = 0; j < 16; j += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(s_xs + c + j);
+        xs[j] = x.x, xs[j + 1] = x.y, xs[j + 2] = x.z, xs[j + 3] = x.w;
       }
-    }
-    if (a.split > 1) {
-      cluster_sync_all();
-      const int j0 = a.bn * rank / a.split, j1 = a.bn * (rank + 1) / a.split;
-      for (int j = j0; j < j1 && t0 + j < a.m; ++j) {
-        const uint32_t at = smem_u32(part + j * kBM + mine);
-        int sum = 0;
-        for (int r = 0; r < a.split; ++r) sum += static_cast<int>(load_shared_cluster(mapa_shared(at, r)));
-        ch.put(a, t0 + j, sum, s_xs[j]);
+    };
+    if (a.split == 1) {
+      for (int c = 0; c < a.bn && t0 + c < a.m; c += 16) {
+        uint32_t v[16];
+        float xs[16];
+        tmem_ld_32x32b_x16(from + c, v);
+        xs_at(c, xs);
+        tmem_ld_wait();
+        ch.put(a, t0 + c, v, xs);
       }
-      cluster_sync_all();
+    } else {
+      const int share = a.bn / a.split;  // columns that a block adds up, at least 2
+      const uint32_t to = smem_u32(landing + rank * share * kBM + mine);
+      cluster_wait();  // the others have started
+      for (int c = 0; c < a.bn && t0 + c < a.m; c += 16) {
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(from + c, v);
+        tmem_ld_wait();
+        int owner = c / share, in = c - owner * share;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {  // two columns go to one block
+          const uint32_t at = mapa_shared(to, owner) + in * (kBM * 4);
+          store_shared_cluster(at, v[j]);
+          store_shared_cluster(at + kBM * 4, v[j + 1]);
+          if ((in += 2) == share) in = 0, ++owner;
+        }
+      }
+      cluster_sync_all();  // every block's sums have arrived
+      const int j0 = share * rank;
+      const uint32_t* mine_at = landing + mine;
+      for (int j = 0; j < share && t0 + j0 + j < a.m; j += 2) {
+        uint32_t v[2] = {0u, 0u};
+        const float xs[2] = {s_xs[j0 + j], s_xs[j0 + j + 1]};
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < a.split) {
+            v[0] += mine_at[(r * share + j) * kBM];
+            v[1] += mine_at[(r * share + j + 1) * kBM];
+          }
+        ch.put(a, t0 + j0 + j, v, xs);
+      }
     }
   }
   if (warp < 2 && a.split > 1) {
-    cluster_sync_all();
+    cluster_wait();
     cluster_sync_all();
   }
   tc_fence_before();
@@ -245,14 +307,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     if (lane == 0) {
       int s = 0;
       uint32_t ph = 0;
-      bool ok = true;
+      int issued = 0;
+      bool ok = true, free = true;
       const uint32_t full_leader = mapa_shared(full0, 0);
       for (int i = unit; i < tiles && ok; i += units) {
         int ct, tt;
         tile_at(i, &ct, &tt);
         const int c0 = (2 * ct + rank) * kBM, t0 = tt * a.bn + rank * (a.bn / 2);
         for (int kb = 0; kb < a.kblocks; ++kb) {
-          if (!mbar_wait_bounded(empty0 + 8 * s, ph ^ 1u, a.limit, a.err, kDevErrTimeoutProducer)) {
+          if (!free && !mbar_wait_bounded(empty0 + 8 * s, ph ^ 1u, a.limit, a.err, kDevErrTimeoutProducer)) {
             ok = false;
             break;
           }
@@ -263,28 +326,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             mbar_arrive_expect_tx_cluster_relaxed(bar, stage);
           tma_load_3d_pair(at, &tm_w, bar, kb * kBK, c0, 0);
           tma_load_3d_pair(at + stage_w, &tm_x, bar, kb * kBK, t0, 0);
+          ++issued;
           if (++s == a.stages) s = 0, ph ^= 1u;
+          free = mbar_test(empty0 + 8 * s, ph ^ 1u);
         }
       }
+      if (!ok && rank == 0) land(full0, a.stages, issued, a);  // both blocks' copies count there; the other waits for the leader below
     }
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0) {
       int s = 0, buf = 0;
       uint32_t ph = 0, acc_ph = 0;
-      bool ok = true;
+      bool ok = true, full = false;
       for (int i = unit; i < tiles && ok; i += units) {
         if (!__all_sync(~0u, mbar_wait_bounded(acce0 + 8 * buf, acc_ph ^ 1u, a.limit, a.err, kDevErrTimeoutMma))) break;
         tc_fence_after();
         for (int kb = 0; kb < a.kblocks; ++kb) {
-          if (!__all_sync(~0u, mbar_wait_bounded(full0 + 8 * s, ph, a.limit, a.err, kDevErrTimeoutMma))) {
+          if (!__all_sync(~0u, full || mbar_wait_bounded(full0 + 8 * s, ph, a.limit, a.err, kDevErrTimeoutMma))) {
             ok = false;
             break;
           }
-          const uint32_t at = smem_u32(smem) + s * stage;
-          tc_mma_i8_pair_kblock4(tmem + buf * a.bn, operand_desc(at), operand_desc(at + stage_w), a.idesc, kb ? 1u : 0u);
-          tc_commit_pair_elect(empty0 + 8 * s);
+          const uint32_t at = smem_u32(smem) + s * stage, bar = empty0 + 8 * s;
           if (++s == a.stages) s = 0, ph ^= 1u;
+          full = mbar_test(full0 + 8 * s, ph);
+          tc_mma_i8_pair_kblock4(tmem + buf * a.bn, operand_desc(at), operand_desc(at + stage_w), a.idesc, kb ? 1u : 0u);
+          tc_commit_pair_elect(bar);
         }
         if (!ok) break;
         tc_commit_pair_elect(accf0 + 8 * buf);
@@ -307,14 +374,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if (!__all_sync(~0u, mbar_wait_bounded(accf0 + 8 * buf, acc_ph, a.limit, a.err, kDevErrTimeoutEpilogue))) break;
       tc_fence_after();
       const uint32_t from = tmem + buf * a.bn + (static_cast<uint32_t>(quarter * 32) << 16);
-      for (int c = 32 * half; c < a.bn; c += 64) {
+      for (int c = 32 * half; c < a.bn && tt * a.bn + c < a.m; c += 64) {
         uint32_t v[32];
+        float xs[32];
         tmem_ld_32x32b_x32(from + c, v);
         const int t = tt * a.bn + c;
-        const float mine = t + lane < a.m ? __ldg(a.xs + t + lane) : 0.0f;
-        tmem_ld_wait();
+        const float one = t + lane < a.m ? __ldg(a.xs + t + lane) : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) ch.put(a, t + j, static_cast<int>(v[j]), __shfl_sync(~0u, mine, j));
+        for (int j = 0; j < 32; ++j) xs[j] = __shfl_sync(~0u, one, j);
+        tmem_ld_wait();
+        ch.put(a, t, v, xs);
       }
       tc_fence_before();
       __syncwarp();
@@ -335,23 +404,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 // How a call is laid out.
 struct Plan {
   bool pair;
-  int bn, split;
+  int bn, split, stages;
 };
 
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
-Plan plan_for(int m, int n, int kblocks, int sms) {
-  Plan p{false, std::min(256, round_up(m, 16)), 1};
-  const int pair_tiles = (n + 255) / 256 * ((m + 255) / 256);
-  if (m > 128 && pair_tiles * 2 >= sms) return {true, 256, 1};
-  const int tiles = (n + kBM - 1) / kBM * ((m + p.bn - 1) / p.bn);
-  while (p.split < 8 && tiles * p.split * 2 <= sms && kblocks >= 2 * p.split) p.split *= 2;
-  return p;
+int stage_bytes(const Plan& p) { return p.pair ? (kBM + p.bn / 2) * kBK : kSteps * (kBM + p.bn) * kBK; }
+int landing_bytes(const Plan& p) { return p.split > 1 ? p.bn * kBM * 4 : 0; }
+
+// Clocks that a plan takes, from timed calls: what a step of a block costs (its barriers and copies, and more with every token), what a
+// tile costs beside its steps, what joining costs, and the bytes at what DRAM gives (4 KB a clock).  The plans differ most where few
+// tiles leave SMs idle: 64 x 4096 x 4096 8.7 us on 2 x 32 tokens, 9.6 on 64, 9.4 on 64 split in four; 1 x 4096 x 4096 5.9 split in four,
+// 7.6 whole; 512 x 4096 x 4096 13.1 on 128 tokens, 17.6 on pairs of 256; 1024 x 4096 x 4096 21.4 on 256 tokens, 18.2 on pairs.
+// `room`: blocks that the GPU holds at once, by the size of their cluster (1, 2, 4, 8: 148, 148, 132, 120 with one a SM).
+double plan_clocks(const Plan& p, int m, int n, int kblocks, const int (&room)[4]) {
+  const long long t_tiles = (m + p.bn - 1) / p.bn;
+  if (p.pair) {
+    const long long tiles = t_tiles * ((n + 255) / 256), waves = (tiles + room[0] / 2 - 1) / (room[0] / 2);
+    return 9000.0 + 30.0 * p.bn + static_cast<double>(waves) * kblocks * (440.0 + 0.9 * p.bn);
+  }
+  const long long blocks = t_tiles * ((n + kBM - 1) / kBM) * p.split;
+  const int steps = (kblocks + p.split - 1) / p.split;
+  // blocks of few tokens share an SM in twos and hide part of each other's steps
+  const bool twos = p.split == 1 && p.bn <= kTwosMost && blocks > room[0];
+  const long long most = twos ? 2ll * room[0] : room[p.split == 1 ? 0 : p.split == 2 ? 1 : p.split == 4 ? 2 : 3];
+  const double waves = static_cast<double>((blocks + most - 1) / most), at_once = twos ? 1.6 : 1.0;
+  const double join = p.split > 1 ? 1700.0 + 300.0 * p.split + 15.0 * p.bn : 0.0;
+  const double clocks = waves * at_once * (steps * (210.0 + 2.8 * p.bn) + 27.0 * p.bn) + 4500.0 + join;
+  return std::max(clocks, (static_cast<double>(n) + m) * kblocks * kBK / 4096.0 + 5000.0 + join);
+}
+
+Plan plan_for(int m, int n, int kblocks, const int (&room)[4]) {
+  Plan best{false, 16, 1, 0};
+  double least = 1e300;
+  const auto offer = [&](Plan p) {
+    const double c = plan_clocks(p, m, n, kblocks, room);
+    if (c < least) least = c, best = p;
+  };
+  const int most = std::min(256, round_up(m, 16));
+  for (int bn = 16; bn <= most; bn += bn < 128 ? 16 : 32)
+    for (int split = 1; split <= 8 && split <= kblocks && (split == 1 || bn <= 128); split *= 2) offer({false, bn, split, 0});
+  offer({false, most, 1, 0});
+  if (m > 64)
+    for (int bn = 64; bn <= 256; bn += 32) offer({true, bn, 1, 0});
+  const int steps = best.pair ? kblocks : ((kblocks + best.split - 1) / best.split + kSteps - 1) / kSteps;
+  const long long blocks = static_cast<long long>((m + best.bn - 1) / best.bn) * ((n + kBM - 1) / kBM);
+  const int smem = !best.pair && best.split == 1 && best.bn <= kTwosMost && blocks > room[0] ? kSmemMost / 2 - 1024 : kSmemMost;
+  best.stages = std::max(2, std::min({kMaxStages, steps, (smem - kSmemFixed - landing_bytes(best)) / stage_bytes(best)}));
+  return best;
 }
 
 template <typename T>
-int launch_plan(const Plan& p, LinArgs a, const CUtensorMap& tm_w, const CUtensorMap& tm_x, int sms, int device,
-                cudaStream_t cs) {
+int launch_plan(const Plan& p, LinArgs a, const CUtensorMap& tm_w, const CUtensorMap& tm_x, int sms, int device, cudaStream_t cs) {
   static std::atomic<bool> ready[kMaxDevices];
   if (!ready[device].load(std::memory_order_relaxed)) {
     cudaError_t e = cudaFuncSetAttribute(linear_s8_split_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
@@ -361,26 +465,49 @@ int launch_plan(const Plan& p, LinArgs a, const CUtensorMap& tm_w, const CUtenso
   }
   a.bn = p.bn;
   a.split = p.split;
-  const int stage = kBM * kBK + (p.pair ? p.bn / 2 : p.bn) * kBK;
-  const int steps = p.pair ? a.kblocks : (a.kblocks + p.split - 1) / p.split;
-  a.stages = std::max(2, std::min({kMaxStages, (kSmemMost - kSmemFixed) / stage, p.pair ? kMaxStages : steps}));
+  a.stages = p.stages;
   a.t_tiles = (a.m + p.bn - 1) / p.bn;
   a.c_tiles = (a.n + (p.pair ? 255 : 127)) / (p.pair ? 256 : 128);
   const uint32_t rows = p.pair ? 256 : 128;
   a.idesc = (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(p.bn >> 3) << 17) | ((rows >> 4) << 24);  // s32 += s8 s8
   for (a.tmem_cols = 32; a.tmem_cols < static_cast<uint32_t>(p.pair ? 2 * p.bn : p.bn);) a.tmem_cols *= 2;
-  size_t smem = static_cast<size_t>(a.stages) * stage + kSmemFixed;
+  size_t smem = static_cast<size_t>(p.stages) * stage_bytes(p) + landing_bytes(p) + kSmemFixed;
+  if (p.pair || p.split > 1) smem = std::max(smem, static_cast<size_t>(kSmemAlone));
   const long long tiles = static_cast<long long>(a.t_tiles) * a.c_tiles;
   if (tiles * 8 > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many tiles");
-  smem = std::max(smem, static_cast<size_t>(kSmemAlone));
-  if (p.pair) {
-    const int pairs = static_cast<int>(std::min<long long>(tiles, sms / 2));
-    return host_launch("linear_s8_pair_kernel launch", linear_s8_pair_kernel<T>, dim3(2 * pairs), kPairThreads, smem, cs, 1, tm_w,
-                       tm_x, a);
-  }
-  if (p.split > 1) smem = std::max(smem, static_cast<size_t>(p.bn) * kBM * 4 + kSmemFixed);
+  if (p.pair)
+    return host_launch("linear_s8_pair_kernel launch", linear_s8_pair_kernel<T>,
+                       dim3(2 * static_cast<unsigned>(std::min<long long>(tiles, sms / 2))), kPairThreads, smem, cs, 1, tm_w, tm_x, a);
   return host_launch("linear_s8_split_kernel launch", linear_s8_split_kernel<T>, dim3(static_cast<unsigned>(tiles * p.split)),
                      kSplitThreads, smem, cs, p.split, tm_w, tm_x, a);
+}
+
+// Found once for a device: clusters lie in one part of the GPU each, whose SMs they do not use up.
+int block_room(int device, int sms, int (*room)[4]) {
+  static std::atomic<int> of[kMaxDevices][4];
+  (*room)[0] = sms;
+  for (int i = 1; i < 4; ++i) {
+    int blocks = of[device][i].load(std::memory_order_relaxed);
+    if (!blocks) {
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(1024);
+      cfg.blockDim = dim3(kSplitThreads);
+      cfg.dynamicSmemBytes = kSmemAlone;
+      cudaLaunchAttribute attr[1] = {};
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim = {1u << i, 1, 1};
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      cudaError_t e = cudaFuncSetAttribute(linear_s8_split_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+      int clusters = 0;
+      if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&clusters, linear_s8_split_kernel<float>, &cfg);
+      if (e != cudaSuccess) return host_cuda_fail(e, "cudaOccupancyMaxActiveClusters(linear_s8_split_kernel)");
+      blocks = std::max(1, clusters) << i;
+      of[device][i].store(blocks, std::memory_order_relaxed);
+    }
+    (*room)[i] = blocks;
+  }
+  return B200Q_OK;
 }
 
 int linear_s8(const b200q_linear_s8_args* p, const Plan* fixed, cudaStream_t cs) {
@@ -411,7 +538,9 @@ int linear_s8(const b200q_linear_s8_args* p, const Plan* fixed, cudaStream_t cs)
   a.kblocks = (k + kBK - 1) / kBK;
   a.limit = host_wait_limit();
   a.err = err;
-  const Plan plan = fixed ? *fixed : plan_for(m, n, a.kblocks, sms);
+  int room[4];
+  if ((rc = block_room(device, sms, &room))) return rc;
+  const Plan plan = fixed ? *fixed : plan_for(m, n, a.kblocks, room);
   CUtensorMap tm_w, tm_x;
   const auto stride = [&](int rows, int64_t ld) { return static_cast<uint64_t>(rows > 1 ? ld : round_up(k, 16)); };
   if ((rc = host_tensor_map(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p->w, {static_cast<uint64_t>(k), static_cast<uint64_t>(n), 1},
