@@ -20,6 +20,7 @@ struct PromptArgs {
   Divisor ratio;   // hq / hk
   int tile_rows;   // rows (token, head of the group) of a tile; a tile holds whole tokens where tile_tokens is not 0
   int tile_tokens;
+  long long most_units;  // key heads times tiles, as many as there may be
   float scale;
   int* err;
   long long limit;
@@ -89,7 +90,7 @@ __device__ inline PromptUnit prompt_unit(const PromptArgs& a, int unit, bool rep
     const unsigned have = __ballot_sync(~0u, s.tiles(a) > lo);
     const int n = __popc(have);
     if (left < n) {
-      const int from = __fns(have, 0, left + 1);
+      const int from = __ffs(__ballot_sync(~0u, (have >> lane & 1) && __popc(have & ((1u << lane) - 1)) == left)) - 1;
       u.s = {__shfl_sync(~0u, s.q0, from), __shfl_sync(~0u, s.lq, from), __shfl_sync(~0u, s.k0, from), __shfl_sync(~0u, s.lk, from),
              false};
       u.tile = lo;

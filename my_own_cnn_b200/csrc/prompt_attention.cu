@@ -314,7 +314,7 @@ bool tensor_core_takes(const b200q_prompt_attention_args& p, long long ratio) {
 }
 
 template <typename T, int D>
-int launch_tc(const PromptArgs& a, long long units, int device, cudaStream_t cs) {
+int launch_tc(const PromptArgs& a, int sms, int device, cudaStream_t cs) {
   static std::atomic<bool> ready[kMaxDevices];
   if (!ready[device].load(std::memory_order_relaxed)) {
     const cudaError_t e =
@@ -335,8 +335,8 @@ int launch_tc(const PromptArgs& a, long long units, int device, cudaStream_t cs)
   if (rc == B200Q_OK) rc = map(&tm_k, a.k, a.hk, a.tk, a.k_ts, a.k_hs, 1, kTcKeys);
   if (rc == B200Q_OK) rc = map(&tm_v, a.v, a.hk, a.tk, a.v_ts, a.v_hs, 1, kTcKeys);
   if (rc) return rc;
-  return host_launch("prompt_tc_kernel launch", prompt_tc_kernel<T, D>, dim3(static_cast<unsigned>(units)), kTcPromptThreads,
-                     TcShape<D>::kSmem, cs, 1, tm_q, tm_k, tm_v, a, a.scale < 0.0f ? 1u : 0u);
+  return host_launch("prompt_tc_kernel launch", prompt_tc_kernel<T, D>, dim3(static_cast<unsigned>(std::min<long long>(a.most_units, sms))),
+                     kTcPromptThreads, TcShape<D>::kSmem, cs, 1, tm_q, tm_k, tm_v, a, a.scale < 0.0f ? 1u : 0u);
 }
 
 }  // namespace
@@ -381,14 +381,14 @@ extern "C" int b200q_prompt_attention(const b200q_prompt_attention_args* p, void
   a.tile_tokens = tensor ? 2 * static_cast<int>(128 / ratio) : 0;
   // as many units as there may be: every sequence's last tile may be short
   const long long tiles = (tensor ? p->tq / a.tile_tokens : p->tq * ratio / kRows) + std::min<long long>(p->b, p->tq);
-  const long long units = tiles * p->hk;
+  const long long units = a.most_units = tiles * p->hk;
   if (units > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
   int rc = B200Q_OK;
   if (tensor) {
     if (p->ftype == B200Q_F16)
-      rc = a.d <= 64 ? launch_tc<__half, 64>(a, units, device, cs) : launch_tc<__half, 128>(a, units, device, cs);
+      rc = a.d <= 64 ? launch_tc<__half, 64>(a, sms, device, cs) : launch_tc<__half, 128>(a, sms, device, cs);
     else
-      rc = a.d <= 64 ? launch_tc<__nv_bfloat16, 64>(a, units, device, cs) : launch_tc<__nv_bfloat16, 128>(a, units, device, cs);
+      rc = a.d <= 64 ? launch_tc<__nv_bfloat16, 64>(a, sms, device, cs) : launch_tc<__nv_bfloat16, 128>(a, sms, device, cs);
   } else {
     const long long strides = p->q_ts | p->q_hs | p->k_ts | p->k_hs | p->v_ts | p->v_hs;
     const bool wide = !(bits & (4 * size - 1)) && strides % 4 == 0;

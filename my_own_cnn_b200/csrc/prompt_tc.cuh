@@ -1,9 +1,10 @@
 // Prompt attention of 16-bit types on tcgen05 (prompt_tc_kernel).
 //
-// A block has two tiles of 128 rows (token, query head of one key head) and goes through the keys 128 at a time.  Warps 0 to 3 and 4
-// to 7 hold a tile each, one row a thread: scores from TMEM, weights back over them as 16-bit operands of the second product; warp 8 loads by TMA, warp
-// 9 issues.  While one tile's scores become weights the tensor core has the other tile's products:
+// One block an SM takes unit after unit: two tiles of 128 rows (token, query head of one key head), all their keys, 128 at a time.
+// Warps 0 to 3 and 4 to 7 hold a tile each, one row a thread: scores from TMEM, weights back over them as 16-bit operands of the second product; warp 8 loads
+// by TMA, warp 9 issues, warp 10 finds the units.  While one tile's scores become weights the tensor core has the other tile's products:
 //   PV_A(j), QK_A(j + 1), PV_B(j), QK_B(j + 1), ...
+// and while the last sums of a unit are scaled and stored, the next one's queries and keys are on their way.
 // Tensor memory: scores of A and B (128 columns each; weights take the first 64), then the sums O of A and B (D columns each).
 // A row's reference is not its maximum but one that may lie up to 2^8 below it: O is then rescaled a few times in a row of any length, by
 // the threads that own it, and not with every tile.  fp16 weights are lifted by 2^6: they stay normal down to 2^-20 of the reference,
@@ -15,35 +16,47 @@
 
 namespace b200q {
 
-constexpr int kTcKeys = 128;
-constexpr int kTcPromptThreads = 320;
+constexpr int kTcKeys = 128;  // of a tile of K or V; scores and weights come in halves
+constexpr int kHalf = 64;
+constexpr int kTcPromptThreads = 384;
 constexpr int kTcMaxStages = 8;
 constexpr float kSlack = 8.0f;  // log2 of how far a row's maximum may pass its reference
 
 template <int D>
 struct TcShape {
   static constexpr int kTile = 128 * D * 2;  // bytes of 128 rows
-  static constexpr int kStages = D == 128 ? 5 : 8;
-  static constexpr int kHead = 1024;  // barriers
-  static constexpr int kSmem = 1024 + kHead + (2 + kStages) * kTile;
+  static constexpr int kStages = D == 128 ? 4 : 8;
+  static constexpr int kHead = 1024;  // barriers and units
+  static constexpr int kSmem = 1024 + kHead + (2 + kStages) * kTile + 8 * 4096;  // queries, ring, results
 };
 
-// D (+)= A B with A from shared memory or from tensor memory: fp16 or bf16 operands, fp32 sums.
-__device__ __forceinline__ void tc_mma_f16_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Four products of 16 of K in one elected block, fp16 or bf16 operands, fp32 sums: D (+)= A B.  Both operands 32 bytes on from slice to
+// slice (K-major tiles); or A in tensor memory, 8 columns a slice, and B 16 rows of 128 bytes on (a tile of V).
+__device__ __forceinline__ void tc_mma_f16_x4_elect(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
+      "{\n\t.reg .pred p, e, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_f16_ts_elect(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void tc_mma_f16_ts_x4_elect(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
+      "{\n\t.reg .pred p, e, t;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "add.s32 a1, %1, 8;\n\tadd.s32 a2, %1, 16;\n\tadd.s32 a3, %1, 24;\n\t"
+      "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
@@ -56,6 +69,14 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
       "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
       "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
+}
+// Nothing that uses these registers comes before this place: tmem_ld_wait() does not name them.
+__device__ __forceinline__ void loaded(uint32_t (&v)[32]) {
+  asm volatile(""
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                 "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]),
+                 "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]),
+                 "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -72,12 +93,19 @@ __device__ __forceinline__ uint32_t pack_16(float lo, float hi) {
     return pack_bf16(lo, hi);
 }
 
-// What one block does: its sequence and tokens, read once by warp 0.
+// What one block does next: a sequence and the tokens of it.
 struct TcUnit {
   Sequence s;
   int token0;  // of tile A in the sequence
+  int kv;      // key head
   int ok;
 };
+
+// Steps of 128 keys that tile i of a unit needs: its last token's.
+__device__ __forceinline__ int unit_steps(const TcUnit& u, int i, int tokens) {
+  const int first = u.token0 + i * tokens, last = min(u.s.lq, first + tokens) - 1;
+  return first < u.s.lq ? (max(0, last + u.s.lk - u.s.lq + 1) + kTcKeys - 1) / kTcKeys : 0;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcPromptThreads, 1)
@@ -90,26 +118,34 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kTcMaxStages;
-  const uint32_t q_full = full0 + 16 * kTcMaxStages, s_full = q_full + 16, p_full = s_full + 16, o_done = p_full + 16;
-  const uint32_t drain = o_done + 16;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * kTcMaxStages + 9);
-  TcUnit* shared_unit = reinterpret_cast<TcUnit*>(slot + 2);
-  const uint32_t s_q = smem_u32(smem) + S::kHead, s_ring = s_q + 2 * S::kTile;
+  const uint32_t q_full = full0 + 16 * kTcMaxStages, q_empty = q_full + 16, o_done = q_empty + 16;
+  const uint32_t s_full = o_done + 16, p_full = s_full + 32;  // [tile][half]
+  const uint32_t u_full = p_full + 32, u_empty = u_full + 16, drain = u_empty + 16;
+  const uint32_t ended = drain + 16;  // a tile's last product of a unit
+  uint32_t* slot = reinterpret_cast<uint32_t*>(bars + 2 * kTcMaxStages + 22);
+  TcUnit* units = reinterpret_cast<TcUnit*>(bars + 2 * kTcMaxStages + 23);  // two
+  const uint32_t s_q = smem_u32(smem) + S::kHead, s_ring = s_q + 2 * S::kTile, s_out = s_ring + S::kStages * S::kTile;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int ratio = static_cast<int>(a.ratio.d), tokens = a.tile_tokens / 2;  // of one tile
 
   if (threadIdx.x == 256) {
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(full0 + 8 * i, 1);
-      mbar_init(empty0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, 2);  // both tiles' products
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + 8 * i, 1);
-      mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_full + 8 * i, 4);
+      mbar_init(q_empty + 8 * i, 1);
       mbar_init(o_done + 8 * i, 1);
+      mbar_init(ended + 8 * i, 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(s_full + 16 * i + 8 * b, 1);
+        mbar_init(p_full + 16 * i + 8 * b, 4);
+      }
+      mbar_init(u_full + 8 * i, 1);
+      mbar_init(u_empty + 8 * i, 11);  // loader, issuers, the tiles' eight warps
+      mbar_init(drain + 8 * i, 1);
     }
-    mbar_init(drain, 1);
     fence_mbar_init();
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
@@ -120,220 +156,270 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
     tmem_relinquish();
   }
   wait_for_previous();
-  const int kv = static_cast<int>(blockIdx.x % a.hk);
-  if (warp == 0) {
-    const PromptUnit u = prompt_unit(a, static_cast<int>(blockIdx.x / a.hk), blockIdx.x == 0);
-    if (lane == 0) *shared_unit = {u.s, u.tile * a.tile_tokens, u.ok};
-  }
+  // The block's r-th unit in the order of their lengths, every other round backwards.
+  auto find = [&](int r, TcUnit* to) {
+    const long long n = static_cast<long long>(r) * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    PromptUnit u{};
+    if (n < a.most_units) u = prompt_unit(a, static_cast<int>(n / a.hk), r == 0 && blockIdx.x == 0);
+    if (lane == 0) *to = {u.s, u.tile * a.tile_tokens, static_cast<int>(n % a.hk), u.ok};
+    return u.ok;
+  };
+  bool more = true;
+  if (warp == 10) more = find(0, units);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(~0u, *slot, 0);
-  const TcUnit u = *shared_unit;
-  const int shift = u.s.lk - u.s.lq;
-  // keys that a tile needs, in steps: its last token's
-  int steps[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int first = u.token0 + i * tokens, last = min(u.s.lq, first + tokens) - 1;
-    steps[i] = u.ok && first < u.s.lq ? (max(0, last + shift + 1) + kTcKeys - 1) / kTcKeys : 0;
-  }
-  const int all = max(steps[0], steps[1]);
 
-  if (warp == 8) {
-    if (lane == 0 && all) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (steps[i]) {
-          const uint32_t bytes = static_cast<uint32_t>(tokens * ratio) * 128u;
-          mbar_arrive_expect_tx(q_full + 8 * i, kChunks * bytes);
-          for (int c = 0; c < kChunks; ++c)
-            tma_load_3d(s_q + i * S::kTile + c * 16384, &tm_q, q_full + 8 * i, 64 * c, kv * ratio, u.s.q0 + u.token0 + i * tokens);
-        }
-      int s = 0, issued = 0;
-      uint32_t ph = 0;
-      for (; issued < 2 * all; ++issued) {  // K 0, V 0, K 1, V 1, ...
-        if (!mbar_wait_bounded(empty0 + 8 * s, ph ^ 1u, a.limit, a.err, kDevErrTimeoutProducer)) break;
-        mbar_arrive_expect_tx(full0 + 8 * s, S::kTile);
-        for (int c = 0; c < kChunks; ++c)
-          tma_load_3d(s_ring + s * S::kTile + c * 16384, issued & 1 ? &tm_v : &tm_k, full0 + 8 * s, 64 * c, kv,
-                      u.s.k0 + issued / 2 * kTcKeys);
-        if (++s == S::kStages) s = 0, ph ^= 1u;
-      }
-      if (issued < 2 * all)  // given up: what is on its way lands before the block ends
-        for (int i = max(0, issued - S::kStages); i < issued; ++i)
-          mbar_wait_bounded(full0 + 8 * (i % S::kStages), (i / S::kStages) & 1, a.limit, a.err, kDevErrTimeoutProducer);
-    }
+  bool ok = true;  // no wait has run out
+  auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+    ok = ok && __all_sync(~0u, mbar_wait_bounded(bar, parity, a.limit, a.err, code));
+    return ok;
+  };
+  // The block's r-th unit (every warp that works on units asks for each of them once); ok == 0: there is none.
+  auto unit_at = [&](int r, int code) {
+    TcUnit u{};
+    if (!wait(u_full + 8 * (r & 1), (r >> 1) & 1, code)) return u;
+    u = units[r & 1];
     __syncwarp();
-  } else if (warp == 9) {
-    constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
-    constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | ((128u >> 4) << 24);
-    const uint32_t qk_desc = kDesc | ((kTcKeys >> 3) << 17) | (negate << 13);
-    const uint32_t pv_desc = kDesc | ((static_cast<uint32_t>(D) >> 3) << 17) | (1u << 16);  // V: channels contiguous
-    bool ok = all > 0;
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-      ok = ok && __all_sync(~0u, mbar_wait_bounded(bar, parity, a.limit, a.err, kDevErrTimeoutMma));
-    };
-    auto tile_at = [&](int n) { return s_ring + n % S::kStages * S::kTile; };
-    auto tile_wait = [&](int n) { wait(full0 + 8 * (n % S::kStages), (n / S::kStages) & 1); };
-    auto release = [&](int n) { tc_commit_elect(empty0 + 8 * (n % S::kStages)); };
-    auto qk = [&](int i, int j) {
-      if (!ok) return;
-      const uint32_t q = s_q + i * S::kTile, k = tile_at(2 * j);
-#pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        const uint32_t off = c / 4 * 16384 + c % 4 * 32;
-        tc_mma_f16_elect(tmem + i * 128, make_smem_desc(q + off, 16, 1024, 2), make_smem_desc(k + off, 16, 1024, 2), qk_desc, c ? 1u : 0u);
-      }
-      tc_commit_elect(s_full + 8 * i);
-    };
-    auto pv = [&](int i, int j) {
-      wait(p_full + 8 * i, j & 1);
-      if (!ok) return;
-      tc_fence_after();
-      const uint32_t v = tile_at(2 * j + 1);
-#pragma unroll
-      for (int c = 0; c < kTcKeys / 16; ++c)
-        tc_mma_f16_ts_elect(tmem + 256 + i * D, tmem + i * 128 + c * 8, make_smem_desc(v + c * 2048, 16384, 1024, 2), pv_desc, j | c ? 1u : 0u);
-      tc_commit_elect(o_done + 8 * i);
-    };
-    if (ok) tile_wait(0);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (steps[i]) {
-        wait(q_full + 8 * i, 0);
-        qk(i, 0);
-      }
-    if (ok) release(0);
-    for (int j = 0; j < all && ok; ++j) {
-      tile_wait(2 * j + 1);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (j < steps[i]) pv(i, j);
-        if (i == 1 && ok) release(2 * j + 1);
-        if (j + 1 < steps[i]) {
-          if (i == 0 || steps[0] <= j + 1) tile_wait(2 * j + 2);
-          wait(o_done + 8 * i, j & 1);  // the weights have been read: new scores may take their place
-          qk(i, j + 1);
-        }
-      }
-      if (ok && j + 1 < all) release(2 * j + 2);
-    }
-    tc_commit_elect(drain);
-    mbar_wait_bounded(drain, 0, a.limit, a.err, kDevErrTimeoutMma);
-    __syncwarp();
-  } else {
-    const int i = warp / 4, row = (warp % 4) * 32 + lane, n = steps[i];
+    if (lane == 0) mbar_arrive(u_empty + 8 * (r & 1));
+    return u;
+  };
+
+  // The tiles' threads hold a row's 128 scores: registers go to them, 12 warps x 168 = 8 x 200 + 4 x 104.
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    constexpr int kCode = kDevErrTimeoutEpilogue;
+    const int i = warp / 4, row = (warp % 4) * 32 + lane;
     const uint32_t quarter = static_cast<uint32_t>((warp % 4) * 32) << 16;
     const uint32_t t_s = tmem + i * 128 + quarter, t_o = tmem + 256 + i * D + quarter;
-    const int of = static_cast<int>(a.ratio.of(row)), token = u.token0 + i * tokens + of, head = kv * ratio + row - of * ratio;
-    const bool mine = u.ok && of < tokens && token < u.s.lq;
-    const int seen = mine ? max(0, token + shift + 1) : 0;
+    const int of = static_cast<int>(a.ratio.of(row));
     const float c = fabsf(a.scale) * kLog2e;
-    float ref = 0.0f, sum = 0.0f;
-    bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      ok = __all_sync(~0u, mbar_wait_bounded(s_full + 8 * i, j & 1, a.limit, a.err, kDevErrTimeoutEpilogue));
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t raw[4][32];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) tmem_ld_32x32b_x32(t_s + 32 * k, raw[k]);
-      tmem_ld_wait();
-      auto s = [&](int k) { return __uint_as_float(raw[k / 32][k % 32]); };
-      const int limit = seen - j * kTcKeys;
-      if (__any_sync(~0u, limit < kTcKeys)) {
-#pragma unroll
-        for (int k = 0; k < 128; ++k)
-          if (k >= limit) raw[k / 32][k % 32] = 0xFF800000u;
-      }
-      float m[4] = {s(0), s(1), s(2), s(3)};
-#pragma unroll
-      for (int k = 4; k < 128; k += 8)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m[e] = k + e + 4 < 128 ? max3(m[e], s(k + e), s(k + e + 4)) : fmaxf(m[e], s(k + e));
-      const float top = fmaxf(max3(m[0], m[1], m[2]), m[3]) * c;  // -inf: nothing seen in this step
-      if (j == 0) {
-        ref = top == -INFINITY ? 0.0f : top;
-      } else if (__any_sync(~0u, top - ref > kSlack)) {
-        const float now = top - ref > kSlack ? top : ref, keep = exp2_approx(ref - now);
-        ok = __all_sync(~0u, mbar_wait_bounded(o_done + 8 * i, (j - 1) & 1, a.limit, a.err, kDevErrTimeoutEpilogue));
-        if (!ok) break;
+    const uint32_t stage = s_out + warp * 4096;  // 64 channels of the warp's rows
+    uint32_t done = 0, units_of = 0;  // halves and units so far
+    for (int r = 0;; ++r) {
+      const TcUnit u = unit_at(r, kCode);
+      if (!u.ok) break;
+      const int n = 2 * unit_steps(u, i, tokens), shift = u.s.lk - u.s.lq;
+      const int first = u.token0 + i * tokens, token = first + of, head = u.kv * ratio + row - of * ratio;
+      if (first >= u.s.lq) continue;
+      const bool mine = of < tokens && token < u.s.lq;
+      const int seen = mine ? max(0, token + shift + 1) : 0;
+      float ref = 0.0f, sum = 0.0f;
+      for (int t = 0; t < n; ++t) {
+        const uint32_t half = t & 1, t_h = t_s + 64 * half;
+        if (!wait(s_full + 16 * i + 8 * half, (done + t) >> 1 & 1, kCode)) break;
         tc_fence_after();
-#pragma unroll 1
-        for (int k = 0; k < D; k += 32) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(t_o + k, o);
-          tmem_ld_wait();
+        uint32_t raw[2][32];
+        tmem_ld_32x32b_x32(t_h, raw[0]);
+        tmem_ld_32x32b_x32(t_h + 32, raw[1]);
+        tmem_ld_wait();
+        loaded(raw[0]);
+        loaded(raw[1]);
+        const auto s = [&](int k) { return __uint_as_float(raw[k / 32][k % 32]); };
+        const int limit = seen - t * kHalf;
+        if (__any_sync(~0u, limit < kHalf)) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-          tmem_st_32x32b_x32(t_o + k, o);
+          for (int k = 0; k < kHalf; ++k)
+            if (k >= limit) raw[k / 32][k % 32] = 0xFF800000u;
         }
-        sum *= keep;
-        ref = now;
-      }
-      const float2 by = both(c), less = both(kLift - ref);
-      float2 add[2] = {both(0.0f), both(0.0f)};
+        float m[2] = {s(0), s(1)};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+        for (int k = 2; k < kHalf - 2; k += 4) m[0] = max3(m[0], s(k), s(k + 1)), m[1] = max3(m[1], s(k + 2), s(k + 3));
+        const float top = max3(fmaxf(m[0], m[1]), s(kHalf - 2), s(kHalf - 1)) * c;  // -inf: nothing seen here
+        if (t == 0) {
+          ref = top == -INFINITY ? 0.0f : top;
+        } else if (__any_sync(~0u, top - ref > kSlack)) {
+          const float now = top - ref > kSlack ? top : ref, keep = exp2_approx(ref - now);
+          if (!wait(o_done + 8 * i, (done + t - 1) & 1, kCode)) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int k = 0; k < D; k += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(t_o + k, o);
+            tmem_ld_wait();
+            loaded(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+            tmem_st_32x32b_x32(t_o + k, o);
+          }
+          sum *= keep;
+          ref = now;
+        }
+        const float less = kLift - ref;
+        float add[4] = {};
         uint32_t w[32];
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
-          const float2 x = fma2(make_float2(s(64 * h + 2 * k), s(64 * h + 2 * k + 1)), by, less);
-          const float2 p = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-          add[k & 1] = add2(add[k & 1], p);
-          w[k] = pack_16<T>(p.x, p.y);
+          const float x = exp2_approx(fmaf(s(2 * k), c, less)), y = exp2_approx(fmaf(s(2 * k + 1), c, less));
+          add[2 * (k & 1)] += x;
+          add[2 * (k & 1) + 1] += y;
+          w[k] = pack_16<T>(x, y);
         }
-        tmem_st_32x32b_x32(t_s + 32 * h, w);
+        tmem_st_32x32b_x32(t_h, w);
+        sum += (add[0] + add[1]) + (add[2] + add[3]);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 16 * i + 8 * half);
       }
-      const float2 both_sums = add2(add[0], add[1]);
-      sum += both_sums.x + both_sums.y;
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + 8 * i);
-    }
-    if (n && ok) ok = __all_sync(~0u, mbar_wait_bounded(o_done + 8 * i, (n - 1) & 1, a.limit, a.err, kDevErrTimeoutEpilogue));
-    tc_fence_after();
-    if (ok && u.ok) {
-      T* out = static_cast<T*>(a.out) + (static_cast<long long>(u.s.q0 + token) * a.hq + head) * a.d;
+      done += n;
+      if (n) wait(ended + 8 * i, units_of++ & 1, kCode);
+      if (!ok) break;
+      tc_fence_after();
+      // Results: whole rows by way of the warp's own shared memory (16-byte piece p of a row's 128 bytes at p ^ (row % 8)), so that
+      // 8 lanes write 128 bytes together; a thread that writes its own row takes as many cycles as it has sectors.
       const float scale = seen ? 1.0f / sum : 0.0f;
-      bool fine = sum > 0.0f && sum < INFINITY;
-      const bool wide = a.d % 16 == 0 && !(reinterpret_cast<uintptr_t>(a.out) & 31u);
+      const long long at = (static_cast<long long>(u.s.q0 + token) * a.hq + head) * a.d;
+      float2 zero = both(0.0f);  // stays so while all results are finite
 #pragma unroll 1
-      for (int k = 0; k < D; k += 32) {
-        uint32_t o[32];
-        if (n) {
-          tmem_ld_32x32b_x32(t_o + k, o);
-          tmem_ld_wait();
-        }
+      for (int ch = 0; 64 * ch < a.d; ++ch) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 16) {
-          uint32_t y[8];
+        for (int k = 0; k < 64; k += 32) {
+          uint32_t o[32], y[16];
+          if (n) {
+            tmem_ld_32x32b_x32(t_o + 64 * ch + k, o);
+            tmem_ld_wait();
+            loaded(o);
+          }
 #pragma unroll
-          for (int f = 0; f < 8; ++f) {
-            const float2 v = seen ? make_float2(__uint_as_float(o[e + 2 * f]) * scale, __uint_as_float(o[e + 2 * f + 1]) * scale) : both(0.0f);
-            if (k + e + 2 * f < a.d) fine = fine && fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY;
-            y[f] = pack_16<T>(v.x, v.y);
+          for (int f = 0; f < 16; ++f) {
+            const float2 v = mul2(make_float2(__uint_as_float(o[2 * f]), __uint_as_float(o[2 * f + 1])), both(scale));
+            zero = fma2(v, both(0.0f), zero);
+            y[f] = seen ? pack_16<T>(v.x, v.y) : 0u;
           }
-          if (mine && k + e < a.d) {
-            if (wide) {
-              store_32(out + k + e, y);
-            } else {
-              *reinterpret_cast<uint4*>(out + k + e) = make_uint4(y[0], y[1], y[2], y[3]);
-              if (k + e + 8 < a.d) *reinterpret_cast<uint4*>(out + k + e + 8) = make_uint4(y[4], y[5], y[6], y[7]);
-            }
-          }
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + (((k / 8 + f) ^ (lane & 7)) << 4)),
+                         "r"(y[4 * f]), "r"(y[4 * f + 1]), "r"(y[4 * f + 2]), "r"(y[4 * f + 3])
+                         : "memory");
         }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int from = 4 * k + lane / 8, piece = lane & 7;
+          const long long to = __shfl_sync(~0u, mine ? at : -1, from);
+          uint4 v;
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                       : "r"(stage + from * 128 + ((piece ^ (from & 7)) << 4))
+                       : "memory");
+          if (to >= 0 && 64 * ch + 8 * piece < a.d) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to + 64 * ch + 8 * piece) = v;
+        }
+        __syncwarp();
       }
+      const bool fine = !seen || (sum > 0.0f && sum < INFINITY && zero.x == 0.0f && zero.y == 0.0f);
       if (a.lse && mine)
         a.lse[static_cast<long long>(u.s.q0 + token) * a.hq + head] = seen ? (ref - kLift + log2f(sum)) * (1.0f / kLog2e) : -INFINITY;
-      unsigned again = __ballot_sync(~0u, seen && !fine);
-      for (; again; again &= again - 1) {
-        const int from = __ffs(again) - 1;
+      for (unsigned rows = __ballot_sync(~0u, !fine); rows; rows &= rows - 1) {
+        const int from = __ffs(rows) - 1;
         prompt_row_with_care<T>(a, u.s.q0 + __shfl_sync(~0u, token, from), __shfl_sync(~0u, head, from), u.s.k0,
                                 __shfl_sync(~0u, seen, from));
       }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 10) {
+      if (lane == 0) mbar_arrive(u_full);
+      for (int r = 1; more; ++r) {
+        if (r > 1 && !wait(u_empty + 8 * (r & 1), ((r >> 1) - 1) & 1, kDevErrTimeoutProducer)) break;
+        more = find(r, units + (r & 1));
+        if (lane == 0) mbar_arrive(u_full + 8 * (r & 1));
+        __syncwarp();
+      }
+    } else if (warp == 8) {
+      uint32_t n = 0, loads[2] = {0, 0};
+      for (int r = 0;; ++r) {
+        const TcUnit u = unit_at(r, kDevErrTimeoutProducer);
+        if (!u.ok) break;
+        const int kv = u.kv;
+        int all = 0;
+        bool go = true;
+  #pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int steps = unit_steps(u, i, tokens);
+          all = max(all, steps);
+          if (!steps || !go) continue;
+          if (loads[i]) go = wait(q_empty + 8 * i, (loads[i] - 1) & 1, kDevErrTimeoutProducer);
+          if (!go) continue;
+          mbar_arrive_expect_tx_elect(q_full + 8 * i, static_cast<uint32_t>(kChunks * tokens * ratio) * 128u);
+          for (int c = 0; c < kChunks; ++c)
+            tma_load_3d_elect(s_q + i * S::kTile + c * 16384, &tm_q, q_full + 8 * i, 64 * c, kv * ratio, u.s.q0 + u.token0 + i * tokens);
+          ++loads[i];
+        }
+        for (int k = 0; k < 2 * all && go; ++k, ++n) {  // K 0, V 0, K 1, V 1, ...
+          const uint32_t st = n % S::kStages;
+          if (n >= S::kStages) go = wait(empty0 + 8 * st, (n / S::kStages - 1) & 1, kDevErrTimeoutProducer);
+          if (!go) break;
+          mbar_arrive_expect_tx_elect(full0 + 8 * st, S::kTile);
+          for (int c = 0; c < kChunks; ++c)
+            tma_load_3d_elect(s_ring + st * S::kTile + c * 16384, k & 1 ? &tm_v : &tm_k, full0 + 8 * st, 64 * c, kv, u.s.k0 + k / 2 * kTcKeys);
+        }
+        if (!go) break;
+      }
+      if (!ok) {  // given up: what is on its way lands before the block ends
+        for (uint32_t i = n > S::kStages ? n - S::kStages : 0; i < n; ++i)
+          mbar_wait_bounded(full0 + 8 * (i % S::kStages), (i / S::kStages) & 1, a.limit, a.err, kDevErrTimeoutProducer);
+        for (int i = 0; i < 2; ++i)
+          if (loads[i]) mbar_wait_bounded(q_full + 8 * i, (loads[i] - 1) & 1, a.limit, a.err, kDevErrTimeoutProducer);
+        __syncwarp();
+      }
+    } else {
+      // A warp for each tile issues its products: QK of the next half while the weights of this one are made, then PV.
+      constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
+      constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | ((128u >> 4) << 24);
+      const uint32_t qk_desc = kDesc | ((kHalf >> 3) << 17) | (negate << 13);
+      const uint32_t pv_desc = kDesc | ((static_cast<uint32_t>(D) >> 3) << 17) | (1u << 16);  // V: channels contiguous
+      constexpr int kCode = kDevErrTimeoutMma;
+      const uint64_t q_at = make_smem_desc(s_q, 16, 1024, 2), k_at = make_smem_desc(s_ring, 16, 1024, 2),
+                     v_at = make_smem_desc(s_ring, 16384, 1024, 2);
+      const int i = warp == 9 ? 0 : 1;
+      const uint32_t t_s = tmem + i * 128, t_o = tmem + 256 + i * D;
+      const uint64_t q = q_at + i * (S::kTile / 16);
+      uint32_t base = 0, done = 0, units_of = 0;  // ring tiles, halves and units so far
+      auto tile_wait = [&](uint32_t n) { return wait(full0 + 8 * (n % S::kStages), (n / S::kStages) & 1, kCode); };
+      auto release = [&](uint32_t n) { tc_commit_elect(empty0 + 8 * (n % S::kStages)); };
+      for (int r = 0; ok; ++r) {
+        const TcUnit u = unit_at(r, kCode);
+        if (!u.ok) break;
+        const int steps = unit_steps(u, i, tokens), all = max(steps, unit_steps(u, 1 - i, tokens)), n = 2 * steps;
+        auto qk = [&](int t) {
+          const uint32_t at = base + (t & ~1);
+          if (!(t & 1) && !tile_wait(at)) return;
+          const uint64_t k = k_at + at % S::kStages * (S::kTile / 16) + (t & 1) * (kHalf * 8);
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) tc_mma_f16_x4_elect(t_s + (t & 1) * kHalf, q + c * 1024, k + c * 1024, qk_desc, c);
+          tc_commit_elect(s_full + 16 * i + 8 * (t & 1));
+          if (t & 1) release(at);
+          if (t + 1 == n) tc_commit_elect(q_empty + 8 * i);
+        };
+        if (n) {
+          // the last unit's weights have been read: scores may take their place
+          if (units_of) wait(ended + 8 * i, (units_of - 1) & 1, kCode);
+          if (wait(q_full + 8 * i, units_of++ & 1, kCode)) qk(0);
+        }
+        for (int t = 0; t < n && ok; ++t) {
+          if (t + 1 < n) {  // in the place of the weights before the last
+            if (t && !wait(o_done + 8 * i, (done + t - 1) & 1, kCode)) break;
+            qk(t + 1);
+          }
+          if (!(t & 1)) tile_wait(base + t + 1);
+          if (!wait(p_full + 16 * i + 8 * (t & 1), (done + t) >> 1 & 1, kCode)) break;
+          tc_fence_after();
+          tc_mma_f16_ts_x4_elect(t_o, t_s + (t & 1) * kHalf, v_at + (base + (t | 1)) % S::kStages * (S::kTile / 16) + (t & 1) * 512,
+                                 pv_desc, t);
+          tc_commit_elect(o_done + 8 * i);
+          if (t & 1) release(base + t);
+          if (t + 1 == n) tc_commit_elect(ended + 8 * i);
+        }
+        for (int k = n; k < 2 * all && ok; ++k)  // the other tile's alone
+          if (tile_wait(base + k)) release(base + k);
+        base += 2 * all;
+        done += n;
+      }
+      tc_commit_elect(drain + 8 * i);
+      mbar_wait_bounded(drain + 8 * i, 0, a.limit, a.err, kCode);
+      __syncwarp();
     }
   }
   tc_fence_before();
