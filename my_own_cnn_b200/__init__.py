@@ -1,7 +1,8 @@
 """my_own_cnn_b200: B200-native (sm_100a) int8 NHWC convolution and batched GEMM, with the
 reference's fp32 conv (forward and both gradients) and fp32 bmm on the same tensor-core engine,
-and decoder operators with 4-bit storage (weight-only linear, per-head norm with rotation, a 4-bit
-paged key / value cache and the attention over it).
+decoder operators with 4-bit storage (weight-only linear, per-head norm with rotation, a 4-bit
+paged key / value cache and the attention over it), and operators of whole prompts in 8 bits (RMS norm
+with the residual into 8-bit rows, linear layers of them, causal attention over packed prompts).
 
 A from-scratch implementation of the quantized conv / bmm hot path of NikitaYak02/my_own_cnn
 behind the reference's own entry points.  The kernels live in ``libb200q.so`` (C ABI:
@@ -22,7 +23,7 @@ from .rope import qk_norm_rope, qk_norm_rope_bprop, rope_table
 from .kv4 import KV4Cache, kv4_append, kv4_attention, kv4_read
 from .s8 import S8Rows, linear_s8, quantize_s8, rms_norm_s8
 from .prompt import prompt_attention
-from .decoder import W4Attention
+from .decoder import S8Attention, W4Attention
 from ._lib import B200QError, device_error, last_path, set_path_policy, tc_launch_count
 
 __all__ = [
@@ -36,4 +37,5 @@ __all__ = [
     "bmm_bprop", "W4Weight", "linear_w4", "pack_w4", "quantize_w4", "qk_norm_rope", "qk_norm_rope_bprop", "rope_table",
     "KV4Cache", "kv4_append", "kv4_attention", "kv4_read", "W4Attention", "device_error",
     "S8Rows", "quantize_s8", "rms_norm_s8", "linear_s8", "prompt_attention",
+    "S8Attention",
 ]

@@ -8,7 +8,8 @@
 // in the low byte of its bits.
 //
 // Bytes bound it: x (and the residual) in, the sum and one byte an element out.  A row lies in the registers of W warps from its only
-// read to its writes, 16 bytes a load and 16 elements (fp32) or 8 to 32 (16 bits) a lane; both reductions meet in one barrier.
+// read to its writes, 16 bytes a load and 16 or 32 elements a lane; both reductions meet in one
+// barrier.
 #include <algorithm>
 #include <cmath>
 
@@ -39,7 +40,6 @@ constexpr float kSmallest = 0x1p-119f;  // rows with nothing larger are zeros: 1
 // VEC elements in memory.
 template <typename T, int VEC>
 struct Chunk {
-  static constexpr int kWords = VEC * static_cast<int>(sizeof(T)) / 4;
   static __device__ __forceinline__ void load(const T* p, float (&v)[VEC]) {
     if constexpr (VEC == 1) {
       v[0] = to_f32(*p);
@@ -292,35 +292,35 @@ struct ReadArgs {
   Divisor chunks;  // of a row
 };
 
-// VEC codes a thread.
+// A thread has one piece of VEC codes; where rows are not aligned 8 codes that lie 32 apart.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) read_s8_kernel(ReadArgs a, uint32_t units) {
   wait_for_previous();
-  const uint32_t unit = blockIdx.x * 256u + threadIdx.x;
+  constexpr int kApart = VEC == 1 ? 8 : 1;
+  const uint32_t unit = VEC == 1 ? (blockIdx.x * 256u + threadIdx.x) / 32 : blockIdx.x * 256u + threadIdx.x;
   if (unit >= units) return;
   const uint32_t row = a.chunks.of(unit);
-  const int c = static_cast<int>(unit - row * a.chunks.d) * VEC;
+  const int c = VEC == 1 ? static_cast<int>(unit - row * a.chunks.d) * 256 + threadIdx.x % 32 : static_cast<int>(unit - row * a.chunks.d) * VEC;
   const int8_t* p = a.codes + static_cast<long long>(row) * a.ldc + c;
   T* y = static_cast<T*>(a.y) + static_cast<long long>(row) * a.ldy + c;
   const float s = __ldg(a.scales + row);
   if constexpr (VEC == 1) {
-    *y = from_f32<T>(static_cast<float>(*p) * s);
+    int8_t code[kApart];
+#pragma unroll
+    for (int i = 0; i < kApart; ++i) code[i] = c + 32 * i < a.n ? p[32 * i] : int8_t{0};
+#pragma unroll
+    for (int i = 0; i < kApart; ++i)
+      if (c + 32 * i < a.n) y[32 * i] = from_f32<T>(static_cast<float>(code[i]) * s);
   } else {
-    constexpr int kPart = 16 / sizeof(T);  // elements of a 16-byte store
-    int8_t code[VEC];
-    if constexpr (VEC == 16)
-      *reinterpret_cast<uint4*>(code) = *reinterpret_cast<const uint4*>(p);
-    else if constexpr (VEC == 8)
+    alignas(8) int8_t code[VEC];
+    if constexpr (VEC == 8)
       *reinterpret_cast<uint2*>(code) = *reinterpret_cast<const uint2*>(p);
     else
       *reinterpret_cast<uint32_t*>(code) = *reinterpret_cast<const uint32_t*>(p);
+    float v[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; i += kPart) {
-      float v[kPart];
-#pragma unroll
-      for (int j = 0; j < kPart; ++j) v[j] = static_cast<float>(code[i + j]) * s;
-      Chunk<T, kPart>::store(y + i, v);
-    }
+    for (int j = 0; j < VEC; ++j) v[j] = static_cast<float>(code[j]) * s;
+    Chunk<T, VEC>::store(y, v);
   }
 }
 
@@ -375,8 +375,12 @@ int rows_s8(const b200q_rows_s8_args* p, bool norm, void* stream) {
                     !((reinterpret_cast<uintptr_t>(a.codes) | (a.t == 1 ? 0 : a.ldc)) & (vec - 1));
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   int rc = B200Q_OK;
-  B200Q_DISPATCH_FTYPE(ftype, rc = wide ? launch_warps<T, 16 / sizeof(T), sizeof(T) == 4 ? 4 : 2>(a, norm, cs)
-                                        : launch_warps<T, 1, 16>(a, norm, cs));
+  // 16 elements a lane up to eight warps a row, then 32: a block of 16 or 32 warps waits long at its barrier for the row's slowest (us:
+  // 500 x 16384 bf16 10.2 with 16, 7.0 with 32; 30000 x 512 fp16 11.9 with 16, 16.5 with 32; 1021 x 5004 fp32 8.1 and 6.6).
+  constexpr int kFew = 4096;
+  B200Q_DISPATCH_FTYPE(ftype, rc = !wide          ? launch_warps<T, 1, 16>(a, norm, cs)
+                                   : a.n <= kFew ? launch_warps<T, 16 / sizeof(T), sizeof(T)>(a, norm, cs)
+                                                 : launch_warps<T, 16 / sizeof(T), 2 * sizeof(T)>(a, norm, cs));
   if (rc == B200Q_OK) host_set_path(21);
   return rc;
 }
@@ -401,10 +405,11 @@ extern "C" int b200q_read_s8(const int8_t* codes, long long ldc, const float* sc
   const int size = ftype == B200Q_F32 ? 4 : 2, vec = 16 / size;
   const bool aligned = n % vec == 0 && !(reinterpret_cast<uintptr_t>(y) & 15u) && (t == 1 || ldy % vec == 0) &&
                        !((reinterpret_cast<uintptr_t>(codes) | (t == 1 ? 0 : ldc)) & (vec - 1));
-  const long long units = static_cast<long long>(t) * (aligned ? n / vec : n);
+  const int chunks = aligned ? n / vec : (n + 255) / 256, per_block = aligned ? 256 : 8;
+  const long long units = static_cast<long long>(t) * chunks;
   if (units > 0x7fffff00ll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many elements");
-  const ReadArgs a{codes, ldc, scales, y, ldy, t, n, Divisor(static_cast<uint32_t>(aligned ? n / vec : n))};
-  const dim3 grid(static_cast<unsigned>((units + 255) / 256));
+  const ReadArgs a{codes, ldc, scales, y, ldy, t, n, Divisor(static_cast<uint32_t>(chunks))};
+  const dim3 grid(static_cast<unsigned>((units + per_block - 1) / per_block));
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   int rc = B200Q_OK;
   B200Q_DISPATCH_FTYPE(ftype, rc = host_launch("read_s8_kernel launch", aligned ? read_s8_kernel<T, 16 / sizeof(T)> : read_s8_kernel<T, 1>,

@@ -44,6 +44,17 @@ class S8Rows:
         return S8Rows(torch.empty(lead + (-(-k // 16) * 16,), dtype=torch.int8, device=device),
                       torch.empty(lead, dtype=torch.float32, device=device), k)
 
+    @staticmethod
+    def _like(x: torch.Tensor) -> "S8Rows":
+        """Uninitialised rows for the values of x, beside it: nothing to check."""
+        shape = x.shape
+        lead, k = shape[:-1], shape[-1]
+        r = S8Rows.__new__(S8Rows)
+        r.k, r._pitch = k, -(-k // 16) * 16
+        r.codes = x.new_empty(lead + (r._pitch,), dtype=torch.int8)
+        r.scales = x.new_empty(lead, dtype=torch.float32)
+        return r
+
     @property
     def shape(self) -> torch.Size:
         return self.scales.shape + (self.k,)
@@ -94,7 +105,7 @@ def _own_rows(x, n, what):
 
 def _out_rows(out, shape, like):
     if out is None:
-        return S8Rows.empty(shape, like.device)
+        return S8Rows._like(like)
     if out.shape != shape or not out.codes.is_cuda:
         raise RuntimeError(f"out must be 8-bit rows of {list(shape)} on the device, got {list(out.shape)}")
     return out
