@@ -85,39 +85,62 @@ struct MmaShape {
   static constexpr int kSmem = kTerms * (kQ + 2 * kK);
 };
 
-// `rows` rows of D channels (zeros past d and where there is no row) into the terms' tiles.
-template <typename T, int D, typename P>
-__device__ __forceinline__ void load_tile(uint32_t to, int term, int rows, int d, bool wide, P row_at) {
-  constexpr int kTerms = Terms<T>::kCount, kPitch = MmaShape<T, D>::kPitch;
-  for (int i = threadIdx.x; i < rows * (D / 4); i += kMmaThreads) {
-    const int r = i / (D / 4), c = i % (D / 4) * 4;
-    const T* p = row_at(r);
-    float x[4] = {};
-    if (p) {
-      if (wide && c + 4 <= d) {
-        if constexpr (sizeof(T) == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p + c);
-          x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(p + c);
-          const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] = to_f32(e[j]);
-        }
+// Four channels from c on of a row (null: zeros; past d too).
+template <typename T>
+__device__ __forceinline__ float4 four_of(const T* p, int c, int d, bool wide) {
+  float x[4] = {};
+  if (p) {
+    if (wide && c + 4 <= d) {
+      if constexpr (sizeof(T) == 4) {
+        return *reinterpret_cast<const float4*>(p + c);
       } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p + c);
+        const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + j < d) x[j] = to_f32(p[c + j]);
+        for (int j = 0; j < 4; ++j) x[j] = to_f32(e[j]);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < d) x[j] = to_f32(p[c + j]);
     }
+  }
+  return make_float4(x[0], x[1], x[2], x[3]);
+}
+
+// A thread's pieces of `ROWS` rows of D channels: from memory into registers, and cut into the terms' tiles.
+template <typename T, int D, int ROWS>
+struct Tile {
+  static constexpr int kPieces = ROWS * (D / 4) / kMmaThreads;
+  template <typename P>
+  static __device__ __forceinline__ void fetch(float4 (&x)[kPieces], int d, bool wide, P row_at) {
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) {
+      const int i = threadIdx.x + k * kMmaThreads;
+      x[k] = four_of<T>(row_at(i / (D / 4)), i % (D / 4) * 4, d, wide);
+    }
+  }
+  static __device__ __forceinline__ void put(uint32_t to, int term, const float4& x, int i) {
+    constexpr int kTerms = Terms<T>::kCount;
     uint32_t lo[kTerms], hi[kTerms];
-    Terms<T>::cut(x[0], x[1], lo);
-    Terms<T>::cut(x[2], x[3], hi);
+    Terms<T>::cut(x.x, x.y, lo);
+    Terms<T>::cut(x.z, x.w, hi);
 #pragma unroll
     for (int t = 0; t < kTerms; ++t)
-      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + t * term + r * kPitch + c * 2), "r"(lo[t]), "r"(hi[t]) : "memory");
+      asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + t * term + i / (D / 4) * (D * 2 + 16) + i % (D / 4) * 8), "r"(lo[t]),
+                   "r"(hi[t])
+                   : "memory");
   }
-}
+  static __device__ __forceinline__ void put(uint32_t to, int term, const float4 (&x)[kPieces]) {
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) put(to, term, x[k], threadIdx.x + k * kMmaThreads);
+  }
+  template <typename P>
+  static __device__ __forceinline__ void load(uint32_t to, int term, int d, bool wide, P row_at) {
+    for (int i = threadIdx.x; i < ROWS * (D / 4); i += kMmaThreads)
+      put(to, term, four_of<T>(row_at(i / (D / 4)), i % (D / 4) * 4, d, wide), i);
+  }
+};
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_constant__ PromptArgs a, int wide) {
@@ -133,7 +156,7 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
   const int ratio = static_cast<int>(a.ratio.d), shift = u.s.lk - u.s.lq;
   const int rows = u.s.lq * ratio, row0 = u.tile * kRows;  // of this key head's rows in the sequence
   const uint32_t s_q = shared_address(smem), s_k = s_q + kTerms * S::kQ, s_v = s_k + kTerms * S::kK;
-  load_tile<T, D>(s_q, S::kQ, kRows, a.d, wide, [&](int r) -> const T* {
+  Tile<T, D, kRows>::load(s_q, S::kQ, a.d, wide, [&](int r) -> const T* {
     if (row0 + r >= rows) return nullptr;
     const int token = static_cast<int>(a.ratio.of(row0 + r)), head = kv * ratio + row0 + r - token * ratio;
     return static_cast<const T*>(a.q) + (u.s.q0 + token) * a.q_ts + head * a.q_hs;
@@ -149,14 +172,34 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
   const int most = min(u.s.lk, static_cast<int>(a.ratio.of(last_row)) + shift + 1);
   const float c = a.scale * kLog2e;
   float o[D / 8][4] = {}, top[2] = {-INFINITY, -INFINITY}, sum[2] = {};
+  // Heads of up to 64 channels: the next keys and values are on their way, in registers, while these are worked on.
+  using KV = Tile<T, D, kKeys>;
+  constexpr bool kAhead = D == 64;
+  float4 next_k[kAhead ? KV::kPieces : 1], next_v[kAhead ? KV::kPieces : 1];
+  const auto key_rows = [&](const void* base, long long ts, long long hs, int j0) {
+    return [=](int r) -> const T* {
+      return j0 + r < u.s.lk ? static_cast<const T*>(base) + (u.s.k0 + j0 + r) * ts + kv * hs : nullptr;
+    };
+  };
+  if constexpr (kAhead) {
+    if (most > 0) {
+      KV::fetch(next_k, a.d, wide, key_rows(a.k, a.k_ts, a.k_hs, 0));
+      KV::fetch(next_v, a.d, wide, key_rows(a.v, a.v_ts, a.v_hs, 0));
+    }
+  }
   for (int j0 = 0; j0 < most; j0 += kKeys) {
     __syncthreads();
-    load_tile<T, D>(s_k, S::kK, kKeys, a.d, wide, [&](int r) -> const T* {
-      return j0 + r < u.s.lk ? static_cast<const T*>(a.k) + (u.s.k0 + j0 + r) * a.k_ts + kv * a.k_hs : nullptr;
-    });
-    load_tile<T, D>(s_v, S::kK, kKeys, a.d, wide, [&](int r) -> const T* {
-      return j0 + r < u.s.lk ? static_cast<const T*>(a.v) + (u.s.k0 + j0 + r) * a.v_ts + kv * a.v_hs : nullptr;
-    });
+    if constexpr (kAhead) {
+      KV::put(s_k, S::kK, next_k);
+      KV::put(s_v, S::kK, next_v);
+      if (j0 + kKeys < most) {
+        KV::fetch(next_k, a.d, wide, key_rows(a.k, a.k_ts, a.k_hs, j0 + kKeys));
+        KV::fetch(next_v, a.d, wide, key_rows(a.v, a.v_ts, a.v_hs, j0 + kKeys));
+      }
+    } else {
+      KV::load(s_k, S::kK, a.d, wide, key_rows(a.k, a.k_ts, a.k_hs, j0));
+      KV::load(s_v, S::kK, a.d, wide, key_rows(a.v, a.v_ts, a.v_hs, j0));
+    }
     __syncthreads();
     float s[kKeys / 8][4] = {}, less[kTerms == 3 ? kKeys / 8 : 1][4] = {};
 #pragma unroll 2

@@ -101,10 +101,10 @@ struct TcUnit {
   int ok;
 };
 
-// Steps of 128 keys that tile i of a unit needs: its last token's.
-__device__ __forceinline__ int unit_steps(const TcUnit& u, int i, int tokens) {
+// Halves (of 64 keys) that tile i of a unit needs: its last token's.
+__device__ __forceinline__ int unit_halves(const TcUnit& u, int i, int tokens) {
   const int first = u.token0 + i * tokens, last = min(u.s.lq, first + tokens) - 1;
-  return first < u.s.lq ? (max(0, last + u.s.lk - u.s.lq + 1) + kTcKeys - 1) / kTcKeys : 0;
+  return first < u.s.lq ? (max(0, last + u.s.lk - u.s.lq + 1) + kHalf - 1) / kHalf : 0;
 }
 
 template <typename T, int D>
@@ -196,11 +196,11 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
     const int of = static_cast<int>(a.ratio.of(row));
     const float c = fabsf(a.scale) * kLog2e;
     const uint32_t stage = s_out + warp * 4096;  // 64 channels of the warp's rows
-    uint32_t done = 0, units_of = 0;  // halves and units so far
+    uint32_t done = 0, units_of = 0, used = 0;  // halves and units so far; a bit for each half's buffer: its next phase
     for (int r = 0;; ++r) {
       const TcUnit u = unit_at(r, kCode);
       if (!u.ok) break;
-      const int n = 2 * unit_steps(u, i, tokens), shift = u.s.lk - u.s.lq;
+      const int n = unit_halves(u, i, tokens), shift = u.s.lk - u.s.lq;
       const int first = u.token0 + i * tokens, token = first + of, head = u.kv * ratio + row - of * ratio;
       if (first >= u.s.lq) continue;
       const bool mine = of < tokens && token < u.s.lq;
@@ -208,7 +208,8 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
       float ref = 0.0f, sum = 0.0f;
       for (int t = 0; t < n; ++t) {
         const uint32_t half = t & 1, t_h = t_s + 64 * half;
-        if (!wait(s_full + 16 * i + 8 * half, (done + t) >> 1 & 1, kCode)) break;
+        if (!wait(s_full + 16 * i + 8 * half, used >> half & 1, kCode)) break;
+        used ^= 1u << half;
         tc_fence_after();
         uint32_t raw[2][32];
         tmem_ld_32x32b_x32(t_h, raw[0]);
@@ -337,9 +338,9 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
         bool go = true;
   #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int steps = unit_steps(u, i, tokens);
-          all = max(all, steps);
-          if (!steps || !go) continue;
+          const int halves = unit_halves(u, i, tokens);
+          all = max(all, (halves + 1) / 2);
+          if (!halves || !go) continue;
           if (loads[i]) go = wait(q_empty + 8 * i, (loads[i] - 1) & 1, kDevErrTimeoutProducer);
           if (!go) continue;
           mbar_arrive_expect_tx_elect(q_full + 8 * i, static_cast<uint32_t>(kChunks * tokens * ratio) * 128u);
@@ -376,13 +377,13 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
       const int i = warp == 9 ? 0 : 1;
       const uint32_t t_s = tmem + i * 128, t_o = tmem + 256 + i * D;
       const uint64_t q = q_at + i * (S::kTile / 16);
-      uint32_t base = 0, done = 0, units_of = 0;  // ring tiles, halves and units so far
+      uint32_t base = 0, done = 0, units_of = 0, used = 0;  // ring tiles, halves and units so far; the buffers' phases
       auto tile_wait = [&](uint32_t n) { return wait(full0 + 8 * (n % S::kStages), (n / S::kStages) & 1, kCode); };
       auto release = [&](uint32_t n) { tc_commit_elect(empty0 + 8 * (n % S::kStages)); };
       for (int r = 0; ok; ++r) {
         const TcUnit u = unit_at(r, kCode);
         if (!u.ok) break;
-        const int steps = unit_steps(u, i, tokens), all = max(steps, unit_steps(u, 1 - i, tokens)), n = 2 * steps;
+        const int n = unit_halves(u, i, tokens), all = (max(n, unit_halves(u, 1 - i, tokens)) + 1) / 2;
         auto qk = [&](int t) {
           const uint32_t at = base + (t & ~1);
           if (!(t & 1) && !tile_wait(at)) return;
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) tc_mma_f16_x4_elect(t_s + (t & 1) * kHalf, q + c * 1024, k + c * 1024, qk_desc, c);
           tc_commit_elect(s_full + 16 * i + 8 * (t & 1));
-          if (t & 1) release(at);
+          if ((t & 1) || t + 1 == n) release(at);
           if (t + 1 == n) tc_commit_elect(q_empty + 8 * i);
         };
         if (n) {
@@ -404,15 +405,16 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
             qk(t + 1);
           }
           if (!(t & 1)) tile_wait(base + t + 1);
-          if (!wait(p_full + 16 * i + 8 * (t & 1), (done + t) >> 1 & 1, kCode)) break;
+          if (!wait(p_full + 16 * i + 8 * (t & 1), used >> (t & 1) & 1, kCode)) break;
+          used ^= 1u << (t & 1);
           tc_fence_after();
           tc_mma_f16_ts_x4_elect(t_o, t_s + (t & 1) * kHalf, v_at + (base + (t | 1)) % S::kStages * (S::kTile / 16) + (t & 1) * 512,
                                  pv_desc, t);
           tc_commit_elect(o_done + 8 * i);
-          if (t & 1) release(base + t);
+          if ((t & 1) || t + 1 == n) release(base + (t | 1));
           if (t + 1 == n) tc_commit_elect(ended + 8 * i);
         }
-        for (int k = n; k < 2 * all && ok; ++k)  // the other tile's alone
+        for (int k = (n + 1) / 2 * 2; k < 2 * all && ok; ++k)  // the other tile's alone
           if (tile_wait(base + k)) release(base + k);
         base += 2 * all;
         done += n;
