@@ -18,8 +18,8 @@ struct PromptArgs {
   float* lse;  // [tq][hq], or null
   int b, tq, tk, hq, hk, d;
   Divisor ratio;   // hq / hk
-  int tile_rows;   // rows (token, head of the group) of a tile; a tile holds whole tokens where tile_tokens is not 0
-  int tile_tokens;
+  int row_scale;   // a tile holds tile.d whole tokens (1), or tile.d rows (token, head of the group; hq / hk)
+  Divisor tile;
   long long most_units;  // key heads times tiles, as many as there may be
   float scale;
   int* err;
@@ -33,8 +33,7 @@ struct Sequence {
   int q0, lq, k0, lk;
   bool bad;
   __device__ __forceinline__ int tiles(const PromptArgs& a) const {
-    if (a.tile_tokens) return (lq + a.tile_tokens - 1) / a.tile_tokens;
-    return static_cast<int>((static_cast<long long>(lq) * a.ratio.d + a.tile_rows - 1) / a.tile_rows);
+    return static_cast<int>(a.tile.of(static_cast<uint32_t>(lq * a.row_scale + static_cast<int>(a.tile.d) - 1)));
   }
 };
 __device__ __forceinline__ Sequence sequence(const PromptArgs& a, int i) {
@@ -46,58 +45,81 @@ __device__ __forceinline__ Sequence sequence(const PromptArgs& a, int i) {
   return s;
 }
 
-// Tile `tile` of a sequence; the order is by tile number, largest first, so that the longest rows of keys start first
-// and the short ones fill up the end.  Found by bisection over n(l) = sum of max(0, tiles - l): the units from level l up.  A warp's work;
-// a lane keeps the first 32 sequences in registers.
+// Tile `tile` of a sequence; the units are in falling order of the keys that they see, in steps of 128, so that the longest start first and the
+// short ones fill up the end.  Found by bisection over the number of units with more than l steps.  A warp's work; a lane
+// keeps the first 32 sequences in registers.
 struct PromptUnit {
   Sequence s;
   int tile;
   bool ok;
 };
 __device__ __forceinline__ int warp_total(int v) { return __reduce_add_sync(~0u, v); }
+// A sequence's units, the last `above(l)` of which have more than l steps.
+struct Units {
+  int tiles, lq, shift, most;  // keys less queries; steps of the last unit
+  __device__ __forceinline__ Units(const PromptArgs& a, const Sequence& s)
+      : tiles(s.tiles(a)), lq(s.lq), shift(s.lk - s.lq), most(tiles ? max(0, s.lk + kUnitKeys - 1) / kUnitKeys : 0) {}
+  static constexpr int kUnitKeys = 128;
+  // all at l < 0; from the first tile whose end passes l steps on
+  __device__ __forceinline__ int above(const PromptArgs& a, int l) const {
+    if (l < 0) return tiles;
+    if (l >= most) return 0;
+    const int tokens = l * kUnitKeys - shift;  // that l steps reach
+    if (tokens < 0) return tiles;
+    return tiles - min(tiles, static_cast<int>(a.tile.of(static_cast<uint32_t>(min(tokens, lq) * a.row_scale))));
+  }
+};
 __device__ inline PromptUnit prompt_unit(const PromptArgs& a, int unit, bool report) {
   const int lane = threadIdx.x % 32;
   const Sequence first = sequence(a, lane);
-  const int tiles = first.tiles(a);
+  const Units mine(a, first);
   bool bad = first.bad;
-  int most = tiles, all = tiles;
+  int most = mine.most, all = mine.tiles;
   for (int i = 32 + lane; i < a.b; i += 32) {
     const Sequence s = sequence(a, i);
+    const Units u(a, s);
     bad |= s.bad;
-    most = max(most, s.tiles(a));
-    all += s.tiles(a);
+    most = max(most, u.most);
+    all += u.tiles;
   }
   if (report && bad) atomicCAS(a.err, 0, kDevErrBadStarts);
   PromptUnit u{};
   if (unit >= warp_total(all)) return u;
-  auto units_from = [&](int level) {
-    int n = max(0, tiles - level);
-    for (int i = 32 + lane; i < a.b; i += 32) n += max(0, sequence(a, i).tiles(a) - level);
+  auto units_above = [&](int l) {
+    int n = mine.above(a, l);
+    for (int i = 32 + lane; i < a.b; i += 32) n += Units(a, sequence(a, i)).above(a, l);
     return warp_total(n);
   };
-  int lo = 0, hi = __reduce_max_sync(~0u, most);  // units_from(lo) > unit >= units_from(hi) = 0 or more
-  int above = 0;
+  // units_above(lo) > unit >= units_above(hi) = longer: the unit has hi steps
+  int lo = -1, hi = __reduce_max_sync(~0u, most), longer = 0;
   while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2, n = units_from(mid);
+    const int mid = (lo + hi) / 2, n = units_above(mid);
     if (n > unit)
       lo = mid;
     else
-      hi = mid, above = n;
+      hi = mid, longer = n;
   }
-  int left = unit - above;  // of the sequences with more than lo tiles
+  int left = unit - longer;  // of the units with hi steps
   for (int i0 = 0; i0 < a.b; i0 += 32) {
     const Sequence s = i0 ? sequence(a, i0 + lane) : first;
-    const unsigned have = __ballot_sync(~0u, s.tiles(a) > lo);
-    const int n = __popc(have);
-    if (left < n) {
-      const int from = __ffs(__ballot_sync(~0u, (have >> lane & 1) && __popc(have & ((1u << lane) - 1)) == left)) - 1;
+    const Units v(a, s);
+    const int end = v.tiles - v.above(a, hi), n = v.above(a, lo) - v.above(a, hi);
+    int upto = n;  // with the sequences before
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int x = __shfl_up_sync(~0u, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned have = __ballot_sync(~0u, upto > left);
+    if (have) {
+      const int from = __ffs(have) - 1;
       u.s = {__shfl_sync(~0u, s.q0, from), __shfl_sync(~0u, s.lq, from), __shfl_sync(~0u, s.k0, from), __shfl_sync(~0u, s.lk, from),
              false};
-      u.tile = lo;
-      u.ok = true;
+      u.tile = __shfl_sync(~0u, end - 1 - (left - (upto - n)), from);
+      u.ok = u.tile >= 0;
       return u;
     }
-    left -= n;
+    left -= __shfl_sync(~0u, upto, 31);
   }
   return u;  // the starts changed meanwhile
 }

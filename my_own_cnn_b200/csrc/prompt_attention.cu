@@ -374,7 +374,7 @@ int launch_tc(const PromptArgs& a, int sms, int device, cudaStream_t cs) {
                            {64, box_heads, box_rows});
   };
   CUtensorMap tm_q, tm_k, tm_v;
-  int rc = map(&tm_q, a.q, a.hq, a.tq, a.q_ts, a.q_hs, a.ratio.d, static_cast<uint32_t>(a.tile_tokens / 2));
+  int rc = map(&tm_q, a.q, a.hq, a.tq, a.q_ts, a.q_hs, a.ratio.d, a.tile.d / 2);
   if (rc == B200Q_OK) rc = map(&tm_k, a.k, a.hk, a.tk, a.k_ts, a.k_hs, 1, kTcKeys);
   if (rc == B200Q_OK) rc = map(&tm_v, a.v, a.hk, a.tk, a.v_ts, a.v_hs, 1, kTcKeys);
   if (rc) return rc;
@@ -420,10 +420,10 @@ extern "C" int b200q_prompt_attention(const b200q_prompt_attention_args* p, void
   const int size = p->ftype == B200Q_F32 ? 4 : 2;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v);
   const bool tensor = tensor_core_takes(*p, ratio);
-  a.tile_rows = kRows;
-  a.tile_tokens = tensor ? 2 * static_cast<int>(128 / ratio) : 0;
+  a.tile = Divisor(tensor ? 2 * static_cast<uint32_t>(128 / ratio) : kRows);
+  a.row_scale = tensor ? 1 : static_cast<int>(ratio);
   // as many units as there may be: every sequence's last tile may be short
-  const long long tiles = (tensor ? p->tq / a.tile_tokens : p->tq * ratio / kRows) + std::min<long long>(p->b, p->tq);
+  const long long tiles = p->tq * static_cast<long long>(a.row_scale) / a.tile.d + std::min<long long>(p->b, p->tq);
   const long long units = a.most_units = tiles * p->hk;
   if (units > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
   int rc = B200Q_OK;

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
   TcUnit* units = reinterpret_cast<TcUnit*>(bars + 2 * kTcMaxStages + 23);  // two
   const uint32_t s_q = smem_u32(smem) + S::kHead, s_ring = s_q + 2 * S::kTile, s_out = s_ring + S::kStages * S::kTile;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int ratio = static_cast<int>(a.ratio.d), tokens = a.tile_tokens / 2;  // of one tile
+  const int ratio = static_cast<int>(a.ratio.d), tokens = static_cast<int>(a.tile.d) / 2;  // of one tile
 
   if (threadIdx.x == 256) {
     for (int i = 0; i < S::kStages; ++i) {
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
     const long long n = static_cast<long long>(r) * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
     PromptUnit u{};
     if (n < a.most_units) u = prompt_unit(a, static_cast<int>(n / a.hk), r == 0 && blockIdx.x == 0);
-    if (lane == 0) *to = {u.s, u.tile * a.tile_tokens, static_cast<int>(n % a.hk), u.ok};
+    if (lane == 0) *to = {u.s, u.tile * static_cast<int>(a.tile.d), static_cast<int>(n % a.hk), u.ok};
     return u.ok;
   };
   bool more = true;
