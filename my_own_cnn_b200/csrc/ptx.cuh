@@ -77,19 +77,6 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
   return true;
 }
 
-// The same without parking: the answer comes 300 clocks earlier, for issue slots.
-__device__ __forceinline__ bool mbar_spin_bounded(uint32_t bar, uint32_t parity, long long limit, int* err, int code) {
-  if (mbar_test(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_test(bar, parity)) {
-    if (clock64() - t0 > limit) {
-      atomicCAS(err, 0, code);
-      return false;
-    }
-  }
-  return true;
-}
-
 // --------------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");

@@ -12,6 +12,7 @@
 // barrier.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "host.h"
 #include "lowbit.cuh"
@@ -37,42 +38,49 @@ struct RowsArgs {
 constexpr uint32_t kInfBits = 0x7f800000u;
 constexpr float kSmallest = 0x1p-119f;  // rows with nothing larger are zeros: 127 / a stays finite
 
-// VEC elements in memory.
+// VEC elements in memory: one, or 16 bytes.
 template <typename T, int VEC>
 struct Chunk {
+  static __device__ __forceinline__ void unpack(const uint32_t (&w)[4], float (&v)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v[i] = __uint_as_float(w[i]);
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    }
+  }
   static __device__ __forceinline__ void load(const T* p, float (&v)[VEC]) {
     if constexpr (VEC == 1) {
       v[0] = to_f32(*p);
     } else {
       const uint4 b = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) {
-          v[i] = __uint_as_float(w[i]);
-        } else {
-          const T* e = reinterpret_cast<const T*>(&w[i]);
-          v[2 * i] = to_f32(e[0]);
-          v[2 * i + 1] = to_f32(e[1]);
-        }
-      }
+      unpack({b.x, b.y, b.z, b.w}, v);
     }
   }
-  static __device__ __forceinline__ void store(T* p, const float (&v)[VEC]) {
+  // Stores v rounded to T, and leaves what was stored in v.
+  static __device__ __forceinline__ void store(T* p, float (&v)[VEC]) {
     if constexpr (VEC == 1) {
-      *p = from_f32<T>(v[0]);
+      const T kept = from_f32<T>(v[0]);
+      *p = kept;
+      v[0] = to_f32(kept);
     } else {
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) {
+        if constexpr (sizeof(T) == 4)
           w[i] = __float_as_uint(v[i]);
-        } else {
-          T e[2] = {from_f32<T>(v[2 * i]), from_f32<T>(v[2 * i + 1])};
-          w[i] = *reinterpret_cast<uint32_t*>(e);
-        }
+        else if constexpr (std::is_same<T, __half>::value)
+          w[i] = pack_f16(v[2 * i], v[2 * i + 1]);
+        else
+          w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
       }
       *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+      unpack(w, v);
     }
   }
 };
@@ -172,7 +180,7 @@ __global__ void __launch_bounds__(32 * (W > 8 ? W : 8)) rows_s8_kernel(RowsArgs 
         float r[VEC];
         Chunk<T, VEC>::load(res + c, r);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = to_f32(from_f32<T>(__fadd_rn(v[i][j], r[j])));
+        for (int j = 0; j < VEC; ++j) v[i][j] = __fadd_rn(v[i][j], r[j]);
         Chunk<T, VEC>::store(static_cast<T*>(a.sum) + row * a.lds + c, v[i]);
       }
     }
@@ -312,14 +320,18 @@ __global__ void __launch_bounds__(256) read_s8_kernel(ReadArgs a, uint32_t units
     for (int i = 0; i < kApart; ++i)
       if (c + 32 * i < a.n) y[32 * i] = from_f32<T>(static_cast<float>(code[i]) * s);
   } else {
-    alignas(8) int8_t code[VEC];
-    if constexpr (VEC == 8)
-      *reinterpret_cast<uint2*>(code) = *reinterpret_cast<const uint2*>(p);
-    else
-      *reinterpret_cast<uint32_t*>(code) = *reinterpret_cast<const uint32_t*>(p);
+    uint32_t words[VEC / 4];
+    if constexpr (VEC == 8) {
+      const uint2 b = *reinterpret_cast<const uint2*>(p);
+      words[0] = b.x, words[1] = b.y;
+    } else {
+      words[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+    // 2^23 + 128 + code in an fp32's bits, exact; the conversion unit takes four times as long as the bytes
     float v[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = static_cast<float>(code[j]) * s;
+    for (int j = 0; j < VEC; ++j)
+      v[j] = (__uint_as_float(__byte_perm(words[j / 4] ^ 0x80808080u, 0x4B000000u, 0x7440 + j % 4)) - 8388736.0f) * s;
     Chunk<T, VEC>::store(y, v);
   }
 }
