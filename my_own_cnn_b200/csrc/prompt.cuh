@@ -45,21 +45,29 @@ __device__ __forceinline__ Sequence sequence(const PromptArgs& a, int i) {
   return s;
 }
 
-// Tile `tile` of a sequence; the units are in falling order of the keys that they see, in steps of 128, so that the longest start first and the
-// short ones fill up the end.  Found by bisection over the number of units with more than l steps.  A warp's work; a lane
-// keeps the first 32 sequences in registers.
+// Tile `tile` of a sequence.
 struct PromptUnit {
   Sequence s;
   int tile;
   bool ok;
 };
 __device__ __forceinline__ int warp_total(int v) { return __reduce_add_sync(~0u, v); }
-// A sequence's units, the last `above(l)` of which have more than l steps.
+// The sum of the lanes up to this one.
+__device__ __forceinline__ int warp_running(int v) {
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int x = __shfl_up_sync(~0u, v, o);
+    if (static_cast<int>(threadIdx.x % 32) >= o) v += x;
+  }
+  return v;
+}
+
+// A sequence's units, the last `above(l)` of which have more than l steps of 128 keys.
+constexpr int kUnitKeys = 128;
 struct Units {
   int tiles, lq, shift, most;  // keys less queries; steps of the last unit
   __device__ __forceinline__ Units(const PromptArgs& a, const Sequence& s)
-      : tiles(s.tiles(a)), lq(s.lq), shift(s.lk - s.lq), most(tiles ? max(0, s.lk + kUnitKeys - 1) / kUnitKeys : 0) {}
-  static constexpr int kUnitKeys = 128;
+      : tiles(s.tiles(a)), lq(s.lq), shift(s.lk - s.lq), most(tiles ? (s.lk + kUnitKeys - 1) / kUnitKeys : 0) {}
   // all at l < 0; from the first tile whose end passes l steps on
   __device__ __forceinline__ int above(const PromptArgs& a, int l) const {
     if (l < 0) return tiles;
@@ -69,91 +77,124 @@ struct Units {
     return tiles - min(tiles, static_cast<int>(a.tile.of(static_cast<uint32_t>(min(tokens, lq) * a.row_scale))));
   }
 };
-__device__ inline PromptUnit prompt_unit(const PromptArgs& a, int unit, bool report) {
-  const int lane = threadIdx.x % 32;
-  const Sequence first = sequence(a, lane);
-  const Units mine(a, first);
-  bool bad = first.bad;
-  int most = mine.most, all = mine.tiles;
-  for (int i = 32 + lane; i < a.b; i += 32) {
-    const Sequence s = sequence(a, i);
+
+// Finds units, each call a later one than the last; a warp's work.  Of up to 32 sequences, one a lane, the units are in falling order of
+// their steps, so that the longest start first and the short ones fill up the end (six sequences with earlier parts 80 us by tile
+// number, 67 so); found by bisection over the units with more than l steps.  Of more sequences they are in the sequences'
+// order, which a search from where the last one ended finds in one pass over all of them.
+class Finder {
+ public:
+  __device__ __forceinline__ Finder(const PromptArgs& args, bool report) : a(args), lane(threadIdx.x % 32) {
+    bool bad = false;
+    if (a.b <= 32) {
+      s = sequence(a, lane), bad = s.bad;
+    } else if (report) {
+      for (int i = lane; i < a.b; i += 32) bad |= sequence(a, i).bad;
+    }
+    if (report && bad) atomicCAS(a.err, 0, kDevErrBadStarts);
+  }
+  __device__ __forceinline__ PromptUnit operator()(int unit) { return a.b <= 32 ? by_length(unit) : by_sequence(unit); }
+
+ private:
+  __device__ __forceinline__ PromptUnit by_length(int unit) {
     const Units u(a, s);
-    bad |= s.bad;
-    most = max(most, u.most);
-    all += u.tiles;
-  }
-  if (report && bad) atomicCAS(a.err, 0, kDevErrBadStarts);
-  PromptUnit u{};
-  if (unit >= warp_total(all)) return u;
-  auto units_above = [&](int l) {
-    int n = mine.above(a, l);
-    for (int i = 32 + lane; i < a.b; i += 32) n += Units(a, sequence(a, i)).above(a, l);
-    return warp_total(n);
-  };
-  // units_above(lo) > unit >= units_above(hi) = longer: the unit has hi steps
-  int lo = -1, hi = __reduce_max_sync(~0u, most), longer = 0;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2, n = units_above(mid);
-    if (n > unit)
-      lo = mid;
-    else
-      hi = mid, longer = n;
-  }
-  int left = unit - longer;  // of the units with hi steps
-  for (int i0 = 0; i0 < a.b; i0 += 32) {
-    const Sequence s = i0 ? sequence(a, i0 + lane) : first;
-    const Units v(a, s);
-    const int end = v.tiles - v.above(a, hi), n = v.above(a, lo) - v.above(a, hi);
-    int upto = n;  // with the sequences before
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const int x = __shfl_up_sync(~0u, upto, o);
-      if (lane >= o) upto += x;
+    auto above = [&](int l) { return warp_total(u.above(a, l)); };
+    if (unit >= above(-1)) return PromptUnit{};
+    // above(lo) > unit >= above(hi) = longer: the unit has hi steps
+    int lo = -1, hi = __reduce_max_sync(~0u, u.most), longer = 0;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2, n = above(mid);
+      if (n > unit)
+        lo = mid;
+      else
+        hi = mid, longer = n;
     }
+    const int left = unit - longer;  // of the units with hi steps
+    const int past = u.above(a, hi), n = u.above(a, lo) - past, upto = warp_running(n);
     const unsigned have = __ballot_sync(~0u, upto > left);
-    if (have) {
-      const int from = __ffs(have) - 1;
-      u.s = {__shfl_sync(~0u, s.q0, from), __shfl_sync(~0u, s.lq, from), __shfl_sync(~0u, s.k0, from), __shfl_sync(~0u, s.lk, from),
-             false};
-      u.tile = __shfl_sync(~0u, end - 1 - (left - (upto - n)), from);
-      u.ok = u.tile >= 0;
-      return u;
-    }
-    left -= __shfl_sync(~0u, upto, 31);
+    return have ? at(s, u.tiles - past - 1 - (left - (upto - n)), __ffs(have) - 1) : PromptUnit{};
   }
-  return u;  // the starts changed meanwhile
-}
+  __device__ __forceinline__ PromptUnit by_sequence(int unit) {
+    constexpr int kEach = 4;  // sequences a lane: their loads are one wait
+    for (; first < a.b; first += 32 * kEach) {
+      Sequence q[kEach];
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) q[i] = sequence(a, first + kEach * lane + i);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) n += q[i].tiles(a);
+      const int upto = warp_running(n), left = unit - before;
+      if (const unsigned have = __ballot_sync(~0u, upto > left)) {
+        int tile = left - (upto - n);
+        Sequence mine = q[0];
+#pragma unroll
+        for (int i = 1; i < kEach; ++i) {
+          const int t = mine.tiles(a);
+          if (tile >= t) tile -= t, mine = q[i];
+          else break;
+        }
+        return at(mine, tile, __ffs(have) - 1);
+      }
+      before += __shfl_sync(~0u, upto, 31);
+    }
+    return PromptUnit{};
+  }
+  __device__ __forceinline__ PromptUnit at(const Sequence& q, int tile, int from) const {
+    PromptUnit u;
+    u.s = {__shfl_sync(~0u, q.q0, from), __shfl_sync(~0u, q.lq, from), __shfl_sync(~0u, q.k0, from), __shfl_sync(~0u, q.lk, from), false};
+    u.tile = __shfl_sync(~0u, tile, from);
+    u.ok = u.tile >= 0;  // not so where the starts change meanwhile
+    return u;
+  }
+  const PromptArgs& a;
+  int lane;
+  Sequence s;
+  int first = 0, before = 0;  // the sequences from here on; units of those before
+};
 
 // One row of attention by one warp, from memory and with what the row sees alone.  A product of a weight of zero and a masked value is
-// zero only while the value is finite, so the fast kernels come here with the rows that they found not finite.
+// zero only while the value is finite, so the fast kernels come here with the rows that they found not finite.  Lanes share out the
+// channels, four keys at a time are on their way.
 template <typename T>
 __device__ __noinline__ void prompt_row_with_care(const PromptArgs& a, int q_row, int head, int k0, int seen) {
   const int lane = threadIdx.x % 32, kv = static_cast<int>(a.ratio.of(head));
-  const T* q = static_cast<const T*>(a.q) + q_row * a.q_ts + head * a.q_hs;
   const T* k = static_cast<const T*>(a.k) + k0 * a.k_ts + kv * a.k_hs;
   const T* v = static_cast<const T*>(a.v) + k0 * a.v_ts + kv * a.v_hs;
-  auto score = [&](int j) {
-    const T* kj = k + j * a.k_ts;
-    float s = 0.0f;
-    for (int c = 0; c < a.d; ++c) s = fmaf(to_f32(q[c]), to_f32(kj[c]), s);
-    return s * a.scale;
-  };
-  float top = -INFINITY;
-  for (int j = lane; j < seen; j += 32) top = max_nan(top, score(j));
-  for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, o));
-  float total = 0.0f, o[8] = {};
-  for (int j0 = 0; j0 < seen; j0 += 32) {
-    const float p = j0 + lane < seen ? expf(score(j0 + lane) - top) : 0.0f;
-    total += p;
-    for (int i = 0; i < min(32, seen - j0); ++i) {
-      const float w = __shfl_sync(~0u, p, i);
-      const T* vj = v + (j0 + i) * a.v_ts;
-      for (int c = 0; c < 8; ++c)
-        if (lane + 32 * c < a.d) o[c] = fmaf(w, to_f32(vj[lane + 32 * c]), o[c]);
+  float q[8], o[8] = {}, top = -INFINITY, total = 0.0f;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    q[c] = lane + 32 * c < a.d ? to_f32(static_cast<const T*>(a.q)[q_row * a.q_ts + head * a.q_hs + lane + 32 * c]) : 0.0f;
+  for (int j0 = 0; j0 < seen; j0 += 4) {
+    T y[4][8], x[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        y[i][c] = x[i][c] = from_f32<T>(0.0f);
+        if (j0 + i < seen && lane + 32 * c < a.d) {
+          y[i][c] = k[(j0 + i) * a.k_ts + lane + 32 * c];
+          x[i][c] = v[(j0 + i) * a.v_ts + lane + 32 * c];
+        }
+      }
+    float s[4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) s[i] = fmaf(q[c], to_f32(y[i][c]), s[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (j0 + i >= seen) break;
+      const float score = warp_sum(s[i]) * a.scale, now = max_nan(top, score);
+      const bool nothing = now == -INFINITY;  // all scores so far
+      const float keep = nothing ? 1.0f : expf(top - now), w = nothing ? 0.0f : expf(score - now);
+      top = now;
+      total = fmaf(total, keep, w);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) o[c] = fmaf(w, to_f32(x[i][c]), o[c] * keep);
     }
   }
-  total = warp_sum(total);
   T* out = static_cast<T*>(a.out) + (static_cast<long long>(q_row) * a.hq + head) * a.d;
+#pragma unroll
   for (int c = 0; c < 8; ++c)
     if (lane + 32 * c < a.d) out[lane + 32 * c] = from_f32<T>(o[c] / total);
   if (a.lse && lane == 0)

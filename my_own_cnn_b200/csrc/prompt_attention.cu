@@ -135,10 +135,21 @@ struct Tile {
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) put(to, term, x[k], threadIdx.x + k * kMmaThreads);
   }
+  // From memory to the tiles, eight pieces on their way at a time.
   template <typename P>
   static __device__ __forceinline__ void load(uint32_t to, int term, int d, bool wide, P row_at) {
-    for (int i = threadIdx.x; i < ROWS * (D / 4); i += kMmaThreads)
-      put(to, term, four_of<T>(row_at(i / (D / 4)), i % (D / 4) * 4, d, wide), i);
+    constexpr int kAtOnce = kPieces < 8 ? kPieces : 8;
+#pragma unroll 1
+    for (int k0 = 0; k0 < kPieces; k0 += kAtOnce) {
+      float4 x[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int i = threadIdx.x + (k0 + k) * kMmaThreads;
+        x[k] = four_of<T>(row_at(i / (D / 4)), i % (D / 4) * 4, d, wide);
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) put(to, term, x[k], threadIdx.x + (k0 + k) * kMmaThreads);
+    }
   }
 };
 
@@ -151,7 +162,8 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
   extern __shared__ __align__(16) uint8_t smem[];
   wait_for_previous();
   const int kv = static_cast<int>(blockIdx.x % a.hk), lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const PromptUnit u = prompt_unit(a, static_cast<int>(blockIdx.x / a.hk), blockIdx.x == 0 && threadIdx.x < 32);
+  Finder finder(a, blockIdx.x == 0 && threadIdx.x < 32);
+  const PromptUnit u = finder(static_cast<int>(blockIdx.x / a.hk));
   if (!u.ok) return;
   const int ratio = static_cast<int>(a.ratio.d), shift = u.s.lk - u.s.lq;
   const int rows = u.s.lq * ratio, row0 = u.tile * kRows;  // of this key head's rows in the sequence
@@ -415,7 +427,8 @@ extern "C" int b200q_prompt_attention(const b200q_prompt_attention_args* p, void
   a.b = p->b, a.tq = p->tq, a.tk = p->tk, a.hq = p->hq, a.hk = p->hk, a.d = p->d;
   a.ratio = Divisor(static_cast<uint32_t>(ratio));
   a.scale = p->scale;
-  a.limit = host_wait_limit();
+  // a warp whose 32 rows are done with care (see prompt_row_with_care) keeps others waiting, 820 clocks a row and key (4096 tokens)
+  a.limit = host_wait_limit() + 32ll * 1024 * p->tk;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const int size = p->ftype == B200Q_F32 ? 4 : 2;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v);

@@ -156,16 +156,18 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
     tmem_relinquish();
   }
   wait_for_previous();
-  // The block's r-th unit in the order of their lengths, every other round backwards.
-  auto find = [&](int r, TcUnit* to) {
+  // The block's r-th unit in the units' order, every other round backwards.
+  auto find = [&](Finder& finder, int r, TcUnit* to) {
     const long long n = static_cast<long long>(r) * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
     PromptUnit u{};
-    if (n < a.most_units) u = prompt_unit(a, static_cast<int>(n / a.hk), r == 0 && blockIdx.x == 0);
+    if (n < a.most_units) u = finder(static_cast<int>(n / a.hk));
     if (lane == 0) *to = {u.s, u.tile * static_cast<int>(a.tile.d), static_cast<int>(n % a.hk), u.ok};
     return u.ok;
   };
-  bool more = true;
-  if (warp == 10) more = find(0, units);
+  if (warp == 10) {
+    Finder finder(a, blockIdx.x == 0);
+    find(finder, 0, units);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -321,10 +323,12 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 10) {
+      Finder finder(a, false);
+      bool more = units[0].ok;
       if (lane == 0) mbar_arrive(u_full);
       for (int r = 1; more; ++r) {
         if (r > 1 && !wait(u_empty + 8 * (r & 1), ((r >> 1) - 1) & 1, kDevErrTimeoutProducer)) break;
-        more = find(r, units + (r & 1));
+        more = find(finder, r, units + (r & 1));
         if (lane == 0) mbar_arrive(u_full + 8 * (r & 1));
         __syncwarp();
       }

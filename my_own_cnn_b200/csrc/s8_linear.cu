@@ -518,7 +518,7 @@ int linear_s8(const b200q_linear_s8_args* p, const Plan* fixed, cudaStream_t cs)
   if (m == 0 || n == 0) return B200Q_OK;
   if (k == 0) return host_fail(B200Q_ERR_INVALID_ARG, "rows of no elements");
   if (k > 131071) return host_fail(B200Q_ERR_UNSUPPORTED, "k = %d: sums of more than 131071 products may pass 32 bits", k);
-  if (n > (1 << 28)) return host_fail(B200Q_ERR_UNSUPPORTED, "n = %d is too large", n);
+  if (m > (1 << 28) || n > (1 << 28)) return host_fail(B200Q_ERR_UNSUPPORTED, "%d x %d results: too large", m, n);
   if (!p->x || !p->w || !p->x_scales || !p->w_scales || !p->y) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
   if ((p->ldx < k && m > 1) || (p->ldw < k && n > 1) || (p->ldy < n && m > 1))
     return host_fail(B200Q_ERR_INVALID_ARG, "row stride smaller than a row");

@@ -369,6 +369,7 @@ int rows_s8(const b200q_rows_s8_args* p, bool norm, void* stream) {
     if (p->t > 0) return host_fail(B200Q_ERR_INVALID_ARG, "rows of no elements have no scale");
     return B200Q_OK;
   }
+  if (p->t > (1 << 30) || p->n > (1 << 30)) return host_fail(B200Q_ERR_UNSUPPORTED, "%d rows of %d: too large", p->t, p->n);
   if (!p->x || !p->codes || !p->scales || (p->residual && !p->sum)) return host_fail(B200Q_ERR_INVALID_ARG, "null tensor pointer");
   if (!norm && (p->w || p->residual)) return host_fail(B200Q_ERR_INVALID_ARG, "a weight or a residual without a norm");
   if (p->ldc < p->n && p->t > 1) return host_fail(B200Q_ERR_INVALID_ARG, "row stride of the codes smaller than a row");
