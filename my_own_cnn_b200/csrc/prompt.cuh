@@ -20,7 +20,11 @@ struct PromptArgs {
   Divisor ratio;   // hq / hk
   int row_scale;   // a tile holds tile.d whole tokens (1), or tile.d rows (token, head of the group; hq / hk)
   Divisor tile;
-  long long most_units;  // key heads times tiles, as many as there may be
+  long long most_units;  // key heads times tiles times parts, as many as there may be
+  int parts;             // of each tile's keys; with more than one the sums meet in part_*, [parts][tq * hq]
+  float4* part_heads;    // reference (of base 2), sum of weights, the bits of the row's first key and of how many it sees
+  float* part_sums;      // [..][d]
+  unsigned* arrived;     // [tq * hq] parts that have been written: zero before and after
   float scale;
   int* err;
   long long limit;
@@ -77,6 +81,17 @@ struct Units {
     return tiles - min(tiles, static_cast<int>(a.tile.of(static_cast<uint32_t>(min(tokens, lq) * a.row_scale))));
   }
 };
+
+// Steps [from, to) of `steps` that are part `part`'s.
+__device__ __forceinline__ int2 part_steps(const PromptArgs& a, int steps, int part) {
+  return make_int2(static_cast<int>(static_cast<long long>(steps) * part / a.parts),
+                   static_cast<int>(static_cast<long long>(steps) * (part + 1) / a.parts));
+}
+// What a part says of a row; the join counts on all of them.
+__device__ __forceinline__ void part_head(const PromptArgs& a, int part, long long row, float ref, float sum, int k0, int seen) {
+  a.part_heads[part * static_cast<long long>(a.tq) * a.hq + row] = make_float4(ref, sum, __int_as_float(k0), __int_as_float(seen));
+  atomicAdd(a.arrived + row, 1u);
+}
 
 // Finds units, each call a later one than the last; a warp's work.  Of up to 32 sequences, one a lane, the units are in falling order of
 // their steps, so that the longest start first and the short ones fill up the end (six sequences with earlier parts 80 us by tile
@@ -199,6 +214,53 @@ __device__ __noinline__ void prompt_row_with_care(const PromptArgs& a, int q_row
     if (lane + 32 * c < a.d) out[lane + 32 * c] = from_f32<T>(o[c] / total);
   if (a.lse && lane == 0)
     a.lse[static_cast<long long>(q_row) * a.hq + head] = fabsf(top) < INFINITY ? top + logf(total) : top;
+}
+
+// Adds up the parts of a row: one warp a row, lanes over channels.
+template <typename T>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ PromptArgs a) {
+  wait_for_previous();
+  const long long rows = static_cast<long long>(a.tq) * a.hq, row = blockIdx.x * 8ll + threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  if (row >= rows) return;
+  const unsigned arrived = a.arrived[row];
+  __syncwarp();
+  if (arrived && lane == 0) a.arrived[row] = 0;
+  if (arrived != static_cast<unsigned>(a.parts)) return;  // a row outside every sequence
+  // a lane has a part's head; up to 32 parts
+  float4 head = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+  if (lane < a.parts) head = a.part_heads[lane * rows + row];
+  float top = head.y == 0.0f ? -INFINITY : head.x;  // a part that sees nothing has no say
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, o));
+  const float w = head.y == 0.0f ? 0.0f : exp2_approx(head.x - top);
+  const float total = warp_sum(head.y == 0.0f ? 0.0f : w * head.y);
+  float o[8] = {};
+#pragma unroll 2
+  for (int p = 0; p < a.parts; ++p) {
+    const float wp = __shfl_sync(~0u, w, p);
+    if (wp == 0.0f) continue;
+    const float* from = a.part_sums + (p * rows + row) * a.d;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (lane + 32 * c < a.d) o[c] = fmaf(wp, from[lane + 32 * c], o[c]);
+  }
+  const int k0 = __float_as_int(__shfl_sync(~0u, head.z, 0)), seen = __float_as_int(__shfl_sync(~0u, head.w, 0));
+  bool fine = total > 0.0f && total < INFINITY;
+  T* out = static_cast<T*>(a.out) + row * a.d;
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    if (lane + 32 * c < a.d) {
+      const float y = seen ? o[c] / total : 0.0f;
+      fine = fine && fabsf(y) < INFINITY;
+      out[lane + 32 * c] = from_f32<T>(y);
+    }
+  if (a.lse && lane == 0) a.lse[row] = seen ? (top + log2f(total)) * (1.0f / kLog2e) : -INFINITY;
+  __syncwarp();
+  if (seen && !__all_sync(~0u, fine)) {
+    const int q_row = static_cast<int>(row / a.hq);
+    prompt_row_with_care<T>(a, q_row, static_cast<int>(row - static_cast<long long>(q_row) * a.hq), k0, seen);
+  }
 }
 
 }  // namespace b200q

@@ -161,9 +161,10 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
   constexpr int kA[5] = {2, 0, 1, 1, 0}, kB[5] = {0, 2, 1, 0, 1};
   extern __shared__ __align__(16) uint8_t smem[];
   wait_for_previous();
-  const int kv = static_cast<int>(blockIdx.x % a.hk), lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int part = static_cast<int>(blockIdx.x % a.parts), whole = static_cast<int>(blockIdx.x / a.parts);
+  const int kv = whole % a.hk, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   Finder finder(a, blockIdx.x == 0 && threadIdx.x < 32);
-  const PromptUnit u = finder(static_cast<int>(blockIdx.x / a.hk));
+  const PromptUnit u = finder(whole / a.hk);
   if (!u.ok) return;
   const int ratio = static_cast<int>(a.ratio.d), shift = u.s.lk - u.s.lq;
   const int rows = u.s.lq * ratio, row0 = u.tile * kRows;  // of this key head's rows in the sequence
@@ -181,7 +182,9 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
     const int r = row0 + warp * 16 + g + 8 * h;
     seen[h] = r < rows ? max(0, static_cast<int>(a.ratio.of(r)) + shift + 1) : 0;
   }
-  const int most = min(u.s.lk, static_cast<int>(a.ratio.of(last_row)) + shift + 1);
+  const int all = max(0, min(u.s.lk, static_cast<int>(a.ratio.of(last_row)) + shift + 1));
+  const int2 steps = part_steps(a, (all + kKeys - 1) / kKeys, part);
+  const int least = steps.x * kKeys, most = min(all, steps.y * kKeys);
   const float c = a.scale * kLog2e;
   float o[D / 8][4] = {}, top[2] = {-INFINITY, -INFINITY}, sum[2] = {};
   // Heads of up to 64 channels: the next keys and values are on their way, in registers, while these are worked on.
@@ -194,12 +197,12 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
     };
   };
   if constexpr (kAhead) {
-    if (most > 0) {
-      KV::fetch(next_k, a.d, wide, key_rows(a.k, a.k_ts, a.k_hs, 0));
-      KV::fetch(next_v, a.d, wide, key_rows(a.v, a.v_ts, a.v_hs, 0));
+    if (most > least) {
+      KV::fetch(next_k, a.d, wide, key_rows(a.k, a.k_ts, a.k_hs, least));
+      KV::fetch(next_v, a.d, wide, key_rows(a.v, a.v_ts, a.v_hs, least));
     }
   }
-  for (int j0 = 0; j0 < most; j0 += kKeys) {
+  for (int j0 = least; j0 < most; j0 += kKeys) {
     __syncthreads();
     if constexpr (kAhead) {
       KV::put(s_k, S::kK, next_k);
@@ -319,6 +322,18 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
     l += __shfl_xor_sync(~0u, l, 2);
     const int token = static_cast<int>(a.ratio.of(min(r, rows - 1))), head = kv * ratio + min(r, rows - 1) - token * ratio;
     const long long at = static_cast<long long>(u.s.q0 + token) * a.hq + head;
+    if (a.parts > 1) {
+      if (r < rows) {
+        if (t == 0) part_head(a, part, at, top[h], l, u.s.k0, min(u.s.lk, seen[h]));
+        float* sums = a.part_sums + (part * static_cast<long long>(a.tq) * a.hq + at) * a.d;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (n * 8 + 2 * t + e < a.d) sums[n * 8 + 2 * t + e] = o[n][2 * h + e];
+      }
+      continue;
+    }
     const float by = l > 0.0f ? 1.0f / l : 0.0f;
     bool fine = l > 0.0f && l < INFINITY;
     if (r < rows) {
@@ -366,6 +381,16 @@ bool tensor_core_takes(const b200q_prompt_attention_args& p, long long ratio) {
   if (bits & 15u) return false;
   const auto fits = [](int64_t stride, int count) { return count == 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); };
   return fits(p.q_ts, p.tq) && fits(p.q_hs, p.hq) && fits(p.k_ts, p.tk) && fits(p.k_hs, p.hk) && fits(p.v_ts, p.tk) && fits(p.v_hs, p.hk);
+}
+
+// Parts that the keys are cut into, 1 where there are tiles enough for half of the SMs or few keys: as many as give every SM one, of no
+// less than 256 keys of an average sequence (128 on mma.sync, four times as slow), as the scratch holds.  28 rows of one key head
+// over 7000 keys in fp32: 254 us in one part, 89 in 4.
+int parts_of(const b200q_prompt_attention_args& p, long long units, int sms, bool tensor) {
+  const long long rows = static_cast<long long>(p.tq) * p.hq, bytes = rows * (p.d * sizeof(float) + sizeof(float4));
+  const long long parts = std::min({sms / std::max(1ll, units), static_cast<long long>(p.tk) / p.b / (tensor ? 256 : 128),
+                                    static_cast<long long>(kScratchBytes) / bytes, 32ll});
+  return rows <= kSplitCounters && parts > 1 ? static_cast<int>(parts) : 1;
 }
 
 template <typename T, int D>
@@ -437,7 +462,15 @@ extern "C" int b200q_prompt_attention(const b200q_prompt_attention_args* p, void
   a.row_scale = tensor ? 1 : static_cast<int>(ratio);
   // as many units as there may be: every sequence's last tile may be short
   const long long tiles = p->tq * static_cast<long long>(a.row_scale) / a.tile.d + std::min<long long>(p->b, p->tq);
-  const long long units = a.most_units = tiles * p->hk;
+  ScratchHold scratch;  // until both kernels are in the stream
+  a.parts = parts_of(*p, tiles * p->hk, sms, tensor);
+  if (a.parts > 1) {
+    if (int rc = host_scratch(cs, &scratch)) return rc;
+    a.arrived = scratch.counters;
+    a.part_heads = static_cast<float4*>(scratch.bytes);
+    a.part_sums = reinterpret_cast<float*>(a.part_heads + a.parts * static_cast<long long>(p->tq) * p->hq);
+  }
+  const long long units = a.most_units = tiles * p->hk * a.parts;
   if (units > 0x7fffffffll) return host_fail(B200Q_ERR_UNSUPPORTED, "too many rows");
   int rc = B200Q_OK;
   if (tensor) {
@@ -451,6 +484,12 @@ extern "C" int b200q_prompt_attention(const b200q_prompt_attention_args* p, void
     B200Q_DISPATCH_FTYPE(p->ftype, rc = a.d <= 64    ? launch_mma<T, 64>(a, wide, units, device, cs)
                                         : a.d <= 128 ? launch_mma<T, 128>(a, wide, units, device, cs)
                                                      : launch_mma<T, 256>(a, wide, units, device, cs));
+  }
+  if (rc == B200Q_OK && a.parts > 1) {
+    const long long rows = static_cast<long long>(p->tq) * p->hq;
+    B200Q_DISPATCH_FTYPE(p->ftype, rc = host_launch("prompt_join_kernel launch", prompt_join_kernel<T>,
+                                                    dim3(static_cast<unsigned>((rows + 7) / 8)), 256, 0, cs, 1, a));
+    scratch.launched();
   }
   if (rc == B200Q_OK) host_set_path(tensor ? 23 : 24);
   return rc;

@@ -98,13 +98,15 @@ struct TcUnit {
   Sequence s;
   int token0;  // of tile A in the sequence
   int kv;      // key head
+  int part, from, to;  // part of the keys: steps of 128
   int ok;
 };
 
-// Halves (of 64 keys) that tile i of a unit needs: its last token's.
+// Halves (of 64 keys) that tile i of a unit has to do: its last token's, as far as they are the part's.
 __device__ __forceinline__ int unit_halves(const TcUnit& u, int i, int tokens) {
   const int first = u.token0 + i * tokens, last = min(u.s.lq, first + tokens) - 1;
-  return first < u.s.lq ? (max(0, last + u.s.lk - u.s.lq + 1) + kHalf - 1) / kHalf : 0;
+  const int all = first < u.s.lq ? (max(0, last + u.s.lk - u.s.lq + 1) + kHalf - 1) / kHalf : 0;
+  return max(0, min(all, 2 * u.to) - 2 * u.from);
 }
 
 template <typename T, int D>
@@ -160,8 +162,15 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
   auto find = [&](Finder& finder, int r, TcUnit* to) {
     const long long n = static_cast<long long>(r) * gridDim.x + (r & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
     PromptUnit u{};
-    if (n < a.most_units) u = finder(static_cast<int>(n / a.hk));
-    if (lane == 0) *to = {u.s, u.tile * static_cast<int>(a.tile.d), static_cast<int>(n % a.hk), u.ok};
+    const long long whole = n / a.parts;
+    if (n < a.most_units) u = finder(static_cast<int>(whole / a.hk));
+    if (lane == 0) {
+      TcUnit v{u.s, u.tile * static_cast<int>(a.tile.d), static_cast<int>(whole % a.hk), static_cast<int>(n - whole * a.parts), 0, 0, u.ok};
+      const int last = min(u.s.lq, v.token0 + static_cast<int>(a.tile.d)) + u.s.lk - u.s.lq;  // keys of the unit's last token
+      const int2 steps = part_steps(a, (max(0, last) + kTcKeys - 1) / kTcKeys, v.part);
+      v.from = steps.x, v.to = steps.y;
+      *to = v;
+    }
     return u.ok;
   };
   if (warp == 10) {
@@ -220,7 +229,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
         loaded(raw[0]);
         loaded(raw[1]);
         const auto s = [&](int k) { return __uint_as_float(raw[k / 32][k % 32]); };
-        const int limit = seen - t * kHalf;
+        const int limit = seen - 2 * u.from * kHalf - t * kHalf;
         if (__any_sync(~0u, limit < kHalf)) {
 #pragma unroll
           for (int k = 0; k < kHalf; ++k)
@@ -270,6 +279,22 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
       if (n) wait(ended + 8 * i, units_of++ & 1, kCode);
       if (!ok) break;
       tc_fence_after();
+      if (a.parts > 1) {
+        const long long row_at = static_cast<long long>(u.s.q0 + token) * a.hq + head;
+        if (mine) part_head(a, u.part, row_at, ref - kLift, sum, u.s.k0, seen);
+        float* sums = a.part_sums + (u.part * static_cast<long long>(a.tq) * a.hq + row_at) * a.d;
+#pragma unroll 1
+        for (int k = 0; n && k < a.d; k += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(t_o + k, o);
+          tmem_ld_wait();
+          loaded(o);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            if (mine && k + e < a.d) *reinterpret_cast<uint4*>(sums + k + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+        continue;
+      }
       // Results: whole rows by way of the warp's own shared memory (16-byte piece p of a row's 128 bytes at p ^ (row % 8)), so that
       // 8 lanes write 128 bytes together; a thread that writes its own row takes as many cycles as it has sectors.
       const float scale = seen ? 1.0f / sum : 0.0f;
@@ -358,7 +383,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
           if (!go) break;
           mbar_arrive_expect_tx_elect(full0 + 8 * st, S::kTile);
           for (int c = 0; c < kChunks; ++c)
-            tma_load_3d_elect(s_ring + st * S::kTile + c * 16384, k & 1 ? &tm_v : &tm_k, full0 + 8 * st, 64 * c, kv, u.s.k0 + k / 2 * kTcKeys);
+            tma_load_3d_elect(s_ring + st * S::kTile + c * 16384, k & 1 ? &tm_v : &tm_k, full0 + 8 * st, 64 * c, kv, u.s.k0 + (u.from + k / 2) * kTcKeys);
         }
         if (!go) break;
       }

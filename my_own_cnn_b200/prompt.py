@@ -27,7 +27,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     h reads head h // (hq / hk).  Rows outside every sequence are left as they are in `out`.  A sequence whose
     starts decrease or pass the tensors is left out and reported by device_error().  scale: 1 / sqrt(d) when None.
     Returns out [tq, hq, d], and lse fp32 [tq, hq] (log of the sum of exp(scale * q.k)) when return_lse.  out shares no memory
-    with the other tensors; starts stay as they are until the call has run."""
+    with the other tensors; starts stay as they are until the call has run.
+
+    Where few rows see many keys (too few tiles of rows for half of the SMs, 512 keys and more a sequence on average) the keys are
+    cut into parts that meet in the stream's scratch: make one such call on the stream before capturing a graph on it."""
     ft = FTYPES.get(q.dtype)
     if ft is None or not q.is_cuda:
         _ftype(q, "q")

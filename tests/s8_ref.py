@@ -47,8 +47,8 @@ def attention(q, k, v, starts, k_starts, scale, dtype):
 
     A score is a sum of d products in fp32, off by at most d 2^-23 sum |scale q k|, its product with the base's factor by two roundings;
     a weight besides by 2^-21 (the exponential) and, in 16-bit calls, its rounding to 16 bits; their sums (of n keys: n / 4 additions a lane and
-    16 more, or n / 16 in the tensor core) by (n / 4 + 16) 2^-23.  fp16 weights below 2^-14 of 2^-6 (the largest is 1, or 2^-8 while
-    a larger one may still come) are off by 2^-25 at most of the largest instead."""
+    16 more, or n / 16 in the tensor core; parts add up to 32 more where n is past 512) by (n / 4 + 16) 2^-23.  fp16 weights, 2^6 to 2^14
+    where the largest has its place, are normal down to 2^-20 of it and off by 2^-25 of it at most below."""
     tq, hq, d = q.shape
     r = hq // k.shape[1]
     out = torch.full((tq, hq, d), math.nan, dtype=torch.float64)

@@ -244,3 +244,73 @@ def test_a_call_repeats_bit_for_bit(cuda_lib, dtype):
     for _ in range(3):
         again = b2q.prompt_attention(q, k, v, starts, return_lse=True)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 80, 256])
+@pytest.mark.parametrize("lq,lk", [([28], [3138]), ([3, 20, 0, 1], [3000, 1500, 700, 5000]), ([1, 1, 64], [4096, 10, 65]), ([70], [7000]),
+                                   ([30, 5], [3, 2500])])
+def test_few_rows_over_many_keys(cuda_lib, dtype, d, lq, lk):
+    """The keys are cut into parts whose sums a second kernel joins: parts that end inside a sequence, that a row does not see, that are empty."""
+    q, k, v = make(sum(lq), sum(lk), 4, 1, d, dtype, d)
+    out, lse = check(q, k, v, starts_of(lq), starts_of(lk))
+    again = b2q.prompt_attention(q, k, v, starts_of(lq), starts_of(lk), return_lse=True)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_parts_leave_other_rows_and_masked_values_out(cuda_lib, dtype):
+    lq, lk = [5, 16], [2600, 3000]
+    q, k, v = make(30, sum(lk) + 9, 4, 2, 64, dtype)
+    starts = torch.tensor([2, 7, 23], dtype=torch.int32, device="cuda")
+    k_starts = torch.tensor([4, 2604, 5604], dtype=torch.int32, device="cuda")
+    for x in (k, v):
+        x[:4] = math.nan
+        x[5604:] = math.inf
+    clean = torch.full_like(q, 3.0)
+    _, clean_lse = b2q.prompt_attention(q, k, v, starts, k_starts, out=clean, return_lse=True)
+    check(q, k, v, starts, k_starts, out=clean, lse=clean_lse)
+    assert (clean[:2] == 3).all() and (clean[23:] == 3).all()
+    most = float(v[4:5604].abs().max())
+    v[2603, 0, 7] = math.nan   # the first sequence's last key: its last row alone sees it
+    v[4000, 1, 9] = -math.inf  # all rows of the second
+    out = torch.full_like(q, 3.0)
+    b2q.prompt_attention(q, k, v, starts, k_starts, out=out)
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[6, :2, 7] = True
+    hit[7:23, 2:, 9] = True
+    assert out[6, :2, 7].isnan().all() and (out[7:23, 2:, 9] == -math.inf).all()
+    unit = 3 * UNIT[dtype] + (3000 / 4 + 16) * 2.0 ** -22
+    assert (out[~hit].double() - clean[~hit].double()).abs().max() < most * unit
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_parts_in_a_graph_beside_cache_attention(cuda_lib, dtype):
+    """The parts' counters are the stream's scratch, which the cache attention uses too: both find it as they left it."""
+    q, k, v = make(12, 4000, 4, 2, 64, dtype)
+    starts, k_starts = starts_of([8, 4]), starts_of([2500, 1500])
+    cache = b2q.KV4Cache.empty(80, 2, 64, 64, 32)
+    b2q.kv4_append(cache, k, v, torch.arange(4000, device="cuda"))
+    table, lens = torch.arange(80, device="cuda").int().view(2, 40), torch.tensor([2500, 1500], device="cuda").int()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = b2q.kv4_attention(q[:2, None], cache, table, lens)
+        out, lse = b2q.prompt_attention(q, k, v, starts, k_starts, return_lse=True)
+        second = b2q.kv4_attention(q[:2, None], cache, table, lens)
+    side.synchronize()
+    # bit for bit: the second sequence's last 60 places were not written (2560 + 1500 of 4000 slots) and may hold NaN
+    assert torch.equal(first.view(torch.uint8), second.view(torch.uint8))
+    check(q, k, v, starts, k_starts, out=out, lse=lse)
+    held = torch.empty_like(out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        _, lse = b2q.prompt_attention(q, k, v, starts, k_starts, out=held, return_lse=True)
+    for cut in ([2500, 1500], [12, 3988], [4000, 0]):
+        k_starts.copy_(starts_of(cut))
+        g.replay()
+        check(q, k, v, starts, k_starts, out=held, lse=lse)
+    fresh = torch.cuda.Stream()  # no scratch yet
+    with pytest.raises(RuntimeError, match="scratch"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=fresh):
+            b2q.prompt_attention(q, k, v, starts, k_starts)
