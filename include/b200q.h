@@ -309,8 +309,15 @@ int b200q_quantize_s8(const b200q_rows_s8_args* args, void* stream);
 int b200q_rms_norm_s8(const b200q_rows_s8_args* args, void* stream);
 
 /* y[t][n] (row stride ldy, of ftype) = codes * scales, rounded once. */
-int b200q_read_s8(const int8_t* codes, long long ldc, const float* scales, void* y, long long ldy, int ftype, int t,
-                  int n, void* stream);
+typedef struct b200q_read_s8_args {
+  const int8_t* codes;
+  int64_t ldc;
+  const float* scales;
+  void* y;
+  int64_t ldy;
+  int ftype, t, n;
+} b200q_read_s8_args;
+int b200q_read_s8(const b200q_read_s8_args* args, void* stream);
 
 /* y[m][n] = (sum_k x[m][k] * w[n][k]) * x_scale[m] * w_scale[n] (+ bias[n]) for 8-bit rows x [m][k] and w [n][k]: the sum exact in
  * 32-bit integers (k <= 131071), the rest in fp32, y of ftype with row stride ldy; bias [n] of ftype or NULL.  Codes lie on

@@ -93,6 +93,11 @@ class CRowsS8Args(Structure):
                 ("ftype", c_int), ("t", c_int), ("n", c_int), ("eps", c_float)]
 
 
+class CReadS8Args(Structure):
+    _fields_ = [("codes", c_void_p), ("ldc", c_int64), ("scales", c_void_p), ("y", c_void_p), ("ldy", c_int64),
+                ("ftype", c_int), ("t", c_int), ("n", c_int)]
+
+
 class CLinearS8Args(Structure):
     _fields_ = [("x", c_void_p), ("ldx", c_int64), ("x_scales", c_void_p), ("w", c_void_p), ("ldw", c_int64),
                 ("w_scales", c_void_p), ("bias", c_void_p), ("y", c_void_p), ("ldy", c_int64), ("ftype", c_int),
@@ -166,7 +171,7 @@ def lib() -> ctypes.CDLL:
         "b200q_kv4_attention": [packed, packed, vp],
         "b200q_quantize_s8": [packed, vp],
         "b200q_rms_norm_s8": [packed, vp],
-        "b200q_read_s8": [vp, ll, vp, vp, ll, i, i, i, vp],
+        "b200q_read_s8": [packed, vp],
         "b200q_linear_s8": [packed, vp],
         "b200q_prompt_attention": [packed, vp],
     }

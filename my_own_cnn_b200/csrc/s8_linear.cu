@@ -434,7 +434,7 @@ double plan_clocks(const Plan& p, int m, int n, int kblocks, const int (&room)[4
   return std::max(clocks, (static_cast<double>(n) + m) * kblocks * kBK / 4096.0 + 5000.0 + join);
 }
 
-Plan plan_for(int m, int n, int kblocks, const int (&room)[4]) {
+Plan search_plan(int m, int n, int kblocks, const int (&room)[4]) {
   Plan best{false, 16, 1, 0};
   double least = 1e300;
   const auto offer = [&](Plan p) {
@@ -452,6 +452,19 @@ Plan plan_for(int m, int n, int kblocks, const int (&room)[4]) {
   const int smem = !best.pair && best.split == 1 && best.bn <= kTwosMost && blocks > room[0] ? kSmemMost / 2 - 1024 : kSmemMost;
   best.stages = std::max(2, std::min({kMaxStages, steps, (smem - kSmemFixed - landing_bytes(best)) / stage_bytes(best)}));
   return best;
+}
+
+// The search takes a microsecond: a thread keeps the plans of its last sizes.
+Plan plan_for(int m, int n, int kblocks, int device, const int (&room)[4]) {
+  struct Kept {
+    int m = -1, n, kblocks, device;
+    Plan plan;
+  };
+  static thread_local Kept kept[64];
+  Kept& at = kept[(static_cast<unsigned>(m) * 31u + static_cast<unsigned>(n) * 7u + static_cast<unsigned>(kblocks)) % 64u];
+  if (at.m != m || at.n != n || at.kblocks != kblocks || at.device != device)
+    at = {m, n, kblocks, device, search_plan(m, n, kblocks, room)};
+  return at.plan;
 }
 
 template <typename T>
@@ -540,7 +553,7 @@ int linear_s8(const b200q_linear_s8_args* p, const Plan* fixed, cudaStream_t cs)
   a.err = err;
   int room[4];
   if ((rc = block_room(device, sms, &room))) return rc;
-  const Plan plan = fixed ? *fixed : plan_for(m, n, a.kblocks, room);
+  const Plan plan = fixed ? *fixed : plan_for(m, n, a.kblocks, device, room);
   CUtensorMap tm_w, tm_x;
   const auto stride = [&](int rows, int64_t ld) { return static_cast<uint64_t>(rows > 1 ? ld : round_up(k, 16)); };
   if ((rc = host_tensor_map(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p->w, {static_cast<uint64_t>(k), static_cast<uint64_t>(n), 1},

@@ -406,8 +406,9 @@ using namespace b200q;
 extern "C" int b200q_quantize_s8(const b200q_rows_s8_args* args, void* stream) { return rows_s8(args, false, stream); }
 extern "C" int b200q_rms_norm_s8(const b200q_rows_s8_args* args, void* stream) { return rows_s8(args, true, stream); }
 
-extern "C" int b200q_read_s8(const int8_t* codes, long long ldc, const float* scales, void* y, long long ldy, int ftype, int t, int n,
-                             void* stream) {
+extern "C" int b200q_read_s8(const b200q_read_s8_args* args, void* stream) {
+  if (!args) return host_fail(B200Q_ERR_INVALID_ARG, "null argument");
+  const auto [codes, ldc, scales, y, ldy, ftype, t, n] = *args;
   if (ftype < B200Q_F32 || ftype > B200Q_BF16) return host_fail(B200Q_ERR_INVALID_ARG, "bad floating type %d", ftype);
   if (t < 0 || n < 0) return host_fail(B200Q_ERR_INVALID_ARG, "negative dimensions");
   if (t == 0 || n == 0) return B200Q_OK;

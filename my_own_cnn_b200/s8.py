@@ -15,6 +15,7 @@ from . import _lib
 from .w4 import FTYPES, _device_tensor, _ftype, _launch_stream, _on
 
 _ROWS = _lib.packer(_lib.CRowsS8Args)
+_READ = _lib.packer(_lib.CReadS8Args)
 _LINEAR = _lib.packer(_lib.CLinearS8Args)
 
 
@@ -51,7 +52,10 @@ class S8Rows:
         lead, k = shape[:-1], shape[-1]
         r = S8Rows.__new__(S8Rows)
         r.k, r._pitch = k, -(-k // 16) * 16
-        r.codes = x.new_empty(lead + (r._pitch,), dtype=torch.int8)
+        if r._pitch == k and x.is_contiguous():
+            r.codes = torch.empty_like(x, dtype=torch.int8)
+        else:
+            r.codes = x.new_empty(lead + (r._pitch,), dtype=torch.int8)
         r.scales = x.new_empty(lead, dtype=torch.float32)
         return r
 
@@ -75,8 +79,8 @@ class S8Rows:
         handle = _launch_stream(stream, self.codes)
         scales = self.scales
         y = scales.new_empty(scales.shape + (self.k,), dtype=dtype)
-        _lib.check(_lib.lib().b200q_read_s8(self.codes.data_ptr(), self._pitch, scales.data_ptr(), y.data_ptr(), self.k, ft,
-                                            scales.numel(), self.k, handle))
+        _lib.check(_lib.lib().b200q_read_s8(_READ.pack(self.codes.data_ptr(), self._pitch, scales.data_ptr(), y.data_ptr(),
+                                                       self.k, ft, scales.numel(), self.k), handle))
         return y
 
 
@@ -109,6 +113,13 @@ def _out_rows(out, shape, like):
     if out.shape != shape or not out.codes.is_cuda:
         raise RuntimeError(f"out must be 8-bit rows of {list(shape)} on the device, got {list(out.shape)}")
     return out
+
+
+def _check_like(t, x, shape, what):
+    if t.dtype != x.dtype or not t.is_cuda:
+        _device_tensor(t, x.dtype, what)
+    if t.shape != shape:
+        raise RuntimeError(f"{what} must be {list(shape)}, got {list(t.shape)}")
 
 
 def quantize_s8(x: torch.Tensor, out: S8Rows | None = None, stream=None) -> S8Rows:
@@ -150,18 +161,17 @@ def rms_norm_s8(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Te
     if not shape or not shape[-1]:
         raise RuntimeError(f"x must be [..., n] with n of at least 1, got {list(shape)}")
     if weight is not None:
-        _device_tensor(weight, x.dtype, "weight")
-        if weight.shape != shape[-1:] or not weight.is_contiguous():
+        if weight.dtype != x.dtype or not weight.is_cuda:
+            _device_tensor(weight, x.dtype, "weight")
+        if weight.dim() != 1 or weight.shape[0] != shape[-1] or not weight.is_contiguous():
             raise RuntimeError(f"weight must be contiguous [{shape[-1]}]")
     if residual is None:
         if residual_out is not None:
             raise RuntimeError("residual_out without a residual")
     else:
-        for t, what in ((residual, "residual"), (residual_out, "residual_out")):
-            if t is not None:
-                _device_tensor(t, x.dtype, what)
-                if t.shape != shape:
-                    raise RuntimeError(f"{what} must be {list(shape)}, got {list(t.shape)}")
+        _check_like(residual, x, shape, "residual")
+        if residual_out is not None:
+            _check_like(residual_out, x, shape, "residual_out")
     if stream is not None:
         with _on(stream):
             return _norm(x, weight, residual, residual_out, eps, out, ft, shape, stream)

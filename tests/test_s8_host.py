@@ -10,7 +10,7 @@ from my_own_cnn_b200 import _lib
 from tests.test_lowbit_host import INVALID, OK, P, UNSUPPORTED, block
 
 
-@pytest.mark.parametrize("layout,size", [(_lib.CRowsS8Args, 96), (_lib.CLinearS8Args, 88), (_lib.CPromptAttentionArgs, 136)])
+@pytest.mark.parametrize("layout,size", [(_lib.CRowsS8Args, 96), (_lib.CReadS8Args, 56), (_lib.CLinearS8Args, 88), (_lib.CPromptAttentionArgs, 136)])
 def test_argument_blocks_have_the_header_layout(layout, size):
     values = [(3 * i + 1) if t is not ctypes.c_float else 0.5 for i, (_, t) in enumerate(layout._fields_)]
     assert ctypes.sizeof(layout) == size
@@ -43,11 +43,14 @@ def test_norm_and_read_refusals():
     assert L.b200q_rms_norm_s8(rows(residual=P, sum=P, lds=63), 0) == INVALID and b"stride" in L.b200q_last_error()
     assert L.b200q_quantize_s8(rows(w=P), 0) == INVALID and L.b200q_quantize_s8(rows(residual=P, sum=P), 0) == INVALID
     assert L.b200q_quantize_s8(None, 0) == INVALID
-    assert L.b200q_read_s8(P, 64, P, P, 64, 5, 1, 64, 0) == INVALID
-    assert L.b200q_read_s8(P, 64, P, P, 64, 0, -1, 64, 0) == INVALID
-    assert L.b200q_read_s8(P, 64, 0, P, 64, 0, 1, 64, 0) == INVALID and b"null" in L.b200q_last_error()
-    assert L.b200q_read_s8(P, 64, P, P, 63, 0, 2, 64, 0) == INVALID and b"stride" in L.b200q_last_error()
-    assert L.b200q_read_s8(0, 0, 0, 0, 0, 0, 0, 64, 0) == OK
+
+    def read(*v):
+        return L.b200q_read_s8(block(_lib.CReadS8Args, v), 0)
+
+    assert read(P, 64, P, P, 64, 5, 1, 64) == INVALID and read(P, 64, P, P, 64, 0, -1, 64) == INVALID
+    assert read(P, 64, 0, P, 64, 0, 1, 64) == INVALID and b"null" in L.b200q_last_error()
+    assert read(P, 64, P, P, 63, 0, 2, 64) == INVALID and b"stride" in L.b200q_last_error()
+    assert L.b200q_read_s8(None, 0) == INVALID and read(0, 0, 0, 0, 0, 0, 0, 64) == OK
 
 
 @pytest.mark.parametrize("rc,message,kw", [
