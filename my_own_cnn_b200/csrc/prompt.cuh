@@ -171,7 +171,7 @@ class Finder {
 // zero only while the value is finite, so the fast kernels come here with the rows that they found not finite.  Lanes share out the
 // channels, four keys at a time are on their way.
 template <typename T>
-__device__ __noinline__ void prompt_row_with_care(const PromptArgs& a, int q_row, int head, int k0, int seen) {
+__device__ __forceinline__ void prompt_row_with_care(const PromptArgs& a, int q_row, int head, int k0, int seen) {
   const int lane = threadIdx.x % 32, kv = static_cast<int>(a.ratio.of(head));
   const T* k = static_cast<const T*>(a.k) + k0 * a.k_ts + kv * a.k_hs;
   const T* v = static_cast<const T*>(a.v) + k0 * a.v_ts + kv * a.v_hs;
@@ -207,6 +207,7 @@ __device__ __noinline__ void prompt_row_with_care(const PromptArgs& a, int q_row
 #pragma unroll
       for (int c = 0; c < 8; ++c) o[c] = fmaf(w, to_f32(x[i][c]), o[c] * keep);
     }
+    if (top != top) break;  // and stays so
   }
   T* out = static_cast<T*>(a.out) + (static_cast<long long>(q_row) * a.hq + head) * a.d;
 #pragma unroll
@@ -214,6 +215,102 @@ __device__ __noinline__ void prompt_row_with_care(const PromptArgs& a, int q_row
     if (lane + 32 * c < a.d) out[lane + 32 * c] = from_f32<T>(o[c] / total);
   if (a.lse && lane == 0)
     a.lse[static_cast<long long>(q_row) * a.hq + head] = fabsf(top) < INFINITY ? top + logf(total) : top;
+}
+
+// What warp_scan() looks for, a bit for each of a lane's channels (lane, lane + 32, ..).
+struct Odd {
+  unsigned nan = 0, plus = 0, minus = 0, large = 0;  // NaN, +inf, -inf; magnitudes of 2^100 and more
+};
+// Some keys (or values) of one head from row `at` on, of `n`.
+constexpr int kScanRows = 2;
+template <typename T>
+__device__ __forceinline__ void warp_scan(Odd& found, const T* base, long long ts, int at, int n, int d) {
+  const int lane = threadIdx.x % 32;
+  T x[kScanRows][8];
+#pragma unroll
+  for (int i = 0; i < kScanRows; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      x[i][c] = from_f32<T>(0.0f);
+      if (at + i < n && lane + 32 * c < d) x[i][c] = base[(at + i) * ts + lane + 32 * c];
+    }
+#pragma unroll
+  for (int i = 0; i < kScanRows; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const float f = to_f32(x[i][c]);
+      found.nan |= f != f ? 1u << c : 0u;
+      found.plus |= f == INFINITY ? 1u << c : 0u;
+      found.minus |= f == -INFINITY ? 1u << c : 0u;
+      found.large |= fabsf(f) >= 0x1p100f ? 1u << c : 0u;
+    }
+}
+
+// A row that a fast kernel wrote and found not finite, by one warp.  Most such results are right as they are, and looking for the reason
+// takes a read of the values up to the first NaN (or all that the row sees), where a row with care costs all keys and values: 8192 tokens,
+// 32 / 8 heads of 128, bf16 take 0.53 ms; with a NaN in the first key as long, in the first value 0.66 ms, in value 4096 79 ms, with an
+// infinity in the first value 170 ms; all rows with care would be minutes.
+//   - The sum of the weights is NaN: a score is, and so is all of the row.  (A score of +inf gives the same row, but its log-sum is
+//     +inf unless there is a NaN as well; one that passes fp32 by the factor log2(e) alone is finite.)  In fp32 a score is NaN also
+//     where a factor is infinite, or rounds to a first term that is: its terms are.
+//   - A channel is NaN or infinite, and the values that the row sees have the NaN or the infinities that make it so.
+enum { kSumOdd = 0, kSumFine = 1, kSumNaN = 2, kSettled = 3 };
+template <typename T>
+__device__ __forceinline__ int prompt_sums(const PromptArgs& a, float top, float sum) {
+  if (sum != sum)
+    return top != INFINITY || (!a.lse && fabsf(a.scale) * kLog2e <= 1.0f) ? (sizeof(T) == 4 ? kSumNaN : kSettled) : kSumOdd;
+  return sum > 0.0f && sum < INFINITY ? kSumFine : kSumOdd;
+}
+template <typename T>
+__device__ __forceinline__ bool prompt_row_right(const PromptArgs& a, int q_row, int head, int k0, int seen, int sums) {
+  const int lane = threadIdx.x % 32, kv = static_cast<int>(a.ratio.of(head));
+  bool right = false;
+  if (sums == kSumFine) {
+    const T* out = static_cast<const T*>(a.out) + (static_cast<long long>(q_row) * a.hq + head) * a.d;
+    float y[8];
+    unsigned open = 0;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      y[c] = lane + 32 * c < a.d ? to_f32(out[lane + 32 * c]) : 0.0f;
+      open |= fabsf(y[c]) < INFINITY ? 0u : 1u << c;
+    }
+    Odd values;
+    for (int at = 0; at < seen && __any_sync(~0u, open & ~values.nan); at += kScanRows)
+      warp_scan(values, static_cast<const T*>(a.v) + k0 * a.v_ts + kv * a.v_hs, a.v_ts, at, seen, a.d);
+    right = true;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const unsigned why = y[c] != y[c] ? values.nan | (values.plus & values.minus)
+                                        : (y[c] > 0.0f ? values.plus & ~values.minus : values.minus & ~values.plus) & ~values.nan;
+      right = right && !((open & ~why) >> c & 1);
+    }
+    right = __all_sync(~0u, right);
+  } else if (sums == kSumNaN) {
+    Odd query, keys;
+    warp_scan(query, static_cast<const T*>(a.q) + head * a.q_hs, a.q_ts, q_row, q_row + 1, a.d);
+    bool nan = __any_sync(~0u, query.nan != 0);
+    for (int at = 0; at < seen && !nan; at += kScanRows) {
+      warp_scan(keys, static_cast<const T*>(a.k) + k0 * a.k_ts + kv * a.k_hs, a.k_ts, at, seen, a.d);
+      nan = __any_sync(~0u, keys.nan != 0);
+    }
+    right = nan || !__any_sync(~0u, (query.large | keys.large) != 0);
+  }
+  return right;
+}
+template <typename T>
+__device__ __noinline__ void prompt_row_again(const PromptArgs& a, int q_row, int head, int k0, int seen_and_sums) {
+  const int seen = seen_and_sums & 0x3fffffff;
+  if (!prompt_row_right<T>(a, q_row, head, k0, seen, static_cast<int>(static_cast<unsigned>(seen_and_sums) >> 30)))
+    prompt_row_with_care<T>(a, q_row, head, k0, seen);
+}
+// The rows of a warp, each in the lane of its bit.
+template <typename T>
+__device__ __forceinline__ void prompt_rows_again(const PromptArgs& a, unsigned rows, int q_row, int head, int k0, int seen, int sums) {
+  for (rows &= ~__ballot_sync(~0u, sums == kSettled); rows; rows &= rows - 1) {
+    const int from = __ffs(rows) - 1;
+    prompt_row_again<T>(a, __shfl_sync(~0u, q_row, from), __shfl_sync(~0u, head, from), k0,
+                        __shfl_sync(~0u, static_cast<int>(static_cast<unsigned>(seen) | static_cast<unsigned>(sums) << 30), from));
+  }
 }
 
 // Adds up the parts of a row: one warp a row, lanes over channels.
@@ -257,9 +354,11 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
     }
   if (a.lse && lane == 0) a.lse[row] = seen ? (top + log2f(total)) * (1.0f / kLog2e) : -INFINITY;
   __syncwarp();
-  if (seen && !__all_sync(~0u, fine)) {
+  // (where starts that are not in order gave rows to two sequences, the heads may be of neither)
+  if (seen > 0 && k0 >= 0 && seen <= a.tk - k0 && !__all_sync(~0u, fine)) {
     const int q_row = static_cast<int>(row / a.hq);
-    prompt_row_with_care<T>(a, q_row, static_cast<int>(row - static_cast<long long>(q_row) * a.hq), k0, seen);
+    prompt_rows_again<T>(a, 1u, q_row, static_cast<int>(row - static_cast<long long>(q_row) * a.hq), k0, seen,
+                         prompt_sums<T>(a, top, total));
   }
 }
 

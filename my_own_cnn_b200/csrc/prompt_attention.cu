@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
       }
       continue;
     }
-    const float by = l > 0.0f ? 1.0f / l : 0.0f;
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
     bool fine = l > 0.0f && l < INFINITY;
     if (r < rows) {
 #pragma unroll
@@ -351,11 +351,7 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
     again |= again >> 1;
     again = (again | again >> 2) & 0x11111111u;  // one bit a row
     __syncwarp();
-    for (; again; again &= again - 1) {
-      const int from = __ffs(again) - 1;
-      prompt_row_with_care<T>(a, u.s.q0 + __shfl_sync(~0u, token, from), __shfl_sync(~0u, head, from), u.s.k0,
-                              min(u.s.lk, __shfl_sync(~0u, seen[h], from)));
-    }
+    if (again) prompt_rows_again<T>(a, again, u.s.q0 + token, head, u.s.k0, min(u.s.lk, seen[h]), prompt_sums<T>(a, top[h], l));
   }
 }
 

@@ -133,6 +133,44 @@ def test_what_is_masked_has_no_part(cuda_lib, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lq", [2500, 40])
+def test_what_is_seen_and_not_finite(cuda_lib, dtype, lq):
+    """NaN and infinities early in a long prompt (all of its rows, or the last 40 over the same keys): the results that see them, no
+    others, with the log-sums and without."""
+    n, hq, hk, d = 2500, 8, 2, 64
+    q, k, v = make(n, n, hq, hk, d, dtype, 3)
+    ends = starts_of([lq]), starts_of([n])
+    call = lambda **kw: b2q.prompt_attention(q[n - lq:], k, v, *ends, **kw)
+    clean, clean_lse = call(return_lse=True)
+    most = float(v.abs().max())
+    unit = 3 * UNIT[dtype] + (n / 4 + 16) * 2.0 ** -22  # as above
+    v[3, 0, 5] = math.nan
+    v[4, 1, 6], v[900, 1, 6], v[70, 1, 40] = math.inf, -math.inf, -math.inf
+    out, lse = call(return_lse=True)
+    at = torch.arange(n - lq, n, device="cuda")
+    assert out[at >= 3, :4, 5].isnan().all() and out[at >= 900, 4:, 6].isnan().all()
+    assert (out[(at >= 4) & (at < 900), 4:, 6] == math.inf).all() and (out[at >= 70, 4:, 40] == -math.inf).all()
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[at >= 3, :4, 5] = True
+    hit[at >= 4, 4:, 6] = True
+    hit[at >= 70, 4:, 40] = True
+    assert (out[~hit].double() - clean[~hit].double()).abs().max() < most * unit
+    within(lse, clean_lse, torch.full_like(lse, 2.0 ** -16))
+    assert torch.equal(call().view(torch.uint8), out.view(torch.uint8))
+    # keys: a NaN, and an infinity in one channel, whose sign in the scores is the query's
+    k[1200, 1, 2] = math.nan
+    k[700, 0, 9] = math.inf
+    out, lse = call(return_lse=True)
+    up = (q[n - lq:, :4, 9] > 0) & (at >= 700)[:, None]
+    down = (q[n - lq:, :4, 9] < 0) & (at >= 700)[:, None]
+    assert out[at >= 1200, 4:].isnan().all() and lse[at >= 1200, 4:].isnan().all()
+    assert out[:, :4][up].isnan().all() and (lse[:, :4][up] == math.inf).all()
+    sees = out[:, :4][down]
+    assert sees[:, 5].isnan().all() and sees[:, :5].isfinite().all() and lse[:, :4][down].isfinite().all()
+    assert torch.equal(call().isnan(), out.isnan())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_large_scores_and_scales(cuda_lib, dtype):
     """Rows whose weight lies on one key, maxima that grow along the row, a scale of zero, a negative one."""
     n = 400
