@@ -9,7 +9,9 @@
 //
 // Bytes bound it: x (and the residual) in, the sum and one byte an element out.  A row lies in the registers of W warps from its only
 // read to its writes, 16 bytes a load and 16 or 32 elements a lane; both reductions meet in one
-// barrier.
+// barrier.  8192 x 4096 fp16 with a residual: 44 us for 235 MB, 5.3 TB/s (82 % of what a copy reaches), at 61 % of the issue
+// slots; read_s8 of the same 18.5 us for 101 MB, 5.4 TB/s.  Few rows are one latency chain (4 x 4096: 3.5 us); rows that do not
+// start on 16 bytes are read by elements (1021 x 5003 fp32 and its read: 15.5 us, half of the copy rate).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
