@@ -352,3 +352,17 @@ def test_parts_in_a_graph_beside_cache_attention(cuda_lib, dtype):
     with pytest.raises(RuntimeError, match="scratch"):
         with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=fresh):
             b2q.prompt_attention(q, k, v, starts, k_starts)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_bad_starts_where_keys_are_in_parts(cuda_lib, dtype):
+    """Rows that two sequences claim are nobody's; what lies outside stays, and the stream's scratch is as it was for the next call."""
+    q, k, v = make(40, 6000, 2, 1, 64, dtype)
+    for rows in ([0, 20, 10, 28], [0, 28, 0, 28], [28, 0, 28, 5]):
+        out = torch.full((40, 2, 64), 7.0, device="cuda", dtype=dtype)
+        starts = torch.tensor(rows, dtype=torch.int32, device="cuda")
+        b2q.prompt_attention(q, k, v, starts, torch.tensor([0, 2000, 4000, 6000], dtype=torch.int32, device="cuda"), out=out)
+        with pytest.raises(b2q.B200QError, match="starts"):
+            b2q.device_error()
+        assert (out[28:] == 7).all()
+        check(q, k, v, starts_of([10, 30]), starts_of([2500, 3500]))
