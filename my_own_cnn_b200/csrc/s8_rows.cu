@@ -307,7 +307,7 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(256) read_s8_kernel(ReadArgs a, uint32_t units) {
   wait_for_previous();
   constexpr int kApart = VEC == 1 ? 8 : 1;
-  const uint32_t unit = VEC == 1 ? (blockIdx.x * 256u + threadIdx.x) / 32 : blockIdx.x * 256u + threadIdx.x;
+  const uint32_t unit = VEC == 1 ? blockIdx.x * 8u + threadIdx.x / 32 : blockIdx.x * 256u + threadIdx.x;  // fewer than 2^31
   if (unit >= units) return;
   const uint32_t row = a.chunks.of(unit);
   const int c = VEC == 1 ? static_cast<int>(unit - row * a.chunks.d) * 256 + threadIdx.x % 32 : static_cast<int>(unit - row * a.chunks.d) * VEC;
