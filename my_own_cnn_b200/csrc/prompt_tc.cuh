@@ -246,9 +246,9 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
 #pragma unroll
         for (int k = 2; k < kHalf - 2; k += 4) m[0] = max3(m[0], s(k), s(k + 1)), m[1] = max3(m[1], s(k + 2), s(k + 3));
         const float top = max3(fmaxf(m[0], m[1]), s(kHalf - 2), s(kHalf - 1)) * c;  // -inf: nothing seen here
-        if (t == 0) {
-          ref = top == -INFINITY ? 0.0f : top;
-        } else if (__any_sync(~0u, top - ref > kSlack)) {
+        // nothing but scores of -inf so far: the sums are zero at any reference
+        if (sum == 0.0f) ref = top == -INFINITY ? 0.0f : top;
+        if (__any_sync(~0u, top - ref > kSlack)) {  // never at t = 0: there are no sums yet
           const float now = top - ref > kSlack ? top : ref, keep = exp2_approx(ref - now);
           if (!wait(o_done + 8 * i, (done + t - 1) & 1, kCode)) break;
           tc_fence_after();
