@@ -1,0 +1,37 @@
+"""prompt_attention where values, scores and weights lie at the ends of their ranges; bounds are s8_ref's unless a test derives its own."""
+import math
+
+import pytest
+import torch
+
+import my_own_cnn_b200 as b2q
+from tests import s8_ref
+from tests.lowbit_ref import within
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def starts_of(*lens):
+    return torch.tensor([0, *lens]).cumsum(0).to(torch.int32).cuda()
+
+
+def make(tq, tk, hq, hk, d, dtype, seed=0, size=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [(torch.randn(n, h, d, generator=g, device="cuda") * s).to(dtype) for n, h, s in ((tq, hq, size), (tk, hk, 1), (tk, hk, 1))]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lq,lk,cut", [(50, 300, 64), (50, 300, 70), (50, 300, 130), (140, 700, 500), (28, 7000, 3000)])
+def test_keys_masked_by_scores_of_minus_infinity(cuda_lib, dtype, d, lq, lk, cut):
+    """The first keys' scores are -inf (a key of -inf in a channel that is 1 in all queries), the others' about -40: softmax of the
+    others alone, whatever lies between them and 0."""
+    q, k, v = make(lq, lk, 2, 1, d, dtype, d, 0.1)
+    q[:, :, :2] = 1
+    k[:, :, 0], k[:, :, 1] = 0, -40
+    k[:cut, :, 0] = -math.inf
+    out, lse = b2q.prompt_attention(q, k, v, starts_of(lq), starts_of(lk), 1.0, return_lse=True)
+    want, want_lse, ob, lb = s8_ref.attention(q, k[cut:], v[cut:], starts_of(lq), starts_of(lk - cut), 1.0, dtype)
+    within(out, want, ob)
+    within(lse, want_lse, lb)
