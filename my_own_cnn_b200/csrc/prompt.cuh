@@ -22,7 +22,7 @@ struct PromptArgs {
   Divisor tile;
   long long most_units;  // key heads times tiles times parts, as many as there may be
   int parts;             // of each tile's keys; with more than one the sums meet in part_*, [parts][tq * hq]
-  float4* part_heads;    // reference (of base 2), sum of weights, the bits of the row's first key and of how many it sees
+  float4* part_heads;    // reference (of base 2; -inf: sees none here), sum of weights, the bits of the row's first key and of how many it sees
   float* part_sums;      // [..][d]
   unsigned* arrived;     // [tq * hq] parts that have been written: zero before and after
   float scale;
@@ -87,9 +87,11 @@ __device__ __forceinline__ int2 part_steps(const PromptArgs& a, int steps, int p
   return make_int2(static_cast<int>(static_cast<long long>(steps) * part / a.parts),
                    static_cast<int>(static_cast<long long>(steps) * (part + 1) / a.parts));
 }
-// What a part says of a row; the join counts on all of them.
-__device__ __forceinline__ void part_head(const PromptArgs& a, int part, long long row, float ref, float sum, int k0, int seen) {
-  a.part_heads[part * static_cast<long long>(a.tq) * a.hq + row] = make_float4(ref, sum, __int_as_float(k0), __int_as_float(seen));
+// What a part says of a row; the join counts on all of them.  `saw`: the row sees some of its keys.  Where it does and their scores are
+// all -inf the sum is zero and the reference any number; where not, it is -inf.
+__device__ __forceinline__ void part_head(const PromptArgs& a, int part, long long row, bool saw, float ref, float sum, int k0, int seen) {
+  const float from = !saw ? -INFINITY : sum == 0.0f ? 0.0f : ref;
+  a.part_heads[part * static_cast<long long>(a.tq) * a.hq + row] = make_float4(from, sum, __int_as_float(k0), __int_as_float(seen));
   atomicAdd(a.arrived + row, 1u);
 }
 
@@ -327,7 +329,8 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
   // a lane has a part's head; up to 32 parts
   float4 head = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
   if (lane < a.parts) head = a.part_heads[lane * rows + row];
-  float top = head.y == 0.0f ? -INFINITY : head.x;  // a part that sees nothing has no say
+  const bool saw = head.x != -INFINITY;
+  float top = head.y == 0.0f ? -INFINITY : head.x;
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(~0u, top, o));
   const float w = head.y == 0.0f ? 0.0f : exp2_approx(head.x - top);
@@ -336,7 +339,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
 #pragma unroll 2
   for (int p = 0; p < a.parts; ++p) {
     const float wp = __shfl_sync(~0u, w, p);
-    if (wp == 0.0f) continue;
+    if (!__shfl_sync(~0u, saw, p)) continue;  // no sums; a weight that is zero alone lets a NaN or an infinity through, as in one part
     const float* from = a.part_sums + (p * rows + row) * a.d;
 #pragma unroll
     for (int c = 0; c < 8; ++c)

@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
     const long long at = static_cast<long long>(u.s.q0 + token) * a.hq + head;
     if (a.parts > 1) {
       if (r < rows) {
-        if (t == 0) part_head(a, part, at, top[h], l, u.s.k0, min(u.s.lk, seen[h]));
+        if (t == 0) part_head(a, part, at, most > least && seen[h] > least, top[h], l, u.s.k0, min(u.s.lk, seen[h]));
         float* sums = a.part_sums + (part * static_cast<long long>(a.tq) * a.hq + at) * a.d;
 #pragma unroll
         for (int n = 0; n < D / 8; ++n)

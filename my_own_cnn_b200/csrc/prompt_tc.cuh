@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
       tc_fence_after();
       if (a.parts > 1) {
         const long long row_at = static_cast<long long>(u.s.q0 + token) * a.hq + head;
-        if (mine) part_head(a, u.part, row_at, ref - kLift, sum, u.s.k0, seen);
+        if (mine) part_head(a, u.part, row_at, n && seen > u.from * kTcKeys, ref - kLift, sum, u.s.k0, seen);
         float* sums = a.part_sums + (u.part * static_cast<long long>(a.tq) * a.hq + row_at) * a.d;
 #pragma unroll 1
         for (int k = 0; n && k < a.d; k += 32) {

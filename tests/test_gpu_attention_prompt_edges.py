@@ -35,3 +35,35 @@ def test_keys_masked_by_scores_of_minus_infinity(cuda_lib, dtype, d, lq, lk, cut
     want, want_lse, ob, lb = s8_ref.attention(q, k[cut:], v[cut:], starts_of(lq), starts_of(lk - cut), 1.0, dtype)
     within(out, want, ob)
     within(lse, want_lse, lb)
+
+
+def same_kind(a, b):
+    """NaN and infinities in the same places."""
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(a == math.inf, b == math.inf) and torch.equal(a == -math.inf, b == -math.inf)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("low", [-30.0, -200.0])
+def test_values_under_weights_that_vanish(cuda_lib, dtype, d, low):
+    """A NaN and an infinity among values whose keys' scores lie far below the others' (their weights are zero in fp32 at -200): what the
+    row gives does not depend on the parts that its keys are cut into.  160 heads of the same numbers are not cut."""
+    q, k, v = make(8, 6000, 2, 1, d, dtype, d)
+    q[:, :, 0] = 1
+    k[:, :, 0] = 0
+    k[:1000, :, 0] = low
+    v[10, 0, 5] = math.nan
+    v[11, 0, 6] = math.inf
+    v[5995, 0, 7] = -math.inf  # at a weight above zero, seen by some rows
+    ends = starts_of(8), starts_of(6000)
+    out, lse = b2q.prompt_attention(q, k, v, *ends, 1.0, return_lse=True)
+    whole, whole_lse = b2q.prompt_attention(q.repeat(1, 80, 1), k.expand(6000, 160, d), v.expand(6000, 160, d), *ends, 1.0, return_lse=True)
+    assert out[:, :, 5].isnan().all()
+    assert same_kind(out, whole[:, :2]) and lse.isfinite().all()
+    assert (out[3:, :, 7] == -math.inf).all() and out[:3, :, 7].isfinite().all()
+    # the rest is the softmax of what is left without the three channels
+    keep = [c for c in range(d) if c not in (5, 6, 7)]
+    want, want_lse, ob, lb = s8_ref.attention(q, k, v.nan_to_num(0, 0, 0), *ends, 1.0, dtype)
+    within(out[..., keep], want[..., keep], ob[..., keep])
+    within(whole[:, :2][..., keep], want[..., keep], ob[..., keep])
+    within(lse, want_lse, lb)
