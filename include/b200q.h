@@ -344,7 +344,8 @@ int b200q_linear_s8(const b200q_linear_s8_args* args, void* stream);
  * h / (hq / hk).  out contiguous [tq][hq][d]; lse fp32 [tq][hq] or NULL: log of the sum of exp(scale * q.k).
  * Rows outside every sequence are left as they are.  A sequence whose starts decrease or pass the rows is left out and
  * reported by b200q_device_error().  What a row does not see has no part in it, NaN and infinities among it.
- * d up to 256.  Uses the stream's scratch where few rows see many keys: their parts are joined by a second kernel. */
+ * d up to 256; scale and its product with log2(e) finite.  Uses the stream's scratch where few rows see many keys: their parts are
+ * joined by a second kernel. */
 typedef struct b200q_prompt_attention_args {
   const void* q;
   int64_t q_ts, q_hs;

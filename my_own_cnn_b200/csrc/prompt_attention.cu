@@ -426,7 +426,8 @@ extern "C" int b200q_prompt_attention(const b200q_prompt_attention_args* p, void
   if (p->ftype < B200Q_F32 || p->ftype > B200Q_BF16) return host_fail(B200Q_ERR_INVALID_ARG, "bad floating type %d", p->ftype);
   if (p->b < 0 || p->tq < 0 || p->tk < 0 || p->hq < 0 || p->hk < 0) return host_fail(B200Q_ERR_INVALID_ARG, "negative dimensions");
   if (p->d < 1 || p->d > 256) return host_fail(B200Q_ERR_UNSUPPORTED, "heads of 1 to 256 channels, got %d", p->d);
-  if (!std::isfinite(p->scale)) return host_fail(B200Q_ERR_INVALID_ARG, "the scale must be finite");
+  if (!std::isfinite(p->scale * kLog2e))  // exponents are of base 2
+    return host_fail(B200Q_ERR_INVALID_ARG, "the scale must be finite, its product with log2(e) too, got %g", static_cast<double>(p->scale));
   if (p->b == 0 || p->tq == 0 || p->hq == 0) return B200Q_OK;
   if (p->hk == 0 || p->hq % p->hk)
     return host_fail(B200Q_ERR_INVALID_ARG, "%d key heads do not divide %d query heads", p->hk, p->hq);

@@ -2,6 +2,8 @@
 (or beside) their way into a cache."""
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -25,7 +27,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     keys, where a sequence has more (an earlier part) or fewer of them than queries.  A sequence's last query is in line with its
     last key: query j of lq sees the first lk - lq + j + 1 keys; where that is none the output is 0 (lse -inf).  Query head
     h reads head h // (hq / hk).  Rows outside every sequence are left as they are in `out`.  A sequence whose
-    starts decrease or pass the tensors is left out and reported by device_error().  scale: 1 / sqrt(d) when None.
+    starts decrease or pass the tensors is left out and reported by device_error().  scale: 1 / sqrt(d) when None; its product
+    with log2(e) has to be finite in fp32.
     Returns out [tq, hq, d], and lse fp32 [tq, hq] (log of the sum of exp(scale * q.k)) when return_lse.  out shares no memory
     with the other tensors; starts stay as they are until the call has run.
 
@@ -63,8 +66,12 @@ def _attention(q, k, v, starts, k_starts, scale, out, return_lse, ft, shape, str
         raise RuntimeError(f"out must be a contiguous {q.dtype} {list(shape)} CUDA tensor")
     lse = starts.new_empty((tq, hq), dtype=torch.float32) if return_lse else None
     (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.stride(), k.stride(), v.stride()
+    if scale is None:
+        scale = d ** -0.5 if d else 1.0
+    elif abs(scale) > 3e38:  # not an fp32: as what it would round to
+        scale = math.inf
     _lib.check(_lib.lib().b200q_prompt_attention(
         _ARGS.pack(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, starts.data_ptr(),
                    0 if k_starts is None else k_starts.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0, ft,
-                   starts.shape[0] - 1, tq, k.shape[0], hq, k.shape[1], d, d ** -0.5 if scale is None else scale), handle))
+                   starts.shape[0] - 1, tq, k.shape[0], hq, k.shape[1], d, scale), handle))
     return (out, lse) if return_lse else out

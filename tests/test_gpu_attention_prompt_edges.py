@@ -67,3 +67,20 @@ def test_values_under_weights_that_vanish(cuda_lib, dtype, d, low):
     within(out[..., keep], want[..., keep], ob[..., keep])
     within(whole[:, :2][..., keep], want[..., keep], ob[..., keep])
     within(lse, want_lse, lb)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scales_at_the_end_of_the_range(cuda_lib, dtype):
+    """2.3e38 is the largest that is taken, in size: scores of zero are all alike."""
+    q, k, v = make(300, 300, 2, 1, 64, dtype)
+    for scale in (2.4e38, -3e38, 1e39, math.inf, math.nan):
+        with pytest.raises(RuntimeError, match="scale"):
+            b2q.prompt_attention(q, k, v, starts_of(300), scale=scale)
+    k.zero_()
+    for scale in (2.3e38, -2.3e38):
+        out, lse = b2q.prompt_attention(q, k, v, starts_of(300), scale=scale, return_lse=True)
+        want, want_lse, ob, lb = s8_ref.attention(q, k, v, starts_of(300), starts_of(300), scale, dtype)
+        within(out, want, ob)
+        within(lse, want_lse, lb)
+    with pytest.raises(RuntimeError, match="256"):
+        b2q.prompt_attention(q[..., :0], k[..., :0], v[..., :0], starts_of(300))
