@@ -346,8 +346,10 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
       const bool fine = !seen || (sum > 0.0f && sum < INFINITY && zero.x == 0.0f && zero.y == 0.0f);
       if (a.lse && mine)
         a.lse[static_cast<long long>(u.s.q0 + token) * a.hq + head] = seen ? (ref - kLift + log2f(sum)) * (1.0f / kLog2e) : -INFINITY;
-      if (const unsigned rows = __ballot_sync(~0u, !fine); __builtin_expect(rows != 0, 0))
+      if (const unsigned rows = __ballot_sync(~0u, !fine); __builtin_expect(rows != 0, 0)) {
+        __syncwarp();  // these results and log-sums before those that other lanes write in their place
         prompt_rows_again<T>(a, rows, u.s.q0 + token, head, u.s.k0, seen, prompt_sums<T>(a, ref, sum));
+      }
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
