@@ -32,6 +32,11 @@ struct PromptArgs {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// A row's log-sum from its reference (base 2) and its sum.  With a score of +inf the sum is NaN.
+__device__ __forceinline__ float log_sum(float top, float sum) {
+  return top == INFINITY ? top : (top + log2f(sum)) * (1.0f / kLog2e);
+}
+
 // A sequence's rows; empty where its starts are not in order or pass the tensors.
 struct Sequence {
   int q0, lq, k0, lk;
@@ -252,15 +257,15 @@ __device__ __forceinline__ void warp_scan(Odd& found, const T* base, long long t
 // takes a read of the values up to the first NaN (or all that the row sees), where a row with care costs all keys and values: 8192 tokens,
 // 32 / 8 heads of 128, bf16 take 0.53 ms; with a NaN in the first key as long, in the first value 0.66 ms, in value 4096 79 ms, with an
 // infinity in the first value 170 ms; all rows with care would be minutes.
-//   - The sum of the weights is NaN: a score is, and so is all of the row.  (A score of +inf gives the same row, but its log-sum is
-//     +inf unless there is a NaN as well; one that passes fp32 by the factor log2(e) alone is finite.)  In fp32 a score is NaN also
-//     where a factor is infinite, or rounds to a first term that is: its terms are.
+//   - The sum of the weights is NaN.  So is the row's reference where a score is, and all of the row.  A reference of +inf: a score is, and none
+//     is NaN; the row is NaN, its log-sum +inf.  (A score may also pass fp32 by the factor |scale| log2(e), where that is above 1: such a row
+//     is done with care.)  In fp32 a score is NaN also where a factor is infinite: its terms are.
 //   - A channel is NaN or infinite, and the values that the row sees have the NaN or the infinities that make it so.
 enum { kSumOdd = 0, kSumFine = 1, kSumNaN = 2, kSettled = 3 };
 template <typename T>
 __device__ __forceinline__ int prompt_sums(const PromptArgs& a, float top, float sum) {
-  if (sum != sum)
-    return top != INFINITY || (!a.lse && fabsf(a.scale) * kLog2e <= 1.0f) ? (sizeof(T) == 4 ? kSumNaN : kSettled) : kSumOdd;
+  if (top != top) return sizeof(T) == 4 ? kSumNaN : kSettled;
+  if (top == INFINITY) return fabsf(a.scale) * kLog2e <= 1.0f ? kSettled : kSumOdd;
   return sum > 0.0f && sum < INFINITY ? kSumFine : kSumOdd;
 }
 template <typename T>
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
       fine = fine && fabsf(y) < INFINITY;
       out[lane + 32 * c] = from_f32<T>(y);
     }
-  if (a.lse && lane == 0) a.lse[row] = seen ? (top + log2f(total)) * (1.0f / kLog2e) : -INFINITY;
+  if (a.lse && lane == 0) a.lse[row] = seen ? log_sum(top, total) : -INFINITY;
   __syncwarp();
   // (where starts that are not in order gave rows to two sequences, the heads may be of neither)
   if (seen > 0 && k0 >= 0 && seen <= a.tk - k0 && !__all_sync(~0u, fine)) {

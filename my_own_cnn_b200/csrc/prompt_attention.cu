@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
           fine = fine && fabsf(y) < INFINITY;
           if (n * 8 + 2 * t + e < a.d) static_cast<T*>(a.out)[at * a.d + n * 8 + 2 * t + e] = from_f32<T>(seen[h] ? y : 0.0f);
         }
-      if (a.lse && t == 0) a.lse[at] = seen[h] ? (top[h] + log2f(l)) * (1.0f / kLog2e) : -INFINITY;
+      if (a.lse && t == 0) a.lse[at] = seen[h] ? log_sum(top[h], l) : -INFINITY;
     }
     unsigned again = __ballot_sync(~0u, r < rows && seen[h] && !fine);
     again |= again >> 1;

@@ -86,9 +86,10 @@ __device__ __forceinline__ void loaded(uint32_t (&v)[32]) {
                  "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]));
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// NaN if one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
         float m[2] = {s(0), s(1)};
 #pragma unroll
         for (int k = 2; k < kHalf - 2; k += 4) m[0] = max3(m[0], s(k), s(k + 1)), m[1] = max3(m[1], s(k + 2), s(k + 3));
-        const float top = max3(fmaxf(m[0], m[1]), s(kHalf - 2), s(kHalf - 1)) * c;  // -inf: nothing seen here
+        const float top = max3(max_nan(m[0], m[1]), s(kHalf - 2), s(kHalf - 1)) * c;  // -inf: nothing seen here
         // nothing but scores of -inf so far: the sums are zero at any reference
         if (sum == 0.0f) ref = top == -INFINITY ? 0.0f : top;
         if (__any_sync(~0u, top - ref > kSlack)) {  // never at t = 0: there are no sums yet
@@ -265,6 +266,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
           sum *= keep;
           ref = now;
         }
+        if (top != top) ref = top;  // a score that is NaN: the row's, whatever else there is
         const float less = kLift - ref;
         float add[4] = {};
         uint32_t w[32];
@@ -345,7 +347,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
       }
       const bool fine = !seen || (sum > 0.0f && sum < INFINITY && zero.x == 0.0f && zero.y == 0.0f);
       if (a.lse && mine)
-        a.lse[static_cast<long long>(u.s.q0 + token) * a.hq + head] = seen ? (ref - kLift + log2f(sum)) * (1.0f / kLog2e) : -INFINITY;
+        a.lse[static_cast<long long>(u.s.q0 + token) * a.hq + head] = seen ? log_sum(ref - kLift, sum) : -INFINITY;
       if (const unsigned rows = __ballot_sync(~0u, !fine); __builtin_expect(rows != 0, 0)) {
         __syncwarp();  // these results and log-sums before those that other lanes write in their place
         prompt_rows_again<T>(a, rows, u.s.q0 + token, head, u.s.k0, seen, prompt_sums<T>(a, ref, sum));

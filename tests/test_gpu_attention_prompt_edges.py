@@ -84,3 +84,46 @@ def test_scales_at_the_end_of_the_range(cuda_lib, dtype):
         within(lse, want_lse, lb)
     with pytest.raises(RuntimeError, match="256"):
         b2q.prompt_attention(q[..., :0], k[..., :0], v[..., :0], starts_of(300))
+
+
+def best_ms(call, times=3):
+    call()
+    best = math.inf
+    for _ in range(times):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        call()
+        end.record()
+        end.synchronize()
+        best = min(best, start.elapsed_time(end))
+    return best
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lq,inf,nan", [(500, 3, 300), (500, 300, 3), (500, 130, 131), (20, 3, 3990), (20, 3990, 3), (20, 1000, 2000)])
+def test_log_sums_of_infinite_scores(cuda_lib, dtype, d, lq, inf, nan):
+    """A score of +inf gives the log-sum +inf unless another one is NaN, and a NaN row either way; -inf has no part in it.  Rows of 500
+    keys, and the last 20 of 4000 (in parts)."""
+    n = 500 if lq == 500 else 4000
+    q, k, v = make(lq, n, 4, 1, d, dtype, d)
+    k[inf, :, 9] = math.inf
+    k[nan, :, 2] = math.nan
+    out, lse = b2q.prompt_attention(q, k, v, starts_of(lq), starts_of(n), return_lse=True)
+    at = torch.arange(n - lq, n, device="cuda")[:, None]
+    bad = (at >= nan).expand(lq, 4)
+    up = (at >= inf) & ~bad & (q[..., 9] > 0)
+    assert lse[bad].isnan().all() and out[bad].isnan().all()
+    assert (lse[up] == math.inf).all() and out[up].isnan().all()
+    left = ~bad & ~up
+    assert lse[left].isfinite().all() and out[left].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("lse", [True, False])
+def test_an_infinite_key_costs_no_more(cuda_lib, dtype, lse):
+    """Every row sees a score of +inf or -inf."""
+    q, k, v = make(2048, 2048, 32, 8, 128, dtype)
+    clean = best_ms(lambda: b2q.prompt_attention(q, k, v, starts_of(2048), return_lse=lse))
+    k[3, :, 5] = math.inf
+    assert best_ms(lambda: b2q.prompt_attention(q, k, v, starts_of(2048), return_lse=lse)) < 10 * clean
