@@ -1,5 +1,7 @@
 // What the kernels of prompt attention share: arguments, the order of the work, rows that are done with care.
 #pragma once
+#include <climits>
+
 #include "host.h"
 #include "lowbit.cuh"
 
@@ -175,92 +177,114 @@ class Finder {
 };
 
 // One row of attention by one warp, from memory and with what the row sees alone.  A product of a weight of zero and a masked value is
-// zero only while the value is finite, so the fast kernels come here with the rows that they found not finite.  Lanes share out the
-// channels, four keys at a time are on their way.
-template <typename T>
-__device__ __forceinline__ void prompt_row_with_care(const PromptArgs& a, int q_row, int head, int k0, int seen) {
-  const int lane = threadIdx.x % 32, kv = static_cast<int>(a.ratio.of(head));
-  const T* k = static_cast<const T*>(a.k) + k0 * a.k_ts + kv * a.k_hs;
-  const T* v = static_cast<const T*>(a.v) + k0 * a.v_ts + kv * a.v_hs;
-  float q[8], o[8] = {}, top = -INFINITY, total = 0.0f;
+// zero only while the value is finite, so the fast kernels come here with rows that they found not finite and prompt_rows_right() cannot
+// explain.  C channels a lane (32 apart), 32 / C keys at a time: their partial sums are added up over the lanes and shared out to them in
+// one exchange, which leaves the score of a key in each C-th of the lanes.
+template <typename T, int C>
+__device__ __noinline__ void prompt_row_with_care(const PromptArgs& a, int q_row, int head, int k0, int seen) {
+  constexpr int kKeys = 32 / C;
+  const int lane = threadIdx.x % 32, kv = static_cast<int>(a.ratio.of(head)), d = a.d;
+  const long long k_ts = a.k_ts, v_ts = a.v_ts;
+  const float scale = a.scale;
+  const T* k = static_cast<const T*>(a.k) + k0 * k_ts + kv * a.k_hs;
+  const T* v = static_cast<const T*>(a.v) + k0 * v_ts + kv * a.v_hs;
+  const T* q_at = static_cast<const T*>(a.q) + q_row * a.q_ts + head * a.q_hs;
+  const T none = from_f32<T>(0.0f);
+  int col[C];  // what lies past d or past the keys is read from a place that there is, and left out
+  float q[C], o[C] = {}, top = -INFINITY, total = 0.0f;
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
-    q[c] = lane + 32 * c < a.d ? to_f32(static_cast<const T*>(a.q)[q_row * a.q_ts + head * a.q_hs + lane + 32 * c]) : 0.0f;
-  for (int j0 = 0; j0 < seen; j0 += 4) {
-    T y[4][8], x[4][8];
+  for (int c = 0; c < C; ++c) {
+    col[c] = min(lane + 32 * c, d - 1);
+    q[c] = lane + 32 * c < d ? to_f32(q_at[col[c]]) : 0.0f;
+  }
+  for (int j0 = 0; j0 < seen; j0 += kKeys) {
+    T x[kKeys][C], y[kKeys][C];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kKeys; ++i) {
+      const int at = min(j0 + i, seen - 1);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        y[i][c] = x[i][c] = from_f32<T>(0.0f);
-        if (j0 + i < seen && lane + 32 * c < a.d) {
-          y[i][c] = k[(j0 + i) * a.k_ts + lane + 32 * c];
-          x[i][c] = v[(j0 + i) * a.v_ts + lane + 32 * c];
-        }
+      for (int c = 0; c < C; ++c) {
+        x[i][c] = k[at * k_ts + col[c]];
+        y[i][c] = v[at * v_ts + col[c]];
       }
-    float s[4] = {};
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kKeys; ++i)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) s[i] = fmaf(q[c], to_f32(y[i][c]), s[i]);
+      for (int c = 0; c < C; ++c) {
+        if (lane + 32 * c >= d) x[i][c] = none;
+        if (j0 + i >= seen) y[i][c] = none;
+      }
+    float s[kKeys] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (j0 + i >= seen) break;
-      const float score = warp_sum(s[i]) * a.scale, now = max_nan(top, score);
-      const bool nothing = now == -INFINITY;  // all scores so far
-      const float keep = nothing ? 1.0f : expf(top - now), w = nothing ? 0.0f : expf(score - now);
-      top = now;
-      total = fmaf(total, keep, w);
+    for (int i = 0; i < kKeys; ++i)
 #pragma unroll
-      for (int c = 0; c < 8; ++c) o[c] = fmaf(w, to_f32(x[i][c]), o[c] * keep);
+      for (int c = 0; c < C; ++c) s[i] = fmaf(q[c], to_f32(x[i][c]), s[i]);
+    // lane l keeps key l / C
+#pragma unroll
+    for (int o2 = 16, n = kKeys / 2; o2 >= C; o2 >>= 1, n >>= 1) {
+      const bool upper = lane & o2;
+#pragma unroll
+      for (int i = 0; i < kKeys / 2; ++i)
+        if (i < n) {
+          const float keep = upper ? s[i + n] : s[i], give = upper ? s[i] : s[i + n];
+          s[i] = keep + __shfl_xor_sync(~0u, give, o2);
+        }
+    }
+#pragma unroll
+    for (int o2 = C / 2; o2; o2 >>= 1) s[0] += __shfl_xor_sync(~0u, s[0], o2);
+    const bool here = j0 + lane / C < seen;
+    const float score = here ? s[0] * scale : -INFINITY;
+    float now = score;
+#pragma unroll
+    for (int o2 = 16; o2 >= C; o2 >>= 1) now = max_nan(now, __shfl_xor_sync(~0u, now, o2));
+    now = max_nan(now, top);
+    const bool nothing = now == -INFINITY;  // all scores so far
+    const float keep = nothing ? 1.0f : expf(top - now), w = nothing || !here ? 0.0f : expf(score - now);
+    float sum = w;
+#pragma unroll
+    for (int o2 = 16; o2 >= C; o2 >>= 1) sum += __shfl_xor_sync(~0u, sum, o2);
+    top = now;
+    total = fmaf(total, keep, sum);
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] *= keep;
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+      const float wi = __shfl_sync(~0u, w, i * C);
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] = fmaf(wi, to_f32(y[i][c]), o[c]);
     }
     if (top != top) break;  // and stays so
   }
-  T* out = static_cast<T*>(a.out) + (static_cast<long long>(q_row) * a.hq + head) * a.d;
+  T* out = static_cast<T*>(a.out) + (static_cast<long long>(q_row) * a.hq + head) * a.d + lane;
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
-    if (lane + 32 * c < a.d) out[lane + 32 * c] = from_f32<T>(o[c] / total);
+  for (int c = 0; c < C; ++c)
+    if (lane + 32 * c < d) out[32 * c] = from_f32<T>(o[c] / total);
   if (a.lse && lane == 0)
     a.lse[static_cast<long long>(q_row) * a.hq + head] = fabsf(top) < INFINITY ? top + logf(total) : top;
 }
 
-// What warp_scan() looks for, a bit for each of a lane's channels (lane, lane + 32, ..).
-struct Odd {
-  unsigned nan = 0, plus = 0, minus = 0, large = 0;  // NaN, +inf, -inf; magnitudes of 2^100 and more
+// Where a channel of some keys (or values) of one head has its first NaN, +inf, -inf and magnitude of 2^100 or more.
+struct FirstOdd {
+  int nan = INT_MAX, plus = INT_MAX, minus = INT_MAX, large = INT_MAX;
+  __device__ __forceinline__ void see(float x, int at) {
+    if (fabsf(x) < 0x1p100f) return;
+    large = min(large, at);
+    if (x != x) nan = min(nan, at);
+    if (x == INFINITY) plus = min(plus, at);
+    if (x == -INFINITY) minus = min(minus, at);
+  }
 };
-// Some keys (or values) of one head from row `at` on, of `n`.
-constexpr int kScanRows = 2;
-template <typename T>
-__device__ __forceinline__ void warp_scan(Odd& found, const T* base, long long ts, int at, int n, int d) {
-  const int lane = threadIdx.x % 32;
-  T x[kScanRows][8];
-#pragma unroll
-  for (int i = 0; i < kScanRows; ++i)
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      x[i][c] = from_f32<T>(0.0f);
-      if (at + i < n && lane + 32 * c < d) x[i][c] = base[(at + i) * ts + lane + 32 * c];
-    }
-#pragma unroll
-  for (int i = 0; i < kScanRows; ++i)
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const float f = to_f32(x[i][c]);
-      found.nan |= f != f ? 1u << c : 0u;
-      found.plus |= f == INFINITY ? 1u << c : 0u;
-      found.minus |= f == -INFINITY ? 1u << c : 0u;
-      found.large |= fabsf(f) >= 0x1p100f ? 1u << c : 0u;
-    }
-}
 
-// A row that a fast kernel wrote and found not finite, by one warp.  Most such results are right as they are, and looking for the reason
-// takes a read of the values up to the first NaN (or all that the row sees), where a row with care costs all keys and values: 8192 tokens,
-// 32 / 8 heads of 128, bf16 take 0.53 ms; with a NaN in the first key as long, in the first value 0.66 ms, in value 4096 79 ms, with an
-// infinity in the first value 170 ms; all rows with care would be minutes.
+// Rows that a fast kernel wrote and found not finite, those of one warp: of one sequence and key head, each in the lane of its bit.
+// Returns the ones that are not right as they are.  Most are, and looking for the reason takes one read of the values for all of them
+// (up to where it is found), where a row with care costs all of its keys and values: 2048 tokens, 32 / 8 heads of 128, bf16 take 0.09 ms, with a
+// NaN or an infinity in value 3 0.13 to 0.23, in value 1024 0.32.
 //   - The sum of the weights is NaN.  So is the row's reference where a score is, and all of the row.  A reference of +inf: a score is, and none
 //     is NaN; the row is NaN, its log-sum +inf.  (A score may also pass fp32 by the factor |scale| log2(e), where that is above 1: such a row
 //     is done with care.)  In fp32 a score is NaN also where a factor is infinite: its terms are.
-//   - A channel is NaN or infinite, and the values that the row sees have the NaN or the infinities that make it so.
+//   - A channel is NaN, and a value that the row sees is, or two are infinities of both signs.  Or it is infinite, and a value that
+//     the row sees is the same (others would have made it NaN; what it does not see gives NaN or nothing).
 enum { kSumOdd = 0, kSumFine = 1, kSumNaN = 2, kSettled = 3 };
 template <typename T>
 __device__ __forceinline__ int prompt_sums(const PromptArgs& a, float top, float sum) {
@@ -268,61 +292,116 @@ __device__ __forceinline__ int prompt_sums(const PromptArgs& a, float top, float
   if (top == INFINITY) return fabsf(a.scale) * kLog2e <= 1.0f ? kSettled : kSumOdd;
   return sum > 0.0f && sum < INFINITY ? kSumFine : kSumOdd;
 }
-template <typename T>
-__device__ __forceinline__ bool prompt_row_right(const PromptArgs& a, int q_row, int head, int k0, int seen, int sums) {
-  const int lane = threadIdx.x % 32, kv = static_cast<int>(a.ratio.of(head));
-  bool right = false;
-  if (sums == kSumFine) {
-    const T* out = static_cast<const T*>(a.out) + (static_cast<long long>(q_row) * a.hq + head) * a.d;
-    float y[8];
-    unsigned open = 0;
+// The first odd places of a head's rows from k0 on, up to `n` or where `enough` (of every lane) says so.
+template <typename T, int C, typename F>
+__device__ __forceinline__ void scan_rows(FirstOdd (&first)[C], const T* base, long long ts, int n, int d, F enough) {
+  constexpr int kRows = 32 / C;
+  const int lane = threadIdx.x % 32;
+  int col[C];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      y[c] = lane + 32 * c < a.d ? to_f32(out[lane + 32 * c]) : 0.0f;
-      open |= fabsf(y[c]) < INFINITY ? 0u : 1u << c;
-    }
-    Odd values;
-    for (int at = 0; at < seen && __any_sync(~0u, open & ~values.nan); at += kScanRows)
-      warp_scan(values, static_cast<const T*>(a.v) + k0 * a.v_ts + kv * a.v_hs, a.v_ts, at, seen, a.d);
-    right = true;
+  for (int c = 0; c < C; ++c) col[c] = min(lane + 32 * c, d - 1);
+  for (int at = 0; at < n && !__all_sync(~0u, enough()); at += kRows) {
+    T x[kRows][C];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const unsigned why = y[c] != y[c] ? values.nan | (values.plus & values.minus)
-                                        : (y[c] > 0.0f ? values.plus & ~values.minus : values.minus & ~values.plus) & ~values.nan;
-      right = right && !((open & ~why) >> c & 1);
-    }
-    right = __all_sync(~0u, right);
-  } else if (sums == kSumNaN) {
-    Odd query, keys;
-    warp_scan(query, static_cast<const T*>(a.q) + head * a.q_hs, a.q_ts, q_row, q_row + 1, a.d);
-    bool nan = __any_sync(~0u, query.nan != 0);
-    for (int at = 0; at < seen && !nan; at += kScanRows) {
-      warp_scan(keys, static_cast<const T*>(a.k) + k0 * a.k_ts + kv * a.k_hs, a.k_ts, at, seen, a.d);
-      nan = __any_sync(~0u, keys.nan != 0);
-    }
-    right = nan || !__any_sync(~0u, (query.large | keys.large) != 0);
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[i][c] = base[min(at + i, n - 1) * ts + col[c]];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+#pragma unroll
+      for (int c = 0; c < C; ++c) first[c].see(to_f32(x[i][c]), min(at + i, n - 1));
   }
-  return right;
 }
-template <typename T>
-__device__ __noinline__ void prompt_row_again(const PromptArgs& a, int q_row, int head, int k0, int seen_and_sums) {
-  const int seen = seen_and_sums & 0x3fffffff;
-  if (!prompt_row_right<T>(a, q_row, head, k0, seen, static_cast<int>(static_cast<unsigned>(seen_and_sums) >> 30)))
-    prompt_row_with_care<T>(a, q_row, head, k0, seen);
+template <typename T, int C>
+__device__ __noinline__ unsigned prompt_rows_right(const PromptArgs& a, unsigned rows, int q_row, int head, int k0, int seen, int sums) {
+  const int lane = threadIdx.x % 32, kv = static_cast<int>(a.ratio.of(__shfl_sync(~0u, head, __ffs(rows) - 1)));
+  const unsigned fine = rows & __ballot_sync(~0u, sums == kSumFine), nan = rows & __ballot_sync(~0u, sums == kSumNaN);
+  unsigned left = rows & ~fine & ~nan;
+  const auto each = [](unsigned of, auto&& f) {
+    for (; of; of &= of - 1) f(__ffs(of) - 1);
+  };
+  if (fine) {
+    // a lane's channels that are NaN (bit c), +inf (8 + c), -inf (16 + c) in a row
+    const auto odd = [&](int row) {
+      const int at = __shfl_sync(~0u, q_row, row), h = __shfl_sync(~0u, head, row);
+      const T* out = static_cast<const T*>(a.out) + (static_cast<long long>(at) * a.hq + h) * a.d + lane;
+      unsigned r = 0;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const float y = lane + 32 * c < a.d ? to_f32(out[32 * c]) : 0.0f;
+        r |= y != y ? 1u << c : y == INFINITY ? 0x100u << c : y == -INFINITY ? 0x10000u << c : 0u;
+      }
+      return r;
+    };
+    unsigned open = 0;
+    each(fine, [&](int row) { open |= odd(row); });
+    FirstOdd first[C];
+    // whether a channel's reasons lie before `n`
+    const auto explained = [&](unsigned of, int n) {
+      bool yes = true;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if (of >> c & 1) yes = yes && (first[c].nan < n || max(first[c].plus, first[c].minus) < n);
+        if (of >> (8 + c) & 1) yes = yes && first[c].plus < n;
+        if (of >> (16 + c) & 1) yes = yes && first[c].minus < n;
+      }
+      return yes;
+    };
+    const int most = __reduce_max_sync(~0u, fine >> lane & 1 ? seen : 0);
+    scan_rows<T, C>(first, static_cast<const T*>(a.v) + k0 * a.v_ts + kv * a.v_hs, a.v_ts, most, a.d, [&] { return explained(open, INT_MAX); });
+    each(fine, [&](int row) {
+      if (!__all_sync(~0u, explained(odd(row), __shfl_sync(~0u, seen, row)))) left |= 1u << row;
+    });
+  }
+  if (nan) {
+    FirstOdd keys[C];
+    const auto any = [&](auto&& get) {
+      int at = INT_MAX;
+#pragma unroll
+      for (int c = 0; c < C; ++c) at = min(at, get(keys[c]));
+      return __reduce_min_sync(~0u, at);
+    };
+    const int most = __reduce_max_sync(~0u, nan >> lane & 1 ? seen : 0);
+    scan_rows<T, C>(keys, static_cast<const T*>(a.k) + k0 * a.k_ts + kv * a.k_hs, a.k_ts, most, a.d,
+                    [&] { return any([](const FirstOdd& f) { return f.nan; }) != INT_MAX; });
+    const int first_nan = any([](const FirstOdd& f) { return f.nan; }), first_large = any([](const FirstOdd& f) { return f.large; });
+    each(nan, [&](int row) {
+      const int at = __shfl_sync(~0u, q_row, row), h = __shfl_sync(~0u, head, row), n = __shfl_sync(~0u, seen, row);
+      const T* q = static_cast<const T*>(a.q) + at * a.q_ts + h * a.q_hs + lane;
+      FirstOdd query;
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (lane + 32 * c < a.d) query.see(to_f32(q[32 * c]), 0);
+      if (__any_sync(~0u, query.nan == 0) || first_nan < n) return;
+      if (__any_sync(~0u, query.large == 0) || first_large < n) left |= 1u << row;
+    });
+  }
+  return left;
 }
-// The rows of a warp, each in the lane of its bit.
+// The rows of a warp that are not finite, each in the lane of its bit.
+template <typename T, int C>
+__device__ __forceinline__ void prompt_rows_again_of(const PromptArgs& a, unsigned rows, int q_row, int head, int k0, int seen, int sums) {
+  rows = prompt_rows_right<T, C>(a, rows, q_row, head, k0, seen, sums);
+  for (; rows; rows &= rows - 1) {
+    const int from = __ffs(rows) - 1;
+    prompt_row_with_care<T, C>(a, __shfl_sync(~0u, q_row, from), __shfl_sync(~0u, head, from), k0, __shfl_sync(~0u, seen, from));
+  }
+}
 template <typename T>
 __device__ __forceinline__ void prompt_rows_again(const PromptArgs& a, unsigned rows, int q_row, int head, int k0, int seen, int sums) {
-  for (rows &= ~__ballot_sync(~0u, sums == kSettled); rows; rows &= rows - 1) {
-    const int from = __ffs(rows) - 1;
-    prompt_row_again<T>(a, __shfl_sync(~0u, q_row, from), __shfl_sync(~0u, head, from), k0,
-                        __shfl_sync(~0u, static_cast<int>(static_cast<unsigned>(seen) | static_cast<unsigned>(sums) << 30), from));
-  }
+  rows &= ~__ballot_sync(~0u, sums == kSettled);
+  if (!rows) return;
+  if (a.d <= 64)
+    prompt_rows_again_of<T, 2>(a, rows, q_row, head, k0, seen, sums);
+  else if (a.d <= 128)
+    prompt_rows_again_of<T, 4>(a, rows, q_row, head, k0, seen, sums);
+  else
+    prompt_rows_again_of<T, 8>(a, rows, q_row, head, k0, seen, sums);
 }
 
 // Adds up the parts of a row: one warp a row, lanes over channels.
 template <typename T>
-__global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ PromptArgs a) {
+__global__ void __launch_bounds__(256, 2) prompt_join_kernel(const __grid_constant__ PromptArgs a) {
   wait_for_previous();
   const long long rows = static_cast<long long>(a.tq) * a.hq, row = blockIdx.x * 8ll + threadIdx.x / 32;
   const int lane = threadIdx.x % 32;

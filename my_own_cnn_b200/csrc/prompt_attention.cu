@@ -450,7 +450,8 @@ extern "C" int b200q_prompt_attention(const b200q_prompt_attention_args* p, void
   a.b = p->b, a.tq = p->tq, a.tk = p->tk, a.hq = p->hq, a.hk = p->hk, a.d = p->d;
   a.ratio = Divisor(static_cast<uint32_t>(ratio));
   a.scale = p->scale;
-  // a warp whose 32 rows are done with care (see prompt_row_with_care) keeps others waiting, 820 clocks a row and key (4096 tokens)
+  // a warp whose 32 rows are done with care (see prompt_row_with_care) keeps others waiting: 300 clocks a row and key (2048 tokens), and
+  // 1024 allowed for
   a.limit = host_wait_limit() + 32ll * 1024 * p->tk;
   const cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const int size = p->ftype == B200Q_F32 ? 4 : 2;

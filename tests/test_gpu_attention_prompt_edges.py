@@ -127,3 +127,44 @@ def test_an_infinite_key_costs_no_more(cuda_lib, dtype, lse):
     clean = best_ms(lambda: b2q.prompt_attention(q, k, v, starts_of(2048), return_lse=lse))
     k[3, :, 5] = math.inf
     assert best_ms(lambda: b2q.prompt_attention(q, k, v, starts_of(2048), return_lse=lse)) < 10 * clean
+
+
+@pytest.mark.parametrize("dtype,value", [(torch.float32, math.nan)] + [(t, x) for t in TYPES[1:] for x in (math.nan, math.inf)])
+@pytest.mark.parametrize("place", [3, 1024])
+def test_a_value_that_is_not_finite_costs_little(cuda_lib, dtype, value, place):
+    """All rows from `place` on have one channel that is not finite; a warp finds the reason for all of its rows in one read."""
+    q, k, v = make(2048, 2048, 32, 8, 128, dtype)
+    call = lambda: b2q.prompt_attention(q, k, v, starts_of(2048))
+    clean = best_ms(call)
+    v[place, :, 5] = value
+    assert best_ms(call) < 10 * clean
+    out = call()
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[place:, :, 5] = True
+    assert out[~hit].isfinite().all() and not out[hit].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [1, 33, 64, 80, 128, 200, 256])
+def test_rows_done_again_key_by_key(cuda_lib, dtype, d):
+    """Poison in the middle of tiles: rows before it see none of it, those after see it (NaN, or two infinities) in some channels; what
+    is left of them is as without."""
+    n, hq, hk = 611, 6, 2
+    q, k, v = make(n, n, hq, hk, d, dtype, d)
+    starts = starts_of(n)
+    want, want_lse, ob, lb = s8_ref.attention(q, k, v, starts, starts, d ** -0.5, dtype)
+    for place in (0, 37, 300, 610):
+        bad = v.clone()
+        bad[place, 0, 0] = math.nan
+        bad[place // 2, 1, d // 2] = math.inf
+        bad[place, 1, d // 2] = -math.inf
+        out, lse = b2q.prompt_attention(q, k, bad, starts, return_lse=True)
+        hit = torch.zeros(n, hq, d, dtype=torch.bool)
+        hit[place:, :3, 0] = True
+        hit[place // 2:, 3:, d // 2] = True
+        assert out.cpu()[place:, :3, 0].isnan().all()
+        assert (out.cpu()[place // 2:place, 3:, d // 2] == math.inf).all()
+        after = out.cpu()[place:, 3:, d // 2]
+        assert after.isnan().all() if place // 2 < place else (after == -math.inf).all()
+        within(out.cpu()[~hit], want[~hit], ob[~hit])
+        within(lse, want_lse, lb)
