@@ -64,6 +64,9 @@ __device__ __forceinline__ void add_product(float (&c)[4], const uint32_t (&a)[4
 #pragma unroll
   for (int e = 0; e < 4; ++e) c[e] += r[e];
 }
+// The sum of the first terms' products and the others'.  Where a factor is infinite the others are NaN (its term times a zero) and the first
+// has the value.
+__device__ __forceinline__ float with_less(float first, float less) { return fabsf(first) == INFINITY ? first : first + less; }
 __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
 #pragma unroll
       for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] += less[n][e];
+        for (int e = 0; e < 4; ++e) s[n][e] = with_less(s[n][e], less[n][e]);
     }
     // softmax: the exponent's base is 2, the scale is in it
     float now[2] = {top[0], top[1]}, from[2];
@@ -311,7 +314,10 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
       }
       if constexpr (kTerms == 3) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[2 * n][e] += small[0][e], o[2 * n + 1][e] += small[1][e];
+        for (int e = 0; e < 4; ++e) {
+          o[2 * n][e] = with_less(o[2 * n][e], small[0][e]);
+          o[2 * n + 1][e] = with_less(o[2 * n + 1][e], small[1][e]);
+        }
       }
     }
   }

@@ -119,7 +119,7 @@ def test_log_sums_of_infinite_scores(cuda_lib, dtype, d, lq, inf, nan):
     assert lse[left].isfinite().all() and out[left].isfinite().all()
 
 
-@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lse", [True, False])
 def test_an_infinite_key_costs_no_more(cuda_lib, dtype, lse):
     """Every row sees a score of +inf or -inf."""
@@ -129,7 +129,8 @@ def test_an_infinite_key_costs_no_more(cuda_lib, dtype, lse):
     assert best_ms(lambda: b2q.prompt_attention(q, k, v, starts_of(2048), return_lse=lse)) < 10 * clean
 
 
-@pytest.mark.parametrize("dtype,value", [(torch.float32, math.nan)] + [(t, x) for t in TYPES[1:] for x in (math.nan, math.inf)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", [math.nan, math.inf])
 @pytest.mark.parametrize("place", [3, 1024])
 def test_a_value_that_is_not_finite_costs_little(cuda_lib, dtype, value, place):
     """All rows from `place` on have one channel that is not finite; a warp finds the reason for all of its rows in one read."""
@@ -168,3 +169,27 @@ def test_rows_done_again_key_by_key(cuda_lib, dtype, d):
         assert after.isnan().all() if place // 2 < place else (after == -math.inf).all()
         within(out.cpu()[~hit], want[~hit], ob[~hit])
         within(lse, want_lse, lb)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_infinite_values_in_fp32_cost_no_more(cuda_lib, d):
+    """Keys masked by a score of -inf and an infinite value in fp32, whose operands are three terms each: right, and at the speed of finite
+    ones."""
+    n, cut = 1024, 100
+    q, k, v = make(n, n, 16, 4, d, torch.float32, d)
+    q[:, :, 0] = 1
+    k[:, :, 0] = 0
+    rows = slice(cut, n)
+    ends = starts_of(n - cut), starts_of(n)
+    clean = best_ms(lambda: b2q.prompt_attention(q[rows], k, v, *ends, return_lse=True))
+    k[:cut, :, 0] = -math.inf
+    v[cut, :, 5] = math.inf
+    call = lambda: b2q.prompt_attention(q[rows], k, v, *ends, return_lse=True)
+    assert best_ms(call) < 5 * clean
+    out, lse = call()
+    assert (out[..., 5] == math.inf).all()
+    v[cut, :, 5] = 0
+    want, want_lse, ob, lb = s8_ref.attention(q[rows], k[rows], v[rows], ends[0], ends[0], d ** -0.5, torch.float32)
+    keep = [c for c in range(d) if c != 5]
+    within(out[..., keep], want[..., keep], ob[..., keep])
+    within(lse, want_lse, lb)
