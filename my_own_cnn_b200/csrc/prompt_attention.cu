@@ -195,9 +195,10 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
   using KV = Tile<T, D, kKeys>;
   constexpr bool kAhead = D == 64;
   float4 next_k[kAhead ? KV::kPieces : 1], next_v[kAhead ? KV::kPieces : 1];
+  // what lies behind the last key that the tile sees is zeros: a weight of zero would let a NaN or an infinity there through
   const auto key_rows = [&](const void* base, long long ts, long long hs, int j0) {
     return [=](int r) -> const T* {
-      return j0 + r < u.s.lk ? static_cast<const T*>(base) + (u.s.k0 + j0 + r) * ts + kv * hs : nullptr;
+      return j0 + r < all ? static_cast<const T*>(base) + (u.s.k0 + j0 + r) * ts + kv * hs : nullptr;
     };
   };
   if constexpr (kAhead) {

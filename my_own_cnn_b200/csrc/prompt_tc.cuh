@@ -421,6 +421,8 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
         const TcUnit u = unit_at(r, kCode);
         if (!u.ok) break;
         const int n = unit_halves(u, i, tokens), all = (max(n, unit_halves(u, 1 - i, tokens)) + 1) / 2;
+        // end of the keys that the unit sees, and the half that it cuts
+        const int end = min(u.s.lq, u.token0 + 2 * tokens) + u.s.lk - u.s.lq, cut = end % kHalf ? end / kHalf - 2 * u.from : -1;
         auto qk = [&](int t) {
           const uint32_t at = base + (t & ~1);
           if (!(t & 1) && !tile_wait(at)) return;
@@ -441,7 +443,20 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
             if (t && !wait(o_done + 8 * i, (done + t - 1) & 1, kCode)) break;
             qk(t + 1);
           }
-          if (!(t & 1)) tile_wait(base + t + 1);
+          if (!(t & 1) && !tile_wait(base + t + 1)) break;
+          if (t == cut) {
+            // Values behind that end (another sequence's, or nobody's) become zeros while the weights are made: weights of zero would let a
+            // NaN or an infinity there through.  Both tiles' warps do so, each before its own product; until both have issued theirs the
+            // ring's tile stays.
+            const uint32_t v = s_ring + (base + (t | 1)) % S::kStages * S::kTile + (t & 1) * (kHalf * 128);
+#pragma unroll 1
+            for (int k = end % kHalf * 8 + lane; k < kHalf * 8; k += 32)
+#pragma unroll
+              for (int c = 0; c < kChunks; ++c)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v + c * 16384 + k * 16), "r"(0) : "memory");
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
           if (!wait(p_full + 16 * i + 8 * (t & 1), used >> (t & 1) & 1, kCode)) break;
           used ^= 1u << (t & 1);
           tc_fence_after();

@@ -193,3 +193,50 @@ def test_infinite_values_in_fp32_cost_no_more(cuda_lib, d):
     keep = [c for c in range(d) if c != 5]
     within(out[..., keep], want[..., keep], ob[..., keep])
     within(lse, want_lse, lb)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 80, 256])
+@pytest.mark.parametrize("lens,b", [((1, 90, 63, 64), 4), ((128, 129, 1), 3), ((300, 0, 77, 500, 31), 5), (tuple(i % 9 for i in range(40)), 40)])
+def test_what_lies_behind_a_sequence_changes_no_bit(cuda_lib, dtype, d, lens, b):
+    """Rows behind the last sequence, and every other sequence: finite or poison, the rest gives the same bits."""
+    n = sum(lens)
+    q, k, v = make(n + 50, n + 50, 4, 2, d, dtype, d)
+    starts = starts_of(*lens)
+    clean, clean_lse = b2q.prompt_attention(q, k, v, starts, return_lse=True)
+    at = starts.tolist()
+    for value in (math.nan, math.inf, -math.inf):
+        p = [x.clone() for x in (q, k, v)]
+        for x in p:
+            x[n:] = value
+            for i in range(1, b, 2):
+                x[at[i]:at[i + 1]] = value
+        out, lse = b2q.prompt_attention(*p, starts, return_lse=True)
+        for i in range(0, b, 2):
+            rows = slice(at[i], at[i + 1])
+            assert torch.equal(out[rows], clean[rows]) and torch.equal(lse[rows], clean_lse[rows])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lq", [28, 200])
+def test_what_lies_behind_earlier_parts_changes_no_bit(cuda_lib, dtype, lq):
+    """The same where the keys are in parts (28 rows) and where sequences have more keys than queries."""
+    lk = (3000 - 7, 2000)
+    q, k, v = make(2 * lq, 5000, 4, 1, 64, dtype)
+    ends = starts_of(lq, lq), starts_of(*lk)
+    clean, clean_lse = b2q.prompt_attention(q, k, v, *ends, return_lse=True)
+    for x in (k, v):
+        x[lk[0]:] = math.nan
+    out, lse = b2q.prompt_attention(q, k, v, *ends, return_lse=True)
+    assert torch.equal(out[:lq], clean[:lq]) and torch.equal(lse[:lq], clean_lse[:lq])
+    assert out[lq:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_poison_behind_a_prompt_costs_no_more(cuda_lib, dtype):
+    q, k, v = make(2048, 2048, 32, 8, 128, dtype)
+    call = lambda: b2q.prompt_attention(q, k, v, starts_of(2028))
+    clean = best_ms(call)
+    for x in (q, k, v):
+        x[2028:] = math.nan
+    assert best_ms(call) < 3 * clean
