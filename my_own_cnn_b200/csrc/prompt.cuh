@@ -34,9 +34,10 @@ struct PromptArgs {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// A row's log-sum from its reference (base 2) and its sum.  With a score of +inf the sum is NaN.
+// A row's log-sum from its reference (base 2) and its sum, which is 2^LIFT times as large.  With a score of +inf the sum is NaN.
+template <int LIFT = 0>
 __device__ __forceinline__ float log_sum(float top, float sum) {
-  return top == INFINITY ? top : (top + log2f(sum)) * (1.0f / kLog2e);
+  return top == INFINITY ? top : (top + log2f(sum * (1.0f / static_cast<float>(1 << LIFT)))) * (1.0f / kLog2e);
 }
 
 // A sequence's rows; empty where its starts are not in order or pass the tensors.

@@ -25,6 +25,8 @@ constexpr int kMmaThreads = 128;
 template <typename T>
 struct Terms {
   static constexpr int kCount = 1;
+  // log2 of what weights are multiplied by, up to 1 without: fp16's are normal down to 2^-29 so (the largest is 2^15).
+  static constexpr int kLift = std::is_same<T, __half>::value ? 15 : 0;
   static __device__ __forceinline__ void cut(float a, float b, uint32_t (&w)[1]) {
     if constexpr (sizeof(T) == 2) w[0] = std::is_same<T, __half>::value ? pack_f16(a, b) : pack_bf16(a, b);
   }
@@ -32,6 +34,7 @@ struct Terms {
 template <>
 struct Terms<float> {
   static constexpr int kCount = 3;
+  static constexpr int kLift = 0;
   static __device__ __forceinline__ void cut(float a, float b, uint32_t (&w)[3]) {
     float x[2] = {a, b};
     uint32_t t[3][2];
@@ -190,6 +193,7 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
   const int2 steps = part_steps(a, (all + kKeys - 1) / kKeys, part);
   const int least = steps.x * kKeys, most = min(all, steps.y * kKeys);
   const float c = a.scale * kLog2e;
+  constexpr int kLift = Terms<T>::kLift;
   float o[D / 8][4] = {}, top[2] = {-INFINITY, -INFINITY}, sum[2] = {};
   // Heads of up to 64 channels: the next keys and values are on their way, in registers, while these are worked on.
   using KV = Tile<T, D, kKeys>;
@@ -269,6 +273,7 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
       now[h] = max_nan(now[h], __shfl_xor_sync(~0u, now[h], 2));
       from[h] = now[h] == -INFINITY ? 0.0f : now[h];
       const float keep = exp2_approx(top[h] - from[h]);
+      from[h] -= kLift;
       top[h] = now[h];
       sum[h] *= keep;
 #pragma unroll
@@ -332,7 +337,7 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
     const long long at = static_cast<long long>(u.s.q0 + token) * a.hq + head;
     if (a.parts > 1) {
       if (r < rows) {
-        if (t == 0) part_head(a, part, at, most > least && seen[h] > least, top[h], l, u.s.k0, min(u.s.lk, seen[h]));
+        if (t == 0) part_head(a, part, at, most > least && seen[h] > least, top[h] - kLift, l, u.s.k0, min(u.s.lk, seen[h]));
         float* sums = a.part_sums + (part * static_cast<long long>(a.tq) * a.hq + at) * a.d;
 #pragma unroll
         for (int n = 0; n < D / 8; ++n)
@@ -353,7 +358,7 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
           fine = fine && fabsf(y) < INFINITY;
           if (n * 8 + 2 * t + e < a.d) static_cast<T*>(a.out)[at * a.d + n * 8 + 2 * t + e] = from_f32<T>(seen[h] ? y : 0.0f);
         }
-      if (a.lse && t == 0) a.lse[at] = seen[h] ? log_sum(top[h], l) : -INFINITY;
+      if (a.lse && t == 0) a.lse[at] = seen[h] ? log_sum<Terms<T>::kLift>(top[h], l) : -INFINITY;
     }
     unsigned again = __ballot_sync(~0u, r < rows && seen[h] && !fine);
     again |= again >> 1;

@@ -7,9 +7,9 @@
 // unit are scaled and stored, the next one's queries and keys are on their way.
 // Tensor memory: scores of A and B (two halves of 64 columns each; weights take the first 32 of a half), then the sums O of A and B (D
 // columns each).
-// A row's reference is not its maximum but one that may lie up to 2^8 below it: O is then rescaled a few times in a row of any
-// length, by the threads that own it, and not with every tile.  fp16 weights are lifted by 2^6: they stay normal down to 2^-20 of
-// the reference, and below 2^14 above it.
+// A row's reference is not its maximum but one that may lie up to 2^8 (fp16: 2^4) below it: O is then rescaled a few times in a row of any
+// length, by the threads that own it, and not with every tile.  fp16 weights are lifted by 2^11: they stay normal down to 2^-25 of
+// the reference, and no more than 2^15 above it.
 //
 // 8192 tokens of one prompt, 32 / 8 heads of 128, bf16: 480 us, 1145 TFLOP/s (69 % of what cuBLAS reaches).  Three things bound it
 // at once: a product of 64 keys takes 48 clocks where its flops take 32 (operands from shared memory; all products alone take 400
@@ -27,7 +27,6 @@ constexpr int kTcKeys = 128;  // of a tile of K or V; scores and weights come in
 constexpr int kHalf = 64;
 constexpr int kTcPromptThreads = 384;
 constexpr int kTcMaxStages = 8;
-constexpr float kSlack = 8.0f;  // log2 of how far a row's maximum may pass its reference
 
 template <int D>
 struct TcShape {
@@ -123,7 +122,8 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PromptArgs a, const uint32_t negate) {
   using S = TcShape<D>;
   constexpr int kChunks = D / 64;  // 128-byte columns of a tile
-  constexpr float kLift = std::is_same<T, __half>::value ? 6.0f : 0.0f;
+  constexpr float kSlack = std::is_same<T, __half>::value ? 4.0f : 8.0f;  // log2 of how far a row's maximum may pass its reference
+  constexpr int kLift = std::is_same<T, __half>::value ? 11 : 0;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
       }
       const bool fine = !seen || (sum > 0.0f && sum < INFINITY && zero.x == 0.0f && zero.y == 0.0f);
       if (a.lse && mine)
-        a.lse[static_cast<long long>(u.s.q0 + token) * a.hq + head] = seen ? log_sum(ref - kLift, sum) : -INFINITY;
+        a.lse[static_cast<long long>(u.s.q0 + token) * a.hq + head] = seen ? log_sum<kLift>(ref, sum) : -INFINITY;
       if (const unsigned rows = __ballot_sync(~0u, !fine); __builtin_expect(rows != 0, 0)) {
         __syncwarp();  // these results and log-sums before those that other lanes write in their place
         prompt_rows_again<T>(a, rows, u.s.q0 + token, head, u.s.k0, seen, prompt_sums<T>(a, ref, sum));

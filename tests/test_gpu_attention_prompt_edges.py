@@ -240,3 +240,26 @@ def test_poison_behind_a_prompt_costs_no_more(cuda_lib, dtype):
     for x in (q, k, v):
         x[2028:] = math.nan
     assert best_ms(call) < 3 * clean
+
+
+@pytest.mark.parametrize("d,aligned", [(64, True), (128, True), (64, False), (256, True)])
+def test_small_fp16_weights_add_up(cuda_lib, d, aligned):
+    """One key far above 20000 others at 2^-24.6 of its weight, whose values alone are not zero: weights of half that precision would be
+    subnormal (1 % off, 50 % without a factor).
+
+    Off by: a weight's rounding and the result's 2^-11 each, the exponent's (24.6 * 2^-24, its product with log2(e) the same, the
+    exponential 2^-21) 2^-18 in all, sums (n / 4 + 16) 2^-23.  So is the log-sum: additions of 2^-24.6 (n / 4 of them one after another in a
+    lane, or sums of 64) to a sum of 1 are each off by up to 2^-24 of it, and its logarithm near 0 by as much."""
+    n, heads = 20000, 80  # heads: enough that the keys are not cut into parts
+    room = 0 if aligned else 1
+    q = torch.zeros(1, heads, d + room, dtype=torch.float16, device="cuda")[..., room:]
+    k, v = (torch.zeros(n, heads, d + room, dtype=torch.float16, device="cuda")[..., room:] for _ in range(2))
+    q[..., 0] = 1
+    k[1:, :, 0] = -17.05
+    v[1:] = 1
+    out, lse = b2q.prompt_attention(q, k, v, starts_of(1), starts_of(n), 1.0, return_lse=True)
+    assert b2q.last_path() == ("tcgen05-prompt-attention" if aligned and d <= 128 else "mma-prompt-attention")
+    rest = (n - 1) * math.exp(float(k[1, 0, 0]))
+    want = torch.full_like(out, 0, dtype=torch.float64) + rest / (1 + rest)
+    within(out, want, want * (2 * 2.0 ** -11 + 2.0 ** -18 + (n / 4 + 16) * 2.0 ** -23))
+    assert (lse.double() - math.log1p(rest)).abs().max() < (n / 4 + 16) * 2.0 ** -23 + 2.0 ** -20
