@@ -279,13 +279,15 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) o[n][2 * h] *= keep, o[n][2 * h + 1] *= keep;
     }
+    float add[2] = {};  // of few keys alone, then to the sum: a long row's small weights are not rounded off one by one
 #pragma unroll
     for (int n = 0; n < kKeys / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[n][e] = exp2_approx(s[n][e] - from[e / 2]);
-        sum[e / 2] += s[n][e];
+        add[e / 2] += s[n][e];
       }
+    sum[0] += add[0], sum[1] += add[1];
     uint32_t p[kKeys / 16][kTerms][4];
 #pragma unroll
     for (int kc = 0; kc < kKeys / 16; ++kc)
@@ -306,8 +308,8 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
         for (int i = 0; i < kTerms; ++i)
           load_matrices_t(v[i], s_v + i * S::kK + (kc * 16 + lane % 16) * S::kPitch + (n * 16 + lane / 16 * 8) * 2);
         if constexpr (kTerms == 1) {
-          mma_16<T>(o[2 * n], p[kc][0], v[0][0], v[0][1]);
-          mma_16<T>(o[2 * n + 1], p[kc][0], v[0][2], v[0][3]);
+          mma_16<T>(small[0], p[kc][0], v[0][0], v[0][1]);
+          mma_16<T>(small[1], p[kc][0], v[0][2], v[0][3]);
         } else {
 #pragma unroll
           for (int i = 0; i < 5; ++i) {
@@ -318,7 +320,10 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
           add_product(o[2 * n + 1], p[kc][0], v[0][2], v[0][3]);
         }
       }
-      if constexpr (kTerms == 3) {
+      if constexpr (kTerms == 1) {  // added with rounding, as below
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[2 * n][e] += small[0][e], o[2 * n + 1][e] += small[1][e];
+      } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           o[2 * n][e] = with_less(o[2 * n][e], small[0][e]);

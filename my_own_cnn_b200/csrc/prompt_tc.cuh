@@ -27,6 +27,9 @@ constexpr int kTcKeys = 128;  // of a tile of K or V; scores and weights come in
 constexpr int kHalf = 64;
 constexpr int kTcPromptThreads = 384;
 constexpr int kTcMaxStages = 8;
+// Halves that the tensor core adds up: its adder truncates, some 1e-7 of a sum for 16 keys (131072 keys 8e-4 low, nearly two roundings to
+// fp16).  After so many a thread adds its row's sums to those before, in fp32 with rounding: 5e-5 low at any length.
+constexpr int kSegment = 128;
 
 template <int D>
 struct TcShape {
@@ -114,6 +117,20 @@ __device__ __forceinline__ int unit_halves(const TcUnit& u, int i, int tokens) {
   const int first = u.token0 + i * tokens, last = min(u.s.lq, first + tokens) - 1;
   const int all = first < u.s.lq ? (max(0, last + u.s.lk - u.s.lq + 1) + kHalf - 1) / kHalf : 0;
   return max(0, min(all, 2 * u.to) - 2 * u.from);
+}
+
+// before = before keep + O of this thread's row; O alone the first time.
+template <int D>
+__device__ __noinline__ void take_sums(float (&before)[D], uint32_t t_o, bool first, float keep) {
+#pragma unroll 1
+  for (int k = 0; k < D; k += 32) {
+    uint32_t o[32];
+    tmem_ld_32x32b_x32(t_o + k, o);
+    tmem_ld_wait();
+    loaded(o);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) before[k + e] = first ? __uint_as_float(o[e]) : fmaf(before[k + e], keep, __uint_as_float(o[e]));
+  }
 }
 
 template <typename T, int D>
@@ -225,65 +242,80 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
       const bool mine = of < tokens && token < u.s.lq;
       const int seen = mine ? max(0, token + shift + 1) : 0;
       float ref = 0.0f, sum = 0.0f;
-      for (int t = 0; t < n; ++t) {
-        const uint32_t half = t & 1, t_h = t_s + 64 * half;
-        if (!wait(s_full + 16 * i + 8 * half, used >> half & 1, kCode)) break;
-        used ^= 1u << half;
-        tc_fence_after();
-        uint32_t raw[2][32];
-        tmem_ld_32x32b_x32(t_h, raw[0]);
-        tmem_ld_32x32b_x32(t_h + 32, raw[1]);
-        tmem_ld_wait();
-        loaded(raw[0]);
-        loaded(raw[1]);
-        const auto s = [&](int k) { return __uint_as_float(raw[k / 32][k % 32]); };
-        const int limit = seen - 2 * u.from * kHalf - t * kHalf;
-        if (__any_sync(~0u, limit < kHalf)) {
-#pragma unroll
-          for (int k = 0; k < kHalf; ++k)
-            if (k >= limit) raw[k / 32][k % 32] = 0xFF800000u;
-        }
-        float m[2] = {s(0), s(1)};
-#pragma unroll
-        for (int k = 2; k < kHalf - 2; k += 4) m[0] = max3(m[0], s(k), s(k + 1)), m[1] = max3(m[1], s(k + 2), s(k + 3));
-        const float top = max3(max_nan(m[0], m[1]), s(kHalf - 2), s(kHalf - 1)) * c;  // -inf: nothing seen here
-        // nothing but scores of -inf so far: the sums are zero at any reference
-        if (sum == 0.0f) ref = top == -INFINITY ? 0.0f : top;
-        if (__any_sync(~0u, top - ref > kSlack)) {  // never at t = 0: there are no sums yet
-          const float now = top - ref > kSlack ? top : ref, keep = exp2_approx(ref - now);
-          if (!wait(o_done + 8 * i, (done + t - 1) & 1, kCode)) break;
+      float before[D], held = -INFINITY;  // sums of the segments before (indexed as it runs: local memory), at this reference
+      for (int t = 0;;) {
+        for (const int stop = min(n, t + kSegment); t < stop; ++t) {
+          const uint32_t half = t & 1, t_h = t_s + 64 * half;
+          if (!wait(s_full + 16 * i + 8 * half, used >> half & 1, kCode)) break;
+          used ^= 1u << half;
           tc_fence_after();
-#pragma unroll 1
-          for (int k = 0; k < D; k += 32) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(t_o + k, o);
-            tmem_ld_wait();
-            loaded(o);
+          uint32_t raw[2][32];
+          tmem_ld_32x32b_x32(t_h, raw[0]);
+          tmem_ld_32x32b_x32(t_h + 32, raw[1]);
+          tmem_ld_wait();
+          loaded(raw[0]);
+          loaded(raw[1]);
+          const auto s = [&](int k) { return __uint_as_float(raw[k / 32][k % 32]); };
+          const int limit = seen - 2 * u.from * kHalf - t * kHalf;
+          if (__any_sync(~0u, limit < kHalf)) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-            tmem_st_32x32b_x32(t_o + k, o);
+            for (int k = 0; k < kHalf; ++k)
+              if (k >= limit) raw[k / 32][k % 32] = 0xFF800000u;
           }
-          sum *= keep;
-          ref = now;
-        }
-        if (top != top) ref = top;  // a score that is NaN: the row's, whatever else there is
-        const float less = kLift - ref;
-        float add[4] = {};
-        uint32_t w[32];
+          float m[2] = {s(0), s(1)};
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const float x = exp2_approx(fmaf(s(2 * k), c, less)), y = exp2_approx(fmaf(s(2 * k + 1), c, less));
-          add[2 * (k & 1)] += x;
-          add[2 * (k & 1) + 1] += y;
-          w[k] = pack_16<T>(x, y);
+          for (int k = 2; k < kHalf - 2; k += 4) m[0] = max3(m[0], s(k), s(k + 1)), m[1] = max3(m[1], s(k + 2), s(k + 3));
+          const float top = max3(max_nan(m[0], m[1]), s(kHalf - 2), s(kHalf - 1)) * c;  // -inf: nothing seen here
+          // nothing but scores of -inf so far: the sums are zero at any reference
+          if (sum == 0.0f) ref = top == -INFINITY ? 0.0f : top;
+          if (__any_sync(~0u, top - ref > kSlack)) {  // never at t = 0: there are no sums yet
+            const float now = top - ref > kSlack ? top : ref, keep = exp2_approx(ref - now);
+            if (!wait(o_done + 8 * i, (done + t - 1) & 1, kCode)) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int k = 0; k < D; k += 32) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(t_o + k, o);
+              tmem_ld_wait();
+              loaded(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+              tmem_st_32x32b_x32(t_o + k, o);
+            }
+            sum *= keep;
+            ref = now;
+          }
+          if (top != top) ref = top;  // a score that is NaN: the row's, whatever else there is
+          const float less = kLift - ref;
+          float add[4] = {};
+          uint32_t w[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const float x = exp2_approx(fmaf(s(2 * k), c, less)), y = exp2_approx(fmaf(s(2 * k + 1), c, less));
+            add[2 * (k & 1)] += x;
+            add[2 * (k & 1) + 1] += y;
+            w[k] = pack_16<T>(x, y);
+          }
+          tmem_st_32x32b_x32(t_h, w);
+          sum += (add[0] + add[1]) + (add[2] + add[3]);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full + 16 * i + 8 * half);
         }
-        tmem_st_32x32b_x32(t_h, w);
-        sum += (add[0] + add[1]) + (add[2] + add[3]);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + 16 * i + 8 * half);
+        if (t >= n || !ok) break;
+        // (the scores say that the product before the last two has ended)
+        if (!wait(o_done + 8 * i, (done + t - 2) & 1, kCode) || !wait(o_done + 8 * i, (done + t - 1) & 1, kCode)) break;
+        tc_fence_after();
+        take_sums<D>(before, t_o, t == kSegment, exp2_approx(held - ref));
+        held = sum == 0.0f ? -INFINITY : ref;
       }
+      const float keep = exp2_approx(held - ref);
+      const auto with_before = [&](uint32_t (&o)[32], int k) {
+        if (n <= kSegment) return;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(fmaf(before[k + e], keep, __uint_as_float(o[e])));
+      };
       done += n;
       if (n) wait(ended + 8 * i, units_of++ & 1, kCode);
       if (!ok) break;
@@ -298,6 +330,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
           tmem_ld_32x32b_x32(t_o + k, o);
           tmem_ld_wait();
           loaded(o);
+          with_before(o, k);
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             if (mine && k + e < a.d) *reinterpret_cast<uint4*>(sums + k + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
@@ -318,6 +351,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
             tmem_ld_32x32b_x32(t_o + 64 * ch + k, o);
             tmem_ld_wait();
             loaded(o);
+            with_before(o, 64 * ch + k);
           }
 #pragma unroll
           for (int f = 0; f < 16; ++f) {
@@ -461,7 +495,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
           used ^= 1u << (t & 1);
           tc_fence_after();
           tc_mma_f16_ts_x4_elect(t_o, t_s + (t & 1) * kHalf, v_at + (base + (t | 1)) % S::kStages * (S::kTile / 16) + (t & 1) * 512,
-                                 pv_desc, t);
+                                 pv_desc, t % kSegment);
           tc_commit_elect(o_done + 8 * i);
           if ((t & 1) || t + 1 == n) release(base + (t | 1));
           if (t + 1 == n) tc_commit_elect(ended + 8 * i);

@@ -6,7 +6,7 @@ import torch
 
 import my_own_cnn_b200 as b2q
 from tests import s8_ref
-from tests.lowbit_ref import within
+from tests.lowbit_ref import UNIT, within
 
 pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -263,3 +263,55 @@ def test_small_fp16_weights_add_up(cuda_lib, d, aligned):
     want = torch.full_like(out, 0, dtype=torch.float64) + rest / (1 + rest)
     within(out, want, want * (2 * 2.0 ** -11 + 2.0 ** -18 + (n / 4 + 16) * 2.0 ** -23))
     assert (lse.double() - math.log1p(rest)).abs().max() < (n / 4 + 16) * 2.0 ** -23 + 2.0 ** -20
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("d,keys", [(64, 131072), (128, 66001), (256, 40000), (64, 8192), (64, 8193)])
+def test_sums_of_many_keys_have_no_bias(cuda_lib, dtype, d, keys):
+    """Values of one sign over many keys, in one part: an adder that truncates makes all results low, the more the longer.
+
+    The mean of (result - value) / value over 80 heads: roundings to 16 bits average out (2^-9 / sqrt(80 * 64 * 3) = 1.6e-5 for bf16), weights'
+    far more so; what is left are the sums of 8192 keys, 512 products of 16 that may lose 2^-23 of the sum each: 6.1e-5."""
+    heads = 80
+    g = torch.Generator(device="cuda").manual_seed(d)
+    q = torch.randn(1, heads, d, generator=g, device="cuda").to(dtype)
+    k, v = (torch.empty(keys, heads, d, dtype=dtype, device="cuda") for _ in range(2))
+    want, want_lse = torch.empty(heads, d, dtype=torch.float64, device="cuda"), torch.empty(heads, dtype=torch.float64, device="cuda")
+    for h in range(heads):
+        k[:, h] = torch.randn(keys, d, generator=g, device="cuda").to(dtype)
+        size = 1 + torch.rand(d, generator=g, device="cuda")
+        v[:, h] = ((0.5 + torch.rand(keys, d, generator=g, device="cuda")) * size).to(dtype)
+        a = (k[:, h].double() @ q[0, h].double()) * d ** -0.5
+        want_lse[h] = torch.logsumexp(a, 0)
+        want[h] = torch.softmax(a, 0) @ v[:, h].double()
+    out, lse = b2q.prompt_attention(q, k, v, starts_of(1), starts_of(keys), return_lse=True)
+    off = (out[0].double() - want) / want
+    assert abs(float(off.mean())) < 4 * 1.6e-5 + 512 * 2.0 ** -23
+    assert float(off.abs().max()) < 2 * UNIT[dtype] + 512 * 2.0 ** -23  # the result and, at worst, all weights alike
+    assert (lse[0].double() - want_lse).abs().max() < 2.0 ** -17
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("d", [64, 128, 80])
+@pytest.mark.parametrize("lq", [130, 5])
+def test_long_rows_whose_maxima_grow(cuda_lib, dtype, d, lq):
+    """More than 8192 keys whose scores grow along the row, shrink along it, or are -inf for the first 9000: what was summed up before
+    is taken over at another reference.  Five rows are in parts."""
+    keys = 20000
+    q, k, v = make(lq, keys, 2, 1, d, dtype, d, 0.3)
+    slope = torch.linspace(-30, 30, keys, device="cuda")
+    q[..., 0] = 1
+    starts, k_starts = starts_of(lq), starts_of(keys)
+    for rise in (slope, -slope, -100 - slope.abs()):
+        k[:, 0, 0] = rise.to(dtype)
+        out, lse = b2q.prompt_attention(q, k, v, starts, k_starts, 1.0, return_lse=True)
+        want, want_lse, ob, lb = s8_ref.attention(q, k, v, starts, k_starts, 1.0, dtype)
+        within(out, want, ob)
+        within(lse, want_lse, lb)
+    q[..., 1], k[..., 1] = 1, 0
+    k[:9000, :, 1] = -math.inf
+    out, lse = b2q.prompt_attention(q, k, v, starts, k_starts, 1.0, return_lse=True)
+    k[:9000, :, 1] = 0
+    want, want_lse, ob, lb = s8_ref.attention(q, k[9000:], v[9000:], starts, starts_of(keys - 9000), 1.0, dtype)
+    within(out, want, ob)
+    within(lse, want_lse, lb)
