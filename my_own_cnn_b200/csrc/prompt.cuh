@@ -1,6 +1,7 @@
 // What the kernels of prompt attention share: arguments, the order of the work, rows that are done with care.
 #pragma once
 #include <climits>
+#include <type_traits>
 
 #include "host.h"
 #include "lowbit.cuh"
@@ -38,6 +39,17 @@ constexpr float kLog2e = 1.4426950408889634f;
 template <int LIFT = 0>
 __device__ __forceinline__ float log_sum(float top, float sum) {
   return top == INFINITY ? top : (top + log2f(sum * (1.0f / static_cast<float>(1 << LIFT)))) * (1.0f / kLog2e);
+}
+
+// A result is an average, no larger than the largest value; weights that are rounded for the second product and a sum of weights that are
+// not can bring it past fp16's range all the same, by a part in 2^11.
+constexpr float kHalfMost = 65504.0f;
+__device__ __forceinline__ float to_half_range(float y) {
+  return fabsf(y) < INFINITY ? fminf(fmaxf(y, -kHalfMost), kHalfMost) : y;
+}
+template <typename T>
+__device__ __forceinline__ T result(float y) {
+  return from_f32<T>(std::is_same<T, __half>::value ? to_half_range(y) : y);
 }
 
 // A sequence's rows; empty where its starts are not in order or pass the tensors.
@@ -260,7 +272,7 @@ __device__ __noinline__ void prompt_row_with_care(const PromptArgs& a, int q_row
   T* out = static_cast<T*>(a.out) + (static_cast<long long>(q_row) * a.hq + head) * a.d + lane;
 #pragma unroll
   for (int c = 0; c < C; ++c)
-    if (lane + 32 * c < d) out[32 * c] = from_f32<T>(o[c] / total);
+    if (lane + 32 * c < d) out[32 * c] = result<T>(o[c] / total);
   if (a.lse && lane == 0)
     a.lse[static_cast<long long>(q_row) * a.hq + head] = fabsf(top) < INFINITY ? top + logf(total) : top;
 }
@@ -438,7 +450,7 @@ __global__ void __launch_bounds__(256, 2) prompt_join_kernel(const __grid_consta
     if (lane + 32 * c < a.d) {
       const float y = seen ? o[c] / total : 0.0f;
       fine = fine && fabsf(y) < INFINITY;
-      out[lane + 32 * c] = from_f32<T>(y);
+      out[lane + 32 * c] = result<T>(y);
     }
   if (a.lse && lane == 0) a.lse[row] = seen ? log_sum(top, total) : -INFINITY;
   __syncwarp();

@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kMmaThreads) prompt_mma_kernel(const __grid_co
         for (int e = 0; e < 2; ++e) {
           const float y = o[n][2 * h + e] * by;
           fine = fine && fabsf(y) < INFINITY;
-          if (n * 8 + 2 * t + e < a.d) static_cast<T*>(a.out)[at * a.d + n * 8 + 2 * t + e] = from_f32<T>(seen[h] ? y : 0.0f);
+          if (n * 8 + 2 * t + e < a.d) static_cast<T*>(a.out)[at * a.d + n * 8 + 2 * t + e] = result<T>(seen[h] ? y : 0.0f);
         }
       if (a.lse && t == 0) a.lse[at] = seen[h] ? log_sum<Terms<T>::kLift>(top[h], l) : -INFINITY;
     }

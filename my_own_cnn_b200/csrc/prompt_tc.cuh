@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
       // 8 lanes write 128 bytes together; a thread that writes its own row takes as many cycles as it has sectors.
       const float scale = seen ? 1.0f / sum : 0.0f;
       const long long at = (static_cast<long long>(u.s.q0 + token) * a.hq + head) * a.d;
-      float2 zero = both(0.0f);  // stays so while all results are finite
+      float most = 0.0f;  // in size; NaN if one is
 #pragma unroll 1
       for (int ch = 0; 64 * ch < a.d; ++ch) {
 #pragma unroll
@@ -353,11 +353,19 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
             loaded(o);
             with_before(o, 64 * ch + k);
           }
+          const auto at_scale = [&](int f) { return mul2(make_float2(__uint_as_float(o[2 * f]), __uint_as_float(o[2 * f + 1])), both(scale)); };
 #pragma unroll
           for (int f = 0; f < 16; ++f) {
-            const float2 v = mul2(make_float2(__uint_as_float(o[2 * f]), __uint_as_float(o[2 * f + 1])), both(scale));
-            zero = fma2(v, both(0.0f), zero);
+            const float2 v = at_scale(f);
+            most = max3(most, fabsf(v.x), fabsf(v.y));
             y[f] = seen ? pack_16<T>(v.x, v.y) : 0u;
+          }
+          if (std::is_same<T, __half>::value && __any_sync(~0u, seen && most > kHalfMost)) {
+#pragma unroll
+            for (int f = 0; f < 16; ++f) {
+              const float2 v = at_scale(f);
+              y[f] = seen ? pack_16<T>(to_half_range(v.x), to_half_range(v.y)) : 0u;
+            }
           }
 #pragma unroll
           for (int f = 0; f < 4; ++f)
@@ -379,7 +387,7 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
         }
         __syncwarp();
       }
-      const bool fine = !seen || (sum > 0.0f && sum < INFINITY && zero.x == 0.0f && zero.y == 0.0f);
+      const bool fine = !seen || (sum > 0.0f && sum < INFINITY && most < INFINITY);
       if (a.lse && mine)
         a.lse[static_cast<long long>(u.s.q0 + token) * a.hq + head] = seen ? log_sum<kLift>(ref, sum) : -INFINITY;
       if (const unsigned rows = __ballot_sync(~0u, !fine); __builtin_expect(rows != 0, 0)) {

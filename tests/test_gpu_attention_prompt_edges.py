@@ -315,3 +315,18 @@ def test_long_rows_whose_maxima_grow(cuda_lib, dtype, d, lq):
     want, want_lse, ob, lb = s8_ref.attention(q, k[9000:], v[9000:], starts, starts_of(keys - 9000), 1.0, dtype)
     within(out, want, ob)
     within(lse, want_lse, lb)
+
+
+@pytest.mark.parametrize("d", [64, 128, 80, 200])
+@pytest.mark.parametrize("lq,lk", [(300, 300), (700, 700), (28, 7000), (130, 9000)])
+def test_saturated_fp16_values_stay_finite(cuda_lib, d, lq, lk):
+    """Channels whose values are all fp16's largest, or lie just below it: their average is no infinity, though a weight is rounded by
+    up to 2^-11 and 65520 rounds to one.  Off by at most that and the result's own rounding."""
+    q, k, v = make(lq, lk, 4, 4, d, torch.float16, d, 3.0)
+    v[..., 3], v[..., 5] = 65504, -65504
+    v[..., 7] = torch.where(v[..., 7] > 0, 65504.0, 65472.0).half()
+    v[..., 9] = math.inf
+    out = b2q.prompt_attention(q, k, v, starts_of(lq), starts_of(lk))
+    for c, sign in ((3, 1), (5, -1), (7, 1)):
+        assert out[..., c].isfinite().all() and (sign * out[..., c].double() >= 65472 * (1 - 2 * 2.0 ** -11 - 2.0 ** -13)).all()
+    assert (out[..., 9] == math.inf).all()
