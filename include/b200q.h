@@ -319,8 +319,8 @@ typedef struct b200q_read_s8_args {
 } b200q_read_s8_args;
 int b200q_read_s8(const b200q_read_s8_args* args, void* stream);
 
-/* y[m][n] = (sum_k x[m][k] * w[n][k]) * x_scale[m] * w_scale[n] (+ bias[n]) for 8-bit rows x [m][k] and w [n][k]: the sum exact in
- * 32-bit integers (k <= 131071), the rest in fp32, y of ftype with row stride ldy; bias [n] of ftype or NULL.  Codes lie on
+/* y[m][n] = (sum_k x[m][k] * w[n][k]) * w_scale[n] * x_scale[m] (+ bias[n]) for 8-bit rows x [m][k] and w [n][k]: the sum exact in
+ * 32-bit integers (k <= 131071), the rest in fp32 in this order, y of ftype with row stride ldy; bias [n] of ftype or NULL.  Codes lie on
  * 16-byte boundaries with row strides that are multiples of 16; what lies past k is not used.  A row or a channel with
  * the scale NaN gives NaN.  y shares no memory with the other tensors. */
 typedef struct b200q_linear_s8_args {

@@ -1,6 +1,6 @@
 // Linear layers of 8-bit rows (b200q_linear_s8).
 //
-//   y[m][n] = (sum_k x[m][k] w[n][k]) xs[m] ws[n] + bias[n]: the sum exact in int32, the rest fp32.
+//   y[m][n] = (sum_k x[m][k] w[n][k]) ws[n] xs[m] + bias[n]: the sum exact in int32, the rest fp32.
 //
 // tcgen05.mma.kind::i8 with the weights as the rows of the product (128 channels, TMEM lanes) and the tokens as its columns: a
 // decode step of one token needs 16 columns, not 128 rows, and the same orientation serves a prompt.  A thread of the epilogue
@@ -526,7 +526,7 @@ int block_room(int device, int sms, int (*room)[4]) {
   return B200Q_OK;
 }
 
-int linear_s8(const b200q_linear_s8_args* p, const Plan* fixed, cudaStream_t cs) {
+int linear_s8(const b200q_linear_s8_args* p, cudaStream_t cs) {
   if (!p) return host_fail(B200Q_ERR_INVALID_ARG, "null argument");
   const int ftype = p->ftype, m = p->m, n = p->n, k = p->k;
   if (ftype < B200Q_F32 || ftype > B200Q_BF16) return host_fail(B200Q_ERR_INVALID_ARG, "bad floating type %d", ftype);
@@ -556,7 +556,7 @@ int linear_s8(const b200q_linear_s8_args* p, const Plan* fixed, cudaStream_t cs)
   a.err = err;
   int room[4];
   if ((rc = block_room(device, sms, &room))) return rc;
-  const Plan plan = fixed ? *fixed : plan_for(m, n, a.kblocks, device, room);
+  const Plan plan = plan_for(m, n, a.kblocks, device, room);
   CUtensorMap tm_w, tm_x;
   const auto stride = [&](int rows, int64_t ld) { return static_cast<uint64_t>(rows > 1 ? ld : round_up(k, 16)); };
   if ((rc = host_tensor_map(&tm_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p->w, {static_cast<uint64_t>(k), static_cast<uint64_t>(n), 1},
@@ -577,5 +577,5 @@ int linear_s8(const b200q_linear_s8_args* p, const Plan* fixed, cudaStream_t cs)
 using namespace b200q;
 
 extern "C" int b200q_linear_s8(const b200q_linear_s8_args* args, void* stream) {
-  return linear_s8(args, nullptr, static_cast<cudaStream_t>(stream));
+  return linear_s8(args, static_cast<cudaStream_t>(stream));
 }
