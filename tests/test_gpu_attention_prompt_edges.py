@@ -330,3 +330,25 @@ def test_saturated_fp16_values_stay_finite(cuda_lib, d, lq, lk):
     for c, sign in ((3, 1), (5, -1), (7, 1)):
         assert out[..., c].isfinite().all() and (sign * out[..., c].double() >= 65472 * (1 - 2 * 2.0 ** -11 - 2.0 ** -13)).all()
     assert (out[..., 9] == math.inf).all()
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_which_kernel_takes_a_call(cuda_lib, dtype):
+    """16-bit heads of up to 128 channels that are a multiple of 8, on 16-byte boundaries, at most 128 of them a key head: tcgen05; the rest and
+    fp32: mma.sync."""
+    starts = starts_of(20, 17)
+
+    def path(q, k, v, **kw):
+        b2q.prompt_attention(q, k, v, starts, **kw)
+        return b2q.last_path()
+
+    fast = "mma-prompt-attention" if dtype == torch.float32 else "tcgen05-prompt-attention"
+    for d in (8, 40, 64, 72, 80, 128):
+        assert path(*make(37, 37, 4, 2, d, dtype)) == fast
+    for d in (1, 33, 60, 136, 256):
+        assert path(*make(37, 37, 4, 2, d, dtype)) == "mma-prompt-attention"
+    assert path(*make(37, 37, 128, 1, 64, dtype)) == fast and path(*make(37, 37, 129, 1, 64, dtype)) == "mma-prompt-attention"
+    q, k, v = make(37, 37, 4, 2, 72, dtype)
+    assert path(q[..., 8:], k[..., 8:], v[..., 8:]) == fast
+    assert path(q[..., 1:65], k[..., 1:65], v[..., 1:65]) == "mma-prompt-attention"
+    assert path(q, k, v, scale=0.0) == "mma-prompt-attention"
+    assert path(q, k[:, :1].expand(37, 2, 72), v) == "mma-prompt-attention"
