@@ -92,24 +92,28 @@ class S8Attention:
             kv4_append(cache, k, v, slots, stream=stream)
         return q, k, v, residual
 
-    def _output(self, attention, dtype, stream):
-        rows = quantize_s8(attention.view(-1, self.heads * self.head_dim), stream=stream)
+    def _output(self, attention, t, dtype, stream):
+        rows = quantize_s8(attention.view(t, self.heads * self.head_dim), stream=stream)
         return linear_s8(rows, self.wo, dtype=dtype, stream=stream)
 
     def prompt(self, x: torch.Tensor, residual: torch.Tensor | None, positions: torch.Tensor, starts: torch.Tensor,
                cache: KV4Cache | None = None, slots: torch.Tensor | None = None, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
         """x [t, hidden]: prompts packed one after another, sequence i in rows starts[i] .. starts[i + 1] (int32 on the device);
         positions int32 [t]; slots int64 [t] place keys and values in the cache (None: they are not kept).  Returns the block's
-        output [t, hidden] and the residual (x + residual, in place of the residual; x when there is none)."""
+        output [t, hidden] (anything in rows outside every prompt) and the residual (x + residual, in place of the residual; x when
+        there is none)."""
+        if (cache is None) != (slots is None):
+            raise RuntimeError("a cache and slots go together")
         q, k, v, residual = self._project(x, residual, cache, positions, slots, stream)
-        return self._output(prompt_attention(q, k, v, starts, stream=stream), x.dtype, stream), residual
+        return self._output(prompt_attention(q, k, v, starts, stream=stream), x.shape[0], x.dtype, stream), residual
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None, cache: KV4Cache, positions: torch.Tensor, slots: torch.Tensor,
                 block_table: torch.Tensor, lens: torch.Tensor, stream=None) -> tuple[torch.Tensor, torch.Tensor]:
         """x [b * tq, hidden]: the next tq tokens of each of the b sequences; lens int32 [b] counts each one's tokens with the new ones."""
         q, _, _, residual = self._project(x, residual, cache, positions, slots, stream)
-        out = kv4_attention(q.unflatten(0, (lens.shape[0], -1)), cache, block_table, lens, stream=stream)
-        return self._output(out, x.dtype, stream), residual
+        b = lens.shape[0]
+        out = kv4_attention(q.unflatten(0, (b, x.shape[0] // max(b, 1))), cache, block_table, lens, stream=stream)
+        return self._output(out, x.shape[0], x.dtype, stream), residual
 
 
 def random_block_s8(hidden: int, heads: int, kv_heads: int, head_dim: int, dtype: torch.dtype, positions: int = 8192,
