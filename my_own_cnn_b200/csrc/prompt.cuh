@@ -291,11 +291,11 @@ struct FirstOdd {
 
 // Rows that a fast kernel wrote and found not finite, those of one warp: of one sequence and key head, each in the lane of its bit.
 // Returns the ones that are not right as they are.  Most are, and looking for the reason takes one read of the values for all of them
-// (up to where it is found), where a row with care costs all of its keys and values: 2048 tokens, 32 / 8 heads of 128, bf16 take 0.09 ms, with a
-// NaN or an infinity in value 3 0.13 to 0.23, in value 1024 0.32.
-//   - The sum of the weights is NaN.  So is the row's reference where a score is, and all of the row.  A reference of +inf: a score is, and none
-//     is NaN; the row is NaN, its log-sum +inf.  (A score may also pass fp32 by the factor |scale| log2(e), where that is above 1: such a row
-//     is done with care.)  In fp32 a score may be NaN also where a factor is infinite and the other one's first term is zero.
+// (up to where it is found), where a row with care costs all of its keys and values: 2048 tokens, 32 / 8 heads of 128, bf16 take
+// 0.09 ms, with a NaN or an infinity in value 3 0.23, in value 1024 0.32.
+//   - The sum of the weights is NaN.  So is the row's reference where a score is, and all of the row.  A reference of +inf: a score is,
+//     and none is NaN; the row is NaN, its log-sum +inf.  (A score may also pass fp32 by the factor |scale| log2(e), where that is above 1:
+//     such a row is done with care.)  In fp32 a score may be NaN also where a factor is infinite and the other one's first term is zero.
 //   - A channel is NaN, and a value that the row sees is, or two are infinities of both signs.  Or it is infinite, and a value that
 //     the row sees is the same (others would have made it NaN; what it does not see gives NaN or nothing).
 enum { kSumOdd = 0, kSumFine = 1, kSumNaN = 2, kSettled = 3 };

@@ -11,11 +11,15 @@
 // length, by the threads that own it, and not with every tile.  fp16 weights are lifted by 2^11: they stay normal down to 2^-25 of
 // the reference, and no more than 2^15 above it.
 //
-// 8192 tokens of one prompt, 32 / 8 heads of 128, bf16: 480 us, 1145 TFLOP/s (69 % of what cuBLAS reaches).  Three things bound it
-// at once: a product of 64 keys takes 48 clocks where its flops take 32 (operands from shared memory; all products alone take 400
-// us), a warp's exponentials 8.4 clocks each, and the answers between the two.  So scores come in halves of 64 keys, two of them in
-// TMEM for each tile: a half's products run while the warps have the other one (whole tiles of 128 keys without a second buffer:
-// 583 us).
+// Weights are rounded to the inputs' type for the second product, by up to 2^-11 or 2^-8 of each: results are 0.0019 off where their own
+// rounding makes 0.0016 (8192 tokens bf16; fp16 0.00022 and 0.0002).  A second term a weight would leave that alone and be a second
+// product over the same values: 596 us where this takes 462.
+//
+// 8192 tokens of one prompt, 32 / 8 heads of 128, bf16: 462 to 485 us in a replayed graph, 1160 TFLOP/s (70 % of what cuBLAS reaches in
+// a burst); call after call 553 to 566, as the power limit lowers the clock.  Three things bound it at once: a product of 64 keys takes
+// 48 clocks where its flops take 32 (operands from shared memory; all products alone take 400 us), a warp's exponentials 8.4 clocks
+// each, and the answers between the two.  So scores come in halves of 64 keys, two of them in TMEM for each tile: a half's products run
+// while the warps have the other one (whole tiles of 128 keys without a second buffer: 583 us).
 #pragma once
 #include "common.cuh"
 #include "prompt.cuh"

@@ -10,9 +10,10 @@
 // 1 to 8 blocks, whose int32 sums meet in shared memory (integers: any order gives the same bits).  It takes the calls whose tiles do
 // not fill the GPU: few tokens (bound by the weights' stream from DRAM), short prompts.  linear_s8_pair_kernel: persistent pairs of SMs,
 // 256 channels x 256 tokens a tile, M = 256 instructions, the epilogue of a tile under the products of the next.
-// Measured: 8192 x 8192 x 8192 in 329 us, 3340 TOP/s, twice the bf16 rate that cuBLAS reaches (tensor pipe 88 % busy): the tensor
-// core bounds it.  16 x 16384 x 8192 bf16 in 23.7 us, 5.7 TB/s (88 % of a copy): DRAM.  1 x 4096 x 4096 in 5.4 us and 77 x 5003 x 4091
-// fp32 in 8.2 us: a launch, the first bytes' latency and the join of the blocks' sums.
+// Measured: 8192 x 8192 x 8192 in 324 to 329 us in a replayed graph, 3340 TOP/s, twice the bf16 rate that cuBLAS reaches (tensor pipe 88 %
+// busy): the tensor core bounds it; call after call 383 to 395, as the power limit lowers the clock.  16 x 16384 x 8192 bf16 in 23.7 to 26.8 us,
+// 5.7 TB/s (88 % of a copy) at best: DRAM.  1 x 4096 x 4096 in 5.4 to 6.9 us and 77 x 5003 x 4091 fp32 in 8.2 us: a launch, the first bytes'
+// latency and the join of the blocks' sums.
 #include <algorithm>
 #include <atomic>
 

@@ -30,7 +30,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     starts decrease or pass the tensors is left out and reported by device_error().  scale: 1 / sqrt(d) when None; its product
     with log2(e) has to be finite in fp32.
     Returns out [tq, hq, d], and lse fp32 [tq, hq] (log of the sum of exp(scale * q.k)) when return_lse.  out shares no memory
-    with the other tensors; starts stay as they are until the call has run.
+    with the other tensors; starts stay as they are until the call has run.  Sums, statistics and log-sums are fp32; fp16 and bf16 calls round the
+    softmax weights to that type before they meet the values.
 
     Where few rows see many keys (too few tiles of rows for half of the SMs, 512 keys and more a sequence on average) the keys are
     cut into parts that meet in the stream's scratch: make one such call on the stream before capturing a graph on it."""

@@ -124,7 +124,7 @@ def _check_like(t, x, shape, what):
 
 def quantize_s8(x: torch.Tensor, out: S8Rows | None = None, stream=None) -> S8Rows:
     """x [..., k] (fp32, fp16 or bf16; rows may be strided) as 8-bit rows: code = rint(x * fl(127 * fl(1 / max|x|))),
-    scale = max|x| / 127.  A row with a NaN or an infinity gets the scale NaN."""
+    scale = max|x| / 127.  A row with a NaN or an infinity gets the scale NaN, one with nothing above 2^-119 zeros."""
     ft = FTYPES.get(x.dtype)
     if ft is None or not x.is_cuda:
         _ftype(x, "x")
@@ -153,7 +153,8 @@ def rms_norm_s8(x: torch.Tensor, weight: torch.Tensor | None, residual: torch.Te
 
     x [..., n] (fp32, fp16 or bf16; rows may be strided), weight [n] or None, residual like x.  h is written to
     residual_out, which may be x; to the residual itself when that is None.  Returns the rows, with a residual
-    (rows, h).  A row with a NaN or an infinity gets the scale NaN."""
+    (rows, h).  A row with a NaN or an infinity gets the scale NaN; one with nothing above 2^-119 in size after the weight is zeros, also where
+    eps is 0."""
     ft = FTYPES.get(x.dtype)
     if ft is None or not x.is_cuda:
         _ftype(x, "x")
