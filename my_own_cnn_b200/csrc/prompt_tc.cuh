@@ -308,8 +308,9 @@ __global__ void __launch_bounds__(kTcPromptThreads, 1)
           if (lane == 0) mbar_arrive(p_full + 16 * i + 8 * half);
         }
         if (t >= n || !ok) break;
-        // (the scores say that the product before the last two has ended)
-        if (!wait(o_done + 8 * i, (done + t - 2) & 1, kCode) || !wait(o_done + 8 * i, (done + t - 1) & 1, kCode)) break;
+        // The next scores, which are waited for again below, come after the last product but one: so the barrier is in the last one's phase, or
+        // past it by one.
+        if (!wait(s_full + 16 * i + 8 * (t & 1), used >> (t & 1) & 1, kCode) || !wait(o_done + 8 * i, (done + t - 1) & 1, kCode)) break;
         tc_fence_after();
         take_sums<D>(before, t_o, t == kSegment, exp2_approx(held - ref));
         held = sum == 0.0f ? -INFINITY : ref;

@@ -352,3 +352,13 @@ def test_which_kernel_takes_a_call(cuda_lib, dtype):
     assert path(q[..., 1:65], k[..., 1:65], v[..., 1:65]) == "mma-prompt-attention"
     assert path(q, k, v, scale=0.0) == "mma-prompt-attention"
     assert path(q, k[:, :1].expand(37, 2, 72), v) == "mma-prompt-attention"
+
+
+def test_many_hand_overs_of_sums(cuda_lib):
+    """Rows of 40000 keys (four hand-overs) in 160 tiles, on all SMs, again and again: the same bits each time, and no wait runs out."""
+    q, k, v = make(4, 160000, 40, 40, 64, torch.bfloat16)
+    ends = starts_of(1, 1, 1, 1), starts_of(*[40000] * 4)
+    first = b2q.prompt_attention(q, k, v, *ends)
+    for _ in range(20):
+        assert torch.equal(b2q.prompt_attention(q, k, v, *ends), first)
+    b2q.device_error()
